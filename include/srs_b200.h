@@ -5,7 +5,8 @@
  * scalars and a cudaStream_t passed as `void*`.  Nothing here allocates
  * device memory: callers own every buffer (inputs, outputs and the row
  * tables of the multi-tensor steps).  Work is enqueued on the given stream
- * of the calling thread's current device; no entry point synchronises.
+ * of the calling thread's current device; no entry point synchronises
+ * (srs_product_status apart).
  *
  * Return value: SRS_OK (0) or a negative SRS_ERR_* code.  The text of the
  * most recent failure on the calling thread is available from
@@ -292,6 +293,87 @@ int srs_sgdm_single(const srs_row* row, int u_format, int u_rule, const srs_sgdm
  */
 int srs_derive_keys(const uint32_t* param_index, uint32_t* out, int64_t n, const srs_rng* rng,
                     void* stream);
+
+/* ---- orthogonalised updates (Newton-Schulz) -------------------------------
+ * No counterpart in the reference.  y = X_steps of
+ *   X_0 = x / (|x|_F + eps);  X_{i+1} = (a I + b G + c G^2) X_i,  G = X_i X_i^T
+ * for `batch` matrices of m rows and n columns (m > n: X_{i+1} = X_i (a I + b G + c G^2),
+ * G = X_i^T X_i).  Products on the tensor cores: FP16 operands, FP32 sums; the
+ * norm is summed in FP64.  x: FP32, BF16 or FP16, element (b, i, j) at
+ * b * batch_stride + i * row_pitch + j; y: contiguous, FP32, BF16 or FP16; x and y
+ * must not overlap.  A matrix with a NaN or infinity, or whose norm plus eps is
+ * zero, gives NaN throughout.  Sizes of zero are a no-op.
+ * `workspace`: srs_newton_workspace(batch, m, n) bytes, 256-byte aligned, not used
+ * by any other call that can overlap in time. */
+#define SRS_NEWTON_MAX_STEPS 32
+typedef struct srs_newton {
+  int32_t steps;         /* 1..SRS_NEWTON_MAX_STEPS */
+  float coefficients[3]; /* a, b, c */
+  float eps;
+} srs_newton;
+
+int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n);
+
+int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch, int64_t batch_stride,
+                      void* y, int y_format, int64_t batch, int64_t m, int64_t n,
+                      const srs_newton* h, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* Muon step of n_rows matrices of one shape (m x n, contiguous): per element, each
+ * FP32 operation rounded once,
+ *   u' = u*momentum + g;  v = nesterov ? u'*momentum + g : u'
+ *   p' = fma(neg_step, O, p*decay),  O = the orthogonalised v of the matrix
+ * u' is stored in u_format by u_rule (counter base state_key(key, 0), as the other
+ * steps).  `rows`: DEVICE array as for srs_adamw_multi; param, grad, state[0],
+ * param_index, offset and flags are used, numel and tile_begin are not.
+ * neg_step = -(lr * the shape's factor), decay = 1 - lr*weight_decay. */
+typedef struct srs_muon_hparams {
+  float momentum, neg_step, decay;
+  int32_t nesterov;
+} srs_muon_hparams;
+
+int srs_muon_multi(const srs_row* rows, int64_t n_rows, int64_t m, int64_t n, int u_format,
+                   int u_rule, const srs_muon_hparams* hp, const srs_newton* h,
+                   const srs_rng* rng, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- FP8 blocks and their products -----------------------------------------
+ * No counterpart in the reference.  A matrix in FP8 blocks is `data` (E4M3 or
+ * E5M2, rows x cols) with one power-of-two scale (UE8M0: byte b stands for
+ * 2^(b-127)) for every 128 consecutive columns of a row (square == 0), or of every
+ * 128 x 128 elements (square == 1); blocks at the edges hold what is left.
+ *
+ * srs_quantize_blocks: per block, k = the smallest exponent >= -127 with
+ * max|finite x| <= largest * 2^k (0 for a block without nonzero finite values);
+ * data = round(x * 2^-k) by `rule` (as srs_cast: infinities saturate, NaN is kept).
+ * `data`/`scale`: of x; `data_t`/`scale_t`: of x transposed (cols x rows, blocks
+ * along x's rows); either pair may be NULL.  Stochastic counters: element (i, j) of
+ * x uses (i*cols + j + offset + state_key(seed, 0)) mod 2^32, its transposed copy
+ * state_key(seed, 1).  x: FP32, BF16 or FP16, element (i, j) at i*x_pitch + j.  Row
+ * pitches of data and data_t are in elements, those of scale and scale_t in blocks.
+ *
+ * srs_matmul_blocks: d[i, j] = sum_k a[i, k] * b[j, k] with FP32 sums, d in FP32,
+ * BF16 or FP16 (contiguous).  The data's base addresses and row pitches must be
+ * multiples of 16 bytes.  k == 0 gives zeros. */
+int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols, int64_t x_pitch,
+                        int out_format, int rule, int square, uint32_t seed, uint32_t offset,
+                        void* data, int64_t data_pitch, void* scale, int64_t scale_pitch,
+                        void* data_t, int64_t data_t_pitch, void* scale_t,
+                        int64_t scale_t_pitch, void* stream);
+
+typedef struct srs_blocks {
+  uint64_t data;  /* device address, row pitch `pitch` bytes */
+  uint64_t scale; /* device address, row pitch `scale_pitch` bytes */
+  int64_t rows, pitch, scale_pitch;
+  int32_t format; /* SRS_FMT_E4M3 or SRS_FMT_E5M2 */
+  int32_t square; /* 1: one scale for 128 rows */
+} srs_blocks;
+
+int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64_t k, void* d, int d_format,
+                      void* stream);
+
+/* Where a bounded wait of a product kernel ran out on the current device (0:
+ * nowhere; results of such a call are not valid).  Synchronises the device. */
+int srs_product_status(uint32_t* status);
 
 #ifdef __cplusplus
 }

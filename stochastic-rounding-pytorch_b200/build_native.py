@@ -47,7 +47,8 @@ FLAGS = [
 
 # (object name, source, extra defines)
 UNITS = [("srs_abi", "srs_abi.cu", []), ("srs_cast", "srs_cast.cu", []),
-         ("srs_sgdm", "srs_sgdm.cu", [])]
+         ("srs_sgdm", "srs_sgdm.cu", []), ("srs_product", "srs_product.cu", []),
+         ("srs_newton", "srs_newton.cu", []), ("srs_blocks", "srs_blocks.cu", [])]
 UNITS += [(f"srs_adamw_m{m}", "srs_adamw.cu", [f"-DSRS_M_FORMAT={m}"]) for m in range(5)]
 
 
@@ -59,7 +60,7 @@ def nvcc() -> str:
 
 
 def _sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "srs_b200.h"]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "srs_b200.h"]
 
 
 def up_to_date() -> bool:

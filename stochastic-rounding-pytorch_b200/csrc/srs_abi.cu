@@ -10,12 +10,21 @@
 
 #include <cuda.h>
 
+#include "srs_host.h"
 #include "srs_kernels.cuh"
 
 namespace srs {
 namespace {
 
 thread_local char g_error[512] = "";
+
+constexpr int kMaxDevices = 128;
+std::mutex g_mutex;
+int g_device_ok[kMaxDevices];  // 0 unknown, 1 usable, -1 unusable
+int g_sm_count[kMaxDevices];
+std::unordered_map<const void*, int> g_blocks_per_sm[kMaxDevices];
+
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -29,11 +38,9 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(SRS_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
 }
 
-constexpr int kMaxDevices = 128;
-std::mutex g_mutex;
-int g_device_ok[kMaxDevices];  // 0 unknown, 1 usable, -1 unusable
-int g_sm_count[kMaxDevices];
-std::unordered_map<const void*, int> g_blocks_per_sm[kMaxDevices];
+void clear_error() { g_error[0] = '\0'; }
+
+namespace {
 
 int current_device(int* dev) {
   const cudaError_t e = cudaGetDevice(dev);
@@ -41,6 +48,8 @@ int current_device(int* dev) {
   if (*dev < 0 || *dev >= kMaxDevices) return fail(SRS_ERR_UNSUPPORTED_DEVICE, "device %d", *dev);
   return SRS_OK;
 }
+
+}  // namespace
 
 int check_device() {
   int dev = 0;
@@ -67,10 +76,14 @@ int check_device() {
   return SRS_OK;
 }
 
-bool valid_format(int f) { return f >= SRS_FMT_F32 && f <= SRS_FMT_E5M2; }
-bool valid_rule(int r) {
-  return r == SRS_RULE_NEAREST || r == SRS_RULE_STOCHASTIC || r == SRS_RULE_TOWARD_ZERO;
+int sm_count() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  return g_sm_count[dev] > 0 ? g_sm_count[dev] : 148;
 }
+
+namespace {
 
 int check_hp_classes(int n) {
   if (n < 1 || n > SRS_MAX_STEP_CLASSES)
@@ -96,8 +109,6 @@ const SgdmLaunch kSgdm[5] = {&launch_sgdm<0>, &launch_sgdm<1>, &launch_sgdm<2>, 
                              &launch_sgdm<4>};
 const CastLaunch kCast[5] = {&launch_cast<0>, &launch_cast<1>, &launch_cast<2>, &launch_cast<3>,
                              &launch_cast<4>};
-
-int fmt_bytes(int f) { return f == SRS_FMT_F32 ? 4 : (f <= SRS_FMT_F16 ? 2 : 1); }
 
 int kind_index(uint32_t uniform_kind) { return uniform_kind <= 3u ? (int)uniform_kind : 4; }
 

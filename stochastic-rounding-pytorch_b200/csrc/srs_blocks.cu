@@ -1,0 +1,362 @@
+// FP8 blocks: quantisation with a power-of-two scale for every 128 elements (or
+// 128 x 128), and the products of such matrices.
+//
+// Why powers of two: scaling is then exact, so an element is rounded once, and
+// the tensor core's block-scaled MMA applies the scales itself (UE8M0), so the
+// product loop has no FP32 work of its own.
+#include "srs_host.h"
+#include "srs_product.cuh"
+
+namespace srs {
+namespace {
+
+constexpr int kBlock = 128;
+
+struct QuantizeArgs {
+  const void* x;
+  int x_format;
+  int64_t rows, cols, x_pitch;
+  int vec;  // x's rows start on 16-byte boundaries
+  int rule;
+  uint32_t ctr, ctr_t;  // counters of element 0 of the copy and of the transposed copy
+  uint8_t* data;
+  uint8_t* scale;
+  uint8_t* data_t;
+  uint8_t* scale_t;
+  int64_t data_pitch, scale_pitch, data_t_pitch, scale_t_pitch;
+};
+
+// Encoding of |x| if finite, else 0 (NaN and infinities do not set a scale).
+__device__ __forceinline__ uint32_t finite_size(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+  return u < 0x7F800000u ? u : 0u;
+}
+
+// k of a block whose largest finite |x| has encoding u: the largest values of
+// both formats are 1.75 * 2^TOP, so k = exponent - TOP, plus one where the
+// significand exceeds 1.75 (adding 0x1FFFFF carries exactly then).
+template <int OF>
+__device__ __forceinline__ int block_exponent(uint32_t u) {
+  constexpr int kTop = OF == SRS_FMT_E4M3 ? 8 : 15;
+  if (u == 0u) return 0;
+  return max((int)((u + 0x1FFFFFu) >> 23) - 127 - kTop, -127);
+}
+
+__device__ __forceinline__ float power_of_two(int k) {  // -126 <= k <= 127
+  return __uint_as_float((uint32_t)(k + 127) << 23);
+}
+
+__device__ __forceinline__ void load_x8(const QuantizeArgs& a, int64_t row, int64_t col,
+                                        float (&x)[kVec]) {
+  const int64_t left = a.cols - col;
+  if (row >= a.rows || left <= 0) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = 0.0f;
+    return;
+  }
+  const int count = left < 8 ? (int)left : 8;
+  const bool vec = a.vec && count == 8;
+  const int64_t at = row * a.x_pitch + col;
+  if (a.x_format == SRS_FMT_F32) load_state8<SRS_FMT_F32>(a.x, at, count, vec, x);
+  else if (a.x_format == SRS_FMT_BF16) load_state8<SRS_FMT_BF16>(a.x, at, count, vec, x);
+  else load_state8<SRS_FMT_F16>(a.x, at, count, vec, x);
+}
+
+// One CTA quantises one 128 x 128 tile of x, read once.  Thread t holds 8 rows x
+// 8 columns in registers: columns 8 * (t % 16) .., rows 8 * (t / 16) .., so a
+// row's block maximum is a reduction over 16 lanes, a column's one over the 16
+// row groups (through shared memory), and the transposed bytes leave as 8 x 8
+// register transposes in 8-byte pieces, swizzled in shared memory so that both
+// sides are conflict-free.  HBM-bound: 2 bytes read and 1 or 2 written an element.
+template <int OF, bool ROWS, bool COLS, bool SQUARE>
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
+  __shared__ uint32_t column_max[COLS && !SQUARE ? 16 * kBlock : 16];
+  __shared__ __align__(16) uint8_t turned[COLS ? kBlock * kBlock : 16];
+  const int lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int64_t row0 = (int64_t)blockIdx.y * kBlock, col0 = (int64_t)blockIdx.x * kBlock;
+  const int64_t row_base = row0 + 8 * group, col = col0 + 8 * lane16;
+
+  float x[8][kVec];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load_x8(a, row_base + i, col, x[i]);
+
+  uint32_t row_top[8], col_top[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) row_top[i] = col_top[i] = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const uint32_t u = finite_size(x[i][j]);
+      if (ROWS || SQUARE) row_top[i] = max(row_top[i], u);
+      if (COLS && !SQUARE) col_top[j] = max(col_top[j], u);
+    }
+  }
+  if constexpr (SQUARE) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, row_top[i]);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if ((threadIdx.x & 31) == 0) column_max[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = 0u;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, column_max[w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row_top[i] = col_top[i] = top;
+  } else {
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+          row_top[i] = max(row_top[i], __shfl_xor_sync(0xFFFFFFFFu, row_top[i], d));
+      }
+    }
+    if constexpr (COLS) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) column_max[group * kBlock + 8 * lane16 + j] = col_top[j];
+      __syncthreads();
+      if (threadIdx.x < kBlock) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) top = max(top, column_max[g * kBlock + threadIdx.x]);
+        column_max[threadIdx.x] = top;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) col_top[j] = column_max[8 * lane16 + j];
+    }
+  }
+
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t row = row_base + i;
+      const int k = block_exponent<OF>(row_top[i]);
+      if (row < a.rows) {
+        const float factor = power_of_two(-k);
+        float y[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) y[j] = x[i][j] * factor;
+        uint32_t w[2];
+        encode8<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, w);
+        if (col < a.data_pitch)
+          *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = make_uint2(w[0], w[1]);
+        if (!SQUARE && lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
+      }
+    }
+    if (SQUARE && threadIdx.x == 0)
+      a.scale[(int64_t)blockIdx.y * a.scale_pitch + blockIdx.x] =
+          (uint8_t)(block_exponent<OF>(row_top[0]) + 127);
+  }
+
+  if constexpr (COLS) {
+    float factor[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) factor[j] = power_of_two(-block_exponent<OF>(col_top[j]));
+    uint32_t w[8][2];  // 8 rows of 8 bytes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float y[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) y[j] = x[i][j] * factor[j];
+      encode8<OF>(y, a.ctr_t + (uint32_t)((row_base + i) * a.cols + col), a.rule, w[i]);
+    }
+    // 8 x 8 byte transpose, then column 8 * lane16 + j gets rows 8 * group .. + 7
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t pick = (uint32_t)j | ((uint32_t)(j + 4) << 4);
+        uint32_t out[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t lo = __byte_perm(w[4 * q][half], w[4 * q + 1][half], pick);
+          const uint32_t hi = __byte_perm(w[4 * q + 2][half], w[4 * q + 3][half], pick);
+          out[q] = __byte_perm(lo, hi, 0x5410u);
+        }
+        const int c = 8 * lane16 + 4 * half + j;
+        *reinterpret_cast<uint2*>(turned + c * kBlock + 8 * (group ^ lane16)) =
+            make_uint2(out[0], out[1]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = 32 * i + (threadIdx.x >> 3), h = threadIdx.x & 7, l = c >> 3;
+      const uint4 v = *reinterpret_cast<const uint4*>(turned + c * kBlock + 16 * (h ^ (l >> 1)));
+      const uint4 o = (l & 1) ? make_uint4(v.z, v.w, v.x, v.y) : v;
+      const int64_t at = row0 + 16 * h;
+      if (col0 + c < a.cols && at < a.data_t_pitch)
+        *reinterpret_cast<uint4*>(a.data_t + (col0 + c) * a.data_t_pitch + at) = o;
+    }
+    if constexpr (SQUARE) {
+      if (threadIdx.x == 0)
+        a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] =
+            (uint8_t)(block_exponent<OF>(col_top[0]) + 127);
+    } else if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (col + j < a.cols)
+          a.scale_t[(col + j) * a.scale_t_pitch + blockIdx.y] =
+              (uint8_t)(block_exponent<OF>(col_top[j]) + 127);
+    }
+  }
+}
+
+template <int OF, bool SQUARE>
+void launch_quantize(const QuantizeArgs& a, dim3 grid, cudaStream_t stream) {
+  if (a.data != nullptr && a.data_t != nullptr)
+    quantize_kernel<OF, true, true, SQUARE><<<grid, kThreads, 0, stream>>>(a);
+  else if (a.data != nullptr)
+    quantize_kernel<OF, true, false, SQUARE><<<grid, kThreads, 0, stream>>>(a);
+  else
+    quantize_kernel<OF, false, true, SQUARE><<<grid, kThreads, 0, stream>>>(a);
+}
+
+uint32_t host_h32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x7FEB352Du;
+  x ^= x >> 15;
+  x *= 0x846CA68Bu;
+  return x ^ (x >> 16);
+}
+
+int64_t blocks_of(int64_t x) { return (x + kBlock - 1) / kBlock; }
+
+int check_copy(const char* what, const void* data, int64_t pitch, const void* scale,
+               int64_t scale_pitch, int64_t cols) {
+  if (scale == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "%s has data but no scale", what);
+  if (reinterpret_cast<uintptr_t>(data) % 16 != 0 || pitch % 16 != 0 || pitch < cols)
+    return fail(SRS_ERR_INVALID_ARGUMENT,
+                "%s needs a 16-byte aligned address and a row pitch that is a multiple of 16 and "
+                "at least the row length (%lld, %lld)",
+                what, (long long)pitch, (long long)cols);
+  if (scale_pitch < blocks_of(cols))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "%s: scale pitch %lld, %lld blocks a row", what,
+                (long long)scale_pitch, (long long)blocks_of(cols));
+  return SRS_OK;
+}
+
+int check_operand(const char* what, const srs_blocks* b, int64_t k) {
+  if (b == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null operand %s", what);
+  if (b->format != SRS_FMT_E4M3 && b->format != SRS_FMT_E5M2)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "operand %s: unknown format %d", what, b->format);
+  if (b->rows < 0 || b->rows > (1ll << 30))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "operand %s: %lld rows", what, (long long)b->rows);
+  if (b->rows == 0 || k == 0) return SRS_OK;
+  if (b->data == 0 || b->scale == 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "operand %s: null address", what);
+  if (b->data % 16 != 0 || b->pitch % 16 != 0 || b->pitch < k)
+    return fail(SRS_ERR_INVALID_ARGUMENT,
+                "operand %s needs a 16-byte aligned address and a row pitch that is a multiple "
+                "of 16 and at least k (%lld, %lld)",
+                what, (long long)b->pitch, (long long)k);
+  if (b->scale_pitch < blocks_of(k))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "operand %s: scale pitch %lld, %lld blocks a row", what,
+                (long long)b->scale_pitch, (long long)blocks_of(k));
+  return SRS_OK;
+}
+
+}  // namespace
+}  // namespace srs
+
+using namespace srs;
+
+extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
+                                   int64_t x_pitch, int out_format, int rule, int square,
+                                   uint32_t seed, uint32_t offset, void* data, int64_t data_pitch,
+                                   void* scale, int64_t scale_pitch, void* data_t,
+                                   int64_t data_t_pitch, void* scale_t, int64_t scale_t_pitch,
+                                   void* stream) {
+  clear_error();
+  if (x_format < SRS_FMT_F32 || x_format > SRS_FMT_F16)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported input format %d", x_format);
+  if (out_format != SRS_FMT_E4M3 && out_format != SRS_FMT_E5M2)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "unknown output format %d (E4M3 or E5M2)", out_format);
+  if (!valid_rule(rule)) return fail(SRS_ERR_INVALID_ARGUMENT, "unknown rounding rule %d", rule);
+  if (rows < 0 || cols < 0 || x_pitch < 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "negative size or pitch");
+  if (rows > 65535ll * kBlock || cols > (1ll << 30))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "%lld x %lld is too large", (long long)rows,
+                (long long)cols);
+  if (data == nullptr && data_t == nullptr)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "null outputs");
+  if (rows == 0 || cols == 0) return SRS_OK;
+  if (x == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null input pointer");
+  if (reinterpret_cast<uintptr_t>(x) % fmt_bytes(x_format) != 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "input pointer is not element aligned");
+  if (data != nullptr)
+    if (int rc = check_copy("the copy", data, data_pitch, scale, scale_pitch, cols)) return rc;
+  if (data_t != nullptr)
+    if (int rc = check_copy("the transposed copy", data_t, data_t_pitch, scale_t, scale_t_pitch,
+                            rows))
+      return rc;
+  if (int rc = check_device()) return rc;
+  QuantizeArgs a{};
+  a.x = x;
+  a.x_format = x_format;
+  a.rows = rows;
+  a.cols = cols;
+  a.x_pitch = x_pitch;
+  a.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_pitch % 8 == 0;
+  a.rule = rule;
+  a.ctr = offset + host_h32(seed);
+  a.ctr_t = offset + host_h32(seed ^ 1u);
+  a.data = static_cast<uint8_t*>(data);
+  a.scale = static_cast<uint8_t*>(scale);
+  a.data_t = static_cast<uint8_t*>(data_t);
+  a.scale_t = static_cast<uint8_t*>(scale_t);
+  a.data_pitch = data_pitch;
+  a.scale_pitch = scale_pitch;
+  a.data_t_pitch = data_t_pitch;
+  a.scale_t_pitch = scale_t_pitch;
+  const dim3 grid((unsigned)blocks_of(cols), (unsigned)blocks_of(rows));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (out_format == SRS_FMT_E4M3) {
+    if (square) launch_quantize<SRS_FMT_E4M3, true>(a, grid, st);
+    else launch_quantize<SRS_FMT_E4M3, false>(a, grid, st);
+  } else {
+    if (square) launch_quantize<SRS_FMT_E5M2, true>(a, grid, st);
+    else launch_quantize<SRS_FMT_E5M2, false>(a, grid, st);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_quantize_blocks launch");
+}
+
+extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64_t k, void* d,
+                                 int d_format, void* stream) {
+  clear_error();
+  if (d_format < SRS_FMT_F32 || d_format > SRS_FMT_F16)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported result format %d", d_format);
+  if (k < 0 || k > (1ll << 30))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "k must be in [0, 2^30], got %lld", (long long)k);
+  if (int rc = check_operand("a", a, k)) return rc;
+  if (int rc = check_operand("b", b, k)) return rc;
+  if (a->rows == 0 || b->rows == 0) return SRS_OK;
+  if (d == nullptr || reinterpret_cast<uintptr_t>(d) % fmt_bytes(d_format) != 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
+  if (int rc = check_device()) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (k == 0) {
+    const cudaError_t e =
+        cudaMemsetAsync(d, 0, (size_t)a->rows * b->rows * fmt_bytes(d_format), st);
+    return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_matmul_blocks");
+  }
+  ProductArgs args{};
+  args.scale_a = reinterpret_cast<const uint8_t*>(a->scale);
+  args.scale_b = reinterpret_cast<const uint8_t*>(b->scale);
+  args.scale_a_pitch = a->scale_pitch;
+  args.scale_b_pitch = b->scale_pitch;
+  args.scale_a_shift = a->square ? 7 : 0;
+  args.scale_b_shift = b->square ? 7 : 0;
+  args.e.alpha = 1.0f;
+  args.e.out = d;
+  args.e.out_format = d_format;
+  args.e.ldd = b->rows;
+  args.e.batch_stride = a->rows * b->rows;
+  const ProductOperand oa{reinterpret_cast<const void*>(a->data), a->rows, k, a->pitch, 0, false};
+  const ProductOperand ob{reinterpret_cast<const void*>(b->data), b->rows, k, b->pitch, 0, false};
+  return launch_product(kOperandF8, kEpilogueStore, oa, ob, 1, a->format, b->format, args, st);
+}

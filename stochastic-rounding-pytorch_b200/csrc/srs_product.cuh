@@ -1,0 +1,704 @@
+// Matrix products on the sm_100a tensor cores (tcgen05, accumulators in TMEM):
+//
+//   D[i, j] = sum_k A[i, k] * B[j, k]      (A: M x K, B: N x K, FP32 accumulation)
+//
+// for FP16 operands, each stored with k or with its row index contiguous, and
+// for FP8 operands (k contiguous) whose blocks of 128 along k carry a
+// power-of-two scale that the tensor core applies (block-scaled MMA).
+//
+// What bounds it: the MMA rate for large products, and the bytes a tile pulls
+// through L2.  A tile of R x C costs (R + C) * 128 B of loads per 128-byte
+// slice of k, so the large form pairs two CTAs (cta_group::2) on a 256 x 256
+// tile: each CTA loads 128 rows of A and 128 rows of B per slice, 32 KB for
+// 512 cycles of MMA.  The small form (one CTA, 128 x 128) keeps the SMs busy
+// when there are too few large tiles; the launcher chooses by tile count.
+//
+// A CTA has 8 warps: warps 0-3 read the accumulator and write the result
+// (warp w owns TMEM lanes 32w..32w+31, one row of the tile per lane), warp 4
+// issues the TMA loads, warp 5 the MMAs, warp 6 stages the FP8 block scales.
+// Grids are persistent; the accumulator is double-buffered in TMEM so that one
+// tile's result is written while the next is computed.
+//
+// Every wait is bounded: a role that waits longer than kWaitCycles records
+// where in *status, stops, and the CTA leaves after its copies had time to land.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "srs_common.cuh"
+
+namespace srs {
+
+constexpr int kSliceBytes = 128;        // bytes of k per pipeline stage and row (one swizzle row)
+constexpr int kProductThreads = 256;
+constexpr int kStages = 6;
+constexpr int kScaleSlots = 3;          // ring of scale groups (each covers 4 slices)
+constexpr int kPanelBytes = 128 * kSliceBytes;  // 128 rows of an operand per stage
+constexpr int kStageRowPitch = 33;      // floats per staged row of 32 (bank-conflict free)
+constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
+
+enum : int { kOperandF16 = 0, kOperandF8 = 1 };
+enum : int { kEpilogueSymmetric = 0, kEpilogueStore = 1, kEpilogueMuon = 2 };
+
+// What happens to the accumulator.
+struct ProductEpilogue {
+  const float* rho;  // per batch entry: the operand X stands for X / rho (null: 1)
+  int rho_power;     // 1 or 2
+  float alpha;       // factor of the accumulator
+  float beta;        // symmetric: factor of `addend`
+  float diagonal;    // symmetric: added where i == j
+  const __half* addend;  // symmetric: M x M, row pitch ldd (null: none)
+  void* out;
+  int out_format;     // SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
+  int64_t ldd;        // row pitch of out (elements)
+  int64_t batch_stride;  // batch pitch of out (elements)
+  const srs_row* rows;   // Muon: one row per batch entry (param address, dtype flag)
+  float decay;        // Muon: p' = fma(step, D, p * decay)
+  float step;
+};
+
+struct ProductArgs {
+  int m, n, k;        // elements
+  int tiles_m, tiles_n;  // tiles per batch entry
+  int64_t n_tiles;    // over the batch
+  int64_t tiles_per_entry;
+  int symmetric;      // only tiles on and below the diagonal are computed
+  uint32_t idesc;     // MMA instruction descriptor without scale ids
+  int a_rows_inner;   // operand A is stored with its row index contiguous
+  int b_rows_inner;
+  // FP8: scales of A and B (UE8M0), row pitch in blocks; shift 7 when one scale
+  // covers 128 rows, else 0
+  const uint8_t* scale_a;
+  const uint8_t* scale_b;
+  int64_t scale_a_pitch, scale_b_pitch;
+  int scale_a_shift, scale_b_shift;
+  unsigned int* status;
+  ProductEpilogue e;
+};
+
+// ------------------------------------------------------------ PTX wrappers --
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// shared::cluster address of `addr` (a shared::cta address) in CTA `rank`.
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+
+// Arrive on a barrier given by its shared::cluster address.
+__device__ __forceinline__ void barrier_arrive(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// Bounded wait for the completion of the phase of `parity`; false (and `where`
+// recorded) when it did not come.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsigned int* status,
+                                             unsigned int where) {
+  if (barrier_try(bar, parity)) return true;
+  const long long start = clock64();
+  while (!barrier_try(bar, parity)) {
+    if (clock64() - start > kWaitCycles) {
+      atomicOr(status, where);
+      return false;
+    }
+  }
+  return true;
+}
+
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t cluster_bar) {
+  if constexpr (CG == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+        "bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t columns) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+
+// Arrive on `bar` (same offset in every CTA of the group) once all MMAs and
+// copies issued so far by this thread are done.
+template <int CG>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (CG == 2) {
+    const uint16_t both = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"(both)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if constexpr (CG == 2) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  if constexpr (CG == 2) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], "
+        "p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], "
+        "p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 32 lanes x 16 bytes of shared memory into 4 TMEM columns, repeated for the
+// four groups of 32 lanes (the layout block scales are read in).
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc)
+                 : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc)
+                 : "memory");
+}
+
+// 32 accumulator columns of this warp's 32 lanes: v[c] = D[lane, column + c].
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// Shared-memory matrix descriptors (sm_100 format: version 1 at bit 46, the
+// swizzle mode at bits 61-63, addresses and offsets in 16-byte units).
+//
+// k contiguous: rows of 128 bytes, 128-byte swizzle; groups of 8 rows are 1024
+// bytes apart.  Row index contiguous: 64 rows (128 bytes) x 64 k per box; groups
+// of 8 k are 1024 bytes apart (stride offset), boxes 8192 bytes (leading offset).
+__device__ __forceinline__ uint64_t operand_descriptor(bool rows_inner) {
+  const uint64_t lead = rows_inner ? 8192u >> 4 : 1u;
+  return (lead << 16) | (uint64_t(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Scale blocks: unswizzled 8 x 16-byte core matrices, 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_descriptor(uint32_t addr) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (1ull << 16) | (uint64_t(128u >> 4) << 32) |
+         (1ull << 46);
+}
+
+// ------------------------------------------------------------------- tiles --
+
+struct TileAt {
+  int batch, m, n;  // tile coordinates
+};
+
+// Tiles of an entry in bands of 8 tile rows, column by column within a band, so
+// that the CTAs running at one time share rows of A and B in L2.
+__device__ __forceinline__ TileAt tile_at(const ProductArgs& a, int64_t t) {
+  TileAt r;
+  r.batch = (int)(t / a.tiles_per_entry);
+  const int64_t i = t - (int64_t)r.batch * a.tiles_per_entry;
+  if (a.symmetric) {
+    int row = (int)((sqrtf(8.0f * (float)i + 1.0f) - 1.0f) * 0.5f);
+    while ((int64_t)(row + 1) * (row + 2) / 2 <= i) ++row;
+    while ((int64_t)row * (row + 1) / 2 > i) --row;
+    r.m = row;
+    r.n = (int)(i - (int64_t)row * (row + 1) / 2);
+  } else {
+    const int64_t band = 8ll * a.tiles_n;
+    const int first = (int)(i / band) * 8;
+    const int rows = min(8, a.tiles_m - first);
+    const int j = (int)(i % band);
+    r.m = first + j % rows;
+    r.n = j / rows;
+  }
+  return r;
+}
+
+// ---------------------------------------------------------------- epilogue --
+
+__device__ __forceinline__ void store_as(void* out, int format, int64_t at, float v) {
+  if (format == SRS_FMT_F32) static_cast<float*>(out)[at] = v;
+  else if (format == SRS_FMT_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(out)[at] = __float2half_rn(v);
+}
+
+// One chunk of 32 columns: lane = tile row on entry (v[c] = D[row0 + lane, col0 + c]).
+// Values pass through the warp's shared rows so that a store covers 32
+// consecutive columns of one row, whatever the row pitch and alignment.
+template <int EPILOGUE>
+__device__ __forceinline__ void write_chunk(const ProductArgs& a, float (&v)[32], int batch,
+                                            int row0, int col0, bool mirror, float factor,
+                                            float* staged, int lane) {
+  const ProductEpilogue& e = a.e;
+  const int row = row0 + lane;
+  if constexpr (EPILOGUE == kEpilogueSymmetric) {
+    __half* out = static_cast<__half*>(e.out) + (int64_t)batch * e.batch_stride;
+    const __half* addend =
+        e.addend == nullptr ? nullptr : e.addend + (int64_t)batch * e.batch_stride;
+    const bool inside = row < a.m;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      float x = v[c] * factor;
+      // addend is symmetric: its transposed element is the coalesced one
+      if (addend != nullptr && inside && col0 + c < a.n)
+        x = fmaf(e.beta, __half2float(addend[(int64_t)(col0 + c) * e.ldd + row]), x);
+      if (row == col0 + c) x += e.diagonal;
+      v[c] = x;
+    }
+    if (mirror && inside) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (col0 + c < a.n) out[(int64_t)(col0 + c) * e.ldd + row] = __float2half_rn(v[c]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] *= factor;
+  }
+#pragma unroll
+  for (int c = 0; c < 32; ++c) staged[lane * kStageRowPitch + c] = v[c];
+  __syncwarp();
+  const int col = col0 + lane;
+  const int rows = min(32, a.m - row0);
+  if (col < a.n) {
+    if constexpr (EPILOGUE == kEpilogueMuon) {
+      const srs_row& target = e.rows[batch];
+      const bool bf16 = (target.flags & SRS_ROW_PARAM_BF16) != 0u;
+      int64_t at = (int64_t)row0 * a.n + col;
+      for (int r = 0; r < rows; ++r, at += a.n) {
+        const float d = staged[r * kStageRowPitch + lane];
+        if (bf16) {
+          __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(target.param) + at;
+          *p = __float2bfloat16_rn(fmaf(e.step, d, __fmul_rn(__bfloat162float(*p), e.decay)));
+        } else {
+          float* p = reinterpret_cast<float*>(target.param) + at;
+          *p = fmaf(e.step, d, __fmul_rn(*p, e.decay));
+        }
+      }
+    } else {
+      int64_t at = (int64_t)batch * e.batch_stride + (int64_t)row0 * e.ldd + col;
+      for (int r = 0; r < rows; ++r, at += e.ldd)
+        store_as(e.out, EPILOGUE == kEpilogueSymmetric ? SRS_FMT_F16 : e.out_format, at,
+                 staged[r * kStageRowPitch + lane]);
+    }
+  }
+  __syncwarp();
+}
+
+// ------------------------------------------------------------------ kernel --
+
+template <int KIND, int CG>
+struct ProductShape {
+  static constexpr int kTileRows = 128 * CG;  // over the CTA group
+  static constexpr int kTileCols = 128 * CG;
+  static constexpr int kScaleBytes = KIND == kOperandF8 ? 512 * (1 + CG) : 0;  // per slot
+  // Accumulator 1 starts after accumulator 0, except that for FP8 pairs both
+  // accumulators and the scales do not fit 512 columns: they then share 32
+  // columns, which the writing warps drain first.
+  static constexpr int kShared = (KIND == kOperandF8 && CG == 2) ? 32 : 0;
+  static constexpr int kSecond = kTileCols - kShared;
+  static constexpr int kScaleColumn = 480;  // 2 slots of 12 columns (pitch 16)
+  static constexpr int kStageBytes = 2 * kPanelBytes;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes +
+                               4 * 32 * kStageRowPitch * 4;
+};
+
+template <int KIND, int CG, int EPILOGUE>
+__global__ void __launch_bounds__(kProductThreads, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ ProductArgs a) {
+  using S = ProductShape<KIND, CG>;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4 + 2 * kScaleSlots];
+  __shared__ uint32_t tmem_slot;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  const uint32_t stage0 = (smem_address(raw) + 1023u) & ~1023u;
+  const uint32_t scales0 = stage0 + kStages * S::kStageBytes;
+  float* staged = reinterpret_cast<float*>(
+      raw + (stage0 - smem_address(raw)) + kStages * S::kStageBytes + kScaleSlots * S::kScaleBytes +
+      (warp & 3) * 32 * kStageRowPitch * 4);
+
+  const uint32_t bar0 = smem_address(bars);
+  const auto full = [&](int s) { return bar0 + 8u * s; };
+  const auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  const auto acc_full = [&](int i) { return bar0 + 8u * (2 * kStages + i); };
+  const auto acc_empty = [&](int i) { return bar0 + 8u * (2 * kStages + 2 + i); };
+  const auto scale_full = [&](int i) { return bar0 + 8u * (2 * kStages + 4 + i); };
+  const auto scale_empty = [&](int i) { return bar0 + 8u * (2 * kStages + 4 + kScaleSlots + i); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      barrier_init(full(s), 1);
+      barrier_init(empty(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(acc_full(i), 1);
+      barrier_init(acc_empty(i), 4 * CG);
+    }
+    for (int i = 0; i < kScaleSlots; ++i) {
+      barrier_init(scale_full(i), CG);
+      barrier_init(scale_empty(i), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) tmem_alloc<CG>(smem_address(&tmem_slot), 512);
+  tmem_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  constexpr int kSliceK = KIND == kOperandF8 ? 128 : 64;  // elements of k per stage
+  const int slices = (a.k + kSliceK - 1) / kSliceK;
+  bool ok = true;
+
+  if (warp == 4 && lane == 0) {
+    // ---- TMA loads: this CTA's 128 rows of A and of B per slice
+    int s = 0;
+    uint32_t phase = 0;
+    for (int64_t t = first; t < a.n_tiles && ok; t += step) {
+      const TileAt at = tile_at(a, t);
+      const int ra = at.m * S::kTileRows + 128 * (int)rank;
+      const int rb = at.n * S::kTileCols + 128 * (int)rank;
+      for (int i = 0; i < slices; ++i) {
+        ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u);
+        if (!ok) break;
+        if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
+        const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
+        const uint32_t pa = stage0 + s * S::kStageBytes, pb = pa + kPanelBytes;
+        const int k = i * kSliceK;
+        if (a.a_rows_inner) {
+          load_box<CG>(pa, &map_a, ra, k, at.batch, bar);
+          load_box<CG>(pa + kPanelBytes / 2, &map_a, ra + 64, k, at.batch, bar);
+        } else {
+          load_box<CG>(pa, &map_a, k, ra, at.batch, bar);
+        }
+        if (a.b_rows_inner) {
+          load_box<CG>(pb, &map_b, rb, k, at.batch, bar);
+          load_box<CG>(pb + kPanelBytes / 2, &map_b, rb + 64, k, at.batch, bar);
+        } else {
+          load_box<CG>(pb, &map_b, k, rb, at.batch, bar);
+        }
+        if (++s == kStages) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // Every stage given back (its commit has reached this CTA) before leaving.
+    for (int i = 0; i < kStages && ok; ++i) {
+      ok = barrier_wait(empty(s), phase ^ 1u, a.status, 2u);
+      if (++s == kStages) {
+        s = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp == 5 && lane == 0 && rank == 0) {
+    // ---- MMAs (the pair's leader issues for both CTAs)
+    const uint64_t desc_a = operand_descriptor(a.a_rows_inner != 0);
+    const uint64_t desc_b = operand_descriptor(a.b_rows_inner != 0);
+    // bytes per MMA step of k (32 bytes; 16 rows of 128 bytes when rows are inner)
+    const uint32_t step_a = (a.a_rows_inner ? 2048u : 32u) >> 4;
+    const uint32_t step_b = (a.b_rows_inner ? 2048u : 32u) >> 4;
+    int s = 0, slot = 0, last_slot = -1, count = 0;
+    uint32_t phase = 0, slot_phase = 0, last_phase = 0, group = 0;
+    for (int64_t t = first; t < a.n_tiles && ok; t += step, ++count) {
+      const int acc = count & 1;
+      const uint32_t d = tmem + acc * S::kSecond;
+      // The accumulator was drained two tiles ago; with shared columns, the
+      // previous tile's first chunk must have been drained too (acc_empty of
+      // that accumulator is then signalled after its shared columns).
+      if (S::kShared == 0) {
+        if (count >= 2) ok = barrier_wait(acc_empty(acc), ((count >> 1) - 1) & 1u, a.status, 4u);
+      } else {
+        if (count >= 1) ok = barrier_wait(acc_empty(acc ^ 1), ((count - 1) >> 1) & 1u, a.status, 4u);
+      }
+      tmem_fence_after();
+      for (int i = 0; i < slices && ok; ++i) {
+        uint32_t scale_tmem = 0;
+        if constexpr (KIND == kOperandF8) {
+          scale_tmem = tmem + S::kScaleColumn + 16u * (group & 1u);
+          if ((i & 3) == 0) {
+            // This group's TMEM columns were last read by the MMAs of the group
+            // before the previous one; they are done once the commit that
+            // followed the previous group's copy has arrived.
+            if (last_slot >= 0) ok = barrier_wait(scale_empty(last_slot), last_phase, a.status, 8u);
+            ok = ok && barrier_wait(scale_full(slot), slot_phase, a.status, 8u);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t src = scales0 + slot * S::kScaleBytes;
+#pragma unroll
+            for (int c = 0; c < 1 + CG; ++c)
+              copy_scales<CG>(scale_tmem + 4 * c, scale_descriptor(src + 512 * c));
+            mma_commit<CG>(scale_empty(slot));
+            last_slot = slot;
+            last_phase = slot_phase;
+            if (++slot == kScaleSlots) {
+              slot = 0;
+              slot_phase ^= 1u;
+            }
+          }
+        }
+        ok = barrier_wait(full(s), phase, a.status, 16u);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t pa = stage0 + s * S::kStageBytes;
+        const uint64_t da = desc_a | uint64_t((pa >> 4) & 0x3FFFu);
+        const uint64_t db = desc_b | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t accumulate = (i | j) != 0 ? 1u : 0u;
+          if constexpr (KIND == kOperandF8) {
+            const uint32_t id = (uint32_t)(i & 3);
+            mma_f8<CG>(d, da + j * step_a, db + j * step_b, a.idesc | (id << 29) | (id << 4),
+                       scale_tmem, scale_tmem + 4, accumulate);
+          } else {
+            mma_f16<CG>(d, da + j * step_a, db + j * step_b, a.idesc, accumulate);
+          }
+        }
+        mma_commit<CG>(empty(s));
+        if (++s == kStages) {
+          s = 0;
+          phase ^= 1u;
+        }
+        if (KIND == kOperandF8 && ((i & 3) == 3 || i == slices - 1)) ++group;
+      }
+      if (ok) mma_commit<CG>(acc_full(acc));
+    }
+  } else if (KIND == kOperandF8 && warp == 6) {
+    // ---- block scales: words of 4 consecutive scales (512 elements of k) per
+    // row, row r at 16 * (r % 32) + 4 * (r / 32) of its 512-byte group, the order
+    // in which the tensor core reads them from 4 TMEM columns
+    int slot = 0;
+    uint32_t phase = 0;
+    const auto word = [&](const uint8_t* scale, int64_t pitch, int shift, int row, int rows,
+                          int kb) {
+      uint32_t w = 0x7F7F7F7Fu;  // scale 1 outside the matrix
+      if (row < rows) {
+        const uint8_t* p = scale + (int64_t)(row >> shift) * pitch;
+        w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w |= (kb + j < slices ? (uint32_t)__ldg(p + kb + j) : 0x7Fu) << (8 * j);
+      }
+      return w;
+    };
+    for (int64_t t = first; t < a.n_tiles && ok; t += step) {
+      const TileAt at = tile_at(a, t);
+      const int ra = at.m * S::kTileRows + 128 * (int)rank;
+      const int rb = at.n * S::kTileCols;
+      for (int kb = 0; kb < slices; kb += 4) {
+        uint32_t w[1 + CG][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[0][j] = word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra + lane + 32 * j, a.m, kb);
+#pragma unroll
+          for (int c = 0; c < CG; ++c)
+            w[1 + c][j] = word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
+                               rb + 128 * c + lane + 32 * j, a.n, kb);
+        }
+        ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 32u);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        const uint32_t dst = scales0 + slot * S::kScaleBytes + 16u * lane;
+#pragma unroll
+        for (int c = 0; c < 1 + CG; ++c)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 * c),
+                       "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
+                       : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive(map_to_rank(scale_full(slot), 0));
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    for (int i = 0; i < kScaleSlots && ok; ++i) {
+      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 64u);
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp < 4) {
+    // ---- results
+    int count = 0;
+    for (int64_t t = first; t < a.n_tiles && ok; t += step, ++count) {
+      const TileAt at = tile_at(a, t);
+      const int acc = count & 1;
+      float factor = a.e.alpha;
+      if (a.e.rho != nullptr) {
+        const float r = __ldg(a.e.rho + at.batch);
+        factor = __fdiv_rn(factor, a.e.rho_power == 2 ? __fmul_rn(r, r) : r);
+      }
+      ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, a.status, 128u);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tmem_fence_after();
+      const uint32_t src = tmem + acc * S::kSecond + ((uint32_t)(warp * 32) << 16);
+      const int row0 = at.m * S::kTileRows + 128 * (int)rank + 32 * warp;
+      const int col0 = at.n * S::kTileCols;
+      const bool mirror = a.symmetric != 0 && at.m != at.n;
+      constexpr int kChunks = S::kTileCols / 32;
+      for (int i = 0; i < kChunks; ++i) {
+        // accumulator 0 gives its last (shared) columns first
+        const int c = (S::kShared != 0 && acc == 0) ? kChunks - 1 - i : i;
+        float v[32];
+        tmem_load32(src + 32 * c, v);
+        if (i == (S::kShared != 0 ? 0 : kChunks - 1)) {
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            barrier_arrive(map_to_rank(acc_empty(acc), 0));
+        }
+        if (row0 < a.m && col0 + 32 * c < a.n)
+          write_chunk<EPILOGUE>(a, v, at.batch, row0, col0 + 32 * c, mirror, factor, staged, lane);
+      }
+    }
+  }
+  __syncwarp();
+  if (!ok) {
+    // A wait ran out: give copies and MMAs already issued time to finish before
+    // shared memory and TMEM are given up.
+    const long long start = clock64();
+    while (clock64() - start < 4000000ll) {
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  tmem_fence_after();
+  if (warp == 5) tmem_free<CG>(tmem, 512);
+}
+
+// An operand in global memory: `rows` x `k` per batch entry.  k contiguous: row
+// pitch `pitch` elements; rows_inner: element (i, k) at k * pitch + i.
+struct ProductOperand {
+  const void* base;
+  int64_t rows, k, pitch, batch_stride;  // elements
+  bool rows_inner;
+};
+
+// Enqueues D = A B^T with the given epilogue over `batch` entries (srs_product.cu).
+// `args` carries the epilogue, the scales and the symmetric flag; the rest is
+// filled in.  Returns SRS_OK or an error code with its text set.
+int launch_product(int kind, int epilogue, const ProductOperand& a, const ProductOperand& b,
+                   int64_t batch, int a_format, int b_format, ProductArgs args,
+                   cudaStream_t stream);
+
+}  // namespace srs

@@ -9,9 +9,20 @@ registry, RNG step, checkpoints) and calls the kernels through a C ABI.
 from .formats import StateFormat
 from .optim._state import StateOptimizer
 from .optim.adamw import AdamWReferenceRN, AdamWReferenceSR
+from .optim.muon import MuonRN, MuonSR
 from .optim.sgd import SGDMReferenceRN, SGDMReferenceSR
 from .rounding import cast, register_rounding
+from .blocks import (  # noqa: E402 (after the registry its rounding rules come from)
+    BlockLinear,
+    BlockTensor,
+    block_linear,
+    matmul_blocks,
+    quantize_blocks,
+)
+from .cuda.muon import orthogonalize
 
+# A star import gives the reference's names; the package's own additions (Muon,
+# orthogonalize, FP8 blocks) are attributes of the package beside them.
 __all__ = [
     "AdamWReferenceRN",
     "AdamWReferenceSR",

@@ -67,6 +67,24 @@ class SrsSgdmHparams(ctypes.Structure):
     _fields_ = [("momentum", ctypes.c_float), ("neg_lr", ctypes.c_float)]
 
 
+class SrsNewton(ctypes.Structure):
+    _fields_ = [("steps", ctypes.c_int32), ("coefficients", ctypes.c_float * 3),
+                ("eps", ctypes.c_float)]
+
+
+class SrsMuonHparams(ctypes.Structure):
+    _fields_ = [("momentum", ctypes.c_float), ("neg_step", ctypes.c_float),
+                ("decay", ctypes.c_float), ("nesterov", ctypes.c_int32)]
+
+
+class SrsBlocks(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_uint64), ("scale", ctypes.c_uint64),
+                ("rows", ctypes.c_int64), ("pitch", ctypes.c_int64),
+                ("scale_pitch", ctypes.c_int64), ("format", ctypes.c_int32),
+                ("square", ctypes.c_int32)]
+
+
+NEWTON_MAX_STEPS = 32
 MAX_PEERS = 7
 IPC_HANDLE_BYTES = 64
 
@@ -128,6 +146,20 @@ _SIGNATURES = {
     "srs_ipc_export": ([_P, _P, ctypes.POINTER(ctypes.c_uint64)], ctypes.c_int),
     "srs_ipc_import": ([_P, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "srs_ipc_close": ([_P], ctypes.c_int),
+    "srs_newton_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+    "srs_orthogonalize": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int,
+                           ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                           ctypes.POINTER(SrsNewton), _P, ctypes.c_int64, _P], ctypes.c_int),
+    "srs_muon_multi": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                        ctypes.c_int, ctypes.POINTER(SrsMuonHparams), ctypes.POINTER(SrsNewton),
+                        ctypes.POINTER(SrsRng), _P, ctypes.c_int64, _P], ctypes.c_int),
+    "srs_quantize_blocks": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_uint32,
+                             ctypes.c_uint32, _P, ctypes.c_int64, _P, ctypes.c_int64, _P,
+                             ctypes.c_int64, _P, ctypes.c_int64, _P], ctypes.c_int),
+    "srs_matmul_blocks": ([ctypes.POINTER(SrsBlocks), ctypes.POINTER(SrsBlocks), ctypes.c_int64,
+                           _P, ctypes.c_int, _P], ctypes.c_int),
+    "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
 }
 NOALLOC_MAX_ROWS = 4096
 ABI_VERSION = 6
@@ -286,6 +318,38 @@ class NativeLauncher:
 
     def derive_keys(self, index_ptr, out_ptr, n, rng, stream):
         _check(load_library().srs_derive_keys(index_ptr, out_ptr, n, ctypes.byref(rng), stream))
+
+    def newton_workspace(self, batch, m, n) -> int:
+        return int(load_library().srs_newton_workspace(batch, m, n))
+
+    def orthogonalize(self, x_ptr, x_fmt, row_pitch, batch_stride, y_ptr, y_fmt, batch, m, n,
+                      newton, workspace, stream):
+        _check(load_library().srs_orthogonalize(
+            x_ptr, x_fmt, row_pitch, batch_stride, y_ptr, y_fmt, batch, m, n,
+            ctypes.byref(newton), workspace.data_ptr(), workspace.numel(), stream))
+
+    def muon_multi(self, rows_ptr, n_rows, m, n, u_fmt, u_rule, hp, newton, rng, workspace,
+                   stream):
+        _check(load_library().srs_muon_multi(
+            rows_ptr, n_rows, m, n, u_fmt, u_rule, ctypes.byref(hp), ctypes.byref(newton),
+            ctypes.byref(rng), workspace.data_ptr(), workspace.numel(), stream))
+
+    def quantize_blocks(self, x_ptr, x_fmt, rows, cols, x_pitch, fmt, rule, square, seed, offset,
+                        data, data_pitch, scale, scale_pitch, data_t, data_t_pitch, scale_t,
+                        scale_t_pitch, stream):
+        _check(load_library().srs_quantize_blocks(
+            x_ptr, x_fmt, rows, cols, x_pitch, fmt, rule, square, seed, offset, data, data_pitch,
+            scale, scale_pitch, data_t, data_t_pitch, scale_t, scale_t_pitch, stream))
+
+    def matmul_blocks(self, a, b, k, d_ptr, d_fmt, stream):
+        _check(load_library().srs_matmul_blocks(ctypes.byref(a), ctypes.byref(b), k, d_ptr,
+                                                d_fmt, stream))
+
+    def product_status(self) -> int:
+        """Where a bounded wait of a product kernel ran out (0: nowhere); synchronises."""
+        status = ctypes.c_uint32()
+        _check(load_library().srs_product_status(ctypes.byref(status)))
+        return int(status.value)
 
 
 _launcher = NativeLauncher()
