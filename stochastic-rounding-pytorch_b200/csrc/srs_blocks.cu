@@ -4,6 +4,8 @@
 // Why powers of two: scaling is then exact, so an element is rounded once, and
 // the tensor core's block-scaled MMA applies the scales itself (UE8M0), so the
 // product loop has no FP32 work of its own.
+#include <utility>
+
 #include "srs_host.h"
 #include "srs_product.cuh"
 
@@ -14,7 +16,6 @@ constexpr int kBlock = 128;
 
 struct QuantizeArgs {
   const void* x;
-  int x_format;
   int64_t rows, cols, x_pitch;
   int vec;  // x's rows start on 16-byte boundaries
   int rule;
@@ -26,13 +27,7 @@ struct QuantizeArgs {
   int64_t data_pitch, scale_pitch, data_t_pitch, scale_t_pitch;
 };
 
-// Encoding of |x| if finite, else 0 (NaN and infinities do not set a scale).
-__device__ __forceinline__ uint32_t finite_size(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
-  return u < 0x7F800000u ? u : 0u;
-}
-
-// k of a block whose largest finite |x| has encoding u: the largest values of
+// k of a block whose largest finite |x| has FP32 encoding u: the largest values of
 // both formats are 1.75 * 2^TOP, so k = exponent - TOP, plus one where the
 // significand exceeds 1.75 (adding 0x1FFFFF carries exactly then).
 template <int OF>
@@ -46,121 +41,205 @@ __device__ __forceinline__ float power_of_two(int k) {  // -126 <= k <= 127
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
-__device__ __forceinline__ void load_x8(const QuantizeArgs& a, int64_t row, int64_t col,
-                                        float (&x)[kVec]) {
+// Sizes are compared as encodings without their sign, two 16-bit ones to a word.
+template <int XF>
+struct Size {
+  static constexpr bool kPacked = Fmt<XF>::kBytes == 2;
+  static constexpr uint32_t kMask = kPacked ? 0x7FFF7FFFu : 0x7FFFFFFFu;
+  // first encoding that is not a finite number
+  static constexpr uint32_t kInfinite =
+      XF == SRS_FMT_F32 ? 0x7F800000u : XF == SRS_FMT_BF16 ? 0x7F80u : 0x7C00u;
+  __device__ static uint32_t of(uint32_t word) { return word & kMask; }
+  __device__ static uint32_t larger(uint32_t a, uint32_t b) {
+    return kPacked ? __vmaxu2(a, b) : max(a, b);
+  }
+  // the word with non-finite elements (NaN, infinities) taken as zero
+  __device__ static uint32_t finite(uint32_t word) {
+    const uint32_t u = word & kMask;
+    if (!kPacked) return u < kInfinite ? u : 0u;
+    return ((u & 0xFFFFu) < kInfinite ? u & 0xFFFFu : 0u) |
+           ((u >> 16) < kInfinite ? u & 0xFFFF0000u : 0u);
+  }
+  // larger half of a word / FP32 encoding of one size
+  __device__ static uint32_t single(uint32_t a) {
+    return kPacked ? max(a & 0xFFFFu, a >> 16) : a;
+  }
+  __device__ static uint32_t as_f32(uint32_t u) {
+    if (XF == SRS_FMT_F32) return u;
+    if (XF == SRS_FMT_BF16) return u << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)u)));
+  }
+};
+
+template <int XF>
+__device__ __forceinline__ void load_words(const QuantizeArgs& a, int64_t row, int64_t col,
+                                           uint32_t (&w)[kWords<XF>]) {
   const int64_t left = a.cols - col;
   if (row >= a.rows || left <= 0) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) x[j] = 0.0f;
-    return;
+    for (int j = 0; j < kWords<XF>; ++j) w[j] = 0u;
+  } else if (a.vec && left >= 8) {
+    load_raw8<XF>(a.x, row * a.x_pitch + col, w);
+  } else {
+    load_raw_partial<XF>(a.x, row * a.x_pitch + col, left < 8 ? (int)left : 8, w);
   }
-  const int count = left < 8 ? (int)left : 8;
-  const bool vec = a.vec && count == 8;
-  const int64_t at = row * a.x_pitch + col;
-  if (a.x_format == SRS_FMT_F32) load_state8<SRS_FMT_F32>(a.x, at, count, vec, x);
-  else if (a.x_format == SRS_FMT_BF16) load_state8<SRS_FMT_BF16>(a.x, at, count, vec, x);
-  else load_state8<SRS_FMT_F16>(a.x, at, count, vec, x);
+}
+
+// Largest finite size (FP32 encoding) of 8 elements a lane over 16 lanes.
+template <int XF>
+__device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>]) {
+  using Z = Size<XF>;
+  uint32_t top = 0u;
+#pragma unroll
+  for (int j = 0; j < kWords<XF>; ++j) top = Z::larger(top, Z::of(w[j]));
+  top = Z::single(top);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  if (__any_sync(0xFFFFFFFFu, top >= Z::kInfinite)) {
+    top = 0u;
+#pragma unroll
+    for (int j = 0; j < kWords<XF>; ++j) top = Z::larger(top, Z::finite(w[j]));
+    top = Z::single(top);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  }
+  return Z::as_f32(top);
+}
+
+template <int OF, int XF>
+__device__ __forceinline__ void encode_row(const QuantizeArgs& a, const uint32_t (&raw)[kWords<XF>],
+                                           int64_t row, int64_t col, int k) {
+  const float factor = power_of_two(-k);
+  float y[kVec];
+  decode8<XF>(raw, y);
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) y[j] *= factor;
+  uint32_t w[2];
+  encode8<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, w);
+  if (col < a.data_pitch)
+    *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = make_uint2(w[0], w[1]);
+}
+
+// Rows alone, 1 x 128 blocks: 16 lanes to a block, kAhead blocks of one column a
+// half-warp with all their loads first.  HBM-bound.
+constexpr int kAhead = 4;
+
+template <int OF, int XF>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a) {
+  const int lane16 = threadIdx.x & 15;
+  const int64_t col = (int64_t)blockIdx.x * kBlock + 8 * lane16;
+  const int64_t row0 = ((int64_t)blockIdx.y * 16 + (threadIdx.x >> 4)) * kAhead;
+  uint32_t raw[kAhead][kWords<XF>];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load_words<XF>(a, row0 + i, col, raw[i]);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int64_t row = row0 + i;
+    const int k = block_exponent<OF>(row_size<XF>(raw[i]));
+    if (row < a.rows) {
+      encode_row<OF, XF>(a, raw[i], row, col, k);
+      if (lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
+    }
+  }
 }
 
 // One CTA quantises one 128 x 128 tile of x, read once.  Thread t holds 8 rows x
-// 8 columns in registers: columns 8 * (t % 16) .., rows 8 * (t / 16) .., so a
-// row's block maximum is a reduction over 16 lanes, a column's one over the 16
+// 8 columns in registers as loaded: columns 8 * (t % 16) .., rows 8 * (t / 16) ..,
+// so a row's block maximum is a reduction over 16 lanes, a column's one over the 16
 // row groups (through shared memory), and the transposed bytes leave as 8 x 8
 // register transposes in 8-byte pieces, swizzled in shared memory so that both
-// sides are conflict-free.  HBM-bound: 2 bytes read and 1 or 2 written an element.
-template <int OF, bool ROWS, bool COLS, bool SQUARE>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
-  __shared__ uint32_t column_max[COLS && !SQUARE ? 16 * kBlock : 16];
+// sides are conflict-free.
+template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
+__global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 3 : 2)
+quantize_tile_kernel(const QuantizeArgs a) {
+  using Z = Size<XF>;
+  constexpr int kW = kWords<XF>;
+  __shared__ uint32_t tops[COLS && !SQUARE ? 16 * 16 * kW : 8];
   __shared__ __align__(16) uint8_t turned[COLS ? kBlock * kBlock : 16];
   const int lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock, col0 = (int64_t)blockIdx.x * kBlock;
   const int64_t row_base = row0 + 8 * group, col = col0 + 8 * lane16;
 
-  float x[8][kVec];
+  uint32_t raw[8][kW];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load_x8(a, row_base + i, col, x[i]);
+  for (int i = 0; i < 8; ++i) load_words<XF>(a, row_base + i, col, raw[i]);
 
-  uint32_t row_top[8], col_top[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) row_top[i] = col_top[i] = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const uint32_t u = finite_size(x[i][j]);
-      if (ROWS || SQUARE) row_top[i] = max(row_top[i], u);
-      if (COLS && !SQUARE) col_top[j] = max(col_top[j], u);
-    }
-  }
+  int tile_k = 0;         // SQUARE: the block's exponent
+  uint32_t col_top[kVec];  // else: FP32 encodings of the columns' largest sizes
   if constexpr (SQUARE) {
     uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, row_top[i]);
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if ((threadIdx.x & 31) == 0) column_max[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = 0u;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) top = max(top, column_max[w]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) row_top[i] = col_top[i] = top;
-  } else {
-    if constexpr (ROWS) {
+    for (int pass = 0; pass < 2; ++pass) {
+      top = 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1)
-          row_top[i] = max(row_top[i], __shfl_xor_sync(0xFFFFFFFFu, row_top[i], d));
+        for (int j = 0; j < kW; ++j)
+          top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
       }
-    }
-    if constexpr (COLS) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) column_max[group * kBlock + 8 * lane16 + j] = col_top[j];
+      top = __reduce_max_sync(0xFFFFFFFFu, Z::single(top));
       __syncthreads();
-      if (threadIdx.x < kBlock) {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int g = 0; g < 16; ++g) top = max(top, column_max[g * kBlock + threadIdx.x]);
-        column_max[threadIdx.x] = top;
-      }
+      if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) col_top[j] = column_max[8 * lane16 + j];
+      for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+      if (top < Z::kInfinite) break;  // the same for the whole CTA
     }
+    tile_k = block_exponent<OF>(Z::as_f32(top));
+  } else if constexpr (COLS) {
+    for (int pass = 0; pass < 2; ++pass) {
+      uint32_t top[kW];
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        top[j] = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          top[j] = Z::larger(top[j], pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
+        tops[(group * kW + j) * 16 + lane16] = top[j];
+      }
+      __syncthreads();
+      bool infinite = false;
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        uint32_t t = 0u;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) t = Z::larger(t, tops[(g * kW + j) * 16 + lane16]);
+        if (Z::kPacked) {
+          col_top[2 * j % kVec] = t & 0xFFFFu;
+          col_top[(2 * j + 1) % kVec] = t >> 16;
+        } else {
+          col_top[j] = t;
+        }
+        infinite = infinite || Z::single(t) >= Z::kInfinite;
+      }
+      if (!__syncthreads_or(infinite)) break;
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) col_top[j] = Z::as_f32(col_top[j]);
   }
 
   if constexpr (ROWS) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t row = row_base + i;
-      const int k = block_exponent<OF>(row_top[i]);
+      const int k = SQUARE ? tile_k : block_exponent<OF>(row_size<XF>(raw[i]));
       if (row < a.rows) {
-        const float factor = power_of_two(-k);
-        float y[kVec];
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) y[j] = x[i][j] * factor;
-        uint32_t w[2];
-        encode8<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, w);
-        if (col < a.data_pitch)
-          *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = make_uint2(w[0], w[1]);
+        encode_row<OF, XF>(a, raw[i], row, col, k);
         if (!SQUARE && lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
       }
     }
     if (SQUARE && threadIdx.x == 0)
-      a.scale[(int64_t)blockIdx.y * a.scale_pitch + blockIdx.x] =
-          (uint8_t)(block_exponent<OF>(row_top[0]) + 127);
+      a.scale[(int64_t)blockIdx.y * a.scale_pitch + blockIdx.x] = (uint8_t)(tile_k + 127);
   }
 
   if constexpr (COLS) {
-    float factor[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) factor[j] = power_of_two(-block_exponent<OF>(col_top[j]));
     uint32_t w[8][2];  // 8 rows of 8 bytes
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float y[kVec];
+      decode8<XF>(raw[i], y);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = x[i][j] * factor[j];
+      for (int j = 0; j < kVec; ++j)
+        y[j] *= power_of_two(-(SQUARE ? tile_k : block_exponent<OF>(col_top[j])));
       encode8<OF>(y, a.ctr_t + (uint32_t)((row_base + i) * a.cols + col), a.rule, w[i]);
     }
     // 8 x 8 byte transpose, then column 8 * lane16 + j gets rows 8 * group .. + 7
@@ -193,8 +272,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
     }
     if constexpr (SQUARE) {
       if (threadIdx.x == 0)
-        a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] =
-            (uint8_t)(block_exponent<OF>(col_top[0]) + 127);
+        a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] = (uint8_t)(tile_k + 127);
     } else if (group == 0) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j)
@@ -205,14 +283,33 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
   }
 }
 
-template <int OF, bool SQUARE>
-void launch_quantize(const QuantizeArgs& a, dim3 grid, cudaStream_t stream) {
-  if (a.data != nullptr && a.data_t != nullptr)
-    quantize_kernel<OF, true, true, SQUARE><<<grid, kThreads, 0, stream>>>(a);
-  else if (a.data != nullptr)
-    quantize_kernel<OF, true, false, SQUARE><<<grid, kThreads, 0, stream>>>(a);
-  else
-    quantize_kernel<OF, false, true, SQUARE><<<grid, kThreads, 0, stream>>>(a);
+template <int OF, int XF>
+void launch_quantize(const QuantizeArgs& a, bool square, cudaStream_t stream) {
+  const unsigned columns = (unsigned)((a.cols + kBlock - 1) / kBlock);
+  const dim3 tiles(columns, (unsigned)((a.rows + kBlock - 1) / kBlock));
+  if (square) {
+    if (a.data != nullptr && a.data_t != nullptr)
+      quantize_tile_kernel<OF, XF, true, true, true><<<tiles, kThreads, 0, stream>>>(a);
+    else if (a.data != nullptr)
+      quantize_tile_kernel<OF, XF, true, false, true><<<tiles, kThreads, 0, stream>>>(a);
+    else
+      quantize_tile_kernel<OF, XF, false, true, true><<<tiles, kThreads, 0, stream>>>(a);
+  } else if (a.data_t == nullptr) {
+    const int64_t rows = 16 * kAhead;
+    const dim3 grid(columns, (unsigned)((a.rows + rows - 1) / rows));
+    quantize_rows_kernel<OF, XF><<<grid, kThreads, 0, stream>>>(a);
+  } else if (a.data != nullptr) {
+    quantize_tile_kernel<OF, XF, true, true, false><<<tiles, kThreads, 0, stream>>>(a);
+  } else {
+    quantize_tile_kernel<OF, XF, false, true, false><<<tiles, kThreads, 0, stream>>>(a);
+  }
+}
+
+template <int OF>
+void launch_quantize(const QuantizeArgs& a, int x_format, bool square, cudaStream_t stream) {
+  if (x_format == SRS_FMT_F32) launch_quantize<OF, SRS_FMT_F32>(a, square, stream);
+  else if (x_format == SRS_FMT_BF16) launch_quantize<OF, SRS_FMT_BF16>(a, square, stream);
+  else launch_quantize<OF, SRS_FMT_F16>(a, square, stream);
 }
 
 uint32_t host_h32(uint32_t x) {
@@ -278,7 +375,7 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
   if (!valid_rule(rule)) return fail(SRS_ERR_INVALID_ARGUMENT, "unknown rounding rule %d", rule);
   if (rows < 0 || cols < 0 || x_pitch < 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "negative size or pitch");
-  if (rows > 65535ll * kBlock || cols > (1ll << 30))
+  if (rows > 65535ll * 16 * kAhead || cols > (1ll << 30))
     return fail(SRS_ERR_INVALID_ARGUMENT, "%lld x %lld is too large", (long long)rows,
                 (long long)cols);
   if (data == nullptr && data_t == nullptr)
@@ -296,7 +393,6 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
   if (int rc = check_device()) return rc;
   QuantizeArgs a{};
   a.x = x;
-  a.x_format = x_format;
   a.rows = rows;
   a.cols = cols;
   a.x_pitch = x_pitch;
@@ -312,15 +408,9 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
   a.scale_pitch = scale_pitch;
   a.data_t_pitch = data_t_pitch;
   a.scale_t_pitch = scale_t_pitch;
-  const dim3 grid((unsigned)blocks_of(cols), (unsigned)blocks_of(rows));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (out_format == SRS_FMT_E4M3) {
-    if (square) launch_quantize<SRS_FMT_E4M3, true>(a, grid, st);
-    else launch_quantize<SRS_FMT_E4M3, false>(a, grid, st);
-  } else {
-    if (square) launch_quantize<SRS_FMT_E5M2, true>(a, grid, st);
-    else launch_quantize<SRS_FMT_E5M2, false>(a, grid, st);
-  }
+  if (out_format == SRS_FMT_E4M3) launch_quantize<SRS_FMT_E4M3>(a, x_format, square != 0, st);
+  else launch_quantize<SRS_FMT_E5M2>(a, x_format, square != 0, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_quantize_blocks launch");
 }
@@ -358,5 +448,14 @@ extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64
   args.e.batch_stride = a->rows * b->rows;
   const ProductOperand oa{reinterpret_cast<const void*>(a->data), a->rows, k, a->pitch, 0, false};
   const ProductOperand ob{reinterpret_cast<const void*>(b->data), b->rows, k, b->pitch, 0, false};
+  // Few rows on one side: the other side's bytes bound the product.
+  if (b->rows <= kThinRows && a->rows >= b->rows)
+    return launch_thin(oa, ob, a->format, b->format, args, d, d_format, b->rows, 1, st);
+  if (a->rows <= kThinRows) {
+    std::swap(args.scale_a, args.scale_b);
+    std::swap(args.scale_a_pitch, args.scale_b_pitch);
+    std::swap(args.scale_a_shift, args.scale_b_shift);
+    return launch_thin(ob, oa, b->format, a->format, args, d, d_format, 1, b->rows, st);
+  }
   return launch_product(kOperandF8, kEpilogueStore, oa, ob, 1, a->format, b->format, args, st);
 }

@@ -4,6 +4,7 @@
 
 #include "srs_host.h"
 #include "srs_product.cuh"
+#include "srs_thin.cuh"
 
 namespace srs {
 namespace {
@@ -35,7 +36,8 @@ int find_encode(EncodeTiled* out) {
 
 // Tensor map of one operand: boxes of 128 rows x 128 bytes of k, or of 64 rows
 // x 64 k when the row index is contiguous; outside elements read as zero.
-int encode_operand(const ProductOperand& o, int kind, int64_t batch, CUtensorMap* map) {
+int encode_operand(const ProductOperand& o, int kind, int64_t batch, CUtensorMap* map,
+                   uint32_t rows = 128) {
   EncodeTiled encode = nullptr;
   if (int rc = find_encode(&encode)) return rc;
   const uint64_t size = kind == kOperandF8 ? 1 : 2;
@@ -43,7 +45,7 @@ int encode_operand(const ProductOperand& o, int kind, int64_t batch, CUtensorMap
                               (cuuint64_t)(o.rows_inner ? o.k : o.rows), (cuuint64_t)batch};
   const uint64_t entry = batch > 1 ? (uint64_t)o.batch_stride : (uint64_t)o.pitch * dims[1];
   const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * size, entry * size};
-  const cuuint32_t box[3] = {(cuuint32_t)(kSliceBytes / size), o.rows_inner ? 64u : 128u, 1u};
+  const cuuint32_t box[3] = {(cuuint32_t)(kSliceBytes / size), o.rows_inner ? 64u : rows, 1u};
   const cuuint32_t ones[3] = {1, 1, 1};
   const CUresult r = encode(
       map, kind == kOperandF8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
@@ -181,6 +183,78 @@ int launch_product(int kind, int epilogue, const ProductOperand& a, const Produc
                    : launch_epilogue<kOperandF16, 1>(epilogue, map_a, map_b, args, stream);
   return cg == 2 ? launch_epilogue<kOperandF8, 2>(epilogue, map_a, map_b, args, stream)
                  : launch_epilogue<kOperandF8, 1>(epilogue, map_a, map_b, args, stream);
+}
+
+namespace {
+
+template <int BN>
+int launch_thin_as(const CUtensorMap& map_a, const CUtensorMap& map_b, const ThinArgs& args,
+                   int splits, cudaStream_t stream) {
+  using S = ThinShape<BN>;
+  const auto kernel = &thin_product_kernel<BN>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  {
+    std::lock_guard<std::mutex> lock(g_lock);
+    int& set = g_clusters[dev][reinterpret_cast<const void*>(kernel)];
+    if (set == 0) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+      if (e != cudaSuccess) return cuda_fail(e, "thin product shared memory");
+      set = 1;
+    }
+  }
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)splits;
+  cluster.val.clusterDim.y = 1;
+  cluster.val.clusterDim.z = 1;
+  config.gridDim = dim3((unsigned)((args.m + 127) / 128 * splits));
+  config.blockDim = dim3(kProductThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, args);
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "thin product launch");
+}
+
+}  // namespace
+
+int launch_thin(const ProductOperand& a, const ProductOperand& b, int a_format, int b_format,
+                const ProductArgs& scales, void* out, int out_format, int64_t row_stride,
+                int64_t col_stride, cudaStream_t stream) {
+  const int columns = b.rows <= 16 ? 16 : b.rows <= 32 ? 32 : 64;
+  CUtensorMap map_a, map_b;
+  if (int rc = encode_operand(a, kOperandF8, 1, &map_a)) return rc;
+  if (int rc = encode_operand(b, kOperandF8, 1, &map_b, (uint32_t)columns)) return rc;
+  ThinArgs args{};
+  if (int rc = status_word(&args.status)) return rc;
+  args.m = (int)a.rows;
+  args.n = (int)b.rows;
+  args.slices = (int)((a.k + kSliceBytes - 1) / kSliceBytes);
+  args.scale_a = scales.scale_a;
+  args.scale_b = scales.scale_b;
+  args.scale_a_pitch = scales.scale_a_pitch;
+  args.scale_b_pitch = scales.scale_b_pitch;
+  args.scale_a_shift = scales.scale_a_shift;
+  args.scale_b_shift = scales.scale_b_shift;
+  args.idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 |
+               (a_format == SRS_FMT_E5M2 ? 1u : 0u) << 7 |
+               (b_format == SRS_FMT_E5M2 ? 1u : 0u) << 10 | 1u << 23;
+  args.out = out;
+  args.out_format = out_format;
+  args.row_stride = row_stride;
+  args.col_stride = col_stride;
+  // Split k while all CTAs still fit at two an SM and each keeps two slices.
+  const int64_t tiles = (a.rows + 127) / 128;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2ll * sm_count() && args.slices >= 4 * splits)
+    splits *= 2;
+  if (columns == 16) return launch_thin_as<16>(map_a, map_b, args, splits, stream);
+  if (columns == 32) return launch_thin_as<32>(map_a, map_b, args, splits, stream);
+  return launch_thin_as<64>(map_a, map_b, args, splits, stream);
 }
 
 int read_product_status(unsigned int* out) {

@@ -38,7 +38,7 @@ constexpr int kProductThreads = 256;
 constexpr int kStages = 6;
 constexpr int kScaleSlots = 3;          // ring of scale groups (each covers 4 slices)
 constexpr int kPanelBytes = 128 * kSliceBytes;  // 128 rows of an operand per stage
-constexpr int kStageRowPitch = 33;      // floats per staged row of 32 (bank-conflict free)
+constexpr int kPieceBytes = 32 * 128;   // a warp's piece of results on its way out
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
 
 enum : int { kOperandF16 = 0, kOperandF8 = 1 };
@@ -255,22 +255,31 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
                  : "memory");
 }
 
-// 32 accumulator columns of this warp's 32 lanes: v[c] = D[lane, column + c].
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 accumulator columns of this warp's 32 lanes: r[c] = D[lane, column + c].  The
+// registers are valid after tmem_wait(r).
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Waits for this warp's TMEM loads; naming the registers keeps their uses behind it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                 "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                 "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_fence_before() {
@@ -294,6 +303,25 @@ __device__ __forceinline__ uint64_t operand_descriptor(bool rows_inner) {
 __device__ __forceinline__ uint64_t scale_descriptor(uint32_t addr) {
   return uint64_t((addr >> 4) & 0x3FFFu) | (1ull << 16) | (uint64_t(128u >> 4) << 32) |
          (1ull << 46);
+}
+
+// Scales of blocks kb .. kb + 3 of a row, one byte each; blocks from `last` on and
+// rows outside the matrix give 1 (127).  Rows on 4-byte boundaries are read a word
+// at a time.
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* scale, int64_t pitch, int shift,
+                                               int row, int rows, int kb, int last) {
+  uint32_t w = 0x7F7F7F7Fu;
+  if (row < rows) {
+    const uint8_t* p = scale + (int64_t)(row >> shift) * pitch + kb;
+    if (kb + 4 <= last && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+      w = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (kb + j < last) w = (w & ~(0xFFu << (8 * j))) | ((uint32_t)__ldg(p + j) << (8 * j));
+    }
+  }
+  return w;
 }
 
 // ------------------------------------------------------------------- tiles --
@@ -327,72 +355,257 @@ __device__ __forceinline__ TileAt tile_at(const ProductArgs& a, int64_t t) {
 
 // ---------------------------------------------------------------- epilogue --
 
-__device__ __forceinline__ void store_as(void* out, int format, int64_t at, float v) {
-  if (format == SRS_FMT_F32) static_cast<float*>(out)[at] = v;
-  else if (format == SRS_FMT_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(out)[at] = __float2half_rn(v);
+// Results leave in pieces of 32 rows x 128 bytes: a lane holds one row's piece (32
+// words), the warp turns it through shared memory (16-byte slots, slot index xor
+// row so that both sides are conflict-free), and 8 lanes then store one row's 128
+// bytes.  Rows that are not on 16-byte boundaries are stored by words, and 16-bit
+// results of odd pitch by elements.
+__device__ __forceinline__ uint32_t staged_slot(uint32_t base, int row, int slot) {
+  return base + row * 128 + 16 * (slot ^ (row & 7));
 }
 
-// One chunk of 32 columns: lane = tile row on entry (v[c] = D[row0 + lane, col0 + c]).
-// Values pass through the warp's shared rows so that a store covers 32
-// consecutive columns of one row, whatever the row pitch and alignment.
-template <int EPILOGUE>
-__device__ __forceinline__ void write_chunk(const ProductArgs& a, float (&v)[32], int batch,
-                                            int row0, int col0, bool mirror, float factor,
-                                            float* staged, int lane) {
-  const ProductEpilogue& e = a.e;
-  const int row = row0 + lane;
-  if constexpr (EPILOGUE == kEpilogueSymmetric) {
-    __half* out = static_cast<__half*>(e.out) + (int64_t)batch * e.batch_stride;
-    const __half* addend =
-        e.addend == nullptr ? nullptr : e.addend + (int64_t)batch * e.batch_stride;
-    const bool inside = row < a.m;
+__device__ __forceinline__ void stage_row(uint32_t base, int lane, const uint32_t (&w)[32]) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-      float x = v[c] * factor;
-      // addend is symmetric: its transposed element is the coalesced one
-      if (addend != nullptr && inside && col0 + c < a.n)
-        x = fmaf(e.beta, __half2float(addend[(int64_t)(col0 + c) * e.ldd + row]), x);
-      if (row == col0 + c) x += e.diagonal;
-      v[c] = x;
+  for (int j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_slot(base, lane, j)),
+                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                 : "memory");
+}
+
+__device__ __forceinline__ uint4 staged_read4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint32_t staged_read(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Staged piece to rows of `size`-byte elements: `out` is the piece's first element,
+// `pitch` and `cols` count elements, `rows` <= 32.
+__device__ __forceinline__ void store_piece(uint32_t base, char* out, int size, int64_t pitch,
+                                            int rows, int cols, int lane) {
+  const uint64_t align = reinterpret_cast<uint64_t>(out) | (uint64_t)(pitch * size);
+  const int bytes = min(cols * size, 128);
+  const int64_t step = pitch * size;
+  if ((align & 15) == 0 && (bytes & 15) == 0) {
+    const int slot = lane & 7, row0 = lane >> 3;
+    char* p = out + row0 * step + 16 * slot;
+    if (16 * slot < bytes) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 4 * i + row0;
+        const uint4 v = staged_read4(staged_slot(base, row, slot));
+        if (row < rows) *reinterpret_cast<uint4*>(p + 4 * i * step) = v;
+      }
     }
-    if (mirror && inside) {
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (col0 + c < a.n) out[(int64_t)(col0 + c) * e.ldd + row] = __float2half_rn(v[c]);
+  } else if ((align & 3) == 0) {
+    const bool whole = 4 * lane + 4 <= bytes, half = !whole && 4 * lane < bytes;
+    char* p = out + 4 * lane;
+#pragma unroll 8
+    for (int row = 0; row < rows; ++row, p += step) {
+      const uint32_t v = staged_read(staged_slot(base, row, lane >> 2) + 4 * (lane & 3));
+      if (whole) *reinterpret_cast<uint32_t*>(p) = v;
+      else if (half) *reinterpret_cast<uint16_t*>(p) = (uint16_t)v;
     }
   } else {
+    char* p = out + 2 * lane;
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row, p += step) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c) v[c] *= factor;
-  }
-#pragma unroll
-  for (int c = 0; c < 32; ++c) staged[lane * kStageRowPitch + c] = v[c];
-  __syncwarp();
-  const int col = col0 + lane;
-  const int rows = min(32, a.m - row0);
-  if (col < a.n) {
-    if constexpr (EPILOGUE == kEpilogueMuon) {
-      const srs_row& target = e.rows[batch];
-      const bool bf16 = (target.flags & SRS_ROW_PARAM_BF16) != 0u;
-      int64_t at = (int64_t)row0 * a.n + col;
-      for (int r = 0; r < rows; ++r, at += a.n) {
-        const float d = staged[r * kStageRowPitch + lane];
-        if (bf16) {
-          __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(target.param) + at;
-          *p = __float2bfloat16_rn(fmaf(e.step, d, __fmul_rn(__bfloat162float(*p), e.decay)));
-        } else {
-          float* p = reinterpret_cast<float*>(target.param) + at;
-          *p = fmaf(e.step, d, __fmul_rn(*p, e.decay));
-        }
+      for (int h = 0; h < 2; ++h) {
+        const int e = lane + 32 * h;
+        const uint32_t v = staged_read(staged_slot(base, row, e >> 3) + 4 * ((e >> 1) & 3));
+        if (2 * e < bytes)
+          *reinterpret_cast<uint16_t*>(p + 64 * h) = (uint16_t)(v >> (16 * (e & 1)));
       }
-    } else {
-      int64_t at = (int64_t)batch * e.batch_stride + (int64_t)row0 * e.ldd + col;
-      for (int r = 0; r < rows; ++r, at += e.ldd)
-        store_as(e.out, EPILOGUE == kEpilogueSymmetric ? SRS_FMT_F16 : e.out_format, at,
-                 staged[r * kStageRowPitch + lane]);
     }
   }
-  __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// p' = fma(step, D, p * decay) for the staged 32 x 32 FP32 piece of D.
+template <bool BF16>
+__device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t pitch, int rows,
+                                             int cols, float step, float decay, int lane) {
+  constexpr int kSize = BF16 ? 2 : 4;
+  const auto next = [&](float p, uint32_t d) {
+    return fmaf(step, __uint_as_float(d), __fmul_rn(p, decay));
+  };
+  const uint64_t align = reinterpret_cast<uint64_t>(param) | (uint64_t)(pitch * kSize);
+  if ((align & (4 * kSize - 1)) == 0 && cols >= 32) {
+    // 4 columns a lane, 4 rows at a time; all loads first
+    const int slot = lane & 7, row0 = lane >> 3;
+    char* p = param + (row0 * pitch + 4 * slot) * kSize;
+    uint4 old[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      old[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (4 * i + row0 < rows) {
+        const char* q = p + 4 * i * pitch * kSize;
+        if constexpr (BF16) {
+          const uint2 t = *reinterpret_cast<const uint2*>(q);
+          old[i] = make_uint4(t.x << 16, t.x & 0xFFFF0000u, t.y << 16, t.y & 0xFFFF0000u);
+        } else {
+          old[i] = *reinterpret_cast<const uint4*>(q);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 4 * i + row0;
+      const uint4 d = staged_read4(staged_slot(base, row, slot));
+      if (row >= rows) continue;
+      char* q = p + 4 * i * pitch * kSize;
+      const float a = next(__uint_as_float(old[i].x), d.x), b = next(__uint_as_float(old[i].y), d.y);
+      const float c = next(__uint_as_float(old[i].z), d.z), e = next(__uint_as_float(old[i].w), d.w);
+      if constexpr (BF16) *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16(a, b), pack_bf16(c, e));
+      else *reinterpret_cast<float4*>(q) = make_float4(a, b, c, e);
+    }
+  } else if (lane < cols) {
+    char* p = param + lane * kSize;
+#pragma unroll 8
+    for (int row = 0; row < rows; ++row, p += pitch * kSize) {
+      const uint32_t d = staged_read(staged_slot(base, row, lane >> 2) + 4 * (lane & 3));
+      if constexpr (BF16) {
+        __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(p);
+        *q = __float2bfloat16_rn(next(__bfloat162float(*q), d));
+      } else {
+        float* q = reinterpret_cast<float*>(p);
+        *q = next(*q, d);
+      }
+    }
+  }
+}
+
+// Where a warp's 32 accumulator rows go.
+struct TileRows {
+  int batch, row0, lane;
+  bool mirror;    // symmetric: also store the transposed tile
+  float factor;
+  uint32_t staged;
+};
+
+// This lane's row of the addend, 64 columns from col0 on (the pitch is a multiple of 8).
+__device__ __forceinline__ void load_addend(const ProductArgs& a, const TileRows& t, int col0,
+                                            uint4 (&add)[8]) {
+  const ProductEpilogue& e = a.e;
+  const int row = t.row0 + t.lane;
+  const __half* from = e.addend + (int64_t)t.batch * e.batch_stride + (int64_t)row * e.ldd + col0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    add[j] = (row < a.m && col0 + 8 * j < e.ldd) ? __ldg(reinterpret_cast<const uint4*>(from) + j)
+                                                 : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// 64 accumulator columns from col0 on: v[0][c] and v[1][c] are columns c and 32 + c.
+// `add` holds the addend's piece; the next piece's (next_col, -1: none) is requested
+// before this one is stored.
+template <int EPILOGUE>
+__device__ __forceinline__ void write_columns(const ProductArgs& a, const TileRows& t, int col0,
+                                              uint32_t (&v)[2][32], uint4 (&add)[8],
+                                              int next_col) {
+  const ProductEpilogue& e = a.e;
+  const int row = t.row0 + t.lane, rows = min(32, a.m - t.row0);
+  const int64_t at = (int64_t)t.batch * e.batch_stride;
+  if constexpr (EPILOGUE == kEpilogueSymmetric) {
+    __half* out = static_cast<__half*>(e.out) + at;
+    uint32_t w[32];
+    if (e.addend != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint4 q = add[i >> 2];
+        const uint32_t pair = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+        const float2 g = f16x2_to_float2(pair);
+        const float x = __uint_as_float(v[i >> 4][(2 * i) & 31]) * t.factor;
+        const float y = __uint_as_float(v[i >> 4][(2 * i + 1) & 31]) * t.factor;
+        const int col = col0 + 2 * i;
+        w[i] = pack_half(fmaf(e.beta, g.x, x) + (row == col ? e.diagonal : 0.0f),
+                         fmaf(e.beta, g.y, y) + (row == col + 1 ? e.diagonal : 0.0f));
+      }
+      if (next_col >= 0) load_addend(a, t, next_col, add);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        w[i] = pack_half(__uint_as_float(v[i >> 4][(2 * i) & 31]) * t.factor,
+                         __uint_as_float(v[i >> 4][(2 * i + 1) & 31]) * t.factor);
+    }
+    if (t.mirror) {
+      // Lane pairs swap halves: the even lane gets two rows of an even column, the
+      // odd lane of the next one, so a store covers 2 x 64 bytes.  (An odd last
+      // row writes one padding element beside it.)
+      const bool odd = (t.lane & 1) != 0;
+      __half* to = out + (int64_t)(col0 + (odd ? 1 : 0)) * e.ldd + (row & ~1);
+#pragma unroll
+      for (int i = 0; i < 32; ++i, to += 2 * e.ldd) {
+        const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, w[i], 1);
+        const uint32_t pair =
+            odd ? __byte_perm(other, w[i], 0x7632u) : __byte_perm(w[i], other, 0x5410u);
+        if ((row & ~1) < a.m && col0 + 2 * i + (odd ? 1 : 0) < a.n)
+          *reinterpret_cast<uint32_t*>(to) = pair;
+      }
+    }
+    stage_row(t.staged, t.lane, w);
+    __syncwarp();
+    store_piece(t.staged, reinterpret_cast<char*>(out + (int64_t)t.row0 * e.ldd + col0), 2, e.ldd,
+                rows, (int)e.ldd - col0, t.lane);
+    __syncwarp();
+  } else if (EPILOGUE == kEpilogueStore && e.out_format != SRS_FMT_F32) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = __uint_as_float(v[i >> 4][(2 * i) & 31]) * t.factor;
+      const float y = __uint_as_float(v[i >> 4][(2 * i + 1) & 31]) * t.factor;
+      w[i] = e.out_format == SRS_FMT_BF16 ? pack_bf16(x, y) : pack_half(x, y);
+    }
+    stage_row(t.staged, t.lane, w);
+    __syncwarp();
+    store_piece(t.staged,
+                static_cast<char*>(e.out) + 2 * (at + (int64_t)t.row0 * e.ldd + col0), 2, e.ldd,
+                rows, a.n - col0, t.lane);
+    __syncwarp();
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = col0 + 32 * h;
+      if (col >= a.n) break;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        v[h][c] = __float_as_uint(__uint_as_float(v[h][c]) * t.factor);
+      stage_row(t.staged, t.lane, v[h]);
+      __syncwarp();
+      if constexpr (EPILOGUE == kEpilogueMuon) {
+        const srs_row& target = e.rows[t.batch];
+        const int64_t first = (int64_t)t.row0 * a.n + col;
+        if (target.flags & SRS_ROW_PARAM_BF16)
+          update_piece<true>(t.staged, reinterpret_cast<char*>(target.param) + 2 * first, a.n,
+                             rows, a.n - col, e.step, e.decay, t.lane);
+        else
+          update_piece<false>(t.staged, reinterpret_cast<char*>(target.param) + 4 * first, a.n,
+                              rows, a.n - col, e.step, e.decay, t.lane);
+      } else {
+        store_piece(t.staged,
+                    static_cast<char*>(e.out) + 4 * (at + (int64_t)t.row0 * e.ldd + col), 4, e.ldd,
+                    rows, a.n - col, t.lane);
+      }
+      __syncwarp();
+    }
+  }
 }
 
 // ------------------------------------------------------------------ kernel --
@@ -410,7 +623,7 @@ struct ProductShape {
   static constexpr int kScaleColumn = 480;  // 2 slots of 12 columns (pitch 16)
   static constexpr int kStageBytes = 2 * kPanelBytes;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes +
-                               4 * 32 * kStageRowPitch * 4;
+                               4 * kPieceBytes;
 };
 
 template <int KIND, int CG, int EPILOGUE>
@@ -426,9 +639,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const uint32_t stage0 = (smem_address(raw) + 1023u) & ~1023u;
   const uint32_t scales0 = stage0 + kStages * S::kStageBytes;
-  float* staged = reinterpret_cast<float*>(
-      raw + (stage0 - smem_address(raw)) + kStages * S::kStageBytes + kScaleSlots * S::kScaleBytes +
-      (warp & 3) * 32 * kStageRowPitch * 4);
+  const uint32_t staged0 = scales0 + kScaleSlots * S::kScaleBytes;
 
   const uint32_t bar0 = smem_address(bars);
   const auto full = [&](int s) { return bar0 + 8u * s; };
@@ -584,18 +795,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // in which the tensor core reads them from 4 TMEM columns
     int slot = 0;
     uint32_t phase = 0;
-    const auto word = [&](const uint8_t* scale, int64_t pitch, int shift, int row, int rows,
-                          int kb) {
-      uint32_t w = 0x7F7F7F7Fu;  // scale 1 outside the matrix
-      if (row < rows) {
-        const uint8_t* p = scale + (int64_t)(row >> shift) * pitch;
-        w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w |= (kb + j < slices ? (uint32_t)__ldg(p + kb + j) : 0x7Fu) << (8 * j);
-      }
-      return w;
-    };
     for (int64_t t = first; t < a.n_tiles && ok; t += step) {
       const TileAt at = tile_at(a, t);
       const int ra = at.m * S::kTileRows + 128 * (int)rank;
@@ -604,11 +803,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         uint32_t w[1 + CG][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          w[0][j] = word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra + lane + 32 * j, a.m, kb);
+          w[0][j] = scale_word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra + lane + 32 * j,
+                               a.m, kb, slices);
 #pragma unroll
           for (int c = 0; c < CG; ++c)
-            w[1 + c][j] = word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
-                               rb + 128 * c + lane + 32 * j, a.n, kb);
+            w[1 + c][j] = scale_word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
+                                     rb + 128 * c + lane + 32 * j, a.n, kb, slices);
         }
         ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 32u);
         ok = __all_sync(0xFFFFFFFFu, ok);
@@ -646,28 +846,39 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const float r = __ldg(a.e.rho + at.batch);
         factor = __fdiv_rn(factor, a.e.rho_power == 2 ? __fmul_rn(r, r) : r);
       }
+      TileRows rows;
+      rows.batch = at.batch;
+      rows.row0 = at.m * S::kTileRows + 128 * (int)rank + 32 * warp;
+      rows.lane = lane;
+      rows.mirror = a.symmetric != 0 && at.m != at.n;
+      rows.factor = factor;
+      rows.staged = staged0 + warp * kPieceBytes;
+      const int col0 = at.n * S::kTileCols;
+      constexpr int kPieces = S::kTileCols / 64;
+      uint4 add[8];
+      if (EPILOGUE == kEpilogueSymmetric && a.e.addend != nullptr) load_addend(a, rows, col0, add);
       ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, a.status, 128u);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       tmem_fence_after();
       const uint32_t src = tmem + acc * S::kSecond + ((uint32_t)(warp * 32) << 16);
-      const int row0 = at.m * S::kTileRows + 128 * (int)rank + 32 * warp;
-      const int col0 = at.n * S::kTileCols;
-      const bool mirror = a.symmetric != 0 && at.m != at.n;
-      constexpr int kChunks = S::kTileCols / 32;
-      for (int i = 0; i < kChunks; ++i) {
+#pragma unroll 1
+      for (int i = 0; i < kPieces; ++i) {
         // accumulator 0 gives its last (shared) columns first
-        const int c = (S::kShared != 0 && acc == 0) ? kChunks - 1 - i : i;
-        float v[32];
-        tmem_load32(src + 32 * c, v);
-        if (i == (S::kShared != 0 ? 0 : kChunks - 1)) {
+        const int c = (S::kShared != 0 && acc == 0) ? kPieces - 1 - i : i;
+        uint32_t v[2][32];
+        tmem_load32(src + 64 * c, v[0]);
+        tmem_load32(src + 64 * c + 32, v[1]);
+        tmem_wait(v[0]);
+        tmem_wait(v[1]);
+        if (i == (S::kShared != 0 ? 0 : kPieces - 1)) {
           tmem_fence_before();
           __syncwarp();
-          if (lane == 0)
-            barrier_arrive(map_to_rank(acc_empty(acc), 0));
+          if (lane == 0) barrier_arrive(map_to_rank(acc_empty(acc), 0));
         }
-        if (row0 < a.m && col0 + 32 * c < a.n)
-          write_chunk<EPILOGUE>(a, v, at.batch, row0, col0 + 32 * c, mirror, factor, staged, lane);
+        if (rows.row0 < a.m && col0 + 64 * c < a.n)
+          write_columns<EPILOGUE>(a, rows, col0 + 64 * c, v, add,
+                                  i + 1 < kPieces ? col0 + 64 * (c + 1) : -1);
       }
     }
   }
@@ -693,6 +904,13 @@ struct ProductOperand {
   int64_t rows, k, pitch, batch_stride;  // elements
   bool rows_inner;
 };
+
+// Enqueues D = A B^T of FP8 blocks where B has at most kThinRows rows (srs_product.cu);
+// element (i, j) of D goes to i * row_stride + j * col_stride.
+constexpr int kThinRows = 64;
+int launch_thin(const ProductOperand& a, const ProductOperand& b, int a_format, int b_format,
+                const ProductArgs& scales, void* out, int out_format, int64_t row_stride,
+                int64_t col_stride, cudaStream_t stream);
 
 // Enqueues D = A B^T with the given epilogue over `batch` entries (srs_product.cu).
 // `args` carries the epilogue, the scales and the symmetric flag; the rest is

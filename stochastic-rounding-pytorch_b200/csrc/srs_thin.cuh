@@ -1,0 +1,291 @@
+// FP8 block products with one thin side (up to 64 rows: decoded tokens):
+//
+//   D[i, j] = sum_k A[i, k] * B[j, k],   A: m x k (the weights), B: n x k, n <= 64
+//
+// What bounds it: A's bytes, read once.  The weights take the 128-row side of the
+// MMA and the thin operand the column side, so that no MMA row is idle, and k is
+// split over a cluster of up to 8 CTAs so that all SMs stream: 4096 rows are only
+// 32 tiles.  The split sums meet in distributed shared memory and are added in
+// rank order (FP32), so results do not depend on timing.  Two CTAs share an SM,
+// each with 4 or 5 slices of 128 rows x 128 bytes on their way.
+//
+// Roles, barriers and bounded waits as in the large product (one tile per CTA).
+#pragma once
+
+#include "srs_product.cuh"
+
+namespace srs {
+
+struct ThinArgs {
+  int m, n;             // rows of A and of B
+  int slices;           // of 128 along k
+  const uint8_t* scale_a;
+  const uint8_t* scale_b;
+  int64_t scale_a_pitch, scale_b_pitch;
+  int scale_a_shift, scale_b_shift;
+  uint32_t idesc;
+  void* out;
+  int out_format;
+  int64_t row_stride, col_stride;  // of D, elements
+  unsigned int* status;
+};
+
+template <int BN>
+struct ThinShape {
+  static constexpr int kStages = BN <= 32 ? 5 : 4;  // two CTAs' worth fit an SM
+  static constexpr int kStageBytes = kPanelBytes + BN * kSliceBytes;
+  static constexpr int kColumns = BN <= 16 ? 32 : BN <= 32 ? 64 : 128;  // TMEM
+  static constexpr int kScaleColumn = BN;  // two groups of 8 columns (A, B)
+  static constexpr int kScaleBytes = 1024;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes;
+  static_assert(BN + 16 <= kColumns, "accumulator and scales fit");
+  static_assert(128 * BN * 4 <= kStages * kStageBytes, "split sums fit the stages");
+};
+
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void store_value(void* out, int format, int64_t at, float v) {
+  if (format == SRS_FMT_F32) static_cast<float*>(out)[at] = v;
+  else if (format == SRS_FMT_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(out)[at] = __float2half_rn(v);
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kProductThreads, 2)
+thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ ThinArgs a) {
+  using S = ThinShape<BN>;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 1 + 2 * kScaleSlots];
+  __shared__ uint32_t tmem_slot;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const uint32_t rank = cluster_rank();
+  const int row0 = (int)(blockIdx.x / splits) * 128;
+  const int first = (int)((int64_t)a.slices * rank / splits);
+  const int last = (int)((int64_t)a.slices * (rank + 1) / splits);
+  const uint32_t stage0 = (smem_address(raw) + 1023u) & ~1023u;
+  const uint32_t scales0 = stage0 + S::kStages * S::kStageBytes;
+  const uint32_t bar0 = smem_address(bars);
+  const auto full = [&](int s) { return bar0 + 8u * s; };
+  const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+  const uint32_t done = bar0 + 8u * (2 * S::kStages);
+  const auto scale_full = [&](int i) { return bar0 + 8u * (2 * S::kStages + 1 + i); };
+  const auto scale_empty = [&](int i) {
+    return bar0 + 8u * (2 * S::kStages + 1 + kScaleSlots + i);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      barrier_init(full(s), 1);
+      barrier_init(empty(s), 1);
+    }
+    barrier_init(done, 1);
+    for (int i = 0; i < kScaleSlots; ++i) {
+      barrier_init(scale_full(i), 1);
+      barrier_init(scale_empty(i), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp == 4 && lane == 0) {
+    int s = 0;
+    uint32_t phase = 0;
+    for (int i = first; i < last; ++i) {
+      ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
+      if (!ok) break;
+      barrier_expect(full(s), S::kStageBytes);
+      const uint32_t pa = stage0 + s * S::kStageBytes;
+      load_box<1>(pa, &map_a, i * kSliceBytes, row0, 0, full(s));
+      load_box<1>(pa + kPanelBytes, &map_b, i * kSliceBytes, 0, 0, full(s));
+      if (++s == S::kStages) {
+        s = 0;
+        phase ^= 1u;
+      }
+    }
+    // Every stage given back before the CTA can leave.
+    for (int i = 0; i < S::kStages && ok; ++i) {
+      ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 14);
+      if (++s == S::kStages) {
+        s = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp == 5 && lane == 0) {
+    const uint64_t desc = operand_descriptor(false);
+    int s = 0, slot = 0, last_slot = -1;
+    uint32_t phase = 0, slot_phase = 0, last_phase = 0, group = 0;
+    for (int i = first; i < last && ok; ++i) {
+      const int j0 = i - first;
+      const uint32_t scale_tmem = tmem + S::kScaleColumn + 8u * (group & 1u);
+      if ((j0 & 3) == 0) {
+        // (see the large product: the columns' last readers are done after this)
+        if (last_slot >= 0) ok = barrier_wait(scale_empty(last_slot), last_phase, a.status, 1u << 9);
+        ok = ok && barrier_wait(scale_full(slot), slot_phase, a.status, 1u << 10);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t src = scales0 + slot * S::kScaleBytes;
+        copy_scales<1>(scale_tmem, scale_descriptor(src));
+        copy_scales<1>(scale_tmem + 4, scale_descriptor(src + 512));
+        mma_commit<1>(scale_empty(slot));
+        last_slot = slot;
+        last_phase = slot_phase;
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          slot_phase ^= 1u;
+        }
+      }
+      ok = barrier_wait(full(s), phase, a.status, 1u << 11);
+      if (!ok) break;
+      tmem_fence_after();
+      const uint32_t pa = stage0 + s * S::kStageBytes;
+      const uint64_t da = desc | uint64_t((pa >> 4) & 0x3FFFu);
+      const uint64_t db = desc | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+      const uint32_t id = (uint32_t)(j0 & 3);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        mma_f8<1>(tmem, da + 2 * j, db + 2 * j, a.idesc | (id << 29) | (id << 4), scale_tmem,
+                  scale_tmem + 4, (j0 | j) != 0 ? 1u : 0u);
+      mma_commit<1>(empty(s));
+      if (++s == S::kStages) {
+        s = 0;
+        phase ^= 1u;
+      }
+      if ((j0 & 3) == 3) ++group;
+    }
+    if (ok) mma_commit<1>(done);
+  } else if (warp == 6) {
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int kb = first; kb < last; kb += 4) {
+      uint32_t w[2][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[0][j] = scale_word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0 + lane + 32 * j,
+                             a.m, kb, last);
+        w[1][j] = 32 * j < BN ? scale_word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
+                                           lane + 32 * j, a.n, kb, last)
+                              : 0x7F7F7F7Fu;
+      }
+      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 1u << 12);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      const uint32_t dst = scales0 + slot * S::kScaleBytes + 16u * lane;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 * c),
+                     "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
+                     : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive(map_to_rank(scale_full(slot), rank));
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
+    for (int i = 0; i < kScaleSlots && ok; ++i) {
+      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 1u << 15);
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+  __syncwarp();
+  // Every warp waits for the last MMA: all loads and commits of this CTA are done
+  // then, and the stages are free for the split sums.
+  const bool finished = barrier_wait(done, 0u, a.status, 1u << 13);
+  ok = __all_sync(0xFFFFFFFFu, ok && finished);
+  if (!ok) {
+    const long long start = clock64();
+    while (clock64() - start < 4000000ll) {
+    }
+  }
+  tmem_fence_after();
+  const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
+  const int row = row0 + 32 * warp + lane;
+  if (splits == 1) {
+    if (warp < 4 && ok) {
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        if (c0 >= a.n) break;
+        uint32_t v[16];
+        tmem_load16(acc + c0, v);
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (row < a.m && c0 + c < a.n)
+            store_value(a.out, a.out_format, row * a.row_stride + (c0 + c) * a.col_stride,
+                        __uint_as_float(v[c]));
+      }
+    }
+  } else {
+    // column c of this CTA's sum at 512 * c bytes, one word a row
+    if (warp < 4) {
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        if (c0 >= a.n) break;
+        uint32_t v[16];
+        tmem_load16(acc + c0, v);
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(stage0 + 512 * (c0 + c) + 128 * warp +
+                                                       4 * lane),
+                       "r"(v[c])
+                       : "memory");
+      }
+    }
+    cluster_sync();
+    // columns rank, rank + splits, ...: half of the CTA's threads a column
+    const int half = threadIdx.x >> 7, at = threadIdx.x & 127;
+    const int out_row = row0 + at;
+    for (int c = (int)rank + half * (int)splits; c < a.n; c += 2 * (int)splits) {
+      float part[8];
+#pragma unroll
+      for (uint32_t r = 0; r < 8; ++r) {
+        part[r] = 0.0f;
+        if (r < splits)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                       : "=f"(part[r])
+                       : "r"(map_to_rank(stage0 + 512 * c + 4 * at, r))
+                       : "memory");
+      }
+      float sum = part[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < (int)splits) sum = __fadd_rn(sum, part[r]);
+      if (out_row < a.m && ok)
+        store_value(a.out, a.out_format, out_row * a.row_stride + c * a.col_stride, sum);
+    }
+    cluster_sync();  // the others have read this CTA's sums
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 5) tmem_free<1>(tmem, S::kColumns);
+}
+
+}  // namespace srs
