@@ -92,6 +92,23 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 
+// The warp's index as a warp-uniform value, and one elected lane of the warp.  The
+// load and MMA roles run with the whole warp in uniform control flow, and only the
+// instruction itself is under the election: descriptors then stay in uniform
+// registers (with the loop itself under `lane == 0`, moving them there for every
+// MMA took 745 cycles a slice instead of the 512 of its FP8 MMAs).
+__device__ __forceinline__ int warp_index() {
+  return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0);
+}
+
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t chosen;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(chosen));
+  return chosen != 0;
+}
+
 // shared::cluster address of `addr` (a shared::cta address) in CTA `rank`.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -305,23 +322,37 @@ __device__ __forceinline__ uint64_t scale_descriptor(uint32_t addr) {
          (1ull << 46);
 }
 
-// Scales of blocks kb .. kb + 3 of a row, one byte each; blocks from `last` on and
-// rows outside the matrix give 1 (127).  Rows on 4-byte boundaries are read a word
-// at a time.
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* scale, int64_t pitch, int shift,
-                                               int row, int rows, int kb, int last) {
-  uint32_t w = 0x7F7F7F7Fu;
-  if (row < rows) {
-    const uint8_t* p = scale + (int64_t)(row >> shift) * pitch + kb;
-    if (kb + 4 <= last && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
-      w = __ldg(reinterpret_cast<const uint32_t*>(p));
+// Scales of one operand for a warp: rows row0 + lane + 32 j (j < 4), blocks kb ..
+// kb + 3 of each, one byte a block.  Rows outside the matrix read its last row
+// instead (their data are zeros and their results are not stored); blocks from
+// `last` on give 1 (127).  Rows on 4-byte boundaries are read a word at a time.
+struct ScaleRows {
+  const uint8_t* row[4];
+  __device__ __forceinline__ void at(const uint8_t* scale, int64_t pitch, int shift, int first,
+                                     int rows, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      row[j] = scale + (int64_t)(min(first + lane + 32 * j, rows - 1) >> shift) * pitch;
+  }
+  __device__ __forceinline__ void read(int kb, int last, bool words, uint32_t (&w)[4]) const {
+    if (words && kb + 4 <= last) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row[j] + kb));
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (kb + j < last) w = (w & ~(0xFFu << (8 * j))) | ((uint32_t)__ldg(p + j) << (8 * j));
+      for (int j = 0; j < 4; ++j) {
+        w[j] = 0x7F7F7F7Fu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kb + i < last)
+            w[j] = (w[j] & ~(0xFFu << (8 * i))) | ((uint32_t)__ldg(row[j] + kb + i) << (8 * i));
+      }
     }
   }
-  return w;
+};
+
+__device__ __forceinline__ bool scale_words(const uint8_t* scale, int64_t pitch, int kb) {
+  return ((reinterpret_cast<uint64_t>(scale) | (uint64_t)pitch | (uint64_t)kb) & 3) == 0;
 }
 
 // ------------------------------------------------------------------- tiles --
@@ -635,7 +666,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   __shared__ __align__(8) uint64_t bars[2 * kStages + 4 + 2 * kScaleSlots];
   __shared__ uint32_t tmem_slot;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const uint32_t stage0 = (smem_address(raw) + 1023u) & ~1023u;
   const uint32_t scales0 = stage0 + kStages * S::kStageBytes;
@@ -676,7 +707,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int slices = (a.k + kSliceK - 1) / kSliceK;
   bool ok = true;
 
-  if (warp == 4 && lane == 0) {
+  if (warp == 4) {
+    const bool leader = elect_lane();
     // ---- TMA loads: this CTA's 128 rows of A and of B per slice
     int s = 0;
     uint32_t phase = 0;
@@ -687,22 +719,25 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       for (int i = 0; i < slices; ++i) {
         ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u);
         if (!ok) break;
-        if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
         const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
         const uint32_t pa = stage0 + s * S::kStageBytes, pb = pa + kPanelBytes;
         const int k = i * kSliceK;
-        if (a.a_rows_inner) {
-          load_box<CG>(pa, &map_a, ra, k, at.batch, bar);
-          load_box<CG>(pa + kPanelBytes / 2, &map_a, ra + 64, k, at.batch, bar);
-        } else {
-          load_box<CG>(pa, &map_a, k, ra, at.batch, bar);
+        if (leader) {
+          if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
+          if (a.a_rows_inner) {
+            load_box<CG>(pa, &map_a, ra, k, at.batch, bar);
+            load_box<CG>(pa + kPanelBytes / 2, &map_a, ra + 64, k, at.batch, bar);
+          } else {
+            load_box<CG>(pa, &map_a, k, ra, at.batch, bar);
+          }
+          if (a.b_rows_inner) {
+            load_box<CG>(pb, &map_b, rb, k, at.batch, bar);
+            load_box<CG>(pb + kPanelBytes / 2, &map_b, rb + 64, k, at.batch, bar);
+          } else {
+            load_box<CG>(pb, &map_b, k, rb, at.batch, bar);
+          }
         }
-        if (a.b_rows_inner) {
-          load_box<CG>(pb, &map_b, rb, k, at.batch, bar);
-          load_box<CG>(pb + kPanelBytes / 2, &map_b, rb + 64, k, at.batch, bar);
-        } else {
-          load_box<CG>(pb, &map_b, k, rb, at.batch, bar);
-        }
+        __syncwarp();
         if (++s == kStages) {
           s = 0;
           phase ^= 1u;
@@ -717,7 +752,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         phase ^= 1u;
       }
     }
-  } else if (warp == 5 && lane == 0 && rank == 0) {
+  } else if (warp == 5 && rank == 0) {
+    const bool leader = elect_lane();
     // ---- MMAs (the pair's leader issues for both CTAs)
     const uint64_t desc_a = operand_descriptor(a.a_rows_inner != 0);
     const uint64_t desc_b = operand_descriptor(a.b_rows_inner != 0);
@@ -751,10 +787,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (!ok) break;
             tmem_fence_after();
             const uint32_t src = scales0 + slot * S::kScaleBytes;
+            if (leader) {
 #pragma unroll
-            for (int c = 0; c < 1 + CG; ++c)
-              copy_scales<CG>(scale_tmem + 4 * c, scale_descriptor(src + 512 * c));
-            mma_commit<CG>(scale_empty(slot));
+              for (int c = 0; c < 1 + CG; ++c)
+                copy_scales<CG>(scale_tmem + 4 * c, scale_descriptor(src + 512 * c));
+              mma_commit<CG>(scale_empty(slot));
+            }
+            __syncwarp();
             last_slot = slot;
             last_phase = slot_phase;
             if (++slot == kScaleSlots) {
@@ -769,47 +808,52 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const uint32_t pa = stage0 + s * S::kStageBytes;
         const uint64_t da = desc_a | uint64_t((pa >> 4) & 0x3FFFu);
         const uint64_t db = desc_b | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+        const uint32_t id = (uint32_t)(i & 3);
+        const uint32_t idesc = KIND == kOperandF8 ? a.idesc | (id << 29) | (id << 4) : a.idesc;
+        if (leader) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t accumulate = (i | j) != 0 ? 1u : 0u;
-          if constexpr (KIND == kOperandF8) {
-            const uint32_t id = (uint32_t)(i & 3);
-            mma_f8<CG>(d, da + j * step_a, db + j * step_b, a.idesc | (id << 29) | (id << 4),
-                       scale_tmem, scale_tmem + 4, accumulate);
-          } else {
-            mma_f16<CG>(d, da + j * step_a, db + j * step_b, a.idesc, accumulate);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t accumulate = (i | j) != 0 ? 1u : 0u;
+            if constexpr (KIND == kOperandF8)
+              mma_f8<CG>(d, da + j * step_a, db + j * step_b, idesc, scale_tmem, scale_tmem + 4,
+                         accumulate);
+            else
+              mma_f16<CG>(d, da + j * step_a, db + j * step_b, idesc, accumulate);
           }
+          mma_commit<CG>(empty(s));
         }
-        mma_commit<CG>(empty(s));
+        __syncwarp();
         if (++s == kStages) {
           s = 0;
           phase ^= 1u;
         }
         if (KIND == kOperandF8 && ((i & 3) == 3 || i == slices - 1)) ++group;
       }
-      if (ok) mma_commit<CG>(acc_full(acc));
+      if (ok && leader) mma_commit<CG>(acc_full(acc));
+      __syncwarp();
     }
   } else if (KIND == kOperandF8 && warp == 6) {
     // ---- block scales: words of 4 consecutive scales (512 elements of k) per
     // row, row r at 16 * (r % 32) + 4 * (r / 32) of its 512-byte group, the order
     // in which the tensor core reads them from 4 TMEM columns
+    const bool words_a = scale_words(a.scale_a, a.scale_a_pitch, 0);
+    const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, 0);
     int slot = 0;
     uint32_t phase = 0;
     for (int64_t t = first; t < a.n_tiles && ok; t += step) {
       const TileAt at = tile_at(a, t);
       const int ra = at.m * S::kTileRows + 128 * (int)rank;
       const int rb = at.n * S::kTileCols;
+      ScaleRows from[1 + CG];
+      from[0].at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra, a.m, lane);
+#pragma unroll
+      for (int c = 0; c < CG; ++c)
+        from[1 + c].at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, rb + 128 * c, a.n, lane);
       for (int kb = 0; kb < slices; kb += 4) {
         uint32_t w[1 + CG][4];
+        from[0].read(kb, slices, words_a, w[0]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[0][j] = scale_word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra + lane + 32 * j,
-                               a.m, kb, slices);
-#pragma unroll
-          for (int c = 0; c < CG; ++c)
-            w[1 + c][j] = scale_word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
-                                     rb + 128 * c + lane + 32 * j, a.n, kb, slices);
-        }
+        for (int c = 0; c < CG; ++c) from[1 + c].read(kb, slices, words_b, w[1 + c]);
         ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 32u);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;

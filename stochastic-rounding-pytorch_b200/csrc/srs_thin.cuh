@@ -74,7 +74,7 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
   __shared__ __align__(8) uint64_t bars[2 * S::kStages + 1 + 2 * kScaleSlots];
   __shared__ uint32_t tmem_slot;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const uint32_t rank = cluster_rank();
@@ -111,16 +111,20 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
   const uint32_t tmem = tmem_slot;
   bool ok = true;
 
-  if (warp == 4 && lane == 0) {
+  if (warp == 4) {
+    const bool leader = elect_lane();
     int s = 0;
     uint32_t phase = 0;
     for (int i = first; i < last; ++i) {
       ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
       if (!ok) break;
-      barrier_expect(full(s), S::kStageBytes);
       const uint32_t pa = stage0 + s * S::kStageBytes;
-      load_box<1>(pa, &map_a, i * kSliceBytes, row0, 0, full(s));
-      load_box<1>(pa + kPanelBytes, &map_b, i * kSliceBytes, 0, 0, full(s));
+      if (leader) {
+        barrier_expect(full(s), S::kStageBytes);
+        load_box<1>(pa, &map_a, i * kSliceBytes, row0, 0, full(s));
+        load_box<1>(pa + kPanelBytes, &map_b, i * kSliceBytes, 0, 0, full(s));
+      }
+      __syncwarp();
       if (++s == S::kStages) {
         s = 0;
         phase ^= 1u;
@@ -134,7 +138,8 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
         phase ^= 1u;
       }
     }
-  } else if (warp == 5 && lane == 0) {
+  } else if (warp == 5) {
+    const bool leader = elect_lane();
     const uint64_t desc = operand_descriptor(false);
     int s = 0, slot = 0, last_slot = -1;
     uint32_t phase = 0, slot_phase = 0, last_phase = 0, group = 0;
@@ -148,9 +153,12 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
         if (!ok) break;
         tmem_fence_after();
         const uint32_t src = scales0 + slot * S::kScaleBytes;
-        copy_scales<1>(scale_tmem, scale_descriptor(src));
-        copy_scales<1>(scale_tmem + 4, scale_descriptor(src + 512));
-        mma_commit<1>(scale_empty(slot));
+        if (leader) {
+          copy_scales<1>(scale_tmem, scale_descriptor(src));
+          copy_scales<1>(scale_tmem + 4, scale_descriptor(src + 512));
+          mma_commit<1>(scale_empty(slot));
+        }
+        __syncwarp();
         last_slot = slot;
         last_phase = slot_phase;
         if (++slot == kScaleSlots) {
@@ -164,32 +172,35 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
       const uint32_t pa = stage0 + s * S::kStageBytes;
       const uint64_t da = desc | uint64_t((pa >> 4) & 0x3FFFu);
       const uint64_t db = desc | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
-      const uint32_t id = (uint32_t)(j0 & 3);
+      const uint32_t id = (uint32_t)(j0 & 3), idesc = a.idesc | (id << 29) | (id << 4);
+      if (leader) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        mma_f8<1>(tmem, da + 2 * j, db + 2 * j, a.idesc | (id << 29) | (id << 4), scale_tmem,
-                  scale_tmem + 4, (j0 | j) != 0 ? 1u : 0u);
-      mma_commit<1>(empty(s));
+        for (int j = 0; j < 4; ++j)
+          mma_f8<1>(tmem, da + 2 * j, db + 2 * j, idesc, scale_tmem, scale_tmem + 4,
+                    (j0 | j) != 0 ? 1u : 0u);
+        mma_commit<1>(empty(s));
+      }
+      __syncwarp();
       if (++s == S::kStages) {
         s = 0;
         phase ^= 1u;
       }
       if ((j0 & 3) == 3) ++group;
     }
-    if (ok) mma_commit<1>(done);
+    if (ok && leader) mma_commit<1>(done);
+    __syncwarp();
   } else if (warp == 6) {
     int slot = 0;
     uint32_t phase = 0;
+    const bool words_a = scale_words(a.scale_a, a.scale_a_pitch, first);
+    const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, first);
+    ScaleRows from_a, from_b;
+    from_a.at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
+    from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, 0, a.n, lane);
     for (int kb = first; kb < last; kb += 4) {
       uint32_t w[2][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[0][j] = scale_word(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0 + lane + 32 * j,
-                             a.m, kb, last);
-        w[1][j] = 32 * j < BN ? scale_word(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
-                                           lane + 32 * j, a.n, kb, last)
-                              : 0x7F7F7F7Fu;
-      }
+      from_a.read(kb, last, words_a, w[0]);
+      from_b.read(kb, last, words_b, w[1]);
       ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 1u << 12);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
