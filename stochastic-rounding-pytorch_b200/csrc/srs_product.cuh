@@ -527,6 +527,7 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
 // Where a warp's 32 accumulator rows go.
 struct TileRows {
   int batch, row0, lane;
+  int col_end;    // end of the tile's columns inside the matrix
   bool mirror;    // symmetric: also store the transposed tile
   float factor;
   uint32_t staged;
@@ -608,13 +609,13 @@ __device__ __forceinline__ void write_columns(const ProductArgs& a, const TileRo
     __syncwarp();
     store_piece(t.staged,
                 static_cast<char*>(e.out) + 2 * (at + (int64_t)t.row0 * e.ldd + col0), 2, e.ldd,
-                rows, a.n - col0, t.lane);
+                rows, t.col_end - col0, t.lane);
     __syncwarp();
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int col = col0 + 32 * h;
-      if (col >= a.n) break;
+      if (col >= t.col_end) break;
 #pragma unroll
       for (int c = 0; c < 32; ++c)
         v[h][c] = __float_as_uint(__uint_as_float(v[h][c]) * t.factor);
@@ -625,14 +626,14 @@ __device__ __forceinline__ void write_columns(const ProductArgs& a, const TileRo
         const int64_t first = (int64_t)t.row0 * a.n + col;
         if (target.flags & SRS_ROW_PARAM_BF16)
           update_piece<true>(t.staged, reinterpret_cast<char*>(target.param) + 2 * first, a.n,
-                             rows, a.n - col, e.step, e.decay, t.lane);
+                             rows, t.col_end - col, e.step, e.decay, t.lane);
         else
           update_piece<false>(t.staged, reinterpret_cast<char*>(target.param) + 4 * first, a.n,
-                              rows, a.n - col, e.step, e.decay, t.lane);
+                              rows, t.col_end - col, e.step, e.decay, t.lane);
       } else {
         store_piece(t.staged,
                     static_cast<char*>(e.out) + 4 * (at + (int64_t)t.row0 * e.ldd + col), 4, e.ldd,
-                    rows, a.n - col, t.lane);
+                    rows, t.col_end - col, t.lane);
       }
       __syncwarp();
     }
@@ -645,13 +646,17 @@ template <int KIND, int CG>
 struct ProductShape {
   static constexpr int kTileRows = 128 * CG;  // over the CTA group
   static constexpr int kTileCols = 128 * CG;
-  static constexpr int kScaleBytes = KIND == kOperandF8 ? 512 * (1 + CG) : 0;  // per slot
   // Accumulator 1 starts after accumulator 0, except that for FP8 pairs both
-  // accumulators and the scales do not fit 512 columns: they then share 32
-  // columns, which the writing warps drain first.
-  static constexpr int kShared = (KIND == kOperandF8 && CG == 2) ? 32 : 0;
+  // accumulators and two groups of scales do not fit the 512 columns of TMEM: the
+  // accumulators then share 32 columns, which the writing warps drain first, and a
+  // tile starts once the one before is drained that far.  (Tiles of 240 columns
+  // need no sharing and take fewer cycles, 17.0k instead of 18.6k for k = 4096, but
+  // load more bytes per operation and were 4-7 % slower in time under the power
+  // cap: 8192 x 14336 x 4096 429 us, with 256 columns 412 us.)
+  static constexpr int kShared = KIND == kOperandF8 && CG == 2 ? 32 : 0;
   static constexpr int kSecond = kTileCols - kShared;
-  static constexpr int kScaleColumn = 480;  // 2 slots of 12 columns (pitch 16)
+  static constexpr int kScaleBytes = KIND == kOperandF8 ? 512 * (1 + CG) : 0;  // per slot
+  static constexpr int kScaleColumn = 480;  // 2 groups of 12 columns (pitch 16)
   static constexpr int kStageBytes = 2 * kPanelBytes;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes +
                                4 * kPieceBytes;
@@ -760,14 +765,39 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // bytes per MMA step of k (32 bytes; 16 rows of 128 bytes when rows are inner)
     const uint32_t step_a = (a.a_rows_inner ? 2048u : 32u) >> 4;
     const uint32_t step_b = (a.b_rows_inner ? 2048u : 32u) >> 4;
-    int s = 0, slot = 0, last_slot = -1, count = 0;
-    uint32_t phase = 0, slot_phase = 0, last_phase = 0, group = 0;
+    int s = 0, slot = 0, count = 0;
+    uint32_t phase = 0, slot_phase = 0;
+    // Scales go to TMEM one group ahead: the copy of group h is issued behind the
+    // second slice of group h - 1, so that no MMA waits for it.  Its columns were
+    // last read by group h - 2, whose last slice gave back stage done_stage.
+    uint32_t group = 0, done_phase = 0;
+    int done_stage = -1;
+    const int groups = (slices + 3) >> 2;
+    const auto copy_group = [&](uint32_t h) {
+      if (done_stage >= 0) ok = barrier_wait(empty(done_stage), done_phase, a.status, 8u);
+      ok = ok && barrier_wait(scale_full(slot), slot_phase, a.status, 8u);
+      if (!ok) return;
+      tmem_fence_after();
+      const uint32_t src = scales0 + slot * S::kScaleBytes;
+      const uint32_t dst = tmem + S::kScaleColumn + 16u * (h & 1u);
+      if (leader) {
+#pragma unroll
+        for (int c = 0; c < 1 + CG; ++c)
+          copy_scales<CG>(dst + 4 * c, scale_descriptor(src + 512 * c));
+        mma_commit<CG>(scale_empty(slot));
+      }
+      __syncwarp();
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        slot_phase ^= 1u;
+      }
+    };
+    if (KIND == kOperandF8 && first < a.n_tiles) copy_group(0);
     for (int64_t t = first; t < a.n_tiles && ok; t += step, ++count) {
       const int acc = count & 1;
       const uint32_t d = tmem + acc * S::kSecond;
-      // The accumulator was drained two tiles ago; with shared columns, the
-      // previous tile's first chunk must have been drained too (acc_empty of
-      // that accumulator is then signalled after its shared columns).
+      // The tile before the previous one has left this accumulator; with shared
+      // columns, the previous tile has left those (and so has the one before it).
       if (S::kShared == 0) {
         if (count >= 2) ok = barrier_wait(acc_empty(acc), ((count >> 1) - 1) & 1u, a.status, 4u);
       } else {
@@ -775,36 +805,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
       tmem_fence_after();
       for (int i = 0; i < slices && ok; ++i) {
-        uint32_t scale_tmem = 0;
-        if constexpr (KIND == kOperandF8) {
-          scale_tmem = tmem + S::kScaleColumn + 16u * (group & 1u);
-          if ((i & 3) == 0) {
-            // This group's TMEM columns were last read by the MMAs of the group
-            // before the previous one; they are done once the commit that
-            // followed the previous group's copy has arrived.
-            if (last_slot >= 0) ok = barrier_wait(scale_empty(last_slot), last_phase, a.status, 8u);
-            ok = ok && barrier_wait(scale_full(slot), slot_phase, a.status, 8u);
-            if (!ok) break;
-            tmem_fence_after();
-            const uint32_t src = scales0 + slot * S::kScaleBytes;
-            if (leader) {
-#pragma unroll
-              for (int c = 0; c < 1 + CG; ++c)
-                copy_scales<CG>(scale_tmem + 4 * c, scale_descriptor(src + 512 * c));
-              mma_commit<CG>(scale_empty(slot));
-            }
-            __syncwarp();
-            last_slot = slot;
-            last_phase = slot_phase;
-            if (++slot == kScaleSlots) {
-              slot = 0;
-              slot_phase ^= 1u;
-            }
-          }
-        }
         ok = barrier_wait(full(s), phase, a.status, 16u);
         if (!ok) break;
         tmem_fence_after();
+        const uint32_t scale_tmem = tmem + S::kScaleColumn + 16u * (group & 1u);
         const uint32_t pa = stage0 + s * S::kStageBytes;
         const uint64_t da = desc_a | uint64_t((pa >> 4) & 0x3FFFu);
         const uint64_t db = desc_b | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
@@ -823,11 +827,21 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           mma_commit<CG>(empty(s));
         }
         __syncwarp();
+        if constexpr (KIND == kOperandF8) {
+          const bool last = id == 3 || i == slices - 1;
+          if (id == 1 || (last && id == 0)) {
+            if ((i >> 2) + 1 < groups || t + step < a.n_tiles) copy_group(group + 1);
+          }
+          if (last) {
+            ++group;
+            done_stage = s;
+            done_phase = phase;
+          }
+        }
         if (++s == kStages) {
           s = 0;
           phase ^= 1u;
         }
-        if (KIND == kOperandF8 && ((i & 3) == 3 || i == slices - 1)) ++group;
       }
       if (ok && leader) mma_commit<CG>(acc_full(acc));
       __syncwarp();
@@ -840,36 +854,57 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, 0);
     int slot = 0;
     uint32_t phase = 0;
-    for (int64_t t = first; t < a.n_tiles && ok; t += step) {
-      const TileAt at = tile_at(a, t);
-      const int ra = at.m * S::kTileRows + 128 * (int)rank;
-      const int rb = at.n * S::kTileCols;
-      ScaleRows from[1 + CG];
-      from[0].at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, ra, a.m, lane);
+    // One group ahead: the next group's scales are requested before this one's
+    // slot is waited for.
+    int64_t t = first;
+    int kb = 0;
+    ScaleRows from[1 + CG];
+    uint32_t next[1 + CG][4];
+    const auto request = [&]() {
+      if (kb == 0) {
+        const TileAt at = tile_at(a, t);
+        from[0].at(a.scale_a, a.scale_a_pitch, a.scale_a_shift,
+                   at.m * S::kTileRows + 128 * (int)rank, a.m, lane);
 #pragma unroll
-      for (int c = 0; c < CG; ++c)
-        from[1 + c].at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, rb + 128 * c, a.n, lane);
-      for (int kb = 0; kb < slices; kb += 4) {
-        uint32_t w[1 + CG][4];
-        from[0].read(kb, slices, words_a, w[0]);
+        for (int c = 0; c < CG; ++c)
+          from[1 + c].at(a.scale_b, a.scale_b_pitch, a.scale_b_shift,
+                         at.n * S::kTileCols + 128 * c, a.n, lane);
+      }
+      from[0].read(kb, slices, words_a, next[0]);
 #pragma unroll
-        for (int c = 0; c < CG; ++c) from[1 + c].read(kb, slices, words_b, w[1 + c]);
-        ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 32u);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
-        const uint32_t dst = scales0 + slot * S::kScaleBytes + 16u * lane;
+      for (int c = 0; c < CG; ++c) from[1 + c].read(kb, slices, words_b, next[1 + c]);
+      kb += 4;
+      if (kb >= slices) {
+        kb = 0;
+        t += step;
+      }
+    };
+    bool more = t < a.n_tiles;
+    if (more) request();
+    while (more) {
+      uint32_t w[1 + CG][4];
 #pragma unroll
-        for (int c = 0; c < 1 + CG; ++c)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 * c),
-                       "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
-                       : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) barrier_arrive(map_to_rank(scale_full(slot), 0));
-        if (++slot == kScaleSlots) {
-          slot = 0;
-          phase ^= 1u;
-        }
+      for (int c = 0; c < 1 + CG; ++c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[c][j] = next[c][j];
+      }
+      more = t < a.n_tiles;
+      if (more) request();
+      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 32u);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      const uint32_t dst = scales0 + slot * S::kScaleBytes + 16u * lane;
+#pragma unroll
+      for (int c = 0; c < 1 + CG; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 * c), "r"(w[c][0]),
+                     "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
+                     : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive(map_to_rank(scale_full(slot), 0));
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        phase ^= 1u;
       }
     }
     for (int i = 0; i < kScaleSlots && ok; ++i) {
@@ -899,6 +934,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       rows.staged = staged0 + warp * kPieceBytes;
       const int col0 = at.n * S::kTileCols;
       constexpr int kPieces = S::kTileCols / 64;
+      rows.col_end = min(a.n, col0 + S::kTileCols);
       uint4 add[8];
       if (EPILOGUE == kEpilogueSymmetric && a.e.addend != nullptr) load_addend(a, rows, col0, add);
       ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, a.status, 128u);
@@ -920,9 +956,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           __syncwarp();
           if (lane == 0) barrier_arrive(map_to_rank(acc_empty(acc), 0));
         }
-        if (rows.row0 < a.m && col0 + 64 * c < a.n)
+        if (rows.row0 < a.m && col0 + 64 * c < rows.col_end)
           write_columns<EPILOGUE>(a, rows, col0 + 64 * c, v, add,
-                                  i + 1 < kPieces ? col0 + 64 * (c + 1) : -1);
+                                  c + 1 < kPieces ? col0 + 64 * (c + 1) : -1);
       }
     }
   }
