@@ -319,21 +319,32 @@ int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch, int64_t ba
                       const srs_newton* h, void* workspace, int64_t workspace_bytes,
                       void* stream);
 
-/* Muon step of n_rows matrices of one shape (m x n, contiguous): per element, each
- * FP32 operation rounded once,
+/* Muon step of the matrices of up to SRS_MUON_MAX_CLASSES shapes (contiguous): per
+ * element, each FP32 operation rounded once,
  *   u' = u*momentum + g;  v = nesterov ? u'*momentum + g : u'
  *   p' = fma(neg_step, O, p*decay),  O = the orthogonalised v of the matrix
  * u' is stored in u_format by u_rule (counter base state_key(key, 0), as the other
  * steps).  `rows`: DEVICE array as for srs_adamw_multi; param, grad, state[0],
- * param_index, offset and flags are used, numel and tile_begin are not.
- * neg_step = -(lr * the shape's factor), decay = 1 - lr*weight_decay. */
+ * param_index, offset and flags are used, numel and tile_begin are not.  `classes`: HOST
+ * array; class i covers rows [first, first + count), matrices of m x n, count > 0.
+ * neg_step = -(lr * the shape's factor), decay = 1 - lr*weight_decay.
+ * `workspace`: srs_muon_workspace(classes, n_classes) bytes (-1: invalid classes). */
+#define SRS_MUON_MAX_CLASSES 16
+typedef struct srs_muon_class {
+  int64_t first, count, m, n;
+  float neg_step;
+  int32_t reserved;
+} srs_muon_class;
+
 typedef struct srs_muon_hparams {
-  float momentum, neg_step, decay;
+  float momentum, decay;
   int32_t nesterov;
 } srs_muon_hparams;
 
-int srs_muon_multi(const srs_row* rows, int64_t n_rows, int64_t m, int64_t n, int u_format,
-                   int u_rule, const srs_muon_hparams* hp, const srs_newton* h,
+int64_t srs_muon_workspace(const srs_muon_class* classes, int n_classes);
+
+int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes, int n_classes,
+                   int u_format, int u_rule, const srs_muon_hparams* hp, const srs_newton* h,
                    const srs_rng* rng, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- FP8 blocks and their products -----------------------------------------

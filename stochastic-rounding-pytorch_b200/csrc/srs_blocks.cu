@@ -4,10 +4,9 @@
 // Why powers of two: scaling is then exact, so an element is rounded once, and
 // the tensor core's block-scaled MMA applies the scales itself (UE8M0), so the
 // product loop has no FP32 work of its own.
-#include <utility>
-
 #include "srs_host.h"
-#include "srs_product.cuh"
+#include "srs_common.cuh"
+#include "srs_launch.h"
 
 namespace srs {
 namespace {
@@ -434,28 +433,9 @@ extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64
         cudaMemsetAsync(d, 0, (size_t)a->rows * b->rows * fmt_bytes(d_format), st);
     return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_matmul_blocks");
   }
-  ProductArgs args{};
-  args.scale_a = reinterpret_cast<const uint8_t*>(a->scale);
-  args.scale_b = reinterpret_cast<const uint8_t*>(b->scale);
-  args.scale_a_pitch = a->scale_pitch;
-  args.scale_b_pitch = b->scale_pitch;
-  args.scale_a_shift = a->square ? 7 : 0;
-  args.scale_b_shift = b->square ? 7 : 0;
-  args.e.alpha = 1.0f;
-  args.e.out = d;
-  args.e.out_format = d_format;
-  args.e.ldd = b->rows;
-  args.e.batch_stride = a->rows * b->rows;
-  const ProductOperand oa{reinterpret_cast<const void*>(a->data), a->rows, k, a->pitch, 0, false};
-  const ProductOperand ob{reinterpret_cast<const void*>(b->data), b->rows, k, b->pitch, 0, false};
   // Few rows on one side: the other side's bytes bound the product.
   if (b->rows <= kThinRows && a->rows >= b->rows)
-    return launch_thin(oa, ob, a->format, b->format, args, d, d_format, b->rows, 1, st);
-  if (a->rows <= kThinRows) {
-    std::swap(args.scale_a, args.scale_b);
-    std::swap(args.scale_a_pitch, args.scale_b_pitch);
-    std::swap(args.scale_a_shift, args.scale_b_shift);
-    return launch_thin(ob, oa, b->format, a->format, args, d, d_format, 1, b->rows, st);
-  }
-  return launch_product(kOperandF8, kEpilogueStore, oa, ob, 1, a->format, b->format, args, st);
+    return launch_thin(*a, *b, k, d, d_format, b->rows, 1, st);
+  if (a->rows <= kThinRows) return launch_thin(*b, *a, k, d, d_format, 1, b->rows, st);
+  return launch_block_product(*a, *b, k, d, d_format, st);
 }

@@ -23,6 +23,12 @@
 // the remaining factor rho enters the first products in FP32.  The norm is
 // summed in FP64, so no input in range overflows or vanishes in it.
 //
+// Three launches: the norm, X_0, and one cooperative grid that runs the 3 * steps
+// products of all matrices, whatever their shapes, as phases with a grid-wide
+// meeting between them (a launch a product took 7 us each where the products
+// themselves take 1 to 3).  G and P are symmetric: only tiles on and below the
+// diagonal are computed and stored twice.
+//
 // Reads of V: one for the norm and one for X_0.  For an optimizer step both
 // passes compute V from the gradient and the momentum (8 or fewer bytes an
 // element) rather than keeping V in FP32 (8 bytes more of traffic and 4 of
@@ -30,30 +36,49 @@
 #include <cmath>
 
 #include "srs_host.h"
+#include "srs_launch.h"
 #include "srs_product.cuh"
 
 namespace srs {
 namespace {
 
-constexpr int kSumChunks = 256;  // most partial sums of a matrix
-constexpr int kPlain = -1;       // source template value: a plain tensor
+constexpr int kMaxClasses = SRS_MUON_MAX_CLASSES;
+static_assert(kMaxPhases <= kThreads, "one CTA zeroes the counters");
+constexpr int kSumChunks = 1024;  // most partial sums of a matrix
+constexpr int kPlain = -1;        // source template value: a plain tensor
 // G and P are held times 2^8: their small elements (1 / m and less in the first
 // steps) then stay among FP16's normal numbers, and eigenvalues up to 255 fit.
 constexpr float kHeld = 256.0f;
 
+// Where the matrices of one shape come from and go to.
 struct NewtonSource {
   const void* x;      // plain: the tensor
   int x_format;       // plain: SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t row_pitch, batch_stride;
   int vec;            // plain: rows start on 16-byte boundaries
   const srs_row* rows;  // Muon: one row per matrix
+  int m, n;           // rows, columns
+  uint32_t units;     // vectors of 8 per matrix: m * ceil(n / 8)
+  uint32_t row_units;
+  int first, count;   // matrices of this shape among all
+  int chunks;         // partial sums of one matrix
+  int target;         // floor(log2(sqrt(min(m, n))))
+  __half* x0;
+  int64_t ld, x_elems;
+  float* rho;
+};
+
+// One launch over the matrices of several shapes (blockIdx.y: the matrix).
+struct NewtonPlan {
+  NewtonSource source[kMaxClasses];
+  int classes;
+  double* partial;    // kSumChunks for each matrix
+  unsigned int* counters;  // of the product grid's phases, set to zero here
+  double eps;
   srs_rng rng;
   float momentum;
   int nesterov;
   int u_rule;
-  int m, n;           // rows, columns
-  uint32_t units;     // vectors of 8 per matrix: m * ceil(n / 8)
-  uint32_t row_units;
 };
 
 struct Unit {
@@ -73,8 +98,9 @@ __device__ __forceinline__ Unit unit_of(const NewtonSource& s, uint32_t u, int64
 // 8 elements of V at `u` (elements beyond the row: zero).  With STORE the new
 // momentum is written back as well.
 template <int U, bool STORE>
-__device__ __forceinline__ void source8(const NewtonSource& s, const srs_row& row, uint32_t ctr,
-                                        int batch, uint32_t u, float (&v)[kVec]) {
+__device__ __forceinline__ void source8(const NewtonPlan& plan, const NewtonSource& s,
+                                        const srs_row& row, uint32_t ctr, int batch, uint32_t u,
+                                        float (&v)[kVec]) {
   if constexpr (U == kPlain) {
     const Unit w = unit_of(s, u, s.row_pitch);
     const bool vec = s.vec && w.count == 8;
@@ -93,24 +119,31 @@ __device__ __forceinline__ void source8(const NewtonSource& s, const srs_row& ro
     float next[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      next[j] = __fadd_rn(__fmul_rn(old[j], s.momentum), g[j]);
-      v[j] = s.nesterov ? __fadd_rn(__fmul_rn(next[j], s.momentum), g[j]) : next[j];
+      next[j] = __fadd_rn(__fmul_rn(old[j], plan.momentum), g[j]);
+      v[j] = plan.nesterov ? __fadd_rn(__fmul_rn(next[j], plan.momentum), g[j]) : next[j];
     }
     if constexpr (STORE)
       store_state8<U>(reinterpret_cast<void*>(row.state[0]), w.at, w.count, vec, next,
-                      ctr + (uint32_t)w.at, s.u_rule);
+                      ctr + (uint32_t)w.at, plan.u_rule);
   }
 }
 
 template <int U>
-__device__ __forceinline__ void open_row(const NewtonSource& s, int batch, srs_row* row,
-                                         uint32_t* ctr) {
+__device__ __forceinline__ void open_row(const NewtonPlan& plan, const NewtonSource& s, int batch,
+                                         srs_row* row, uint32_t* ctr) {
   if constexpr (U != kPlain) {
     *row = s.rows[batch];
-    const uint32_t key = (s.rng.key_mode == SRS_KEY_GIVEN) ? row->param_index
-                                                           : update_key(s.rng, row->param_index);
+    const uint32_t key = (plan.rng.key_mode == SRS_KEY_GIVEN)
+                             ? row->param_index
+                             : update_key(plan.rng, row->param_index);
     *ctr = row->offset + state_key(key, 0u);
   }
+}
+
+__device__ __forceinline__ int class_of(const NewtonPlan& plan, int matrix) {
+  int c = 0;
+  while (c + 1 < plan.classes && matrix >= plan.source[c + 1].first) ++c;
+  return c;
 }
 
 __device__ __forceinline__ double block_sum(double x, double* shared) {
@@ -125,189 +158,403 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {
 
 // Partial sums of squares, in an order that depends on the sizes alone.
 template <int U>
-__global__ void __launch_bounds__(kThreads) newton_sum_kernel(const NewtonSource s,
-                                                              double* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads)
+newton_sum_kernel(const __grid_constant__ NewtonPlan plan) {
   __shared__ double shared[kThreads / 32];
-  const int batch = blockIdx.y;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kMaxPhases)
+    plan.counters[threadIdx.x] = 0u;
+  const NewtonSource& s = plan.source[class_of(plan, (int)blockIdx.y)];
+  if ((int)blockIdx.x >= s.chunks) return;
+  const int batch = (int)blockIdx.y - s.first;
   srs_row row{};
   uint32_t ctr = 0;
-  open_row<U>(s, batch, &row, &ctr);
+  open_row<U>(plan, s, batch, &row, &ctr);
   double sum = 0.0;
-  for (uint32_t u = blockIdx.x * kThreads + threadIdx.x; u < s.units; u += gridDim.x * kThreads) {
+  const uint32_t stride = (uint32_t)s.chunks * kThreads;
+#pragma unroll 2
+  for (uint32_t u = blockIdx.x * kThreads + threadIdx.x; u < s.units; u += stride) {
     float v[kVec];
-    source8<U, false>(s, row, ctr, batch, u, v);
+    source8<U, false>(plan, s, row, ctr, batch, u, v);
 #pragma unroll
     for (int j = 0; j < kVec; ++j) sum = fma((double)v[j], (double)v[j], sum);
   }
   const double total = block_sum(sum, shared);
-  if (threadIdx.x == 0) partial[(int64_t)batch * gridDim.x + blockIdx.x] = total;
+  if (threadIdx.x == 0) plan.partial[(int64_t)blockIdx.y * kSumChunks + blockIdx.x] = total;
 }
 
 // X_0 = V * 2^j in FP16 (row pitch `ld`, padding zero) and rho = (|V|_F + eps) * 2^j.
 template <int U>
 __global__ void __launch_bounds__(kThreads)
-newton_scale_kernel(const NewtonSource s, const double* __restrict__ partial, int chunks,
-                    double eps, int target, __half* __restrict__ x0, int64_t ld,
-                    int64_t batch_stride, float* __restrict__ rho) {
+newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
   __shared__ double shared[kThreads / 32];
-  const int batch = blockIdx.y;
-  const double part =
-      (int)threadIdx.x < chunks ? partial[(int64_t)batch * chunks + threadIdx.x] : 0.0;
-  const double norm = sqrt(block_sum(part, shared)) + eps;
+  const NewtonSource& s = plan.source[class_of(plan, (int)blockIdx.y)];
+  if ((int)blockIdx.x >= s.chunks) return;
+  const int batch = (int)blockIdx.y - s.first;
+  double part = 0.0;
+  for (int i = threadIdx.x; i < s.chunks; i += kThreads)
+    part += plan.partial[(int64_t)blockIdx.y * kSumChunks + i];
+  const double norm = sqrt(block_sum(part, shared)) + plan.eps;
   int exponent = 0;
   const bool finite = norm < INFINITY;  // false for NaN
   const double fraction = finite ? frexp(norm, &exponent) : 0.0;
-  const int j = target - exponent;
+  const int j = s.target - exponent;
   // Two exact factors, as 2^j itself may not be an FP32 number.
   const float scale0 = finite ? (float)ldexp(1.0, j / 2) : __int_as_float(0x7FC00000);
   const float scale1 = (float)ldexp(1.0, j - j / 2);
   if (blockIdx.x == 0 && threadIdx.x == 0)
-    rho[batch] = finite ? (float)ldexp(fraction, target) : __int_as_float(0x7FC00000);
+    s.rho[batch] = finite ? (float)ldexp(fraction, s.target) : __int_as_float(0x7FC00000);
 
   srs_row row{};
   uint32_t ctr = 0;
-  open_row<U>(s, batch, &row, &ctr);
-  __half* out = x0 + (int64_t)batch * batch_stride;
-  for (uint32_t u = blockIdx.x * kThreads + threadIdx.x; u < s.units; u += gridDim.x * kThreads) {
+  open_row<U>(plan, s, batch, &row, &ctr);
+  __half* out = s.x0 + (int64_t)batch * s.x_elems;
+  const uint32_t stride = (uint32_t)s.chunks * kThreads;
+#pragma unroll 2
+  for (uint32_t u = blockIdx.x * kThreads + threadIdx.x; u < s.units; u += stride) {
     float v[kVec];
-    source8<U, true>(s, row, ctr, batch, u, v);
+    source8<U, true>(plan, s, row, ctr, batch, u, v);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) v[i] = v[i] * scale0 * scale1;
     encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
-    const Unit at = unit_of(s, u, ld);
+    const Unit at = unit_of(s, u, s.ld);
     *reinterpret_cast<uint4*>(out + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+// ------------------------------------------------------------------ products --
 
-// Workspace: partial sums, rho, two copies of X and G and P, each aligned to 256 bytes.
-struct NewtonSpace {
-  int64_t ld, small_ld, x_elems, small_elems;
-  int64_t partial, rho, x[2], g, p, bytes;
+// Matrices of one shape in the product grid.
+struct NewtonClass {
+  CUtensorMap along[2];   // X, both copies, as the operands of G
+  CUtensorMap across[2];  // X as the operand of X = P X
+  CUtensorMap g, p;
+  int m, n, small, tall;
+  int long_slices, small_slices;
+  uint32_t triangle, grid_m, grid_n;  // tiles of G and P; of X
+  int64_t ld, x_elems, small_ld, small_elems;
+  __half* x[2];
+  __half* g_at;
+  __half* p_at;
+  const float* rho;
+  char* out;             // orthogonalize: the result, contiguous matrices
+  int out_format;
+  const srs_row* rows;   // Muon: the parameters
+  float step, decay;
 };
 
-NewtonSpace newton_space(int64_t batch, int64_t m, int64_t n) {
-  NewtonSpace s{};
-  const int64_t small = m < n ? m : n;
-  s.ld = round_up(n, 8);
-  s.small_ld = round_up(small, 8);
-  s.x_elems = m * s.ld;
-  s.small_elems = small * s.small_ld;
-  int64_t at = 0;
-  const auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += round_up(bytes, 256);
-    return here;
+struct NewtonWork {
+  NewtonClass shape[kMaxClasses];
+  uint32_t triangles[kMaxClasses + 1];  // first tile of each class in a G or P phase
+  uint32_t grids[kMaxClasses + 1];      // ... in an X phase
+  int classes, steps, edge;
+  float a, b, c;
+  unsigned int* counters;  // one a phase
+  unsigned int* status_at;
+};
+
+// Phase 3 i: G = X X^T; 3 i + 1: P = a I + b G + c G G; 3 i + 2: X = P X.
+struct NewtonProducts {
+  const NewtonWork& w;
+  struct Place {
+    int shape, batch, row, col;
   };
-  s.partial = take(batch * kSumChunks * 8);
-  s.rho = take(batch * 4);
-  s.x[0] = take(batch * s.x_elems * 2);
-  s.x[1] = take(batch * s.x_elems * 2);
-  s.g = take(batch * s.small_elems * 2);
-  s.p = take(batch * s.small_elems * 2);
-  s.bytes = at;
+  __device__ int phases() const { return 3 * w.steps; }
+  __device__ uint32_t tiles(int p) const {
+    return p % 3 == 2 ? w.grids[w.classes] : w.triangles[w.classes];
+  }
+  __device__ uint32_t formats() const { return 0u; }
+  __device__ unsigned int* counter(int p) const { return w.counters + p; }
+  __device__ unsigned int* status() const { return w.status_at; }
+  __device__ Place place(int p, uint32_t t) const {
+    const bool grid = p % 3 == 2;
+    const uint32_t* begin = grid ? w.grids : w.triangles;
+    Place r;
+    r.shape = 0;
+    while (t >= begin[r.shape + 1]) ++r.shape;
+    t -= begin[r.shape];
+    const NewtonClass& s = w.shape[r.shape];
+    const uint32_t each = grid ? s.grid_m * s.grid_n : s.triangle;
+    r.batch = (int)(t / each);
+    t -= (uint32_t)r.batch * each;
+    if (grid) banded_tile(t, s.grid_m, s.grid_n, &r.row, &r.col);
+    else triangle_tile(t, &r.row, &r.col);
+    r.row *= w.edge;
+    r.col *= w.edge;
+    return r;
+  }
+  __device__ TileLoad load(int p, uint32_t t) const {
+    const Place at = place(p, t);
+    const NewtonClass& s = w.shape[at.shape];
+    const int step = p / 3, kind = p - 3 * step;
+    const bool tall = s.tall != 0;
+    TileLoad r;
+    r.row0 = at.row;
+    r.col0 = at.col;
+    r.batch = at.batch;
+    if (kind == 0) {
+      r.map_a = r.map_b = &s.along[step & 1];
+      r.slices = s.long_slices;
+      r.a_rows_inner = r.b_rows_inner = tall;
+    } else if (kind == 1) {
+      r.map_a = r.map_b = &s.g;
+      r.slices = s.small_slices;
+      r.a_rows_inner = r.b_rows_inner = false;
+    } else {
+      // P X: P by its rows, X with its row index (the summed one) outer; X P: X by
+      // its rows, and P's columns are its rows
+      r.map_a = tall ? &s.across[step & 1] : &s.p;
+      r.map_b = tall ? &s.p : &s.across[step & 1];
+      r.slices = s.small_slices;
+      r.a_rows_inner = false;
+      r.b_rows_inner = !tall;
+    }
+    return r;
+  }
+  __device__ TileStore store(int p, uint32_t t) const {
+    const Place at = place(p, t);
+    const NewtonClass& s = w.shape[at.shape];
+    const int step = p / 3, kind = p - 3 * step;
+    TileStore r{};
+    r.row0 = at.row;
+    r.col0 = at.col;
+    // The first step's operand stands for X / rho.
+    float rho = 1.0f;
+    if (step == 0 && kind != 1) rho = s.rho[at.batch];
+    r.format = SRS_FMT_F16;
+    if (kind != 2) {
+      const int64_t from = (int64_t)at.batch * s.small_elems;
+      r.m = r.n = s.small;
+      r.mirror = at.row != at.col;
+      r.pitch = s.small_ld;
+      if (kind == 0) {
+        r.factor = __fdiv_rn(kHeld, __fmul_rn(rho, rho));
+        r.out = reinterpret_cast<char*>(s.g_at + from);
+      } else {
+        r.factor = w.c / kHeld;
+        r.beta = w.b;
+        r.diagonal = w.a * kHeld;
+        r.addend = s.g_at + from;
+        r.out = reinterpret_cast<char*>(s.p_at + from);
+      }
+    } else {
+      r.m = s.m;
+      r.n = s.n;
+      r.factor = __fdiv_rn(1.0f / kHeld, rho);
+      if (step + 1 < w.steps) {
+        r.pitch = s.ld;
+        r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
+      } else if (s.rows != nullptr) {
+        const srs_row& row = s.rows[at.batch];
+        r.update = 1;
+        r.format = (row.flags & SRS_ROW_PARAM_BF16) ? SRS_FMT_BF16 : SRS_FMT_F32;
+        r.out = reinterpret_cast<char*>(row.param);
+        r.pitch = s.n;
+        r.step = s.step;
+        r.decay = s.decay;
+      } else {
+        r.format = s.out_format;
+        r.pitch = s.n;
+        r.out = s.out + (int64_t)at.batch * s.m * s.n * (s.out_format == SRS_FMT_F32 ? 4 : 2);
+      }
+    }
+    return r;
+  }
+};
+
+template <int CG>
+__global__ void __launch_bounds__(kProductThreads, 1)
+newton_kernel(const __grid_constant__ NewtonWork w) {
+  run_products<kOperandF16, CG, true>(NewtonProducts{w});
+}
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// The matrices of one shape and their part of the workspace: rho, two copies of X
+// and G and P, each aligned to 256 bytes.
+struct NewtonShape {
+  int64_t batch, m, n, small, ld, small_ld, x_elems, small_elems;
+  int64_t rho, x[2], g, p;  // byte offsets
+};
+
+int64_t take(int64_t* at, int64_t bytes) {
+  const int64_t here = *at;
+  *at += round_up(bytes, 256);
+  return here;
+}
+
+NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, int64_t* at) {
+  NewtonShape s{};
+  s.batch = batch;
+  s.m = m;
+  s.n = n;
+  s.small = m < n ? m : n;
+  s.ld = round_up(n, 8);
+  s.small_ld = round_up(s.small, 8);
+  s.x_elems = m * s.ld;
+  s.small_elems = s.small * s.small_ld;
+  s.rho = take(at, batch * 4);
+  s.x[0] = take(at, batch * s.x_elems * 2);
+  s.x[1] = take(at, batch * s.x_elems * 2);
+  s.g = take(at, batch * s.small_elems * 2);
+  s.p = take(at, batch * s.small_elems * 2);
   return s;
 }
 
+// Shared by all shapes of a call: the grid's counters and the partial sums.
+int64_t lay_out_head(int64_t matrices, int64_t* at) {
+  take(at, kMaxPhases * 4);
+  return take(at, matrices * kSumChunks * 8);
+}
+
 template <int U>
-int prepare(const NewtonSource& source, int64_t batch, const NewtonSpace& w, char* space,
-            double eps, cudaStream_t stream) {
-  // Enough CTAs for a few per SM; each gets at least 4 vectors a thread.
-  int64_t chunks = (4ll * sm_count() + batch - 1) / batch;
-  const int64_t most = (source.units + 4 * kThreads - 1) / (4 * kThreads);
-  if (chunks > most) chunks = most;
-  if (chunks > kSumChunks) chunks = kSumChunks;
-  if (chunks < 1) chunks = 1;
-  const dim3 grid((unsigned)chunks, (unsigned)batch);
-  double* partial = reinterpret_cast<double*>(space + w.partial);
-  newton_sum_kernel<U><<<grid, kThreads, 0, stream>>>(source, partial);
+int launch_prepare(const NewtonPlan& plan, int64_t matrices, int chunks, cudaStream_t stream) {
+  const dim3 grid((unsigned)chunks, (unsigned)matrices);
+  newton_sum_kernel<U><<<grid, kThreads, 0, stream>>>(plan);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "newton_sum_kernel launch");
-  const int64_t small = source.m < source.n ? source.m : source.n;
-  int target = 0;  // floor(log2(sqrt(small)))
-  while ((1ll << (2 * (target + 1))) <= small) ++target;
-  newton_scale_kernel<U><<<grid, kThreads, 0, stream>>>(
-      source, partial, (int)chunks, eps, target, reinterpret_cast<__half*>(space + w.x[0]), w.ld,
-      w.x_elems, reinterpret_cast<float*>(space + w.rho));
+  newton_scale_kernel<U><<<grid, kThreads, 0, stream>>>(plan);
   e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "newton_scale_kernel launch");
 }
 
+// Where results go, per class.
 struct NewtonResult {
-  int epilogue;  // kEpilogueStore or kEpilogueMuon
   void* out;
   int out_format;
-  int64_t ldd, batch_stride;
   const srs_row* rows;
   float decay, step;
 };
 
-int newton_steps(int64_t batch, int64_t m, int64_t n, const srs_newton* h, const NewtonSpace& w,
-                 char* space, const NewtonResult& result, cudaStream_t stream) {
-  const bool tall = m > n;
-  const int64_t small = tall ? n : m;
-  const float* rho = reinterpret_cast<const float*>(space + w.rho);
-  __half* g = reinterpret_cast<__half*>(space + w.g);
-  __half* p = reinterpret_cast<__half*>(space + w.p);
-  for (int i = 0; i < h->steps; ++i) {
-    const void* x = space + w.x[i & 1];
-    void* next = space + w.x[(i + 1) & 1];
-    const bool last = i == h->steps - 1;
-    const auto symmetric = [&](float alpha, float beta, float diagonal, const __half* addend,
-                               __half* out, const float* scale) {
-      ProductArgs args{};
-      args.symmetric = 1;
-      args.e.alpha = alpha;
-      args.e.beta = beta;
-      args.e.diagonal = diagonal;
-      args.e.addend = addend;
-      args.e.out = out;
-      args.e.ldd = w.small_ld;
-      args.e.batch_stride = w.small_elems;
-      args.e.rho = scale;
-      args.e.rho_power = 2;
-      return args;
-    };
-    // G = X X^T (X^T X): both operands are X, k along the longer side
-    const ProductOperand along{x, small, tall ? m : n, w.ld, w.x_elems, tall};
-    if (int rc = launch_product(kOperandF16, kEpilogueSymmetric, along, along, batch, 0, 0,
-                                symmetric(kHeld, 0.0f, 0.0f, nullptr, g, i == 0 ? rho : nullptr),
-                                stream))
-      return rc;
-    // P = a I + b G + c G G
-    const ProductOperand gram{g, small, small, w.small_ld, w.small_elems, false};
-    if (int rc = launch_product(
-            kOperandF16, kEpilogueSymmetric, gram, gram, batch, 0, 0,
-            symmetric(h->coefficients[2] / kHeld, h->coefficients[1], h->coefficients[0] * kHeld,
-                      g, p, nullptr),
-            stream))
-      return rc;
-    // X = P X (X P): P is symmetric, so either of its sides serves as k
-    const ProductOperand poly{p, small, small, w.small_ld, w.small_elems, false};
-    const ProductOperand across{x, tall ? m : n, small, w.ld, w.x_elems, !tall};
-    ProductArgs args{};
-    args.e.alpha = 1.0f / kHeld;
-    args.e.rho = i == 0 ? rho : nullptr;
-    args.e.rho_power = 1;
-    args.e.out = last ? result.out : next;
-    args.e.out_format = last ? result.out_format : SRS_FMT_F16;
-    args.e.ldd = last ? result.ldd : w.ld;
-    args.e.batch_stride = last ? result.batch_stride : w.x_elems;
-    args.e.rows = result.rows;
-    args.e.decay = result.decay;
-    args.e.step = result.step;
-    if (int rc = launch_product(kOperandF16, last ? result.epilogue : kEpilogueStore,
-                                tall ? across : poly, tall ? poly : across, batch, 0, 0, args,
-                                stream))
-      return rc;
-  }
-  return SRS_OK;
+// Fills what the two preparing kernels and the product grid share.  The sources'
+// own fields (x or rows) are set by the caller.
+void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
+                 NewtonSource* f) {
+  f->m = (int)s.m;
+  f->n = (int)s.n;
+  f->row_units = (uint32_t)((s.n + 7) / 8);
+  f->units = (uint32_t)(s.m * f->row_units);
+  f->first = first;
+  f->count = (int)s.batch;
+  // Enough CTAs for several per SM; each thread gets at least 4 vectors.
+  int64_t chunks = (8ll * sm_count() + matrices - 1) / matrices;
+  const int64_t most = (f->units + 4 * kThreads - 1) / (4 * kThreads);
+  if (chunks > most) chunks = most;
+  if (chunks > kSumChunks) chunks = kSumChunks;
+  f->chunks = chunks < 1 ? 1 : (int)chunks;
+  f->target = 0;
+  while ((1ll << (2 * (f->target + 1))) <= s.small) ++f->target;
+  f->x0 = reinterpret_cast<__half*>(space + s.x[0]);
+  f->ld = s.ld;
+  f->x_elems = s.x_elems;
+  f->rho = reinterpret_cast<float*>(space + s.rho);
 }
 
-int check_newton(int64_t batch, int64_t m, int64_t n, const srs_newton* h) {
-  if (h == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null Newton-Schulz settings");
+int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, NewtonClass* c) {
+  const bool tall = s.m > s.n;
+  const int64_t longer = tall ? s.m : s.n;
+  c->m = (int)s.m;
+  c->n = (int)s.n;
+  c->small = (int)s.small;
+  c->tall = tall ? 1 : 0;
+  c->long_slices = (int)((longer + 63) / 64);
+  c->small_slices = (int)((s.small + 63) / 64);
+  c->ld = s.ld;
+  c->x_elems = s.x_elems;
+  c->small_ld = s.small_ld;
+  c->small_elems = s.small_elems;
+  c->g_at = reinterpret_cast<__half*>(space + s.g);
+  c->p_at = reinterpret_cast<__half*>(space + s.p);
+  c->rho = reinterpret_cast<const float*>(space + s.rho);
+  c->out = static_cast<char*>(result.out);
+  c->out_format = result.out_format;
+  c->rows = result.rows;
+  c->step = result.step;
+  c->decay = result.decay;
+  for (int i = 0; i < 2; ++i) {
+    c->x[i] = reinterpret_cast<__half*>(space + s.x[i]);
+    // G sums along the longer side, which is contiguous unless X is tall; X = P X
+    // sums along the shorter one
+    const ProductOperand along{c->x[i], s.small, longer, s.ld, s.x_elems, tall};
+    const ProductOperand across{c->x[i], longer, s.small, s.ld, s.x_elems, !tall};
+    if (int rc = encode_operand(along, 2, s.batch, 128, &c->along[i])) return rc;
+    if (int rc = encode_operand(across, 2, s.batch, 128, &c->across[i])) return rc;
+  }
+  const ProductOperand g{c->g_at, s.small, s.small, s.small_ld, s.small_elems, false};
+  const ProductOperand p{c->p_at, s.small, s.small, s.small_ld, s.small_elems, false};
+  if (int rc = encode_operand(g, 2, s.batch, 128, &c->g)) return rc;
+  return encode_operand(p, 2, s.batch, 128, &c->p);
+}
+
+template <int CG>
+int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
+  const void* kernel = reinterpret_cast<const void*>(&newton_kernel<CG>);
+  constexpr int kSmem = ProductShape<kOperandF16, CG>::kSmem;
+  int resident = 0;
+  if (int rc = prepare_kernel(kernel, CG, kProductThreads, kSmem, &resident)) return rc;
+  w.edge = 128 * CG;
+  int64_t triangles = 0, grids = 0;
+  for (int i = 0; i < w.classes; ++i) {
+    NewtonClass& c = w.shape[i];
+    const uint32_t edge = (uint32_t)((c.small + w.edge - 1) / w.edge);
+    c.triangle = edge * (edge + 1) / 2;
+    c.grid_m = (uint32_t)((c.m + w.edge - 1) / w.edge);
+    c.grid_n = (uint32_t)((c.n + w.edge - 1) / w.edge);
+    w.triangles[i] = (uint32_t)triangles;
+    w.grids[i] = (uint32_t)grids;
+    triangles += batch[i] * c.triangle;
+    grids += batch[i] * c.grid_m * c.grid_n;
+  }
+  w.triangles[w.classes] = (uint32_t)triangles;
+  w.grids[w.classes] = (uint32_t)grids;
+  if (triangles >= (1ll << 31) || grids >= (1ll << 31))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "too many matrices for one call");
+  const int64_t most = triangles > grids ? triangles : grids;
+  return launch_groups(kernel, most < resident ? most : resident, CG, kProductThreads, kSmem, true,
+                       &w, stream, "newton_kernel launch");
+}
+
+// Rough time of the three products of a step with tiles of 128 * cg, in cycles of
+// one SM: 512 a slice for the pair, 300 for the single CTA (256 of MMA, but twice
+// the loads for it), and what a tile's results take.
+double step_cycles(const NewtonWork& w, const int64_t* batch, int cg) {
+  const int64_t groups = sm_count() / cg;
+  const double slice = cg == 2 ? 512.0 : 300.0, rest = cg == 2 ? 3000.0 : 1500.0;
+  double total = 0.0;
+  for (int kind = 0; kind < 3; ++kind) {
+    double work = 0.0, longest = 0.0;
+    int64_t tiles = 0;
+    for (int i = 0; i < w.classes; ++i) {
+      const NewtonClass& c = w.shape[i];
+      const int64_t edge = 128 * cg, t = (c.small + edge - 1) / edge;
+      const int64_t each = kind < 2 ? t * (t + 1) / 2
+                                    : (c.m + edge - 1) / edge * ((c.n + edge - 1) / edge);
+      const double cycles = slice * (kind == 0 ? c.long_slices : c.small_slices) + rest;
+      tiles += batch[i] * each;
+      work += cycles * (double)(batch[i] * each);
+      if (cycles > longest) longest = cycles;
+    }
+    // whole rounds of the grid, at the tiles' mean cost
+    const double rounds = (double)((tiles + groups - 1) / groups);
+    const double time = tiles > 0 ? rounds * work / (double)tiles : 0.0;
+    total += time > longest ? time : longest;
+  }
+  return total;
+}
+
+int run_newton(NewtonWork& w, const int64_t* batch, const srs_newton* h, unsigned int* counters,
+               cudaStream_t stream) {
+  w.steps = h->steps;
+  w.a = h->coefficients[0];
+  w.b = h->coefficients[1];
+  w.c = h->coefficients[2];
+  w.counters = counters;
+  if (int rc = status_word(&w.status_at)) return rc;
+  return step_cycles(w, batch, 2) <= step_cycles(w, batch, 1) ? launch_newton<2>(w, batch, stream)
+                                                              : launch_newton<1>(w, batch, stream);
+}
+
+int check_matrices(int64_t batch, int64_t m, int64_t n) {
   if (batch < 0 || m < 0 || n < 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "negative size (%lld, %lld, %lld)", (long long)batch,
                 (long long)m, (long long)n);
@@ -316,6 +563,11 @@ int check_newton(int64_t batch, int64_t m, int64_t n, const srs_newton* h) {
                 "matrices of %lld x %lld (batch %lld) are too large: at most 2^32 elements, 2^24 "
                 "rows or columns and 65535 matrices",
                 (long long)m, (long long)n, (long long)batch);
+  return SRS_OK;
+}
+
+int check_newton(const srs_newton* h) {
+  if (h == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null Newton-Schulz settings");
   if (h->steps < 1 || h->steps > SRS_NEWTON_MAX_STEPS)
     return fail(SRS_ERR_INVALID_ARGUMENT, "steps must be in [1, %d], got %d",
                 SRS_NEWTON_MAX_STEPS, h->steps);
@@ -342,7 +594,10 @@ using namespace srs;
 
 extern "C" int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
-  return newton_space(batch, m, n).bytes;
+  int64_t at = 0;
+  lay_out_head(batch, &at);
+  lay_out(batch, m, n, &at);
+  return at;
 }
 
 extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
@@ -353,7 +608,8 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   if (x_format < SRS_FMT_F32 || x_format > SRS_FMT_F16 || y_format < SRS_FMT_F32 ||
       y_format > SRS_FMT_F16)
     return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported matrix format (%d, %d)", x_format, y_format);
-  if (int rc = check_newton(batch, m, n, h)) return rc;
+  if (int rc = check_newton(h)) return rc;
+  if (int rc = check_matrices(batch, m, n)) return rc;
   if (batch == 0 || m == 0 || n == 0) return SRS_OK;
   if (x == nullptr || y == nullptr)
     return fail(SRS_ERR_INVALID_ARGUMENT, "null input or output pointer");
@@ -363,32 +619,64 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   if (at % fmt_bytes(x_format) != 0 ||
       reinterpret_cast<uintptr_t>(y) % fmt_bytes(y_format) != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "input/output pointers are not element aligned");
-  const NewtonSpace w = newton_space(batch, m, n);
-  if (int rc = check_space(workspace, workspace_bytes, w.bytes)) return rc;
+  if (int rc = check_space(workspace, workspace_bytes, srs_newton_workspace(batch, m, n)))
+    return rc;
   if (int rc = check_device()) return rc;
-  NewtonSource s{};
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* space = static_cast<char*>(workspace);
+  int64_t used = 0;
+  const int64_t partial = lay_out_head(batch, &used);
+  const NewtonShape shape = lay_out(batch, m, n, &used);
+  NewtonPlan plan{};
+  plan.classes = 1;
+  plan.partial = reinterpret_cast<double*>(space + partial);
+  plan.counters = reinterpret_cast<unsigned int*>(space);
+  plan.eps = h->eps;
+  NewtonSource& s = plan.source[0];
   s.x = x;
   s.x_format = x_format;
   s.row_pitch = row_pitch;
   s.batch_stride = batch_stride;
   s.vec = at % 16 == 0 && row_pitch % 8 == 0 && batch_stride % 8 == 0;
-  s.m = (int)m;
-  s.n = (int)n;
-  s.row_units = (uint32_t)((n + 7) / 8);
-  s.units = (uint32_t)(m * s.row_units);
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  char* space = static_cast<char*>(workspace);
-  if (int rc = prepare<kPlain>(s, batch, w, space, h->eps, st)) return rc;
-  NewtonResult r{};
-  r.epilogue = kEpilogueStore;
-  r.out = y;
-  r.out_format = y_format;
-  r.ldd = n;
-  r.batch_stride = m * n;
-  return newton_steps(batch, m, n, h, w, space, r, st);
+  fill_source(shape, space, 0, batch, &s);
+  NewtonWork work{};
+  work.classes = 1;
+  const NewtonResult result{y, y_format, nullptr, 0.0f, 0.0f};
+  if (int rc = fill_class(shape, space, result, &work.shape[0])) return rc;
+  if (int rc = launch_prepare<kPlain>(plan, batch, s.chunks, st)) return rc;
+  return run_newton(work, &batch, h, plan.counters, st);
 }
 
-extern "C" int srs_muon_multi(const srs_row* rows, int64_t n_rows, int64_t m, int64_t n,
+static int check_classes(const srs_muon_class* classes, int n_classes, int64_t* matrices) {
+  if (n_classes < 0 || n_classes > SRS_MUON_MAX_CLASSES)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "between 0 and %d shapes in a call, got %d",
+                SRS_MUON_MAX_CLASSES, n_classes);
+  if (n_classes > 0 && classes == nullptr)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "null shape table");
+  *matrices = 0;
+  for (int i = 0; i < n_classes; ++i) {
+    if (int rc = check_matrices(classes[i].count, classes[i].m, classes[i].n)) return rc;
+    if (classes[i].count == 0 || classes[i].m == 0 || classes[i].n == 0)
+      return fail(SRS_ERR_INVALID_ARGUMENT, "shape %d is empty", i);
+    if (classes[i].first < 0) return fail(SRS_ERR_INVALID_ARGUMENT, "shape %d: negative row", i);
+    *matrices += classes[i].count;
+  }
+  if (*matrices > 65535)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "too many matrices for one call (at most 65535)");
+  return SRS_OK;
+}
+
+extern "C" int64_t srs_muon_workspace(const srs_muon_class* classes, int n_classes) {
+  clear_error();
+  int64_t matrices = 0, at = 0;
+  if (check_classes(classes, n_classes, &matrices) != SRS_OK) return -1;
+  if (n_classes == 0) return 0;
+  lay_out_head(matrices, &at);
+  for (int i = 0; i < n_classes; ++i) lay_out(classes[i].count, classes[i].m, classes[i].n, &at);
+  return at;
+}
+
+extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes, int n_classes,
                               int u_format, int u_rule, const srs_muon_hparams* hp,
                               const srs_newton* h, const srs_rng* rng, void* workspace,
                               int64_t workspace_bytes, void* stream) {
@@ -400,38 +688,52 @@ extern "C" int srs_muon_multi(const srs_row* rows, int64_t n_rows, int64_t m, in
     return fail(SRS_ERR_INVALID_ARGUMENT, "null hyperparameter or rng pointer");
   if (rng->key_mode != SRS_KEY_DERIVE && rng->key_mode != SRS_KEY_GIVEN)
     return fail(SRS_ERR_INVALID_ARGUMENT, "unknown key_mode %d", rng->key_mode);
-  if (int rc = check_newton(n_rows, m, n, h)) return rc;
-  if (n_rows == 0 || m == 0 || n == 0) return SRS_OK;
+  if (int rc = check_newton(h)) return rc;
+  int64_t matrices = 0;
+  if (int rc = check_classes(classes, n_classes, &matrices)) return rc;
+  if (matrices == 0) return SRS_OK;
   if (rows == nullptr || reinterpret_cast<uintptr_t>(rows) % 16 != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "row table must be 16-byte aligned");
-  const NewtonSpace w = newton_space(n_rows, m, n);
-  if (int rc = check_space(workspace, workspace_bytes, w.bytes)) return rc;
+  if (int rc = check_space(workspace, workspace_bytes, srs_muon_workspace(classes, n_classes)))
+    return rc;
   if (int rc = check_device()) return rc;
-  NewtonSource s{};
-  s.rows = rows;
-  s.rng = *rng;
-  s.momentum = hp->momentum;
-  s.nesterov = hp->nesterov;
-  s.u_rule = u_rule;
-  s.m = (int)m;
-  s.n = (int)n;
-  s.row_units = (uint32_t)((n + 7) / 8);
-  s.units = (uint32_t)(m * s.row_units);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* space = static_cast<char*>(workspace);
+  int64_t used = 0;
+  const int64_t partial = lay_out_head(matrices, &used);
+  NewtonPlan plan{};
+  plan.classes = n_classes;
+  plan.partial = reinterpret_cast<double*>(space + partial);
+  plan.counters = reinterpret_cast<unsigned int*>(space);
+  plan.eps = h->eps;
+  plan.rng = *rng;
+  plan.momentum = hp->momentum;
+  plan.nesterov = hp->nesterov;
+  plan.u_rule = u_rule;
+  NewtonWork work{};
+  work.classes = n_classes;
+  int64_t batch[kMaxClasses];
+  int first = 0, chunks = 1;
+  for (int i = 0; i < n_classes; ++i) {
+    const srs_muon_class& c = classes[i];
+    const NewtonShape shape = lay_out(c.count, c.m, c.n, &used);
+    NewtonSource& s = plan.source[i];
+    s.rows = rows + c.first;
+    fill_source(shape, space, first, matrices, &s);
+    if (s.chunks > chunks) chunks = s.chunks;
+    const NewtonResult result{nullptr, 0, s.rows, hp->decay, c.neg_step};
+    if (int rc = fill_class(shape, space, result, &work.shape[i])) return rc;
+    batch[i] = c.count;
+    first += (int)c.count;
+  }
   int rc = SRS_OK;
   switch (u_format) {
-    case SRS_FMT_F32: rc = prepare<SRS_FMT_F32>(s, n_rows, w, space, h->eps, st); break;
-    case SRS_FMT_BF16: rc = prepare<SRS_FMT_BF16>(s, n_rows, w, space, h->eps, st); break;
-    case SRS_FMT_F16: rc = prepare<SRS_FMT_F16>(s, n_rows, w, space, h->eps, st); break;
-    case SRS_FMT_E4M3: rc = prepare<SRS_FMT_E4M3>(s, n_rows, w, space, h->eps, st); break;
-    default: rc = prepare<SRS_FMT_E5M2>(s, n_rows, w, space, h->eps, st); break;
+    case SRS_FMT_F32: rc = launch_prepare<SRS_FMT_F32>(plan, matrices, chunks, st); break;
+    case SRS_FMT_BF16: rc = launch_prepare<SRS_FMT_BF16>(plan, matrices, chunks, st); break;
+    case SRS_FMT_F16: rc = launch_prepare<SRS_FMT_F16>(plan, matrices, chunks, st); break;
+    case SRS_FMT_E4M3: rc = launch_prepare<SRS_FMT_E4M3>(plan, matrices, chunks, st); break;
+    default: rc = launch_prepare<SRS_FMT_E5M2>(plan, matrices, chunks, st); break;
   }
   if (rc != SRS_OK) return rc;
-  NewtonResult r{};
-  r.epilogue = kEpilogueMuon;
-  r.rows = rows;
-  r.decay = hp->decay;
-  r.step = hp->neg_step;
-  return newton_steps(n_rows, m, n, h, w, space, r, st);
+  return run_newton(work, batch, h, plan.counters, st);
 }

@@ -1,8 +1,9 @@
-// Instantiations and launches of the tensor-core products.
+// Launches of the tensor-core products, and the products of FP8 blocks.
 #include <mutex>
 #include <unordered_map>
 
 #include "srs_host.h"
+#include "srs_launch.h"
 #include "srs_product.cuh"
 #include "srs_thin.cuh"
 
@@ -14,9 +15,20 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+constexpr int kMaxDevices = 128;
 std::mutex g_lock;
 EncodeTiled g_encode = nullptr;
-std::unordered_map<const void*, int> g_clusters[128];  // resident CTA groups per device
+std::unordered_map<const void*, int> g_resident[kMaxDevices];
+unsigned int* g_status[kMaxDevices];
+
+__device__ unsigned int g_product_status;  // where a bounded wait ran out (0: nowhere)
+
+int device_index(int* dev) {
+  const cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (*dev < 0 || *dev >= kMaxDevices) return fail(SRS_ERR_UNSUPPORTED_DEVICE, "device %d", *dev);
+  return SRS_OK;
+}
 
 int find_encode(EncodeTiled* out) {
   std::lock_guard<std::mutex> lock(g_lock);
@@ -34,21 +46,22 @@ int find_encode(EncodeTiled* out) {
   return SRS_OK;
 }
 
-// Tensor map of one operand: boxes of 128 rows x 128 bytes of k, or of 64 rows
-// x 64 k when the row index is contiguous; outside elements read as zero.
-int encode_operand(const ProductOperand& o, int kind, int64_t batch, CUtensorMap* map,
-                   uint32_t rows = 128) {
+}  // namespace
+
+int encode_operand(const ProductOperand& o, int element_bytes, int64_t batch, int box_rows,
+                   CUtensorMap* map) {
   EncodeTiled encode = nullptr;
   if (int rc = find_encode(&encode)) return rc;
-  const uint64_t size = kind == kOperandF8 ? 1 : 2;
+  const uint64_t size = (uint64_t)element_bytes;
   const cuuint64_t dims[3] = {(cuuint64_t)(o.rows_inner ? o.rows : o.k),
                               (cuuint64_t)(o.rows_inner ? o.k : o.rows), (cuuint64_t)batch};
   const uint64_t entry = batch > 1 ? (uint64_t)o.batch_stride : (uint64_t)o.pitch * dims[1];
   const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * size, entry * size};
-  const cuuint32_t box[3] = {(cuuint32_t)(kSliceBytes / size), o.rows_inner ? 64u : rows, 1u};
+  const cuuint32_t box[3] = {(cuuint32_t)(kSliceBytes / size),
+                             o.rows_inner ? 64u : (cuuint32_t)box_rows, 1u};
   const cuuint32_t ones[3] = {1, 1, 1};
   const CUresult r = encode(
-      map, kind == kOperandF8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
       const_cast<void*>(o.base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -59,192 +72,244 @@ int encode_operand(const ProductOperand& o, int kind, int64_t batch, CUtensorMap
   return SRS_OK;
 }
 
-__device__ unsigned int g_product_status;  // where a bounded wait ran out (0: nowhere)
-
 int status_word(unsigned int** word) {
-  void* p = nullptr;
-  const cudaError_t e = cudaGetSymbolAddress(&p, g_product_status);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(product status)");
-  *word = static_cast<unsigned int*>(p);
+  int dev = 0;
+  if (int rc = device_index(&dev)) return rc;
+  std::lock_guard<std::mutex> lock(g_lock);
+  if (g_status[dev] == nullptr) {
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_product_status);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(product status)");
+    g_status[dev] = static_cast<unsigned int*>(p);
+  }
+  *word = g_status[dev];
   return SRS_OK;
 }
 
-template <int KIND, int CG, int EPILOGUE>
-int launch(const CUtensorMap& map_a, const CUtensorMap& map_b, const ProductArgs& args,
-           cudaStream_t stream) {
-  using S = ProductShape<KIND, CG>;
-  const auto kernel = &product_kernel<KIND, CG, EPILOGUE>;
+int prepare_kernel(const void* kernel, int group, int threads, int smem, int* resident) {
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute cluster{};
-  config.blockDim = dim3(kProductThreads);
-  config.dynamicSmemBytes = S::kSmem;
-  config.stream = stream;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = CG;
-  cluster.val.clusterDim.y = 1;
-  cluster.val.clusterDim.z = 1;
-  if (CG == 2) {
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-  }
-  int groups = 0;
+  if (int rc = device_index(&dev)) return rc;
+  const int sms = sm_count();
   {
     std::lock_guard<std::mutex> lock(g_lock);
-    const auto it = g_clusters[dev].find(reinterpret_cast<const void*>(kernel));
-    if (it != g_clusters[dev].end()) groups = it->second;
-  }
-  if (groups == 0) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return cuda_fail(e, "product shared memory");
-    if (CG == 2) {
-      config.gridDim = dim3((unsigned)(sm_count() / CG * CG));
-      e = cudaOccupancyMaxActiveClusters(&groups, kernel, &config);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
-      if (groups < 1) return fail(SRS_ERR_CUDA, "the product kernel's CTA pairs do not fit");
-      if (groups > sm_count() / CG) groups = sm_count() / CG;
-    } else {
-      groups = sm_count();
+    const auto it = g_resident[dev].find(kernel);
+    if (it != g_resident[dev].end()) {
+      *resident = it->second;
+      return SRS_OK;
     }
-    std::lock_guard<std::mutex> lock(g_lock);
-    g_clusters[dev][reinterpret_cast<const void*>(kernel)] = groups;
   }
-  const int64_t used = args.n_tiles < groups ? args.n_tiles : groups;
-  config.gridDim = dim3((unsigned)(used * CG));
-  e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, args);
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "product launch");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_fail(e, "kernel shared memory");
+  int groups = 0;
+  if (group > 1) {
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)group;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.gridDim = dim3((unsigned)(sms / group * group));
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&groups, kernel, &config);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+    if (groups > sms / group) groups = sms / group;
+  } else {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&groups, kernel, threads, (size_t)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+    groups *= sms;
+    if (groups > sms) groups = sms;
+  }
+  if (groups < 1) return fail(SRS_ERR_CUDA, "the product kernel does not fit the device");
+  std::lock_guard<std::mutex> lock(g_lock);
+  g_resident[dev][kernel] = groups;
+  *resident = groups;
+  return SRS_OK;
 }
 
-template <int KIND, int CG>
-int launch_epilogue(int epilogue, const CUtensorMap& map_a, const CUtensorMap& map_b,
-                    const ProductArgs& args, cudaStream_t stream) {
-  if constexpr (KIND == kOperandF16) {
-    if (epilogue == kEpilogueSymmetric)
-      return launch<KIND, CG, kEpilogueSymmetric>(map_a, map_b, args, stream);
-    if (epilogue == kEpilogueMuon)
-      return launch<KIND, CG, kEpilogueMuon>(map_a, map_b, args, stream);
+int launch_groups(const void* kernel, int64_t groups, int group, int threads, int smem,
+                  bool cooperative, void* argument, cudaStream_t stream, const char* what) {
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attributes[2]{};
+  config.gridDim = dim3((unsigned)(groups * group));
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = (size_t)smem;
+  config.stream = stream;
+  config.attrs = attributes;
+  if (group > 1) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = (unsigned)group;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
   }
-  return launch<KIND, CG, kEpilogueStore>(map_a, map_b, args, stream);
+  if (cooperative) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeCooperative;
+    a.val.cooperative = 1;
+  }
+  void* arguments[1] = {argument};
+  const cudaError_t e = cudaLaunchKernelExC(&config, kernel, arguments);
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, what);
 }
 
-int64_t tiles_for(int64_t m, int64_t n, int64_t edge, bool symmetric) {
-  const int64_t tm = (m + edge - 1) / edge, tn = (n + edge - 1) / edge;
-  return symmetric ? tm * (tm + 1) / 2 : tm * tn;
+namespace {
+
+// One product of FP8 blocks: a single list of tiles.
+struct BlockProduct {
+  CUtensorMap map_a, map_b;
+  int m, n, slices;
+  uint32_t tiles_m, tiles_n, instruction_formats;
+  const uint8_t* scale_a;
+  const uint8_t* scale_b;
+  int64_t scale_a_pitch, scale_b_pitch;
+  int scale_a_shift, scale_b_shift;  // 7 when one scale covers 128 rows
+  char* out;
+  int format;
+  unsigned int* status_at;
+  int edge;  // of a tile
+};
+
+struct BlockScales {
+  const uint8_t* a;
+  const uint8_t* b;
+  int64_t a_pitch, b_pitch;
+  int a_shift, b_shift, m, n;
+  bool a_words, b_words;
+};
+
+struct BlockSource {
+  const BlockProduct& w;
+  __device__ int phases() const { return 1; }
+  __device__ uint32_t tiles(int) const { return w.tiles_m * w.tiles_n; }
+  __device__ uint32_t formats() const { return w.instruction_formats; }
+  __device__ unsigned int* counter(int) const { return nullptr; }
+  __device__ unsigned int* status() const { return w.status_at; }
+  __device__ TileLoad load(int, uint32_t t) const {
+    int row, col;
+    banded_tile(t, w.tiles_m, w.tiles_n, &row, &col);
+    return {&w.map_a, &w.map_b, row * w.edge, col * w.edge, 0, w.slices, false, false};
+  }
+  __device__ TileStore store(int, uint32_t t) const {
+    int row, col;
+    banded_tile(t, w.tiles_m, w.tiles_n, &row, &col);
+    TileStore s{};
+    s.row0 = row * w.edge;
+    s.col0 = col * w.edge;
+    s.m = w.m;
+    s.n = w.n;
+    s.factor = 1.0f;
+    s.out = w.out;
+    s.format = w.format;
+    s.pitch = w.n;
+    return s;
+  }
+  __device__ BlockScales scales() const {
+    return {w.scale_a,       w.scale_b,       w.scale_a_pitch, w.scale_b_pitch,
+            w.scale_a_shift, w.scale_b_shift, w.m,             w.n,
+            scale_words(w.scale_a, w.scale_a_pitch, 0),
+            scale_words(w.scale_b, w.scale_b_pitch, 0)};
+  }
+};
+
+template <int CG>
+__global__ void __launch_bounds__(kProductThreads, 1)
+block_product_kernel(const __grid_constant__ BlockProduct w) {
+  run_products<kOperandF8, CG, false>(BlockSource{w});
+}
+
+template <int CG>
+int launch_blocks(BlockProduct& w, cudaStream_t stream) {
+  const void* kernel = reinterpret_cast<const void*>(&block_product_kernel<CG>);
+  constexpr int kSmem = ProductShape<kOperandF8, CG>::kSmem;
+  int resident = 0;
+  if (int rc = prepare_kernel(kernel, CG, kProductThreads, kSmem, &resident)) return rc;
+  const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n;
+  return launch_groups(kernel, tiles < resident ? tiles : resident, CG, kProductThreads, kSmem,
+                       false, &w, stream, "block product launch");
+}
+
+int operand_map(const srs_blocks& b, int64_t k, int box_rows, CUtensorMap* map) {
+  const ProductOperand o{reinterpret_cast<const void*>(b.data), b.rows, k, b.pitch, 0, false};
+  return encode_operand(o, 1, 1, box_rows, map);
+}
+
+uint32_t format_bits(const srs_blocks& a, const srs_blocks& b) {
+  return (a.format == SRS_FMT_E5M2 ? 1u : 0u) << 7 | (b.format == SRS_FMT_E5M2 ? 1u : 0u) << 10;
 }
 
 }  // namespace
 
-int launch_product(int kind, int epilogue, const ProductOperand& a, const ProductOperand& b,
-                   int64_t batch, int a_format, int b_format, ProductArgs args,
-                   cudaStream_t stream) {
-  const int sms = sm_count();
+int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d,
+                         int d_format, cudaStream_t stream) {
+  const auto tiles = [&](int64_t edge) {
+    return ((a.rows + edge - 1) / edge) * ((b.rows + edge - 1) / edge);
+  };
   // Time in units of one 128 x 128 tile on one SM: the 256 x 256 pair does two
   // such units per SM at a time; the single-CTA form loads twice the bytes per
   // unit, which makes its units about a fifth longer.
-  const bool symmetric = args.symmetric != 0;
-  const int64_t small = batch * tiles_for(a.rows, b.rows, 128, symmetric);
-  const int64_t large = batch * tiles_for(a.rows, b.rows, 256, symmetric);
-  const int64_t pairs = sms / 2;
-  const double time_small = 1.2 * (double)((small + sms - 1) / sms);
-  const double time_large = 2.0 * (double)((large + pairs - 1) / pairs);
+  const int64_t sms = sm_count(), pairs = sms / 2;
+  const double time_small = 1.2 * (double)((tiles(128) + sms - 1) / sms);
+  const double time_large = 2.0 * (double)((tiles(256) + pairs - 1) / pairs);
   const int cg = time_large <= time_small ? 2 : 1;
-  const int edge = 128 * cg;
-
-  CUtensorMap map_a, map_b;
-  if (int rc = encode_operand(a, kind, batch, &map_a)) return rc;
-  if (int rc = encode_operand(b, kind, batch, &map_b)) return rc;
-  if (int rc = status_word(&args.status)) return rc;
-  args.m = (int)a.rows;
-  args.n = (int)b.rows;
-  args.k = (int)a.k;
-  args.tiles_m = (int)((a.rows + edge - 1) / edge);
-  args.tiles_n = (int)((b.rows + edge - 1) / edge);
-  args.tiles_per_entry = cg == 2 ? large / batch : small / batch;
-  args.n_tiles = batch * args.tiles_per_entry;
-  args.a_rows_inner = a.rows_inner ? 1 : 0;
-  args.b_rows_inner = b.rows_inner ? 1 : 0;
-  // Instruction descriptor: operand formats, operand orders, N / 8, M / 16 and,
-  // for FP16, FP32 accumulation; for FP8, UE8M0 scales.
-  uint32_t idesc = (uint32_t)(edge >> 3) << 17 | (uint32_t)(edge >> 4) << 24;
-  if (kind == kOperandF16) {
-    idesc |= 1u << 4;
-    if (a.rows_inner) idesc |= 1u << 15;
-    if (b.rows_inner) idesc |= 1u << 16;
-  } else {
-    idesc |= (a_format == SRS_FMT_E5M2 ? 1u : 0u) << 7;
-    idesc |= (b_format == SRS_FMT_E5M2 ? 1u : 0u) << 10;
-    idesc |= 1u << 23;
-  }
-  args.idesc = idesc;
-  if (kind == kOperandF16)
-    return cg == 2 ? launch_epilogue<kOperandF16, 2>(epilogue, map_a, map_b, args, stream)
-                   : launch_epilogue<kOperandF16, 1>(epilogue, map_a, map_b, args, stream);
-  return cg == 2 ? launch_epilogue<kOperandF8, 2>(epilogue, map_a, map_b, args, stream)
-                 : launch_epilogue<kOperandF8, 1>(epilogue, map_a, map_b, args, stream);
+  if (tiles(128 * cg) >= (1ll << 31))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "a result of %lld x %lld is too large",
+                (long long)a.rows, (long long)b.rows);
+  BlockProduct w{};
+  if (int rc = operand_map(a, k, 128, &w.map_a)) return rc;
+  if (int rc = operand_map(b, k, 128, &w.map_b)) return rc;
+  if (int rc = status_word(&w.status_at)) return rc;
+  w.m = (int)a.rows;
+  w.n = (int)b.rows;
+  w.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
+  w.edge = 128 * cg;
+  w.tiles_m = (uint32_t)((a.rows + w.edge - 1) / w.edge);
+  w.tiles_n = (uint32_t)((b.rows + w.edge - 1) / w.edge);
+  w.instruction_formats = format_bits(a, b);
+  w.scale_a = reinterpret_cast<const uint8_t*>(a.scale);
+  w.scale_b = reinterpret_cast<const uint8_t*>(b.scale);
+  w.scale_a_pitch = a.scale_pitch;
+  w.scale_b_pitch = b.scale_pitch;
+  w.scale_a_shift = a.square ? 7 : 0;
+  w.scale_b_shift = b.square ? 7 : 0;
+  w.out = static_cast<char*>(d);
+  w.format = d_format;
+  return cg == 2 ? launch_blocks<2>(w, stream) : launch_blocks<1>(w, stream);
 }
 
 namespace {
 
 template <int BN>
-int launch_thin_as(const CUtensorMap& map_a, const CUtensorMap& map_b, const ThinArgs& args,
-                   int splits, cudaStream_t stream) {
+int launch_thin_as(ThinArgs& args, int splits, cudaStream_t stream) {
   using S = ThinShape<BN>;
-  const auto kernel = &thin_product_kernel<BN>;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  {
-    std::lock_guard<std::mutex> lock(g_lock);
-    int& set = g_clusters[dev][reinterpret_cast<const void*>(kernel)];
-    if (set == 0) {
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-      if (e != cudaSuccess) return cuda_fail(e, "thin product shared memory");
-      set = 1;
-    }
-  }
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = (unsigned)splits;
-  cluster.val.clusterDim.y = 1;
-  cluster.val.clusterDim.z = 1;
-  config.gridDim = dim3((unsigned)((args.m + 127) / 128 * splits));
-  config.blockDim = dim3(kProductThreads);
-  config.dynamicSmemBytes = S::kSmem;
-  config.stream = stream;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, args);
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "thin product launch");
+  const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN>);
+  int resident = 0;
+  if (int rc = prepare_kernel(kernel, 1, kThinThreads, S::kSmem, &resident)) return rc;
+  return launch_groups(kernel, (args.m + 127) / 128, splits, kThinThreads, S::kSmem, false, &args,
+                       stream, "thin product launch");
 }
 
 }  // namespace
 
-int launch_thin(const ProductOperand& a, const ProductOperand& b, int a_format, int b_format,
-                const ProductArgs& scales, void* out, int out_format, int64_t row_stride,
-                int64_t col_stride, cudaStream_t stream) {
+int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
+                int64_t row_stride, int64_t col_stride, cudaStream_t stream) {
   const int columns = b.rows <= 16 ? 16 : b.rows <= 32 ? 32 : 64;
-  CUtensorMap map_a, map_b;
-  if (int rc = encode_operand(a, kOperandF8, 1, &map_a)) return rc;
-  if (int rc = encode_operand(b, kOperandF8, 1, &map_b, (uint32_t)columns)) return rc;
   ThinArgs args{};
+  if (int rc = operand_map(a, k, 128, &args.map_a)) return rc;
+  if (int rc = operand_map(b, k, columns, &args.map_b)) return rc;
   if (int rc = status_word(&args.status)) return rc;
   args.m = (int)a.rows;
   args.n = (int)b.rows;
-  args.slices = (int)((a.k + kSliceBytes - 1) / kSliceBytes);
-  args.scale_a = scales.scale_a;
-  args.scale_b = scales.scale_b;
-  args.scale_a_pitch = scales.scale_a_pitch;
-  args.scale_b_pitch = scales.scale_b_pitch;
-  args.scale_a_shift = scales.scale_a_shift;
-  args.scale_b_shift = scales.scale_b_shift;
-  args.idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 |
-               (a_format == SRS_FMT_E5M2 ? 1u : 0u) << 7 |
-               (b_format == SRS_FMT_E5M2 ? 1u : 0u) << 10 | 1u << 23;
-  args.out = out;
-  args.out_format = out_format;
+  args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
+  args.scale_a = reinterpret_cast<const uint8_t*>(a.scale);
+  args.scale_b = reinterpret_cast<const uint8_t*>(b.scale);
+  args.scale_a_pitch = a.scale_pitch;
+  args.scale_b_pitch = b.scale_pitch;
+  args.scale_a_shift = a.square ? 7 : 0;
+  args.scale_b_shift = b.square ? 7 : 0;
+  args.idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 | format_bits(a, b) | 1u << 23;
+  args.out = d;
+  args.out_format = d_format;
   args.row_stride = row_stride;
   args.col_stride = col_stride;
   // Split k while all CTAs still fit at two an SM and each keeps two slices.
@@ -252,14 +317,9 @@ int launch_thin(const ProductOperand& a, const ProductOperand& b, int a_format, 
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 2ll * sm_count() && args.slices >= 4 * splits)
     splits *= 2;
-  if (columns == 16) return launch_thin_as<16>(map_a, map_b, args, splits, stream);
-  if (columns == 32) return launch_thin_as<32>(map_a, map_b, args, splits, stream);
-  return launch_thin_as<64>(map_a, map_b, args, splits, stream);
-}
-
-int read_product_status(unsigned int* out) {
-  const cudaError_t e = cudaMemcpyFromSymbol(out, g_product_status, sizeof(*out));
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "product status");
+  if (columns == 16) return launch_thin_as<16>(args, splits, stream);
+  if (columns == 32) return launch_thin_as<32>(args, splits, stream);
+  return launch_thin_as<64>(args, splits, stream);
 }
 
 }  // namespace srs
@@ -269,5 +329,6 @@ extern "C" int srs_product_status(uint32_t* status) {
   clear_error();
   if (status == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null status");
   if (int rc = check_device()) return rc;
-  return read_product_status(status);
+  const cudaError_t e = cudaMemcpyFromSymbol(status, g_product_status, sizeof(*status));
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "product status");
 }

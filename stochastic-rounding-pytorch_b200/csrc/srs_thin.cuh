@@ -16,7 +16,10 @@
 
 namespace srs {
 
+constexpr int kThinThreads = 256;
+
 struct ThinArgs {
+  CUtensorMap map_a, map_b;
   int m, n;             // rows of A and of B
   int slices;           // of 128 along k
   const uint8_t* scale_a;
@@ -65,10 +68,8 @@ __device__ __forceinline__ void store_value(void* out, int format, int64_t at, f
 }
 
 template <int BN>
-__global__ void __launch_bounds__(kProductThreads, 2)
-thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
-                    const __grid_constant__ CUtensorMap map_b,
-                    const __grid_constant__ ThinArgs a) {
+__global__ void __launch_bounds__(kThinThreads, 2)
+thin_product_kernel(const __grid_constant__ ThinArgs a) {
   using S = ThinShape<BN>;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2 * S::kStages + 1 + 2 * kScaleSlots];
@@ -121,8 +122,8 @@ thin_product_kernel(const __grid_constant__ CUtensorMap map_a,
       const uint32_t pa = stage0 + s * S::kStageBytes;
       if (leader) {
         barrier_expect(full(s), S::kStageBytes);
-        load_box<1>(pa, &map_a, i * kSliceBytes, row0, 0, full(s));
-        load_box<1>(pa + kPanelBytes, &map_b, i * kSliceBytes, 0, 0, full(s));
+        load_box<1>(pa, &a.map_a, i * kSliceBytes, row0, 0, full(s));
+        load_box<1>(pa + kPanelBytes, &a.map_b, i * kSliceBytes, 0, 0, full(s));
       }
       __syncwarp();
       if (++s == S::kStages) {

@@ -73,8 +73,14 @@ class SrsNewton(ctypes.Structure):
 
 
 class SrsMuonHparams(ctypes.Structure):
-    _fields_ = [("momentum", ctypes.c_float), ("neg_step", ctypes.c_float),
-                ("decay", ctypes.c_float), ("nesterov", ctypes.c_int32)]
+    _fields_ = [("momentum", ctypes.c_float), ("decay", ctypes.c_float),
+                ("nesterov", ctypes.c_int32)]
+
+
+class SrsMuonClass(ctypes.Structure):
+    _fields_ = [("first", ctypes.c_int64), ("count", ctypes.c_int64), ("m", ctypes.c_int64),
+                ("n", ctypes.c_int64), ("neg_step", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
 
 
 class SrsBlocks(ctypes.Structure):
@@ -85,6 +91,7 @@ class SrsBlocks(ctypes.Structure):
 
 
 NEWTON_MAX_STEPS = 32
+MUON_MAX_CLASSES = 16
 MAX_PEERS = 7
 IPC_HANDLE_BYTES = 64
 
@@ -150,7 +157,8 @@ _SIGNATURES = {
     "srs_orthogonalize": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int,
                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                            ctypes.POINTER(SrsNewton), _P, ctypes.c_int64, _P], ctypes.c_int),
-    "srs_muon_multi": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+    "srs_muon_workspace": ([ctypes.POINTER(SrsMuonClass), ctypes.c_int], ctypes.c_int64),
+    "srs_muon_multi": ([_P, ctypes.POINTER(SrsMuonClass), ctypes.c_int, ctypes.c_int,
                         ctypes.c_int, ctypes.POINTER(SrsMuonHparams), ctypes.POINTER(SrsNewton),
                         ctypes.POINTER(SrsRng), _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_quantize_blocks": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
@@ -328,11 +336,15 @@ class NativeLauncher:
             x_ptr, x_fmt, row_pitch, batch_stride, y_ptr, y_fmt, batch, m, n,
             ctypes.byref(newton), workspace.data_ptr(), workspace.numel(), stream))
 
-    def muon_multi(self, rows_ptr, n_rows, m, n, u_fmt, u_rule, hp, newton, rng, workspace,
-                   stream):
+    def muon_workspace(self, classes) -> int:
+        """Workspace bytes of a muon_multi call over ``classes`` (an array of SrsMuonClass)."""
+        return int(load_library().srs_muon_workspace(classes, len(classes)))
+
+    def muon_multi(self, rows_ptr, classes, u_fmt, u_rule, hp, newton, rng, workspace, stream):
         _check(load_library().srs_muon_multi(
-            rows_ptr, n_rows, m, n, u_fmt, u_rule, ctypes.byref(hp), ctypes.byref(newton),
-            ctypes.byref(rng), workspace.data_ptr(), workspace.numel(), stream))
+            rows_ptr, classes, len(classes), u_fmt, u_rule, ctypes.byref(hp),
+            ctypes.byref(newton), ctypes.byref(rng), workspace.data_ptr(), workspace.numel(),
+            stream))
 
     def quantize_blocks(self, x_ptr, x_fmt, rows, cols, x_pitch, fmt, rule, square, seed, offset,
                         data, data_pitch, scale, scale_pitch, data_t, data_t_pitch, scale_t,

@@ -93,44 +93,59 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
 
 
 def _shape_classes(updates):
-    """[(m, n, [index, ...])] of the updates, by shape, in order of first appearance."""
+    """[(m, n, [index, ...])] of the updates, by shape, those with the longest sums first
+    (they set the length of a phase, so the others fill in behind them)."""
     classes = {}
     for i, u in enumerate(updates):
         m = u.tensors[0].shape[0]
         classes.setdefault((m, u.numel // m), []).append(i)
-    return [(m, n, members) for (m, n), members in classes.items()]
+    return sorted(((m, n, members) for (m, n), members in classes.items()),
+                  key=lambda c: -max(c[0], c[1]))
+
+
+def _calls(classes, launcher):
+    """The classes as calls of at most MUON_MAX_CLASSES shapes whose workspace stays within
+    _WORKSPACE_BYTES (one matrix is always taken): [[(first, count, m, n), ...], ...]."""
+    calls, current, room, first = [], [], _WORKSPACE_BYTES, 0
+    for m, n, members in classes:
+        size, done = launcher.newton_workspace(1, m, n), 0
+        while done < len(members):
+            fits = min(len(members) - done, room // size)
+            if (fits < 1 and current) or len(current) == _native.MUON_MAX_CLASSES:
+                calls.append(current)
+                current, room = [], _WORKSPACE_BYTES
+                continue
+            fits = max(1, fits)
+            current.append((first, fits, m, n))
+            room -= fits * size
+            first, done = first + fits, done + fits
+    return calls + [current] if current else calls
 
 
 def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, newton, rng):
-    """Enqueue the step of ``updates`` (matrices of one device) on its current stream:
-    one sequence of launches for all matrices of a shape."""
+    """Enqueue the step of ``updates`` (matrices of one device) on its current stream."""
     device = updates[0].tensors[0].device
     launcher = _native.launcher()
     fmt, rule = codes
     classes = _shape_classes(updates)
     ordered = [updates[i] for _, _, members in classes for i in members]
     host = build_table(ordered, [0] * len(ordered), launcher.tile_elems())
+    hp = _native.SrsMuonHparams()
+    hp.momentum, hp.decay = np.float32(momentum), np.float32(1.0 - lr * weight_decay)
+    hp.nesterov = int(nesterov)
+    calls = []
+    for call in _calls(classes, launcher):
+        table = (_native.SrsMuonClass * len(call))()
+        for entry, (first, count, m, n) in zip(table, call):
+            entry.first, entry.count, entry.m, entry.n = first, count, m, n
+            entry.neg_step = np.float32(-(lr * update_scale(scale, m, n)))
+        calls.append((table, launcher.muon_workspace(table)))
     with device_guard(device):
-        table = upload(host, device)
+        rows = upload(host, device)
         stream = stream_handle(device)
-        sizes = [launcher.newton_workspace(1, m, n) for m, n, _ in classes]
-        counts = [max(1, min(len(members), _WORKSPACE_BYTES // size))
-                  for size, (_, _, members) in zip(sizes, classes)]
-        space = torch.empty(max(launcher.newton_workspace(c, m, n)
-                                for c, (m, n, _) in zip(counts, classes)),
-                            dtype=torch.uint8, device=device)
-        first = 0
-        for count, (m, n, members) in zip(counts, classes):
-            hp = _native.SrsMuonHparams()
-            hp.momentum = np.float32(momentum)
-            hp.neg_step = np.float32(-(lr * update_scale(scale, m, n)))
-            hp.decay = np.float32(1.0 - lr * weight_decay)
-            hp.nesterov = int(nesterov)
-            for lo in range(0, len(members), count):
-                now = min(count, len(members) - lo)
-                launcher.muon_multi(table.data_ptr() + (first + lo) * host.itemsize, now, m, n,
-                                    fmt, rule, hp, newton, rng, space, stream)
-            first += len(members)
+        space = torch.empty(max(size for _, size in calls), dtype=torch.uint8, device=device)
+        for table, _ in calls:
+            launcher.muon_multi(rows.data_ptr(), table, fmt, rule, hp, newton, rng, space, stream)
 
 
 def check_muon(lr, momentum, weight_decay, scale) -> None:

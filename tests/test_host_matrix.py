@@ -70,13 +70,24 @@ def test_entry_points_check_before_any_cuda_call():
     assert orth(w=1025) == bad
     assert orth(m=0) == _native.SRS_OK and orth(b=0) == _native.SRS_OK
     hp, rng = _native.SrsMuonHparams(), _native.SrsRng()
+
+    def shapes(count=1, m=8, n=8, first=0):
+        table = (_native.SrsMuonClass * 1)()
+        table[0].first, table[0].count, table[0].m, table[0].n = first, count, m, n
+        return table
+
     muon = lambda **k: lib.srs_muon_multi(*{  # noqa: E731
-        "r": 256, "c": 1, "m": 8, "n": 8, "f": 1, "rule": 1, "hp": ctypes.byref(hp),
+        "r": 256, "c": shapes(), "k": 1, "f": 1, "rule": 1, "hp": ctypes.byref(hp),
         "h": ctypes.byref(h), "rng": ctypes.byref(rng), "w": 1024, "wb": 1 << 30, "s": None,
         **k}.values())
     assert muon(f=9) == bad and muon(rule=9) == bad and muon(hp=None) == bad
     assert muon(r=None) == bad and muon(r=8) == bad and muon(wb=0) == bad
-    assert muon(c=0) == _native.SRS_OK
+    assert muon(c=None) == bad and muon(k=17) == bad and muon(k=-1) == bad
+    for table in (shapes(count=0), shapes(m=0), shapes(n=-1), shapes(first=-1), shapes(m=1 << 25),
+                  shapes(count=70000)):
+        assert muon(c=table) == bad and lib.srs_muon_workspace(table, 1) == -1
+    assert lib.srs_muon_workspace(shapes(), 1) > 0 and lib.srs_muon_workspace(None, 0) == 0
+    assert muon(k=0) == _native.SRS_OK
     quant = lambda **k: lib.srs_quantize_blocks(*{  # noqa: E731
         "x": 256, "xf": 0, "rows": 4, "cols": 64, "xp": 64, "of": 3, "rule": 0, "sq": 0,
         "seed": 0, "off": 0, "d": 512, "dp": 64, "s": 1024, "sp": 1, "dt": None, "dtp": 0,
@@ -111,9 +122,10 @@ def test_structure_layouts(tmp_path):
 #include <stdio.h>
 #include "{HEADER}"
 int main(void) {{
-  printf("%zu %zu %zu %zu %zu %zu %d\\n", sizeof(srs_newton), offsetof(srs_newton, eps),
-         sizeof(srs_muon_hparams), offsetof(srs_muon_hparams, nesterov), sizeof(srs_blocks),
-         offsetof(srs_blocks, format), SRS_NEWTON_MAX_STEPS);
+  printf("%zu %zu %zu %zu %zu %zu %d %zu %zu %d\\n", sizeof(srs_newton),
+         offsetof(srs_newton, eps), sizeof(srs_muon_hparams), offsetof(srs_muon_hparams, nesterov),
+         sizeof(srs_blocks), offsetof(srs_blocks, format), SRS_NEWTON_MAX_STEPS,
+         sizeof(srs_muon_class), offsetof(srs_muon_class, neg_step), SRS_MUON_MAX_CLASSES);
   return 0;
 }}
 """)
@@ -124,4 +136,5 @@ int main(void) {{
     assert got == [ctypes.sizeof(_native.SrsNewton), _native.SrsNewton.eps.offset,
                    ctypes.sizeof(_native.SrsMuonHparams), _native.SrsMuonHparams.nesterov.offset,
                    ctypes.sizeof(_native.SrsBlocks), _native.SrsBlocks.format.offset,
-                   _native.NEWTON_MAX_STEPS]
+                   _native.NEWTON_MAX_STEPS, ctypes.sizeof(_native.SrsMuonClass),
+                   _native.SrsMuonClass.neg_step.offset, _native.MUON_MAX_CLASSES]
