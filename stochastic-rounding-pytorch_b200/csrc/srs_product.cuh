@@ -122,19 +122,26 @@ __device__ __forceinline__ void triangle_tile(uint32_t i, int* row, int* col) {
 
 // ---------------------------------------------------------------- epilogue --
 
-// Results leave in pieces of 32 rows x 128 bytes: a lane holds one row's piece (32
-// words), the warp turns it through shared memory (16-byte slots, slot index xor
-// row so that both sides are conflict-free), and 8 lanes then store one row's 128
-// bytes.  Rows that are not on 16-byte boundaries are stored by words, and 16-bit
-// results of odd pitch by elements.
+// Results leave in pieces of 32 rows x 32 columns: a lane holds one row's piece, the
+// warp turns it through shared memory (16-byte slots, xored so that both sides are
+// conflict-free), and the lanes then store whole rows, 64 bytes of 16-bit results or
+// 128 of FP32 ones.  Rows that are not on 16-byte boundaries are stored by words,
+// and 16-bit results of odd pitch by elements.  (Pieces and loops are small on
+// purpose: a phase of few tiles runs this code once, from a cold instruction cache.)
+//
+// SLOTS: 16-byte slots of a row, 4 (16-bit results) or 8 (FP32).
+template <int SLOTS>
 __device__ __forceinline__ uint32_t staged_slot(uint32_t base, int row, int slot) {
-  return base + row * 128 + 16 * (slot ^ (row & 7));
+  const int turn = SLOTS == 8 ? row & 7 : (row >> 1) & 3;
+  return base + row * 16 * SLOTS + 16 * (slot ^ turn);
 }
 
-__device__ __forceinline__ void stage_row(uint32_t base, int lane, const uint32_t (&w)[32]) {
+template <int SLOTS>
+__device__ __forceinline__ void stage_row(uint32_t base, int lane,
+                                          const uint32_t (&w)[4 * SLOTS]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_slot(base, lane, j)),
+  for (int j = 0; j < SLOTS; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_slot<SLOTS>(base, lane, j)),
                  "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                  : "memory");
 }
@@ -154,30 +161,36 @@ __device__ __forceinline__ uint32_t staged_read(uint32_t addr) {
   return v;
 }
 
-// Staged piece to rows of `size`-byte elements: `out` is the piece's first element,
-// `pitch` and `cols` count elements, `rows` <= 32.
-__device__ __forceinline__ void store_piece(uint32_t base, char* out, int size, int64_t pitch,
-                                            int rows, int cols, int lane) {
-  const uint64_t align = reinterpret_cast<uint64_t>(out) | (uint64_t)(pitch * size);
-  const int bytes = min(cols * size, 128);
-  const int64_t step = pitch * size;
+// Staged piece to rows of elements of SLOTS / 2 bytes: `out` is the piece's first
+// element, `pitch` and `cols` count elements, `rows` <= 32.
+template <int SLOTS>
+__device__ __forceinline__ void store_piece(uint32_t base, char* out, int64_t pitch, int rows,
+                                            int cols, int lane) {
+  constexpr int kSize = SLOTS / 2, kAtOnce = 32 / SLOTS;  // element bytes; rows a pass
+  const int64_t step = pitch * kSize;
+  const uint64_t align = reinterpret_cast<uint64_t>(out) | (uint64_t)step;
+  const int bytes = min(cols * kSize, 16 * SLOTS);
   if ((align & 15) == 0 && (bytes & 15) == 0) {
-    const int slot = lane & 7, row0 = lane >> 3;
+    const int slot = lane % SLOTS, row0 = lane / SLOTS;
     char* p = out + row0 * step + 16 * slot;
     if (16 * slot < bytes) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = 4 * i + row0;
-        const uint4 v = staged_read4(staged_slot(base, row, slot));
-        if (row < rows) *reinterpret_cast<uint4*>(p + 4 * i * step) = v;
+      for (int i = 0; i < SLOTS; ++i) {
+        const int row = kAtOnce * i + row0;
+        const uint4 v = staged_read4(staged_slot<SLOTS>(base, row, slot));
+        if (row < rows) *reinterpret_cast<uint4*>(p) = v;
+        p += kAtOnce * step;
       }
     }
   } else if ((align & 3) == 0) {
-    const bool whole = 4 * lane + 4 <= bytes, half = !whole && 4 * lane < bytes;
-    char* p = out + 4 * lane;
-#pragma unroll 8
-    for (int row = 0; row < rows; ++row, p += step) {
-      const uint32_t v = staged_read(staged_slot(base, row, lane >> 2) + 4 * (lane & 3));
+    // 4 * SLOTS words a row: a warp takes one row of 32 words, or two of 16
+    constexpr int kRows = SLOTS == 8 ? 1 : 2;
+    const int word = lane % (4 * SLOTS), row0 = lane / (4 * SLOTS);
+    const bool whole = 4 * word + 4 <= bytes, half = !whole && 4 * word < bytes;
+    char* p = out + row0 * step + 4 * word;
+#pragma unroll 4
+    for (int row = row0; row < rows; row += kRows, p += kRows * step) {
+      const uint32_t v = staged_read(staged_slot<SLOTS>(base, row, word >> 2) + 4 * (word & 3));
       if (whole) *reinterpret_cast<uint32_t*>(p) = v;
       else if (half) *reinterpret_cast<uint16_t*>(p) = (uint16_t)v;
     }
@@ -185,13 +198,9 @@ __device__ __forceinline__ void store_piece(uint32_t base, char* out, int size, 
     char* p = out + 2 * lane;
 #pragma unroll 4
     for (int row = 0; row < rows; ++row, p += step) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int e = lane + 32 * h;
-        const uint32_t v = staged_read(staged_slot(base, row, e >> 3) + 4 * ((e >> 1) & 3));
-        if (2 * e < bytes)
-          *reinterpret_cast<uint16_t*>(p + 64 * h) = (uint16_t)(v >> (16 * (e & 1)));
-      }
+      const uint32_t v =
+          staged_read(staged_slot<SLOTS>(base, row, lane >> 3) + 4 * ((lane >> 1) & 3));
+      if (2 * lane < bytes) *reinterpret_cast<uint16_t*>(p) = (uint16_t)(v >> (16 * (lane & 1)));
     }
   }
 }
@@ -236,7 +245,7 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int row = 4 * i + row0;
-      const uint4 d = staged_read4(staged_slot(base, row, slot));
+      const uint4 d = staged_read4(staged_slot<8>(base, row, slot));
       if (row >= rows) continue;
       char* q = p + 4 * i * pitch * kSize;
       const float a = next(__uint_as_float(old[i].x), d.x), b = next(__uint_as_float(old[i].y), d.y);
@@ -248,7 +257,7 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
     char* p = param + lane * kSize;
 #pragma unroll 8
     for (int row = 0; row < rows; ++row, p += pitch * kSize) {
-      const uint32_t d = staged_read(staged_slot(base, row, lane >> 2) + 4 * (lane & 3));
+      const uint32_t d = staged_read(staged_slot<8>(base, row, lane >> 2) + 4 * (lane & 3));
       if constexpr (BF16) {
         __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(p);
         *q = __float2bfloat16_rn(next(__bfloat162float(*q), d));
@@ -260,92 +269,84 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
   }
 }
 
-// This lane's row of the addend, 64 columns from col0 on (the pitch is a multiple of
+// This lane's row of the addend, 32 columns from col0 on (the pitch is a multiple of
 // 8).  Written by an earlier phase of the same kernel: never through the
 // non-coherent path.
 __device__ __forceinline__ void load_addend(const TileStore& t, int row, int col0,
-                                            uint4 (&add)[8]) {
+                                            uint4 (&add)[4]) {
   const __half* from = t.addend + (int64_t)row * t.pitch + col0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 4; ++j)
     add[j] = (row < t.m && col0 + 8 * j < t.pitch)
                  ? __ldcg(reinterpret_cast<const uint4*>(from) + j)
                  : make_uint4(0u, 0u, 0u, 0u);
 }
 
-// 64 accumulator columns from col0 on for a warp's 32 rows from row0 on: v[0][c] and
-// v[1][c] are columns c and 32 + c of row row0 + lane.  `add` holds the addend's
-// piece; the next piece's (next_col, -1: none) is requested before this one is stored.
+// 32 accumulator columns from col0 on for a warp's 32 rows from row0 on: v[c] is
+// column col0 + c of row row0 + lane.  `add` holds the addend's piece; the next piece's
+// (next_col, -1: none) is requested before this one is stored.
 template <bool NEWTON>
 __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int col0, int lane,
-                                              uint32_t staged, uint32_t (&v)[2][32],
-                                              uint4 (&add)[8], int next_col) {
+                                              uint32_t staged, uint32_t (&v)[32],
+                                              uint4 (&add)[4], int next_col) {
   const int row = row0 + lane, rows = min(32, t.m - row0);
   const int64_t at = (int64_t)row0 * t.pitch + col0;
-  const auto value = [&](int c) { return __uint_as_float(v[c >> 5][c & 31]) * t.factor; };
-  if (t.format != SRS_FMT_F32 && !(NEWTON && t.update != 0)) {
-    uint32_t w[32];
-    if (NEWTON && t.addend != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint4 q = add[i >> 2];
-        const uint32_t pair = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
-        const float2 g = f16x2_to_float2(pair);
+  for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * t.factor);
+  const auto value = [&](int c) { return __uint_as_float(v[c]); };
+  if (t.format != SRS_FMT_F32 && !(NEWTON && t.update != 0)) {
+    uint32_t w[16];
+    if (NEWTON && t.addend != nullptr) {
+      const uint32_t* pairs = reinterpret_cast<const uint32_t*>(add);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 g = f16x2_to_float2(pairs[i]);
         const int col = col0 + 2 * i;
         w[i] = pack_half(fmaf(t.beta, g.x, value(2 * i)) + (row == col ? t.diagonal : 0.0f),
                          fmaf(t.beta, g.y, value(2 * i + 1)) +
                              (row == col + 1 ? t.diagonal : 0.0f));
       }
       if (next_col >= 0) load_addend(t, row, next_col, add);
+    } else if (t.format == SRS_FMT_BF16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(value(2 * i), value(2 * i + 1));
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        w[i] = t.format == SRS_FMT_BF16 ? pack_bf16(value(2 * i), value(2 * i + 1))
-                                        : pack_half(value(2 * i), value(2 * i + 1));
+      for (int i = 0; i < 16; ++i) w[i] = pack_half(value(2 * i), value(2 * i + 1));
     }
     if (NEWTON && t.mirror) {
       // Lane pairs swap halves: the even lane gets two rows of an even column, the
       // odd lane of the next one, so a store covers 2 x 64 bytes.  (An odd last
       // row writes one padding element beside it.)
-      const bool odd = (lane & 1) != 0;
-      __half* to = reinterpret_cast<__half*>(t.out) + (int64_t)(col0 + (odd ? 1 : 0)) * t.pitch +
-                   (row & ~1);
+      const int odd = lane & 1;
+      __half* to = reinterpret_cast<__half*>(t.out) + (int64_t)(col0 + odd) * t.pitch + (row & ~1);
+      const int cols = (row & ~1) < t.m ? t.n - col0 - odd : 0;
 #pragma unroll
-      for (int i = 0; i < 32; ++i, to += 2 * t.pitch) {
+      for (int i = 0; i < 16; ++i, to += 2 * t.pitch) {
         const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, w[i], 1);
         const uint32_t pair =
             odd ? __byte_perm(other, w[i], 0x7632u) : __byte_perm(w[i], other, 0x5410u);
-        if ((row & ~1) < t.m && col0 + 2 * i + (odd ? 1 : 0) < t.n)
-          *reinterpret_cast<uint32_t*>(to) = pair;
+        if (2 * i < cols) *reinterpret_cast<uint32_t*>(to) = pair;
       }
     }
-    stage_row(staged, lane, w);
+    stage_row<4>(staged, lane, w);
     __syncwarp();
-    store_piece(staged, t.out + 2 * at, 2, t.pitch, rows, t.n - col0, lane);
-    __syncwarp();
+    store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
   } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int cols = t.n - col0 - 32 * h;
-      if (cols <= 0) break;
-      uint32_t w[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(value(32 * h + c));
-      stage_row(staged, lane, w);
-      __syncwarp();
-      const int64_t first = at + 32 * h;
-      if (NEWTON && t.update != 0) {
-        if (t.format == SRS_FMT_BF16)
-          update_piece<true>(staged, t.out + 2 * first, t.pitch, rows, cols, t.step, t.decay, lane);
-        else
-          update_piece<false>(staged, t.out + 4 * first, t.pitch, rows, cols, t.step, t.decay,
-                              lane);
-      } else {
-        store_piece(staged, t.out + 4 * first, 4, t.pitch, rows, cols, lane);
-      }
-      __syncwarp();
+    stage_row<8>(staged, lane, v);
+    __syncwarp();
+    if (NEWTON && t.update != 0) {
+      if (t.format == SRS_FMT_BF16)
+        update_piece<true>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, t.step, t.decay,
+                           lane);
+      else
+        update_piece<false>(staged, t.out + 4 * at, t.pitch, rows, t.n - col0, t.step, t.decay,
+                            lane);
+    } else {
+      store_piece<8>(staged, t.out + 4 * at, t.pitch, rows, t.n - col0, lane);
     }
   }
+  __syncwarp();
 }
 
 // ------------------------------------------------------------------ kernel --
@@ -437,15 +438,21 @@ __device__ __forceinline__ void run_products(const Source& src) {
     int s = 0;
     uint32_t parity = 0;
     for (int p = 0; p < phases && ok; ++p) {
+      const uint32_t tiles = src.tiles(p);
+      TileLoad at{};
+      if (first < tiles) {
+        at = src.load(p, first);
+        prefetch_map(at.map_a);
+        prefetch_map(at.map_b);
+      }
       if (p > 0) {
         // what the earlier phase wrote, seen by the copies that follow
         if (lane == 0) ok = counter_wait(src.counter(p - 1), gridDim.x, status, 1u << 16);
         ok = __all_sync(0xFFFFFFFFu, ok);
         asm volatile("fence.proxy.async;" ::: "memory");
       }
-      const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step) {
-        const TileLoad at = src.load(p, t);
+        if (t != first) at = src.load(p, t);
         const int ra = at.row0 + 128 * (int)rank, rb = at.col0 + 128 * (int)rank;
         for (int i = 0; i < at.slices; ++i) {
           ok = barrier_wait(empty(s), parity ^ 1u, status, 1u);
@@ -649,8 +656,8 @@ __device__ __forceinline__ void run_products(const Source& src) {
       }
     }
   } else if (warp < kWriters) {
-    // ---- results: this warp's 32 rows, its half of the tile's 64-column pieces
-    constexpr int kPieces = S::kTileCols / 128;
+    // ---- results: this warp's 32 rows, its half of the tile's 32-column pieces
+    constexpr int kPieces = S::kTileCols / 64;
     const int half = warp >> 2, quarter = warp & 3;
     const uint32_t staged = staged0 + warp * kPieceBytes;
     int count = 0;
@@ -661,7 +668,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         const TileStore at = src.store(p, t);
         const int acc = count & 1;
         const int row0 = at.row0 + 128 * (int)rank + 32 * quarter;
-        uint4 add[8];
+        uint4 add[4];
         if (NEWTON && at.addend != nullptr) {
           // the one thing these warps read of an earlier phase
           if (!met) {
@@ -671,7 +678,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
             if (!ok) break;
             met = true;
           }
-          load_addend(at, row0 + lane, at.col0 + 64 * half * kPieces, add);
+          load_addend(at, row0 + lane, at.col0 + 32 * half * kPieces, add);
         }
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u);
         ok = __all_sync(0xFFFFFFFFu, ok);
@@ -682,31 +689,26 @@ __device__ __forceinline__ void run_products(const Source& src) {
         for (int i = 0; i < kPieces; ++i) {
           // accumulator 0 gives its last (shared) columns first
           const int c = half * kPieces + ((S::kShared != 0 && acc == 0) ? kPieces - 1 - i : i);
-          uint32_t v[2][32];
-          tmem_load32(from + 64 * c, v[0]);
-          tmem_load32(from + 64 * c + 32, v[1]);
-          tmem_wait(v[0]);
-          tmem_wait(v[1]);
+          uint32_t v[32];
+          tmem_load32(from + 32 * c, v);
+          tmem_wait(v);
           if (i == (S::kShared != 0 ? 0 : kPieces - 1)) {
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) barrier_arrive(map_to_rank(acc_empty(acc), 0));
+            if (lane == 0) barrier_arrive_relaxed(map_to_rank(acc_empty(acc), 0));
           }
-          if (row0 < at.m && at.col0 + 64 * c < at.n)
-            write_columns<NEWTON>(at, row0, at.col0 + 64 * c, lane, staged, v, add,
-                                  i + 1 < kPieces ? at.col0 + 64 * (c + 1) : -1);
+          if (row0 < at.m && at.col0 + 32 * c < at.n)
+            write_columns<NEWTON>(at, row0, at.col0 + 32 * c, lane, staged, v, add,
+                                  i + 1 < kPieces ? at.col0 + 32 * (c + 1) : -1);
         }
       }
       if (NEWTON && p + 1 < phases && ok) {
-        // This CTA's results of the phase, for the copies of every other CTA; the last
-        // of its warps reports.
-        asm volatile("fence.proxy.async;" ::: "memory");
-        __threadfence();
+        // This CTA's results of the phase: each warp's stores, passed on inside the CTA,
+        // then released to the grid by the last warp.  (The reading side orders them
+        // before its copies.)
         __syncwarp();
-        if (lane == 0 && atomicAdd(&phase_warps[p], 1u) == kWriters - 1u) {
-          __threadfence();
+        if (lane == 0 && shared_count(&phase_warps[p]) == kWriters - 1u)
           counter_arrive(src.counter(p));
-        }
       }
     }
   }

@@ -69,6 +69,13 @@ __device__ __forceinline__ void barrier_arrive(uint32_t cluster_bar) {
                : "memory");
 }
 
+// The same without ordering this thread's stores before it, which would wait for them:
+// for giving back an accumulator, whose loads are complete and fenced.
+__device__ __forceinline__ void barrier_arrive_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -94,6 +101,10 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsi
     }
   }
   return true;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 template <int CG>
@@ -268,6 +279,17 @@ __device__ __forceinline__ bool counter_wait(const unsigned int* counter, unsign
       return false;
     }
   }
+}
+
+// Adds one to a counter in shared memory, ordered after and before the CTA's accesses
+// (the count before it is returned).
+__device__ __forceinline__ unsigned int shared_count(unsigned int* counter) {
+  unsigned int before;
+  asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;"
+               : "=r"(before)
+               : "r"(smem_address(counter))
+               : "memory");
+  return before;
 }
 
 __device__ __forceinline__ void counter_arrive(unsigned int* counter) {
