@@ -231,7 +231,9 @@ struct NewtonClass {
   CUtensorMap g, p;
   int m, n, small, tall;
   int long_slices, small_slices;
-  uint32_t triangle, grid_m, grid_n;  // tiles of G and P; of X
+  TileGrid grid;          // tiles of X
+  Divider each_triangle;  // tiles of one G or P
+  Divider each_grid;      // tiles of one X
   int64_t ld, x_elems, small_ld, small_elems;
   __half* x[2];
   __half* g_at;
@@ -274,10 +276,11 @@ struct NewtonProducts {
     while (t >= begin[r.shape + 1]) ++r.shape;
     t -= begin[r.shape];
     const NewtonClass& s = w.shape[r.shape];
-    const uint32_t each = grid ? s.grid_m * s.grid_n : s.triangle;
-    r.batch = (int)(t / each);
-    t -= (uint32_t)r.batch * each;
-    if (grid) banded_tile(t, s.grid_m, s.grid_n, &r.row, &r.col);
+    const Divider& each = grid ? s.each_grid : s.each_triangle;
+    const uint32_t batch = each.quotient(t);
+    r.batch = (int)batch;
+    t -= batch * each.d;
+    if (grid) s.grid.at(t, &r.row, &r.col);
     else triangle_tile(t, &r.row, &r.col);
     r.row *= w.edge;
     r.col *= w.edge;
@@ -377,6 +380,11 @@ struct NewtonShape {
   int64_t rho, x[2], g, p;  // byte offsets
 };
 
+// Rows on 128-byte boundaries, so that a box's 128-byte rows are whole cache lines
+// (3000 x 3000 with a pitch of 3000: 754 us, of 3008: 574 us); narrow matrices only need
+// the 16 bytes of a copy.
+int64_t row_pitch_of(int64_t n) { return round_up(n, n >= 64 ? 64 : 8); }
+
 int64_t take(int64_t* at, int64_t bytes) {
   const int64_t here = *at;
   *at += round_up(bytes, 256);
@@ -389,8 +397,8 @@ NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, int64_t* at) {
   s.m = m;
   s.n = n;
   s.small = m < n ? m : n;
-  s.ld = round_up(n, 8);
-  s.small_ld = round_up(s.small, 8);
+  s.ld = row_pitch_of(n);
+  s.small_ld = row_pitch_of(s.small);
   s.x_elems = m * s.ld;
   s.small_elems = s.small * s.small_ld;
   s.rho = take(at, batch * 4);
@@ -497,13 +505,14 @@ int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
   for (int i = 0; i < w.classes; ++i) {
     NewtonClass& c = w.shape[i];
     const uint32_t edge = (uint32_t)((c.small + w.edge - 1) / w.edge);
-    c.triangle = edge * (edge + 1) / 2;
-    c.grid_m = (uint32_t)((c.m + w.edge - 1) / w.edge);
-    c.grid_n = (uint32_t)((c.n + w.edge - 1) / w.edge);
+    c.each_triangle = make_divider(edge * (edge + 1) / 2);
+    c.grid = make_grid((uint32_t)((c.m + w.edge - 1) / w.edge),
+                       (uint32_t)((c.n + w.edge - 1) / w.edge));
+    c.each_grid = make_divider(c.grid.rows * c.grid.cols);
     w.triangles[i] = (uint32_t)triangles;
     w.grids[i] = (uint32_t)grids;
-    triangles += batch[i] * c.triangle;
-    grids += batch[i] * c.grid_m * c.grid_n;
+    triangles += batch[i] * c.each_triangle.d;
+    grids += batch[i] * c.each_grid.d;
   }
   w.triangles[w.classes] = (uint32_t)triangles;
   w.grids[w.classes] = (uint32_t)grids;
@@ -515,11 +524,13 @@ int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
 }
 
 // Rough time of the three products of a step with tiles of 128 * cg, in cycles of
-// one SM: 512 a slice for the pair, 300 for the single CTA (256 of MMA, but twice
-// the loads for it), and what a tile's results take.
+// one SM: 512 a slice for the pair, 350 for the single CTA (256 of MMA, but twice
+// the loads for it), and what a tile's results take.  Measured (us, single against
+// pair): 1024^2 144, 201; 2048^2 241, 285; 2500^2 422, 390; 3500^2 894, 783;
+// 16 x 768^2 295, 367; 24 x 768^2 402, 365; 4 x (1024 x 4096) 347, 381.
 double step_cycles(const NewtonWork& w, const int64_t* batch, int cg) {
   const int64_t groups = sm_count() / cg;
-  const double slice = cg == 2 ? 512.0 : 300.0, rest = cg == 2 ? 3000.0 : 1500.0;
+  const double slice = cg == 2 ? 512.0 : 350.0, rest = cg == 2 ? 5000.0 : 2000.0;
   double total = 0.0;
   for (int kind = 0; kind < 3; ++kind) {
     double work = 0.0, longest = 0.0;

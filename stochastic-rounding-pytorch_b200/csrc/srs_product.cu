@@ -159,7 +159,8 @@ namespace {
 struct BlockProduct {
   CUtensorMap map_a, map_b;
   int m, n, slices;
-  uint32_t tiles_m, tiles_n, instruction_formats;
+  TileGrid grid;
+  uint32_t instruction_formats;
   const uint8_t* scale_a;
   const uint8_t* scale_b;
   int64_t scale_a_pitch, scale_b_pitch;
@@ -181,18 +182,18 @@ struct BlockScales {
 struct BlockSource {
   const BlockProduct& w;
   __device__ int phases() const { return 1; }
-  __device__ uint32_t tiles(int) const { return w.tiles_m * w.tiles_n; }
+  __device__ uint32_t tiles(int) const { return w.grid.rows * w.grid.cols; }
   __device__ uint32_t formats() const { return w.instruction_formats; }
   __device__ unsigned int* counter(int) const { return nullptr; }
   __device__ unsigned int* status() const { return w.status_at; }
   __device__ TileLoad load(int, uint32_t t) const {
     int row, col;
-    banded_tile(t, w.tiles_m, w.tiles_n, &row, &col);
+    w.grid.at(t, &row, &col);
     return {&w.map_a, &w.map_b, row * w.edge, col * w.edge, 0, w.slices, false, false};
   }
   __device__ TileStore store(int, uint32_t t) const {
     int row, col;
-    banded_tile(t, w.tiles_m, w.tiles_n, &row, &col);
+    w.grid.at(t, &row, &col);
     TileStore s{};
     s.row0 = row * w.edge;
     s.col0 = col * w.edge;
@@ -224,7 +225,7 @@ int launch_blocks(BlockProduct& w, cudaStream_t stream) {
   constexpr int kSmem = ProductShape<kOperandF8, CG>::kSmem;
   int resident = 0;
   if (int rc = prepare_kernel(kernel, CG, kProductThreads, kSmem, &resident)) return rc;
-  const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n;
+  const int64_t tiles = (int64_t)w.grid.rows * w.grid.cols;
   return launch_groups(kernel, tiles < resident ? tiles : resident, CG, kProductThreads, kSmem,
                        false, &w, stream, "block product launch");
 }
@@ -245,12 +246,11 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
   const auto tiles = [&](int64_t edge) {
     return ((a.rows + edge - 1) / edge) * ((b.rows + edge - 1) / edge);
   };
-  // Time in units of one 128 x 128 tile on one SM: the 256 x 256 pair does two
-  // such units per SM at a time; the single-CTA form loads twice the bytes per
-  // unit, which makes its units about a fifth longer.
-  const int64_t sms = sm_count(), pairs = sms / 2;
-  const double time_small = 1.2 * (double)((tiles(128) + sms - 1) / sms);
-  const double time_large = 2.0 * (double)((tiles(256) + pairs - 1) / pairs);
+  // Rough times in cycles: 512 a slice for a 256 x 256 pair, 350 for a 128 x 128 tile
+  // (256 of MMA, but twice the loads for it), and what a tile's results take.
+  const int64_t sms = sm_count(), pairs = sms / 2, slices = (k + kSliceBytes - 1) / kSliceBytes;
+  const double time_small = (350.0 * slices + 2000.0) * (double)((tiles(128) + sms - 1) / sms);
+  const double time_large = (512.0 * slices + 5000.0) * (double)((tiles(256) + pairs - 1) / pairs);
   const int cg = time_large <= time_small ? 2 : 1;
   if (tiles(128 * cg) >= (1ll << 31))
     return fail(SRS_ERR_INVALID_ARGUMENT, "a result of %lld x %lld is too large",
@@ -263,8 +263,8 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
   w.n = (int)b.rows;
   w.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
   w.edge = 128 * cg;
-  w.tiles_m = (uint32_t)((a.rows + w.edge - 1) / w.edge);
-  w.tiles_n = (uint32_t)((b.rows + w.edge - 1) / w.edge);
+  w.grid = make_grid((uint32_t)((a.rows + w.edge - 1) / w.edge),
+                     (uint32_t)((b.rows + w.edge - 1) / w.edge));
   w.instruction_formats = format_bits(a, b);
   w.scale_a = reinterpret_cast<const uint8_t*>(a.scale);
   w.scale_b = reinterpret_cast<const uint8_t*>(b.scale);

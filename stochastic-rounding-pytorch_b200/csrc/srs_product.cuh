@@ -100,15 +100,49 @@ __device__ __forceinline__ bool scale_words(const uint8_t* scale, int64_t pitch,
   return ((reinterpret_cast<uint64_t>(scale) | (uint64_t)pitch | (uint64_t)kb) & 3) == 0;
 }
 
-// Tile i of tiles_m x tiles_n in bands of 8 tile rows, column by column within a band,
-// so that the CTAs running at one time share rows of A and B in L2.
-__device__ __forceinline__ void banded_tile(uint32_t i, uint32_t tiles_m, uint32_t tiles_n,
-                                            int* row, int* col) {
-  const uint32_t band = 8u * tiles_n;
-  const uint32_t first = i / band * 8u, j = i % band;
-  const uint32_t rows = min(8u, tiles_m - first);
-  *row = (int)(first + j % rows);
-  *col = (int)(j / rows);
+// Division of a 31-bit number by a number the host knows: with 2^(s-1) < d <= 2^s and
+// mul = floor(2^(31+s) / d) + 1, n / d = floor(n * mul / 2^(31+s)) for n < 2^31, as
+// the excess mul * d - 2^(31+s) is at most 2^s.
+struct Divider {
+  uint32_t d, mul;
+  int shift;  // s - 1; -1: d == 1
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return shift < 0 ? n : __umulhi(n, mul) >> shift;
+  }
+};
+
+inline Divider make_divider(uint32_t d) {
+  Divider r{d, 0u, -1};
+  if (d > 1) {
+    int s = 1;
+    while (s < 32 && (1ull << s) < d) ++s;
+    r.mul = (uint32_t)((1ull << (31 + s)) / d + 1);
+    r.shift = s - 1;
+  }
+  return r;
+}
+
+// Tiles of a matrix in bands of 8 tile rows, column by column within a band, so that
+// the CTAs running at one time share rows of A and B in L2.
+struct TileGrid {
+  uint32_t rows, cols;
+  Divider band;  // 8 * cols
+  Divider last;  // rows of the last band
+  __device__ __forceinline__ void at(uint32_t i, int* row, int* col) const {
+    const uint32_t b = band.quotient(i), j = i - b * band.d;
+    if (8u * b + 8u <= rows) {
+      *row = (int)(8u * b + (j & 7u));
+      *col = (int)(j >> 3);
+    } else {
+      const uint32_t c = last.quotient(j);
+      *row = (int)(8u * b + (j - c * last.d));
+      *col = (int)c;
+    }
+  }
+};
+
+inline TileGrid make_grid(uint32_t rows, uint32_t cols) {
+  return {rows, cols, make_divider(8u * cols), make_divider(rows % 8u ? rows % 8u : 8u)};
 }
 
 // Tile i of those on and below the diagonal, row by row.
