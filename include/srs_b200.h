@@ -382,6 +382,12 @@ typedef struct srs_blocks {
 int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64_t k, void* d, int d_format,
                       void* stream);
 
+/* Rows of `cols` bytes at src_pitch copied to rows at dst_pitch (zeros behind them up to
+ * dst_pitch): for operands whose rows do not start on 16-byte boundaries.  dst and
+ * dst_pitch must be multiples of 16 bytes. */
+int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols, void* dst,
+                  int64_t dst_pitch, void* stream);
+
 /* Where a bounded wait of a product kernel ran out on the current device (0:
  * nowhere; results of such a call are not valid).  Synchronises the device. */
 int srs_product_status(uint32_t* status);

@@ -1,5 +1,5 @@
 """Build libsrs_b200.so (the sm_100a kernels and their C ABI) in-tree, and the
-host helper module _srs_host (C++, CPython API and libtorch headers).
+host modules _srs_host and _srs_blocks (C++, CPython API and libtorch headers).
 
     python stochastic-rounding-pytorch_b200/build_native.py [--force] [--verbose]
 
@@ -30,6 +30,9 @@ SELFTEST = HERE / "sr_states" / "_native" / "libsrs_selftest.so"
 # Host helper of the optimizer steps (tensor signatures for the repeated-step check).
 HOST = HERE / "sr_states" / "_native" / "_srs_host.so"
 HOST_SOURCE = CSRC / "host_signature.cpp"
+# Tensor front end of the FP8 block entry points.
+BLOCKS = HERE / "sr_states" / "_native" / "_srs_blocks.so"
+BLOCKS_SOURCE = CSRC / "host_blocks.cpp"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
@@ -75,32 +78,51 @@ def _kernels_up_to_date() -> bool:
 
 
 def _host_up_to_date() -> bool:
-    return HOST.exists() and HOST.stat().st_mtime >= max(HOST_SOURCE.stat().st_mtime,
-                                                         Path(__file__).stat().st_mtime)
+    return (_module_up_to_date(HOST, [HOST_SOURCE])
+            and _module_up_to_date(BLOCKS, [BLOCKS_SOURCE, INCLUDE / "srs_b200.h"]))
+
+
+def _module_up_to_date(module: Path, sources: list[Path]) -> bool:
+    return module.exists() and all(module.stat().st_mtime >= p.stat().st_mtime
+                                   for p in sources + [Path(__file__)])
 
 
 def build_host(force: bool = False) -> Path:
-    """g++ the _srs_host CPython module against the installed torch (its headers
-    for at::Tensor access, its libraries at run time)."""
-    if not force and _host_up_to_date():
-        return HOST
+    """The CPython modules against the installed torch (its headers for at::Tensor
+    access, its libraries at run time)."""
+    with ThreadPoolExecutor(2) as pool:
+        jobs = [pool.submit(_build_module, *m) for m in (
+            (HOST, HOST_SOURCE, [], []),
+            (BLOCKS, BLOCKS_SOURCE, [f"-I{INCLUDE}", f"-I{_cuda_include()}"], ["-lc10_cuda"]))
+            if force or not _module_up_to_date(m[0], [m[1], INCLUDE / "srs_b200.h"])]
+        for job in jobs:
+            job.result()
+    return HOST
+
+
+def _cuda_include() -> Path:
+    return Path(nvcc()).resolve().parents[1] / "include"
+
+
+def _build_module(module: Path, source: Path, includes: list[str], libraries: list[str]) -> None:
+    """g++ one module."""
     import sysconfig
 
     import torch
 
     torch_dir = Path(torch.__file__).resolve().parent
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    tmp = HOST.with_suffix(".so.tmp")
+    module.parent.mkdir(parents=True, exist_ok=True)
+    tmp = module.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{torch_dir / 'include'}",
-           f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-           str(HOST_SOURCE), f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{torch_dir / 'lib'}", "-o", str(tmp)]
+           f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", *includes,
+           str(source), f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", *libraries, f"-Wl,-rpath,{torch_dir / 'lib'}", "-o", str(tmp)]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"g++ failed for {HOST_SOURCE.name}:\n{result.stderr}")
-    os.replace(tmp, HOST)
-    return HOST
+        raise RuntimeError(f"g++ failed for {source.name}:\n{result.stderr}")
+    os.replace(tmp, module)
 
 
 def _compile(unit, verbose: bool) -> str:

@@ -311,6 +311,24 @@ void launch_quantize(const QuantizeArgs& a, int x_format, bool square, cudaStrea
   else launch_quantize<OF, SRS_FMT_F16>(a, square, stream);
 }
 
+// 16 bytes of the copy a thread, from any source alignment.
+__global__ void __launch_bounds__(kThreads)
+copy_rows_kernel(const uint8_t* __restrict__ src, int64_t src_pitch, int64_t rows, int64_t cols,
+                 uint8_t* __restrict__ dst, int64_t dst_pitch) {
+  const int64_t chunks = dst_pitch / 16;
+  const int64_t stride = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * chunks; i += stride) {
+    const int64_t row = i / chunks, col = (i - row * chunks) * 16;
+    const uint8_t* from = src + row * src_pitch + col;
+    const int64_t left = cols - col;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < left) w[j >> 2] |= (uint32_t)__ldg(from + j) << (8 * (j & 3));
+    *reinterpret_cast<uint4*>(dst + row * dst_pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 uint32_t host_h32(uint32_t x) {
   x ^= x >> 16;
   x *= 0x7FEB352Du;
@@ -412,6 +430,30 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
   else launch_quantize<SRS_FMT_E5M2>(a, x_format, square != 0, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_quantize_blocks launch");
+}
+
+extern "C" int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols,
+                             void* dst, int64_t dst_pitch, void* stream) {
+  clear_error();
+  if (rows < 0 || cols < 0 || src_pitch < 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "negative size or pitch");
+  if (rows == 0 || cols == 0) return SRS_OK;
+  if (src == nullptr || dst == nullptr)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if (reinterpret_cast<uintptr_t>(dst) % 16 != 0 || dst_pitch % 16 != 0 || dst_pitch < cols)
+    return fail(SRS_ERR_INVALID_ARGUMENT,
+                "the copy needs a 16-byte aligned address and a row pitch that is a multiple of "
+                "16 and at least the row length (%lld, %lld)",
+                (long long)dst_pitch, (long long)cols);
+  if (int rc = check_device()) return rc;
+  const int64_t work = (rows * (dst_pitch / 16) + kThreads - 1) / kThreads;
+  const int64_t most = 8ll * sm_count();
+  copy_rows_kernel<<<(unsigned)(work < most ? work : most), kThreads, 0,
+                     static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(src), src_pitch, rows, cols, static_cast<uint8_t*>(dst),
+      dst_pitch);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_copy_rows launch");
 }
 
 extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64_t k, void* d,

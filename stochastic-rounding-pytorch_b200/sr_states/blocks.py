@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from ._hash import update_key
-from .cuda.blocks import BLOCK, BlockTensor, matmul_blocks, quantize_blocks
+from .cuda.blocks import BLOCK, BlockTensor, linear_blocks, matmul_blocks, quantize_blocks
 
 __all__ = ["BlockLinear", "BlockTensor", "block_linear", "matmul_blocks", "quantize_blocks"]
 
@@ -68,9 +68,7 @@ def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("a BlockTensor weight has no backward pass; pass the weight itself "
                              "or run under torch.no_grad()")
-        tokens = quantize_blocks(x.reshape(-1, x.shape[-1]), dtype=dtype)
-        y = matmul_blocks(tokens, weight, dtype=x.dtype)
-        return y.reshape(*x.shape[:-1], columns[0])
+        return linear_blocks(x, weight, dtype)
     return _BlockLinear.apply(x, weight, dtype, grad_dtype, grad_rounding, seed)
 
 

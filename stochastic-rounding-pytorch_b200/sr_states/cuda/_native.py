@@ -16,6 +16,7 @@ import numpy as np
 
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "_native" / "libsrs_b200.so"
 HOST_PATH = LIBRARY_PATH.parent / "_srs_host.so"
+BLOCKS_PATH = LIBRARY_PATH.parent / "_srs_blocks.so"
 
 SRS_OK = 0
 SRS_ERR_INVALID_ARGUMENT = -1
@@ -167,6 +168,8 @@ _SIGNATURES = {
                              ctypes.c_int64, _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_matmul_blocks": ([ctypes.POINTER(SrsBlocks), ctypes.POINTER(SrsBlocks), ctypes.c_int64,
                            _P, ctypes.c_int, _P], ctypes.c_int),
+    "srs_copy_rows": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
+                       _P], ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
 }
 NOALLOC_MAX_ROWS = 4096
@@ -197,24 +200,41 @@ def load_library() -> ctypes.CDLL:
 
 
 _host = None
+_blocks = None
+
+
+def _load_module(name: str, path: Path):
+    import importlib.machinery
+    import importlib.util
+
+    if not path.exists():
+        raise RuntimeError(f"{path} is missing: build it with "
+                           "`python stochastic-rounding-pytorch_b200/build_native.py`")
+    loader = importlib.machinery.ExtensionFileLoader(name, str(path))
+    spec = importlib.util.spec_from_file_location(name, str(path), loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
 
 
 def host_module():
     """The _srs_host helper module (raises if it has not been built)."""
     global _host
     if _host is None:
-        import importlib.machinery
-        import importlib.util
-
-        if not HOST_PATH.exists():
-            raise RuntimeError(f"{HOST_PATH} is missing: build it with "
-                               "`python stochastic-rounding-pytorch_b200/build_native.py`")
-        loader = importlib.machinery.ExtensionFileLoader("_srs_host", str(HOST_PATH))
-        spec = importlib.util.spec_from_file_location("_srs_host", str(HOST_PATH), loader=loader)
-        module = importlib.util.module_from_spec(spec)
-        loader.exec_module(module)
-        _host = module
+        _host = _load_module("_srs_host", HOST_PATH)
     return _host
+
+
+def blocks_module():
+    """The _srs_blocks tensor front end, bound to the library's entry points."""
+    global _blocks
+    if _blocks is None:
+        lib = load_library()
+        module = _load_module("_srs_blocks", BLOCKS_PATH)
+        module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            lib.srs_quantize_blocks, lib.srs_matmul_blocks, lib.srs_copy_rows)))
+        _blocks = module
+    return _blocks
 
 
 def _check(rc: int) -> None:
@@ -346,16 +366,18 @@ class NativeLauncher:
             ctypes.byref(newton), ctypes.byref(rng), workspace.data_ptr(), workspace.numel(),
             stream))
 
-    def quantize_blocks(self, x_ptr, x_fmt, rows, cols, x_pitch, fmt, rule, square, seed, offset,
-                        data, data_pitch, scale, scale_pitch, data_t, data_t_pitch, scale_t,
-                        scale_t_pitch, stream):
-        _check(load_library().srs_quantize_blocks(
-            x_ptr, x_fmt, rows, cols, x_pitch, fmt, rule, square, seed, offset, data, data_pitch,
-            scale, scale_pitch, data_t, data_t_pitch, scale_t, scale_t_pitch, stream))
+    def quantize_blocks(self, x, fmt, rule, square, seed, offset, orientation):
+        """(data, scale) of x in blocks, of its transpose, or both (orientation 1, 2, 3)."""
+        got = blocks_module().quantize(x, fmt, rule, square, seed, offset, orientation)
+        return got if type(got) is tuple else _check(got)
 
-    def matmul_blocks(self, a, b, k, d_ptr, d_fmt, stream):
-        _check(load_library().srs_matmul_blocks(ctypes.byref(a), ctypes.byref(b), k, d_ptr,
-                                                d_fmt, stream))
+    def matmul_blocks(self, a, a_scale, b, b_scale, fmt):
+        got = blocks_module().matmul(a, a_scale, b, b_scale, fmt)
+        return got if type(got) is not int else _check(got)
+
+    def block_linear(self, x, w, w_scale, fmt):
+        got = blocks_module().linear(x, w, w_scale, fmt)
+        return got if type(got) is not int else _check(got)
 
     def product_status(self) -> int:
         """Where a bounded wait of a product kernel ran out (0: nowhere); synchronises."""
