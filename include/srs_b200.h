@@ -382,6 +382,15 @@ typedef struct srs_blocks {
 int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64_t k, void* d, int d_format,
                       void* stream);
 
+/* d = x w^T: x (tokens x k, FP32, BF16 or FP16, row pitch x_pitch elements) quantised to
+ * nearest in block_format (1 x 128 blocks) into `workspace` (srs_linear_workspace(tokens, k)
+ * bytes, 16-byte aligned), times the blocks of w; d in x's format, contiguous tokens x
+ * w->rows.  The same values as the two calls one after the other. */
+int64_t srs_linear_workspace(int64_t tokens, int64_t k);
+int srs_linear_blocks(const void* x, int x_format, int64_t tokens, int64_t k, int64_t x_pitch,
+                      int block_format, const srs_blocks* w, void* d, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* Rows of `cols` bytes at src_pitch copied to rows at dst_pitch (zeros behind them up to
  * dst_pitch): for operands whose rows do not start on 16-byte boundaries.  dst and
  * dst_pitch must be multiples of 16 bytes. */

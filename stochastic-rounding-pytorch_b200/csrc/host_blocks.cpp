@@ -26,6 +26,8 @@ constexpr int64_t kBlock = 128;
 decltype(&srs_quantize_blocks) g_quantize = nullptr;
 decltype(&srs_matmul_blocks) g_matmul = nullptr;
 decltype(&srs_copy_rows) g_copy_rows = nullptr;
+decltype(&srs_linear_blocks) g_linear = nullptr;
+decltype(&srs_linear_workspace) g_linear_workspace = nullptr;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -158,8 +160,13 @@ PyObject* pack(const Blocks& straight, const Blocks& turned, int orientation) {
 }
 
 PyObject* py_bind(PyObject*, PyObject* args) {
-  unsigned long long quantize_at, matmul_at, copy_at;
-  if (!PyArg_ParseTuple(args, "KKK", &quantize_at, &matmul_at, &copy_at)) return nullptr;
+  unsigned long long quantize_at, matmul_at, copy_at, linear_at, workspace_at;
+  if (!PyArg_ParseTuple(args, "KKKKK", &quantize_at, &matmul_at, &copy_at, &linear_at,
+                        &workspace_at))
+    return nullptr;
+  g_linear = reinterpret_cast<decltype(g_linear)>(static_cast<uintptr_t>(linear_at));
+  g_linear_workspace =
+      reinterpret_cast<decltype(g_linear_workspace)>(static_cast<uintptr_t>(workspace_at));
   g_quantize = reinterpret_cast<decltype(g_quantize)>(static_cast<uintptr_t>(quantize_at));
   g_matmul = reinterpret_cast<decltype(g_matmul)>(static_cast<uintptr_t>(matmul_at));
   g_copy_rows = reinterpret_cast<decltype(g_copy_rows)>(static_cast<uintptr_t>(copy_at));
@@ -212,11 +219,22 @@ PyObject* py_linear(PyObject*, PyObject* args) {
   const at::Tensor& weight = tensor(w, "the weight's data");
   const c10::cuda::OptionalCUDAGuard guard(t.device());
   const int x_format = source_format(t, "block_linear");
-  const at::Tensor flat = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  Blocks tokens, none;
-  int rc = quantize(flat, format, SRS_RULE_NEAREST, false, 0, 0, 1, &tokens, &none);
+  TORCH_CHECK_VALUE(t.device() == weight.device(), "all tensors must be on the same CUDA device");
+  at::Tensor flat = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  const int64_t tokens = flat.size(0), k = flat.size(1);
+  if (flat.stride(1) != 1 && k > 1) flat = flat.contiguous();
+  Blocks blocks{weight, tensor(w_scale, "the weight's scale")};
+  srs_blocks matrix{};
+  int rc = operand("weight", &blocks, &matrix);
   at::Tensor out;
-  if (rc == SRS_OK) rc = matmul(tokens, {weight, tensor(w_scale, "the weight's scale")}, x_format, &out);
+  if (rc == SRS_OK) {
+    out = at::empty({tokens, matrix.rows}, t.options());
+    const int64_t bytes = g_linear_workspace(tokens, k);
+    const at::Tensor space = at::empty({bytes}, t.options().dtype(at::kByte));
+    rc = g_linear(flat.data_ptr(), x_format, tokens, k, flat.stride(0), format, &matrix,
+                  out.data_ptr(), space.data_ptr(), bytes,
+                  c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+  }
   if (rc != SRS_OK) return PyLong_FromLong(rc);
   if (t.dim() != 2) {
     std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
@@ -228,7 +246,7 @@ PyObject* py_linear(PyObject*, PyObject* args) {
 }
 
 PyMethodDef kMethods[] = {
-    {"bind", py_bind, METH_VARARGS, "bind(quantize, matmul, copy_rows): entry point addresses."},
+    {"bind", py_bind, METH_VARARGS, "bind(quantize, matmul, copy_rows, linear, linear_workspace): entry point addresses."},
     {"quantize", py_quantize, METH_VARARGS,
      "quantize(x, format, rule, square, seed, offset, orientation) -> tensors or a status."},
     {"matmul", py_matmul, METH_VARARGS,

@@ -84,9 +84,10 @@ __device__ __forceinline__ void load_words(const QuantizeArgs& a, int64_t row, i
   }
 }
 
-// Largest finite size (FP32 encoding) of 8 elements a lane over 16 lanes.
+// Largest finite size (FP32 encoding) of 8 elements a lane over 16 lanes; `finite`:
+// the warp's two rows hold neither infinities nor NaN.
 template <int XF>
-__device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>]) {
+__device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>], bool* finite) {
   using Z = Size<XF>;
   uint32_t top = 0u;
 #pragma unroll
@@ -94,7 +95,8 @@ __device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>]) {
   top = Z::single(top);
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-  if (__any_sync(0xFFFFFFFFu, top >= Z::kInfinite)) {
+  *finite = !__any_sync(0xFFFFFFFFu, top >= Z::kInfinite);
+  if (!*finite) {
     top = 0u;
 #pragma unroll
     for (int j = 0; j < kWords<XF>; ++j) top = Z::larger(top, Z::finite(w[j]));
@@ -105,210 +107,295 @@ __device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>]) {
   return Z::as_f32(top);
 }
 
-template <int OF, int XF>
-__device__ __forceinline__ void encode_row(const QuantizeArgs& a, const uint32_t (&raw)[kWords<XF>],
-                                           int64_t row, int64_t col, int k) {
-  const float factor = power_of_two(-k);
-  float y[kVec];
-  decode8<XF>(raw, y);
-#pragma unroll
-  for (int j = 0; j < kVec; ++j) y[j] *= factor;
+// Rounds 8 scaled values to 8 bytes.  Values of a block are finite and at most the
+// format's largest after scaling unless the block held infinities or NaN: `plain` says
+// that it did not, and the stochastic rule then needs no screen.  The general form (any
+// value, toward zero) is kept out of the way of the instruction cache: it costs 4 of
+// 5 issue slots of the stochastic form when it is compiled into every row.
+template <int OF>
+__device__ __forceinline__ uint2 encode_plain(const float (&y)[kVec], uint32_t ctr, bool nearest) {
   uint32_t w[2];
-  encode8<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, w);
-  if (col < a.data_pitch)
-    *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = make_uint2(w[0], w[1]);
+  if (nearest) encode8<OF>(y, 0u, SRS_RULE_NEAREST, w);
+  else encode8_stochastic_fast<OF>(y, ctr, w);
+  return make_uint2(w[0], w[1]);
+}
+
+template <int OF>
+__device__ __noinline__ uint2 encode_general(float4 a, float4 b, uint32_t ctr, int rule) {
+  const float y[kVec] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t w[2];
+  encode8<OF>(y, ctr, rule, w);
+  return make_uint2(w[0], w[1]);
+}
+
+template <int OF>
+__device__ __forceinline__ uint2 encode_values(const float (&y)[kVec], uint32_t ctr, int rule,
+                                               bool plain) {
+  if (plain) return encode_plain<OF>(y, ctr, rule == SRS_RULE_NEAREST);
+  return encode_general<OF>(make_float4(y[0], y[1], y[2], y[3]),
+                            make_float4(y[4], y[5], y[6], y[7]), ctr, rule);
 }
 
 // Rows alone, 1 x 128 blocks: 16 lanes to a block, kAhead blocks of one column a
-// half-warp with all their loads first.  HBM-bound.
+// half-warp with all their loads first.  HBM-bound when rounding to nearest (8192 x
+// 4096: 27 us with the launch; 3 bytes an element at 6.5 TB/s would be 15), by the integer
+// units for the stochastic rule's hashes (45 us).
 constexpr int kAhead = 4;
 
 template <int OF, int XF>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a) {
+  // A product launched to overlap this kernel (srs_linear_blocks) may start.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane16 = threadIdx.x & 15;
   const int64_t col = (int64_t)blockIdx.x * kBlock + 8 * lane16;
   const int64_t row0 = ((int64_t)blockIdx.y * 16 + (threadIdx.x >> 4)) * kAhead;
   uint32_t raw[kAhead][kWords<XF>];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) load_words<XF>(a, row0 + i, col, raw[i]);
+  int k[kAhead];
+  bool plain = a.rule != SRS_RULE_TOWARD_ZERO;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    bool finite;
+    k[i] = block_exponent<OF>(row_size<XF>(raw[i], &finite));
+    plain = plain && finite;
+  }
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int64_t row = row0 + i;
-    const int k = block_exponent<OF>(row_size<XF>(raw[i]));
-    if (row < a.rows) {
-      encode_row<OF, XF>(a, raw[i], row, col, k);
-      if (lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
-    }
+    if (row >= a.rows) break;
+    const float factor = power_of_two(-k[i]);
+    float y[kVec];
+    decode8<XF>(raw[i], y);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) y[j] *= factor;
+    const uint2 w =
+        encode_values<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, plain);
+    if (col < a.data_pitch) *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = w;
+    if (lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k[i] + 127);
   }
 }
 
-// One CTA quantises one 128 x 128 tile of x, read once.  Thread t holds 8 rows x
-// 8 columns in registers as loaded: columns 8 * (t % 16) .., rows 8 * (t / 16) ..,
-// so a row's block maximum is a reduction over 16 lanes, a column's one over the 16
-// row groups (through shared memory), and the transposed bytes leave as 8 x 8
-// register transposes in 8-byte pieces, swizzled in shared memory so that both
-// sides are conflict-free.
+// One CTA quantises one 128 x 128 tile of x, read once into shared memory.  Thread t has
+// columns 8 * (t % 16) .. of rows 8 * (t / 16) ..: a row's block maximum is a reduction
+// over 16 lanes, a column's one over the 16 row groups.  The transposed copy's bytes
+// are kept by rows (32-bit words rotated by 4 * (row / 16), so that both sides are
+// conflict-free) and leave as 4 x 4 byte transposes, 128 bytes of a column at a time.
+// Nearest: HBM-bound; stochastic both ways: bound by the hashes (two a element, about
+// 25 integer operations).  8192 x 4096 from BF16, both ways: 51 us to nearest,
+// 90 us stochastic (E5M2); the bytes alone would take 20.
 template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
-__global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 4 : 2)
 quantize_tile_kernel(const QuantizeArgs a) {
   using Z = Size<XF>;
   constexpr int kW = kWords<XF>;
+  extern __shared__ __align__(16) uint8_t tile_raw[];  // 128 x 128 elements of x
   __shared__ uint32_t tops[COLS && !SQUARE ? 16 * 16 * kW : 8];
-  __shared__ __align__(16) uint8_t turned[COLS ? kBlock * kBlock : 16];
+  __shared__ int row_k[kBlock];
+  __shared__ __align__(16) uint32_t turned[COLS ? kBlock * 32 : 4];
   const int lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock, col0 = (int64_t)blockIdx.x * kBlock;
   const int64_t row_base = row0 + 8 * group, col = col0 + 8 * lane16;
+  // this thread's words of row i of its group: kW / 4 vectors of 16 bytes, 256 threads apart
+  uint4* const mine = reinterpret_cast<uint4*>(tile_raw) + threadIdx.x;
+  const auto slot = [&](int i, int v) { return (i * (kW / 4) + v) * kThreads; };
 
-  uint32_t raw[8][kW];
+  bool plain = a.rule != SRS_RULE_TOWARD_ZERO;
+  int tile_k = 0;          // SQUARE: the block's exponent
+  float col_factor[kVec];  // else: the columns' factors
+  {
+    uint32_t raw[8][kW];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load_words<XF>(a, row_base + i, col, raw[i]);
-
-  int tile_k = 0;         // SQUARE: the block's exponent
-  uint32_t col_top[kVec];  // else: FP32 encodings of the columns' largest sizes
-  if constexpr (SQUARE) {
-    uint32_t top = 0u;
-    for (int pass = 0; pass < 2; ++pass) {
-      top = 0u;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-#pragma unroll
-        for (int j = 0; j < kW; ++j)
-          top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
-      }
-      top = __reduce_max_sync(0xFFFFFFFFu, Z::single(top));
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
-      if (top < Z::kInfinite) break;  // the same for the whole CTA
-    }
-    tile_k = block_exponent<OF>(Z::as_f32(top));
-  } else if constexpr (COLS) {
-    for (int pass = 0; pass < 2; ++pass) {
-      uint32_t top[kW];
-#pragma unroll
-      for (int j = 0; j < kW; ++j) {
-        top[j] = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          top[j] = Z::larger(top[j], pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
-        tops[(group * kW + j) * 16 + lane16] = top[j];
-      }
-      __syncthreads();
-      bool infinite = false;
-#pragma unroll
-      for (int j = 0; j < kW; ++j) {
-        uint32_t t = 0u;
-#pragma unroll
-        for (int g = 0; g < 16; ++g) t = Z::larger(t, tops[(g * kW + j) * 16 + lane16]);
-        if (Z::kPacked) {
-          col_top[2 * j % kVec] = t & 0xFFFFu;
-          col_top[(2 * j + 1) % kVec] = t >> 16;
-        } else {
-          col_top[j] = t;
-        }
-        infinite = infinite || Z::single(t) >= Z::kInfinite;
-      }
-      if (!__syncthreads_or(infinite)) break;
-    }
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) col_top[j] = Z::as_f32(col_top[j]);
-  }
-
-  if constexpr (ROWS) {
+    for (int i = 0; i < 8; ++i) load_words<XF>(a, row_base + i, col, raw[i]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t row = row_base + i;
-      const int k = SQUARE ? tile_k : block_exponent<OF>(row_size<XF>(raw[i]));
+#pragma unroll
+      for (int v = 0; v < kW / 4; ++v)
+        mine[slot(i, v)] =
+            make_uint4(raw[i][4 * v], raw[i][4 * v + 1], raw[i][4 * v + 2], raw[i][4 * v + 3]);
+    }
+    if constexpr (SQUARE) {
+      uint32_t top = 0u;
+      for (int pass = 0; pass < 2; ++pass) {
+        top = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int j = 0; j < kW; ++j)
+            top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
+        }
+        top = __reduce_max_sync(0xFFFFFFFFu, Z::single(top));
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+        if (top < Z::kInfinite) break;  // the same for the whole CTA
+        plain = false;
+      }
+      tile_k = block_exponent<OF>(Z::as_f32(top));
+    } else {
+      if constexpr (ROWS) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          bool finite;
+          const int k = block_exponent<OF>(row_size<XF>(raw[i], &finite));
+          plain = plain && finite;
+          if (lane16 == 0) row_k[8 * group + i] = k;
+        }
+      }
+      if constexpr (COLS) {
+        uint32_t col_top[kVec];
+        for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+          for (int j = 0; j < kW; ++j) {
+            uint32_t top = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
+            tops[(group * kW + j) * 16 + lane16] = top;
+          }
+          __syncthreads();
+          bool infinite = false;
+#pragma unroll
+          for (int j = 0; j < kW; ++j) {
+            uint32_t t = 0u;
+#pragma unroll
+            for (int g = 0; g < 16; ++g) t = Z::larger(t, tops[(g * kW + j) * 16 + lane16]);
+            if (Z::kPacked) {
+              col_top[2 * j % kVec] = t & 0xFFFFu;
+              col_top[(2 * j + 1) % kVec] = t >> 16;
+            } else {
+              col_top[j] = t;
+            }
+            infinite = infinite || Z::single(t) >= Z::kInfinite;
+          }
+          if (!__syncthreads_or(infinite)) break;
+          plain = false;
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const int k = block_exponent<OF>(Z::as_f32(col_top[j]));
+          col_factor[j] = power_of_two(-k);
+          if (group == 0 && col + j < a.cols)
+            a.scale_t[(col + j) * a.scale_t_pitch + blockIdx.y] = (uint8_t)(k + 127);
+        }
+      }
+    }
+  }
+  __syncwarp();
+
+  uint32_t ctr = a.ctr + (uint32_t)(row_base * a.cols + col);
+  uint32_t ctr_t = a.ctr_t + (uint32_t)(row_base * a.cols + col);
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    uint32_t raw[kW];
+#pragma unroll
+    for (int v = 0; v < kW / 4; ++v) {
+      const uint4 q = mine[slot(i, v)];
+      raw[4 * v] = q.x;
+      raw[4 * v + 1] = q.y;
+      raw[4 * v + 2] = q.z;
+      raw[4 * v + 3] = q.w;
+    }
+    float x[kVec], y[kVec];
+    decode8<XF>(raw, x);
+    const int64_t row = row_base + i;
+    if constexpr (ROWS) {
+      const int k = SQUARE ? tile_k : row_k[8 * group + i];
+      const float factor = power_of_two(-k);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) y[j] = x[j] * factor;
+      const uint2 w = encode_values<OF>(y, ctr, a.rule, plain);
       if (row < a.rows) {
-        encode_row<OF, XF>(a, raw[i], row, col, k);
+        if (col < a.data_pitch) *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = w;
         if (!SQUARE && lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
       }
     }
-    if (SQUARE && threadIdx.x == 0)
+    if constexpr (COLS) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        y[j] = x[j] * (SQUARE ? power_of_two(-tile_k) : col_factor[j]);
+      const uint2 w = encode_values<OF>(y, ctr_t, a.rule, plain);
+      const int r = 8 * group + i;
+      *reinterpret_cast<uint2*>(turned + r * 32 + ((2 * lane16 + 4 * (r >> 4)) & 31)) = w;
+    }
+    ctr += (uint32_t)a.cols;
+    ctr_t += (uint32_t)a.cols;
+  }
+  if (SQUARE && threadIdx.x == 0) {
+    if (ROWS)
       a.scale[(int64_t)blockIdx.y * a.scale_pitch + blockIdx.x] = (uint8_t)(tile_k + 127);
+    if (COLS)
+      a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] = (uint8_t)(tile_k + 127);
   }
 
   if constexpr (COLS) {
-    uint32_t w[8][2];  // 8 rows of 8 bytes
+    __syncthreads();
+    // 16 rows of 4 columns a thread
+    const int h = threadIdx.x & 7, word = threadIdx.x >> 3;
+    uint32_t out[4][4];  // column, 4 rows a word
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float y[kVec];
-      decode8<XF>(raw[i], y);
+    for (int q = 0; q < 4; ++q) {
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        y[j] *= power_of_two(-(SQUARE ? tile_k : block_exponent<OF>(col_top[j])));
-      encode8<OF>(y, a.ctr_t + (uint32_t)((row_base + i) * a.cols + col), a.rule, w[i]);
-    }
-    // 8 x 8 byte transpose, then column 8 * lane16 + j gets rows 8 * group .. + 7
+      for (int r = 0; r < 4; ++r)
+        w[r] = turned[(16 * h + 4 * q + r) * 32 + ((word + 4 * h) & 31)];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t pick = (uint32_t)j | ((uint32_t)(j + 4) << 4);
-        uint32_t out[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t lo = __byte_perm(w[4 * q][half], w[4 * q + 1][half], pick);
-          const uint32_t hi = __byte_perm(w[4 * q + 2][half], w[4 * q + 3][half], pick);
-          out[q] = __byte_perm(lo, hi, 0x5410u);
-        }
-        const int c = 8 * lane16 + 4 * half + j;
-        *reinterpret_cast<uint2*>(turned + c * kBlock + 8 * (group ^ lane16)) =
-            make_uint2(out[0], out[1]);
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t pick = (uint32_t)c | ((uint32_t)(c + 4) << 4);
+        out[c][q] = __byte_perm(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick),
+                                0x5410u);
       }
     }
-    __syncthreads();
+    const int64_t at = row0 + 16 * h;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 32 * i + (threadIdx.x >> 3), h = threadIdx.x & 7, l = c >> 3;
-      const uint4 v = *reinterpret_cast<const uint4*>(turned + c * kBlock + 16 * (h ^ (l >> 1)));
-      const uint4 o = (l & 1) ? make_uint4(v.z, v.w, v.x, v.y) : v;
-      const int64_t at = row0 + 16 * h;
-      if (col0 + c < a.cols && at < a.data_t_pitch)
-        *reinterpret_cast<uint4*>(a.data_t + (col0 + c) * a.data_t_pitch + at) = o;
-    }
-    if constexpr (SQUARE) {
-      if (threadIdx.x == 0)
-        a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] = (uint8_t)(tile_k + 127);
-    } else if (group == 0) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (col + j < a.cols)
-          a.scale_t[(col + j) * a.scale_t_pitch + blockIdx.y] =
-              (uint8_t)(block_exponent<OF>(col_top[j]) + 127);
+    for (int c = 0; c < 4; ++c) {
+      const int64_t to = col0 + 4 * word + c;
+      if (to < a.cols && at < a.data_t_pitch)
+        *reinterpret_cast<uint4*>(a.data_t + to * a.data_t_pitch + at) =
+            make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
     }
   }
+}
+
+template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
+cudaError_t launch_tile(const QuantizeArgs& a, dim3 grid, cudaStream_t stream) {
+  constexpr int kTileBytes = kBlock * kBlock * Fmt<XF>::kBytes;
+  const auto kernel = &quantize_tile_kernel<OF, XF, ROWS, COLS, SQUARE>;
+  if (kTileBytes + (COLS ? 24 * 1024 : 0) > 40 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileBytes);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<grid, kThreads, kTileBytes, stream>>>(a);
+  return cudaGetLastError();
 }
 
 template <int OF, int XF>
-void launch_quantize(const QuantizeArgs& a, bool square, cudaStream_t stream) {
+cudaError_t launch_quantize(const QuantizeArgs& a, bool square, cudaStream_t stream) {
   const unsigned columns = (unsigned)((a.cols + kBlock - 1) / kBlock);
   const dim3 tiles(columns, (unsigned)((a.rows + kBlock - 1) / kBlock));
+  const bool rows = a.data != nullptr, cols = a.data_t != nullptr;
   if (square) {
-    if (a.data != nullptr && a.data_t != nullptr)
-      quantize_tile_kernel<OF, XF, true, true, true><<<tiles, kThreads, 0, stream>>>(a);
-    else if (a.data != nullptr)
-      quantize_tile_kernel<OF, XF, true, false, true><<<tiles, kThreads, 0, stream>>>(a);
-    else
-      quantize_tile_kernel<OF, XF, false, true, true><<<tiles, kThreads, 0, stream>>>(a);
-  } else if (a.data_t == nullptr) {
-    const int64_t rows = 16 * kAhead;
-    const dim3 grid(columns, (unsigned)((a.rows + rows - 1) / rows));
-    quantize_rows_kernel<OF, XF><<<grid, kThreads, 0, stream>>>(a);
-  } else if (a.data != nullptr) {
-    quantize_tile_kernel<OF, XF, true, true, false><<<tiles, kThreads, 0, stream>>>(a);
-  } else {
-    quantize_tile_kernel<OF, XF, false, true, false><<<tiles, kThreads, 0, stream>>>(a);
+    if (rows && cols) return launch_tile<OF, XF, true, true, true>(a, tiles, stream);
+    return rows ? launch_tile<OF, XF, true, false, true>(a, tiles, stream)
+                : launch_tile<OF, XF, false, true, true>(a, tiles, stream);
   }
+  if (cols)
+    return rows ? launch_tile<OF, XF, true, true, false>(a, tiles, stream)
+                : launch_tile<OF, XF, false, true, false>(a, tiles, stream);
+  const dim3 grid(columns, (unsigned)((a.rows + 16 * kAhead - 1) / (16 * kAhead)));
+  quantize_rows_kernel<OF, XF><<<grid, kThreads, 0, stream>>>(a);
+  return cudaGetLastError();
 }
 
 template <int OF>
-void launch_quantize(const QuantizeArgs& a, int x_format, bool square, cudaStream_t stream) {
-  if (x_format == SRS_FMT_F32) launch_quantize<OF, SRS_FMT_F32>(a, square, stream);
-  else if (x_format == SRS_FMT_BF16) launch_quantize<OF, SRS_FMT_BF16>(a, square, stream);
-  else launch_quantize<OF, SRS_FMT_F16>(a, square, stream);
+cudaError_t launch_quantize(const QuantizeArgs& a, int x_format, bool square,
+                            cudaStream_t stream) {
+  if (x_format == SRS_FMT_F32) return launch_quantize<OF, SRS_FMT_F32>(a, square, stream);
+  if (x_format == SRS_FMT_BF16) return launch_quantize<OF, SRS_FMT_BF16>(a, square, stream);
+  return launch_quantize<OF, SRS_FMT_F16>(a, square, stream);
 }
 
 // 16 bytes of the copy a thread, from any source alignment.
@@ -378,13 +465,11 @@ int check_operand(const char* what, const srs_blocks* b, int64_t k) {
 
 using namespace srs;
 
-extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
-                                   int64_t x_pitch, int out_format, int rule, int square,
-                                   uint32_t seed, uint32_t offset, void* data, int64_t data_pitch,
-                                   void* scale, int64_t scale_pitch, void* data_t,
-                                   int64_t data_t_pitch, void* scale_t, int64_t scale_t_pitch,
-                                   void* stream) {
-  clear_error();
+static int quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
+                           int64_t x_pitch, int out_format, int rule, int square, uint32_t seed,
+                           uint32_t offset, void* data, int64_t data_pitch, void* scale,
+                           int64_t scale_pitch, void* data_t, int64_t data_t_pitch, void* scale_t,
+                           int64_t scale_t_pitch, cudaStream_t stream) {
   if (x_format < SRS_FMT_F32 || x_format > SRS_FMT_F16)
     return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported input format %d", x_format);
   if (out_format != SRS_FMT_E4M3 && out_format != SRS_FMT_E5M2)
@@ -425,11 +510,23 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
   a.scale_pitch = scale_pitch;
   a.data_t_pitch = data_t_pitch;
   a.scale_t_pitch = scale_t_pitch;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (out_format == SRS_FMT_E4M3) launch_quantize<SRS_FMT_E4M3>(a, x_format, square != 0, st);
-  else launch_quantize<SRS_FMT_E5M2>(a, x_format, square != 0, st);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      out_format == SRS_FMT_E4M3
+          ? launch_quantize<SRS_FMT_E4M3>(a, x_format, square != 0, stream)
+          : launch_quantize<SRS_FMT_E5M2>(a, x_format, square != 0, stream);
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_quantize_blocks launch");
+}
+
+extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
+                                   int64_t x_pitch, int out_format, int rule, int square,
+                                   uint32_t seed, uint32_t offset, void* data, int64_t data_pitch,
+                                   void* scale, int64_t scale_pitch, void* data_t,
+                                   int64_t data_t_pitch, void* scale_t, int64_t scale_t_pitch,
+                                   void* stream) {
+  clear_error();
+  return quantize_blocks(x, x_format, rows, cols, x_pitch, out_format, rule, square, seed, offset,
+                         data, data_pitch, scale, scale_pitch, data_t, data_t_pitch, scale_t,
+                         scale_t_pitch, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols,
@@ -477,7 +574,50 @@ extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64
   }
   // Few rows on one side: the other side's bytes bound the product.
   if (b->rows <= kThinRows && a->rows >= b->rows)
-    return launch_thin(*a, *b, k, d, d_format, b->rows, 1, st);
-  if (a->rows <= kThinRows) return launch_thin(*b, *a, k, d, d_format, 1, b->rows, st);
+    return launch_thin(*a, *b, k, d, d_format, b->rows, 1, false, st);
+  if (a->rows <= kThinRows) return launch_thin(*b, *a, k, d, d_format, 1, b->rows, false, st);
   return launch_block_product(*a, *b, k, d, d_format, st);
+}
+
+extern "C" int64_t srs_linear_workspace(int64_t tokens, int64_t k) {
+  if (tokens <= 0 || k <= 0) return 0;
+  const int64_t pitch = (k + 15) / 16 * 16;
+  return tokens * (pitch + blocks_of(k));
+}
+
+extern "C" int srs_linear_blocks(const void* x, int x_format, int64_t tokens, int64_t k,
+                                 int64_t x_pitch, int block_format, const srs_blocks* w, void* d,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_operand("w", w, k)) return rc;
+  if (tokens < 0 || k < 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "negative size (%lld, %lld)", (long long)tokens,
+                (long long)k);
+  if (tokens == 0 || w->rows == 0) return SRS_OK;
+  if (workspace_bytes < srs_linear_workspace(tokens, k) ||
+      (k > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+    return fail(SRS_ERR_INVALID_ARGUMENT,
+                "workspace of %lld bytes, %lld needed at a 16-byte aligned address",
+                (long long)workspace_bytes, (long long)srs_linear_workspace(tokens, k));
+  srs_blocks rows{};
+  rows.data = reinterpret_cast<uint64_t>(workspace);
+  rows.rows = tokens;
+  rows.pitch = (k + 15) / 16 * 16;
+  rows.scale = rows.data + (uint64_t)(tokens * rows.pitch);
+  rows.scale_pitch = blocks_of(k);
+  rows.format = block_format;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = quantize_blocks(x, x_format, tokens, k, x_pitch, block_format, SRS_RULE_NEAREST, 0,
+                               0u, 0u, workspace, rows.pitch,
+                               static_cast<char*>(workspace) + tokens * rows.pitch,
+                               rows.scale_pitch, nullptr, 0, nullptr, 0, st))
+    return rc;
+  // With few tokens the product starts beside the quantisation and streams the
+  // weights, which that kernel does not write, before it needs the tokens.
+  if (k > 0 && tokens <= kThinRows && w->rows >= tokens) {
+    if (d == nullptr || reinterpret_cast<uintptr_t>(d) % fmt_bytes(x_format) != 0)
+      return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
+    return launch_thin(*w, rows, k, d, x_format, 1, w->rows, true, st);
+  }
+  return srs_matmul_blocks(&rows, w, k, d, x_format, stream);
 }

@@ -31,17 +31,20 @@ int status_word(unsigned int** word);
 int prepare_kernel(const void* kernel, int group, int threads, int smem, int* resident);
 
 // Launches `kernel` with one argument on groups * group CTAs; `cooperative` when its CTAs
-// wait for one another.
+// wait for one another; `overlap` when it may start before the kernel ahead of it in the
+// stream has finished (it then waits for that kernel itself).
 int launch_groups(const void* kernel, int64_t groups, int group, int threads, int smem,
-                  bool cooperative, void* argument, cudaStream_t stream, const char* what);
+                  bool cooperative, void* argument, cudaStream_t stream, const char* what,
+                  bool overlap = false);
 
 // FP8 blocks: d = a b^T (srs_blocks.h's operands, checked by the caller).  Element (i, j)
 // of d is stored at i * row_stride + j * col_stride; only products with a thin side
-// (at most kThinRows rows) take a col_stride other than 1.
+// (at most kThinRows rows) take a col_stride other than 1.  `overlap`: the kernel ahead
+// writes nothing of a.
 constexpr int kThinRows = 64;
 int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d,
                          int d_format, cudaStream_t stream);
 int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
-                int64_t row_stride, int64_t col_stride, cudaStream_t stream);
+                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream);
 
 }  // namespace srs

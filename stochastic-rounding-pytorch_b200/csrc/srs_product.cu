@@ -129,9 +129,10 @@ int prepare_kernel(const void* kernel, int group, int threads, int smem, int* re
 }
 
 int launch_groups(const void* kernel, int64_t groups, int group, int threads, int smem,
-                  bool cooperative, void* argument, cudaStream_t stream, const char* what) {
+                  bool cooperative, void* argument, cudaStream_t stream, const char* what,
+                  bool overlap) {
   cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attributes[2]{};
+  cudaLaunchAttribute attributes[3]{};
   config.gridDim = dim3((unsigned)(groups * group));
   config.blockDim = dim3((unsigned)threads);
   config.dynamicSmemBytes = (size_t)smem;
@@ -147,6 +148,11 @@ int launch_groups(const void* kernel, int64_t groups, int group, int threads, in
     cudaLaunchAttribute& a = attributes[config.numAttrs++];
     a.id = cudaLaunchAttributeCooperative;
     a.val.cooperative = 1;
+  }
+  if (overlap) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
   }
   void* arguments[1] = {argument};
   const cudaError_t e = cudaLaunchKernelExC(&config, kernel, arguments);
@@ -280,19 +286,19 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
 namespace {
 
 template <int BN>
-int launch_thin_as(ThinArgs& args, int splits, cudaStream_t stream) {
+int launch_thin_as(ThinArgs& args, int splits, bool overlap, cudaStream_t stream) {
   using S = ThinShape<BN>;
   const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN>);
   int resident = 0;
   if (int rc = prepare_kernel(kernel, 1, kThinThreads, S::kSmem, &resident)) return rc;
   return launch_groups(kernel, (args.m + 127) / 128, splits, kThinThreads, S::kSmem, false, &args,
-                       stream, "thin product launch");
+                       stream, "thin product launch", overlap);
 }
 
 }  // namespace
 
 int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
-                int64_t row_stride, int64_t col_stride, cudaStream_t stream) {
+                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream) {
   const int columns = b.rows <= 16 ? 16 : b.rows <= 32 ? 32 : 64;
   ThinArgs args{};
   if (int rc = operand_map(a, k, 128, &args.map_a)) return rc;
@@ -317,9 +323,9 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 2ll * sm_count() && args.slices >= 4 * splits)
     splits *= 2;
-  if (columns == 16) return launch_thin_as<16>(args, splits, stream);
-  if (columns == 32) return launch_thin_as<32>(args, splits, stream);
-  return launch_thin_as<64>(args, splits, stream);
+  if (columns == 16) return launch_thin_as<16>(args, splits, overlap, stream);
+  if (columns == 32) return launch_thin_as<32>(args, splits, overlap, stream);
+  return launch_thin_as<64>(args, splits, overlap, stream);
 }
 
 }  // namespace srs

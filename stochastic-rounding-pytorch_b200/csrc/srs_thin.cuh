@@ -9,6 +9,10 @@
 // rank order (FP32), so results do not depend on timing.  Two CTAs share an SM,
 // each with 4 or 5 slices of 128 rows x 128 bytes on their way.
 //
+// Launched behind the quantisation of its B (srs_linear_blocks) the kernel may start
+// while that one runs: it loads A first and waits for the other kernel before it
+// touches B.
+//
 // Roles, barriers and bounded waits as in the large product (one tile per CTA).
 #pragma once
 
@@ -93,17 +97,29 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     return bar0 + 8u * (2 * S::kStages + 1 + kScaleSlots + i);
   };
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
-      barrier_init(full(s), 1);
-      barrier_init(empty(s), 1);
+  // The loading warp sets up its barriers and sends for its first slices of A at once,
+  // before TMEM is there.
+  const int ahead = min(S::kStages, last - first);
+  if (warp == 4) {
+    if (elect_lane()) {
+      for (int s = 0; s < S::kStages; ++s) {
+        barrier_init(full(s), 1);
+        barrier_init(empty(s), 1);
+      }
+      barrier_init(done, 1);
+      for (int i = 0; i < kScaleSlots; ++i) {
+        barrier_init(scale_full(i), 1);
+        barrier_init(scale_empty(i), 1);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      for (int i = 0; i < ahead; ++i) {
+        barrier_expect(full(i), S::kStageBytes);
+        load_box<1>(stage0 + i * S::kStageBytes, &a.map_a, (first + i) * kSliceBytes, row0, 0,
+                    full(i));
+      }
     }
-    barrier_init(done, 1);
-    for (int i = 0; i < kScaleSlots; ++i) {
-      barrier_init(scale_full(i), 1);
-      barrier_init(scale_empty(i), 1);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
   }
   if (warp == 5) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
   tmem_fence_before();
@@ -114,15 +130,20 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
 
   if (warp == 4) {
     const bool leader = elect_lane();
+    // B may come from the kernel this one overlaps.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int s = 0;
     uint32_t phase = 0;
     for (int i = first; i < last; ++i) {
-      ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
-      if (!ok) break;
       const uint32_t pa = stage0 + s * S::kStageBytes;
+      const bool sent = i - first < ahead;
+      if (!sent) ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
+      if (!ok) break;
       if (leader) {
-        barrier_expect(full(s), S::kStageBytes);
-        load_box<1>(pa, &a.map_a, i * kSliceBytes, row0, 0, full(s));
+        if (!sent) {
+          barrier_expect(full(s), S::kStageBytes);
+          load_box<1>(pa, &a.map_a, i * kSliceBytes, row0, 0, full(s));
+        }
         load_box<1>(pa + kPanelBytes, &a.map_b, i * kSliceBytes, 0, 0, full(s));
       }
       __syncwarp();
@@ -195,6 +216,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     uint32_t phase = 0;
     const bool words_a = scale_words(a.scale_a, a.scale_a_pitch, first);
     const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, first);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     ScaleRows from_a, from_b;
     from_a.at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
     from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, 0, a.n, lane);

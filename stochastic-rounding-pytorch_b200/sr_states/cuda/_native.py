@@ -168,6 +168,10 @@ _SIGNATURES = {
                              ctypes.c_int64, _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_matmul_blocks": ([ctypes.POINTER(SrsBlocks), ctypes.POINTER(SrsBlocks), ctypes.c_int64,
                            _P, ctypes.c_int, _P], ctypes.c_int),
+    "srs_linear_workspace": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+    "srs_linear_blocks": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                           ctypes.c_int, ctypes.POINTER(SrsBlocks), _P, _P, ctypes.c_int64, _P],
+                          ctypes.c_int),
     "srs_copy_rows": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
                        _P], ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
@@ -232,7 +236,8 @@ def blocks_module():
         lib = load_library()
         module = _load_module("_srs_blocks", BLOCKS_PATH)
         module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
-            lib.srs_quantize_blocks, lib.srs_matmul_blocks, lib.srs_copy_rows)))
+            lib.srs_quantize_blocks, lib.srs_matmul_blocks, lib.srs_copy_rows,
+            lib.srs_linear_blocks, lib.srs_linear_workspace)))
         _blocks = module
     return _blocks
 

@@ -112,6 +112,20 @@ def test_entry_points_check_before_any_cuda_call():
     assert mm(good, good, 128, None, 0, None) == bad and mm(good, good, -1, 4096, 0, None) == bad
     assert mm(good, good, 128, 4096, 4, None) == bad
     assert mm(operand(rows=0), good, 128, None, 0, None) == _native.SRS_OK
+    need = lib.srs_linear_workspace(3, 100)
+    assert need == 3 * (112 + 1) and lib.srs_linear_workspace(0, 5) == 0
+    linear = lambda **k: lib.srs_linear_blocks(*{  # noqa: E731
+        "x": 256, "xf": 0, "t": 3, "k": 100, "xp": 100, "bf": 3, "w": good, "d": 4096,
+        "ws": 512, "wb": need, "s": None, **k}.values())
+    assert linear(wb=need - 1) == bad and linear(ws=None) == bad and linear(ws=520) == bad
+    assert linear(xf=5) == bad and linear(bf=1) == bad and linear(t=-1) == bad
+    assert linear(w=None) == bad and linear(w=operand(pitch=96)) == bad and linear(x=None) == bad
+    assert linear(t=0) == _native.SRS_OK
+    assert lib.srs_copy_rows(256, 5, -1, 5, 512, 16, None) == bad
+    assert lib.srs_copy_rows(256, 5, 1, 5, 520, 16, None) == bad
+    assert lib.srs_copy_rows(256, 5, 1, 17, 512, 16, None) == bad
+    assert lib.srs_copy_rows(None, 5, 1, 5, 512, 16, None) == bad
+    assert lib.srs_copy_rows(None, 5, 0, 5, None, 16, None) == _native.SRS_OK
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs a C compiler")
