@@ -2,12 +2,13 @@
 //
 //   D[i, j] = sum_k A[i, k] * B[j, k],   A: m x k (the weights), B: n x k, n <= 64
 //
-// What bounds it: A's bytes, read once.  The weights take the 128-row side of the
-// MMA and the thin operand the column side, so that no MMA row is idle, and k is
-// split over a cluster of up to 8 CTAs so that all SMs stream: 4096 rows are only
-// 32 tiles.  The split sums meet in distributed shared memory and are added in
-// rank order (FP32), so results do not depend on timing.  Two CTAs share an SM,
-// each with 4 or 5 slices of 128 rows x 128 bytes on their way.
+// What bounds it: A's bytes, read once, and about 6 us of launch, first loads and last
+// sums.  The weights take the 128-row side of the MMA and the thin operand the column
+// side, so that no MMA row is idle, and k is split over a cluster of up to 8 CTAs so
+// that all SMs stream: 4096 rows are only 32 tiles.  The split sums meet in distributed
+// shared memory and are added in rank order (FP32), so results do not depend on
+// timing.  Two CTAs share an SM, each with about 90 KB of slices on their way.
+// 14336 x 4096 by one token (58.7 MB): 15.2 us; 28672 x 8192: 42.3 us, 5.55 TB/s.
 //
 // Launched behind the quantisation of its B (srs_linear_blocks) the kernel may start
 // while that one runs: it loads A first and waits for the other kernel before it
@@ -22,9 +23,16 @@ namespace srs {
 
 constexpr int kThinThreads = 256;
 
+constexpr int kThinMaxStages = 12;
+constexpr int kThinSlots = 8;    // scale groups on their way
+constexpr int kThinLoaders = 6;  // warps that bring them
+
 struct ThinArgs {
   CUtensorMap map_a, map_b;
   int m, n;             // rows of A and of B
+  int rows;             // of a tile
+  int panel_bytes;      // of A in a stage (whole 8-row groups)
+  int stages;
   int slices;           // of 128 along k
   const uint8_t* scale_a;
   const uint8_t* scale_b;
@@ -39,14 +47,16 @@ struct ThinArgs {
 
 template <int BN>
 struct ThinShape {
-  static constexpr int kStages = BN <= 32 ? 5 : 4;  // two CTAs' worth fit an SM
-  static constexpr int kStageBytes = kPanelBytes + BN * kSliceBytes;
   static constexpr int kColumns = BN <= 16 ? 32 : BN <= 32 ? 64 : 128;  // TMEM
   static constexpr int kScaleColumn = BN;  // two groups of 8 columns (A, B)
   static constexpr int kScaleBytes = 1024;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes;
+  static constexpr int kFixed = 1024 + kThinSlots * kScaleBytes;  // alignment, scales
+  // Two CTAs fit an SM.  The MMA reads 128 rows of A whatever the tile has: behind the
+  // last stage's panel a whole one stays inside the CTA's memory.
+  static constexpr int kBudget = 110 * 1024 - kFixed;
+  static constexpr int kSums = 128 * BN * 4;  // split sums, in the stages' place
   static_assert(BN + 16 <= kColumns, "accumulator and scales fit");
-  static_assert(128 * BN * 4 <= kStages * kStageBytes, "split sums fit the stages");
+  static_assert(kSums <= kBudget, "split sums fit the stages");
 };
 
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
@@ -76,46 +86,50 @@ __global__ void __launch_bounds__(kThinThreads, 2)
 thin_product_kernel(const __grid_constant__ ThinArgs a) {
   using S = ThinShape<BN>;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 1 + 2 * kScaleSlots];
+  __shared__ __align__(8) uint64_t bars[2 * kThinMaxStages + 1 + 2 * kThinSlots];
   __shared__ uint32_t tmem_slot;
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const uint32_t rank = cluster_rank();
-  const int row0 = (int)(blockIdx.x / splits) * 128;
+  const int row0 = (int)(blockIdx.x / splits) * a.rows;
   const int first = (int)((int64_t)a.slices * rank / splits);
   const int last = (int)((int64_t)a.slices * (rank + 1) / splits);
-  const uint32_t stage0 = (smem_address(raw) + 1023u) & ~1023u;
-  const uint32_t scales0 = stage0 + S::kStages * S::kStageBytes;
+  const uint32_t scales0 = (smem_address(raw) + 1023u) & ~1023u;
+  const uint32_t stage0 = scales0 + kThinSlots * S::kScaleBytes;
+  const int stages = a.stages;
+  const uint32_t panel_bytes = (uint32_t)a.panel_bytes;
+  const uint32_t stage_bytes = panel_bytes + BN * kSliceBytes;
+  const uint32_t load_bytes = (uint32_t)a.rows * kSliceBytes + BN * kSliceBytes;
   const uint32_t bar0 = smem_address(bars);
   const auto full = [&](int s) { return bar0 + 8u * s; };
-  const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
-  const uint32_t done = bar0 + 8u * (2 * S::kStages);
-  const auto scale_full = [&](int i) { return bar0 + 8u * (2 * S::kStages + 1 + i); };
+  const auto empty = [&](int s) { return bar0 + 8u * (kThinMaxStages + s); };
+  const uint32_t done = bar0 + 8u * (2 * kThinMaxStages);
+  const auto scale_full = [&](int i) { return bar0 + 8u * (2 * kThinMaxStages + 1 + i); };
   const auto scale_empty = [&](int i) {
-    return bar0 + 8u * (2 * S::kStages + 1 + kScaleSlots + i);
+    return bar0 + 8u * (2 * kThinMaxStages + 1 + kThinSlots + i);
   };
 
   // The loading warp sets up its barriers and sends for its first slices of A at once,
   // before TMEM is there.
-  const int ahead = min(S::kStages, last - first);
+  const int ahead = min(stages, last - first);
   if (warp == 4) {
     if (elect_lane()) {
-      for (int s = 0; s < S::kStages; ++s) {
+      for (int s = 0; s < stages; ++s) {
         barrier_init(full(s), 1);
         barrier_init(empty(s), 1);
       }
       barrier_init(done, 1);
-      for (int i = 0; i < kScaleSlots; ++i) {
+      for (int i = 0; i < kThinSlots; ++i) {
         barrier_init(scale_full(i), 1);
         barrier_init(scale_empty(i), 1);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       for (int i = 0; i < ahead; ++i) {
-        barrier_expect(full(i), S::kStageBytes);
-        load_box<1>(stage0 + i * S::kStageBytes, &a.map_a, (first + i) * kSliceBytes, row0, 0,
+        barrier_expect(full(i), load_bytes);
+        load_box<1>(stage0 + i * stage_bytes, &a.map_a, (first + i) * kSliceBytes, row0, 0,
                     full(i));
       }
     }
@@ -135,27 +149,27 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     int s = 0;
     uint32_t phase = 0;
     for (int i = first; i < last; ++i) {
-      const uint32_t pa = stage0 + s * S::kStageBytes;
+      const uint32_t pa = stage0 + s * stage_bytes;
       const bool sent = i - first < ahead;
       if (!sent) ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
       if (!ok) break;
       if (leader) {
         if (!sent) {
-          barrier_expect(full(s), S::kStageBytes);
+          barrier_expect(full(s), load_bytes);
           load_box<1>(pa, &a.map_a, i * kSliceBytes, row0, 0, full(s));
         }
-        load_box<1>(pa + kPanelBytes, &a.map_b, i * kSliceBytes, 0, 0, full(s));
+        load_box<1>(pa + panel_bytes, &a.map_b, i * kSliceBytes, 0, 0, full(s));
       }
       __syncwarp();
-      if (++s == S::kStages) {
+      if (++s == stages) {
         s = 0;
         phase ^= 1u;
       }
     }
     // Every stage given back before the CTA can leave.
-    for (int i = 0; i < S::kStages && ok; ++i) {
+    for (int i = 0; i < stages && ok; ++i) {
       ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 14);
-      if (++s == S::kStages) {
+      if (++s == stages) {
         s = 0;
         phase ^= 1u;
       }
@@ -183,7 +197,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
         __syncwarp();
         last_slot = slot;
         last_phase = slot_phase;
-        if (++slot == kScaleSlots) {
+        if (++slot == kThinSlots) {
           slot = 0;
           slot_phase ^= 1u;
         }
@@ -191,9 +205,9 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       ok = barrier_wait(full(s), phase, a.status, 1u << 11);
       if (!ok) break;
       tmem_fence_after();
-      const uint32_t pa = stage0 + s * S::kStageBytes;
+      const uint32_t pa = stage0 + s * stage_bytes;
       const uint64_t da = desc | uint64_t((pa >> 4) & 0x3FFFu);
-      const uint64_t db = desc | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+      const uint64_t db = desc | uint64_t(((pa + panel_bytes) >> 4) & 0x3FFFu);
       const uint32_t id = (uint32_t)(j0 & 3), idesc = a.idesc | (id << 29) | (id << 4);
       if (leader) {
 #pragma unroll
@@ -203,7 +217,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
         mma_commit<1>(empty(s));
       }
       __syncwarp();
-      if (++s == S::kStages) {
+      if (++s == stages) {
         s = 0;
         phase ^= 1u;
       }
@@ -211,20 +225,26 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     }
     if (ok && leader) mma_commit<1>(done);
     __syncwarp();
-  } else if (warp == 6) {
-    int slot = 0;
-    uint32_t phase = 0;
+  } else {
+    // ---- block scales: the writing warps and two more take a group each in turn, as a
+    // group's loads take microseconds behind the weights' in DRAM (one warp, a group
+    // after the other, held a product of 58.7 MB at 18.6 us)
     const bool words_a = scale_words(a.scale_a, a.scale_a_pitch, first);
     const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, first);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     ScaleRows from_a, from_b;
     from_a.at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
     from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, 0, a.n, lane);
-    for (int kb = first; kb < last; kb += 4) {
+    const int groups = (last - first + 3) >> 2;
+    bool waited = false;
+    for (int g = warp < 4 ? warp : warp - 2; g < groups; g += kThinLoaders) {
+      const int slot = g % kThinSlots, kb = first + 4 * g;
       uint32_t w[2][4];
       from_a.read(kb, last, words_a, w[0]);
+      if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
       from_b.read(kb, last, words_b, w[1]);
-      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 1u << 12);
+      ok = barrier_wait(scale_empty(slot), ((uint32_t)(g / kThinSlots) & 1u) ^ 1u, a.status,
+                        1u << 12);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       const uint32_t dst = scales0 + slot * S::kScaleBytes + 16u * lane;
@@ -236,16 +256,13 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) barrier_arrive(map_to_rank(scale_full(slot), rank));
-      if (++slot == kScaleSlots) {
-        slot = 0;
-        phase ^= 1u;
-      }
     }
-    for (int i = 0; i < kScaleSlots && ok; ++i) {
-      ok = barrier_wait(scale_empty(slot), phase ^ 1u, a.status, 1u << 15);
-      if (++slot == kScaleSlots) {
-        slot = 0;
-        phase ^= 1u;
+    if (warp == 6) {
+      for (int i = 0; i < kThinSlots && i < groups && ok; ++i) {
+        // the last copy out of every slot
+        const int g = groups - 1 - i;
+        ok = barrier_wait(scale_empty(g % kThinSlots), (uint32_t)(g / kThinSlots) & 1u, a.status,
+                          1u << 15);
       }
     }
   }
@@ -261,7 +278,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   }
   tmem_fence_after();
   const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
-  const int row = row0 + 32 * warp + lane;
+  const int row = row0 + 32 * warp + lane, row_end = min(a.m, row0 + a.rows);
   if (splits == 1) {
     if (warp < 4 && ok) {
 #pragma unroll
@@ -271,7 +288,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
         tmem_load16(acc + c0, v);
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          if (row < a.m && c0 + c < a.n)
+          if (row < row_end && c0 + c < a.n)
             store_value(a.out, a.out_format, row * a.row_stride + (c0 + c) * a.col_stride,
                         __uint_as_float(v[c]));
       }
@@ -311,7 +328,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
 #pragma unroll
       for (int r = 1; r < 8; ++r)
         if (r < (int)splits) sum = __fadd_rn(sum, part[r]);
-      if (out_row < a.m && ok)
+      if (out_row < row_end && ok)
         store_value(a.out, a.out_format, out_row * a.row_stride + c * a.col_stride, sum);
     }
     cluster_sync();  // the others have read this CTA's sums
