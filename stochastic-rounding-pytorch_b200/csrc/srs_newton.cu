@@ -366,7 +366,7 @@ struct NewtonProducts {
 };
 
 template <int CG>
-__global__ void __launch_bounds__(kProductThreads, 1)
+__global__ void __launch_bounds__(ProductShape<kOperandF16, CG>::kThreads, 1)
 newton_kernel(const __grid_constant__ NewtonWork w) {
   run_products<kOperandF16, CG, true>(NewtonProducts{w});
 }
@@ -497,9 +497,9 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, Ne
 template <int CG>
 int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(&newton_kernel<CG>);
-  constexpr int kSmem = ProductShape<kOperandF16, CG>::kSmem;
+  using S = ProductShape<kOperandF16, CG>;
   int resident = 0;
-  if (int rc = prepare_kernel(kernel, CG, kProductThreads, kSmem, &resident)) return rc;
+  if (int rc = prepare_kernel(kernel, CG, S::kThreads, S::kSmem, &resident)) return rc;
   w.edge = 128 * CG;
   int64_t triangles = 0, grids = 0;
   for (int i = 0; i < w.classes; ++i) {
@@ -519,7 +519,7 @@ int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
   if (triangles >= (1ll << 31) || grids >= (1ll << 31))
     return fail(SRS_ERR_INVALID_ARGUMENT, "too many matrices for one call");
   const int64_t most = triangles > grids ? triangles : grids;
-  return launch_groups(kernel, most < resident ? most : resident, CG, kProductThreads, kSmem, true,
+  return launch_groups(kernel, most < resident ? most : resident, CG, S::kThreads, S::kSmem, true,
                        &w, stream, "newton_kernel launch");
 }
 

@@ -220,7 +220,7 @@ struct BlockSource {
 };
 
 template <int CG>
-__global__ void __launch_bounds__(kProductThreads, 1)
+__global__ void __launch_bounds__(ProductShape<kOperandF8, CG>::kThreads, 1)
 block_product_kernel(const __grid_constant__ BlockProduct w) {
   run_products<kOperandF8, CG, false>(BlockSource{w});
 }
@@ -228,11 +228,11 @@ block_product_kernel(const __grid_constant__ BlockProduct w) {
 template <int CG>
 int launch_blocks(BlockProduct& w, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(&block_product_kernel<CG>);
-  constexpr int kSmem = ProductShape<kOperandF8, CG>::kSmem;
+  using S = ProductShape<kOperandF8, CG>;
   int resident = 0;
-  if (int rc = prepare_kernel(kernel, CG, kProductThreads, kSmem, &resident)) return rc;
+  if (int rc = prepare_kernel(kernel, CG, S::kThreads, S::kSmem, &resident)) return rc;
   const int64_t tiles = (int64_t)w.grid.rows * w.grid.cols;
-  return launch_groups(kernel, tiles < resident ? tiles : resident, CG, kProductThreads, kSmem,
+  return launch_groups(kernel, tiles < resident ? tiles : resident, CG, S::kThreads, S::kSmem,
                        false, &w, stream, "block product launch");
 }
 

@@ -13,10 +13,10 @@
 // and 128 rows of B per slice, 32 KB for 512 cycles of MMA.  The small form (one
 // CTA, 128 x 128) keeps the SMs busy when there are too few large tiles.
 //
-// A CTA has 12 warps: warps 0-7 read the accumulator and write the result (warp w
-// owns TMEM lanes 32 (w % 4) .., one row of the tile per lane, and half of the
-// columns), warp 8 issues the TMA loads, warp 9 the MMAs, warp 10 stages the FP8
-// block scales.  Grids are persistent; the accumulator is double-buffered in TMEM
+// A CTA has 8 or 16 warps that read the accumulator and write the result (warp w owns
+// TMEM lanes 32 (w % 4) .., one row of the tile per lane, and its part of the
+// columns), then one that issues the TMA loads, one for the MMAs and one that stages the
+// FP8 block scales.  Grids are persistent; the accumulator is double-buffered in TMEM
 // so that one tile's result is written while the next is computed.
 //
 // The work comes from a Source: one list of tiles, or several lists (phases), each
@@ -33,8 +33,6 @@
 
 namespace srs {
 
-constexpr int kProductThreads = 384;
-constexpr int kWriters = 8;             // warps that write results
 constexpr int kMaxPhases = 3 * SRS_NEWTON_MAX_STEPS;
 constexpr int kScaleSlots = 3;          // ring of scale groups (each covers 4 slices)
 constexpr int kPieceBytes = 32 * 128;   // a warp's piece of results on its way out
@@ -398,7 +396,12 @@ struct ProductShape {
   // cap: 8192 x 14336 x 4096 429 us, with 256 columns 412 us.)
   static constexpr int kShared = KIND == kOperandF8 && CG == 2 ? 32 : 0;
   static constexpr int kSecond = kTileCols - kShared;
-  static constexpr int kStages = KIND == kOperandF8 ? 5 : 6;  // 5 and 6 measure the same
+  // Writing warps: 16 where phases of few tiles wait for results (orthogonalising 768^2
+  // 134.6 us with 8, 130.6 with 16), 8 where the MMAs hide them (4096^2 1093 us with 8,
+  // 1109 with 16).
+  static constexpr int kWriters = KIND == kOperandF16 && CG == 1 ? 16 : 8;
+  static constexpr int kThreads = 32 * (kWriters + 4);
+  static constexpr int kStages = KIND == kOperandF16 && CG == 2 ? 6 : 5;  // 4 to 6 measure the same
   static constexpr int kScaleBytes = KIND == kOperandF8 ? 512 * (1 + CG) : 0;  // per slot
   static constexpr int kScaleColumn = 480;  // 2 groups of 12 columns (pitch 16)
   static constexpr int kStageBytes = 2 * kPanelBytes;
@@ -446,7 +449,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
     }
     for (int i = 0; i < 2; ++i) {
       barrier_init(acc_full(i), 1);
-      barrier_init(acc_empty(i), kWriters * CG);
+      barrier_init(acc_empty(i), S::kWriters * CG);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       barrier_init(scale_full(i), CG);
@@ -454,7 +457,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) tmem_alloc<CG>(smem_address(&tmem_slot), 512);
+  if (warp == S::kWriters + 1) tmem_alloc<CG>(smem_address(&tmem_slot), 512);
   tmem_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
@@ -466,7 +469,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
   const int phases = src.phases();
   bool ok = true;
 
-  if (warp == 8) {
+  if (warp == S::kWriters) {
     // ---- TMA loads: this CTA's 128 rows of A and of B per slice
     const bool leader = elect_lane();
     int s = 0;
@@ -525,7 +528,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         parity ^= 1u;
       }
     }
-  } else if (warp == 9 && rank == 0) {
+  } else if (warp == S::kWriters + 1 && rank == 0) {
     // ---- MMAs (the pair's leader issues for both CTAs)
     const bool leader = elect_lane();
     int s = 0, slot = 0, count = 0;
@@ -619,7 +622,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         __syncwarp();
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == S::kWriters + 2) {
     if constexpr (KIND == kOperandF8) {
       // ---- block scales: words of 4 consecutive scales (512 elements of k) per row,
       // row r at 16 * (r % 32) + 4 * (r / 32) of its 512-byte group, the order in
@@ -689,10 +692,10 @@ __device__ __forceinline__ void run_products(const Source& src) {
         }
       }
     }
-  } else if (warp < kWriters) {
-    // ---- results: this warp's 32 rows, its half of the tile's 32-column pieces
-    constexpr int kPieces = S::kTileCols / 64;
-    const int half = warp >> 2, quarter = warp & 3;
+  } else if (warp < S::kWriters) {
+    // ---- results: this warp's 32 rows, its part of the tile's 32-column pieces
+    constexpr int kPieces = S::kTileCols / (8 * S::kWriters);
+    const int part = warp >> 2, quarter = warp & 3;
     const uint32_t staged = staged0 + warp * kPieceBytes;
     int count = 0;
     for (int p = 0; p < phases && ok; ++p) {
@@ -712,7 +715,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
             if (!ok) break;
             met = true;
           }
-          load_addend(at, row0 + lane, at.col0 + 32 * half * kPieces, add);
+          load_addend(at, row0 + lane, at.col0 + 32 * part * kPieces, add);
         }
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u);
         ok = __all_sync(0xFFFFFFFFu, ok);
@@ -722,7 +725,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
 #pragma unroll 1
         for (int i = 0; i < kPieces; ++i) {
           // accumulator 0 gives its last (shared) columns first
-          const int c = half * kPieces + ((S::kShared != 0 && acc == 0) ? kPieces - 1 - i : i);
+          const int c = part * kPieces + ((S::kShared != 0 && acc == 0) ? kPieces - 1 - i : i);
           uint32_t v[32];
           tmem_load32(from + 32 * c, v);
           tmem_wait(v);
@@ -741,7 +744,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         // then released to the grid by the last warp.  (The reading side orders them
         // before its copies.)
         __syncwarp();
-        if (lane == 0 && shared_count(&phase_warps[p]) == kWriters - 1u)
+        if (lane == 0 && shared_count(&phase_warps[p]) == S::kWriters - 1u)
           counter_arrive(src.counter(p));
       }
     }
@@ -758,7 +761,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
   tmem_fence_after();
-  if (warp == 9) tmem_free<CG>(tmem, 512);
+  if (warp == S::kWriters + 1) tmem_free<CG>(tmem, 512);
 }
 
 }  // namespace srs
