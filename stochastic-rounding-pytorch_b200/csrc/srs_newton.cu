@@ -228,7 +228,8 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
 struct NewtonClass {
   CUtensorMap along[2];   // X, both copies, as the operands of G
   CUtensorMap across[2];  // X as the operand of X = P X
-  CUtensorMap g, p;
+  CUtensorMap g, p;       // by rows
+  CUtensorMap g_t, p_t;   // by columns
   int m, n, small, tall;
   int long_slices, small_slices;
   TileGrid grid;          // tiles of X
@@ -291,7 +292,7 @@ struct NewtonProducts {
     const NewtonClass& s = w.shape[at.shape];
     const int step = p / 3, kind = p - 3 * step;
     const bool tall = s.tall != 0;
-    TileLoad r;
+    TileLoad r{};
     r.row0 = at.row;
     r.col0 = at.col;
     r.batch = at.batch;
@@ -301,15 +302,18 @@ struct NewtonProducts {
       r.a_rows_inner = r.b_rows_inner = tall;
     } else if (kind == 1) {
       r.map_a = r.map_b = &s.g;
+      r.map_a_t = r.map_b_t = &s.g_t;
       r.slices = s.small_slices;
-      r.a_rows_inner = r.b_rows_inner = false;
+      r.a_symmetric = r.b_symmetric = true;
     } else {
       // P X: P by its rows, X with its row index (the summed one) outer; X P: X by
       // its rows, and P's columns are its rows
       r.map_a = tall ? &s.across[step & 1] : &s.p;
       r.map_b = tall ? &s.p : &s.across[step & 1];
+      r.map_a_t = r.map_b_t = &s.p_t;
       r.slices = s.small_slices;
-      r.a_rows_inner = false;
+      r.a_symmetric = !tall;
+      r.b_symmetric = tall;
       r.b_rows_inner = !tall;
     }
     return r;
@@ -328,7 +332,6 @@ struct NewtonProducts {
     if (kind != 2) {
       const int64_t from = (int64_t)at.batch * s.small_elems;
       r.m = r.n = s.small;
-      r.mirror = at.row != at.col;
       r.pitch = s.small_ld;
       if (kind == 0) {
         r.factor = __fdiv_rn(kHeld, __fmul_rn(rho, rho));
@@ -490,8 +493,12 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, Ne
   }
   const ProductOperand g{c->g_at, s.small, s.small, s.small_ld, s.small_elems, false};
   const ProductOperand p{c->p_at, s.small, s.small, s.small_ld, s.small_elems, false};
+  ProductOperand g_t = g, p_t = p;
+  g_t.rows_inner = p_t.rows_inner = true;
   if (int rc = encode_operand(g, 2, s.batch, 128, &c->g)) return rc;
-  return encode_operand(p, 2, s.batch, 128, &c->p);
+  if (int rc = encode_operand(p, 2, s.batch, 128, &c->p)) return rc;
+  if (int rc = encode_operand(g_t, 2, s.batch, 128, &c->g_t)) return rc;
+  return encode_operand(p_t, 2, s.batch, 128, &c->p_t);
 }
 
 template <int CG>

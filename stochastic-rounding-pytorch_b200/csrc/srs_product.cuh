@@ -47,6 +47,12 @@ struct TileLoad {
   int batch;
   int slices;      // of 128 bytes along k
   bool a_rows_inner, b_rows_inner;
+  // A symmetric operand is stored on and below its diagonal tiles alone: slices of k
+  // past the tile's rows are read from the transposed tiles, with the row index
+  // contiguous (maps map_a_t, map_b_t).
+  bool a_symmetric, b_symmetric;
+  const CUtensorMap* map_a_t;
+  const CUtensorMap* map_b_t;
 };
 
 // What happens to a tile's accumulator.
@@ -54,7 +60,6 @@ struct TileStore {
   int row0, col0;  // in the matrix
   int m, n;        // size of the matrix
   int update;      // 1: Muon's parameter update instead of a store
-  bool mirror;     // symmetric: also store the transposed tile
   float factor;    // of the accumulator
   float beta;      // of `addend`
   float diagonal;  // added where i == j
@@ -346,21 +351,6 @@ __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int 
 #pragma unroll
       for (int i = 0; i < 16; ++i) w[i] = pack_half(value(2 * i), value(2 * i + 1));
     }
-    if (NEWTON && t.mirror) {
-      // Lane pairs swap halves: the even lane gets two rows of an even column, the
-      // odd lane of the next one, so a store covers 2 x 64 bytes.  (An odd last
-      // row writes one padding element beside it.)
-      const int odd = lane & 1;
-      __half* to = reinterpret_cast<__half*>(t.out) + (int64_t)(col0 + odd) * t.pitch + (row & ~1);
-      const int cols = (row & ~1) < t.m ? t.n - col0 - odd : 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i, to += 2 * t.pitch) {
-        const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, w[i], 1);
-        const uint32_t pair =
-            odd ? __byte_perm(other, w[i], 0x7632u) : __byte_perm(w[i], other, 0x5410u);
-        if (2 * i < cols) *reinterpret_cast<uint32_t*>(to) = pair;
-      }
-    }
     stage_row<4>(staged, lane, w);
     __syncwarp();
     store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
@@ -499,15 +489,19 @@ __device__ __forceinline__ void run_products(const Source& src) {
           const int k = i * kSliceK;
           if (leader) {
             if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
-            if (NEWTON && at.a_rows_inner) {
-              load_box<CG>(pa, at.map_a, ra, k, at.batch, bar);
-              load_box<CG>(pa + kPanelBytes / 2, at.map_a, ra + 64, k, at.batch, bar);
+            const bool past_a = NEWTON && at.a_symmetric && k >= at.row0 + S::kTileRows;
+            const bool past_b = NEWTON && at.b_symmetric && k >= at.col0 + S::kTileCols;
+            if (NEWTON && (at.a_rows_inner || past_a)) {
+              const CUtensorMap* map = past_a ? at.map_a_t : at.map_a;
+              load_box<CG>(pa, map, ra, k, at.batch, bar);
+              load_box<CG>(pa + kPanelBytes / 2, map, ra + 64, k, at.batch, bar);
             } else {
               load_box<CG>(pa, at.map_a, k, ra, at.batch, bar);
             }
-            if (NEWTON && at.b_rows_inner) {
-              load_box<CG>(pb, at.map_b, rb, k, at.batch, bar);
-              load_box<CG>(pb + kPanelBytes / 2, at.map_b, rb + 64, k, at.batch, bar);
+            if (NEWTON && (at.b_rows_inner || past_b)) {
+              const CUtensorMap* map = past_b ? at.map_b_t : at.map_b;
+              load_box<CG>(pb, map, rb, k, at.batch, bar);
+              load_box<CG>(pb + kPanelBytes / 2, map, rb + 64, k, at.batch, bar);
             } else {
               load_box<CG>(pb, at.map_b, k, rb, at.batch, bar);
             }
@@ -562,12 +556,6 @@ __device__ __forceinline__ void run_products(const Source& src) {
       const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step, ++count) {
         const TileLoad at = src.load(p, t);
-        const bool a_inner = NEWTON && at.a_rows_inner, b_inner = NEWTON && at.b_rows_inner;
-        const uint64_t desc_a = operand_descriptor(a_inner), desc_b = operand_descriptor(b_inner);
-        // 16-byte units per MMA step of k (32 bytes; 16 rows of 128 bytes when rows are inner)
-        const uint32_t step_a = (a_inner ? 2048u : 32u) >> 4, step_b = (b_inner ? 2048u : 32u) >> 4;
-        const uint32_t base = S::kInstruction | src.formats() | (a_inner ? 1u << 15 : 0u) |
-                              (b_inner ? 1u << 16 : 0u);
         const int groups = (at.slices + 3) >> 2;
         const int acc = count & 1;
         const uint32_t d = tmem + acc * S::kSecond;
@@ -585,8 +573,18 @@ __device__ __forceinline__ void run_products(const Source& src) {
           tmem_fence_after();
           const uint32_t scale_tmem = tmem + S::kScaleColumn + 16u * (group & 1u);
           const uint32_t pa = stage0 + s * S::kStageBytes;
-          const uint64_t da = desc_a | uint64_t((pa >> 4) & 0x3FFFu);
-          const uint64_t db = desc_b | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+          const int k = i * kSliceK;
+          const bool a_inner = NEWTON && (at.a_rows_inner ||
+                                          (at.a_symmetric && k >= at.row0 + S::kTileRows));
+          const bool b_inner = NEWTON && (at.b_rows_inner ||
+                                          (at.b_symmetric && k >= at.col0 + S::kTileCols));
+          const uint64_t da = operand_descriptor(a_inner) | uint64_t((pa >> 4) & 0x3FFFu);
+          const uint64_t db =
+              operand_descriptor(b_inner) | uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+          // 16-byte units per MMA step of k (32 bytes; 16 rows of 128 bytes when rows are inner)
+          const uint32_t step_a = (a_inner ? 2048u : 32u) >> 4, step_b = (b_inner ? 2048u : 32u) >> 4;
+          const uint32_t base = S::kInstruction | src.formats() | (a_inner ? 1u << 15 : 0u) |
+                                (b_inner ? 1u << 16 : 0u);
           const uint32_t id = (uint32_t)(i & 3);
           const uint32_t idesc = KIND == kOperandF8 ? base | (id << 29) | (id << 4) : base;
           if (leader) {
