@@ -298,12 +298,13 @@ int srs_derive_keys(const uint32_t* param_index, uint32_t* out, int64_t n, const
  * No counterpart in the reference.  y = X_steps of
  *   X_0 = x / (|x|_F + eps);  X_{i+1} = (a I + b G + c G^2) X_i,  G = X_i X_i^T
  * for `batch` matrices of m rows and n columns (m > n: X_{i+1} = X_i (a I + b G + c G^2),
- * G = X_i^T X_i).  Products on the tensor cores: FP16 operands, FP32 sums; the
- * norm is summed in FP64.  x: FP32, BF16 or FP16, element (b, i, j) at
+ * G = X_i^T X_i).  Products on the tensor cores with FP32 sums: FP16 operands for y in
+ * BF16 (errors of about 1e-3), pairs of FP16 operands for y in FP32 or FP16 (1e-5 for
+ * sides of some hundreds, 1e-4 for ten thousand; three times the work); the norm is summed in FP64.  x: FP32, BF16 or FP16, element (b, i, j) at
  * b * batch_stride + i * row_pitch + j; y: contiguous, FP32, BF16 or FP16; x and y
  * must not overlap.  A matrix with a NaN or infinity, or whose norm plus eps is
  * zero, gives NaN throughout.  Sizes of zero are a no-op.
- * `workspace`: srs_newton_workspace(batch, m, n) bytes, 256-byte aligned, not used
+ * `workspace`: srs_newton_workspace(batch, m, n, y_format) bytes, 256-byte aligned, not used
  * by any other call that can overlap in time. */
 #define SRS_NEWTON_MAX_STEPS 32
 typedef struct srs_newton {
@@ -312,7 +313,7 @@ typedef struct srs_newton {
   float eps;
 } srs_newton;
 
-int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n);
+int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n, int y_format);
 
 int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch, int64_t batch_stride,
                       void* y, int y_format, int64_t batch, int64_t m, int64_t n,

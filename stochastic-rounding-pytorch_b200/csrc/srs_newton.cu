@@ -23,6 +23,13 @@
 // the remaining factor rho enters the first products in FP32.  The norm is
 // summed in FP64, so no input in range overflows or vanishes in it.
 //
+// Results in FP32 or FP16 hold more digits than that.  For them every held matrix is
+// the sum of two FP16 matrices, what the first leaves of a value in the second, and a
+// product of two such is high by high + high by low + low by high: three times the
+// MMAs, errors from 4e-6 (128 x 512) to 1.3e-4 (4096 x 14336; the tensor core truncates
+// its FP32 sums, so they grow with the sides) (SPLIT).  X is then held times 2^t, about sqrt of its
+// longer side, so that the second matrices stay clear of FP16's smallest numbers.
+//
 // Three launches: the norm, X_0, and one cooperative grid that runs the 3 * steps
 // products of all matrices, whatever their shapes, as phases with a grid-wide
 // meeting between them (a launch a product took 7 us each where the products
@@ -64,6 +71,7 @@ struct NewtonSource {
   int chunks;         // partial sums of one matrix
   int target;         // floor(log2(sqrt(min(m, n))))
   __half* x0;
+  int64_t low;        // elements from X_0 to its low part (0: none)
   int64_t ld, x_elems;
   float* rho;
 };
@@ -219,37 +227,52 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
     encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
     const Unit at = unit_of(s, u, s.ld);
     *reinterpret_cast<uint4*>(out + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (U == kPlain && s.low != 0) {
+      float high[kVec];
+      decode8<SRS_FMT_F16>(w, high);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[i] -= high[i];
+      encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
+      *reinterpret_cast<uint4*>(out + s.low + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
 // ------------------------------------------------------------------ products --
 
-// Matrices of one shape in the product grid.
+// Matrices of one shape in the product grid.  SPLIT: every map is followed by that of
+// the matrix's low part.
+template <bool SPLIT>
 struct NewtonClass {
-  CUtensorMap along[2];   // X, both copies, as the operands of G
-  CUtensorMap across[2];  // X as the operand of X = P X
-  CUtensorMap g, p;       // by rows
-  CUtensorMap g_t, p_t;   // by columns
+  static constexpr int kParts = SPLIT ? 2 : 1;
+  CUtensorMap along[2][kParts];   // X, both copies, as the operands of G
+  CUtensorMap across[2][kParts];  // X as the operand of X = P X
+  CUtensorMap g[kParts], p[kParts];      // by rows
+  CUtensorMap g_t[kParts], p_t[kParts];  // by columns
   int m, n, small, tall;
   int long_slices, small_slices;
   TileGrid grid;          // tiles of X
   Divider each_triangle;  // tiles of one G or P
   Divider each_grid;      // tiles of one X
   int64_t ld, x_elems, small_ld, small_elems;
+  int64_t x_low, small_low;  // SPLIT: bytes from a matrix to its low part
   __half* x[2];
   __half* g_at;
   __half* p_at;
   const float* rho;
+  float held;            // X is held times this after the first step
   char* out;             // orthogonalize: the result, contiguous matrices
   int out_format;
   const srs_row* rows;   // Muon: the parameters
   float step, decay;
 };
 
+template <bool SPLIT>
 struct NewtonWork {
-  NewtonClass shape[kMaxClasses];
-  uint32_t triangles[kMaxClasses + 1];  // first tile of each class in a G or P phase
-  uint32_t grids[kMaxClasses + 1];      // ... in an X phase
+  static constexpr int kClasses = SPLIT ? 1 : kMaxClasses;
+  NewtonClass<SPLIT> shape[kClasses];
+  uint32_t triangles[kClasses + 1];  // first tile of each class in a G or P phase
+  uint32_t grids[kClasses + 1];      // ... in an X phase
   int classes, steps, edge;
   float a, b, c;
   unsigned int* counters;  // one a phase
@@ -257,8 +280,9 @@ struct NewtonWork {
 };
 
 // Phase 3 i: G = X X^T; 3 i + 1: P = a I + b G + c G G; 3 i + 2: X = P X.
+template <bool SPLIT>
 struct NewtonProducts {
-  const NewtonWork& w;
+  const NewtonWork<SPLIT>& w;
   struct Place {
     int shape, batch, row, col;
   };
@@ -276,7 +300,7 @@ struct NewtonProducts {
     r.shape = 0;
     while (t >= begin[r.shape + 1]) ++r.shape;
     t -= begin[r.shape];
-    const NewtonClass& s = w.shape[r.shape];
+    const NewtonClass<SPLIT>& s = w.shape[r.shape];
     const Divider& each = grid ? s.each_grid : s.each_triangle;
     const uint32_t batch = each.quotient(t);
     r.batch = (int)batch;
@@ -289,7 +313,7 @@ struct NewtonProducts {
   }
   __device__ TileLoad load(int p, uint32_t t) const {
     const Place at = place(p, t);
-    const NewtonClass& s = w.shape[at.shape];
+    const NewtonClass<SPLIT>& s = w.shape[at.shape];
     const int step = p / 3, kind = p - 3 * step;
     const bool tall = s.tall != 0;
     TileLoad r{};
@@ -297,42 +321,44 @@ struct NewtonProducts {
     r.col0 = at.col;
     r.batch = at.batch;
     if (kind == 0) {
-      r.map_a = r.map_b = &s.along[step & 1];
+      r.map_a = r.map_b = s.along[step & 1];
       r.slices = s.long_slices;
       r.a_rows_inner = r.b_rows_inner = tall;
     } else if (kind == 1) {
-      r.map_a = r.map_b = &s.g;
-      r.map_a_t = r.map_b_t = &s.g_t;
+      r.map_a = r.map_b = s.g;
+      r.map_a_t = r.map_b_t = s.g_t;
       r.slices = s.small_slices;
       r.a_symmetric = r.b_symmetric = true;
     } else {
       // P X: P by its rows, X with its row index (the summed one) outer; X P: X by
       // its rows, and P's columns are its rows
-      r.map_a = tall ? &s.across[step & 1] : &s.p;
-      r.map_b = tall ? &s.p : &s.across[step & 1];
-      r.map_a_t = r.map_b_t = &s.p_t;
+      r.map_a = tall ? s.across[step & 1] : s.p;
+      r.map_b = tall ? s.p : s.across[step & 1];
+      r.map_a_t = r.map_b_t = s.p_t;
       r.slices = s.small_slices;
       r.a_symmetric = !tall;
       r.b_symmetric = tall;
       r.b_rows_inner = !tall;
     }
+    if (SPLIT) r.slices *= 3;
     return r;
   }
   __device__ TileStore store(int p, uint32_t t) const {
     const Place at = place(p, t);
-    const NewtonClass& s = w.shape[at.shape];
+    const NewtonClass<SPLIT>& s = w.shape[at.shape];
     const int step = p / 3, kind = p - 3 * step;
     TileStore r{};
     r.row0 = at.row;
     r.col0 = at.col;
-    // The first step's operand stands for X / rho.
-    float rho = 1.0f;
+    // The first step's operand stands for X / rho, the others for X / held.
+    float rho = s.held;
     if (step == 0 && kind != 1) rho = s.rho[at.batch];
     r.format = SRS_FMT_F16;
     if (kind != 2) {
       const int64_t from = (int64_t)at.batch * s.small_elems;
       r.m = r.n = s.small;
       r.pitch = s.small_ld;
+      r.low = s.small_low;
       if (kind == 0) {
         r.factor = __fdiv_rn(kHeld, __fmul_rn(rho, rho));
         r.out = reinterpret_cast<char*>(s.g_at + from);
@@ -348,7 +374,9 @@ struct NewtonProducts {
       r.n = s.n;
       r.factor = __fdiv_rn(1.0f / kHeld, rho);
       if (step + 1 < w.steps) {
+        r.factor *= s.held;
         r.pitch = s.ld;
+        r.low = s.x_low;
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
       } else if (s.rows != nullptr) {
         const srs_row& row = s.rows[at.batch];
@@ -368,10 +396,10 @@ struct NewtonProducts {
   }
 };
 
-template <int CG>
+template <int CG, bool SPLIT>
 __global__ void __launch_bounds__(ProductShape<kOperandF16, CG>::kThreads, 1)
-newton_kernel(const __grid_constant__ NewtonWork w) {
-  run_products<kOperandF16, CG, true>(NewtonProducts{w});
+newton_kernel(const __grid_constant__ NewtonWork<SPLIT> w) {
+  run_products<kOperandF16, CG, true, SPLIT>(NewtonProducts<SPLIT>{w});
 }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -380,7 +408,8 @@ int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 // and G and P, each aligned to 256 bytes.
 struct NewtonShape {
   int64_t batch, m, n, small, ld, small_ld, x_elems, small_elems;
-  int64_t rho, x[2], g, p;  // byte offsets
+  int64_t x_low, small_low;  // bytes from a matrix to its low part (0: none)
+  int64_t rho, x[2], g, p;   // byte offsets
 };
 
 // Rows on 128-byte boundaries, so that a box's 128-byte rows are whole cache lines
@@ -394,7 +423,7 @@ int64_t take(int64_t* at, int64_t bytes) {
   return here;
 }
 
-NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, int64_t* at) {
+NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, bool split, int64_t* at) {
   NewtonShape s{};
   s.batch = batch;
   s.m = m;
@@ -404,11 +433,15 @@ NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, int64_t* at) {
   s.small_ld = row_pitch_of(s.small);
   s.x_elems = m * s.ld;
   s.small_elems = s.small * s.small_ld;
+  const int64_t x_bytes = round_up(batch * s.x_elems * 2, 256);
+  const int64_t small_bytes = round_up(batch * s.small_elems * 2, 256);
+  s.x_low = split ? x_bytes : 0;
+  s.small_low = split ? small_bytes : 0;
   s.rho = take(at, batch * 4);
-  s.x[0] = take(at, batch * s.x_elems * 2);
-  s.x[1] = take(at, batch * s.x_elems * 2);
-  s.g = take(at, batch * s.small_elems * 2);
-  s.p = take(at, batch * s.small_elems * 2);
+  s.x[0] = take(at, x_bytes + s.x_low);
+  s.x[1] = take(at, x_bytes + s.x_low);
+  s.g = take(at, small_bytes + s.small_low);
+  s.p = take(at, small_bytes + s.small_low);
   return s;
 }
 
@@ -453,15 +486,29 @@ void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
   if (chunks > most) chunks = most;
   if (chunks > kSumChunks) chunks = kSumChunks;
   f->chunks = chunks < 1 ? 1 : (int)chunks;
+  // SPLIT holds X_0 with elements of about 1, as the later X.
+  const int64_t size = s.x_low != 0 ? s.m * s.n : s.small;
   f->target = 0;
-  while ((1ll << (2 * (f->target + 1))) <= s.small) ++f->target;
+  while (f->target < 15 && (1ll << (2 * (f->target + 1))) <= size) ++f->target;
   f->x0 = reinterpret_cast<__half*>(space + s.x[0]);
+  f->low = s.x_low / 2;
   f->ld = s.ld;
   f->x_elems = s.x_elems;
   f->rho = reinterpret_cast<float*>(space + s.rho);
 }
 
-int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, NewtonClass* c) {
+// The map of a matrix and, for SPLIT, that of its low part behind it.
+template <bool SPLIT>
+int encode_parts(ProductOperand o, int64_t low, int64_t batch, CUtensorMap* maps) {
+  if (int rc = encode_operand(o, 2, batch, 128, &maps[0])) return rc;
+  if (!SPLIT) return SRS_OK;
+  o.base = static_cast<const char*>(o.base) + low;
+  return encode_operand(o, 2, batch, 128, &maps[1]);
+}
+
+template <bool SPLIT>
+int fill_class(const NewtonShape& s, char* space, const NewtonResult& result,
+               NewtonClass<SPLIT>* c) {
   const bool tall = s.m > s.n;
   const int64_t longer = tall ? s.m : s.n;
   c->m = (int)s.m;
@@ -474,9 +521,16 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, Ne
   c->x_elems = s.x_elems;
   c->small_ld = s.small_ld;
   c->small_elems = s.small_elems;
+  c->x_low = s.x_low;
+  c->small_low = s.small_low;
   c->g_at = reinterpret_cast<__half*>(space + s.g);
   c->p_at = reinterpret_cast<__half*>(space + s.p);
   c->rho = reinterpret_cast<const float*>(space + s.rho);
+  c->held = 1.0f;
+  if (SPLIT) {
+    // at most 2^13: |X| stays below a few units, FP16 ends at 65504
+    while (c->held < 8192.0f && 4.0f * c->held * c->held <= (float)longer) c->held *= 2.0f;
+  }
   c->out = static_cast<char*>(result.out);
   c->out_format = result.out_format;
   c->rows = result.rows;
@@ -488,29 +542,28 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result, Ne
     // sums along the shorter one
     const ProductOperand along{c->x[i], s.small, longer, s.ld, s.x_elems, tall};
     const ProductOperand across{c->x[i], longer, s.small, s.ld, s.x_elems, !tall};
-    if (int rc = encode_operand(along, 2, s.batch, 128, &c->along[i])) return rc;
-    if (int rc = encode_operand(across, 2, s.batch, 128, &c->across[i])) return rc;
+    if (int rc = encode_parts<SPLIT>(along, s.x_low, s.batch, c->along[i])) return rc;
+    if (int rc = encode_parts<SPLIT>(across, s.x_low, s.batch, c->across[i])) return rc;
   }
-  const ProductOperand g{c->g_at, s.small, s.small, s.small_ld, s.small_elems, false};
-  const ProductOperand p{c->p_at, s.small, s.small, s.small_ld, s.small_elems, false};
-  ProductOperand g_t = g, p_t = p;
-  g_t.rows_inner = p_t.rows_inner = true;
-  if (int rc = encode_operand(g, 2, s.batch, 128, &c->g)) return rc;
-  if (int rc = encode_operand(p, 2, s.batch, 128, &c->p)) return rc;
-  if (int rc = encode_operand(g_t, 2, s.batch, 128, &c->g_t)) return rc;
-  return encode_operand(p_t, 2, s.batch, 128, &c->p_t);
+  ProductOperand g{c->g_at, s.small, s.small, s.small_ld, s.small_elems, false};
+  ProductOperand p{c->p_at, s.small, s.small, s.small_ld, s.small_elems, false};
+  if (int rc = encode_parts<SPLIT>(g, s.small_low, s.batch, c->g)) return rc;
+  if (int rc = encode_parts<SPLIT>(p, s.small_low, s.batch, c->p)) return rc;
+  g.rows_inner = p.rows_inner = true;
+  if (int rc = encode_parts<SPLIT>(g, s.small_low, s.batch, c->g_t)) return rc;
+  return encode_parts<SPLIT>(p, s.small_low, s.batch, c->p_t);
 }
 
-template <int CG>
-int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
-  const void* kernel = reinterpret_cast<const void*>(&newton_kernel<CG>);
+template <int CG, bool SPLIT>
+int launch_newton(NewtonWork<SPLIT>& w, const int64_t* batch, cudaStream_t stream) {
+  const void* kernel = reinterpret_cast<const void*>(&newton_kernel<CG, SPLIT>);
   using S = ProductShape<kOperandF16, CG>;
   int resident = 0;
   if (int rc = prepare_kernel(kernel, CG, S::kThreads, S::kSmem, &resident)) return rc;
   w.edge = 128 * CG;
   int64_t triangles = 0, grids = 0;
   for (int i = 0; i < w.classes; ++i) {
-    NewtonClass& c = w.shape[i];
+    NewtonClass<SPLIT>& c = w.shape[i];
     const uint32_t edge = (uint32_t)((c.small + w.edge - 1) / w.edge);
     c.each_triangle = make_divider(edge * (edge + 1) / 2);
     c.grid = make_grid((uint32_t)((c.m + w.edge - 1) / w.edge),
@@ -535,7 +588,8 @@ int launch_newton(NewtonWork& w, const int64_t* batch, cudaStream_t stream) {
 // the loads for it), and what a tile's results take.  Measured (us, single against
 // pair): 1024^2 144, 201; 2048^2 241, 285; 2500^2 422, 390; 3500^2 894, 783;
 // 16 x 768^2 295, 367; 24 x 768^2 402, 365; 4 x (1024 x 4096) 347, 381.
-double step_cycles(const NewtonWork& w, const int64_t* batch, int cg) {
+template <bool SPLIT>
+double step_cycles(const NewtonWork<SPLIT>& w, const int64_t* batch, int cg) {
   const int64_t groups = sm_count() / cg;
   const double slice = cg == 2 ? 512.0 : 350.0, rest = cg == 2 ? 5000.0 : 2000.0;
   double total = 0.0;
@@ -543,11 +597,12 @@ double step_cycles(const NewtonWork& w, const int64_t* batch, int cg) {
     double work = 0.0, longest = 0.0;
     int64_t tiles = 0;
     for (int i = 0; i < w.classes; ++i) {
-      const NewtonClass& c = w.shape[i];
+      const NewtonClass<SPLIT>& c = w.shape[i];
       const int64_t edge = 128 * cg, t = (c.small + edge - 1) / edge;
       const int64_t each = kind < 2 ? t * (t + 1) / 2
                                     : (c.m + edge - 1) / edge * ((c.n + edge - 1) / edge);
-      const double cycles = slice * (kind == 0 ? c.long_slices : c.small_slices) + rest;
+      const double cycles =
+          (SPLIT ? 3.0 : 1.0) * slice * (kind == 0 ? c.long_slices : c.small_slices) + rest;
       tiles += batch[i] * each;
       work += cycles * (double)(batch[i] * each);
       if (cycles > longest) longest = cycles;
@@ -560,7 +615,8 @@ double step_cycles(const NewtonWork& w, const int64_t* batch, int cg) {
   return total;
 }
 
-int run_newton(NewtonWork& w, const int64_t* batch, const srs_newton* h, unsigned int* counters,
+template <bool SPLIT>
+int run_newton(NewtonWork<SPLIT>& w, const int64_t* batch, const srs_newton* h, unsigned int* counters,
                cudaStream_t stream) {
   w.steps = h->steps;
   w.a = h->coefficients[0];
@@ -568,8 +624,9 @@ int run_newton(NewtonWork& w, const int64_t* batch, const srs_newton* h, unsigne
   w.c = h->coefficients[2];
   w.counters = counters;
   if (int rc = status_word(&w.status_at)) return rc;
-  return step_cycles(w, batch, 2) <= step_cycles(w, batch, 1) ? launch_newton<2>(w, batch, stream)
-                                                              : launch_newton<1>(w, batch, stream);
+  return step_cycles(w, batch, 2) <= step_cycles(w, batch, 1)
+             ? launch_newton<2, SPLIT>(w, batch, stream)
+             : launch_newton<1, SPLIT>(w, batch, stream);
 }
 
 int check_matrices(int64_t batch, int64_t m, int64_t n) {
@@ -610,11 +667,11 @@ int check_space(const void* space, int64_t bytes, int64_t need) {
 
 using namespace srs;
 
-extern "C" int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n) {
+extern "C" int64_t srs_newton_workspace(int64_t batch, int64_t m, int64_t n, int y_format) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
   int64_t at = 0;
   lay_out_head(batch, &at);
-  lay_out(batch, m, n, &at);
+  lay_out(batch, m, n, y_format != SRS_FMT_BF16, &at);
   return at;
 }
 
@@ -637,14 +694,14 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   if (at % fmt_bytes(x_format) != 0 ||
       reinterpret_cast<uintptr_t>(y) % fmt_bytes(y_format) != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "input/output pointers are not element aligned");
-  if (int rc = check_space(workspace, workspace_bytes, srs_newton_workspace(batch, m, n)))
+  if (int rc = check_space(workspace, workspace_bytes, srs_newton_workspace(batch, m, n, y_format)))
     return rc;
   if (int rc = check_device()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* space = static_cast<char*>(workspace);
   int64_t used = 0;
   const int64_t partial = lay_out_head(batch, &used);
-  const NewtonShape shape = lay_out(batch, m, n, &used);
+  const NewtonShape shape = lay_out(batch, m, n, y_format != SRS_FMT_BF16, &used);
   NewtonPlan plan{};
   plan.classes = 1;
   plan.partial = reinterpret_cast<double*>(space + partial);
@@ -657,12 +714,19 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   s.batch_stride = batch_stride;
   s.vec = at % 16 == 0 && row_pitch % 8 == 0 && batch_stride % 8 == 0;
   fill_source(shape, space, 0, batch, &s);
-  NewtonWork work{};
-  work.classes = 1;
   const NewtonResult result{y, y_format, nullptr, 0.0f, 0.0f};
-  if (int rc = fill_class(shape, space, result, &work.shape[0])) return rc;
-  if (int rc = launch_prepare<kPlain>(plan, batch, s.chunks, st)) return rc;
-  return run_newton(work, &batch, h, plan.counters, st);
+  const auto run = [&](auto& work) {
+    work.classes = 1;
+    if (int rc = fill_class(shape, space, result, &work.shape[0])) return rc;
+    if (int rc = launch_prepare<kPlain>(plan, batch, s.chunks, st)) return rc;
+    return run_newton(work, &batch, h, plan.counters, st);
+  };
+  if (y_format != SRS_FMT_BF16) {
+    NewtonWork<true> work{};
+    return run(work);
+  }
+  NewtonWork<false> work{};
+  return run(work);
 }
 
 static int check_classes(const srs_muon_class* classes, int n_classes, int64_t* matrices) {
@@ -690,7 +754,7 @@ extern "C" int64_t srs_muon_workspace(const srs_muon_class* classes, int n_class
   if (check_classes(classes, n_classes, &matrices) != SRS_OK) return -1;
   if (n_classes == 0) return 0;
   lay_out_head(matrices, &at);
-  for (int i = 0; i < n_classes; ++i) lay_out(classes[i].count, classes[i].m, classes[i].n, &at);
+  for (int i = 0; i < n_classes; ++i) lay_out(classes[i].count, classes[i].m, classes[i].n, false, &at);
   return at;
 }
 
@@ -728,13 +792,13 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
   plan.momentum = hp->momentum;
   plan.nesterov = hp->nesterov;
   plan.u_rule = u_rule;
-  NewtonWork work{};
+  NewtonWork<false> work{};
   work.classes = n_classes;
   int64_t batch[kMaxClasses];
   int first = 0, chunks = 1;
   for (int i = 0; i < n_classes; ++i) {
     const srs_muon_class& c = classes[i];
-    const NewtonShape shape = lay_out(c.count, c.m, c.n, &used);
+    const NewtonShape shape = lay_out(c.count, c.m, c.n, false, &used);
     NewtonSource& s = plan.source[i];
     s.rows = rows + c.first;
     fill_source(shape, space, first, matrices, &s);

@@ -222,7 +222,7 @@ struct BlockSource {
 template <int CG>
 __global__ void __launch_bounds__(ProductShape<kOperandF8, CG>::kThreads, 1)
 block_product_kernel(const __grid_constant__ BlockProduct w) {
-  run_products<kOperandF8, CG, false>(BlockSource{w});
+  run_products<kOperandF8, CG, false, false>(BlockSource{w});
 }
 
 template <int CG>

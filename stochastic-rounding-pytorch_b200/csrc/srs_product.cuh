@@ -53,6 +53,11 @@ struct TileLoad {
   bool a_symmetric, b_symmetric;
   const CUtensorMap* map_a_t;
   const CUtensorMap* map_b_t;
+  // SPLIT: an operand is the sum of two FP16 matrices, high and low, whose maps lie
+  // beside one another ([0] and [1] of every pointer above).  `slices` counts k three
+  // times: low by high, high by low, then high by high parts.  (The tensor core truncates
+  // its FP32 sums at every step: the small parts go first, while the sum is small;
+  // 4096 x 14336 to FP32 is 1.3e-4 off, with the high parts first 2.5e-4.)
 };
 
 // What happens to a tile's accumulator.
@@ -65,6 +70,7 @@ struct TileStore {
   float diagonal;  // added where i == j
   const __half* addend;  // m x n, row pitch `pitch` (null: none)
   char* out;       // first element of the matrix (update: of the parameter)
+  int64_t low;     // SPLIT: bytes from a 16-bit result (and addend) to its low part; 0: none
   int format;      // SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t pitch;   // elements
   float step, decay;  // update: p' = fma(step, D, p * decay)
@@ -310,8 +316,8 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
 // 8).  Written by an earlier phase of the same kernel: never through the
 // non-coherent path.
 __device__ __forceinline__ void load_addend(const TileStore& t, int row, int col0,
-                                            uint4 (&add)[4]) {
-  const __half* from = t.addend + (int64_t)row * t.pitch + col0;
+                                            uint4 (&add)[4], int64_t bytes = 0) {
+  const char* from = reinterpret_cast<const char*>(t.addend + (int64_t)row * t.pitch + col0) + bytes;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     add[j] = (row < t.m && col0 + 8 * j < t.pitch)
@@ -322,7 +328,7 @@ __device__ __forceinline__ void load_addend(const TileStore& t, int row, int col
 // 32 accumulator columns from col0 on for a warp's 32 rows from row0 on: v[c] is
 // column col0 + c of row row0 + lane.  `add` holds the addend's piece; the next piece's
 // (next_col, -1: none) is requested before this one is stored.
-template <bool NEWTON>
+template <bool NEWTON, bool SPLIT>
 __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int col0, int lane,
                                               uint32_t staged, uint32_t (&v)[32],
                                               uint4 (&add)[4], int next_col) {
@@ -334,15 +340,26 @@ __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int 
   if (t.format != SRS_FMT_F32 && !(NEWTON && t.update != 0)) {
     uint32_t w[16];
     if (NEWTON && t.addend != nullptr) {
-      const uint32_t* pairs = reinterpret_cast<const uint32_t*>(add);
+      const auto accumulate = [&](const uint4 (&part)[4]) {
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(part);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 g = f16x2_to_float2(pairs[i]);
-        const int col = col0 + 2 * i;
-        w[i] = pack_half(fmaf(t.beta, g.x, value(2 * i)) + (row == col ? t.diagonal : 0.0f),
-                         fmaf(t.beta, g.y, value(2 * i + 1)) +
-                             (row == col + 1 ? t.diagonal : 0.0f));
+        for (int i = 0; i < 16; ++i) {
+          const float2 g = f16x2_to_float2(pairs[i]);
+          v[2 * i] = __float_as_uint(fmaf(t.beta, g.x, value(2 * i)));
+          v[2 * i + 1] = __float_as_uint(fmaf(t.beta, g.y, value(2 * i + 1)));
+        }
+      };
+      accumulate(add);
+      if (SPLIT) {
+        uint4 low[4];
+        load_addend(t, row, col0, low, t.low);
+        accumulate(low);
       }
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (row == col0 + i) v[i] = __float_as_uint(value(i) + t.diagonal);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack_half(value(2 * i), value(2 * i + 1));
       if (next_col >= 0) load_addend(t, row, next_col, add);
     } else if (t.format == SRS_FMT_BF16) {
 #pragma unroll
@@ -354,6 +371,18 @@ __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int 
     stage_row<4>(staged, lane, w);
     __syncwarp();
     store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
+    if (SPLIT && t.low != 0) {
+      // what the high part leaves of the value (exact in FP32)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 high = f16x2_to_float2(w[i]);
+        w[i] = pack_half(value(2 * i) - high.x, value(2 * i + 1) - high.y);
+      }
+      __syncwarp();
+      stage_row<4>(staged, lane, w);
+      __syncwarp();
+      store_piece<4>(staged, t.out + t.low + 2 * at, t.pitch, rows, t.n - col0, lane);
+    }
   } else {
     stage_row<8>(staged, lane, v);
     __syncwarp();
@@ -407,7 +436,7 @@ struct ProductShape {
 // The CTA's work.  Source gives: phases(), tiles(phase), load(phase, tile),
 // store(phase, tile), formats() (bits of the instruction descriptor), counter(phase)
 // and status(); for FP8 also scales(): the operands' block scales.
-template <int KIND, int CG, bool NEWTON, class Source>
+template <int KIND, int CG, bool NEWTON, bool SPLIT, class Source>
 __device__ __forceinline__ void run_products(const Source& src) {
   using S = ProductShape<KIND, CG>;
   constexpr int kStages = S::kStages;
@@ -481,29 +510,32 @@ __device__ __forceinline__ void run_products(const Source& src) {
       for (uint32_t t = first; t < tiles && ok; t += step) {
         if (t != first) at = src.load(p, t);
         const int ra = at.row0 + 128 * (int)rank, rb = at.col0 + 128 * (int)rank;
+        const int third = SPLIT ? at.slices / 3 : 0;
         for (int i = 0; i < at.slices; ++i) {
           ok = barrier_wait(empty(s), parity ^ 1u, status, 1u);
           if (!ok) break;
           const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
           const uint32_t pa = stage0 + s * S::kStageBytes, pb = pa + kPanelBytes;
-          const int k = i * kSliceK;
+          const int part = SPLIT ? (i >= third) + (i >= 2 * third) : 0;
+          const int k = (i - part * third) * kSliceK;
+          const int low_a = SPLIT && part == 0 ? 1 : 0, low_b = SPLIT && part == 1 ? 1 : 0;
           if (leader) {
             if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
             const bool past_a = NEWTON && at.a_symmetric && k >= at.row0 + S::kTileRows;
             const bool past_b = NEWTON && at.b_symmetric && k >= at.col0 + S::kTileCols;
             if (NEWTON && (at.a_rows_inner || past_a)) {
-              const CUtensorMap* map = past_a ? at.map_a_t : at.map_a;
+              const CUtensorMap* map = (past_a ? at.map_a_t : at.map_a) + low_a;
               load_box<CG>(pa, map, ra, k, at.batch, bar);
               load_box<CG>(pa + kPanelBytes / 2, map, ra + 64, k, at.batch, bar);
             } else {
-              load_box<CG>(pa, at.map_a, k, ra, at.batch, bar);
+              load_box<CG>(pa, at.map_a + low_a, k, ra, at.batch, bar);
             }
             if (NEWTON && (at.b_rows_inner || past_b)) {
-              const CUtensorMap* map = past_b ? at.map_b_t : at.map_b;
+              const CUtensorMap* map = (past_b ? at.map_b_t : at.map_b) + low_b;
               load_box<CG>(pb, map, rb, k, at.batch, bar);
               load_box<CG>(pb + kPanelBytes / 2, map, rb + 64, k, at.batch, bar);
             } else {
-              load_box<CG>(pb, at.map_b, k, rb, at.batch, bar);
+              load_box<CG>(pb, at.map_b + low_b, k, rb, at.batch, bar);
             }
           }
           __syncwarp();
@@ -556,6 +588,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
       const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step, ++count) {
         const TileLoad at = src.load(p, t);
+        const int third = SPLIT ? at.slices / 3 : 0;
         const int groups = (at.slices + 3) >> 2;
         const int acc = count & 1;
         const uint32_t d = tmem + acc * S::kSecond;
@@ -573,7 +606,8 @@ __device__ __forceinline__ void run_products(const Source& src) {
           tmem_fence_after();
           const uint32_t scale_tmem = tmem + S::kScaleColumn + 16u * (group & 1u);
           const uint32_t pa = stage0 + s * S::kStageBytes;
-          const int k = i * kSliceK;
+          const int part = SPLIT ? (i >= third) + (i >= 2 * third) : 0;
+          const int k = (i - part * third) * kSliceK;
           const bool a_inner = NEWTON && (at.a_rows_inner ||
                                           (at.a_symmetric && k >= at.row0 + S::kTileRows));
           const bool b_inner = NEWTON && (at.b_rows_inner ||
@@ -733,7 +767,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
             if (lane == 0) barrier_arrive_relaxed(map_to_rank(acc_empty(acc), 0));
           }
           if (row0 < at.m && at.col0 + 32 * c < at.n)
-            write_columns<NEWTON>(at, row0, at.col0 + 32 * c, lane, staged, v, add,
+            write_columns<NEWTON, SPLIT>(at, row0, at.col0 + 32 * c, lane, staged, v, add,
                                   i + 1 < kPieces ? at.col0 + 32 * (c + 1) : -1);
         }
       }

@@ -154,7 +154,8 @@ _SIGNATURES = {
     "srs_ipc_export": ([_P, _P, ctypes.POINTER(ctypes.c_uint64)], ctypes.c_int),
     "srs_ipc_import": ([_P, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "srs_ipc_close": ([_P], ctypes.c_int),
-    "srs_newton_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+    "srs_newton_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int],
+                             ctypes.c_int64),
     "srs_orthogonalize": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int,
                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                            ctypes.POINTER(SrsNewton), _P, ctypes.c_int64, _P], ctypes.c_int),
@@ -352,8 +353,8 @@ class NativeLauncher:
     def derive_keys(self, index_ptr, out_ptr, n, rng, stream):
         _check(load_library().srs_derive_keys(index_ptr, out_ptr, n, ctypes.byref(rng), stream))
 
-    def newton_workspace(self, batch, m, n) -> int:
-        return int(load_library().srs_newton_workspace(batch, m, n))
+    def newton_workspace(self, batch, m, n, y_fmt) -> int:
+        return int(load_library().srs_newton_workspace(batch, m, n, y_fmt))
 
     def orthogonalize(self, x_ptr, x_fmt, row_pitch, batch_stride, y_ptr, y_fmt, batch, m, n,
                       newton, workspace, stream):

@@ -59,10 +59,12 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
     """Newton-Schulz orthogonalisation of the matrices in the last two dimensions of ``x``.
 
     X_0 = x / (|x|_F + eps), then ``steps`` times X <- (a I + b G + c G^2) X with
-    G = X X^T (for tall matrices X (a I + b G + c G^2), G = X^T X).  Products run
-    on the tensor cores with FP16 operands and FP32 sums, so results carry about
-    three digits whatever ``dtype`` (default: that of ``x``; FP32, BF16 or FP16)
-    holds.  ``x``: FP32, BF16 or FP16, any strides; leading dimensions are a batch.
+    G = X X^T (for tall matrices X (a I + b G + c G^2), G = X^T X).  ``dtype``
+    (default: that of ``x``) is the result's and sets the products' precision: BF16
+    results come from FP16 operands (errors of about 1e-3, below their own rounding),
+    FP16 and FP32 results from pairs of FP16 operands (1e-5 for sides of some
+    hundreds, 1e-4 for ten thousand; three times the products); sums are FP32.
+    ``x``: FP32, BF16 or FP16, any strides; leading dimensions are a batch.
     A matrix with a NaN or infinity gives NaN.  Returns a new contiguous tensor.
     """
     newton = newton_settings(steps, coefficients, eps)
@@ -84,7 +86,7 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
         src = src.contiguous()
     launcher = _native.launcher()
     with device_guard(x.device):
-        space = torch.empty(launcher.newton_workspace(src.shape[0], m, n), dtype=torch.uint8,
+        space = torch.empty(launcher.newton_workspace(src.shape[0], m, n, _FORMATS[out_dtype]), dtype=torch.uint8,
                             device=x.device)
         launcher.orthogonalize(src.data_ptr(), _FORMATS[src.dtype], src.stride(1), src.stride(0),
                                y.data_ptr(), _FORMATS[out_dtype], src.shape[0], m, n, newton,
@@ -108,7 +110,7 @@ def _calls(classes, launcher):
     _WORKSPACE_BYTES (one matrix is always taken): [[(first, count, m, n), ...], ...]."""
     calls, current, room, first = [], [], _WORKSPACE_BYTES, 0
     for m, n, members in classes:
-        size, done = launcher.newton_workspace(1, m, n), 0
+        size, done = launcher.newton_workspace(1, m, n, _FORMATS[torch.bfloat16]), 0
         while done < len(members):
             fits = min(len(members) - done, room // size)
             if (fits < 1 and current) or len(current) == _native.MUON_MAX_CLASSES:

@@ -58,6 +58,22 @@ def test_orthogonalize_matches_fp64(size, kind, cuda_device):
     assert relative(y, newton(x)) <= 16 * U + ROUNDING[y.dtype]
 
 
+@pytest.mark.parametrize("size", SIZES + [(1, 2048, 2048), (2, 3000, 700)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_fp32_and_fp16_results_hold_more_digits(size, cuda_device):
+    """Held as pairs of FP16 numbers, values keep 22 bits (or 2^-25 of a matrix's
+    typical element) and products drop 2^-22 of their size, with FP32 sums (sqrt(K) *
+    2^-24 over K terms, K up to 4100): 15 products and their amplification stay within
+    2^-12; an FP16 result adds its own 2^-11 per element, 0.3 of it in the mean."""
+    from sr_states import orthogonalize
+
+    gen = torch.Generator().manual_seed(sum(size))
+    x = (torch.randn(size, generator=gen) * 1e-3).to(cuda_device)
+    want = newton(x)
+    assert relative(orthogonalize(x), want) <= 2.0**-12
+    assert relative(orthogonalize(x, dtype=torch.float16), want) <= 2.0**-12 + U
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-4, 1.0, 1e4, 1e30])
 def test_scale_of_the_input_does_not_matter(scale, cuda_device):
     """Squares of 1e30 and 1e-30 leave FP32's range; the norm is summed in FP64."""
