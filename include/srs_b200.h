@@ -325,14 +325,16 @@ int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch, int64_t ba
  *   u' = u*momentum + g;  v = nesterov ? u'*momentum + g : u'
  *   p' = fma(neg_step, O, p*decay),  O = the orthogonalised v of the matrix
  * u' is stored in u_format by u_rule (counter base state_key(key, 0), as the other
- * steps).  `rows`: DEVICE array as for srs_adamw_multi; param, grad, state[0],
- * param_index, offset and flags are used, numel and tile_begin are not.  `classes`: HOST
- * array; class i covers rows [first, first + count), matrices of m x n, count > 0.
+ * steps).  `rows`: HOST array, one row a matrix, read during the call: param, grad,
+ * state[0], param_index, offset and flags are used and checked, numel and tile_begin are
+ * not.  `classes`: HOST array; class i covers the next `count` rows, matrices of m x n,
+ * count > 0, at most SRS_MUON_MAX_MATRICES rows in all.
  * neg_step = -(lr * the shape's factor), decay = 1 - lr*weight_decay.
  * `workspace`: srs_muon_workspace(classes, n_classes) bytes (-1: invalid classes). */
 #define SRS_MUON_MAX_CLASSES 16
+#define SRS_MUON_MAX_MATRICES 64
 typedef struct srs_muon_class {
-  int64_t first, count, m, n;
+  int64_t count, m, n;
   float neg_step;
   int32_t reserved;
 } srs_muon_class;

@@ -13,33 +13,39 @@
 // the products read either operand with k or with its row index contiguous, so
 // nothing is ever transposed.
 //
-// Number formats.  G, P and X are held in FP16, accumulated in FP32.  Their
-// sizes are bounded (eigenvalues of a few units), so FP16's 11 significant bits are usable where
-// BF16 would keep 8: the steps multiply rounding errors of small singular
-// directions by up to a^5 = 485, and eight times smaller errors keep the result
-// within about 1e-3 of exact arithmetic for gradient-like spectra (1e-2 with BF16).
-// X_0 is held as V * 2^j with a power of two that puts |V * 2^j|_F between
-// sqrt(min(m, n)) / 4 and sqrt(min(m, n)): BF16 inputs are then held exactly, and
-// the remaining factor rho enters the first products in FP32.  The norm is
-// summed in FP64, so no input in range overflows or vanishes in it.
+// Number formats.  G, P and X are held in FP16, accumulated in FP32.  Their sizes are
+// bounded (eigenvalues of a few units), so FP16's 11 significant bits are usable where
+// BF16 would keep 8: the steps multiply rounding errors of small singular directions
+// by up to a^5 = 485, and eight times smaller errors keep the result within about 1e-3
+// of exact arithmetic for gradient-like spectra (1e-2 with BF16).  X_0 is held as
+// V * 2^j with a power of two that puts |V * 2^j|_F between sqrt(min(m, n)) / 4 and
+// sqrt(min(m, n)): BF16 inputs are then held exactly, and the remaining factor rho
+// enters the first products in FP32.  The norm is summed in FP64, so no input in range
+// overflows or vanishes in it.
 //
-// Results in FP32 or FP16 hold more digits than that.  For them every held matrix is
-// the sum of two FP16 matrices, what the first leaves of a value in the second, and a
-// product of two such is high by high + high by low + low by high: three times the
-// MMAs, errors from 4e-6 (128 x 512) to 1.3e-4 (4096 x 14336; the tensor core truncates
-// its FP32 sums, so they grow with the sides) (SPLIT).  X is then held times 2^t, about sqrt of its
-// longer side, so that the second matrices stay clear of FP16's smallest numbers.
+// Results in FP32 or FP16 hold more digits than that.  For them (SPLIT) every held
+// matrix is the sum of two FP16 matrices, what the first leaves of a value in the
+// second, and a product of two such is low by high + high by low + high by high: three
+// times the MMAs, errors from 4e-6 (128 x 512) to 1.3e-4 (4096 x 14336; the tensor core
+// truncates its FP32 sums, so they grow with the sides).  X is then held times 2^t,
+// about sqrt of its longer side, so that the second matrices stay clear of FP16's
+// smallest numbers.
 //
 // Three launches: the norm, X_0, and one cooperative grid that runs the 3 * steps
-// products of all matrices, whatever their shapes, as phases with a grid-wide
-// meeting between them (a launch a product took 7 us each where the products
-// themselves take 1 to 3).  G and P are symmetric: only tiles on and below the
-// diagonal are computed and stored twice.
+// products of all matrices, whatever their shapes, as phases with a grid-wide meeting
+// between them (a launch a product took 7 us each where the products themselves take 1
+// to 3).  G and P are symmetric: only tiles on and below the diagonal are computed and
+// stored; products read the others from their transposes.
 //
-// Reads of V: one for the norm and one for X_0.  For an optimizer step both
-// passes compute V from the gradient and the momentum (8 or fewer bytes an
-// element) rather than keeping V in FP32 (8 bytes more of traffic and 4 of
-// memory); the second pass stores u'.
+// What bounds it: the MMAs and the power they draw for large matrices (4096 x 14336:
+// 3.2 ms, 1.2 PFLOP/s of the 3 m^2 n + m^3 a step needs; the X = P X product keeps the
+// tensor pipe busy 99 % of its cycles), about 4 us a phase of meeting, first loads and
+// results for small ones (768 x 768: 125 us in 15 phases).
+//
+// Reads of V: one for the norm and one for X_0.  For an optimizer step both passes
+// compute V from the gradient and the momentum (8 or fewer bytes an element) rather than
+// keeping V in FP32 (8 bytes more of traffic and 4 of memory); the second pass stores
+// u'.  4096 x 14336 from BF16: 44 us each, 1.4 % of the whole.
 #include <cmath>
 
 #include "srs_host.h"
@@ -50,6 +56,7 @@ namespace srs {
 namespace {
 
 constexpr int kMaxClasses = SRS_MUON_MAX_CLASSES;
+constexpr int kMaxMatrices = SRS_MUON_MAX_MATRICES;
 static_assert(kMaxPhases <= kThreads, "one CTA zeroes the counters");
 constexpr int kSumChunks = 1024;  // most partial sums of a matrix
 constexpr int kPlain = -1;        // source template value: a plain tensor
@@ -57,13 +64,18 @@ constexpr int kPlain = -1;        // source template value: a plain tensor
 // steps) then stay among FP16's normal numbers, and eigenvalues up to 255 fit.
 constexpr float kHeld = 256.0f;
 
+// A matrix of an optimizer step.
+struct MuonMatrix {
+  uint64_t param, grad, state;
+  uint32_t key, offset, flags, unused;  // key or parameter index; SRS_ROW_* bits
+};
+
 // Where the matrices of one shape come from and go to.
 struct NewtonSource {
   const void* x;      // plain: the tensor
   int x_format;       // plain: SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t row_pitch, batch_stride;
   int vec;            // plain: rows start on 16-byte boundaries
-  const srs_row* rows;  // Muon: one row per matrix
   int m, n;           // rows, columns
   uint32_t units;     // vectors of 8 per matrix: m * ceil(n / 8)
   uint32_t row_units;
@@ -79,6 +91,7 @@ struct NewtonSource {
 // One launch over the matrices of several shapes (blockIdx.y: the matrix).
 struct NewtonPlan {
   NewtonSource source[kMaxClasses];
+  MuonMatrix matrix[kMaxMatrices];  // Muon: by place among all matrices
   int classes;
   double* partial;    // kSumChunks for each matrix
   unsigned int* counters;  // of the product grid's phases, set to zero here
@@ -107,7 +120,7 @@ __device__ __forceinline__ Unit unit_of(const NewtonSource& s, uint32_t u, int64
 // momentum is written back as well.
 template <int U, bool STORE>
 __device__ __forceinline__ void source8(const NewtonPlan& plan, const NewtonSource& s,
-                                        const srs_row& row, uint32_t ctr, int batch, uint32_t u,
+                                        const MuonMatrix& row, uint32_t ctr, int batch, uint32_t u,
                                         float (&v)[kVec]) {
   if constexpr (U == kPlain) {
     const Unit w = unit_of(s, u, s.row_pitch);
@@ -123,7 +136,7 @@ __device__ __forceinline__ void source8(const NewtonPlan& plan, const NewtonSour
     const void* grad = reinterpret_cast<const void*>(row.grad);
     if (row.flags & SRS_ROW_GRAD_BF16) load_param8<true>(grad, w.at, w.count, vec, g);
     else load_param8<false>(grad, w.at, w.count, vec, g);
-    load_state8<U>(reinterpret_cast<const void*>(row.state[0]), w.at, w.count, vec, old);
+    load_state8<U>(reinterpret_cast<const void*>(row.state), w.at, w.count, vec, old);
     float next[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
@@ -131,19 +144,18 @@ __device__ __forceinline__ void source8(const NewtonPlan& plan, const NewtonSour
       v[j] = plan.nesterov ? __fadd_rn(__fmul_rn(next[j], plan.momentum), g[j]) : next[j];
     }
     if constexpr (STORE)
-      store_state8<U>(reinterpret_cast<void*>(row.state[0]), w.at, w.count, vec, next,
+      store_state8<U>(reinterpret_cast<void*>(row.state), w.at, w.count, vec, next,
                       ctr + (uint32_t)w.at, plan.u_rule);
   }
 }
 
 template <int U>
-__device__ __forceinline__ void open_row(const NewtonPlan& plan, const NewtonSource& s, int batch,
-                                         srs_row* row, uint32_t* ctr) {
+__device__ __forceinline__ void open_row(const NewtonPlan& plan, int matrix, MuonMatrix* row,
+                                         uint32_t* ctr) {
   if constexpr (U != kPlain) {
-    *row = s.rows[batch];
-    const uint32_t key = (plan.rng.key_mode == SRS_KEY_GIVEN)
-                             ? row->param_index
-                             : update_key(plan.rng, row->param_index);
+    *row = plan.matrix[matrix];
+    const uint32_t key =
+        (plan.rng.key_mode == SRS_KEY_GIVEN) ? row->key : update_key(plan.rng, row->key);
     *ctr = row->offset + state_key(key, 0u);
   }
 }
@@ -174,9 +186,9 @@ newton_sum_kernel(const __grid_constant__ NewtonPlan plan) {
   const NewtonSource& s = plan.source[class_of(plan, (int)blockIdx.y)];
   if ((int)blockIdx.x >= s.chunks) return;
   const int batch = (int)blockIdx.y - s.first;
-  srs_row row{};
+  MuonMatrix row{};
   uint32_t ctr = 0;
-  open_row<U>(plan, s, batch, &row, &ctr);
+  open_row<U>(plan, (int)blockIdx.y, &row, &ctr);
   double sum = 0.0;
   const uint32_t stride = (uint32_t)s.chunks * kThreads;
 #pragma unroll 2
@@ -212,9 +224,9 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
   if (blockIdx.x == 0 && threadIdx.x == 0)
     s.rho[batch] = finite ? (float)ldexp(fraction, s.target) : __int_as_float(0x7FC00000);
 
-  srs_row row{};
+  MuonMatrix row{};
   uint32_t ctr = 0;
-  open_row<U>(plan, s, batch, &row, &ctr);
+  open_row<U>(plan, (int)blockIdx.y, &row, &ctr);
   __half* out = s.x0 + (int64_t)batch * s.x_elems;
   const uint32_t stride = (uint32_t)s.chunks * kThreads;
 #pragma unroll 2
@@ -263,7 +275,8 @@ struct NewtonClass {
   float held;            // X is held times this after the first step
   char* out;             // orthogonalize: the result, contiguous matrices
   int out_format;
-  const srs_row* rows;   // Muon: the parameters
+  int update;            // Muon: the result updates parameters
+  int first;             // their place among all matrices
   float step, decay;
 };
 
@@ -271,6 +284,8 @@ template <bool SPLIT>
 struct NewtonWork {
   static constexpr int kClasses = SPLIT ? 1 : kMaxClasses;
   NewtonClass<SPLIT> shape[kClasses];
+  uint64_t param[SPLIT ? 1 : kMaxMatrices];       // Muon: the parameters
+  uint8_t param_bf16[SPLIT ? 1 : kMaxMatrices];
   uint32_t triangles[kClasses + 1];  // first tile of each class in a G or P phase
   uint32_t grids[kClasses + 1];      // ... in an X phase
   int classes, steps, edge;
@@ -378,11 +393,10 @@ struct NewtonProducts {
         r.pitch = s.ld;
         r.low = s.x_low;
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
-      } else if (s.rows != nullptr) {
-        const srs_row& row = s.rows[at.batch];
+      } else if (!SPLIT && s.update != 0) {
         r.update = 1;
-        r.format = (row.flags & SRS_ROW_PARAM_BF16) ? SRS_FMT_BF16 : SRS_FMT_F32;
-        r.out = reinterpret_cast<char*>(row.param);
+        r.format = w.param_bf16[s.first + at.batch] ? SRS_FMT_BF16 : SRS_FMT_F32;
+        r.out = reinterpret_cast<char*>(w.param[s.first + at.batch]);
         r.pitch = s.n;
         r.step = s.step;
         r.decay = s.decay;
@@ -466,12 +480,13 @@ int launch_prepare(const NewtonPlan& plan, int64_t matrices, int chunks, cudaStr
 struct NewtonResult {
   void* out;
   int out_format;
-  const srs_row* rows;
+  bool update;
+  int first;
   float decay, step;
 };
 
 // Fills what the two preparing kernels and the product grid share.  The sources'
-// own fields (x or rows) are set by the caller.
+// own fields are set by the caller.
 void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
                  NewtonSource* f) {
   f->m = (int)s.m;
@@ -533,7 +548,8 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result,
   }
   c->out = static_cast<char*>(result.out);
   c->out_format = result.out_format;
-  c->rows = result.rows;
+  c->update = result.update ? 1 : 0;
+  c->first = result.first;
   c->step = result.step;
   c->decay = result.decay;
   for (int i = 0; i < 2; ++i) {
@@ -714,7 +730,7 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   s.batch_stride = batch_stride;
   s.vec = at % 16 == 0 && row_pitch % 8 == 0 && batch_stride % 8 == 0;
   fill_source(shape, space, 0, batch, &s);
-  const NewtonResult result{y, y_format, nullptr, 0.0f, 0.0f};
+  const NewtonResult result{y, y_format, false, 0, 0.0f, 0.0f};
   const auto run = [&](auto& work) {
     work.classes = 1;
     if (int rc = fill_class(shape, space, result, &work.shape[0])) return rc;
@@ -740,11 +756,11 @@ static int check_classes(const srs_muon_class* classes, int n_classes, int64_t* 
     if (int rc = check_matrices(classes[i].count, classes[i].m, classes[i].n)) return rc;
     if (classes[i].count == 0 || classes[i].m == 0 || classes[i].n == 0)
       return fail(SRS_ERR_INVALID_ARGUMENT, "shape %d is empty", i);
-    if (classes[i].first < 0) return fail(SRS_ERR_INVALID_ARGUMENT, "shape %d: negative row", i);
     *matrices += classes[i].count;
   }
-  if (*matrices > 65535)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "too many matrices for one call (at most 65535)");
+  if (*matrices > kMaxMatrices)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "%lld matrices in one call (at most %d)",
+                (long long)*matrices, kMaxMatrices);
   return SRS_OK;
 }
 
@@ -774,8 +790,19 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
   int64_t matrices = 0;
   if (int rc = check_classes(classes, n_classes, &matrices)) return rc;
   if (matrices == 0) return SRS_OK;
-  if (rows == nullptr || reinterpret_cast<uintptr_t>(rows) % 16 != 0)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "row table must be 16-byte aligned");
+  if (rows == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null row table");
+  for (int64_t i = 0; i < matrices; ++i) {
+    const srs_row& r = rows[i];
+    if (r.param == 0 || r.grad == 0 || r.state[0] == 0)
+      return fail(SRS_ERR_INVALID_ARGUMENT, "row %lld: null address", (long long)i);
+    const uint64_t p = (r.flags & SRS_ROW_PARAM_BF16) ? 2 : 4;
+    const uint64_t g = (r.flags & SRS_ROW_GRAD_BF16) ? 2 : 4, u = (uint64_t)fmt_bytes(u_format);
+    const bool vec = (r.flags & SRS_ROW_VECTOR_OK) != 0u;
+    if (r.param % p != 0 || r.grad % (vec ? 16 : g) != 0 ||
+        r.state[0] % (vec ? (u == 1 ? 8 : 16) : u) != 0)
+      return fail(SRS_ERR_INVALID_ARGUMENT,
+                  "row %lld: an address is not aligned as its flags promise", (long long)i);
+  }
   if (int rc = check_space(workspace, workspace_bytes, srs_muon_workspace(classes, n_classes)))
     return rc;
   if (int rc = check_device()) return rc;
@@ -800,13 +827,18 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
     const srs_muon_class& c = classes[i];
     const NewtonShape shape = lay_out(c.count, c.m, c.n, false, &used);
     NewtonSource& s = plan.source[i];
-    s.rows = rows + c.first;
     fill_source(shape, space, first, matrices, &s);
     if (s.chunks > chunks) chunks = s.chunks;
-    const NewtonResult result{nullptr, 0, s.rows, hp->decay, c.neg_step};
+    const NewtonResult result{nullptr, 0, true, first, hp->decay, c.neg_step};
     if (int rc = fill_class(shape, space, result, &work.shape[i])) return rc;
     batch[i] = c.count;
     first += (int)c.count;
+  }
+  for (int64_t i = 0; i < matrices; ++i) {
+    const srs_row& r = rows[i];
+    plan.matrix[i] = {r.param, r.grad, r.state[0], r.param_index, r.offset, r.flags, 0u};
+    work.param[i] = r.param;
+    work.param_bf16[i] = (r.flags & SRS_ROW_PARAM_BF16) ? 1 : 0;
   }
   int rc = SRS_OK;
   switch (u_format) {

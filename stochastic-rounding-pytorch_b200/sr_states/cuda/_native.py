@@ -79,9 +79,8 @@ class SrsMuonHparams(ctypes.Structure):
 
 
 class SrsMuonClass(ctypes.Structure):
-    _fields_ = [("first", ctypes.c_int64), ("count", ctypes.c_int64), ("m", ctypes.c_int64),
-                ("n", ctypes.c_int64), ("neg_step", ctypes.c_float),
-                ("reserved", ctypes.c_int32)]
+    _fields_ = [("count", ctypes.c_int64), ("m", ctypes.c_int64), ("n", ctypes.c_int64),
+                ("neg_step", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
 class SrsBlocks(ctypes.Structure):
@@ -93,6 +92,7 @@ class SrsBlocks(ctypes.Structure):
 
 NEWTON_MAX_STEPS = 32
 MUON_MAX_CLASSES = 16
+MUON_MAX_MATRICES = 64
 MAX_PEERS = 7
 IPC_HANDLE_BYTES = 64
 
@@ -366,9 +366,9 @@ class NativeLauncher:
         """Workspace bytes of a muon_multi call over ``classes`` (an array of SrsMuonClass)."""
         return int(load_library().srs_muon_workspace(classes, len(classes)))
 
-    def muon_multi(self, rows_ptr, classes, u_fmt, u_rule, hp, newton, rng, workspace, stream):
+    def muon_multi(self, rows, classes, u_fmt, u_rule, hp, newton, rng, workspace, stream):
         _check(load_library().srs_muon_multi(
-            rows_ptr, classes, len(classes), u_fmt, u_rule, ctypes.byref(hp),
+            ctypes.byref(rows), classes, len(classes), u_fmt, u_rule, ctypes.byref(hp),
             ctypes.byref(newton), ctypes.byref(rng), workspace.data_ptr(), workspace.numel(),
             stream))
 

@@ -7,9 +7,10 @@ with products alone; ``cuda_muon_step_`` is the optimizer step built on it
 
 from __future__ import annotations
 
+import ctypes
 import math
+import struct
 
-import numpy as np
 import torch
 
 from ..formats import StateFormat, resolve_formats
@@ -17,7 +18,7 @@ from ..rounding import native_codes
 from . import _native
 from ._fused import rng_words
 from ._launch import device_guard, stream_handle
-from ._tables import Update, build_table, upload
+from ._tables import Update, _row_flags
 from ._validate import check_disjoint, check_layout, check_nonnegative, spans_of
 
 # a, b, c of X <- (a I + b G + c G^2) X, G = X X^T: the quintic steps that bring
@@ -106,22 +107,25 @@ def _shape_classes(updates):
 
 
 def _calls(classes, launcher):
-    """The classes as calls of at most MUON_MAX_CLASSES shapes whose workspace stays within
-    _WORKSPACE_BYTES (one matrix is always taken): [[(first, count, m, n), ...], ...]."""
-    calls, current, room, first = [], [], _WORKSPACE_BYTES, 0
+    """The classes as calls of at most MUON_MAX_CLASSES shapes and MUON_MAX_MATRICES matrices
+    whose workspace stays within _WORKSPACE_BYTES (one matrix is always taken):
+    [[(m, n, members), ...], ...]."""
+    calls, current, room, places = [], [], _WORKSPACE_BYTES, _native.MUON_MAX_MATRICES
     for m, n, members in classes:
         size, done = launcher.newton_workspace(1, m, n, _FORMATS[torch.bfloat16]), 0
         while done < len(members):
-            fits = min(len(members) - done, room // size)
+            fits = min(len(members) - done, room // size, places)
             if (fits < 1 and current) or len(current) == _native.MUON_MAX_CLASSES:
                 calls.append(current)
-                current, room = [], _WORKSPACE_BYTES
+                current, room, places = [], _WORKSPACE_BYTES, _native.MUON_MAX_MATRICES
                 continue
             fits = max(1, fits)
-            current.append((first, fits, m, n))
-            room -= fits * size
-            first, done = first + fits, done + fits
+            current.append((m, n, members[done:done + fits]))
+            room, places, done = room - fits * size, places - fits, done + fits
     return calls + [current] if current else calls
+
+
+_ROW = struct.Struct("<QQQQqqIIII")  # srs_row
 
 
 def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, newton, rng):
@@ -129,25 +133,27 @@ def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, 
     device = updates[0].tensors[0].device
     launcher = _native.launcher()
     fmt, rule = codes
-    classes = _shape_classes(updates)
-    ordered = [updates[i] for _, _, members in classes for i in members]
-    host = build_table(ordered, [0] * len(ordered), launcher.tile_elems())
     hp = _native.SrsMuonHparams()
-    hp.momentum, hp.decay = np.float32(momentum), np.float32(1.0 - lr * weight_decay)
+    hp.momentum, hp.decay = momentum, 1.0 - lr * weight_decay
     hp.nesterov = int(nesterov)
     calls = []
-    for call in _calls(classes, launcher):
+    for call in _calls(_shape_classes(updates), launcher):
         table = (_native.SrsMuonClass * len(call))()
-        for entry, (first, count, m, n) in zip(table, call):
-            entry.first, entry.count, entry.m, entry.n = first, count, m, n
-            entry.neg_step = np.float32(-(lr * update_scale(scale, m, n)))
-        calls.append((table, launcher.muon_workspace(table)))
+        members = [updates[i] for _, _, chosen in call for i in chosen]
+        rows = ctypes.create_string_buffer(_ROW.size * len(members))
+        for i, u in enumerate(members):
+            p, g, state = u.tensors
+            _ROW.pack_into(rows, _ROW.size * i, p.data_ptr(), g.data_ptr(), state.data_ptr(), 0,
+                           u.numel, 0, u.param_index & 0xFFFFFFFF, u.offset, _row_flags(u, 0), 0)
+        for entry, (m, n, chosen) in zip(table, call):
+            entry.count, entry.m, entry.n = len(chosen), m, n
+            entry.neg_step = -(lr * update_scale(scale, m, n))
+        calls.append((rows, table, launcher.muon_workspace(table)))
     with device_guard(device):
-        rows = upload(host, device)
         stream = stream_handle(device)
-        space = torch.empty(max(size for _, size in calls), dtype=torch.uint8, device=device)
-        for table, _ in calls:
-            launcher.muon_multi(rows.data_ptr(), table, fmt, rule, hp, newton, rng, space, stream)
+        space = torch.empty(max(size for _, _, size in calls), dtype=torch.uint8, device=device)
+        for rows, table, _ in calls:
+            launcher.muon_multi(rows, table, fmt, rule, hp, newton, rng, space, stream)
 
 
 def check_muon(lr, momentum, weight_decay, scale) -> None:

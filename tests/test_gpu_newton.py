@@ -311,6 +311,24 @@ def test_muon_unaligned_parameters_and_skipped_gradients(cuda_device):
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
 
 
+def test_more_matrices_and_shapes_than_one_call_takes(cuda_device, monkeypatch):
+    """70 matrices of one shape, 18 shapes, and a workspace limit that splits both: each
+    matrix ends as it does alone."""
+    from sr_states.cuda import cuda_muon_step_, muon
+
+    shapes = [(24, 40)] * 70 + [(16 + i, 90 - i) for i in range(18)]
+    ps, gs, us = _case(cuda_device, shapes, torch.bfloat16, torch.bfloat16, torch.float16)
+    alone = [[t.clone() for t in (p, u)] for p, u in zip(ps, us)]
+    for i, ((p, u), g) in enumerate(zip(alone, gs)):
+        cuda_muon_step_([p], [g], [u], lr=0.02, seeds=[i])
+    for limit in (2 << 30, 100_000):
+        monkeypatch.setattr(muon, "_WORKSPACE_BYTES", limit)
+        now = [[t.clone() for t in column] for column in (ps, us)]
+        cuda_muon_step_(now[0], gs, now[1], lr=0.02, seeds=range(len(shapes)))
+        for i, (p, u) in enumerate(alone):
+            assert torch.equal(now[0][i], p) and torch.equal(now[1][i], u), (limit, i)
+
+
 def test_muon_refusals(cuda_device):
     from sr_states import MuonSR
     from sr_states.cuda import cuda_muon_step_

@@ -71,20 +71,32 @@ def test_entry_points_check_before_any_cuda_call():
     assert orth(m=0) == _native.SRS_OK and orth(b=0) == _native.SRS_OK
     hp, rng = _native.SrsMuonHparams(), _native.SrsRng()
 
-    def shapes(count=1, m=8, n=8, first=0):
+    def shapes(count=1, m=8, n=8):
         table = (_native.SrsMuonClass * 1)()
-        table[0].first, table[0].count, table[0].m, table[0].n = first, count, m, n
+        table[0].count, table[0].m, table[0].n = count, m, n
         return table
 
+    def matrix(param=256, grad=512, state=1024, flags=0):
+        row = _native.SrsRow()
+        row.param, row.grad, row.flags = param, grad, flags
+        row.state[0] = state
+        return ctypes.byref(row)
+
+    rows = (_native.SrsRow * 1)()
+    rows[0].param, rows[0].grad, rows[0].flags = 256, 512, 0
+    rows[0].state[0] = 1024
+
     muon = lambda **k: lib.srs_muon_multi(*{  # noqa: E731
-        "r": 256, "c": shapes(), "k": 1, "f": 1, "rule": 1, "hp": ctypes.byref(hp),
+        "r": ctypes.byref(rows), "c": shapes(), "k": 1, "f": 1, "rule": 1, "hp": ctypes.byref(hp),
         "h": ctypes.byref(h), "rng": ctypes.byref(rng), "w": 1024, "wb": 1 << 30, "s": None,
         **k}.values())
     assert muon(f=9) == bad and muon(rule=9) == bad and muon(hp=None) == bad
-    assert muon(r=None) == bad and muon(r=8) == bad and muon(wb=0) == bad
+    assert muon(r=None) == bad and muon(wb=0) == bad
+    for r in (matrix(param=0), matrix(grad=0), matrix(state=0), matrix(param=258),
+              matrix(grad=520, flags=_native.ROW_VECTOR_OK), matrix(state=1025)):
+        assert muon(r=r) == bad, bytes(lib.srs_last_error())
     assert muon(c=None) == bad and muon(k=17) == bad and muon(k=-1) == bad
-    for table in (shapes(count=0), shapes(m=0), shapes(n=-1), shapes(first=-1), shapes(m=1 << 25),
-                  shapes(count=70000)):
+    for table in (shapes(count=0), shapes(m=0), shapes(n=-1), shapes(m=1 << 25), shapes(count=65)):
         assert muon(c=table) == bad and lib.srs_muon_workspace(table, 1) == -1
     assert lib.srs_muon_workspace(shapes(), 1) > 0 and lib.srs_muon_workspace(None, 0) == 0
     assert muon(k=0) == _native.SRS_OK
@@ -136,10 +148,11 @@ def test_structure_layouts(tmp_path):
 #include <stdio.h>
 #include "{HEADER}"
 int main(void) {{
-  printf("%zu %zu %zu %zu %zu %zu %d %zu %zu %d\\n", sizeof(srs_newton),
+  printf("%zu %zu %zu %zu %zu %zu %d %zu %zu %d %d\\n", sizeof(srs_newton),
          offsetof(srs_newton, eps), sizeof(srs_muon_hparams), offsetof(srs_muon_hparams, nesterov),
          sizeof(srs_blocks), offsetof(srs_blocks, format), SRS_NEWTON_MAX_STEPS,
-         sizeof(srs_muon_class), offsetof(srs_muon_class, neg_step), SRS_MUON_MAX_CLASSES);
+         sizeof(srs_muon_class), offsetof(srs_muon_class, neg_step), SRS_MUON_MAX_CLASSES,
+         SRS_MUON_MAX_MATRICES);
   return 0;
 }}
 """)
@@ -151,4 +164,5 @@ int main(void) {{
                    ctypes.sizeof(_native.SrsMuonHparams), _native.SrsMuonHparams.nesterov.offset,
                    ctypes.sizeof(_native.SrsBlocks), _native.SrsBlocks.format.offset,
                    _native.NEWTON_MAX_STEPS, ctypes.sizeof(_native.SrsMuonClass),
-                   _native.SrsMuonClass.neg_step.offset, _native.MUON_MAX_CLASSES]
+                   _native.SrsMuonClass.neg_step.offset, _native.MUON_MAX_CLASSES,
+                   _native.MUON_MAX_MATRICES]
