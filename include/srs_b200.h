@@ -300,9 +300,9 @@ int srs_derive_keys(const uint32_t* param_index, uint32_t* out, int64_t n, const
  * for `batch` matrices of m rows and n columns (m > n: X_{i+1} = X_i (a I + b G + c G^2),
  * G = X_i^T X_i).  Products on the tensor cores with FP32 sums: FP16 operands for y in
  * BF16 (errors of about 1e-3), pairs of FP16 operands for y in FP32 or FP16 (1e-5 for
- * sides of some hundreds, 1e-4 for ten thousand; three times the work); the norm is summed in FP64.  x: FP32, BF16 or FP16, element (b, i, j) at
- * b * batch_stride + i * row_pitch + j; y: contiguous, FP32, BF16 or FP16; x and y
- * must not overlap.  A matrix with a NaN or infinity, or whose norm plus eps is
+ * sides of some hundreds, 1e-4 for ten thousand; three times the work); the norm is
+ * summed in FP64.  x: FP32, BF16 or FP16, element (b, i, j) at b * batch_stride +
+ * i * row_pitch + j; y: contiguous, FP32, BF16 or FP16; x and y must not overlap.  A matrix with a NaN or infinity, or whose norm plus eps is
  * zero, gives NaN throughout.  Sizes of zero are a no-op.
  * `workspace`: srs_newton_workspace(batch, m, n, y_format) bytes, 256-byte aligned, not used
  * by any other call that can overlap in time. */

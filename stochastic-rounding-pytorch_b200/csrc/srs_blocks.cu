@@ -110,8 +110,8 @@ __device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>], bo
 // Rounds 8 scaled values to 8 bytes.  Values of a block are finite and at most the
 // format's largest after scaling unless the block held infinities or NaN: `plain` says
 // that it did not, and the stochastic rule then needs no screen.  The general form (any
-// value, toward zero) is kept out of the way of the instruction cache: it costs 4 of
-// 5 issue slots of the stochastic form when it is compiled into every row.
+// value, toward zero) is kept out of line: compiled into every row, it left each warp of
+// the stochastic form waiting 4.3 cycles an instruction for the instruction cache.
 template <int OF>
 __device__ __forceinline__ uint2 encode_plain(const float (&y)[kVec], uint32_t ctr, bool nearest) {
   uint32_t w[2];

@@ -37,7 +37,7 @@ int launch_groups(const void* kernel, int64_t groups, int group, int threads, in
                   bool cooperative, void* argument, cudaStream_t stream, const char* what,
                   bool overlap = false);
 
-// FP8 blocks: d = a b^T (srs_blocks.h's operands, checked by the caller).  Element (i, j)
+// FP8 blocks: d = a b^T (operands checked by the caller).  Element (i, j)
 // of d is stored at i * row_stride + j * col_stride; only products with a thin side
 // (at most kThinRows rows) take a col_stride other than 1.  `overlap`: the kernel ahead
 // writes nothing of a.

@@ -79,7 +79,7 @@ struct NewtonSource {
   int m, n;           // rows, columns
   uint32_t units;     // vectors of 8 per matrix: m * ceil(n / 8)
   uint32_t row_units;
-  int first, count;   // matrices of this shape among all
+  int first;          // number of this shape's first matrix among all
   int chunks;         // partial sums of one matrix
   int target;         // floor(log2(sqrt(min(m, n))))
   __half* x0;
@@ -494,7 +494,6 @@ void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
   f->row_units = (uint32_t)((s.n + 7) / 8);
   f->units = (uint32_t)(s.m * f->row_units);
   f->first = first;
-  f->count = (int)s.batch;
   // Enough CTAs for several per SM; each thread gets at least 4 vectors.
   int64_t chunks = (8ll * sm_count() + matrices - 1) / matrices;
   const int64_t most = (f->units + 4 * kThreads - 1) / (4 * kThreads);
@@ -632,8 +631,8 @@ double step_cycles(const NewtonWork<SPLIT>& w, const int64_t* batch, int cg) {
 }
 
 template <bool SPLIT>
-int run_newton(NewtonWork<SPLIT>& w, const int64_t* batch, const srs_newton* h, unsigned int* counters,
-               cudaStream_t stream) {
+int run_newton(NewtonWork<SPLIT>& w, const int64_t* batch, const srs_newton* h,
+               unsigned int* counters, cudaStream_t stream) {
   w.steps = h->steps;
   w.a = h->coefficients[0];
   w.b = h->coefficients[1];
@@ -770,7 +769,8 @@ extern "C" int64_t srs_muon_workspace(const srs_muon_class* classes, int n_class
   if (check_classes(classes, n_classes, &matrices) != SRS_OK) return -1;
   if (n_classes == 0) return 0;
   lay_out_head(matrices, &at);
-  for (int i = 0; i < n_classes; ++i) lay_out(classes[i].count, classes[i].m, classes[i].n, false, &at);
+  for (int i = 0; i < n_classes; ++i)
+    lay_out(classes[i].count, classes[i].m, classes[i].n, false, &at);
   return at;
 }
 

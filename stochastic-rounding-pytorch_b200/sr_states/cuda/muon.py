@@ -87,8 +87,8 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
         src = src.contiguous()
     launcher = _native.launcher()
     with device_guard(x.device):
-        space = torch.empty(launcher.newton_workspace(src.shape[0], m, n, _FORMATS[out_dtype]), dtype=torch.uint8,
-                            device=x.device)
+        need = launcher.newton_workspace(src.shape[0], m, n, _FORMATS[out_dtype])
+        space = torch.empty(need, dtype=torch.uint8, device=x.device)
         launcher.orthogonalize(src.data_ptr(), _FORMATS[src.dtype], src.stride(1), src.stride(0),
                                y.data_ptr(), _FORMATS[out_dtype], src.shape[0], m, n, newton,
                                space, stream_handle(x.device))
