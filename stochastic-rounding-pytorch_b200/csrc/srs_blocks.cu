@@ -50,11 +50,16 @@ struct Size {
       XF == SRS_FMT_F32 ? 0x7F800000u : XF == SRS_FMT_BF16 ? 0x7F80u : 0x7C00u;
   __device__ static uint32_t of(uint32_t word) { return word & kMask; }
   __device__ static uint32_t larger(uint32_t a, uint32_t b) {
-    return kPacked ? __vmaxu2(a, b) : max(a, b);
+    if constexpr (kPacked) {
+      uint32_t r;
+      asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+      return r;
+    } else {
+      return max(a, b);
+    }
   }
-  // the word with non-finite elements (NaN, infinities) taken as zero
-  __device__ static uint32_t finite(uint32_t word) {
-    const uint32_t u = word & kMask;
+  // sizes with those that are not of finite numbers taken as zero
+  __device__ static uint32_t finite(uint32_t u) {
     if (!kPacked) return u < kInfinite ? u : 0u;
     return ((u & 0xFFFFu) < kInfinite ? u & 0xFFFFu : 0u) |
            ((u >> 16) < kInfinite ? u & 0xFFFF0000u : 0u);
@@ -84,27 +89,52 @@ __device__ __forceinline__ void load_words(const QuantizeArgs& a, int64_t row, i
   }
 }
 
-// Largest finite size (FP32 encoding) of 8 elements a lane over 16 lanes; `finite`:
-// the warp's two rows hold neither infinities nor NaN.
-template <int XF>
-__device__ __forceinline__ uint32_t row_size(const uint32_t (&w)[kWords<XF>], bool* finite) {
+// `to`: the sizes in `w`, those of infinities and NaN set to zero.
+template <int XF, int N>
+__device__ __forceinline__ void only_finite(const uint32_t (&w)[N][kWords<XF>],
+                                            uint32_t (&to)[N][kWords<XF>]) {
   using Z = Size<XF>;
-  uint32_t top = 0u;
 #pragma unroll
-  for (int j = 0; j < kWords<XF>; ++j) top = Z::larger(top, Z::of(w[j]));
-  top = Z::single(top);
+  for (int i = 0; i < N; ++i) {
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-  *finite = !__any_sync(0xFFFFFFFFu, top >= Z::kInfinite);
-  if (!*finite) {
-    top = 0u;
-#pragma unroll
-    for (int j = 0; j < kWords<XF>; ++j) top = Z::larger(top, Z::finite(w[j]));
-    top = Z::single(top);
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    for (int j = 0; j < kWords<XF>; ++j) to[i][j] = Z::finite(Z::of(w[i][j]));
   }
-  return Z::as_f32(top);
+}
+
+// Largest sizes of N rows of 128 elements, 8 of each row a lane of 16: lane l is given that
+// of row l % N.  Two rows of 16-bit elements share a word, and each exchange between lanes
+// halves the words that a lane keeps: 5 shuffles for 8 such rows instead of 32.
+template <int XF, int N>
+__device__ __forceinline__ uint32_t row_sizes(const uint32_t (&w)[N][kWords<XF>], int lane16) {
+  using Z = Size<XF>;
+  constexpr int kHeld = Z::kPacked ? N / 2 : N;
+  uint32_t r[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r[i] = Z::of(w[i][0]);
+#pragma unroll
+    for (int j = 1; j < kWords<XF>; ++j) r[i] = Z::larger(r[i], Z::of(w[i][j]));
+  }
+  if constexpr (Z::kPacked) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      r[i] = Z::larger(__byte_perm(r[i], r[i + kHeld], 0x5410u),
+                       __byte_perm(r[i], r[i + kHeld], 0x7632u));
+  }
+#pragma unroll
+  for (int d = kHeld / 2; d > 0; d >>= 1) {
+    const bool upper = (lane16 & d) != 0;
+#pragma unroll
+    for (int i = 0; i < d; ++i) {
+      const uint32_t keep = upper ? r[i + d] : r[i], give = upper ? r[i] : r[i + d];
+      r[i] = Z::larger(keep, __shfl_xor_sync(0xFFFFFFFFu, give, d));
+    }
+  }
+#pragma unroll
+  for (int d = kHeld; d < 16; d <<= 1)
+    r[0] = Z::larger(r[0], __shfl_xor_sync(0xFFFFFFFFu, r[0], d));
+  if constexpr (Z::kPacked) return (lane16 & kHeld) != 0 ? r[0] >> 16 : r[0] & 0xFFFFu;
+  return r[0];
 }
 
 // Rounds 8 scaled values to 8 bytes.  Values of a block are finite and at most the
@@ -138,8 +168,8 @@ __device__ __forceinline__ uint2 encode_values(const float (&y)[kVec], uint32_t 
 
 // Rows alone, 1 x 128 blocks: 16 lanes to a block, kAhead blocks of one column a
 // half-warp with all their loads first.  HBM-bound when rounding to nearest (8192 x
-// 4096: 27 us with the launch; 3 bytes an element at 6.5 TB/s would be 15), by the integer
-// units for the stochastic rule's hashes (45 us).
+// 4096: 25 us with the launch; 3 bytes an element at 6.5 TB/s would be 15), by the integer
+// units for the stochastic rule's hashes (41 us).
 constexpr int kAhead = 4;
 
 template <int OF, int XF>
@@ -152,19 +182,23 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
   uint32_t raw[kAhead][kWords<XF>];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) load_words<XF>(a, row0 + i, col, raw[i]);
-  int k[kAhead];
-  bool plain = a.rule != SRS_RULE_TOWARD_ZERO;
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    bool finite;
-    k[i] = block_exponent<OF>(row_size<XF>(raw[i], &finite));
-    plain = plain && finite;
+  uint32_t top = row_sizes<XF, kAhead>(raw, lane16);
+  bool plain = !__any_sync(0xFFFFFFFFu, top >= Size<XF>::kInfinite);
+  if (!plain) {
+    uint32_t sizes[kAhead][kWords<XF>];
+    only_finite<XF>(raw, sizes);
+    top = row_sizes<XF, kAhead>(sizes, lane16);
   }
+  const int own_k = block_exponent<OF>(Size<XF>::as_f32(top));
+  if (lane16 < kAhead && row0 + lane16 < a.rows)
+    a.scale[(row0 + lane16) * a.scale_pitch + blockIdx.x] = (uint8_t)(own_k + 127);
+  const float own_factor = power_of_two(-own_k);
+  plain = plain && a.rule != SRS_RULE_TOWARD_ZERO;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int64_t row = row0 + i;
-    if (row >= a.rows) break;
-    const float factor = power_of_two(-k[i]);
+    const float factor = __shfl_sync(0xFFFFFFFFu, own_factor, i, 16);
+    if (row >= a.rows) continue;
     float y[kVec];
     decode8<XF>(raw[i], y);
 #pragma unroll
@@ -172,7 +206,6 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
     const uint2 w =
         encode_values<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, plain);
     if (col < a.data_pitch) *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = w;
-    if (lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k[i] + 127);
   }
 }
 
@@ -181,17 +214,19 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
 // over 16 lanes, a column's one over the 16 row groups.  The transposed copy's bytes
 // are kept by rows (32-bit words rotated by 4 * (row / 16), so that both sides are
 // conflict-free) and leave as 4 x 4 byte transposes, 128 bytes of a column at a time.
-// Nearest: HBM-bound; stochastic both ways: bound by the hashes (two a element, about
-// 25 integer operations).  8192 x 4096 from BF16, both ways: 51 us to nearest,
-// 90 us stochastic (E5M2); the bytes alone would take 20.
+// Nearest: bound by waits for the loads and at the barriers (integer pipe 51 % busy);
+// stochastic both ways: by the hashes (two an element, about 25 integer operations).
+// 8192 x 4096 from BF16, both ways: 45 us to nearest, 76 us stochastic (E5M2); the bytes
+// alone would take 20.  A reduction of 4 shuffles for every row, and 16 partial maxima a
+// column instead of 8, took 51 and 90.
 template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
 __global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 4 : 2)
 quantize_tile_kernel(const QuantizeArgs a) {
   using Z = Size<XF>;
   constexpr int kW = kWords<XF>;
   extern __shared__ __align__(16) uint8_t tile_raw[];  // 128 x 128 elements of x
-  __shared__ uint32_t tops[COLS && !SQUARE ? 16 * 16 * kW : 8];
-  __shared__ int row_k[kBlock];
+  __shared__ __align__(16) uint32_t tops[COLS && !SQUARE ? 8 * 16 * kW : 8];
+  __shared__ float row_factor[kBlock];
   __shared__ __align__(16) uint32_t turned[COLS ? kBlock * 32 : 4];
   const int lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock, col0 = (int64_t)blockIdx.x * kBlock;
@@ -213,16 +248,18 @@ quantize_tile_kernel(const QuantizeArgs a) {
       for (int v = 0; v < kW / 4; ++v)
         mine[slot(i, v)] =
             make_uint4(raw[i][4 * v], raw[i][4 * v + 1], raw[i][4 * v + 2], raw[i][4 * v + 3]);
+#pragma unroll
+      for (int j = 0; j < kW; ++j) raw[i][j] = Z::of(raw[i][j]);  // from here on: the sizes
     }
     if constexpr (SQUARE) {
-      uint32_t top = 0u;
-      for (int pass = 0; pass < 2; ++pass) {
+      uint32_t top;
+#pragma unroll 1
+      while (true) {
         top = 0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
 #pragma unroll
-          for (int j = 0; j < kW; ++j)
-            top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
+          for (int j = 0; j < kW; ++j) top = Z::larger(top, raw[i][j]);
         }
         top = __reduce_max_sync(0xFFFFFFFFu, Z::single(top));
         __syncthreads();
@@ -232,46 +269,70 @@ quantize_tile_kernel(const QuantizeArgs a) {
         for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
         if (top < Z::kInfinite) break;  // the same for the whole CTA
         plain = false;
+        only_finite<XF>(raw, raw);
       }
       tile_k = block_exponent<OF>(Z::as_f32(top));
     } else {
       if constexpr (ROWS) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          bool finite;
-          const int k = block_exponent<OF>(row_size<XF>(raw[i], &finite));
-          plain = plain && finite;
-          if (lane16 == 0) row_k[8 * group + i] = k;
+        uint32_t top;
+#pragma unroll 1
+        while (__any_sync(0xFFFFFFFFu,
+                          (top = row_sizes<XF, 8>(raw, lane16)) >= Z::kInfinite)) {
+          plain = false;
+          only_finite<XF>(raw, raw);
+        }
+        const int k = block_exponent<OF>(Z::as_f32(top));
+        if (lane16 < 8) {
+          row_factor[8 * group + lane16] = power_of_two(-k);
+          if (row_base + lane16 < a.rows)
+            a.scale[(row_base + lane16) * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
         }
       }
       if constexpr (COLS) {
         uint32_t col_top[kVec];
-        for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+        while (true) {
+          uint32_t top[kW];
 #pragma unroll
           for (int j = 0; j < kW; ++j) {
-            uint32_t top = 0u;
+            top[j] = raw[0][j];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              top = Z::larger(top, pass == 0 ? Z::of(raw[i][j]) : Z::finite(raw[i][j]));
-            tops[(group * kW + j) * 16 + lane16] = top;
+            for (int i = 1; i < 8; ++i) top[j] = Z::larger(top[j], raw[i][j]);
+            top[j] = Z::larger(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], 16));
+          }
+          uint4* const all = reinterpret_cast<uint4*>(tops) + lane16;
+          if ((group & 1) == 0) {
+#pragma unroll
+            for (int v = 0; v < kW / 4; ++v)
+              all[((group >> 1) * (kW / 4) + v) * 16] =
+                  make_uint4(top[4 * v], top[4 * v + 1], top[4 * v + 2], top[4 * v + 3]);
           }
           __syncthreads();
+#pragma unroll
+          for (int v = 0; v < kW / 4; ++v) {
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              const uint4 q = all[(g * (kW / 4) + v) * 16];
+              top[4 * v] = Z::larger(top[4 * v], q.x);
+              top[4 * v + 1] = Z::larger(top[4 * v + 1], q.y);
+              top[4 * v + 2] = Z::larger(top[4 * v + 2], q.z);
+              top[4 * v + 3] = Z::larger(top[4 * v + 3], q.w);
+            }
+          }
           bool infinite = false;
 #pragma unroll
           for (int j = 0; j < kW; ++j) {
-            uint32_t t = 0u;
-#pragma unroll
-            for (int g = 0; g < 16; ++g) t = Z::larger(t, tops[(g * kW + j) * 16 + lane16]);
             if (Z::kPacked) {
-              col_top[2 * j % kVec] = t & 0xFFFFu;
-              col_top[(2 * j + 1) % kVec] = t >> 16;
+              col_top[2 * j % kVec] = top[j] & 0xFFFFu;
+              col_top[(2 * j + 1) % kVec] = top[j] >> 16;
             } else {
-              col_top[j] = t;
+              col_top[j] = top[j];
             }
-            infinite = infinite || Z::single(t) >= Z::kInfinite;
+            infinite = infinite || Z::single(top[j]) >= Z::kInfinite;
           }
           if (!__syncthreads_or(infinite)) break;
           plain = false;
+          only_finite<XF>(raw, raw);
         }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
@@ -287,6 +348,10 @@ quantize_tile_kernel(const QuantizeArgs a) {
 
   uint32_t ctr = a.ctr + (uint32_t)(row_base * a.cols + col);
   uint32_t ctr_t = a.ctr_t + (uint32_t)(row_base * a.cols + col);
+  const float tile_factor = power_of_two(-tile_k);
+  const int rows_left = col < a.data_pitch ? (int)min(a.rows - row_base, (int64_t)8) : 0;
+  uint8_t* out = a.data + row_base * a.data_pitch + col;
+  uint32_t* turn = turned + (COLS ? 8 * group * 32 + ((2 * lane16 + 4 * (group >> 1)) & 31) : 0);
 #pragma unroll 1
   for (int i = 0; i < 8; ++i) {
     uint32_t raw[kW];
@@ -300,25 +365,19 @@ quantize_tile_kernel(const QuantizeArgs a) {
     }
     float x[kVec], y[kVec];
     decode8<XF>(raw, x);
-    const int64_t row = row_base + i;
     if constexpr (ROWS) {
-      const int k = SQUARE ? tile_k : row_k[8 * group + i];
-      const float factor = power_of_two(-k);
+      const float factor = SQUARE ? tile_factor : row_factor[8 * group + i];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) y[j] = x[j] * factor;
       const uint2 w = encode_values<OF>(y, ctr, a.rule, plain);
-      if (row < a.rows) {
-        if (col < a.data_pitch) *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = w;
-        if (!SQUARE && lane16 == 0) a.scale[row * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
-      }
+      if (i < rows_left) *reinterpret_cast<uint2*>(out) = w;
+      out += a.data_pitch;
     }
     if constexpr (COLS) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        y[j] = x[j] * (SQUARE ? power_of_two(-tile_k) : col_factor[j]);
-      const uint2 w = encode_values<OF>(y, ctr_t, a.rule, plain);
-      const int r = 8 * group + i;
-      *reinterpret_cast<uint2*>(turned + r * 32 + ((2 * lane16 + 4 * (r >> 4)) & 31)) = w;
+      for (int j = 0; j < kVec; ++j) y[j] = x[j] * (SQUARE ? tile_factor : col_factor[j]);
+      *reinterpret_cast<uint2*>(turn) = encode_values<OF>(y, ctr_t, a.rule, plain);
+      turn += 32;
     }
     ctr += (uint32_t)a.cols;
     ctr_t += (uint32_t)a.cols;
