@@ -220,7 +220,8 @@ PyObject* py_linear(PyObject*, PyObject* args) {
   const c10::cuda::OptionalCUDAGuard guard(t.device());
   const int x_format = source_format(t, "block_linear");
   TORCH_CHECK_VALUE(t.device() == weight.device(), "all tensors must be on the same CUDA device");
-  at::Tensor flat = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  TORCH_CHECK_VALUE(t.dim() > 0, "block_linear needs at least one dimension");
+  at::Tensor flat = t.dim() == 2 ? t : t.dim() == 1 ? t.unsqueeze(0) : t.flatten(0, -2);
   const int64_t tokens = flat.size(0), k = flat.size(1);
   if (flat.stride(1) != 1 && k > 1) flat = flat.contiguous();
   Blocks blocks{weight, tensor(w_scale, "the weight's scale")};
@@ -246,7 +247,8 @@ PyObject* py_linear(PyObject*, PyObject* args) {
 }
 
 PyMethodDef kMethods[] = {
-    {"bind", py_bind, METH_VARARGS, "bind(quantize, matmul, copy_rows, linear, linear_workspace): entry point addresses."},
+    {"bind", py_bind, METH_VARARGS,
+     "bind(quantize, matmul, copy_rows, linear, linear_workspace): entry point addresses."},
     {"quantize", py_quantize, METH_VARARGS,
      "quantize(x, format, rule, square, seed, offset, orientation) -> tensors or a status."},
     {"matmul", py_matmul, METH_VARARGS,

@@ -666,6 +666,7 @@ extern "C" int srs_linear_blocks(const void* x, int x_format, int64_t tokens, in
   rows.scale_pitch = blocks_of(k);
   rows.format = block_format;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (k == 0) return srs_matmul_blocks(&rows, w, k, d, x_format, stream);
   if (int rc = quantize_blocks(x, x_format, tokens, k, x_pitch, block_format, SRS_RULE_NEAREST, 0,
                                0u, 0u, workspace, rows.pitch,
                                static_cast<char*>(workspace) + tokens * rows.pitch,
@@ -673,7 +674,7 @@ extern "C" int srs_linear_blocks(const void* x, int x_format, int64_t tokens, in
     return rc;
   // With few tokens the product starts beside the quantisation and streams the
   // weights, which that kernel does not write, before it needs the tokens.
-  if (k > 0 && tokens <= kThinRows && w->rows >= tokens) {
+  if (tokens <= kThinRows && w->rows >= tokens) {
     if (d == nullptr || reinterpret_cast<uintptr_t>(d) % fmt_bytes(x_format) != 0)
       return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
     return launch_thin(*w, rows, k, d, x_format, 1, w->rows, true, st);

@@ -11,16 +11,22 @@ from __future__ import annotations
 import torch
 
 from ._hash import update_key
-from .cuda.blocks import BLOCK, BlockTensor, linear_blocks, matmul_blocks, quantize_blocks
+from .cuda.blocks import (BLOCK, BlockTensor, check_blocks, linear_blocks, matmul_blocks,
+                          quantize_blocks)
 
 __all__ = ["BlockLinear", "BlockTensor", "block_linear", "matmul_blocks", "quantize_blocks"]
+
+
+def _matrix(x):
+    # all but the last dimension in one; sizes of zero included, unlike reshape(-1, K)
+    return x.flatten(0, -2) if x.dim() > 1 else x.unsqueeze(0)
 
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, dtype, grad_dtype, grad_rounding, seed):
         need_x, need_w = ctx.needs_input_grad[:2]
-        flat = x.reshape(-1, x.shape[-1])
+        flat = _matrix(x)
         tokens = quantize_blocks(flat, dtype=dtype, orientation="both" if need_w else "rows")
         matrix = quantize_blocks(weight, dtype=dtype, block=(BLOCK, BLOCK),
                                  orientation="both" if need_x else "rows")
@@ -39,7 +45,7 @@ class _BlockLinear(torch.autograd.Function):
         saved = list(ctx.saved_tensors)
         tokens_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_w else None
         matrix_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_x else None
-        flat = dy.reshape(-1, dy.shape[-1])
+        flat = _matrix(dy)
         orientation = "both" if need_x and need_w else "rows" if need_x else "columns"
         got = quantize_blocks(flat, dtype=grad_dtype, rounding=rounding, seed=seed,
                               orientation=orientation)
@@ -69,6 +75,7 @@ def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float
             raise ValueError("a BlockTensor weight has no backward pass; pass the weight itself "
                              "or run under torch.no_grad()")
         return linear_blocks(x, weight, dtype)
+    check_blocks(grad_dtype, grad_rounding)
     return _BlockLinear.apply(x, weight, dtype, grad_dtype, grad_rounding, seed)
 
 

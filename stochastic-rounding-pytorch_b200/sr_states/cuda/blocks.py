@@ -35,6 +35,13 @@ class BlockTensor(NamedTuple):
         return (self.data.float() * factor).to(dtype)
 
 
+def check_blocks(dtype, rounding):
+    """The entry points' codes of a block format and a rounding rule."""
+    if dtype not in _FP8:
+        raise TypeError(f"blocks are held in float8_e4m3fn or float8_e5m2, got {dtype}")
+    return native_codes(dtype, rounding)
+
+
 def quantize_blocks(x, *, dtype=torch.float8_e4m3fn, rounding="nearest", seed=0, offset=0,
                     block=(1, BLOCK), orientation="rows"):
     """Quantise a matrix to FP8 blocks of 128, read once.
@@ -51,9 +58,7 @@ def quantize_blocks(x, *, dtype=torch.float8_e4m3fn, rounding="nearest", seed=0,
 
     ``x``: FP32, BF16 or FP16 on an sm_100a GPU, two dimensions.
     """
-    if dtype not in _FP8:
-        raise TypeError(f"blocks are held in float8_e4m3fn or float8_e5m2, got {dtype}")
-    fmt, rule = native_codes(dtype, rounding)
+    fmt, rule = check_blocks(dtype, rounding)
     if tuple(block) not in ((1, BLOCK), (BLOCK, BLOCK)):
         raise ValueError(f"block must be (1, {BLOCK}) or ({BLOCK}, {BLOCK})")
     if orientation not in ORIENTATIONS:

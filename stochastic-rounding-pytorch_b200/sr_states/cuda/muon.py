@@ -66,7 +66,8 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
     FP16 and FP32 results from pairs of FP16 operands (1e-5 for sides of some
     hundreds, 1e-4 for ten thousand; three times the products); sums are FP32.
     ``x``: FP32, BF16 or FP16, any strides; leading dimensions are a batch.
-    A matrix with a NaN or infinity gives NaN.  Returns a new contiguous tensor.
+    A matrix with a NaN or infinity gives NaN.  Returns a new contiguous tensor without a
+    gradient.
     """
     newton = newton_settings(steps, coefficients, eps)
     _native.launcher().check_device(x.device, "orthogonalize")

@@ -342,6 +342,41 @@ def test_serving_form_and_module(cuda_device):
         assert torch.equal(other, block_linear(x, kept))
 
 
+@pytest.mark.parametrize("shape,outputs", [((0, 256), 128), ((2, 0, 256), 128), ((3, 0), 128),
+                                           ((2, 3, 0), 64), ((2, 3, 256), 0), ((256,), 64),
+                                           ((0,), 64)], ids=str)
+def test_linear_of_vectors_and_sizes_of_zero(shape, outputs, cuda_device):
+    from sr_states import block_linear, quantize_blocks
+
+    # small integers: every block holds them exactly, and BF16 their sums below 256
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randint(-1, 2, shape, generator=gen).to(cuda_device, torch.bfloat16)
+    w = torch.randint(-1, 2, (outputs, shape[-1]), generator=gen).to(cuda_device, torch.bfloat16)
+    x.requires_grad_(), w.requires_grad_()
+    want = x.detach().double() @ w.detach().double().T
+    y = block_linear(x, w)
+    assert y.shape == want.shape and torch.equal(y.double(), want)
+    kept = quantize_blocks(w.detach(), block=(128, 128))
+    with torch.no_grad():
+        assert torch.equal(block_linear(x, kept).double(), want)
+    y.backward(torch.ones_like(y))
+    assert torch.equal(x.grad.double(), torch.ones_like(want) @ w.detach().double())
+    flat = x.detach().double().reshape(want.numel() // outputs if outputs else 6, shape[-1])
+    assert torch.equal(w.grad.double(), torch.ones(
+        (flat.shape[0], outputs), dtype=torch.float64, device=cuda_device).T @ flat)
+
+
+def test_settings_of_the_gradient_are_refused_in_the_forward_pass(cuda_device):
+    from sr_states import block_linear
+
+    x = torch.ones((4, 128), device=cuda_device, requires_grad=True)
+    w = torch.ones((128, 128), device=cuda_device)
+    with pytest.raises(TypeError):
+        block_linear(x, w, grad_dtype=torch.float16)
+    with pytest.raises(ValueError):
+        block_linear(x, w, grad_rounding="upward")
+
+
 def test_refusals(cuda_device):
     from sr_states import BlockTensor, block_linear, matmul_blocks, quantize_blocks
 
