@@ -56,7 +56,7 @@ def quantize_blocks(x, *, dtype=torch.float8_e4m3fn, rounding="nearest", seed=0,
     the pair.  Stochastic counters: element (i, j) of ``x`` uses the hash of its
     flat index + offset + state_key(seed, 0), its transposed copy state_key(seed, 1).
 
-    ``x``: FP32, BF16 or FP16 on an sm_100a GPU, two dimensions.
+    ``x``: FP32, BF16 or FP16 on an sm_100a GPU, two dimensions, at most 4194240 rows.
     """
     fmt, rule = check_blocks(dtype, rounding)
     if tuple(block) not in ((1, BLOCK), (BLOCK, BLOCK)):
