@@ -13,23 +13,28 @@
 // the products read either operand with k or with its row index contiguous, so
 // nothing is ever transposed.
 //
-// Number formats.  G, P and X are held in FP16, accumulated in FP32.  Their sizes are
-// bounded (eigenvalues of a few units), so FP16's 11 significant bits are usable where
-// BF16 would keep 8: the steps multiply rounding errors of small singular directions
-// by up to a^5 = 485, and eight times smaller errors keep the result within about 1e-3
-// of exact arithmetic for gradient-like spectra (1e-2 with BF16).  X_0 is held as
-// V * 2^j with a power of two that puts |V * 2^j|_F between sqrt(min(m, n)) / 4 and
-// sqrt(min(m, n)): BF16 inputs are then held exactly, and the remaining factor rho
-// enters the first products in FP32.  The norm is summed in FP64, so no input in range
-// overflows or vanishes in it.
+// Number formats.  G, P and X are held in FP16, accumulated in FP32: 11 significant bits
+// where BF16 would keep 8.  Errors of G and P act on X from the side of its shorter
+// dimension: they turn directions that X has.  Those of X itself are different: they have
+// directions that X has not (a gradient of few tokens has few), where P is a I, and a
+// step multiplies them by a, five of them by a^5 = 485 (rank 1: 15 % of the result).  So X
+// is carried with what its FP16 leaves, in a second FP16 matrix, until the last step, and
+// the epilogue of X = P X adds a times that second matrix: P acts as a I where it
+// matters, and the product needs no MMA more.  The norms of errors are then 1e-3 to 2e-3 of
+// the result's for noise, low ranks and spectra that fall by any power, 6e-3 for a few
+// orthogonal rows (restated in FP64 and measured; rounding to BF16 adds 1.7e-3).
+//
+// X_0 is held as V * 2^j with a power of two that puts |V * 2^j|_F between 2^14 and 2^15;
+// the remaining factor rho enters the first products in FP32.  The norm is summed in FP64,
+// so no input in range overflows or vanishes in it.  The later X are held times 2^12, far
+// from FP16's smallest numbers.  (Singular values up to 15 fit; the default coefficients
+// keep them below 1.3.)
 //
 // Results in FP32 or FP16 hold more digits than that.  For them (SPLIT) every held
 // matrix is the sum of two FP16 matrices, what the first leaves of a value in the
 // second, and a product of two such is low by high + high by low + high by high: three
 // times the MMAs, errors from 4e-6 (128 x 512) to 1.3e-4 (4096 x 14336; the tensor core
-// truncates its FP32 sums, so they grow with the sides).  X is then held times 2^t,
-// about sqrt of its longer side, so that the second matrices stay clear of FP16's
-// smallest numbers.
+// truncates its FP32 sums, so they grow with the sides).
 //
 // Three launches: the norm, X_0, and one cooperative grid that runs the 3 * steps
 // products of all matrices, whatever their shapes, as phases with a grid-wide meeting
@@ -63,6 +68,9 @@ constexpr int kPlain = -1;        // source template value: a plain tensor
 // G and P are held times 2^8: their small elements (1 / m and less in the first
 // steps) then stay among FP16's normal numbers, and eigenvalues up to 255 fit.
 constexpr float kHeld = 256.0f;
+// X_0 is held with a norm below 2^kTarget, the later X times kHeldX.
+constexpr int kTarget = 15;
+constexpr float kHeldX = 4096.0f;
 
 // A matrix of an optimizer step.
 struct MuonMatrix {
@@ -81,9 +89,8 @@ struct NewtonSource {
   uint32_t row_units;
   int first;          // number of this shape's first matrix among all
   int chunks;         // partial sums of one matrix
-  int target;         // floor(log2(sqrt(min(m, n))))
   __half* x0;
-  int64_t low;        // elements from X_0 to its low part (0: none)
+  int64_t low;        // elements from X_0 to its low part
   int64_t ld, x_elems;
   float* rho;
 };
@@ -202,7 +209,8 @@ newton_sum_kernel(const __grid_constant__ NewtonPlan plan) {
   if (threadIdx.x == 0) plan.partial[(int64_t)blockIdx.y * kSumChunks + blockIdx.x] = total;
 }
 
-// X_0 = V * 2^j in FP16 (row pitch `ld`, padding zero) and rho = (|V|_F + eps) * 2^j.
+// X_0 = V * 2^j in two FP16 matrices (row pitch `ld`, padding zero) and
+// rho = (|V|_F + eps) * 2^j.
 template <int U>
 __global__ void __launch_bounds__(kThreads)
 newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
@@ -217,12 +225,12 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
   int exponent = 0;
   const bool finite = norm < INFINITY;  // false for NaN
   const double fraction = finite ? frexp(norm, &exponent) : 0.0;
-  const int j = s.target - exponent;
+  const int j = kTarget - exponent;
   // Two exact factors, as 2^j itself may not be an FP32 number.
   const float scale0 = finite ? (float)ldexp(1.0, j / 2) : __int_as_float(0x7FC00000);
   const float scale1 = (float)ldexp(1.0, j - j / 2);
   if (blockIdx.x == 0 && threadIdx.x == 0)
-    s.rho[batch] = finite ? (float)ldexp(fraction, s.target) : __int_as_float(0x7FC00000);
+    s.rho[batch] = finite ? (float)ldexp(fraction, kTarget) : __int_as_float(0x7FC00000);
 
   MuonMatrix row{};
   uint32_t ctr = 0;
@@ -239,14 +247,12 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
     encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
     const Unit at = unit_of(s, u, s.ld);
     *reinterpret_cast<uint4*>(out + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (U == kPlain && s.low != 0) {
-      float high[kVec];
-      decode8<SRS_FMT_F16>(w, high);
+    float high[kVec];
+    decode8<SRS_FMT_F16>(w, high);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) v[i] -= high[i];
-      encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
-      *reinterpret_cast<uint4*>(out + s.low + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int i = 0; i < kVec; ++i) v[i] -= high[i];
+    encode8<SRS_FMT_F16>(v, 0u, SRS_RULE_NEAREST, w);
+    *reinterpret_cast<uint4*>(out + s.low + at.at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -267,12 +273,11 @@ struct NewtonClass {
   Divider each_triangle;  // tiles of one G or P
   Divider each_grid;      // tiles of one X
   int64_t ld, x_elems, small_ld, small_elems;
-  int64_t x_low, small_low;  // SPLIT: bytes from a matrix to its low part
+  int64_t x_low, small_low;  // bytes from a matrix to its low part (G, P: SPLIT alone)
   __half* x[2];
   __half* g_at;
   __half* p_at;
   const float* rho;
-  float held;            // X is held times this after the first step
   char* out;             // orthogonalize: the result, contiguous matrices
   int out_format;
   int update;            // Muon: the result updates parameters
@@ -365,8 +370,8 @@ struct NewtonProducts {
     TileStore r{};
     r.row0 = at.row;
     r.col0 = at.col;
-    // The first step's operand stands for X / rho, the others for X / held.
-    float rho = s.held;
+    // The first step's operand stands for X / rho, the others for X / kHeldX.
+    float rho = kHeldX;
     if (step == 0 && kind != 1) rho = s.rho[at.batch];
     r.format = SRS_FMT_F16;
     if (kind != 2) {
@@ -382,6 +387,7 @@ struct NewtonProducts {
         r.beta = w.b;
         r.diagonal = w.a * kHeld;
         r.addend = s.g_at + from;
+        r.addend_phase = p - 1;
         r.out = reinterpret_cast<char*>(s.p_at + from);
       }
     } else {
@@ -389,9 +395,19 @@ struct NewtonProducts {
       r.n = s.n;
       r.factor = __fdiv_rn(1.0f / kHeld, rho);
       if (step + 1 < w.steps) {
-        r.factor *= s.held;
+        r.factor *= kHeldX;
         r.pitch = s.ld;
-        r.low = s.x_low;
+        if (SPLIT) {
+          r.low = s.x_low;
+        } else {
+          // the low part of X, times a; the last step's X has none
+          r.addend = reinterpret_cast<const __half*>(
+              reinterpret_cast<const char*>(s.x[step & 1] + (int64_t)at.batch * s.x_elems) +
+              s.x_low);
+          r.addend_phase = p - 3;  // (below 0: the kernel before this one)
+          r.beta = w.a * __fdiv_rn(kHeldX, rho);
+          if (step + 2 < w.steps) r.low = s.x_low;
+        }
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
       } else if (!SPLIT && s.update != 0) {
         r.update = 1;
@@ -422,7 +438,7 @@ int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 // and G and P, each aligned to 256 bytes.
 struct NewtonShape {
   int64_t batch, m, n, small, ld, small_ld, x_elems, small_elems;
-  int64_t x_low, small_low;  // bytes from a matrix to its low part (0: none)
+  int64_t x_low, small_low;  // bytes from a matrix to its low part (small_low 0: none)
   int64_t rho, x[2], g, p;   // byte offsets
 };
 
@@ -449,7 +465,7 @@ NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, bool split, int64_t* at
   s.small_elems = s.small * s.small_ld;
   const int64_t x_bytes = round_up(batch * s.x_elems * 2, 256);
   const int64_t small_bytes = round_up(batch * s.small_elems * 2, 256);
-  s.x_low = split ? x_bytes : 0;
+  s.x_low = x_bytes;
   s.small_low = split ? small_bytes : 0;
   s.rho = take(at, batch * 4);
   s.x[0] = take(at, x_bytes + s.x_low);
@@ -500,10 +516,6 @@ void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
   if (chunks > most) chunks = most;
   if (chunks > kSumChunks) chunks = kSumChunks;
   f->chunks = chunks < 1 ? 1 : (int)chunks;
-  // SPLIT holds X_0 with elements of about 1, as the later X.
-  const int64_t size = s.x_low != 0 ? s.m * s.n : s.small;
-  f->target = 0;
-  while (f->target < 15 && (1ll << (2 * (f->target + 1))) <= size) ++f->target;
   f->x0 = reinterpret_cast<__half*>(space + s.x[0]);
   f->low = s.x_low / 2;
   f->ld = s.ld;
@@ -540,11 +552,6 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result,
   c->g_at = reinterpret_cast<__half*>(space + s.g);
   c->p_at = reinterpret_cast<__half*>(space + s.p);
   c->rho = reinterpret_cast<const float*>(space + s.rho);
-  c->held = 1.0f;
-  if (SPLIT) {
-    // at most 2^13: |X| stays below a few units, FP16 ends at 65504
-    while (c->held < 8192.0f && 4.0f * c->held * c->held <= (float)longer) c->held *= 2.0f;
-  }
   c->out = static_cast<char*>(result.out);
   c->out_format = result.out_format;
   c->update = result.update ? 1 : 0;

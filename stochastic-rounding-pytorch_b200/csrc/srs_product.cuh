@@ -69,8 +69,9 @@ struct TileStore {
   float beta;      // of `addend`
   float diagonal;  // added where i == j
   const __half* addend;  // m x n, row pitch `pitch` (null: none)
+  int addend_phase;      // the phase that wrote it (negative: an earlier kernel)
   char* out;       // first element of the matrix (update: of the parameter)
-  int64_t low;     // SPLIT: bytes from a 16-bit result (and addend) to its low part; 0: none
+  int64_t low;     // bytes from a 16-bit result (SPLIT: and its addend) to its low part; 0: none
   int format;      // SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t pitch;   // elements
   float step, decay;  // update: p' = fma(step, D, p * decay)
@@ -179,14 +180,22 @@ __device__ __forceinline__ uint32_t staged_slot(uint32_t base, int row, int slot
   return base + row * 16 * SLOTS + 16 * (slot ^ turn);
 }
 
-template <int SLOTS>
-__device__ __forceinline__ void stage_row(uint32_t base, int lane,
-                                          const uint32_t (&w)[4 * SLOTS]) {
+__device__ __forceinline__ void staged_write4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                              uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+
+// A lane's row of a piece: words FIRST, FIRST + STEP, ... of `w`.
+template <int SLOTS, int FIRST = 0, int STEP = 1>
+__device__ __forceinline__ void stage_row(uint32_t base, int lane, const uint32_t (&w)[32]) {
 #pragma unroll
-  for (int j = 0; j < SLOTS; ++j)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_slot<SLOTS>(base, lane, j)),
-                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                 : "memory");
+  for (int j = 0; j < SLOTS; ++j) {
+    const int i = FIRST + 4 * STEP * j;
+    staged_write4(staged_slot<SLOTS>(base, lane, j), w[i], w[i + STEP], w[i + 2 * STEP],
+                  w[i + 3 * STEP]);
+  }
 }
 
 __device__ __forceinline__ uint4 staged_read4(uint32_t addr) {
@@ -312,17 +321,41 @@ __device__ __forceinline__ void update_piece(uint32_t base, char* param, int64_t
   }
 }
 
-// This lane's row of the addend, 32 columns from col0 on (the pitch is a multiple of
-// 8).  Written by an earlier phase of the same kernel: never through the
-// non-coherent path.
-__device__ __forceinline__ void load_addend(const TileStore& t, int row, int col0,
+// The addend's piece of 32 rows and columns from (row0, col0) on, whole rows at a time (the
+// pitch is a multiple of 8): columns 8 (lane % 4) .. of rows lane / 4 + 8 i.  Written by an
+// earlier phase of the same kernel: never through the non-coherent path.
+__device__ __forceinline__ void load_addend(const TileStore& t, int row0, int col0, int lane,
                                             uint4 (&add)[4], int64_t bytes = 0) {
-  const char* from = reinterpret_cast<const char*>(t.addend + (int64_t)row * t.pitch + col0) + bytes;
+  const int row = row0 + (lane >> 2), col = col0 + 8 * (lane & 3);
+  const char* from = reinterpret_cast<const char*>(t.addend + (int64_t)row * t.pitch + col) + bytes;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    add[j] = (row < t.m && col0 + 8 * j < t.pitch)
-                 ? __ldcg(reinterpret_cast<const uint4*>(from) + j)
+  for (int i = 0; i < 4; ++i)
+    add[i] = (row + 8 * i < t.m && col < t.pitch)
+                 ? __ldcg(reinterpret_cast<const uint4*>(from + 16 * i * t.pitch))
                  : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// v += beta * that piece, turned to this lane's row in the staging memory.
+__device__ __forceinline__ void add_piece(const uint4 (&add)[4], float beta, uint32_t staged,
+                                          int lane, uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    staged_write4(staged_slot<4>(staged, 8 * i + (lane >> 2), lane & 3), add[i].x, add[i].y,
+                  add[i].z, add[i].w);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 q = staged_read4(staged_slot<4>(staged, lane, j));
+    const uint32_t pairs[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 g = f16x2_to_float2(pairs[i]);
+      uint32_t* to = v + 8 * j + 2 * i;
+      to[0] = __float_as_uint(fmaf(beta, g.x, __uint_as_float(to[0])));
+      to[1] = __float_as_uint(fmaf(beta, g.y, __uint_as_float(to[1])));
+    }
+  }
+  __syncwarp();
 }
 
 // 32 accumulator columns from col0 on for a warp's 32 rows from row0 on: v[c] is
@@ -338,51 +371,43 @@ __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int 
   for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * t.factor);
   const auto value = [&](int c) { return __uint_as_float(v[c]); };
   if (t.format != SRS_FMT_F32 && !(NEWTON && t.update != 0)) {
-    uint32_t w[16];
     if (NEWTON && t.addend != nullptr) {
-      const auto accumulate = [&](const uint4 (&part)[4]) {
-        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(part);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 g = f16x2_to_float2(pairs[i]);
-          v[2 * i] = __float_as_uint(fmaf(t.beta, g.x, value(2 * i)));
-          v[2 * i + 1] = __float_as_uint(fmaf(t.beta, g.y, value(2 * i + 1)));
-        }
-      };
-      accumulate(add);
+      add_piece(add, t.beta, staged, lane, v);
       if (SPLIT) {
-        uint4 low[4];
-        load_addend(t, row, col0, low, t.low);
-        accumulate(low);
+        load_addend(t, row0, col0, lane, add, t.low);
+        add_piece(add, t.beta, staged, lane, v);
       }
+      if (next_col >= 0) load_addend(t, row0, next_col, lane, add);
+      if (t.diagonal != 0.0f) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (row == col0 + i) v[i] = __float_as_uint(value(i) + t.diagonal);
+        for (int i = 0; i < 32; ++i)
+          if (row == col0 + i) v[i] = __float_as_uint(value(i) + t.diagonal);
+      }
+    }
+    // Pairs in place: the rounded pair at 2 i and what it leaves (exact in FP32) at 2 i + 1.
+    const bool low = NEWTON && t.low != 0;
+    if (t.format == SRS_FMT_BF16) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_half(value(2 * i), value(2 * i + 1));
-      if (next_col >= 0) load_addend(t, row, next_col, add);
-    } else if (t.format == SRS_FMT_BF16) {
+      for (int i = 0; i < 32; i += 2) v[i] = pack_bf16(value(i), value(i + 1));
+    } else if (low) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(value(2 * i), value(2 * i + 1));
+      for (int i = 0; i < 32; i += 2) {
+        const uint32_t pair = pack_half(value(i), value(i + 1));
+        const float2 high = f16x2_to_float2(pair);
+        v[i + 1] = pack_half(value(i) - high.x, value(i + 1) - high.y);
+        v[i] = pair;
+      }
+      stage_row<4, 1, 2>(staged + kPieceBytes / 2, lane, v);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_half(value(2 * i), value(2 * i + 1));
+      for (int i = 0; i < 32; i += 2) v[i] = pack_half(value(i), value(i + 1));
     }
-    stage_row<4>(staged, lane, w);
+    stage_row<4, 0, 2>(staged, lane, v);
     __syncwarp();
     store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
-    if (SPLIT && t.low != 0) {
-      // what the high part leaves of the value (exact in FP32)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 high = f16x2_to_float2(w[i]);
-        w[i] = pack_half(value(2 * i) - high.x, value(2 * i + 1) - high.y);
-      }
-      __syncwarp();
-      stage_row<4>(staged, lane, w);
-      __syncwarp();
-      store_piece<4>(staged, t.out + t.low + 2 * at, t.pitch, rows, t.n - col0, lane);
-    }
+    if (low)
+      store_piece<4>(staged + kPieceBytes / 2, t.out + t.low + 2 * at, t.pitch, rows, t.n - col0,
+                     lane);
   } else {
     stage_row<8>(staged, lane, v);
     __syncwarp();
@@ -729,9 +754,8 @@ __device__ __forceinline__ void run_products(const Source& src) {
     constexpr int kPieces = S::kTileCols / (8 * S::kWriters);
     const int part = warp >> 2, quarter = warp & 3;
     const uint32_t staged = staged0 + warp * kPieceBytes;
-    int count = 0;
+    int count = 0, met = -1;  // met: the last phase known to be complete
     for (int p = 0; p < phases && ok; ++p) {
-      bool met = p == 0;
       const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step, ++count) {
         const TileStore at = src.store(p, t);
@@ -740,14 +764,15 @@ __device__ __forceinline__ void run_products(const Source& src) {
         uint4 add[4];
         if (NEWTON && at.addend != nullptr) {
           // the one thing these warps read of an earlier phase
-          if (!met) {
+          if (met < at.addend_phase) {
             if (lane == 0)
-              ok = counter_wait(src.counter(p - 1), gridDim.x, status, 1u << 17);
+              ok = counter_wait(src.counter(at.addend_phase), gridDim.x, status, 1u << 17);
             ok = __all_sync(0xFFFFFFFFu, ok);
+            __syncwarp();  // what lane 0 has acquired, for the other lanes' loads
             if (!ok) break;
-            met = true;
+            met = at.addend_phase;
           }
-          load_addend(at, row0 + lane, at.col0 + 32 * part * kPieces, add);
+          load_addend(at, row0, at.col0 + 32 * part * kPieces, lane, add);
         }
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u);
         ok = __all_sync(0xFFFFFFFFu, ok);
