@@ -33,8 +33,13 @@
 // Results in FP32 or FP16 hold more digits than that.  For them (SPLIT) every held
 // matrix is the sum of two FP16 matrices, what the first leaves of a value in the
 // second, and a product of two such is low by high + high by low + high by high: three
-// times the MMAs, errors from 4e-6 (128 x 512) to 1.3e-4 (4096 x 14336; the tensor core
-// truncates its FP32 sums, so they grow with the sides).
+// times the MMAs, errors for noise from 4e-6 (128 x 512) to 7e-5 (4096 x 14336).  The
+// tensor core truncates its FP32 sums, so errors grow with the sides, and with few
+// directions, as above, to more: rank 2 4e-5 (128 x 128), 2.5e-4 (768 x 768), 1.4e-3
+// (4096 x 4096); FP32 sums rounded to nearest 5e-5 at 768.  So P is held without its
+// a I, and the epilogue adds all of a X: shorter sums to truncate (with a I in P: noise
+// 9e-5, rank 8 at 768 1.7e-4 instead of 8e-5).  (Sums of the first two steps in parts of
+// 512 of k, joined in the epilogue: rank 1 worse, 15 % more time at 4096 x 14336; not kept.)
 //
 // Three launches: the norm, X_0, and one cooperative grid that runs the 3 * steps
 // products of all matrices, whatever their shapes, as phases with a grid-wide meeting
@@ -299,7 +304,8 @@ struct NewtonWork {
   unsigned int* status_at;
 };
 
-// Phase 3 i: G = X X^T; 3 i + 1: P = a I + b G + c G G; 3 i + 2: X = P X.
+// Phase 3 i: G = X X^T; 3 i + 1: P = a I + b G + c G G; 3 i + 2: X = P X.  (SPLIT: a X by
+// itself, so that P has no a I, except in the last step, whose result is not in FP16.)
 template <bool SPLIT>
 struct NewtonProducts {
   const NewtonWork<SPLIT>& w;
@@ -385,7 +391,7 @@ struct NewtonProducts {
       } else {
         r.factor = w.c / kHeld;
         r.beta = w.b;
-        r.diagonal = w.a * kHeld;
+        if (!SPLIT || step + 1 == w.steps) r.diagonal = w.a * kHeld;
         r.addend = s.g_at + from;
         r.addend_phase = p - 1;
         r.out = reinterpret_cast<char*>(s.p_at + from);
@@ -397,17 +403,14 @@ struct NewtonProducts {
       if (step + 1 < w.steps) {
         r.factor *= kHeldX;
         r.pitch = s.ld;
-        if (SPLIT) {
-          r.low = s.x_low;
-        } else {
-          // the low part of X, times a; the last step's X has none
-          r.addend = reinterpret_cast<const __half*>(
-              reinterpret_cast<const char*>(s.x[step & 1] + (int64_t)at.batch * s.x_elems) +
-              s.x_low);
-          r.addend_phase = p - 3;  // (below 0: the kernel before this one)
-          r.beta = w.a * __fdiv_rn(kHeldX, rho);
-          if (step + 2 < w.steps) r.low = s.x_low;
-        }
+        // a times X (SPLIT) or its low part; the last step's X has none
+        const __half* const x = s.x[step & 1] + (int64_t)at.batch * s.x_elems;
+        r.addend = SPLIT ? x
+                         : reinterpret_cast<const __half*>(reinterpret_cast<const char*>(x) +
+                                                           s.x_low);
+        r.addend_phase = p - 3;  // (below 0: the kernel before this one)
+        r.beta = w.a * __fdiv_rn(kHeldX, rho);
+        if (SPLIT || step + 2 < w.steps) r.low = s.x_low;
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
       } else if (!SPLIT && s.update != 0) {
         r.update = 1;

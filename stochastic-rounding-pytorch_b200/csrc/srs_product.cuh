@@ -57,7 +57,7 @@ struct TileLoad {
   // beside one another ([0] and [1] of every pointer above).  `slices` counts k three
   // times: low by high, high by low, then high by high parts.  (The tensor core truncates
   // its FP32 sums at every step: the small parts go first, while the sum is small;
-  // 4096 x 14336 to FP32 is 1.3e-4 off, with the high parts first 2.5e-4.)
+  // 4096 x 14336 to FP32 was 1.3e-4 off so, with the high parts first 2.5e-4.)
 };
 
 // What happens to a tile's accumulator.

@@ -59,6 +59,20 @@ def test_low_ranks_and_falling_spectra(size, source, cuda_device):
         assert off <= 16 * U + BF16, (name, off)
 
 
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_fp32_results_of_low_ranks_and_falling_spectra(size, cuda_device):
+    """Pairs of FP16 numbers leave 2^-22 of an element, 2^-12 after the amplification.  The
+    tensor core truncates: each of the k terms of a sum takes up to 2^-24 of it, all of one
+    sign, and the steps that follow multiply what the first ones lose by 3.4445^4 + 3.4445^3
+    + ... < 200."""
+    from sr_states import orthogonalize
+
+    for name, x in matrices(*size).items():
+        x = x.float().to(cuda_device)
+        off = relative(orthogonalize(x), newton(x))
+        assert off <= 2.0**-12 + 200 * min(size) * 2.0**-24, (name, off)
+
+
 @pytest.mark.parametrize("param", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_muon_updates_of_low_rank_gradients(param, cuda_device):
     """The first step of a run: no momentum, gradients of few tokens."""
