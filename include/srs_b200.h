@@ -350,6 +350,11 @@ typedef struct srs_muon_hparams {
 
 int64_t srs_muon_workspace(const srs_muon_class* classes, int n_classes);
 
+/* Side of the tiles in which a call with these matrices computes its products: 256 (two
+ * CTAs a tile) or 128; negative: invalid sizes.  y_format as for srs_orthogonalize; Muon
+ * steps take SRS_FMT_BF16. */
+int srs_newton_tile(const srs_muon_class* classes, int n_classes, int y_format);
+
 int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes, int n_classes,
                    int u_format, int u_rule, const srs_muon_hparams* hp, const srs_newton* h,
                    const srs_rng* rng, void* workspace, int64_t workspace_bytes, void* stream);

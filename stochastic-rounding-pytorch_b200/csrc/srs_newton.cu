@@ -580,7 +580,7 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result,
 }
 
 template <int CG, bool SPLIT>
-int launch_newton(NewtonWork<SPLIT>& w, const int64_t* batch, cudaStream_t stream) {
+int launch_newton(NewtonWork<SPLIT>& w, const srs_muon_class* shapes, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(&newton_kernel<CG, SPLIT>);
   using S = ProductShape<kOperandF16, CG>;
   int resident = 0;
@@ -596,8 +596,8 @@ int launch_newton(NewtonWork<SPLIT>& w, const int64_t* batch, cudaStream_t strea
     c.each_grid = make_divider(c.grid.rows * c.grid.cols);
     w.triangles[i] = (uint32_t)triangles;
     w.grids[i] = (uint32_t)grids;
-    triangles += batch[i] * c.each_triangle.d;
-    grids += batch[i] * c.each_grid.d;
+    triangles += shapes[i].count * c.each_triangle.d;
+    grids += shapes[i].count * c.each_grid.d;
   }
   w.triangles[w.classes] = (uint32_t)triangles;
   w.grids[w.classes] = (uint32_t)grids;
@@ -613,23 +613,23 @@ int launch_newton(NewtonWork<SPLIT>& w, const int64_t* batch, cudaStream_t strea
 // the loads for it), and what a tile's results take.  Measured (us, single against
 // pair): 1024^2 144, 201; 2048^2 241, 285; 2500^2 422, 390; 3500^2 894, 783;
 // 16 x 768^2 295, 367; 24 x 768^2 402, 365; 4 x (1024 x 4096) 347, 381.
-template <bool SPLIT>
-double step_cycles(const NewtonWork<SPLIT>& w, const int64_t* batch, int cg) {
-  const int64_t groups = sm_count() / cg;
+double step_cycles(const srs_muon_class* shapes, int count, bool split, int cg) {
+  const int64_t groups = sm_count() / cg, edge = 128 * cg;
   const double slice = cg == 2 ? 512.0 : 350.0, rest = cg == 2 ? 5000.0 : 2000.0;
   double total = 0.0;
   for (int kind = 0; kind < 3; ++kind) {
     double work = 0.0, longest = 0.0;
     int64_t tiles = 0;
-    for (int i = 0; i < w.classes; ++i) {
-      const NewtonClass<SPLIT>& c = w.shape[i];
-      const int64_t edge = 128 * cg, t = (c.small + edge - 1) / edge;
-      const int64_t each = kind < 2 ? t * (t + 1) / 2
-                                    : (c.m + edge - 1) / edge * ((c.n + edge - 1) / edge);
+    for (int i = 0; i < count; ++i) {
+      const srs_muon_class& c = shapes[i];
+      const int64_t small = c.m < c.n ? c.m : c.n, t = (small + edge - 1) / edge;
+      const int64_t each =
+          kind < 2 ? t * (t + 1) / 2 : (c.m + edge - 1) / edge * ((c.n + edge - 1) / edge);
+      const int64_t summed = kind == 0 ? c.m + c.n - small : small;
       const double cycles =
-          (SPLIT ? 3.0 : 1.0) * slice * (kind == 0 ? c.long_slices : c.small_slices) + rest;
-      tiles += batch[i] * each;
-      work += cycles * (double)(batch[i] * each);
+          (split ? 3.0 : 1.0) * slice * (double)((summed + 63) / 64) + rest;
+      tiles += c.count * each;
+      work += cycles * (double)(c.count * each);
       if (cycles > longest) longest = cycles;
     }
     // whole rounds of the grid, at the tiles' mean cost
@@ -640,8 +640,13 @@ double step_cycles(const NewtonWork<SPLIT>& w, const int64_t* batch, int cg) {
   return total;
 }
 
+// CTAs to a tile: 2 or 1.
+int tile_group(const srs_muon_class* shapes, int count, bool split) {
+  return step_cycles(shapes, count, split, 2) <= step_cycles(shapes, count, split, 1) ? 2 : 1;
+}
+
 template <bool SPLIT>
-int run_newton(NewtonWork<SPLIT>& w, const int64_t* batch, const srs_newton* h,
+int run_newton(NewtonWork<SPLIT>& w, const srs_muon_class* shapes, const srs_newton* h,
                unsigned int* counters, cudaStream_t stream) {
   w.steps = h->steps;
   w.a = h->coefficients[0];
@@ -649,9 +654,8 @@ int run_newton(NewtonWork<SPLIT>& w, const int64_t* batch, const srs_newton* h,
   w.c = h->coefficients[2];
   w.counters = counters;
   if (int rc = status_word(&w.status_at)) return rc;
-  return step_cycles(w, batch, 2) <= step_cycles(w, batch, 1)
-             ? launch_newton<2, SPLIT>(w, batch, stream)
-             : launch_newton<1, SPLIT>(w, batch, stream);
+  return tile_group(shapes, w.classes, SPLIT) == 2 ? launch_newton<2, SPLIT>(w, shapes, stream)
+                                                   : launch_newton<1, SPLIT>(w, shapes, stream);
 }
 
 int check_matrices(int64_t batch, int64_t m, int64_t n) {
@@ -744,7 +748,8 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
     work.classes = 1;
     if (int rc = fill_class(shape, space, result, &work.shape[0])) return rc;
     if (int rc = launch_prepare<kPlain>(plan, batch, s.chunks, st)) return rc;
-    return run_newton(work, &batch, h, plan.counters, st);
+    const srs_muon_class matrices{batch, m, n, 0.0f, 0};
+    return run_newton(work, &matrices, h, plan.counters, st);
   };
   if (y_format != SRS_FMT_BF16) {
     NewtonWork<true> work{};
@@ -771,6 +776,16 @@ static int check_classes(const srs_muon_class* classes, int n_classes, int64_t* 
     return fail(SRS_ERR_INVALID_ARGUMENT, "%lld matrices in one call (at most %d)",
                 (long long)*matrices, kMaxMatrices);
   return SRS_OK;
+}
+
+extern "C" int srs_newton_tile(const srs_muon_class* classes, int n_classes, int y_format) {
+  clear_error();
+  if (n_classes < 0 || n_classes > SRS_MUON_MAX_CLASSES || (n_classes > 0 && classes == nullptr))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "between 0 and %d shapes in a call, got %d",
+                SRS_MUON_MAX_CLASSES, n_classes);
+  for (int i = 0; i < n_classes; ++i)
+    if (int rc = check_matrices(classes[i].count, classes[i].m, classes[i].n)) return rc;
+  return 128 * tile_group(classes, n_classes, y_format != SRS_FMT_BF16);
 }
 
 extern "C" int64_t srs_muon_workspace(const srs_muon_class* classes, int n_classes) {
@@ -831,7 +846,6 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
   plan.u_rule = u_rule;
   NewtonWork<false> work{};
   work.classes = n_classes;
-  int64_t batch[kMaxClasses];
   int first = 0, chunks = 1;
   for (int i = 0; i < n_classes; ++i) {
     const srs_muon_class& c = classes[i];
@@ -841,7 +855,6 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
     if (s.chunks > chunks) chunks = s.chunks;
     const NewtonResult result{nullptr, 0, true, first, hp->decay, c.neg_step};
     if (int rc = fill_class(shape, space, result, &work.shape[i])) return rc;
-    batch[i] = c.count;
     first += (int)c.count;
   }
   for (int64_t i = 0; i < matrices; ++i) {
@@ -859,5 +872,5 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
     default: rc = launch_prepare<SRS_FMT_E5M2>(plan, matrices, chunks, st); break;
   }
   if (rc != SRS_OK) return rc;
-  return run_newton(work, batch, h, plan.counters, st);
+  return run_newton(work, classes, h, plan.counters, st);
 }

@@ -160,6 +160,7 @@ _SIGNATURES = {
                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                            ctypes.POINTER(SrsNewton), _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_muon_workspace": ([ctypes.POINTER(SrsMuonClass), ctypes.c_int], ctypes.c_int64),
+    "srs_newton_tile": ([ctypes.POINTER(SrsMuonClass), ctypes.c_int, ctypes.c_int], ctypes.c_int),
     "srs_muon_multi": ([_P, ctypes.POINTER(SrsMuonClass), ctypes.c_int, ctypes.c_int,
                         ctypes.c_int, ctypes.POINTER(SrsMuonHparams), ctypes.POINTER(SrsNewton),
                         ctypes.POINTER(SrsRng), _P, ctypes.c_int64, _P], ctypes.c_int),
