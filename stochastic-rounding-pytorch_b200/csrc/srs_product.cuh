@@ -81,6 +81,10 @@ struct TileStore {
 // kb + 3 of each, one byte a block.  Rows outside the matrix read its last row
 // instead (their data are zeros and their results are not stored); blocks from
 // `last` on give 1 (127).  Rows on 4-byte boundaries are read a word at a time.
+//
+// FRESH: the kernel ahead in the stream may write the scales while this one runs; they are
+// then read (behind the wait for that kernel) through L2, never through the non-coherent
+// path, which may hold what an earlier call left at their address.
 struct ScaleRows {
   const uint8_t* row[4];
   __device__ __forceinline__ void at(const uint8_t* scale, int64_t pitch, int shift, int first,
@@ -89,10 +93,17 @@ struct ScaleRows {
     for (int j = 0; j < 4; ++j)
       row[j] = scale + (int64_t)(min(first + lane + 32 * j, rows - 1) >> shift) * pitch;
   }
+  template <bool FRESH = false, class T>
+  __device__ static __forceinline__ T load(const T* p) {
+    if constexpr (FRESH) return __ldcg(p);
+    return __ldg(p);
+  }
+  template <bool FRESH = false>
   __device__ __forceinline__ void read(int kb, int last, bool words, uint32_t (&w)[4]) const {
     if (words && kb + 4 <= last) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row[j] + kb));
+      for (int j = 0; j < 4; ++j)
+        w[j] = load<FRESH>(reinterpret_cast<const uint32_t*>(row[j] + kb));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -100,7 +111,8 @@ struct ScaleRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (kb + i < last)
-            w[j] = (w[j] & ~(0xFFu << (8 * i))) | ((uint32_t)__ldg(row[j] + kb + i) << (8 * i));
+            w[j] = (w[j] & ~(0xFFu << (8 * i))) |
+                   ((uint32_t)load<FRESH>(row[j] + kb + i) << (8 * i));
       }
     }
   }

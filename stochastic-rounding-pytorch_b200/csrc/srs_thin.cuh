@@ -242,7 +242,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       from_a.read(kb, last, words_a, w[0]);
       if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
       waited = true;
-      from_b.read(kb, last, words_b, w[1]);
+      from_b.read<true>(kb, last, words_b, w[1]);
       ok = barrier_wait(scale_empty(slot), ((uint32_t)(g / kThinSlots) & 1u) ^ 1u, a.status,
                         1u << 12);
       ok = __all_sync(0xFFFFFFFFu, ok);
