@@ -372,8 +372,9 @@ int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes, int n_cla
  * along x's rows); either pair may be NULL.  Stochastic counters: element (i, j) of
  * x uses (i*cols + j + offset + state_key(seed, 0)) mod 2^32, its transposed copy
  * state_key(seed, 1).  x: FP32, BF16 or FP16, element (i, j) at i*x_pitch + j.  Row
- * pitches of data and data_t are in elements, those of scale and scale_t in blocks.  At
- * most 4194240 rows and 2^30 columns a call.
+ * pitches of data and data_t are in elements, those of scale and scale_t in blocks; the
+ * copies' addresses and pitches are multiples of 16, and nothing is written outside their
+ * rows and columns.  At most 4194240 rows and 2^30 columns a call.
  *
  * srs_matmul_blocks: d[i, j] = sum_k a[i, k] * b[j, k] with FP32 sums, d in FP32,
  * BF16 or FP16 (contiguous).  The data's base addresses and row pitches must be

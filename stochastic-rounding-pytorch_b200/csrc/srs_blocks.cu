@@ -166,6 +166,18 @@ __device__ __forceinline__ uint2 encode_values(const float (&y)[kVec], uint32_t 
                             make_float4(y[4], y[5], y[6], y[7]), ctr, rule);
 }
 
+// `left` of the bytes in `w` (all, or those up to the end of a row): nothing is written outside
+// the matrix, so that a copy may be columns of a wider buffer.
+__device__ __forceinline__ void store_bytes(uint8_t* out, uint2 w, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<uint2*>(out) = w;
+  } else {
+    uint64_t bytes = (uint64_t)w.y << 32 | w.x;
+#pragma unroll 1
+    for (int j = 0; j < left; ++j, bytes >>= 8) out[j] = (uint8_t)bytes;
+  }
+}
+
 // Rows alone, 1 x 128 blocks: 16 lanes to a block, kAhead blocks of one column a
 // half-warp with all their loads first.  HBM-bound when rounding to nearest (8192 x
 // 4096: 25 us with the launch; 3 bytes an element at 6.5 TB/s would be 15), by the integer
@@ -194,6 +206,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
     a.scale[(row0 + lane16) * a.scale_pitch + blockIdx.x] = (uint8_t)(own_k + 127);
   const float own_factor = power_of_two(-own_k);
   plain = plain && a.rule != SRS_RULE_TOWARD_ZERO;
+  const int cols_left = (int)min(a.cols - col, (int64_t)kVec);
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int64_t row = row0 + i;
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
     for (int j = 0; j < kVec; ++j) y[j] *= factor;
     const uint2 w =
         encode_values<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, plain);
-    if (col < a.data_pitch) *reinterpret_cast<uint2*>(a.data + row * a.data_pitch + col) = w;
+    store_bytes(a.data + row * a.data_pitch + col, w, cols_left);
   }
 }
 
@@ -349,7 +362,8 @@ quantize_tile_kernel(const QuantizeArgs a) {
   uint32_t ctr = a.ctr + (uint32_t)(row_base * a.cols + col);
   uint32_t ctr_t = a.ctr_t + (uint32_t)(row_base * a.cols + col);
   const float tile_factor = power_of_two(-tile_k);
-  const int rows_left = col < a.data_pitch ? (int)min(a.rows - row_base, (int64_t)8) : 0;
+  const int rows_left = (int)min(a.rows - row_base, (int64_t)8);
+  const int cols_left = (int)min(a.cols - col, (int64_t)kVec);
   uint8_t* out = a.data + row_base * a.data_pitch + col;
   uint32_t* turn = turned + (COLS ? 8 * group * 32 + ((2 * lane16 + 4 * (group >> 1)) & 31) : 0);
 #pragma unroll 1
@@ -370,7 +384,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) y[j] = x[j] * factor;
       const uint2 w = encode_values<OF>(y, ctr, a.rule, plain);
-      if (i < rows_left) *reinterpret_cast<uint2*>(out) = w;
+      if (i < rows_left) store_bytes(out, w, cols_left);
       out += a.data_pitch;
     }
     if constexpr (COLS) {
@@ -408,12 +422,18 @@ quantize_tile_kernel(const QuantizeArgs a) {
       }
     }
     const int64_t at = row0 + 16 * h;
+    const int left = (int)min(a.rows - at, (int64_t)16);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t to = col0 + 4 * word + c;
-      if (to < a.cols && at < a.data_t_pitch)
-        *reinterpret_cast<uint4*>(a.data_t + to * a.data_t_pitch + at) =
-            make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+      if (to >= a.cols) continue;
+      uint8_t* const dst = a.data_t + to * a.data_t_pitch + at;
+      if (left >= 16) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+      } else {
+        store_bytes(dst, make_uint2(out[c][0], out[c][1]), left);
+        store_bytes(dst + 8, make_uint2(out[c][2], out[c][3]), left - 8);
+      }
     }
   }
 }
