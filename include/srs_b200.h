@@ -36,6 +36,7 @@ extern "C" {
 #define SRS_ERR_INVALID_ARGUMENT (-1) /* bad pointer, size, format, rule or flag */
 #define SRS_ERR_UNSUPPORTED_DEVICE (-2) /* current device is not compute capability 10.0 */
 #define SRS_ERR_CUDA (-3)             /* a CUDA runtime call failed (launch, attribute query) */
+#define SRS_ERR_WAIT (-4)             /* a wait in an earlier product kernel ran out */
 
 /* ---- storage formats (state, cast output) ------------------------------ */
 #define SRS_FMT_F32 0
@@ -411,9 +412,16 @@ int srs_linear_blocks(const void* x, int x_format, int64_t tokens, int64_t k, in
 int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols, void* dst,
                   int64_t dst_pitch, void* stream);
 
-/* Where a bounded wait of a product kernel ran out on the current device (0:
- * nowhere; results of such a call are not valid).  Synchronises the device. */
+/* Waits inside the product kernels are bounded (about 2 s).  One that runs out is recorded
+ * in a word of host memory, one a device, and the results of that call are not valid (a
+ * Muon step's parameters and momentum neither).  The next srs_orthogonalize,
+ * srs_muon_multi, srs_matmul_blocks or srs_linear_blocks on the device enqueues nothing,
+ * clears the word and returns SRS_ERR_WAIT.
+ * srs_product_status: synchronises the current device, gives the word (0: no wait ran out
+ * since it was last cleared) and clears it.
+ * srs_product_status_word: the word's host address, to look at without synchronising. */
 int srs_product_status(uint32_t* status);
+int srs_product_status_word(uint32_t** word);
 
 #ifdef __cplusplus
 }

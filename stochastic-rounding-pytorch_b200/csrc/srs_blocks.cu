@@ -544,9 +544,10 @@ int check_operand(const char* what, const srs_blocks* b, int64_t k) {
 
 using namespace srs;
 
-static int quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
-                           int64_t x_pitch, int out_format, int rule, int square, uint32_t seed,
-                           uint32_t offset, void* data, int64_t data_pitch, void* scale,
+// `for_product`: ahead of a product in the same call.
+static int quantize_blocks(bool for_product, const void* x, int x_format, int64_t rows,
+                           int64_t cols, int64_t x_pitch, int out_format, int rule, int square,
+                           uint32_t seed, uint32_t offset, void* data, int64_t data_pitch, void* scale,
                            int64_t scale_pitch, void* data_t, int64_t data_t_pitch, void* scale_t,
                            int64_t scale_t_pitch, cudaStream_t stream) {
   if (x_format < SRS_FMT_F32 || x_format > SRS_FMT_F16)
@@ -572,6 +573,8 @@ static int quantize_blocks(const void* x, int x_format, int64_t rows, int64_t co
                             rows))
       return rc;
   if (int rc = check_device()) return rc;
+  if (for_product)
+    if (int rc = check_products()) return rc;
   QuantizeArgs a{};
   a.x = x;
   a.rows = rows;
@@ -603,9 +606,9 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
                                    int64_t data_t_pitch, void* scale_t, int64_t scale_t_pitch,
                                    void* stream) {
   clear_error();
-  return quantize_blocks(x, x_format, rows, cols, x_pitch, out_format, rule, square, seed, offset,
-                         data, data_pitch, scale, scale_pitch, data_t, data_t_pitch, scale_t,
-                         scale_t_pitch, static_cast<cudaStream_t>(stream));
+  return quantize_blocks(false, x, x_format, rows, cols, x_pitch, out_format, rule, square, seed,
+                         offset, data, data_pitch, scale, scale_pitch, data_t, data_t_pitch,
+                         scale_t, scale_t_pitch, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols,
@@ -645,6 +648,7 @@ extern "C" int srs_matmul_blocks(const srs_blocks* a, const srs_blocks* b, int64
   if (d == nullptr || reinterpret_cast<uintptr_t>(d) % fmt_bytes(d_format) != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
   if (int rc = check_device()) return rc;
+  if (int rc = check_products()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (k == 0) {
     const cudaError_t e =
@@ -687,8 +691,8 @@ extern "C" int srs_linear_blocks(const void* x, int x_format, int64_t tokens, in
   rows.format = block_format;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (k == 0) return srs_matmul_blocks(&rows, w, k, d, x_format, stream);
-  if (int rc = quantize_blocks(x, x_format, tokens, k, x_pitch, block_format, SRS_RULE_NEAREST, 0,
-                               0u, 0u, workspace, rows.pitch,
+  if (int rc = quantize_blocks(true, x, x_format, tokens, k, x_pitch, block_format,
+                               SRS_RULE_NEAREST, 0, 0u, 0u, workspace, rows.pitch,
                                static_cast<char*>(workspace) + tokens * rows.pitch,
                                rows.scale_pitch, nullptr, 0, nullptr, 0, st))
     return rc;

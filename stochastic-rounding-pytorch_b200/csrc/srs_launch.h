@@ -23,8 +23,12 @@ struct ProductOperand {
 int encode_operand(const ProductOperand& o, int element_bytes, int64_t batch, int box_rows,
                    CUtensorMap* map);
 
-// Device address of the word in which bounded waits record where they ran out.
+// The word of the current device in which bounded waits record where they ran out.
 int status_word(unsigned int** word);
+
+// SRS_ERR_WAIT, once, when a wait has run out since the last check: every entry point that
+// launches products asks before its first launch.
+int check_products();
 
 // Opt-in shared memory of a kernel, and how many of its CTA groups (1 or 2 CTAs) can be
 // resident on the current device; remembered per kernel and device.

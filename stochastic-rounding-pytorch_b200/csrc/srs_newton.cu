@@ -726,6 +726,7 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   if (int rc = check_space(workspace, workspace_bytes, srs_newton_workspace(batch, m, n, y_format)))
     return rc;
   if (int rc = check_device()) return rc;
+  if (int rc = check_products()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* space = static_cast<char*>(workspace);
   int64_t used = 0;
@@ -831,6 +832,7 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
   if (int rc = check_space(workspace, workspace_bytes, srs_muon_workspace(classes, n_classes)))
     return rc;
   if (int rc = check_device()) return rc;
+  if (int rc = check_products()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* space = static_cast<char*>(workspace);
   int64_t used = 0;

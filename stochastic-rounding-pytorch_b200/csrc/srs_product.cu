@@ -19,9 +19,7 @@ constexpr int kMaxDevices = 128;
 std::mutex g_lock;
 EncodeTiled g_encode = nullptr;
 std::unordered_map<const void*, int> g_resident[kMaxDevices];
-unsigned int* g_status[kMaxDevices];
-
-__device__ unsigned int g_product_status;  // where a bounded wait ran out (0: nowhere)
+unsigned int* g_status[kMaxDevices];  // host memory: where a bounded wait ran out (0: nowhere)
 
 int device_index(int* dev) {
   const cudaError_t e = cudaGetDevice(dev);
@@ -77,13 +75,26 @@ int status_word(unsigned int** word) {
   if (int rc = device_index(&dev)) return rc;
   std::lock_guard<std::mutex> lock(g_lock);
   if (g_status[dev] == nullptr) {
-    void* p = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&p, g_product_status);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(product status)");
+    void* p = nullptr;  // one address for the host and the device (unified addressing)
+    const cudaError_t e =
+        cudaHostAlloc(&p, sizeof(unsigned int), cudaHostAllocMapped | cudaHostAllocPortable);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaHostAlloc(product status)");
     g_status[dev] = static_cast<unsigned int*>(p);
+    *g_status[dev] = 0u;
   }
   *word = g_status[dev];
   return SRS_OK;
+}
+
+int check_products() {
+  unsigned int* word = nullptr;
+  if (int rc = status_word(&word)) return rc;
+  if (__atomic_load_n(word, __ATOMIC_RELAXED) == 0u) return SRS_OK;
+  const unsigned int where = __atomic_exchange_n(word, 0u, __ATOMIC_RELAXED);
+  return fail(SRS_ERR_WAIT,
+              "a wait inside an earlier product kernel on this device ran out (0x%x): the results "
+              "of product calls since the last check are not valid",
+              where);
 }
 
 int prepare_kernel(const void* kernel, int group, int threads, int smem, int* resident) {
@@ -353,6 +364,18 @@ extern "C" int srs_product_status(uint32_t* status) {
   clear_error();
   if (status == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null status");
   if (int rc = check_device()) return rc;
-  const cudaError_t e = cudaMemcpyFromSymbol(status, g_product_status, sizeof(*status));
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "product status");
+  unsigned int* word = nullptr;
+  if (int rc = status_word(&word)) return rc;
+  const cudaError_t e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return cuda_fail(e, "product status");
+  *status = __atomic_exchange_n(word, 0u, __ATOMIC_RELAXED);
+  return SRS_OK;
+}
+
+extern "C" int srs_product_status_word(uint32_t** word) {
+  using namespace srs;
+  clear_error();
+  if (word == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null word");
+  if (int rc = check_device()) return rc;
+  return status_word(word);
 }

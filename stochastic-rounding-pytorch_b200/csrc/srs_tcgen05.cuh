@@ -2,7 +2,8 @@
 // TMA box loads, mbarriers with bounded waits), as small inline functions.
 //
 // Every wait is bounded: a role that waits longer than kWaitCycles records where
-// in a status word, stops, and its CTA leaves after its copies had time to land.
+// in a status word (in host memory, so that the host sees it without a copy), stops, and
+// its CTA leaves after its copies had time to land.
 #pragma once
 
 #include <cstdint>
@@ -88,6 +89,10 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+__device__ __forceinline__ void record_wait(unsigned int* status, unsigned int where) {
+  asm volatile("st.relaxed.sys.global.u32 [%0], %1;" ::"l"(status), "r"(where) : "memory");
+}
+
 // Bounded wait for the completion of the phase of `parity`; false (and `where`
 // recorded) when it did not come.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsigned int* status,
@@ -96,7 +101,7 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsi
   const long long start = clock64();
   while (!barrier_try(bar, parity)) {
     if (clock64() - start > kWaitCycles) {
-      atomicOr(status, where);
+      record_wait(status, where);
       return false;
     }
   }
@@ -275,7 +280,7 @@ __device__ __forceinline__ bool counter_wait(const unsigned int* counter, unsign
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
     if (seen >= count) return true;
     if (clock64() - start > kWaitCycles) {
-      atomicOr(status, where);
+      record_wait(status, where);
       return false;
     }
   }

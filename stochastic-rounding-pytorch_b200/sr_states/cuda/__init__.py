@@ -4,7 +4,7 @@ from ._native import load_library
 from .adamw import AdamWCuda, cuda_adamw_step_
 from .blocks import BlockTensor, matmul_blocks, quantize_blocks
 from .cast import cast, rn_cast_bf16, sr_cast_bf16
-from .muon import cuda_muon_step_, orthogonalize
+from .muon import check_products, cuda_muon_step_, orthogonalize
 from .sgd import SGDMCuda, cuda_sgdm_step_
 
 
@@ -22,6 +22,6 @@ def is_available() -> bool:
     return torch.cuda.get_device_capability() == (10, 0)
 
 
-__all__ = ["AdamWCuda", "BlockTensor", "SGDMCuda", "cast", "cuda_adamw_step_",
+__all__ = ["AdamWCuda", "BlockTensor", "SGDMCuda", "cast", "check_products", "cuda_adamw_step_",
            "cuda_muon_step_", "cuda_sgdm_step_", "is_available", "matmul_blocks",
            "orthogonalize", "quantize_blocks", "rn_cast_bf16", "sr_cast_bf16"]

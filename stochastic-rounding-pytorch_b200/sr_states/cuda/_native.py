@@ -177,6 +177,7 @@ _SIGNATURES = {
     "srs_copy_rows": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
                        _P], ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
+    "srs_product_status_word": ([ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32))], ctypes.c_int),
 }
 NOALLOC_MAX_ROWS = 4096
 ABI_VERSION = 6
@@ -387,10 +388,17 @@ class NativeLauncher:
         return got if type(got) is not int else _check(got)
 
     def product_status(self) -> int:
-        """Where a bounded wait of a product kernel ran out (0: nowhere); synchronises."""
+        """Where a bounded wait of a product kernel ran out since the last call (0: nowhere);
+        synchronises the current device."""
         status = ctypes.c_uint32()
         _check(load_library().srs_product_status(ctypes.byref(status)))
         return int(status.value)
+
+    def product_status_word(self):
+        """The current device's status word (a ctypes pointer into host memory)."""
+        word = ctypes.POINTER(ctypes.c_uint32)()
+        _check(load_library().srs_product_status_word(ctypes.byref(word)))
+        return word
 
 
 _launcher = NativeLauncher()

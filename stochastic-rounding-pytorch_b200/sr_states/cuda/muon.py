@@ -161,6 +161,17 @@ def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, 
             launcher.muon_multi(rows, table, fmt, rule, hp, newton, rng, space, stream)
 
 
+def check_products(device) -> None:
+    """RuntimeError when a wait inside a product kernel (Newton-Schulz, FP8 blocks) has run out
+    on ``device`` since the last check: the results since then are not valid.  Waits for the
+    device; the product calls themselves ask, without waiting, about the calls before."""
+    with device_guard(device):
+        where = _native.launcher().product_status()
+    if where:
+        raise RuntimeError(f"a wait inside a product kernel on {device} ran out ({where:#x}): the "
+                           "results of product calls since the last check are not valid")
+
+
 def check_muon(lr, momentum, weight_decay, scale) -> None:
     check_nonnegative("learning rate", lr)
     check_nonnegative("weight_decay", weight_decay)

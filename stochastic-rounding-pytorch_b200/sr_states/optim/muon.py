@@ -45,6 +45,15 @@ class MuonSR(StateOptimizer):
                 if hasattr(parameter, "dim"):  # a checkpoint's group holds indices
                     check_matrix(parameter)
 
+    def state_dict(self):
+        """The optimizer's state; RuntimeError if a product kernel of a step gave up (waits
+        for the parameters' devices)."""
+        from ..cuda.muon import check_products
+
+        for device in {p.device for p in self.state if p.device.type == "cuda"}:
+            check_products(device)
+        return super().state_dict()
+
     def _step_group(self, group, formats, items, rng_step):
         from ..cuda.muon import muon_group_step  # the backend imports this module
 
