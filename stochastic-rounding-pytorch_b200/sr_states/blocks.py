@@ -24,8 +24,7 @@ def _matrix(x):
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, dtype, grad_dtype, grad_rounding, seed):
-        need_x, need_w = ctx.needs_input_grad[:2]
+    def forward(ctx, x, weight, dtype, grad_dtype, grad_rounding, seed, need_x, need_w):
         flat = _matrix(x)
         tokens = quantize_blocks(flat, dtype=dtype, orientation="both" if need_w else "rows")
         matrix = quantize_blocks(weight, dtype=dtype, block=(BLOCK, BLOCK),
@@ -33,15 +32,15 @@ class _BlockLinear(torch.autograd.Function):
         tokens, tokens_t = tokens if need_w else (tokens, None)
         matrix, matrix_t = matrix if need_x else (matrix, None)
         ctx.save_for_backward(*(tokens_t or ()), *(matrix_t or ()))
-        ctx.settings = (grad_dtype, grad_rounding, seed, x.shape, x.dtype, weight.dtype)
+        ctx.settings = (grad_dtype, grad_rounding, seed, x.shape, x.dtype, weight.dtype, need_x,
+                        need_w)
         y = matmul_blocks(tokens, matrix, dtype=x.dtype)
         return y.reshape(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        grad_dtype, rounding, seed, shape, x_dtype, w_dtype = ctx.settings
+        grad_dtype, rounding, seed, shape, x_dtype, w_dtype, need_x, need_w = ctx.settings
         saved = list(ctx.saved_tensors)
         tokens_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_w else None
         matrix_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_x else None
@@ -52,7 +51,7 @@ class _BlockLinear(torch.autograd.Function):
         rows, columns = got if orientation == "both" else (got, got)
         dx = matmul_blocks(rows, matrix_t, dtype=x_dtype).reshape(shape) if need_x else None
         dw = matmul_blocks(columns, tokens_t, dtype=w_dtype) if need_w else None
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None, None, None, None
 
 
 def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float8_e4m3fn,
@@ -76,7 +75,10 @@ def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float
                              "or run under torch.no_grad()")
         return linear_blocks(x, weight, dtype)
     check_blocks(grad_dtype, grad_rounding)
-    return _BlockLinear.apply(x, weight, dtype, grad_dtype, grad_rounding, seed)
+    # asked here: inside a Function inputs "need" gradients under torch.no_grad() as well
+    grad = torch.is_grad_enabled()
+    return _BlockLinear.apply(x, weight, dtype, grad_dtype, grad_rounding, seed,
+                              grad and x.requires_grad, grad and weight.requires_grad)
 
 
 class BlockLinear(torch.nn.Module):
