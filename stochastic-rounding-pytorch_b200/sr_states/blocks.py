@@ -8,6 +8,8 @@ gradients and 128 x 128 for weights.
 
 from __future__ import annotations
 
+import itertools
+
 import torch
 
 from ._hash import update_key
@@ -81,26 +83,57 @@ def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float
                               grad and x.requires_grad, grad and weight.requires_grad)
 
 
+def _rank():
+    distributed = torch.distributed
+    if distributed.is_available() and distributed.is_initialized():
+        return distributed.get_rank()
+    return 0
+
+
 class BlockLinear(torch.nn.Module):
-    """A linear layer without bias on ``block_linear``; the gradient rounding draws
-    anew on every call (seed, call number)."""
+    """A linear layer without bias on ``block_linear``.
+
+    The gradient's rounding draws anew on every call that a gradient will follow:
+    (seed, number of such calls, rank of the process).  ``seed=None`` gives a layer the
+    number of layers that the process made before it, so that layers draw apart.  The
+    ``state_dict`` carries the seed and the calls: a run that goes on from a checkpoint
+    rounds as the run that wrote it would have.
+    """
+
+    _made = itertools.count()
 
     def __init__(self, in_features, out_features, *, grad_dtype=torch.float8_e4m3fn,
-                 grad_rounding="stochastic", seed=0, device=None, dtype=torch.bfloat16):
+                 grad_rounding="stochastic", seed=None, device=None, dtype=torch.bfloat16):
         super().__init__()
         self.in_features, self.out_features = in_features, out_features
         self.grad_dtype, self.grad_rounding = grad_dtype, grad_rounding
-        self.seed, self.calls = int(seed), 0
+        self.seed, self.calls = int(next(self._made) if seed is None else seed), 0
         self.weight = torch.nn.Parameter(torch.empty((out_features, in_features), device=device,
                                                      dtype=dtype))
         torch.nn.init.normal_(self.weight, std=in_features ** -0.5)
+
+    def get_extra_state(self):
+        return torch.tensor([self.seed, self.calls], dtype=torch.int64)
+
+    def set_extra_state(self, state):
+        self.seed, self.calls = (int(v) for v in state)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+        # a state_dict of the weight alone is whole, too
+        key = prefix + "_extra_state"
+        if key in missing_keys:
+            missing_keys.remove(key)
 
     def quantized(self) -> BlockTensor:
         """The weight in FP8 blocks, to keep for inference."""
         return quantize_blocks(self.weight, block=(BLOCK, BLOCK))
 
     def forward(self, x):
-        self.calls += 1
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad):
+            self.calls += 1
         return block_linear(x, self.weight, grad_dtype=self.grad_dtype,
                             grad_rounding=self.grad_rounding,
-                            seed=update_key(self.seed, self.calls, 0))
+                            seed=update_key(self.seed, self.calls, _rank()))
