@@ -27,8 +27,10 @@
 // X_0 is held as V * 2^j with a power of two that puts |V * 2^j|_F between 2^14 and 2^15;
 // the remaining factor rho enters the first products in FP32.  The norm is summed in FP64,
 // so no input in range overflows or vanishes in it.  The later X are held times 2^12, far
-// from FP16's smallest numbers.  (Singular values up to 15 fit; the default coefficients
-// keep them below 1.3.)
+// from FP16's smallest numbers.  Where eps dwarfs the norm the X_k are small: while their
+// bound |V| / (|V| + eps) * (|a| + |b| + |c|)^k is below 1, they are held times a power of
+// two more (at most 2^100) that it leaves room for.  (Singular values up to 15 fit; the default coefficients keep them below
+// 1.3.)
 //
 // Results in FP32 or FP16 hold more digits than that.  For them (SPLIT) every held
 // matrix is the sum of two FP16 matrices, what the first leaves of a value in the
@@ -76,6 +78,7 @@ constexpr float kHeld = 256.0f;
 // X_0 is held with a norm below 2^kTarget, the later X times kHeldX.
 constexpr int kTarget = 15;
 constexpr float kHeldX = 4096.0f;
+constexpr int kFactors = 2 * SRS_NEWTON_MAX_STEPS;  // of a matrix: two a step (G, X)
 
 // A matrix of an optimizer step.
 struct MuonMatrix {
@@ -97,7 +100,7 @@ struct NewtonSource {
   __half* x0;
   int64_t low;        // elements from X_0 to its low part
   int64_t ld, x_elems;
-  float* rho;
+  float* factors;
 };
 
 // One launch over the matrices of several shapes (blockIdx.y: the matrix).
@@ -108,6 +111,8 @@ struct NewtonPlan {
   double* partial;    // kSumChunks for each matrix
   unsigned int* counters;  // of the product grid's phases, set to zero here
   double eps;
+  double growth;  // log2(|a| + |b| + |c|), at least 0: of X in a step
+  int steps;
   srs_rng rng;
   float momentum;
   int nesterov;
@@ -214,8 +219,9 @@ newton_sum_kernel(const __grid_constant__ NewtonPlan plan) {
   if (threadIdx.x == 0) plan.partial[(int64_t)blockIdx.y * kSumChunks + blockIdx.x] = total;
 }
 
-// X_0 = V * 2^j in two FP16 matrices (row pitch `ld`, padding zero) and
-// rho = (|V|_F + eps) * 2^j.
+// X_0 = V * 2^j in two FP16 matrices (row pitch `ld`, padding zero) and the factors of the
+// products' sums: X_0 stands for X times rho = (|V|_F + eps) * 2^j, the later X_k for X times
+// kHeldX or, while a bound on X_k is below 1, more.
 template <int U>
 __global__ void __launch_bounds__(kThreads)
 newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
@@ -226,16 +232,26 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
   double part = 0.0;
   for (int i = threadIdx.x; i < s.chunks; i += kThreads)
     part += plan.partial[(int64_t)blockIdx.y * kSumChunks + i];
-  const double norm = sqrt(block_sum(part, shared)) + plan.eps;
+  const double length = sqrt(block_sum(part, shared)), norm = length + plan.eps;
   int exponent = 0;
   const bool finite = norm < INFINITY;  // false for NaN
-  const double fraction = finite ? frexp(norm, &exponent) : 0.0;
+  if (finite) frexp(length, &exponent);
   const int j = kTarget - exponent;
   // Two exact factors, as 2^j itself may not be an FP32 number.
   const float scale0 = finite ? (float)ldexp(1.0, j / 2) : __int_as_float(0x7FC00000);
   const float scale1 = (float)ldexp(1.0, j - j / 2);
-  if (blockIdx.x == 0 && threadIdx.x == 0)
-    s.rho[batch] = finite ? (float)ldexp(fraction, kTarget) : __int_as_float(0x7FC00000);
+  if (blockIdx.x == 0 && threadIdx.x < plan.steps) {
+    const int step = threadIdx.x;
+    const double below = finite && length > 0.0 ? log2(norm / length) : 0.0;
+    const auto held = [&](int k) {
+      return ldexp((double)kHeldX, (int)fmin(fmax(floor(below - k * plan.growth), 0.0), 100.0));
+    };
+    const double rho = !finite ? (double)NAN : step == 0 ? ldexp(norm, j) : held(step);
+    const double next = step + 1 < plan.steps ? held(step + 1) : 1.0;
+    float* const to = s.factors + kFactors * batch + 2 * step;
+    to[0] = (float)(kHeld / rho / rho);
+    to[1] = (float)(next / kHeld / rho);
+  }
 
   MuonMatrix row{};
   uint32_t ctr = 0;
@@ -282,7 +298,7 @@ struct NewtonClass {
   __half* x[2];
   __half* g_at;
   __half* p_at;
-  const float* rho;
+  const float* factors;  // of each matrix and step
   char* out;             // orthogonalize: the result, contiguous matrices
   int out_format;
   int update;            // Muon: the result updates parameters
@@ -376,9 +392,8 @@ struct NewtonProducts {
     TileStore r{};
     r.row0 = at.row;
     r.col0 = at.col;
-    // The first step's operand stands for X / rho, the others for X / kHeldX.
-    float rho = kHeldX;
-    if (step == 0 && kind != 1) rho = s.rho[at.batch];
+    r.factor = 1.0f;
+    if (kind != 1) r.late = s.factors + kFactors * at.batch + 2 * step + (kind >> 1);
     r.format = SRS_FMT_F16;
     if (kind != 2) {
       const int64_t from = (int64_t)at.batch * s.small_elems;
@@ -386,7 +401,6 @@ struct NewtonProducts {
       r.pitch = s.small_ld;
       r.low = s.small_low;
       if (kind == 0) {
-        r.factor = __fdiv_rn(kHeld, __fmul_rn(rho, rho));
         r.out = reinterpret_cast<char*>(s.g_at + from);
       } else {
         r.factor = w.c / kHeld;
@@ -399,9 +413,7 @@ struct NewtonProducts {
     } else {
       r.m = s.m;
       r.n = s.n;
-      r.factor = __fdiv_rn(1.0f / kHeld, rho);
       if (step + 1 < w.steps) {
-        r.factor *= kHeldX;
         r.pitch = s.ld;
         // a times X (SPLIT) or its low part; the last step's X has none
         const __half* const x = s.x[step & 1] + (int64_t)at.batch * s.x_elems;
@@ -409,7 +421,7 @@ struct NewtonProducts {
                          : reinterpret_cast<const __half*>(reinterpret_cast<const char*>(x) +
                                                            s.x_low);
         r.addend_phase = p - 3;  // (below 0: the kernel before this one)
-        r.beta = w.a * __fdiv_rn(kHeldX, rho);
+        r.beta = w.a * kHeld;  // (times the sum's factor)
         if (SPLIT || step + 2 < w.steps) r.low = s.x_low;
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
       } else if (!SPLIT && s.update != 0) {
@@ -437,12 +449,12 @@ newton_kernel(const __grid_constant__ NewtonWork<SPLIT> w) {
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The matrices of one shape and their part of the workspace: rho, two copies of X
+// The matrices of one shape and their part of the workspace: factors, two copies of X
 // and G and P, each aligned to 256 bytes.
 struct NewtonShape {
   int64_t batch, m, n, small, ld, small_ld, x_elems, small_elems;
   int64_t x_low, small_low;  // bytes from a matrix to its low part (small_low 0: none)
-  int64_t rho, x[2], g, p;   // byte offsets
+  int64_t factors, x[2], g, p;  // byte offsets
 };
 
 // Rows on 128-byte boundaries, so that a box's 128-byte rows are whole cache lines
@@ -470,7 +482,7 @@ NewtonShape lay_out(int64_t batch, int64_t m, int64_t n, bool split, int64_t* at
   const int64_t small_bytes = round_up(batch * s.small_elems * 2, 256);
   s.x_low = x_bytes;
   s.small_low = split ? small_bytes : 0;
-  s.rho = take(at, batch * 4);
+  s.factors = take(at, batch * kFactors * 4);
   s.x[0] = take(at, x_bytes + s.x_low);
   s.x[1] = take(at, x_bytes + s.x_low);
   s.g = take(at, small_bytes + s.small_low);
@@ -504,6 +516,15 @@ struct NewtonResult {
   float decay, step;
 };
 
+// The settings that the two preparing kernels need.
+void fill_plan(const srs_newton& h, NewtonPlan* plan) {
+  plan->eps = h.eps;
+  plan->steps = h.steps;
+  double bound = 0.0;
+  for (float c : h.coefficients) bound += std::fabs((double)c);
+  plan->growth = bound > 1.0 ? std::log2(bound) : 0.0;
+}
+
 // Fills what the two preparing kernels and the product grid share.  The sources'
 // own fields are set by the caller.
 void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
@@ -523,7 +544,7 @@ void fill_source(const NewtonShape& s, char* space, int first, int64_t matrices,
   f->low = s.x_low / 2;
   f->ld = s.ld;
   f->x_elems = s.x_elems;
-  f->rho = reinterpret_cast<float*>(space + s.rho);
+  f->factors = reinterpret_cast<float*>(space + s.factors);
 }
 
 // The map of a matrix and, for SPLIT, that of its low part behind it.
@@ -554,7 +575,7 @@ int fill_class(const NewtonShape& s, char* space, const NewtonResult& result,
   c->small_low = s.small_low;
   c->g_at = reinterpret_cast<__half*>(space + s.g);
   c->p_at = reinterpret_cast<__half*>(space + s.p);
-  c->rho = reinterpret_cast<const float*>(space + s.rho);
+  c->factors = reinterpret_cast<const float*>(space + s.factors);
   c->out = static_cast<char*>(result.out);
   c->out_format = result.out_format;
   c->update = result.update ? 1 : 0;
@@ -736,7 +757,7 @@ extern "C" int srs_orthogonalize(const void* x, int x_format, int64_t row_pitch,
   plan.classes = 1;
   plan.partial = reinterpret_cast<double*>(space + partial);
   plan.counters = reinterpret_cast<unsigned int*>(space);
-  plan.eps = h->eps;
+  fill_plan(*h, &plan);
   NewtonSource& s = plan.source[0];
   s.x = x;
   s.x_format = x_format;
@@ -841,7 +862,7 @@ extern "C" int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes
   plan.classes = n_classes;
   plan.partial = reinterpret_cast<double*>(space + partial);
   plan.counters = reinterpret_cast<unsigned int*>(space);
-  plan.eps = h->eps;
+  fill_plan(*h, &plan);
   plan.rng = *rng;
   plan.momentum = hp->momentum;
   plan.nesterov = hp->nesterov;

@@ -66,6 +66,7 @@ struct TileStore {
   int m, n;        // size of the matrix
   int update;      // 1: Muon's parameter update instead of a store
   float factor;    // of the accumulator
+  const float* late;  // multiplies factor and beta (null: nothing), read while the sum runs
   float beta;      // of `addend`
   float diagonal;  // added where i == j
   const __half* addend;  // m x n, row pitch `pitch` (null: none)
@@ -770,7 +771,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
     for (int p = 0; p < phases && ok; ++p) {
       const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step, ++count) {
-        const TileStore at = src.store(p, t);
+        TileStore at = src.store(p, t);
         const int acc = count & 1;
         const int row0 = at.row0 + 128 * (int)rank + 32 * quarter;
         uint4 add[4];
@@ -786,10 +787,16 @@ __device__ __forceinline__ void run_products(const Source& src) {
           }
           load_addend(at, row0, at.col0 + 32 * part * kPieces, lane, add);
         }
+        float late = 1.0f;
+        if (NEWTON && at.late != nullptr) late = __ldg(at.late);
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         tmem_fence_after();
+        if (NEWTON) {
+          at.factor *= late;
+          at.beta *= late;
+        }
         const uint32_t from = tmem + acc * S::kSecond + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
         for (int i = 0; i < kPieces; ++i) {

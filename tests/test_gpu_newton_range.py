@@ -1,4 +1,5 @@
-"""Newton-Schulz over the matrices it meets in earnest: low ranks and falling spectra.
+"""Newton-Schulz over the matrices it meets in earnest: low ranks, falling spectra and norms
+far below eps.
 
 Tolerances.  A BF16 result (and Muon's update) comes from G, P and X held in FP16, each
 rounded to within u = 2^-11 of its elements: 15 matrices in a run of five steps, 16 u
@@ -87,3 +88,31 @@ def test_muon_updates_of_low_rank_gradients(param, cuda_device):
                             max(1.0, shape[0] / shape[1]) ** 0.5)
             off = relative(p, want)
             assert off <= 16 * U + (BF16 if param == torch.bfloat16 else 0.0), (shape, name, off)
+
+
+@pytest.mark.parametrize("ratio", [1e-1, 1e-3, 1e-6, 1e-12, 1e-25])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_norms_below_eps(ratio, dtype, cuda_device):
+    """X_0 = x / (|x| + eps) is then small, and keeps its digits."""
+    from sr_states import orthogonalize
+
+    gen = torch.Generator().manual_seed(5)
+    for shape in ((60, 100), (300, 40)):
+        x = torch.randn(shape, generator=gen).to(cuda_device)
+        x *= ratio / torch.linalg.matrix_norm(x)
+        off = relative(orthogonalize(x, eps=1.0, dtype=dtype), newton(x, eps=1.0))
+        assert off <= 16 * U + (BF16 if dtype == torch.bfloat16 else 0.0), (shape, off)
+
+
+def test_muon_steps_of_vanishing_gradients(cuda_device):
+    """Gradients far below eps move a parameter by 485 times their share of it."""
+    from sr_states.cuda import cuda_muon_step_
+
+    gen = torch.Generator().manual_seed(9)
+    for ratio in (1e-4, 1e-9):
+        g = torch.randn(80, 130, generator=gen).to(cuda_device)
+        g *= ratio * 1e-7 / torch.linalg.matrix_norm(g)
+        p, u = torch.zeros_like(g), torch.zeros_like(g)
+        cuda_muon_step_([p], [g], [u], lr=1.0, seeds=[0])
+        want, _ = _want(torch.zeros_like(g), g, torch.zeros_like(g), 1.0, 0.95, 0.0, True, 1.0)
+        assert relative(p, want) <= 16 * U
