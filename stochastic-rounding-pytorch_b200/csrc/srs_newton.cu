@@ -73,7 +73,8 @@ static_assert(kMaxPhases <= kThreads, "one CTA zeroes the counters");
 constexpr int kSumChunks = 1024;  // most partial sums of a matrix
 constexpr int kPlain = -1;        // source template value: a plain tensor
 // G and P are held times 2^8: their small elements (1 / m and less in the first
-// steps) then stay among FP16's normal numbers, and eigenvalues up to 255 fit.
+// steps) then stay among FP16's normal numbers, and eigenvalues up to 255 fit.  (P is held
+// times less where the coefficients are larger than that: see hold_of_p.)
 constexpr float kHeld = 256.0f;
 // X_0 is held with a norm below 2^kTarget, the later X times kHeldX.
 constexpr int kTarget = 15;
@@ -113,6 +114,7 @@ struct NewtonPlan {
   double eps;
   double growth;  // log2(|a| + |b| + |c|), at least 0: of X in a step
   int steps;
+  float hold_p;   // P is held times this
   srs_rng rng;
   float momentum;
   int nesterov;
@@ -250,7 +252,7 @@ newton_scale_kernel(const __grid_constant__ NewtonPlan plan) {
     const double next = step + 1 < plan.steps ? held(step + 1) : 1.0;
     float* const to = s.factors + kFactors * batch + 2 * step;
     to[0] = (float)(kHeld / rho / rho);
-    to[1] = (float)(next / kHeld / rho);
+    to[1] = (float)(next / plan.hold_p / rho);
   }
 
   MuonMatrix row{};
@@ -315,7 +317,7 @@ struct NewtonWork {
   uint32_t triangles[kClasses + 1];  // first tile of each class in a G or P phase
   uint32_t grids[kClasses + 1];      // ... in an X phase
   int classes, steps, edge;
-  float a, b, c;
+  float a, b, c, hold_p;
   unsigned int* counters;  // one a phase
   unsigned int* status_at;
 };
@@ -403,9 +405,9 @@ struct NewtonProducts {
       if (kind == 0) {
         r.out = reinterpret_cast<char*>(s.g_at + from);
       } else {
-        r.factor = w.c / kHeld;
-        r.beta = w.b;
-        if (!SPLIT || step + 1 == w.steps) r.diagonal = w.a * kHeld;
+        r.factor = w.c * (w.hold_p / (kHeld * kHeld));
+        r.beta = w.b * (w.hold_p / kHeld);
+        if (!SPLIT || step + 1 == w.steps) r.diagonal = w.a * w.hold_p;
         r.addend = s.g_at + from;
         r.addend_phase = p - 1;
         r.out = reinterpret_cast<char*>(s.p_at + from);
@@ -421,7 +423,7 @@ struct NewtonProducts {
                          : reinterpret_cast<const __half*>(reinterpret_cast<const char*>(x) +
                                                            s.x_low);
         r.addend_phase = p - 3;  // (below 0: the kernel before this one)
-        r.beta = w.a * kHeld;  // (times the sum's factor)
+        r.beta = w.a * w.hold_p;  // (times the sum's factor)
         if (SPLIT || step + 2 < w.steps) r.low = s.x_low;
         r.out = reinterpret_cast<char*>(s.x[(step + 1) & 1] + (int64_t)at.batch * s.x_elems);
       } else if (!SPLIT && s.update != 0) {
@@ -516,10 +518,23 @@ struct NewtonResult {
   float decay, step;
 };
 
+// What P is held times: 2^8, or the largest power of two with which the eigenvalues of P
+// for singular values up to 1.4 stay below 60000 (FP16 ends at 65504).
+float hold_of_p(const srs_newton& h) {
+  const double a = h.coefficients[0], b = h.coefficients[1], c = h.coefficients[2];
+  double most = std::fmax(std::fabs(a), std::fabs(a + 2.0 * b + 4.0 * c));
+  const double vertex = -b / (2.0 * c);  // of a + b l + c l^2
+  if (vertex > 0.0 && vertex < 2.0) most = std::fmax(most, std::fabs(a + 0.5 * b * vertex));
+  float hold = kHeld;
+  while (hold * most > 60000.0) hold *= 0.5f;
+  return hold;
+}
+
 // The settings that the two preparing kernels need.
 void fill_plan(const srs_newton& h, NewtonPlan* plan) {
   plan->eps = h.eps;
   plan->steps = h.steps;
+  plan->hold_p = hold_of_p(h);
   double bound = 0.0;
   for (float c : h.coefficients) bound += std::fabs((double)c);
   plan->growth = bound > 1.0 ? std::log2(bound) : 0.0;
@@ -673,6 +688,7 @@ int run_newton(NewtonWork<SPLIT>& w, const srs_muon_class* shapes, const srs_new
   w.a = h->coefficients[0];
   w.b = h->coefficients[1];
   w.c = h->coefficients[2];
+  w.hold_p = hold_of_p(*h);
   w.counters = counters;
   if (int rc = status_word(&w.status_at)) return rc;
   return tile_group(shapes, w.classes, SPLIT) == 2 ? launch_newton<2, SPLIT>(w, shapes, stream)

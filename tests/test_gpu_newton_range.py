@@ -1,5 +1,5 @@
-"""Newton-Schulz over the matrices it meets in earnest: low ranks, falling spectra and norms
-far below eps.
+"""Newton-Schulz over the matrices it meets in earnest: low ranks, falling spectra, norms
+far below eps and large coefficients.
 
 Tolerances.  A BF16 result (and Muon's update) comes from G, P and X held in FP16, each
 rounded to within u = 2^-11 of its elements: 15 matrices in a run of five steps, 16 u
@@ -116,3 +116,28 @@ def test_muon_steps_of_vanishing_gradients(cuda_device):
         cuda_muon_step_([p], [g], [u], lr=1.0, seeds=[0])
         want, _ = _want(torch.zeros_like(g), g, torch.zeros_like(g), 1.0, 0.95, 0.0, True, 1.0)
         assert relative(p, want) <= 16 * U
+
+
+@pytest.mark.parametrize("a", [100.0, 300.0, 1e5])
+def test_large_coefficients(a, cuda_device):
+    """One step with G's part zero: P = a I, beyond FP16's range in part."""
+    from sr_states import orthogonalize
+
+    x = torch.randn(50, 90, generator=torch.Generator().manual_seed(6)).to(cuda_device)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = orthogonalize(x, steps=1, coefficients=(a, 0.0, 0.0), dtype=dtype)
+        assert relative(y, newton(x, 1, (a, 0.0, 0.0))) <= 3 * U + (
+            BF16 if dtype == torch.bfloat16 else 0.0)
+
+
+@pytest.mark.parametrize("coefficients", [(400.0, -500.0, 150.0), (-300.0, 900.0, -300.0),
+                                          (3.0, 2000.0, 0.0), (2.0, 0.0, 1e4)], ids=str)
+def test_steps_of_large_coefficients(coefficients, cuda_device):
+    """One step whose P has eigenvalues beyond 255 in places."""
+    from sr_states import orthogonalize
+
+    for name, x in matrices(60, 130).items():
+        x = x.float().to(cuda_device)
+        want = newton(x, 1, coefficients)
+        assert relative(orthogonalize(x, steps=1, coefficients=coefficients,
+                                      dtype=torch.bfloat16), want) <= 16 * U + BF16, name
