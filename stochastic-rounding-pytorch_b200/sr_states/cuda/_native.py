@@ -366,7 +366,10 @@ class NativeLauncher:
 
     def muon_workspace(self, classes) -> int:
         """Workspace bytes of a muon_multi call over ``classes`` (an array of SrsMuonClass)."""
-        return int(load_library().srs_muon_workspace(classes, len(classes)))
+        size = int(load_library().srs_muon_workspace(classes, len(classes)))
+        if size < 0:
+            _check(SRS_ERR_INVALID_ARGUMENT)
+        return size
 
     def muon_multi(self, rows, classes, u_fmt, u_rule, hp, newton, rng, workspace, stream):
         _check(load_library().srs_muon_multi(

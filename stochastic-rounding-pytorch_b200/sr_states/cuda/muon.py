@@ -133,14 +133,10 @@ def _calls(classes, launcher):
 _ROW = struct.Struct("<QQQQqqIIII")  # srs_row
 
 
-def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, newton, rng):
-    """Enqueue the step of ``updates`` (matrices of one device) on its current stream."""
-    device = updates[0].tensors[0].device
+def _plan(updates, *, lr, scale):
+    """The calls of a step of ``updates`` (matrices of one device): [(rows, classes, workspace
+    bytes), ...].  Sizes that the kernels do not take are refused here, before any launch."""
     launcher = _native.launcher()
-    fmt, rule = codes
-    hp = _native.SrsMuonHparams()
-    hp.momentum, hp.decay = momentum, 1.0 - lr * weight_decay
-    hp.nesterov = int(nesterov)
     calls = []
     for call in _calls(_shape_classes(updates), launcher):
         table = (_native.SrsMuonClass * len(call))()
@@ -154,6 +150,21 @@ def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, 
             entry.count, entry.m, entry.n = len(chosen), m, n
             entry.neg_step = -(lr * update_scale(scale, m, n))
         calls.append((rows, table, launcher.muon_workspace(table)))
+    return calls
+
+
+def muon_launch(updates, codes, *, lr, momentum, weight_decay, nesterov, scale, newton, rng,
+                calls=None):
+    """Enqueue the step of ``updates`` (matrices of one device) on its current stream;
+    ``calls``: their plan, if it has been made."""
+    device = updates[0].tensors[0].device
+    launcher = _native.launcher()
+    fmt, rule = codes
+    hp = _native.SrsMuonHparams()
+    hp.momentum, hp.decay = momentum, 1.0 - lr * weight_decay
+    hp.nesterov = int(nesterov)
+    if calls is None:
+        calls = _plan(updates, lr=lr, scale=scale)
     with device_guard(device):
         stream = stream_handle(device)
         space = torch.empty(max(size for _, _, size in calls), dtype=torch.uint8, device=device)
@@ -255,10 +266,12 @@ def muon_group_step(optimizer, group, formats, items, rng_step) -> None:
             by_device.setdefault(parameter.device, []).append(
                 Update(tensors, int(param_index), parameter.numel(), int(offset) & 0xFFFFFFFF,
                        None))
+    plans = []
     for updates in by_device.values():
         check_updates(updates)
+        plans.append((updates, _plan(updates, lr=group["lr"], scale=group["scale"])))
     rng = rng_words(group["sr_seed"], rng_step)
-    for updates in by_device.values():
+    for updates, calls in plans:
         muon_launch(updates, codes, lr=group["lr"], momentum=group["momentum"],
                     weight_decay=group["weight_decay"], nesterov=group["nesterov"],
-                    scale=group["scale"], newton=newton, rng=rng)
+                    scale=group["scale"], newton=newton, rng=rng, calls=calls)
