@@ -543,6 +543,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         // what the earlier phase wrote, seen by the copies that follow
         if (lane == 0) ok = counter_wait(src.counter(p - 1), gridDim.x, status, 1u << 16);
         ok = __all_sync(0xFFFFFFFFu, ok);
+        __syncwarp();  // a vote orders no memory: what lane 0 has acquired, for the others
         asm volatile("fence.proxy.async;" ::: "memory");
       }
       for (uint32_t t = first; t < tiles && ok; t += step) {
