@@ -217,6 +217,9 @@ def cuda_muon_step_(parameters, gradients, momenta, *, lr, momentum_factor=0.95,
     with the momenta's format (one for all) under counter base
     state_key(seeds[i], 0).  Parameters and gradients FP32 or BF16; dimensions
     after the first are flattened.  Matrices of a shape are updated together.
+
+    In a CUDA graph (after one such call outside it) a step replays with the learning rate
+    and the seeds of its capture: the same rounding draws every time.
     """
     parameters, gradients, momenta = list(parameters), list(gradients), list(momenta)
     seeds = list(seeds)
