@@ -647,8 +647,9 @@ int launch_newton(NewtonWork<SPLIT>& w, const srs_muon_class* shapes, cudaStream
 // Rough time of the three products of a step with tiles of 128 * cg, in cycles of
 // one SM: 512 a slice for the pair, 350 for the single CTA (256 of MMA, but twice
 // the loads for it), and what a tile's results take.  Measured (us, single against
-// pair): 1024^2 144, 201; 2048^2 241, 285; 2500^2 422, 390; 3500^2 894, 783;
-// 16 x 768^2 295, 367; 24 x 768^2 402, 365; 4 x (1024 x 4096) 347, 381.
+// pair): 1024^2 140, 184; 2048^2 243, 265; 2500^2 423, 371; 3500^2 958, 787;
+// 12 x 768^2 218, 222; 24 x 768^2 400, 359; 4 x (1024 x 4096) 414, 435; the rule is wrong
+// between the two kinds by up to a ninth (3001 x 3333, single: 750, 669).
 double step_cycles(const srs_muon_class* shapes, int count, bool split, int cg) {
   const int64_t groups = sm_count() / cg, edge = 128 * cg;
   const double slice = cg == 2 ? 512.0 : 350.0, rest = cg == 2 ? 5000.0 : 2000.0;

@@ -13,7 +13,7 @@
 // and 128 rows of B per slice, 32 KB for 512 cycles of MMA.  The small form (one
 // CTA, 128 x 128) keeps the SMs busy when there are too few large tiles.
 //
-// A CTA has 8 or 16 warps that read the accumulator and write the result (warp w owns
+// A CTA has 8 warps that read the accumulator and write the result (warp w owns
 // TMEM lanes 32 (w % 4) .., one row of the tile per lane, and its part of the
 // columns), then one that issues the TMA loads, one for the MMAs and one that stages the
 // FP8 block scales.  Grids are persistent; the accumulator is double-buffered in TMEM
@@ -453,10 +453,10 @@ struct ProductShape {
   // cap: 8192 x 14336 x 4096 429 us, with 256 columns 412 us.)
   static constexpr int kShared = KIND == kOperandF8 && CG == 2 ? 32 : 0;
   static constexpr int kSecond = kTileCols - kShared;
-  // Writing warps: 16 where phases of few tiles wait for results (orthogonalising 768^2
-  // 134.6 us with 8, 130.6 with 16), 8 where the MMAs hide them (4096^2 1093 us with 8,
-  // 1109 with 16).
-  static constexpr int kWriters = KIND == kOperandF16 && CG == 1 ? 16 : 8;
+  // Writing warps.  16 leave 96 registers a thread, too few for a piece, its addend and its
+  // low part: orthogonalising 768^2 took 141 us with 16 (single-CTA tiles) and 143 with 8,
+  // 2048^2 252 and 242, 12 x 768^2 231 and 218, 4 x (1024 x 4096) 438 and 416.
+  static constexpr int kWriters = 8;
   static constexpr int kThreads = 32 * (kWriters + 4);
   static constexpr int kStages = KIND == kOperandF16 && CG == 2 ? 6 : 5;  // 4 to 6 measure the same
   static constexpr int kScaleBytes = KIND == kOperandF8 ? 512 * (1 + CG) : 0;  // per slot
