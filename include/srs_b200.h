@@ -377,8 +377,9 @@ int srs_muon_multi(const srs_row* rows, const srs_muon_class* classes, int n_cla
  * copies' addresses and pitches are multiples of 16, and nothing is written outside their
  * rows and columns.  At most 4194240 rows and 2^30 columns a call.
  *
- * srs_matmul_blocks: d[i, j] = sum_k a[i, k] * b[j, k] with FP32 sums, d in FP32,
- * BF16 or FP16 (contiguous).  The data's base addresses and row pitches must be
+ * srs_matmul_blocks: d[i, j] = sum_k a[i, k] * b[j, k] with FP32 sums (terms truncated:
+ * within (k + 2) 2^-23 of the sum of their sizes), k at most 2^30, d in FP32, BF16 or FP16
+ * (contiguous).  The data's base addresses and row pitches must be
  * multiples of 16 bytes.  k == 0 gives zeros. */
 int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols, int64_t x_pitch,
                         int out_format, int rule, int square, uint32_t seed, uint32_t offset,
@@ -412,7 +413,7 @@ int srs_linear_blocks(const void* x, int x_format, int64_t tokens, int64_t k, in
 int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols, void* dst,
                   int64_t dst_pitch, void* stream);
 
-/* Waits inside the product kernels are bounded (about 2 s).  One that runs out is recorded
+/* Waits inside the product kernels are bounded (about 2 s beyond what their work takes).  One that runs out is recorded
  * in a word of host memory, one a device, and the results of that call are not valid (a
  * Muon step's parameters and momentum neither).  The next srs_orthogonalize,
  * srs_muon_multi, srs_matmul_blocks or srs_linear_blocks on the device enqueues nothing,

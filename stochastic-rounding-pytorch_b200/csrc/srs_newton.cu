@@ -337,6 +337,7 @@ struct NewtonProducts {
   __device__ uint32_t formats() const { return 0u; }
   __device__ unsigned int* counter(int p) const { return w.counters + p; }
   __device__ unsigned int* status() const { return w.status_at; }
+  __device__ int longest() const { return 0; }  // at most 2^18 slices, three times
   __device__ Place place(int p, uint32_t t) const {
     const bool grid = p % 3 == 2;
     const uint32_t* begin = grid ? w.grids : w.triangles;

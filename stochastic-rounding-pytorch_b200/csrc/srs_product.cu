@@ -203,6 +203,7 @@ struct BlockSource {
   __device__ uint32_t formats() const { return w.instruction_formats; }
   __device__ unsigned int* counter(int) const { return nullptr; }
   __device__ unsigned int* status() const { return w.status_at; }
+  __device__ int longest() const { return w.slices; }
   __device__ TileLoad load(int, uint32_t t) const {
     int row, col;
     w.grid.at(t, &row, &col);

@@ -472,8 +472,9 @@ struct ProductShape {
 };
 
 // The CTA's work.  Source gives: phases(), tiles(phase), load(phase, tile),
-// store(phase, tile), formats() (bits of the instruction descriptor), counter(phase)
-// and status(); for FP8 also scales(): the operands' block scales.
+// store(phase, tile), formats() (bits of the instruction descriptor), counter(phase),
+// status() and longest() (slices of a tile, where they can take seconds); for FP8 also
+// scales(): the operands' block scales.
 template <int KIND, int CG, bool NEWTON, bool SPLIT, class Source>
 __device__ __forceinline__ void run_products(const Source& src) {
   using S = ProductShape<KIND, CG>;
@@ -769,6 +770,9 @@ __device__ __forceinline__ void run_products(const Source& src) {
     const int part = warp >> 2, quarter = warp & 3;
     const uint32_t staged = staged0 + warp * kPieceBytes;
     int count = 0, met = -1;  // met: the last phase known to be complete
+    // These warps wait for whole tiles: beyond the limit of other waits, 4096 cycles a slice
+    // of k.  (A tile alone on the GPU takes 700 to 840: 3 s for 2^30 of k.)
+    const long long patience = kWaitCycles + 4096ll * src.longest();
     for (int p = 0; p < phases && ok; ++p) {
       const uint32_t tiles = src.tiles(p);
       for (uint32_t t = first; t < tiles && ok; t += step, ++count) {
@@ -790,7 +794,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
         }
         float late = 1.0f;
         if (NEWTON && at.late != nullptr) late = __ldg(at.late);
-        ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u);
+        ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u, patience);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         tmem_fence_after();

@@ -96,11 +96,11 @@ __device__ __forceinline__ void record_wait(unsigned int* status, unsigned int w
 // Bounded wait for the completion of the phase of `parity`; false (and `where`
 // recorded) when it did not come.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsigned int* status,
-                                             unsigned int where) {
+                                             unsigned int where, long long limit = kWaitCycles) {
   if (barrier_try(bar, parity)) return true;
   const long long start = clock64();
   while (!barrier_try(bar, parity)) {
-    if (clock64() - start > kWaitCycles) {
+    if (clock64() - start > limit) {
       record_wait(status, where);
       return false;
     }

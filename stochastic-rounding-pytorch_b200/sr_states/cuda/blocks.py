@@ -76,8 +76,10 @@ def matmul_blocks(a, b, *, dtype=torch.bfloat16):
     """``a @ b.T`` of two BlockTensors (a: M x K, b: N x K), summed in FP32.
 
     Either operand may be E4M3 or E5M2 with scales of either block form; the
-    result is FP32, BF16 or FP16.  K = 0 gives zeros.  Data whose rows do not start on
-    16-byte boundaries are copied once (those of ``quantize_blocks`` do)."""
+    result is FP32, BF16 or FP16.  The tensor core truncates the terms of its sums: an
+    element is within (K + 2) 2^-23 of the sum of its terms' sizes.  K = 0 gives zeros; K is
+    at most 2^30.  Data whose rows do not start on 16-byte boundaries are copied once (those
+    of ``quantize_blocks`` do)."""
     if dtype not in _FORMATS:
         raise TypeError(f"matmul_blocks gives FP32, BF16 or FP16, got {dtype}")
     launcher = _native.launcher()
