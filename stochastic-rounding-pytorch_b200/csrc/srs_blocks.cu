@@ -180,8 +180,8 @@ __device__ __forceinline__ void store_bytes(uint8_t* out, uint2 w, int left) {
 
 // Rows alone, 1 x 128 blocks: 16 lanes to a block, kAhead blocks of one column a
 // half-warp with all their loads first.  HBM-bound when rounding to nearest (8192 x
-// 4096: 25 us with the launch; 3 bytes an element at 6.5 TB/s would be 15), by the integer
-// units for the stochastic rule's hashes (41 us).
+// 4096: 20.5 us a call among others; 3 bytes an element at 6.5 TB/s would be 15), by the
+// integer units for the stochastic rule's hashes (37 us).
 constexpr int kAhead = 4;
 
 template <int OF, int XF>
@@ -229,9 +229,10 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
 // conflict-free) and leave as 4 x 4 byte transposes, 128 bytes of a column at a time.
 // Nearest: bound by waits for the loads and at the barriers (integer pipe 51 % busy);
 // stochastic both ways: by the hashes (two an element, about 25 integer operations).
-// 8192 x 4096 from BF16, both ways: 45 us to nearest, 76 us stochastic (E5M2); the bytes
-// alone would take 20.  A reduction of 4 shuffles for every row, and 16 partial maxima a
-// column instead of 8, took 51 and 90.
+// 8192 x 4096 from BF16, both ways: 39 us to nearest, 72 us stochastic; the bytes alone
+// would take 20.  128 x 128 blocks: 21 us rows, 31 both ways; stochastic 37 and 65.  A
+// reduction of 4 shuffles for every row and 16 partial maxima a column instead of 8 took
+// a fifth more.
 template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
 __global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 4 : 2)
 quantize_tile_kernel(const QuantizeArgs a) {

@@ -50,14 +50,16 @@
 // stored; products read the others from their transposes.
 //
 // What bounds it: the MMAs and the power they draw for large matrices (4096 x 14336:
-// 3.2 ms, 1.2 PFLOP/s of the 3 m^2 n + m^3 a step needs; the X = P X product keeps the
-// tensor pipe busy 99 % of its cycles), about 4 us a phase of meeting, first loads and
-// results for small ones (768 x 768: 125 us in 15 phases).
+// 3.55 ms among other calls, 1.11 PFLOP/s of the 3 m^2 n + m^3 a step needs, 3.35 before X
+// had a low part), about 4 us a phase of meeting, first loads and results for small ones
+// (768 x 768: 126 us in 15 phases), and the tiles of G alone for long, narrow ones: G has
+// one tile for every 128 x 128 of the shorter side, and a tile's sum runs over the whole
+// longer side on one CTA or pair.
 //
 // Reads of V: one for the norm and one for X_0.  For an optimizer step both passes
 // compute V from the gradient and the momentum (8 or fewer bytes an element) rather than
 // keeping V in FP32 (8 bytes more of traffic and 4 of memory); the second pass stores
-// u'.  4096 x 14336 from BF16: 44 us each, 1.4 % of the whole.
+// u'.  4096 x 14336 from BF16: 44 us and, with two matrices to write, 62: 3 % of the whole.
 #include <cmath>
 
 #include "srs_host.h"
@@ -195,7 +197,8 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {
   return total;
 }
 
-// Partial sums of squares, in an order that depends on the sizes alone.
+// Partial sums of squares, in an order that depends on the sizes, the number of matrices and
+// that of SMs.
 template <int U>
 __global__ void __launch_bounds__(kThreads)
 newton_sum_kernel(const __grid_constant__ NewtonPlan plan) {

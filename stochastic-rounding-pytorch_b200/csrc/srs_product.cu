@@ -301,7 +301,8 @@ template <int BN>
 int launch_thin_as(ThinArgs& args, int splits, bool overlap, cudaStream_t stream) {
   using S = ThinShape<BN>;
   const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN>);
-  // As many stages as fit; the last panel is followed by the rest of 128 rows.
+  // As many stages as fit before a whole panel: the MMA reads 128 rows from the start of
+  // the last stage's panel, past the end of that stage when its tile has fewer.
   args.panel_bytes = (args.rows + 7) / 8 * 8 * kSliceBytes;
   const int stage = args.panel_bytes + BN * kSliceBytes, slack = kPanelBytes;
   args.stages = (S::kBudget - slack) / stage;
@@ -326,9 +327,9 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
   args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
   // Tiles of 128 rows, k split while two CTAs an SM hold all of them and each keeps two
   // slices.  With more tiles than SMs nothing is split, and the tiles take the size
-  // that fills whole rounds of two CTAs an SM: 28672 x 8192 by one token 44.7 -> 42.3 us
-  // (5.55 TB/s).  (Such sizes below that, too: 4096 x 4096 in 74 tiles of 56 rows and
-  // clusters of four 8.9 us, in 32 tiles and clusters of eight 7.5.)
+  // that fills whole rounds of two CTAs an SM: 28672 x 8192 by one token 44.7 -> 42.3 us.
+  // (Such sizes below that, too: 4096 x 4096 in 74 tiles of 56 rows and clusters of four
+  // 8.9 us, in 32 tiles and clusters of eight 7.5.)
   const int64_t sms = sm_count(), tiles = (a.rows + 127) / 128;
   int splits = 1;
   args.rows = 128;

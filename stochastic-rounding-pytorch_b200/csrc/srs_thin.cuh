@@ -7,8 +7,9 @@
 // side, so that no MMA row is idle, and k is split over a cluster of up to 8 CTAs so
 // that all SMs stream: 4096 rows are only 32 tiles.  The split sums meet in distributed
 // shared memory and are added in rank order (FP32), so results do not depend on
-// timing.  Two CTAs share an SM, each with about 90 KB of slices on their way.
-// 14336 x 4096 by one token (58.7 MB): 15.2 us; 28672 x 8192: 42.3 us, 5.55 TB/s.
+// timing.  Two CTAs share an SM, each with 72 KB of slices on their way in tiles of 128 rows
+// and up to 85 KB in smaller ones.
+// 14336 x 4096 by one token (58.7 MB): 16.7 us a call; 28672 x 8192: 42.9 us, 5.5 TB/s.
 //
 // Launched behind the quantisation of its B (srs_linear_blocks) the kernel may start
 // while that one runs: it loads A first and waits for the other kernel before it
