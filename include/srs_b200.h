@@ -300,10 +300,10 @@ int srs_derive_keys(const uint32_t* param_index, uint32_t* out, int64_t n, const
  *   X_0 = x / (|x|_F + eps);  X_{i+1} = (a I + b G + c G^2) X_i,  G = X_i X_i^T
  * for `batch` matrices of m rows and n columns (m > n: X_{i+1} = X_i (a I + b G + c G^2),
  * G = X_i^T X_i).  Products on the tensor cores with FP32 sums: FP16 operands for y in
- * BF16 (relative errors of the whole matrix of 1e-3 to 2e-3, of 6e-3 for a few orthogonal
- * rows, whatever the singular values), pairs of FP16 operands for y in FP32 or FP16 (1e-5
- * for sides of some hundreds, 1e-4 for ten thousand; with ranks of a few 3e-4 and 2e-3;
- * three times the work); the norm is summed in FP64.  Singular values must stay below 15
+ * BF16 (relative errors of the whole matrix of 1e-3 to 3e-3 whatever the singular values, of
+ * 6e-3 for a few orthogonal rows and for ranks of a few at sides of ten thousand), pairs of
+ * FP16 operands for y in FP32 or FP16 (1e-5 for sides of some hundreds, 1e-4 for ten thousand;
+ * with ranks of a few 3e-4 and 3e-3; three times the work); the norm is summed in FP64.  Singular values must stay below 15
  * through the steps (those of the usual coefficients stay below 1.3).  x: FP32, BF16 or FP16, element (b, i, j) at
  * b * batch_stride + i * row_pitch + j; y: contiguous, FP32, BF16 or FP16; x and y must not
  * overlap.  At most 65535 matrices of 2^32 elements and 2^24 rows or columns.  A matrix with

@@ -20,9 +20,10 @@
 // step multiplies them by a, five of them by a^5 = 485 (rank 1: 15 % of the result).  So X
 // is carried with what its FP16 leaves, in a second FP16 matrix, until the last step, and
 // the epilogue of X = P X adds a times that second matrix: P acts as a I where it
-// matters, and the product needs no MMA more.  The norms of errors are then 1e-3 to 2e-3 of
+// matters, and the product needs no MMA more.  The norms of errors are then 1e-3 to 3e-3 of
 // the result's for noise, low ranks and spectra that fall by any power, 6e-3 for a few
-// orthogonal rows (restated in FP64 and measured; rounding to BF16 adds 1.7e-3).
+// orthogonal rows (restated in FP64 and measured; rounding to BF16 adds 1.7e-3).  At sides of
+// ten thousand the truncation below adds to low ranks: rank 2, 8192 x 8192 4.6e-3.
 //
 // X_0 is held as V * 2^j with a power of two that puts |V * 2^j|_F between 2^14 and 2^15;
 // the remaining factor rho enters the first products in FP32.  The norm is summed in FP64,
@@ -38,7 +39,7 @@
 // times the MMAs, errors for noise from 4e-6 (128 x 512) to 7e-5 (4096 x 14336).  The
 // tensor core truncates its FP32 sums, so errors grow with the sides, and with few
 // directions, as above, to more: rank 2 4e-5 (128 x 128), 2.5e-4 (768 x 768), 1.4e-3
-// (4096 x 4096); FP32 sums rounded to nearest 5e-5 at 768.  So P is held without its
+// (4096 x 4096), 2.8e-3 (8192 x 8192); FP32 sums rounded to nearest 5e-5 at 768.  So P is held without its
 // a I, and the epilogue adds all of a X: shorter sums to truncate (with a I in P: noise
 // 9e-5, rank 8 at 768 1.7e-4 instead of 8e-5).  (Sums of the first two steps in parts of
 // 512 of k, joined in the epilogue: rank 1 worse, 15 % more time at 4096 x 14336; not kept.)

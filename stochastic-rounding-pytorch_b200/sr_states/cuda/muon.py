@@ -62,11 +62,11 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=Non
     X_0 = x / (|x|_F + eps), then ``steps`` times X <- (a I + b G + c G^2) X with
     G = X X^T (for tall matrices X (a I + b G + c G^2), G = X^T X).  ``dtype``
     (default: that of ``x``) is the result's and sets the products' precision: BF16
-    results come from FP16 operands (relative errors of the whole matrix of 1e-3 to 2e-3,
-    about those of rounding it to BF16, and up to 6e-3 for a few orthogonal rows),
-    FP16 and FP32 results from pairs of FP16 operands (1e-5 for sides of some
-    hundreds, 1e-4 for ten thousand; 3e-4 and 2e-3 with ranks of a few; three times
-    the products); sums are FP32.
+    results come from FP16 operands (relative errors of the whole matrix of 1e-3 to 3e-3,
+    about those of rounding it to BF16; up to 6e-3 for a few orthogonal rows and for ranks
+    of a few at sides of ten thousand), FP16 and FP32 results from pairs of FP16 operands
+    (1e-5 for sides of some hundreds, 1e-4 for ten thousand; 3e-4 and 3e-3 with ranks of a
+    few; three times the products); sums are FP32.
     Singular values must stay below 15 through the steps (the default coefficients keep
     them below 1.3).  ``x``: FP32, BF16 or FP16, any strides; leading dimensions are a
     batch (at most 65535 matrices, of 2^32 elements and 2^24 rows or columns).

@@ -93,3 +93,27 @@ def test_fp32_sources_and_bf16_results(cuda_device):
         for source in (torch.float32, torch.float16):
             y = orthogonalize(x.to(source), dtype=torch.bfloat16)
             assert relative(y, newton(x.to(source))) <= 6 * U + BF16, (size, source)
+
+
+@pytest.mark.parametrize("size", [(3333, 3501), (3501, 3301), (4096, 4096)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_low_ranks_in_pairs(size, cuda_device):
+    """What FP16 leaves of X is carried in this form, too: without it, rank 1 is 15 % off.  16 u
+    for the roundings of any matrix; the sums' truncated terms, 200 k 2^-24 at most."""
+    from sr_states import orthogonalize
+    from sr_states.cuda import cuda_muon_step_
+
+    m, n = size
+    assert tile(m, n) == 256
+    gen = torch.Generator().manual_seed(10)
+    for rank in (1, 2, 40):
+        x = (torch.randn(m, rank, generator=gen) @ torch.randn(rank, n, generator=gen))
+        x = x.to(cuda_device)
+        want = newton(x)
+        cut = 200 * min(m, n) * 2.0**-24
+        assert relative(orthogonalize(x, dtype=torch.bfloat16), want) <= 16 * U + BF16 + cut, rank
+        assert relative(orthogonalize(x), want) <= 2.0**-12 + cut, rank
+        p, u = torch.zeros_like(x), torch.zeros_like(x)
+        cuda_muon_step_([p], [x], [u], lr=1.0, nesterov=False, seeds=[0])
+        factor = max(1.0, m / n) ** 0.5
+        assert relative(p, -factor * want) <= 16 * U + cut, rank
