@@ -186,7 +186,7 @@ def _sizes(rng, rows, groups, active):
 
 
 def _plan(index, groups):
-    """(index, order, ends): rows in the order of their groups, others behind."""
+    """(order, ends): rows in the order of their groups, others behind."""
     kept = [i if 0 <= i < groups else groups for i in index]
     order = sorted(range(len(kept)), key=kept.__getitem__)
     count = [0] * (groups + 1)
@@ -246,7 +246,7 @@ def prepare(case, seed):
         rng.shuffle(index)
     order, ends = _plan(index, case["adapters"])
     # the plan of the batch, made once for all layers that its tokens go through
-    state["plan"] = (_ints(index), _ints(order), _ints(ends))
+    state["index"], state["plan"] = _ints(index), (_ints(order), _ints(ends))
     state["sizes"] = sizes
     rank, many = case["rank"], case["adapters"]
     down = torch.randn((many, rank, k), generator=gen, device="cuda") * k ** -0.5
@@ -380,8 +380,7 @@ def _plain_expert(state):
 def _plain_adapter(state):
     case, x = state["case"], state["x"].detach()
     dtype, train = x.dtype, case["train"]
-    _, order, _ = state["plan"]
-    order, scale = order.long(), state["scale"]
+    order, scale = state["plan"][0].long(), state["scale"]
     down, up = state["down"].detach(), state["up"].detach()
     y = _values(*_quantize(x, "e4m3", "nearest", "row", 0)) @ _values(*state["w"]).t()
     if train:
@@ -527,7 +526,7 @@ def _exact_expert(state):
 
 def _exact_adapter(state):
     case, x = state["case"], state["x"].detach()
-    index, x64 = state["plan"][0], x.double()
+    index, x64 = state["index"], x.double()
     down, up = state["down"].detach().double(), state["up"].detach().double()
     scale = state["scale"].double()
     y = _exact_held(x, "e4m3") @ _exact_stored(*state["w"]).mT
