@@ -387,6 +387,20 @@ int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
                         void* data_t, int64_t data_t_pitch, void* scale_t,
                         int64_t scale_t_pitch, void* stream);
 
+/* Where a quantised copy goes: row pitches in elements and in blocks; in a stack, elements and
+ * blocks from one matrix to the next. */
+typedef struct srs_block_copy {
+  uint64_t data, scale; /* device addresses; data == 0: no such copy */
+  int64_t pitch, scale_pitch, stride, scale_stride;
+} srs_block_copy;
+
+/* A stack of at most 65535 matrices, each quantised as by srs_quantize_blocks; counters go on
+ * from one matrix to the next: (b*rows + i)*cols + j. */
+int srs_quantize_stack(const void* x, int x_format, int64_t matrices, int64_t rows, int64_t cols,
+                       int64_t x_pitch, int64_t x_stride, int out_format, int rule, int square,
+                       uint32_t seed, uint32_t offset, const srs_block_copy* copy,
+                       const srs_block_copy* copy_t, void* stream);
+
 typedef struct srs_blocks {
   uint64_t data;  /* device address, row pitch `pitch` bytes */
   uint64_t scale; /* device address, row pitch `scale_pitch` bytes */
@@ -406,6 +420,50 @@ int64_t srs_linear_workspace(int64_t tokens, int64_t k);
 int srs_linear_blocks(const void* x, int x_format, int64_t tokens, int64_t k, int64_t x_pitch,
                       int block_format, const srs_blocks* w, void* d, void* workspace,
                       int64_t workspace_bytes, void* stream);
+
+/* ---- rows in groups ---------------------------------------------------------
+ * No counterpart in the reference.  Group g of `groups` (at most SRS_MAX_GROUPS) has rows
+ * ends[g-1] .. ends[g] - 1 of a matrix (from 0 for the first); rows from the last end on
+ * belong to none.  `ends` is in device memory; it is read as its running maximum, cut to
+ * 0 .. rows, so that no value in it leads outside the matrix.
+ *
+ * srs_group_rows: stable sort of rows by their group.  index[i]: int32 (index_bytes 4) or int64
+ * (8); values outside 0 .. groups - 1 mean no group.  order: the rows of group 0 in order, then
+ * group 1's, .. , then those of none; ends[g]: rows with a group of at most g. */
+#define SRS_MAX_GROUPS 1024
+int srs_group_rows(const void* index, int index_bytes, int64_t rows, int groups, int32_t* order,
+                   int32_t* ends, void* stream);
+
+/* FP8 blocks of a matrix whose rows are in groups, for srs_expert_gradient: the transposed copy
+ * in blocks of 128 rows counted from each group's first, srs_group_columns(rows, groups)
+ * columns of data and srs_group_scales(rows, groups) of scales (a layout of the library's
+ * own); beside it, on demand, the copy by rows.  Rows of no group are not written.  Counters are
+ * those of srs_quantize_blocks. */
+int64_t srs_group_columns(int64_t rows, int groups);
+int64_t srs_group_scales(int64_t rows, int groups);
+int srs_quantize_groups(const void* x, int x_format, int64_t rows, int64_t cols, int64_t x_pitch,
+                        const int32_t* ends, int groups, int out_format, int rule, uint32_t seed,
+                        uint32_t offset, const srs_block_copy* copy, const srs_block_copy* copy_t,
+                        void* stream);
+
+/* d[i, :] = a[i, :] w_e^T for the rows i of group e; zeros for rows of none.  a: rows x k;
+ * w: `experts` matrices of n x k one after the other (w->rows = experts * n; square blocks start
+ * anew with every matrix); d: a->rows x n, contiguous.  Sums and limits as srs_matmul_blocks.
+ * experts * n is at most 2^30. */
+int srs_expert_matmul(const srs_blocks* a, const srs_blocks* w, int experts, const int32_t* ends,
+                      int64_t k, void* d, int d_format, void* stream);
+
+/* The same of x quantised to nearest in block_format (1 x 128 blocks) into `workspace`
+ * (srs_linear_workspace(rows, k) bytes, 16-byte aligned); d in x's format. */
+int srs_expert_linear(const void* x, int x_format, int64_t rows, int64_t k, int64_t x_pitch,
+                      int block_format, const srs_blocks* w, int experts, const int32_t* ends,
+                      void* d, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* d_e = a_e^T b_e for every group e: a_t and b_t are the transposed copies (srs_quantize_groups)
+ * of two matrices of `rows` rows, m x rows and n x rows; d: experts x m x n, contiguous; zeros
+ * for groups without rows. */
+int srs_expert_gradient(const srs_blocks* a_t, const srs_blocks* b_t, int64_t rows, int experts,
+                        const int32_t* ends, void* d, int d_format, void* stream);
 
 /* Rows of `cols` bytes at src_pitch copied to rows at dst_pitch (zeros behind them up to
  * dst_pitch): for operands whose rows do not start on 16-byte boundaries.  dst and

@@ -1,5 +1,5 @@
 """Build libsrs_b200.so (the sm_100a kernels and their C ABI) in-tree, and the
-host modules _srs_host and _srs_blocks (C++, CPython API and libtorch headers).
+host modules _srs_host, _srs_blocks and _srs_groups (C++, CPython API and libtorch headers).
 
     python stochastic-rounding-pytorch_b200/build_native.py [--force] [--verbose]
 
@@ -33,6 +33,11 @@ HOST_SOURCE = CSRC / "host_signature.cpp"
 # Tensor front end of the FP8 block entry points.
 BLOCKS = HERE / "sr_states" / "_native" / "_srs_blocks.so"
 BLOCKS_SOURCE = CSRC / "host_blocks.cpp"
+# Tensor front end of the operators on rows in groups.
+GROUPS = HERE / "sr_states" / "_native" / "_srs_groups.so"
+GROUPS_SOURCE = CSRC / "host_groups.cpp"
+# What both front ends include.
+FRONT_END = [CSRC / "host_blocks.h", INCLUDE / "srs_b200.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
@@ -51,7 +56,8 @@ FLAGS = [
 # (object name, source, extra defines)
 UNITS = [("srs_abi", "srs_abi.cu", []), ("srs_cast", "srs_cast.cu", []),
          ("srs_sgdm", "srs_sgdm.cu", []), ("srs_product", "srs_product.cu", []),
-         ("srs_newton", "srs_newton.cu", []), ("srs_blocks", "srs_blocks.cu", [])]
+         ("srs_newton", "srs_newton.cu", []), ("srs_blocks", "srs_blocks.cu", []),
+         ("srs_groups", "srs_groups.cu", []), ("srs_experts", "srs_experts.cu", [])]
 UNITS += [(f"srs_adamw_m{m}", "srs_adamw.cu", [f"-DSRS_M_FORMAT={m}"]) for m in range(5)]
 
 
@@ -79,7 +85,8 @@ def _kernels_up_to_date() -> bool:
 
 def _host_up_to_date() -> bool:
     return (_module_up_to_date(HOST, [HOST_SOURCE])
-            and _module_up_to_date(BLOCKS, [BLOCKS_SOURCE, INCLUDE / "srs_b200.h"]))
+            and _module_up_to_date(BLOCKS, [BLOCKS_SOURCE, *FRONT_END])
+            and _module_up_to_date(GROUPS, [GROUPS_SOURCE, *FRONT_END]))
 
 
 def _module_up_to_date(module: Path, sources: list[Path]) -> bool:
@@ -90,11 +97,13 @@ def _module_up_to_date(module: Path, sources: list[Path]) -> bool:
 def build_host(force: bool = False) -> Path:
     """The CPython modules against the installed torch (its headers for at::Tensor
     access, its libraries at run time)."""
-    with ThreadPoolExecutor(2) as pool:
+    includes = [f"-I{INCLUDE}", f"-I{CSRC}", f"-I{_cuda_include()}"]
+    with ThreadPoolExecutor(3) as pool:
         jobs = [pool.submit(_build_module, *m) for m in (
             (HOST, HOST_SOURCE, [], []),
-            (BLOCKS, BLOCKS_SOURCE, [f"-I{INCLUDE}", f"-I{_cuda_include()}"], ["-lc10_cuda"]))
-            if force or not _module_up_to_date(m[0], [m[1], INCLUDE / "srs_b200.h"])]
+            (BLOCKS, BLOCKS_SOURCE, includes, ["-lc10_cuda"]),
+            (GROUPS, GROUPS_SOURCE, includes, ["-lc10_cuda"]))
+            if force or not _module_up_to_date(m[0], [m[1], *FRONT_END])]
         for job in jobs:
             job.result()
     return HOST

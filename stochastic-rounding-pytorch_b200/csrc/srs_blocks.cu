@@ -6,6 +6,7 @@
 // product loop has no FP32 work of its own.
 #include "srs_host.h"
 #include "srs_common.cuh"
+#include "srs_groups.cuh"
 #include "srs_launch.h"
 
 namespace srs {
@@ -24,7 +25,20 @@ struct QuantizeArgs {
   uint8_t* data_t;
   uint8_t* scale_t;
   int64_t data_pitch, scale_pitch, data_t_pitch, scale_t_pitch;
+  // kStack: elements (scales: bytes) from one matrix to the next
+  int64_t x_stride, data_stride, scale_stride, data_t_stride, scale_t_stride;
+  // kGroups: see below
+  const int32_t* ends;
+  int groups;
+  const int32_t* order;  // rows kernel: row i of the copy is row order[i] of x (null: i)
 };
+
+// What a tile kernel's grid covers: one matrix; a stack of them (blockIdx.z), whose counters
+// go on from one to the next; or the rows of groups, tiles counted from a group's first
+// row.  The transposed copy of groups has the columns of tile i of all groups' tiles at
+// 128 i, zeros behind a group's last row, and a group's scales start at a multiple of 4
+// columns (products read them by words): rows of no group are not written.
+enum : int { kMatrix = 0, kStack = 1, kGroups = 2 };
 
 // k of a block whose largest finite |x| has FP32 encoding u: the largest values of
 // both formats are 1.75 * 2^TOP, so k = exponent - TOP, plus one where the
@@ -76,10 +90,10 @@ struct Size {
 };
 
 template <int XF>
-__device__ __forceinline__ void load_words(const QuantizeArgs& a, int64_t row, int64_t col,
-                                           uint32_t (&w)[kWords<XF>]) {
+__device__ __forceinline__ void load_words(const QuantizeArgs& a, int64_t row, int64_t row_end,
+                                           int64_t col, uint32_t (&w)[kWords<XF>]) {
   const int64_t left = a.cols - col;
-  if (row >= a.rows || left <= 0) {
+  if (row >= row_end || left <= 0) {
 #pragma unroll
     for (int j = 0; j < kWords<XF>; ++j) w[j] = 0u;
   } else if (a.vec && left >= 8) {
@@ -184,7 +198,12 @@ __device__ __forceinline__ void store_bytes(uint8_t* out, uint2 w, int left) {
 // integer units for the stochastic rule's hashes (37 us).
 constexpr int kAhead = 4;
 
-template <int OF, int XF>
+__device__ __forceinline__ int64_t ordered_row(const QuantizeArgs& a, int64_t row) {
+  const int64_t from = __ldg(a.order + row);
+  return from >= 0 && from < a.rows ? from : 0;
+}
+
+template <int OF, int XF, bool ORDERED>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a) {
   // A product launched to overlap this kernel (srs_linear_blocks) may start.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -193,7 +212,12 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
   const int64_t row0 = ((int64_t)blockIdx.y * 16 + (threadIdx.x >> 4)) * kAhead;
   uint32_t raw[kAhead][kWords<XF>];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) load_words<XF>(a, row0 + i, col, raw[i]);
+  for (int i = 0; i < kAhead; ++i) {
+    int64_t row = row0 + i;
+    // an entry of `order` that names no row of x reads its first
+    if (ORDERED && row < a.rows) row = ordered_row(a, row);
+    load_words<XF>(a, ORDERED && row0 + i >= a.rows ? a.rows : row, a.rows, col, raw[i]);
+  }
   uint32_t top = row_sizes<XF, kAhead>(raw, lane16);
   bool plain = !__any_sync(0xFFFFFFFFu, top >= Size<XF>::kInfinite);
   if (!plain) {
@@ -216,8 +240,9 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
     decode8<XF>(raw[i], y);
 #pragma unroll
     for (int j = 0; j < kVec; ++j) y[j] *= factor;
+    const int64_t from = ORDERED ? ordered_row(a, row) : row;
     const uint2 w =
-        encode_values<OF>(y, a.ctr + (uint32_t)(row * a.cols + col), a.rule, plain);
+        encode_values<OF>(y, a.ctr + (uint32_t)(from * a.cols + col), a.rule, plain);
     store_bytes(a.data + row * a.data_pitch + col, w, cols_left);
   }
 }
@@ -233,9 +258,20 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
 // would take 20.  128 x 128 blocks: 21 us rows, 31 both ways; stochastic 37 and 65.  A
 // reduction of 4 shuffles for every row and 16 partial maxima a column instead of 8 took
 // a fifth more.
-template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
+template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE, int COVER>
 __global__ void __launch_bounds__(kThreads, Fmt<XF>::kBytes == 2 ? 4 : 2)
-quantize_tile_kernel(const QuantizeArgs a) {
+quantize_tile_kernel(const __grid_constant__ QuantizeArgs args) {
+  QuantizeArgs a = args;
+  if constexpr (COVER == kStack) {
+    const int64_t z = blockIdx.z;
+    a.x = static_cast<const char*>(a.x) + z * a.x_stride * Fmt<XF>::kBytes;
+    a.data += z * a.data_stride;
+    a.scale += z * a.scale_stride;
+    a.data_t += z * a.data_t_stride;
+    a.scale_t += z * a.scale_t_stride;
+    a.ctr += (uint32_t)(z * a.rows * a.cols);
+    a.ctr_t += (uint32_t)(z * a.rows * a.cols);
+  }
   using Z = Size<XF>;
   constexpr int kW = kWords<XF>;
   extern __shared__ __align__(16) uint8_t tile_raw[];  // 128 x 128 elements of x
@@ -243,7 +279,17 @@ quantize_tile_kernel(const QuantizeArgs a) {
   __shared__ float row_factor[kBlock];
   __shared__ __align__(16) uint32_t turned[COLS ? kBlock * 32 : 4];
   const int lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
-  const int64_t row0 = (int64_t)blockIdx.y * kBlock, col0 = (int64_t)blockIdx.x * kBlock;
+  int64_t row0 = (int64_t)blockIdx.y * kBlock, row_end = a.rows;
+  const int64_t col0 = (int64_t)blockIdx.x * kBlock;
+  int64_t scale_t_at = blockIdx.y;  // column of the transposed copy's scales
+  if constexpr (COVER == kGroups) {
+    const GroupTile tile = find_group_tile(a.ends, a.groups, (int)a.rows, kBlock,
+                                           (int)blockIdx.y, (int)(threadIdx.x & 31));
+    if (tile.group < 0) return;
+    row0 = tile.row0;
+    row_end = tile.end;
+    scale_t_at = tile.quads;
+  }
   const int64_t row_base = row0 + 8 * group, col = col0 + 8 * lane16;
   // this thread's words of row i of its group: kW / 4 vectors of 16 bytes, 256 threads apart
   uint4* const mine = reinterpret_cast<uint4*>(tile_raw) + threadIdx.x;
@@ -255,7 +301,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
   {
     uint32_t raw[8][kW];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_words<XF>(a, row_base + i, col, raw[i]);
+    for (int i = 0; i < 8; ++i) load_words<XF>(a, row_base + i, row_end, col, raw[i]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
@@ -298,7 +344,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
         const int k = block_exponent<OF>(Z::as_f32(top));
         if (lane16 < 8) {
           row_factor[8 * group + lane16] = power_of_two(-k);
-          if (row_base + lane16 < a.rows)
+          if (row_base + lane16 < row_end)
             a.scale[(row_base + lane16) * a.scale_pitch + blockIdx.x] = (uint8_t)(k + 127);
         }
       }
@@ -353,7 +399,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
           const int k = block_exponent<OF>(Z::as_f32(col_top[j]));
           col_factor[j] = power_of_two(-k);
           if (group == 0 && col + j < a.cols)
-            a.scale_t[(col + j) * a.scale_t_pitch + blockIdx.y] = (uint8_t)(k + 127);
+            a.scale_t[(col + j) * a.scale_t_pitch + scale_t_at] = (uint8_t)(k + 127);
         }
       }
     }
@@ -363,7 +409,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
   uint32_t ctr = a.ctr + (uint32_t)(row_base * a.cols + col);
   uint32_t ctr_t = a.ctr_t + (uint32_t)(row_base * a.cols + col);
   const float tile_factor = power_of_two(-tile_k);
-  const int rows_left = (int)min(a.rows - row_base, (int64_t)8);
+  const int rows_left = (int)min(row_end - row_base, (int64_t)8);
   const int cols_left = (int)min(a.cols - col, (int64_t)kVec);
   uint8_t* out = a.data + row_base * a.data_pitch + col;
   uint32_t* turn = turned + (COLS ? 8 * group * 32 + ((2 * lane16 + 4 * (group >> 1)) & 31) : 0);
@@ -401,7 +447,7 @@ quantize_tile_kernel(const QuantizeArgs a) {
     if (ROWS)
       a.scale[(int64_t)blockIdx.y * a.scale_pitch + blockIdx.x] = (uint8_t)(tile_k + 127);
     if (COLS)
-      a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + blockIdx.y] = (uint8_t)(tile_k + 127);
+      a.scale_t[(int64_t)blockIdx.x * a.scale_t_pitch + scale_t_at] = (uint8_t)(tile_k + 127);
   }
 
   if constexpr (COLS) {
@@ -422,8 +468,9 @@ quantize_tile_kernel(const QuantizeArgs a) {
                                 0x5410u);
       }
     }
-    const int64_t at = row0 + 16 * h;
-    const int left = (int)min(a.rows - at, (int64_t)16);
+    // of groups: whole tiles, the rows behind a group's last are the zeros that were loaded
+    const int64_t at = (int64_t)blockIdx.y * kBlock + 16 * h;
+    const int left = COVER == kGroups ? 16 : (int)min(a.rows - at, (int64_t)16);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t to = col0 + 4 * word + c;
@@ -439,10 +486,10 @@ quantize_tile_kernel(const QuantizeArgs a) {
   }
 }
 
-template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE>
+template <int OF, int XF, bool ROWS, bool COLS, bool SQUARE, int COVER = kMatrix>
 cudaError_t launch_tile(const QuantizeArgs& a, dim3 grid, cudaStream_t stream) {
   constexpr int kTileBytes = kBlock * kBlock * Fmt<XF>::kBytes;
-  const auto kernel = &quantize_tile_kernel<OF, XF, ROWS, COLS, SQUARE>;
+  const auto kernel = &quantize_tile_kernel<OF, XF, ROWS, COLS, SQUARE, COVER>;
   if (kTileBytes + (COLS ? 24 * 1024 : 0) > 40 * 1024) {
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileBytes);
@@ -452,30 +499,52 @@ cudaError_t launch_tile(const QuantizeArgs& a, dim3 grid, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// One form of block and of copies, for a matrix, a stack or groups.
+template <int OF, int XF, int COVER>
+cudaError_t launch_tiles(const QuantizeArgs& a, bool square, dim3 tiles, cudaStream_t stream) {
+  const bool rows = a.data != nullptr, cols = a.data_t != nullptr;
+  if constexpr (COVER != kGroups) {
+    if (square) {
+      if (rows && cols) return launch_tile<OF, XF, true, true, true, COVER>(a, tiles, stream);
+      return rows ? launch_tile<OF, XF, true, false, true, COVER>(a, tiles, stream)
+                  : launch_tile<OF, XF, false, true, true, COVER>(a, tiles, stream);
+    }
+    if (COVER == kStack && !cols)
+      return launch_tile<OF, XF, true, false, false, COVER>(a, tiles, stream);
+  }
+  return rows ? launch_tile<OF, XF, true, true, false, COVER>(a, tiles, stream)
+              : launch_tile<OF, XF, false, true, false, COVER>(a, tiles, stream);
+}
+
 template <int OF, int XF>
-cudaError_t launch_quantize(const QuantizeArgs& a, bool square, cudaStream_t stream) {
+cudaError_t launch_quantize(const QuantizeArgs& a, bool square, int matrices,
+                            cudaStream_t stream) {
   const unsigned columns = (unsigned)((a.cols + kBlock - 1) / kBlock);
   const dim3 tiles(columns, (unsigned)((a.rows + kBlock - 1) / kBlock));
-  const bool rows = a.data != nullptr, cols = a.data_t != nullptr;
-  if (square) {
-    if (rows && cols) return launch_tile<OF, XF, true, true, true>(a, tiles, stream);
-    return rows ? launch_tile<OF, XF, true, false, true>(a, tiles, stream)
-                : launch_tile<OF, XF, false, true, true>(a, tiles, stream);
+  if (a.ends != nullptr) {
+    const dim3 grid(columns, (unsigned)most_group_tiles(a.rows, a.groups, kBlock));
+    return launch_tiles<OF, XF, kGroups>(a, false, grid, stream);
   }
-  if (cols)
-    return rows ? launch_tile<OF, XF, true, true, false>(a, tiles, stream)
-                : launch_tile<OF, XF, false, true, false>(a, tiles, stream);
+  if (matrices > 1)
+    return launch_tiles<OF, XF, kStack>(a, square, dim3(tiles.x, tiles.y, (unsigned)matrices),
+                                        stream);
+  if (square || a.data_t != nullptr) return launch_tiles<OF, XF, kMatrix>(a, square, tiles, stream);
   const dim3 grid(columns, (unsigned)((a.rows + 16 * kAhead - 1) / (16 * kAhead)));
-  quantize_rows_kernel<OF, XF><<<grid, kThreads, 0, stream>>>(a);
+  if (a.order != nullptr)
+    quantize_rows_kernel<OF, XF, true><<<grid, kThreads, 0, stream>>>(a);
+  else
+    quantize_rows_kernel<OF, XF, false><<<grid, kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 template <int OF>
-cudaError_t launch_quantize(const QuantizeArgs& a, int x_format, bool square,
+cudaError_t launch_quantize(const QuantizeArgs& a, int x_format, bool square, int matrices,
                             cudaStream_t stream) {
-  if (x_format == SRS_FMT_F32) return launch_quantize<OF, SRS_FMT_F32>(a, square, stream);
-  if (x_format == SRS_FMT_BF16) return launch_quantize<OF, SRS_FMT_BF16>(a, square, stream);
-  return launch_quantize<OF, SRS_FMT_F16>(a, square, stream);
+  if (x_format == SRS_FMT_F32)
+    return launch_quantize<OF, SRS_FMT_F32>(a, square, matrices, stream);
+  if (x_format == SRS_FMT_BF16)
+    return launch_quantize<OF, SRS_FMT_BF16>(a, square, matrices, stream);
+  return launch_quantize<OF, SRS_FMT_F16>(a, square, matrices, stream);
 }
 
 // 16 bytes of the copy a thread, from any source alignment.
@@ -506,17 +575,28 @@ uint32_t host_h32(uint32_t x) {
 
 int64_t blocks_of(int64_t x) { return (x + kBlock - 1) / kBlock; }
 
-int check_copy(const char* what, const void* data, int64_t pitch, const void* scale,
-               int64_t scale_pitch, int64_t cols) {
-  if (scale == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "%s has data but no scale", what);
-  if (reinterpret_cast<uintptr_t>(data) % 16 != 0 || pitch % 16 != 0 || pitch < cols)
+int check_copy(const char* what, const srs_block_copy& c, int64_t cols, int64_t blocks,
+               int64_t matrices) {
+  if (c.scale == 0) return fail(SRS_ERR_INVALID_ARGUMENT, "%s has data but no scale", what);
+  if (c.data % 16 != 0 || c.pitch % 16 != 0 || c.pitch < cols ||
+      (matrices > 1 && c.stride % 16 != 0))
     return fail(SRS_ERR_INVALID_ARGUMENT,
                 "%s needs a 16-byte aligned address and a row pitch that is a multiple of 16 and "
                 "at least the row length (%lld, %lld)",
-                what, (long long)pitch, (long long)cols);
-  if (scale_pitch < blocks_of(cols))
+                what, (long long)c.pitch, (long long)cols);
+  if (c.scale_pitch < blocks)
     return fail(SRS_ERR_INVALID_ARGUMENT, "%s: scale pitch %lld, %lld blocks a row", what,
-                (long long)scale_pitch, (long long)blocks_of(cols));
+                (long long)c.scale_pitch, (long long)blocks);
+  return SRS_OK;
+}
+
+}  // namespace
+
+int check_groups(const int32_t* ends, int groups) {
+  if (groups < 1 || groups > kMaxGroups)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "groups must be in [1, %d], got %d", kMaxGroups, groups);
+  if (ends == nullptr || reinterpret_cast<uintptr_t>(ends) % 4 != 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned ends");
   return SRS_OK;
 }
 
@@ -540,64 +620,69 @@ int check_operand(const char* what, const srs_blocks* b, int64_t k) {
   return SRS_OK;
 }
 
-}  // namespace
 }  // namespace srs
 
 using namespace srs;
 
-// `for_product`: ahead of a product in the same call.
-static int quantize_blocks(bool for_product, const void* x, int x_format, int64_t rows,
-                           int64_t cols, int64_t x_pitch, int out_format, int rule, int square,
-                           uint32_t seed, uint32_t offset, void* data, int64_t data_pitch, void* scale,
-                           int64_t scale_pitch, void* data_t, int64_t data_t_pitch, void* scale_t,
-                           int64_t scale_t_pitch, cudaStream_t stream) {
-  if (x_format < SRS_FMT_F32 || x_format > SRS_FMT_F16)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported input format %d", x_format);
-  if (out_format != SRS_FMT_E4M3 && out_format != SRS_FMT_E5M2)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "unknown output format %d (E4M3 or E5M2)", out_format);
-  if (!valid_rule(rule)) return fail(SRS_ERR_INVALID_ARGUMENT, "unknown rounding rule %d", rule);
-  if (rows < 0 || cols < 0 || x_pitch < 0)
+int srs::quantize(const QuantizeCall& q, cudaStream_t stream) {
+  if (q.x_format < SRS_FMT_F32 || q.x_format > SRS_FMT_F16)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "unsupported input format %d", q.x_format);
+  if (q.out_format != SRS_FMT_E4M3 && q.out_format != SRS_FMT_E5M2)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "unknown output format %d (E4M3 or E5M2)", q.out_format);
+  if (!valid_rule(q.rule)) return fail(SRS_ERR_INVALID_ARGUMENT, "unknown rounding rule %d", q.rule);
+  if (q.rows < 0 || q.cols < 0 || q.x_pitch < 0 || q.matrices < 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "negative size or pitch");
-  if (rows > 65535ll * 16 * kAhead || cols > (1ll << 30))
-    return fail(SRS_ERR_INVALID_ARGUMENT, "%lld x %lld is too large", (long long)rows,
-                (long long)cols);
-  if (data == nullptr && data_t == nullptr)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "null outputs");
-  if (rows == 0 || cols == 0) return SRS_OK;
-  if (x == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null input pointer");
-  if (reinterpret_cast<uintptr_t>(x) % fmt_bytes(x_format) != 0)
+  if (q.rows > 65535ll * 16 * kAhead || q.cols > (1ll << 30) || q.matrices > 65535)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "%lld x %lld is too large", (long long)q.rows,
+                (long long)q.cols);
+  const srs_block_copy &copy = q.copy, &turned = q.turned;
+  if (copy.data == 0 && turned.data == 0) return fail(SRS_ERR_INVALID_ARGUMENT, "null outputs");
+  if (q.rows == 0 || q.cols == 0 || q.matrices == 0) return SRS_OK;
+  if (q.x == nullptr) return fail(SRS_ERR_INVALID_ARGUMENT, "null input pointer");
+  if (reinterpret_cast<uintptr_t>(q.x) % fmt_bytes(q.x_format) != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "input pointer is not element aligned");
-  if (data != nullptr)
-    if (int rc = check_copy("the copy", data, data_pitch, scale, scale_pitch, cols)) return rc;
-  if (data_t != nullptr)
-    if (int rc = check_copy("the transposed copy", data_t, data_t_pitch, scale_t, scale_t_pitch,
-                            rows))
-      return rc;
+  const int64_t tiles = q.ends == nullptr ? 0 : most_group_tiles(q.rows, q.groups, kBlock);
+  if (copy.data != 0)
+    if (int rc = check_copy("the copy", copy, q.cols, blocks_of(q.cols), q.matrices)) return rc;
+  if (turned.data != 0) {
+    const int64_t cols = q.ends == nullptr ? q.rows : tiles * kBlock;
+    const int64_t scales = q.ends == nullptr ? blocks_of(q.rows) : srs_group_scales(q.rows, q.groups);
+    if (int rc = check_copy("the transposed copy", turned, cols, scales, q.matrices)) return rc;
+  }
   if (int rc = check_device()) return rc;
-  if (for_product)
+  if (q.for_product)
     if (int rc = check_products()) return rc;
   QuantizeArgs a{};
-  a.x = x;
-  a.rows = rows;
-  a.cols = cols;
-  a.x_pitch = x_pitch;
-  a.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_pitch % 8 == 0;
-  a.rule = rule;
-  a.ctr = offset + host_h32(seed);
-  a.ctr_t = offset + host_h32(seed ^ 1u);
-  a.data = static_cast<uint8_t*>(data);
-  a.scale = static_cast<uint8_t*>(scale);
-  a.data_t = static_cast<uint8_t*>(data_t);
-  a.scale_t = static_cast<uint8_t*>(scale_t);
-  a.data_pitch = data_pitch;
-  a.scale_pitch = scale_pitch;
-  a.data_t_pitch = data_t_pitch;
-  a.scale_t_pitch = scale_t_pitch;
+  a.x = q.x;
+  a.rows = q.rows;
+  a.cols = q.cols;
+  a.x_pitch = q.x_pitch;
+  a.x_stride = q.x_stride;
+  a.vec = reinterpret_cast<uintptr_t>(q.x) % 16 == 0 && q.x_pitch % 8 == 0 &&
+          (q.matrices == 1 || q.x_stride % 8 == 0);
+  a.rule = q.rule;
+  a.ctr = q.offset + host_h32(q.seed);
+  a.ctr_t = q.offset + host_h32(q.seed ^ 1u);
+  a.data = reinterpret_cast<uint8_t*>(copy.data);
+  a.scale = reinterpret_cast<uint8_t*>(copy.scale);
+  a.data_t = reinterpret_cast<uint8_t*>(turned.data);
+  a.scale_t = reinterpret_cast<uint8_t*>(turned.scale);
+  a.data_pitch = copy.pitch;
+  a.scale_pitch = copy.scale_pitch;
+  a.data_stride = copy.stride;
+  a.scale_stride = copy.scale_stride;
+  a.data_t_pitch = turned.pitch;
+  a.scale_t_pitch = turned.scale_pitch;
+  a.data_t_stride = turned.stride;
+  a.scale_t_stride = turned.scale_stride;
+  a.ends = q.ends;
+  a.groups = q.groups;
+  a.order = q.order;
   const cudaError_t e =
-      out_format == SRS_FMT_E4M3
-          ? launch_quantize<SRS_FMT_E4M3>(a, x_format, square != 0, stream)
-          : launch_quantize<SRS_FMT_E5M2>(a, x_format, square != 0, stream);
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_quantize_blocks launch");
+      q.out_format == SRS_FMT_E4M3
+          ? launch_quantize<SRS_FMT_E4M3>(a, q.x_format, q.square, (int)q.matrices, stream)
+          : launch_quantize<SRS_FMT_E5M2>(a, q.x_format, q.square, (int)q.matrices, stream);
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "FP8 block quantisation launch");
 }
 
 extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, int64_t cols,
@@ -607,9 +692,54 @@ extern "C" int srs_quantize_blocks(const void* x, int x_format, int64_t rows, in
                                    int64_t data_t_pitch, void* scale_t, int64_t scale_t_pitch,
                                    void* stream) {
   clear_error();
-  return quantize_blocks(false, x, x_format, rows, cols, x_pitch, out_format, rule, square, seed,
-                         offset, data, data_pitch, scale, scale_pitch, data_t, data_t_pitch,
-                         scale_t, scale_t_pitch, static_cast<cudaStream_t>(stream));
+  QuantizeCall q{x, x_format, rows, cols, x_pitch, out_format, rule, square != 0, seed, offset};
+  q.copy = {reinterpret_cast<uint64_t>(data), reinterpret_cast<uint64_t>(scale), data_pitch,
+            scale_pitch, 0, 0};
+  q.turned = {reinterpret_cast<uint64_t>(data_t), reinterpret_cast<uint64_t>(scale_t),
+              data_t_pitch, scale_t_pitch, 0, 0};
+  return quantize(q, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int srs_quantize_stack(const void* x, int x_format, int64_t matrices, int64_t rows,
+                                  int64_t cols, int64_t x_pitch, int64_t x_stride, int out_format,
+                                  int rule, int square, uint32_t seed, uint32_t offset,
+                                  const srs_block_copy* copy, const srs_block_copy* copy_t,
+                                  void* stream) {
+  clear_error();
+  QuantizeCall q{x, x_format, rows, cols, x_pitch, out_format, rule, square != 0, seed, offset};
+  q.matrices = matrices;
+  q.x_stride = x_stride;
+  if (copy != nullptr) q.copy = *copy;
+  if (copy_t != nullptr) q.turned = *copy_t;
+  return quantize(q, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t srs_group_columns(int64_t rows, int groups) {
+  return rows <= 0 || groups <= 0 ? 0 : kBlock * most_group_tiles(rows, groups, kBlock);
+}
+
+extern "C" int64_t srs_group_scales(int64_t rows, int groups) {
+  // every group with rows takes a multiple of 4 columns
+  return rows <= 0 || groups <= 0
+             ? 0
+             : most_group_tiles(rows, groups, kBlock) + 3 * (groups < rows ? groups : rows);
+}
+
+extern "C" int srs_quantize_groups(const void* x, int x_format, int64_t rows, int64_t cols,
+                                   int64_t x_pitch, const int32_t* ends, int groups,
+                                   int out_format, int rule, uint32_t seed, uint32_t offset,
+                                   const srs_block_copy* copy, const srs_block_copy* copy_t,
+                                   void* stream) {
+  clear_error();
+  if (int rc = check_groups(ends, groups)) return rc;
+  if (copy_t == nullptr || copy_t->data == 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "groups need the transposed copy");
+  QuantizeCall q{x, x_format, rows, cols, x_pitch, out_format, rule, false, seed, offset};
+  q.ends = ends;
+  q.groups = groups;
+  if (copy != nullptr) q.copy = *copy;
+  q.turned = *copy_t;
+  return quantize(q, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int srs_copy_rows(const void* src, int64_t src_pitch, int64_t rows, int64_t cols,
@@ -692,11 +822,11 @@ extern "C" int srs_linear_blocks(const void* x, int x_format, int64_t tokens, in
   rows.format = block_format;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (k == 0) return srs_matmul_blocks(&rows, w, k, d, x_format, stream);
-  if (int rc = quantize_blocks(true, x, x_format, tokens, k, x_pitch, block_format,
-                               SRS_RULE_NEAREST, 0, 0u, 0u, workspace, rows.pitch,
-                               static_cast<char*>(workspace) + tokens * rows.pitch,
-                               rows.scale_pitch, nullptr, 0, nullptr, 0, st))
-    return rc;
+  QuantizeCall q{x,     x_format, tokens, k, x_pitch, block_format, SRS_RULE_NEAREST,
+                 false, 0u,       0u};
+  q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
+  q.for_product = true;
+  if (int rc = quantize(q, st)) return rc;
   // With few tokens the product starts beside the quantisation and streams the
   // weights, which that kernel does not write, before it needs the tokens.
   if (tokens <= kThinRows && w->rows >= tokens) {

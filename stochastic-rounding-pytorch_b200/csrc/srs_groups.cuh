@@ -1,0 +1,88 @@
+// Rows in groups: group g has rows ends[g-1] .. ends[g] - 1 of a matrix (from 0 for the
+// first), rows from the last end on belong to none.  `ends` is in device memory and the
+// host never reads it: grids are sized by a bound and every CTA finds its own part.
+//
+// Ends are read as their running maximum, cut to 0 .. rows: whatever the array holds, the
+// groups lie inside the matrix, do not overlap, and their tiles stay within the bound
+//   rows / edge + groups
+// that buffers and grids are sized by.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace srs {
+
+constexpr int kMaxGroups = 1024;
+
+__device__ __forceinline__ int warp_scan_sum(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int warp_scan_max(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+    if (lane >= d) v = max(v, u);
+  }
+  return v;
+}
+
+// Groups base .. base + 31 for a warp, one a lane; `carry`: end of the group before.
+// Groups from `groups` on are empty.
+__device__ __forceinline__ void group_span(const int32_t* __restrict__ ends, int groups, int rows,
+                                           int base, int lane, int* carry, int* start, int* end) {
+  const int g = base + lane;
+  int e = g < groups ? min(max(ends[g], 0), rows) : 0;
+  e = max(warp_scan_max(e, lane), *carry);
+  const int before = __shfl_up_sync(0xFFFFFFFFu, e, 1);
+  *start = lane == 0 ? *carry : before;
+  *end = e;
+  *carry = __shfl_sync(0xFFFFFFFFu, e, 31);
+}
+
+// One tile of `edge` rows at most, counted from its group's first row.
+struct GroupTile {
+  int group;      // -1: there is no such tile
+  int row0, end;  // first row of the tile, end of its group
+  int quads;      // 4 * (words of 4 tiles that groups before it take) + tiles before it in its own
+};
+
+// Tile `index` of all groups' tiles in order, found by a warp (the same in all lanes).
+__device__ __forceinline__ GroupTile find_group_tile(const int32_t* __restrict__ ends, int groups,
+                                                     int rows, int edge, int index, int lane) {
+  GroupTile r{-1, 0, 0, 0};
+  int carry = 0, tiles_before = 0, quads_before = 0;
+  for (int base = 0; base < groups; base += 32) {
+    int start, end;
+    group_span(ends, groups, rows, base, lane, &carry, &start, &end);
+    const int tiles = (end - start + edge - 1) / edge, quads = (tiles + 3) & ~3;
+    const int upto = tiles_before + warp_scan_sum(tiles, lane);
+    const int quads_upto = quads_before + warp_scan_sum(quads, lane);
+    const unsigned found = __ballot_sync(0xFFFFFFFFu, upto > index);
+    if (found != 0u) {
+      const int at = __ffs(found) - 1, inside = index - (upto - tiles);
+      r.group = base + at;
+      r.row0 = __shfl_sync(0xFFFFFFFFu, start + inside * edge, at);
+      r.end = __shfl_sync(0xFFFFFFFFu, end, at);
+      r.quads = __shfl_sync(0xFFFFFFFFu, quads_upto - quads + inside, at);
+      return r;
+    }
+    tiles_before = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    quads_before = __shfl_sync(0xFFFFFFFFu, quads_upto, 31);
+  }
+  return r;
+}
+
+// Most tiles of `edge` rows that `groups` groups of `rows` rows in all can have.
+inline int64_t most_group_tiles(int64_t rows, int64_t groups, int64_t edge) {
+  // every group with rows has at most one tile that is not full
+  return rows / edge + (groups < rows ? groups : rows);
+}
+
+}  // namespace srs

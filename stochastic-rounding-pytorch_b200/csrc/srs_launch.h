@@ -41,6 +41,29 @@ int launch_groups(const void* kernel, int64_t groups, int group, int threads, in
                   bool cooperative, void* argument, cudaStream_t stream, const char* what,
                   bool overlap = false);
 
+// What is quantised to FP8 blocks, and where to (srs_quantize_blocks, _stack and _groups):
+// one matrix, a stack of them (`matrices`, `x_stride` elements apart), rows of groups (`ends`;
+// the transposed copy in the products' form), or rows in another order (`order`: row i of
+// the copy is row order[i] of x; rows alone).  `for_product`: ahead of a product of the same call.
+struct QuantizeCall {
+  const void* x;
+  int x_format;
+  int64_t rows, cols, x_pitch;
+  int out_format, rule;
+  bool square;
+  uint32_t seed, offset;
+  srs_block_copy copy{}, turned{};
+  int64_t matrices = 1, x_stride = 0;
+  const int32_t* ends = nullptr;
+  int groups = 0;
+  const int32_t* order = nullptr;
+  bool for_product = false;
+};
+int quantize(const QuantizeCall& q, cudaStream_t stream);
+
+int check_operand(const char* what, const srs_blocks* b, int64_t k);
+int check_groups(const int32_t* ends, int groups);
+
 // FP8 blocks: d = a b^T (operands checked by the caller).  Element (i, j)
 // of d is stored at i * row_stride + j * col_stride; only products with a thin side
 // (at most kThinRows rows) take a col_stride other than 1.  `overlap`: the kernel ahead
@@ -50,5 +73,8 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
                          int d_format, cudaStream_t stream);
 int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
                 int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream);
+// The same for rows in groups: a's rows by their group's matrix of w (few rows a group).
+int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
+                       int64_t k, void* d, int d_format, bool overlap, cudaStream_t stream);
 
 }  // namespace srs

@@ -188,14 +188,6 @@ struct BlockProduct {
   int edge;  // of a tile
 };
 
-struct BlockScales {
-  const uint8_t* a;
-  const uint8_t* b;
-  int64_t a_pitch, b_pitch;
-  int a_shift, b_shift, m, n;
-  bool a_words, b_words;
-};
-
 struct BlockSource {
   const BlockProduct& w;
   __device__ int phases() const { return 1; }
@@ -223,12 +215,13 @@ struct BlockSource {
     s.pitch = w.n;
     return s;
   }
-  __device__ BlockScales scales() const {
-    return {w.scale_a,       w.scale_b,       w.scale_a_pitch, w.scale_b_pitch,
-            w.scale_a_shift, w.scale_b_shift, w.m,             w.n,
-            scale_words(w.scale_a, w.scale_a_pitch, 0),
-            scale_words(w.scale_b, w.scale_b_pitch, 0)};
+  __device__ BlockScales scales(uint32_t t) const {
+    const TileLoad at = load(0, t);
+    return {w.scale_a,       w.scale_b, w.scale_a_pitch, w.scale_b_pitch, w.scale_a_shift,
+            w.scale_b_shift, at.row0,   at.col0,         w.m,             w.n,
+            w.slices};
   }
+  __device__ void spare(int) const {}
 };
 
 template <int CG>
@@ -297,10 +290,11 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
 
 namespace {
 
-template <int BN>
-int launch_thin_as(ThinArgs& args, int splits, bool overlap, cudaStream_t stream) {
+// `tiles`: of the grid (clusters of `splits` CTAs).
+template <int BN, bool GROUPED>
+int launch_thin_as(ThinArgs& args, int64_t tiles, int splits, bool overlap, cudaStream_t stream) {
   using S = ThinShape<BN>;
-  const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN>);
+  const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN, GROUPED>);
   // As many stages as fit before a whole panel: the MMA reads 128 rows from the start of
   // the last stage's panel, past the end of that stage when its tile has fewer.
   args.panel_bytes = (args.rows + 7) / 8 * 8 * kSliceBytes;
@@ -313,8 +307,8 @@ int launch_thin_as(ThinArgs& args, int splits, bool overlap, cudaStream_t stream
   int resident = 0;
   if (int rc = prepare_kernel(kernel, 1, kThinThreads, S::kFixed + S::kBudget, &resident))
     return rc;
-  return launch_groups(kernel, (args.m + args.rows - 1) / args.rows, splits, kThinThreads,
-                       S::kFixed + bytes, false, &args, stream, "thin product launch", overlap);
+  return launch_groups(kernel, tiles, splits, kThinThreads, S::kFixed + bytes, false, &args,
+                       stream, "thin product launch", overlap);
 }
 
 }  // namespace
@@ -354,9 +348,50 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
   args.out_format = d_format;
   args.row_stride = row_stride;
   args.col_stride = col_stride;
-  if (columns == 16) return launch_thin_as<16>(args, splits, overlap, stream);
-  if (columns == 32) return launch_thin_as<32>(args, splits, overlap, stream);
-  return launch_thin_as<64>(args, splits, overlap, stream);
+  const int64_t grid = (args.m + args.rows - 1) / args.rows;
+  if (columns == 16) return launch_thin_as<16, false>(args, grid, splits, overlap, stream);
+  if (columns == 32) return launch_thin_as<32, false>(args, grid, splits, overlap, stream);
+  return launch_thin_as<64, false>(args, grid, splits, overlap, stream);
+}
+
+int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
+                       int64_t k, void* d, int d_format, bool overlap, cudaStream_t stream) {
+  const int64_t n = w.rows / experts, busy = experts < a.rows ? experts : a.rows;
+  // Columns for the mean group and half of it more; a larger group takes several tiles.
+  const int64_t mean = (3 * a.rows + 2 * busy - 1) / (2 * busy);
+  const int columns = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  ThinArgs args{};
+  args.m = (int)n;
+  args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
+  args.rows = 128;
+  const int64_t sms = sm_count(), tiles = (n + 127) / 128;
+  const int64_t likely = tiles * busy, most = tiles * most_group_tiles(a.rows, experts, columns);
+  int splits = 1;
+  while (splits < 8 && likely * splits <= sms && args.slices >= 4 * splits) splits *= 2;
+  if (most * splits >= (1ll << 31))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "a result of %lld x %lld is too large",
+                (long long)a.rows, (long long)n);
+  if (int rc = operand_map(w, k, args.rows, &args.map_a)) return rc;
+  if (int rc = operand_map(a, k, columns, &args.map_b)) return rc;
+  if (int rc = status_word(&args.status)) return rc;
+  args.n = (int)a.rows;
+  args.scale_a = reinterpret_cast<const uint8_t*>(w.scale);
+  args.scale_b = reinterpret_cast<const uint8_t*>(a.scale);
+  args.scale_a_pitch = w.scale_pitch;
+  args.scale_b_pitch = a.scale_pitch;
+  args.scale_a_shift = w.square ? 7 : 0;
+  args.scale_b_shift = 0;
+  args.scale_a_group = (w.square ? (n + 127) / 128 : n) * w.scale_pitch;
+  args.idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 | format_bits(w, a) | 1u << 23;
+  args.out = d;
+  args.out_format = d_format;
+  args.row_stride = 1;
+  args.col_stride = n;
+  args.ends = ends;
+  args.groups = experts;
+  if (columns == 16) return launch_thin_as<16, true>(args, most, splits, overlap, stream);
+  if (columns == 32) return launch_thin_as<32, true>(args, most, splits, overlap, stream);
+  return launch_thin_as<64, true>(args, most, splits, overlap, stream);
 }
 
 }  // namespace srs

@@ -58,6 +58,7 @@ struct TileLoad {
   // times: low by high, high by low, then high by high parts.  (The tensor core truncates
   // its FP32 sums at every step: the small parts go first, while the sum is small;
   // 4096 x 14336 to FP32 was 1.3e-4 off so, with the high parts first 2.5e-4.)
+  int k0;  // FP8: the first element of k of both operands
 };
 
 // What happens to a tile's accumulator.
@@ -117,6 +118,16 @@ struct ScaleRows {
       }
     }
   }
+};
+
+// Block scales of a tile's operands: rows row0 .. of `a` (m rows), col0 .. of `b`
+// (n rows), `slices` blocks of each from the first on.
+struct BlockScales {
+  const uint8_t* a;
+  const uint8_t* b;
+  int64_t a_pitch, b_pitch;
+  int a_shift, b_shift;  // 7 when one scale covers 128 rows
+  int row0, col0, m, n, slices;
 };
 
 __device__ __forceinline__ bool scale_words(const uint8_t* scale, int64_t pitch, int kb) {
@@ -474,7 +485,8 @@ struct ProductShape {
 // The CTA's work.  Source gives: phases(), tiles(phase), load(phase, tile),
 // store(phase, tile), formats() (bits of the instruction descriptor), counter(phase),
 // status() and longest() (slices of a tile, where they can take seconds); for FP8 also
-// scales(): the operands' block scales.
+// scales(tile): the operands' block scales, and spare(lane): work of the warp that has
+// no role (results that are zero without a product).
 template <int KIND, int CG, bool NEWTON, bool SPLIT, class Source>
 __device__ __forceinline__ void run_products(const Source& src) {
   using S = ProductShape<KIND, CG>;
@@ -557,7 +569,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
           const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
           const uint32_t pa = stage0 + s * S::kStageBytes, pb = pa + kPanelBytes;
           const int part = SPLIT ? (i >= third) + (i >= 2 * third) : 0;
-          const int k = (i - part * third) * kSliceK;
+          const int k = (i - part * third) * kSliceK + (KIND == kOperandF8 ? at.k0 : 0);
           const int low_a = SPLIT && part == 0 ? 1 : 0, low_b = SPLIT && part == 1 ? 1 : 0;
           if (leader) {
             if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
@@ -700,28 +712,30 @@ __device__ __forceinline__ void run_products(const Source& src) {
       // row r at 16 * (r % 32) + 4 * (r / 32) of its 512-byte group, the order in
       // which the tensor core reads them from 4 TMEM columns.  One group ahead: the
       // next group's scales are requested before this one's slot is waited for.
-      const auto scales = src.scales();
       int slot = 0;
       uint32_t parity = 0;
       uint32_t t = first;
       int kb = 0, slices = 0;
+      bool a_words = false, b_words = false;
       ScaleRows from[1 + CG];
       uint32_t next[1 + CG][4];
       const uint32_t tiles = src.tiles(0);
       const auto request = [&]() {
         if (kb == 0) {
-          const TileLoad at = src.load(0, t);
-          slices = at.slices;
-          from[0].at(scales.a, scales.a_pitch, scales.a_shift, at.row0 + 128 * (int)rank, scales.m,
-                     lane);
+          const BlockScales scales = src.scales(t);
+          slices = scales.slices;
+          a_words = scale_words(scales.a, scales.a_pitch, 0);
+          b_words = scale_words(scales.b, scales.b_pitch, 0);
+          from[0].at(scales.a, scales.a_pitch, scales.a_shift, scales.row0 + 128 * (int)rank,
+                     scales.m, lane);
 #pragma unroll
           for (int c = 0; c < CG; ++c)
-            from[1 + c].at(scales.b, scales.b_pitch, scales.b_shift, at.col0 + 128 * c, scales.n,
-                           lane);
+            from[1 + c].at(scales.b, scales.b_pitch, scales.b_shift, scales.col0 + 128 * c,
+                           scales.n, lane);
         }
-        from[0].read(kb, slices, scales.a_words, next[0]);
+        from[0].read(kb, slices, a_words, next[0]);
 #pragma unroll
-        for (int c = 0; c < CG; ++c) from[1 + c].read(kb, slices, scales.b_words, next[1 + c]);
+        for (int c = 0; c < CG; ++c) from[1 + c].read(kb, slices, b_words, next[1 + c]);
         kb += 4;
         if (kb >= slices) {
           kb = 0;
@@ -764,6 +778,8 @@ __device__ __forceinline__ void run_products(const Source& src) {
         }
       }
     }
+  } else if (warp == S::kWriters + 3) {
+    if constexpr (KIND == kOperandF8) src.spare(lane);
   } else if (warp < S::kWriters) {
     // ---- results: this warp's 32 rows, its part of the tile's 32-column pieces
     constexpr int kPieces = S::kTileCols / (8 * S::kWriters);

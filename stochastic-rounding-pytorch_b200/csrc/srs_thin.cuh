@@ -16,8 +16,14 @@
 // touches B.
 //
 // Roles, barriers and bounded waits as in the large product (one tile per CTA).
+//
+// GROUPED: the rows of B are in groups, each with a matrix A of its own.  A CTA's tile is 128
+// rows of one group's A by up to BN of its rows; which, it finds from the ends (all its warps
+// do, so that nothing waits for a barrier).  Grids are sized by a bound: the CTAs left over write
+// zeros for the rows of no group, as the others do behind their tile, and leave.
 #pragma once
 
+#include "srs_groups.cuh"
 #include "srs_product.cuh"
 
 namespace srs {
@@ -44,6 +50,10 @@ struct ThinArgs {
   int out_format;
   int64_t row_stride, col_stride;  // of D, elements
   unsigned int* status;
+  // GROUPED: m is the rows of one group's A, n those of all of B
+  const int32_t* ends;
+  int groups;
+  int64_t scale_a_group;  // bytes of scales from one group's A to the next
 };
 
 template <int BN>
@@ -82,7 +92,21 @@ __device__ __forceinline__ void store_value(void* out, int format, int64_t at, f
   else static_cast<__half*>(out)[at] = __float2half_rn(v);
 }
 
-template <int BN>
+// Zeros in the rows of D (B's rows) that belong to no group, by all threads of the grid.
+__device__ __forceinline__ void zero_ungrouped(const ThinArgs& a) {
+  // the last end as the groups' own reading of them has it
+  int carry = 0;
+  for (int base = 0; base < a.groups; base += 32) {
+    int start, end;
+    group_span(a.ends, a.groups, a.n, base, (int)(threadIdx.x & 31), &carry, &start, &end);
+  }
+  const int64_t last = (int64_t)a.n * a.m;
+  for (int64_t i = (int64_t)carry * a.m + (int64_t)blockIdx.x * kThinThreads + threadIdx.x;
+       i < last; i += (int64_t)gridDim.x * kThinThreads)
+    store_value(a.out, a.out_format, i, 0.0f);
+}
+
+template <int BN, bool GROUPED>
 __global__ void __launch_bounds__(kThinThreads, 2)
 thin_product_kernel(const __grid_constant__ ThinArgs a) {
   using S = ThinShape<BN>;
@@ -94,7 +118,26 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const uint32_t rank = cluster_rank();
-  const int row0 = (int)(blockIdx.x / splits) * a.rows;
+  int row0 = (int)(blockIdx.x / splits) * a.rows;
+  // first row of A in its map, first row of B and of D's columns, and how many of them
+  int map_row = row0, b_row0 = 0, n = a.n;
+  const uint8_t* scale_a = a.scale_a;
+  if constexpr (GROUPED) {
+    const int row_tiles = (a.m + a.rows - 1) / a.rows, t = (int)(blockIdx.x / splits);
+    const GroupTile tile =
+        find_group_tile(a.ends, a.groups, a.n, BN, t / row_tiles, lane);
+    row0 = t % row_tiles * a.rows;
+    map_row = tile.group * a.m + row0;
+    b_row0 = tile.row0;
+    n = tile.group < 0 ? 0 : min(BN, tile.end - tile.row0);
+    scale_a += (int64_t)tile.group * a.scale_a_group;
+    if (tile.group < 0) {
+      // the same for all CTAs of the cluster; no later kernel before the one ahead is done
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      zero_ungrouped(a);
+      return;
+    }
+  }
   const int first = (int)((int64_t)a.slices * rank / splits);
   const int last = (int)((int64_t)a.slices * (rank + 1) / splits);
   const uint32_t scales0 = (smem_address(raw) + 1023u) & ~1023u;
@@ -130,7 +173,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       for (int i = 0; i < ahead; ++i) {
         barrier_expect(full(i), load_bytes);
-        load_box<1>(stage0 + i * stage_bytes, &a.map_a, (first + i) * kSliceBytes, row0, 0,
+        load_box<1>(stage0 + i * stage_bytes, &a.map_a, (first + i) * kSliceBytes, map_row, 0,
                     full(i));
       }
     }
@@ -157,9 +200,9 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       if (leader) {
         if (!sent) {
           barrier_expect(full(s), load_bytes);
-          load_box<1>(pa, &a.map_a, i * kSliceBytes, row0, 0, full(s));
+          load_box<1>(pa, &a.map_a, i * kSliceBytes, map_row, 0, full(s));
         }
-        load_box<1>(pa + panel_bytes, &a.map_b, i * kSliceBytes, 0, 0, full(s));
+        load_box<1>(pa + panel_bytes, &a.map_b, i * kSliceBytes, b_row0, 0, full(s));
       }
       __syncwarp();
       if (++s == stages) {
@@ -230,11 +273,11 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     // ---- block scales: the writing warps and two more take a group each in turn, as a
     // group's loads take microseconds behind the weights' in DRAM (one warp, a group
     // after the other, held a product of 58.7 MB at 18.6 us)
-    const bool words_a = scale_words(a.scale_a, a.scale_a_pitch, first);
+    const bool words_a = scale_words(scale_a, a.scale_a_pitch, first);
     const bool words_b = scale_words(a.scale_b, a.scale_b_pitch, first);
     ScaleRows from_a, from_b;
-    from_a.at(a.scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
-    from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, 0, a.n, lane);
+    from_a.at(scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
+    from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, b_row0, a.n, lane);
     const int groups = (last - first + 3) >> 2;
     bool waited = false;
     for (int g = warp < 4 ? warp : warp - 2; g < groups; g += kThinLoaders) {
@@ -284,13 +327,14 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     if (warp < 4 && ok) {
 #pragma unroll
       for (int c0 = 0; c0 < BN; c0 += 16) {
-        if (c0 >= a.n) break;
+        if (c0 >= n) break;
         uint32_t v[16];
         tmem_load16(acc + c0, v);
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          if (row < row_end && c0 + c < a.n)
-            store_value(a.out, a.out_format, row * a.row_stride + (c0 + c) * a.col_stride,
+          if (row < row_end && c0 + c < n)
+            store_value(a.out, a.out_format,
+                        row * a.row_stride + (b_row0 + c0 + c) * a.col_stride,
                         __uint_as_float(v[c]));
       }
     }
@@ -299,7 +343,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     if (warp < 4) {
 #pragma unroll
       for (int c0 = 0; c0 < BN; c0 += 16) {
-        if (c0 >= a.n) break;
+        if (c0 >= n) break;
         uint32_t v[16];
         tmem_load16(acc + c0, v);
 #pragma unroll
@@ -314,7 +358,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     // columns rank, rank + splits, ...: half of the CTA's threads a column
     const int half = threadIdx.x >> 7, at = threadIdx.x & 127;
     const int out_row = row0 + at;
-    for (int c = (int)rank + half * (int)splits; c < a.n; c += 2 * (int)splits) {
+    for (int c = (int)rank + half * (int)splits; c < n; c += 2 * (int)splits) {
       float part[8];
 #pragma unroll
       for (uint32_t r = 0; r < 8; ++r) {
@@ -330,7 +374,8 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       for (int r = 1; r < 8; ++r)
         if (r < (int)splits) sum = __fadd_rn(sum, part[r]);
       if (out_row < row_end && ok)
-        store_value(a.out, a.out_format, out_row * a.row_stride + c * a.col_stride, sum);
+        store_value(a.out, a.out_format,
+                    out_row * a.row_stride + (b_row0 + c) * a.col_stride, sum);
     }
     cluster_sync();  // the others have read this CTA's sums
   }
@@ -338,6 +383,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   __syncthreads();
   tmem_fence_after();
   if (warp == 5) tmem_free<1>(tmem, S::kColumns);
+  if constexpr (GROUPED) zero_ungrouped(a);
 }
 
 }  // namespace srs

@@ -18,11 +18,14 @@ from .blocks import (  # noqa: E402 (after the registry its rounding rules come 
     block_linear,
     matmul_blocks,
     quantize_blocks,
+    quantize_stack,
 )
+from .cuda.groups import RowGroups, group_rows
 from .cuda.muon import orthogonalize
+from .experts import BlockExperts, expert_linear
 
 # A star import gives the reference's names; the package's own additions (Muon,
-# orthogonalize, FP8 blocks) are attributes of the package beside them.
+# orthogonalize, FP8 blocks, rows in groups) are attributes of the package beside them.
 __all__ = [
     "AdamWReferenceRN",
     "AdamWReferenceSR",

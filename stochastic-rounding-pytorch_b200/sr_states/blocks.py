@@ -14,9 +14,10 @@ import torch
 
 from ._hash import update_key
 from .cuda.blocks import (BLOCK, BlockTensor, check_blocks, linear_blocks, matmul_blocks,
-                          quantize_blocks)
+                          quantize_blocks, quantize_stack)
 
-__all__ = ["BlockLinear", "BlockTensor", "block_linear", "matmul_blocks", "quantize_blocks"]
+__all__ = ["BlockLinear", "BlockTensor", "block_linear", "matmul_blocks", "quantize_blocks",
+           "quantize_stack"]
 
 
 def _matrix(x):
@@ -90,27 +91,19 @@ def _rank():
     return 0
 
 
-class BlockLinear(torch.nn.Module):
-    """A linear layer without bias on ``block_linear``.
-
-    The gradient's rounding draws anew on every call that a gradient will follow:
-    (seed, number of such calls, rank of the process).  ``seed=None`` gives a layer the
-    number of layers that the process made before it, so that layers draw apart.  The
-    ``state_dict`` carries the seed and the calls: a run that goes on from a checkpoint
-    rounds as the run that wrote it would have.
-    """
+class BlockLayer(torch.nn.Module):
+    """The weight of a layer on FP8 block products, and the draws of its gradient's rounding."""
 
     _made = itertools.count()
 
-    def __init__(self, in_features, out_features, *, grad_dtype=torch.float8_e4m3fn,
-                 grad_rounding="stochastic", seed=None, device=None, dtype=torch.bfloat16):
+    def __init__(self, *shape, grad_dtype=torch.float8_e4m3fn, grad_rounding="stochastic",
+                 seed=None, device=None, dtype=torch.bfloat16):
         super().__init__()
-        self.in_features, self.out_features = in_features, out_features
+        self.out_features, self.in_features = shape[-2:]
         self.grad_dtype, self.grad_rounding = grad_dtype, grad_rounding
         self.seed, self.calls = int(next(self._made) if seed is None else seed), 0
-        self.weight = torch.nn.Parameter(torch.empty((out_features, in_features), device=device,
-                                                     dtype=dtype))
-        torch.nn.init.normal_(self.weight, std=in_features ** -0.5)
+        self.weight = torch.nn.Parameter(torch.empty(shape, device=device, dtype=dtype))
+        torch.nn.init.normal_(self.weight, std=self.in_features ** -0.5)
 
     def get_extra_state(self):
         return torch.tensor([self.seed, self.calls], dtype=torch.int64)
@@ -131,9 +124,28 @@ class BlockLinear(torch.nn.Module):
         """The weight in FP8 blocks, to keep for inference."""
         return quantize_blocks(self.weight, block=(BLOCK, BLOCK))
 
-    def forward(self, x):
+    def _settings(self, x):
+        """The gradient's settings for one call on ``x``."""
         if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad):
             self.calls += 1
-        return block_linear(x, self.weight, grad_dtype=self.grad_dtype,
-                            grad_rounding=self.grad_rounding,
-                            seed=update_key(self.seed, self.calls, _rank()))
+        return {"grad_dtype": self.grad_dtype, "grad_rounding": self.grad_rounding,
+                "seed": update_key(self.seed, self.calls, _rank())}
+
+
+class BlockLinear(BlockLayer):
+    """A linear layer without bias on ``block_linear``.
+
+    The gradient's rounding draws anew on every call that a gradient will follow:
+    (seed, number of such calls, rank of the process).  ``seed=None`` gives a layer the
+    number of layers that the process made before it, so that layers draw apart.  The
+    ``state_dict`` carries the seed and the calls: a run that goes on from a checkpoint
+    rounds as the run that wrote it would have.
+    """
+
+    def __init__(self, in_features, out_features, *, grad_dtype=torch.float8_e4m3fn,
+                 grad_rounding="stochastic", seed=None, device=None, dtype=torch.bfloat16):
+        super().__init__(out_features, in_features, grad_dtype=grad_dtype,
+                         grad_rounding=grad_rounding, seed=seed, device=device, dtype=dtype)
+
+    def forward(self, x):
+        return block_linear(x, self.weight, **self._settings(x))

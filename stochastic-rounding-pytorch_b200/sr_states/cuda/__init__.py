@@ -2,8 +2,9 @@
 
 from ._native import load_library
 from .adamw import AdamWCuda, cuda_adamw_step_
-from .blocks import BlockTensor, matmul_blocks, quantize_blocks
+from .blocks import BlockTensor, matmul_blocks, quantize_blocks, quantize_stack
 from .cast import cast, rn_cast_bf16, sr_cast_bf16
+from .groups import RowGroups, group_rows
 from .muon import check_products, cuda_muon_step_, orthogonalize
 from .sgd import SGDMCuda, cuda_sgdm_step_
 
@@ -22,6 +23,7 @@ def is_available() -> bool:
     return torch.cuda.get_device_capability() == (10, 0)
 
 
-__all__ = ["AdamWCuda", "BlockTensor", "SGDMCuda", "cast", "check_products", "cuda_adamw_step_",
-           "cuda_muon_step_", "cuda_sgdm_step_", "is_available", "matmul_blocks",
-           "orthogonalize", "quantize_blocks", "rn_cast_bf16", "sr_cast_bf16"]
+__all__ = ["AdamWCuda", "BlockTensor", "RowGroups", "SGDMCuda", "cast", "check_products",
+           "cuda_adamw_step_", "cuda_muon_step_", "cuda_sgdm_step_", "group_rows",
+           "is_available", "matmul_blocks",
+           "orthogonalize", "quantize_blocks", "quantize_stack", "rn_cast_bf16", "sr_cast_bf16"]

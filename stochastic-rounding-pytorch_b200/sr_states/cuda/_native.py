@@ -17,6 +17,7 @@ import numpy as np
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "_native" / "libsrs_b200.so"
 HOST_PATH = LIBRARY_PATH.parent / "_srs_host.so"
 BLOCKS_PATH = LIBRARY_PATH.parent / "_srs_blocks.so"
+GROUPS_PATH = LIBRARY_PATH.parent / "_srs_groups.so"
 
 SRS_OK = 0
 SRS_ERR_INVALID_ARGUMENT = -1
@@ -176,6 +177,22 @@ _SIGNATURES = {
                           ctypes.c_int),
     "srs_copy_rows": ([_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
                        _P], ctypes.c_int),
+    "srs_quantize_stack": ([_P, ctypes.c_int, *[ctypes.c_int64] * 5, ctypes.c_int, ctypes.c_int,
+                            ctypes.c_int, ctypes.c_uint32, ctypes.c_uint32, _P, _P, _P],
+                           ctypes.c_int),
+    "srs_group_rows": ([_P, ctypes.c_int, ctypes.c_int64, ctypes.c_int, _P, _P, _P],
+                       ctypes.c_int),
+    "srs_group_columns": ([ctypes.c_int64, ctypes.c_int], ctypes.c_int64),
+    "srs_group_scales": ([ctypes.c_int64, ctypes.c_int], ctypes.c_int64),
+    "srs_quantize_groups": ([_P, ctypes.c_int, *[ctypes.c_int64] * 3, _P, ctypes.c_int,
+                             ctypes.c_int, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint32, _P,
+                             _P, _P], ctypes.c_int),
+    "srs_expert_matmul": ([_P, _P, ctypes.c_int, _P, ctypes.c_int64, _P, ctypes.c_int, _P],
+                          ctypes.c_int),
+    "srs_expert_linear": ([_P, ctypes.c_int, *[ctypes.c_int64] * 3, ctypes.c_int, _P,
+                           ctypes.c_int, _P, _P, _P, ctypes.c_int64, _P], ctypes.c_int),
+    "srs_expert_gradient": ([_P, _P, ctypes.c_int64, ctypes.c_int, _P, _P, ctypes.c_int, _P],
+                            ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "srs_product_status_word": ([ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32))], ctypes.c_int),
 }
@@ -208,6 +225,7 @@ def load_library() -> ctypes.CDLL:
 
 _host = None
 _blocks = None
+_groups = None
 
 
 def _load_module(name: str, path: Path):
@@ -243,6 +261,18 @@ def blocks_module():
             lib.srs_linear_blocks, lib.srs_linear_workspace)))
         _blocks = module
     return _blocks
+
+
+def groups_module():
+    """The _srs_groups tensor front end, bound to the library's entry points."""
+    global _groups
+    if _groups is None:
+        lib = load_library()
+        module = _load_module("_srs_groups", GROUPS_PATH)
+        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                     for name in _SIGNATURES})
+        _groups = module
+    return _groups
 
 
 def _check(rc: int) -> None:
@@ -388,6 +418,33 @@ class NativeLauncher:
 
     def block_linear(self, x, w, w_scale, fmt):
         got = blocks_module().linear(x, w, w_scale, fmt)
+        return got if type(got) is not int else _check(got)
+
+    def quantize_stack(self, x, fmt, rule, square, seed, offset, orientation):
+        """As quantize_blocks, of every matrix of a stack."""
+        got = groups_module().quantize_stack(x, fmt, rule, square, seed, offset, orientation)
+        return got if type(got) is tuple else _check(got)
+
+    def group_rows(self, index, groups):
+        got = groups_module().group_rows(index, groups)
+        return got if type(got) is tuple else _check(got)
+
+    def quantize_groups(self, x, ends, fmt, rule, seed, rows):
+        """(data, scale) of the transposed copy for expert_gradient, with ``rows`` behind those
+        of the copy by rows."""
+        got = groups_module().quantize_groups(x, ends, fmt, rule, seed, rows)
+        return got if type(got) is tuple else _check(got)
+
+    def expert_matmul(self, a, a_scale, w, w_scale, ends, fmt):
+        got = groups_module().expert_matmul(a, a_scale, w, w_scale, ends, fmt)
+        return got if type(got) is not int else _check(got)
+
+    def expert_linear(self, x, w, w_scale, ends, fmt):
+        got = groups_module().expert_linear(x, w, w_scale, ends, fmt)
+        return got if type(got) is not int else _check(got)
+
+    def expert_gradient(self, a_t, a_scale, b_t, b_scale, rows, ends, fmt):
+        got = groups_module().expert_gradient(a_t, a_scale, b_t, b_scale, rows, ends, fmt)
         return got if type(got) is not int else _check(got)
 
     def product_status(self) -> int:

@@ -21,17 +21,18 @@ class BlockTensor(NamedTuple):
 
     ``data``: E4M3 or E5M2, rows x columns; ``scale``: float8_e8m0fnu (powers of
     two), one a 1 x 128 block (rows x ceil(columns / 128)) or one a 128 x 128 block
-    (ceil(rows / 128) x ceil(columns / 128))."""
+    (ceil(rows / 128) x ceil(columns / 128)).  A stack of matrices has one dimension more
+    in front in both."""
 
     data: torch.Tensor
     scale: torch.Tensor
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """The values the blocks stand for."""
-        rows, cols = self.data.shape
-        factor = self.scale.float().repeat_interleave(BLOCK, 1)[:, :cols]
-        if self.scale.shape[0] != rows:
-            factor = factor.repeat_interleave(BLOCK, 0)[:rows]
+        rows, cols = self.data.shape[-2:]
+        factor = self.scale.float().repeat_interleave(BLOCK, -1)[..., :cols]
+        if self.scale.shape[-2] != rows:
+            factor = factor.repeat_interleave(BLOCK, -2)[..., :rows, :]
         return (self.data.float() * factor).to(dtype)
 
 
@@ -58,15 +59,29 @@ def quantize_blocks(x, *, dtype=torch.float8_e4m3fn, rounding="nearest", seed=0,
 
     ``x``: FP32, BF16 or FP16 on an sm_100a GPU, two dimensions, at most 4194240 rows.
     """
+    launcher = _native.launcher()
+    return _quantize(launcher, launcher.quantize_blocks, x, dtype, rounding, seed, offset, block,
+                     orientation)
+
+
+def quantize_stack(x, *, dtype=torch.float8_e4m3fn, rounding="nearest", seed=0, offset=0,
+                   block=(1, BLOCK), orientation="rows"):
+    """``quantize_blocks`` of every matrix of a stack (three dimensions, at most 65535
+    matrices), each with blocks of its own; flat indices go on from one to the next."""
+    launcher = _native.launcher()
+    return _quantize(launcher, launcher.quantize_stack, x, dtype, rounding, seed, offset, block,
+                     orientation)
+
+
+def _quantize(launcher, quantize, x, dtype, rounding, seed, offset, block, orientation):
     fmt, rule = check_blocks(dtype, rounding)
     if tuple(block) not in ((1, BLOCK), (BLOCK, BLOCK)):
         raise ValueError(f"block must be (1, {BLOCK}) or ({BLOCK}, {BLOCK})")
     if orientation not in ORIENTATIONS:
         raise ValueError(f"orientation must be one of {tuple(ORIENTATIONS)}")
-    launcher = _native.launcher()
     launcher.check_device(x.device, "quantize_blocks")
-    got = launcher.quantize_blocks(x, fmt, rule, int(block[0] == BLOCK), int(seed) & _MASK32,
-                                   int(offset) & _MASK32, ORIENTATIONS[orientation])
+    got = quantize(x, fmt, rule, int(block[0] == BLOCK), int(seed) & _MASK32,
+                   int(offset) & _MASK32, ORIENTATIONS[orientation])
     if orientation == "both":
         return BlockTensor(got[0], got[1]), BlockTensor(got[2], got[3])
     return BlockTensor(*got)
