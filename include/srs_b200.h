@@ -465,6 +465,45 @@ int srs_expert_linear(const void* x, int x_format, int64_t rows, int64_t k, int6
 int srs_expert_gradient(const srs_blocks* a_t, const srs_blocks* b_t, int64_t rows, int experts,
                         const int32_t* ends, void* d, int d_format, void* stream);
 
+/* ---- low-rank adapters beside a projection in FP8 blocks -----------------------
+ * No counterpart in the reference.  Token t has adapter a, the group that order and ends
+ * (srs_group_rows) give it, or none.  16-bit matrices `down` (count x rank x in) and `up`
+ * (count x out x rank); addresses, row pitches and strides are multiples of 16 bytes; a row's
+ * elements follow one another.  scale: FP32, one an adapter (0: none), times `factor`.
+ *
+ * srs_adapter_linear: with x (tokens x k, in the adapters' format) quantised in 1 x 128 blocks of
+ * block_format by `rule` and `seed`,
+ *   turned == 0:  low_t = s_a down_a x_t;    d_t = w x_t + up_a low_t        (k = in, w->rows = out)
+ *   turned == 1:  low_t = s_a up_a^T x_t;    d_t = w x_t + down_a^T low_t    (k = out, w->rows = in)
+ * Sums of both parts in FP32, d (tokens x w->rows, in the adapters' format) rounded once.  low:
+ * FP32, tokens (in the order of `order`) x rank, or NULL; rows of tokens without an adapter are
+ * not written.  largest: encodings of max |low| an adapter, or NULL.  d == NULL: `low` alone.
+ * An FP16 |low| above 65504 does not fit the second product.
+ *
+ * srs_adapter_gradient: out_a = sum over its tokens of low_t z_t^T (rank x cols) or, turned, z_t
+ * low_t^T (cols x rank), in z's format; zeros without tokens.  `largest` as given above (FP16).
+ *
+ * `workspace`: 256-byte aligned, not used by any other call that can overlap in time. */
+#define SRS_ADAPTER_MAX_RANK 256
+typedef struct srs_adapters {
+  uint64_t down, up, scale, order, ends; /* device addresses */
+  int64_t down_pitch, down_stride, up_pitch, up_stride; /* elements */
+  float factor;
+  int32_t count, rank, format;
+} srs_adapters;
+
+int64_t srs_adapter_workspace(int64_t tokens, int64_t k, int64_t n, int adapters, int rank);
+int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int64_t x_pitch,
+                       int block_format, int rule, uint32_t seed, const srs_blocks* w,
+                       const srs_adapters* a, int turned, void* d, float* low, uint32_t* largest,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters, int rank);
+int srs_adapter_gradient(const void* z, int format, int64_t tokens, int64_t cols, int64_t z_pitch,
+                         const float* low, const uint32_t* largest, int adapters, int rank,
+                         const int32_t* order, const int32_t* ends, int turned, void* out,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Rows of `cols` bytes at src_pitch copied to rows at dst_pitch (zeros behind them up to
  * dst_pitch): for operands whose rows do not start on 16-byte boundaries.  dst and
  * dst_pitch must be multiples of 16 bytes. */

@@ -15,6 +15,10 @@ decltype(&srs_expert_matmul) g_expert_matmul = nullptr;
 decltype(&srs_expert_linear) g_expert_linear = nullptr;
 decltype(&srs_expert_gradient) g_expert_gradient = nullptr;
 decltype(&srs_linear_workspace) g_linear_workspace = nullptr;
+decltype(&srs_adapter_workspace) g_adapter_workspace = nullptr;
+decltype(&srs_adapter_linear) g_adapter_linear = nullptr;
+decltype(&srs_adapter_gradient_workspace) g_gradient_workspace = nullptr;
+decltype(&srs_adapter_gradient) g_adapter_gradient = nullptr;
 
 void* stream_of(const at::Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
@@ -147,6 +151,10 @@ PyObject* py_bind(PyObject*, PyObject* args) {
       !bind_one(t, "srs_expert_linear", &g_expert_linear) ||
       !bind_one(t, "srs_expert_gradient", &g_expert_gradient) ||
       !bind_one(t, "srs_linear_workspace", &g_linear_workspace) ||
+      !bind_one(t, "srs_adapter_workspace", &g_adapter_workspace) ||
+      !bind_one(t, "srs_adapter_linear", &g_adapter_linear) ||
+      !bind_one(t, "srs_adapter_gradient_workspace", &g_gradient_workspace) ||
+      !bind_one(t, "srs_adapter_gradient", &g_adapter_gradient) ||
       !bind_one(t, "srs_copy_rows", &g_copy_rows))
     return nullptr;
   Py_RETURN_NONE;
@@ -347,6 +355,197 @@ PyObject* py_expert_gradient(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+// A 16-bit matrix, or a stack of them, whose rows start on 16-byte boundaries; one laid out
+// otherwise is copied once.  `whole`: rows of whole 16 bytes as well.
+at::Tensor aligned(const at::Tensor& t, bool whole) {
+  const int64_t last = t.dim() - 1, cols = t.size(last);
+  bool good = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+              (cols <= 1 || t.stride(last) == 1) && (!whole || cols % 8 == 0);
+  for (int64_t d = 0; d < last; ++d)
+    good = good && (t.size(d) <= 1 || (t.stride(d) % 8 == 0 && (d != last - 1 || t.stride(d) >= cols)));
+  if (good || t.numel() == 0) return t;
+  std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
+  sizes[last] = ceil_div(cols, 8) * 8;
+  at::Tensor copy = at::empty(sizes, t.options()).narrow(last, 0, cols);
+  copy.copy_(t);
+  return copy;
+}
+
+// Elements from one index of dimension `d` to the next; of one index alone, `otherwise`.
+int64_t step_of(const at::Tensor& t, int64_t d, int64_t otherwise) {
+  return t.size(d) > 1 ? t.stride(d) : otherwise;
+}
+
+struct Adapters {
+  at::Tensor down, up, scale, order, ends;
+  srs_adapters c{};
+};
+
+void set_adapters(Adapters* a, const at::Tensor& x, int64_t in, int64_t out, PyObject* down,
+                  PyObject* up, PyObject* scale, double factor, PyObject* order, PyObject* ends) {
+  const char* what = "adapter_linear";
+  a->down = tensor(down, "down");
+  a->up = tensor(up, "up");
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what,
+                   " takes BF16 or FP16, got ", x.scalar_type());
+  TORCH_CHECK_TYPE(
+      a->down.scalar_type() == x.scalar_type() && a->up.scalar_type() == x.scalar_type(), what,
+      ": adapters in x's dtype ", x.scalar_type(), " needed, got ", a->down.scalar_type(), " and ",
+      a->up.scalar_type());
+  TORCH_CHECK_VALUE(a->down.device() == x.device() && a->up.device() == x.device(),
+                    "all tensors must be on the same CUDA device");
+  TORCH_CHECK_VALUE(a->down.dim() == 3 && a->up.dim() == 3 && a->down.size(0) == a->up.size(0) &&
+                        a->down.size(1) == a->up.size(2) && a->down.size(2) == in &&
+                        a->up.size(1) == out,
+                    what, ": down of shape ", a->down.sizes(), " and up of shape ", a->up.sizes(),
+                    " do not fit a projection from ", in, " to ", out);
+  const int64_t count = a->down.size(0), rank = a->down.size(1);
+  TORCH_CHECK_VALUE(rank > 0 && rank <= SRS_ADAPTER_MAX_RANK, what, ": the rank must be in [1, ",
+                    SRS_ADAPTER_MAX_RANK, "], got ", rank);
+  a->ends = checked_ends(tensor(ends, "ends"), x, what);
+  TORCH_CHECK_VALUE(a->ends.numel() == count, what, ": ends of ", a->ends.numel(),
+                    " groups do not fit ", count, " adapters");
+  const at::Tensor& places = tensor(order, "order");
+  TORCH_CHECK_TYPE(places.scalar_type() == at::kInt || places.scalar_type() == at::kLong, what,
+                   ": the order is int32 or int64, got ", places.scalar_type());
+  TORCH_CHECK_VALUE(places.device() == x.device() && places.dim() == 1 &&
+                        places.numel() == x.size(0),
+                    what, ": order of shape ", places.sizes(), " does not fit ", x.size(0),
+                    " tokens on ", x.device());
+  a->order = places.to(at::kInt).contiguous();
+  if (scale != Py_None) {
+    a->scale = tensor(scale, "scale");
+    TORCH_CHECK_TYPE(a->scale.scalar_type() == at::kFloat, what, ": scales are FP32, got ",
+                     a->scale.scalar_type());
+    TORCH_CHECK_VALUE(a->scale.device() == x.device() && a->scale.dim() == 1 &&
+                          a->scale.numel() == count,
+                      what, ": scales of shape ", a->scale.sizes(), " do not fit ", count,
+                      " adapters on ", x.device());
+    a->scale = a->scale.contiguous();
+    a->c.scale = reinterpret_cast<uint64_t>(a->scale.data_ptr());
+  }
+  a->down = aligned(a->down, false);
+  a->up = aligned(a->up, true);
+  srs_adapters& c = a->c;
+  c.down = reinterpret_cast<uint64_t>(a->down.data_ptr());
+  c.up = reinterpret_cast<uint64_t>(a->up.data_ptr());
+  c.order = reinterpret_cast<uint64_t>(a->order.data_ptr());
+  c.ends = reinterpret_cast<uint64_t>(a->ends.data_ptr());
+  c.down_pitch = step_of(a->down, 1, ceil_div(in, 8) * 8);
+  c.down_stride = step_of(a->down, 0, 0);
+  c.up_pitch = step_of(a->up, 1, ceil_div(rank, 8) * 8);
+  c.up_stride = step_of(a->up, 0, 0);
+  c.factor = (float)factor;
+  c.count = (int32_t)count;
+  c.rank = (int32_t)rank;
+  c.format = x.scalar_type() == at::kBFloat16 ? SRS_FMT_BF16 : SRS_FMT_F16;
+}
+
+// x (tokens, k), blocks of the projection (None: the low part alone) -> (d or None, low,
+// largest).  turned: x is the output's gradient.
+PyObject* py_adapter_linear(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *x_obj, *w_obj, *w_scale, *down, *up, *scale, *order, *ends;
+  int format, rule, turned, keep;
+  unsigned int seed;
+  double factor;
+  if (!PyArg_ParseTuple(args, "OiiIOOOOOdOOii", &x_obj, &format, &rule, &seed, &w_obj, &w_scale,
+                        &down, &up, &scale, &factor, &order, &ends, &turned, &keep))
+    return nullptr;
+  c10::NoGradGuard no_grad;
+  const at::Tensor& given = tensor(x_obj, "x");
+  const c10::cuda::OptionalCUDAGuard guard(given.device());
+  const int64_t tokens = given.size(0), k = given.size(1);
+  Blocks blocks;
+  const bool project = w_obj != Py_None;
+  const int64_t n = tensor(turned ? down : up, "adapters").size(turned ? 2 : 1);
+  if (project) {
+    blocks = {tensor(w_obj, "the weight's data"), tensor(w_scale, "the weight's scale")};
+    TORCH_CHECK_VALUE(given.device() == blocks.data.device(),
+                      "all tensors must be on the same CUDA device");
+    TORCH_CHECK_VALUE(blocks.data.dim() == 2 && blocks.data.size(1) == k &&
+                          blocks.data.size(0) == n,
+                      "adapter_linear: a weight of shape ", blocks.data.sizes(),
+                      " does not fit a projection from ", k, " to ", n);
+  }
+  Adapters a;
+  set_adapters(&a, given, turned ? n : k, turned ? k : n, down, up, scale, factor, order, ends);
+  const at::Tensor x = aligned(given, false);
+  srs_blocks matrix{};
+  int rc = project ? operand("weight", &blocks, &matrix) : SRS_OK;
+  at::Tensor out, low, largest;
+  if (rc == SRS_OK) {
+    if (project) out = at::empty({tokens, n}, x.options());
+    if (keep) {
+      low = at::empty({tokens, a.c.rank}, x.options().dtype(at::kFloat));
+      // (the sums of FP16 gradients are scaled by it)
+      if (a.c.format == SRS_FMT_F16)
+        largest = at::empty({a.c.count}, x.options().dtype(at::kInt));
+    }
+    const int64_t bytes =
+        g_adapter_workspace(tokens, k, project ? n : 0, a.c.count, a.c.rank);
+    const at::Tensor space = at::empty({bytes}, x.options().dtype(at::kByte));
+    if (tokens != 0)
+      rc = g_adapter_linear(
+          x.data_ptr(), tokens, k, step_of(x, 0, ceil_div(k, 8) * 8), format, rule, seed,
+          project ? &matrix : nullptr, &a.c, turned, project ? out.data_ptr() : nullptr,
+          keep ? static_cast<float*>(low.data_ptr()) : nullptr,
+          largest.defined() ? static_cast<uint32_t*>(largest.data_ptr()) : nullptr,
+          space.data_ptr(), bytes, stream_of(x));
+  }
+  if (rc != SRS_OK) return PyLong_FromLong(rc);
+  PyObject* result = PyTuple_New(3);
+  if (result == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor* t : {&out, &low, &largest}) {
+    if (t->defined()) {
+      PyTuple_SET_ITEM(result, i++, THPVariable_Wrap(*t));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(result, i++, Py_None);
+    }
+  }
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// Sums over the tokens of each adapter of z (tokens, cols) by low: (count, rank, cols) or,
+// turned, (count, cols, rank).
+PyObject* py_adapter_gradient(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *z_obj, *low_obj, *largest_obj, *order_obj, *ends_obj;
+  int turned;
+  if (!PyArg_ParseTuple(args, "OOOOOi", &z_obj, &low_obj, &largest_obj, &order_obj, &ends_obj,
+                        &turned))
+    return nullptr;
+  c10::NoGradGuard no_grad;
+  const at::Tensor& given = tensor(z_obj, "z");
+  const c10::cuda::OptionalCUDAGuard guard(given.device());
+  const at::Tensor &low = tensor(low_obj, "low");
+  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), given, "adapter_linear");
+  const at::Tensor order = tensor(order_obj, "order").to(at::kInt).contiguous();
+  const at::Tensor z = aligned(given, false);
+  const int64_t tokens = z.size(0), cols = z.size(1), rank = low.size(1), count = ends.numel();
+  at::Tensor out = turned ? at::empty({count, cols, rank}, z.options())
+                          : at::empty({count, rank, cols}, z.options());
+  const int64_t bytes = g_gradient_workspace(tokens, cols, (int)count, (int)rank);
+  const at::Tensor space = at::empty({bytes}, z.options().dtype(at::kByte));
+  int rc = SRS_OK;
+  if (out.numel() != 0)
+    rc = g_adapter_gradient(
+        z.data_ptr(), z.scalar_type() == at::kBFloat16 ? SRS_FMT_BF16 : SRS_FMT_F16, tokens, cols,
+        step_of(z, 0, ceil_div(cols, 8) * 8), static_cast<const float*>(low.data_ptr()),
+        largest_obj != Py_None
+            ? static_cast<const uint32_t*>(tensor(largest_obj, "largest").data_ptr())
+            : nullptr,
+        (int)count, (int)rank, static_cast<const int32_t*>(order.data_ptr()),
+        static_cast<const int32_t*>(ends.data_ptr()), turned, out.data_ptr(), space.data_ptr(),
+        bytes, stream_of(z));
+  if (rc != SRS_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"bind", py_bind, METH_VARARGS, "bind({name: address}): the library's entry points."},
     {"group_rows", py_group_rows, METH_VARARGS, "group_rows(index, groups) -> order, ends."},
@@ -360,6 +559,11 @@ PyMethodDef kMethods[] = {
      "expert_linear(x, w, w_scale, ends, format) -> tensor."},
     {"expert_gradient", py_expert_gradient, METH_VARARGS,
      "expert_gradient(a_t, a_scale, b_t, b_scale, rows, ends, format) -> tensor."},
+    {"adapter_linear", py_adapter_linear, METH_VARARGS,
+     "adapter_linear(x, format, rule, seed, w, w_scale, down, up, scale, factor, order, ends, "
+     "turned, keep) -> (d, low, largest)."},
+    {"adapter_gradient", py_adapter_gradient, METH_VARARGS,
+     "adapter_gradient(z, low, largest, order, ends, turned) -> tensor."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_srs_groups",

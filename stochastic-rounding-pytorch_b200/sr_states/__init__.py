@@ -20,6 +20,7 @@ from .blocks import (  # noqa: E402 (after the registry its rounding rules come 
     quantize_blocks,
     quantize_stack,
 )
+from .adapters import adapter_linear
 from .cuda.groups import RowGroups, group_rows
 from .cuda.muon import orthogonalize
 from .experts import BlockExperts, expert_linear

@@ -193,6 +193,16 @@ _SIGNATURES = {
                            ctypes.c_int, _P, _P, _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_expert_gradient": ([_P, _P, ctypes.c_int64, ctypes.c_int, _P, _P, ctypes.c_int, _P],
                             ctypes.c_int),
+    "srs_adapter_workspace": ([*[ctypes.c_int64] * 3, ctypes.c_int, ctypes.c_int],
+                              ctypes.c_int64),
+    "srs_adapter_linear": ([_P, *[ctypes.c_int64] * 3, ctypes.c_int, ctypes.c_int,
+                            ctypes.c_uint32, _P, _P, ctypes.c_int, _P, _P, _P, _P,
+                            ctypes.c_int64, _P], ctypes.c_int),
+    "srs_adapter_gradient_workspace": ([*[ctypes.c_int64] * 2, ctypes.c_int, ctypes.c_int],
+                                       ctypes.c_int64),
+    "srs_adapter_gradient": ([_P, ctypes.c_int, *[ctypes.c_int64] * 3, _P, _P, ctypes.c_int,
+                              ctypes.c_int, _P, _P, ctypes.c_int, _P, _P, ctypes.c_int64, _P],
+                             ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "srs_product_status_word": ([ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32))], ctypes.c_int),
 }
@@ -445,6 +455,17 @@ class NativeLauncher:
 
     def expert_gradient(self, a_t, a_scale, b_t, b_scale, rows, ends, fmt):
         got = groups_module().expert_gradient(a_t, a_scale, b_t, b_scale, rows, ends, fmt)
+        return got if type(got) is not int else _check(got)
+
+    def adapter_linear(self, x, fmt, rule, seed, w, w_scale, down, up, scale, factor, order, ends,
+                       turned, keep):
+        """(result, low part, its largest values); with ``w`` None the low part alone."""
+        got = groups_module().adapter_linear(x, fmt, rule, seed, w, w_scale, down, up, scale,
+                                             factor, order, ends, turned, keep)
+        return got if type(got) is tuple else _check(got)
+
+    def adapter_gradient(self, z, low, largest, order, ends, turned):
+        got = groups_module().adapter_gradient(z, low, largest, order, ends, turned)
         return got if type(got) is not int else _check(got)
 
     def product_status(self) -> int:

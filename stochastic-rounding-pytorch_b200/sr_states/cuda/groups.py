@@ -67,3 +67,34 @@ def expert_gradient(a_t, b_t, rows, ends, *, dtype):
     launcher = _native.launcher()
     launcher.check_device(a_t.data.device, "expert_linear")
     return launcher.expert_gradient(*a_t, *b_t, rows, ends, _FORMATS[dtype])
+
+
+class Low(NamedTuple):
+    """The low part of an ``adapter_product`` (FP32, tokens in their groups' order), and what the
+    sums over it need."""
+
+    values: torch.Tensor
+    largest: torch.Tensor | None
+
+
+def adapter_product(x, weight, down, up, groups, *, scale, dtype, rounding="nearest", seed=0,
+                    turned=False, keep=False):
+    """(``x @ weight.T`` in FP8 blocks plus the adapters' part, Low); ``turned``: x is the
+    gradient of the result.  ``weight`` None: the low part alone."""
+    fmt, rule = check_blocks(dtype, rounding)
+    launcher = _native.launcher()
+    launcher.check_device(x.device, "adapter_linear")
+    scale, factor = (scale, 1.0) if isinstance(scale, torch.Tensor) else (None, float(scale))
+    w, w_scale = (None, None) if weight is None else weight
+    out, low, largest = launcher.adapter_linear(
+        x, fmt, rule, int(seed) & _MASK32, w, w_scale, down, up, scale, factor, groups.order,
+        groups.ends, int(turned), int(keep))
+    return out, Low(low, largest)
+
+
+def adapter_gradient(z, low, groups, *, turned=False):
+    """Sums over each adapter's tokens of low by z (rank x columns), or turned."""
+    launcher = _native.launcher()
+    launcher.check_device(z.device, "adapter_linear")
+    return launcher.adapter_gradient(z, low.values, low.largest, groups.order, groups.ends,
+                                     int(turned))
