@@ -58,7 +58,8 @@ UNITS = [("srs_abi", "srs_abi.cu", []), ("srs_cast", "srs_cast.cu", []),
          ("srs_sgdm", "srs_sgdm.cu", []), ("srs_product", "srs_product.cu", []),
          ("srs_newton", "srs_newton.cu", []), ("srs_blocks", "srs_blocks.cu", []),
          ("srs_groups", "srs_groups.cu", []), ("srs_experts", "srs_experts.cu", []),
-         ("srs_adapters", "srs_adapters.cu", [])]
+         ("srs_adapters", "srs_adapters.cu", []),
+         ("srs_adapter_product", "srs_adapter_product.cu", [])]
 UNITS += [(f"srs_adamw_m{m}", "srs_adamw.cu", [f"-DSRS_M_FORMAT={m}"]) for m in range(5)]
 
 

@@ -109,7 +109,9 @@ struct LowArgs {
   const int32_t* ends;
   const float* scale;  // null: `factor` alone
   float factor;
-  float* low;             // tokens (in order) x rank
+  float* low;             // tokens (in order) x rank (null: not wanted)
+  uint16_t* pairs;        // items for a large product (null: not wanted)
+  int edge, pitch, rest_at;
   unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
 };
 
@@ -230,17 +232,47 @@ __global__ void __launch_bounds__(32 * kLowWarps, 2) low_kernel(const LowArgs a)
   const float factor = a.factor * (a.scale != nullptr ? __ldg(a.scale + tile.group) : 1.0f);
   float most = 0.0f;
   // token t of the tile by CTA t % splits
+  const int whole = (ranks + 15) & ~15;
   for (int i = threadIdx.x; i < kLowTokens / (int)splits * kLowRank; i += 32 * kLowWarps) {
     const int t = i / kLowRank * (int)splits + (int)split, r = i % kLowRank;
-    if (t >= count || r >= ranks) continue;
+    if (t >= count || r >= whole) continue;
     float v = 0.0f;
-    for (uint32_t p = 0; p < splits; ++p) {
-      const float* const theirs = splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums;
-      v += theirs[t * kPitch + r];
+    if (r < ranks) {
+      for (uint32_t p = 0; p < splits; ++p) {
+        const float* const theirs = splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums;
+        v += theirs[t * kPitch + r];
+      }
+      v *= factor;
+      if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + rank0 + r] = v;
+      most = fmaxf(most, isfinite(v) ? fabsf(v) : 0.0f);
     }
-    v *= factor;
-    a.low[(int64_t)(tile.row0 + t) * a.rank + rank0 + r] = v;
-    most = fmaxf(most, isfinite(v) ? fabsf(v) : 0.0f);
+    if (a.pairs != nullptr) {
+      const int place = tile.row0 + t;
+      uint16_t* const to = a.pairs + ((int64_t)(place / a.edge + tile.rank) * a.edge +
+                                      place % a.edge) * a.pitch + rank0 + r;
+      const uint32_t high = encode16<F>(v);
+      const float left = v - decode16<F>(high);
+      to[0] = (uint16_t)high;
+      to[a.rest_at] = (uint16_t)encode16<F>(isfinite(left) ? left : 0.0f);
+    }
+  }
+  if (a.pairs != nullptr) {
+    // zeros in the rows of the adapter's first and last item that are not its own
+    const int words = whole / 2;
+    const auto clear = [&](int item, int from, int to) {
+      const int rows = to - from;
+      for (int i = threadIdx.x + 32 * kLowWarps * (int)split; i < rows * words;
+           i += 32 * kLowWarps * (int)splits) {
+        uint16_t* const p = a.pairs + ((int64_t)item * a.edge + from + i / words) * a.pitch +
+                            rank0 + 2 * (i % words);
+        *reinterpret_cast<uint32_t*>(p) = 0u;
+        *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
+      }
+    };
+    if (tile.row0 == tile.start) clear(tile.start / a.edge + tile.rank, 0, tile.start % a.edge);
+    const int last = tile.end - 1;
+    if (last - tile.row0 < kLowTokens)
+      clear(last / a.edge + tile.rank, last % a.edge + 1, a.edge);
   }
   if (a.largest != nullptr) {
     const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
@@ -598,10 +630,35 @@ int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, 
 
 using namespace srs;
 
+// Few tokens: the projection's thin form with an FP32 result and the expansion; else the adapters
+// enter the large product.
+static bool few(int64_t tokens) { return tokens <= kThinRows; }
+
+// Parts of a call's workspace, each on a 256-byte boundary.
+struct AdapterSpace {
+  int64_t rows, low, base, total;  // rows: quantised tokens; low: FP32 or pairs; base: FP32
+};
+
+static AdapterSpace adapter_space(int64_t tokens, int64_t k, int64_t n, int adapters, int rank) {
+  AdapterSpace s{};
+  int64_t at = whole(srs_linear_workspace(tokens, k));
+  s.low = at;
+  if (few(tokens)) {
+    at += whole(tokens * rank * 4);
+    s.base = at;
+    at += whole(tokens * n * 4);
+  } else if (n > 0) {
+    const int64_t edge = adapter_edge(tokens, n, k);
+    at += whole(pair_items(tokens, adapters, edge) * edge * pair_shape(rank).pitch * 2);
+  }
+  s.total = at;
+  return s;
+}
+
 extern "C" int64_t srs_adapter_workspace(int64_t tokens, int64_t k, int64_t n, int adapters,
                                          int rank) {
   if (tokens <= 0 || k < 0 || n < 0 || adapters < 1 || rank < 1) return 0;
-  return whole(srs_linear_workspace(tokens, k)) + whole(tokens * rank * 4) + whole(tokens * n * 4);
+  return adapter_space(tokens, k, n, adapters, rank).total;
 }
 
 extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int64_t x_pitch,
@@ -610,32 +667,36 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
                                   uint32_t* largest, void* workspace, int64_t workspace_bytes,
                                   void* stream) {
   clear_error();
-  const int64_t n = w == nullptr ? 0 : w->rows;
+  const int64_t n = w == nullptr || d == nullptr ? 0 : w->rows;
   if (d != nullptr)
     if (int rc = check_operand("w", w, k)) return rc;
-  if (int rc = check_adapters(a, tokens, k, d != nullptr ? n : 0, turned != 0)) return rc;
-  if (tokens == 0 || (d != nullptr && n == 0 && low == nullptr)) return SRS_OK;
+  if (int rc = check_adapters(a, tokens, k, n, turned != 0)) return rc;
+  if (tokens == 0 || (n == 0 && low == nullptr)) return SRS_OK;
   if (k > 0 && (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0 || x_pitch % 8 != 0 ||
                 x_pitch < k))
     return fail(SRS_ERR_INVALID_ARGUMENT, "x needs a 16-byte aligned address and row pitch");
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-      workspace_bytes < srs_adapter_workspace(tokens, k, n, a->count, a->rank))
+  if (n > 0 && reinterpret_cast<uintptr_t>(d) % 2 != 0)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "misaligned result pointer");
+  const AdapterSpace space = adapter_space(tokens, k, n, a->count, a->rank);
+  if (workspace_bytes < space.total ||
+      (space.total > 0 &&
+       (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)))
     return fail(SRS_ERR_INVALID_ARGUMENT,
                 "workspace of %lld bytes, %lld needed at a 256-byte aligned address",
-                (long long)workspace_bytes,
-                (long long)srs_adapter_workspace(tokens, k, n, a->count, a->rank));
+                (long long)workspace_bytes, (long long)space.total);
   if (int rc = check_device()) return rc;
   if (int rc = check_products()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  char* const space = static_cast<char*>(workspace);
-  float* const own_low = reinterpret_cast<float*>(space + whole(srs_linear_workspace(tokens, k)));
-  float* const base = own_low + whole(tokens * a->rank * 4) / 4;
-  const bool bf16 = a->format == SRS_FMT_BF16;
+  char* const at = static_cast<char*>(workspace);
+  const bool bf16 = a->format == SRS_FMT_BF16, thin = few(tokens);
 
-  if (largest != nullptr) {
-    const cudaError_t e = cudaMemsetAsync(largest, 0, (size_t)a->count * 4, st);
-    if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
-  }
+  cudaError_t e = cudaSuccess;
+  if (largest != nullptr) e = cudaMemsetAsync(largest, 0, (size_t)a->count * 4, st);
+  // without a sum there is neither a projection nor a low part
+  if (e == cudaSuccess && n > 0 && k == 0) e = cudaMemsetAsync(d, 0, (size_t)(tokens * n * 2), st);
+  if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
+  const int edge = thin || n == 0 ? 0 : adapter_edge(tokens, n, k);
+  const PairShape pairs = pair_shape(a->rank);
   LowArgs l{};
   l.x = static_cast<const char*>(x);
   l.w = reinterpret_cast<const char*>(turned ? a->up : a->down);
@@ -650,14 +711,20 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.ends = reinterpret_cast<const int32_t*>(a->ends);
   l.scale = reinterpret_cast<const float*>(a->scale);
   l.factor = a->factor;
-  l.low = low != nullptr ? low : own_low;
+  l.low = low != nullptr ? low : thin ? reinterpret_cast<float*>(at + space.low) : nullptr;
   l.largest = largest;
+  if (edge != 0) {
+    l.pairs = reinterpret_cast<uint16_t*>(at + space.low);
+    l.edge = edge;
+    l.pitch = pairs.pitch;
+    l.rest_at = pairs.rest_at;
+  }
   if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, st)
                               : launch_low<SRS_FMT_F16, false>(l, st))
                       : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, st)
                               : launch_low<SRS_FMT_F16, true>(l, st)))
     return rc;
-  if (d == nullptr || n == 0) return SRS_OK;
+  if (n == 0 || k == 0) return SRS_OK;
 
   srs_blocks rows{};
   rows.data = reinterpret_cast<uint64_t>(workspace);
@@ -666,29 +733,37 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   rows.scale = rows.data + (uint64_t)(tokens * rows.pitch);
   rows.scale_pitch = ceil_div(k, 128);
   rows.format = block_format;
-  if (k > 0) {
-    QuantizeCall q{x, a->format, tokens, k, x_pitch, block_format, rule, false, seed, 0u};
-    q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
-    if (int rc = quantize(q, st)) return rc;
+  QuantizeCall q{x, a->format, tokens, k, x_pitch, block_format, rule, false, seed, 0u};
+  q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
+  q.order = thin ? nullptr : l.order;
+  if (int rc = quantize(q, st)) return rc;
+  const void* const up = reinterpret_cast<const void*>(turned ? a->down : a->up);
+  const int64_t up_pitch = turned ? a->down_pitch : a->up_pitch;
+  const int64_t up_stride = turned ? a->down_stride : a->up_stride;
+  if (!thin) {
+    const AdapterCall call{l.pairs,  up,       up_pitch,  up_stride, turned != 0,
+                           a->count, a->rank,  a->format, l.order,   l.ends};
+    return launch_adapter_product(rows, *w, k, call, edge, d, st);
   }
+  float* const base = reinterpret_cast<float*>(at + space.base);
   if (int rc = srs_matmul_blocks(&rows, w, k, base, SRS_FMT_F32, stream)) return rc;
-  ExpandArgs e{};
-  e.base = base;
-  e.u = reinterpret_cast<const char*>(turned ? a->down : a->up);
-  e.u_pitch = turned ? a->down_pitch : a->up_pitch;
-  e.u_stride = turned ? a->down_stride : a->up_stride;
-  e.low = l.low;
-  e.tokens = (int)tokens;
-  e.n = (int)n;
-  e.rank = a->rank;
-  e.adapters = a->count;
-  e.order = l.order;
-  e.ends = l.ends;
-  e.out = d;
-  return turned ? (bf16 ? launch_expand<SRS_FMT_BF16, false>(e, st)
-                        : launch_expand<SRS_FMT_F16, false>(e, st))
-                : (bf16 ? launch_expand<SRS_FMT_BF16, true>(e, st)
-                        : launch_expand<SRS_FMT_F16, true>(e, st));
+  ExpandArgs x_args{};
+  x_args.base = base;
+  x_args.u = static_cast<const char*>(up);
+  x_args.u_pitch = up_pitch;
+  x_args.u_stride = up_stride;
+  x_args.low = l.low;
+  x_args.tokens = (int)tokens;
+  x_args.n = (int)n;
+  x_args.rank = a->rank;
+  x_args.adapters = a->count;
+  x_args.order = l.order;
+  x_args.ends = l.ends;
+  x_args.out = d;
+  return turned ? (bf16 ? launch_expand<SRS_FMT_BF16, false>(x_args, st)
+                        : launch_expand<SRS_FMT_F16, false>(x_args, st))
+                : (bf16 ? launch_expand<SRS_FMT_BF16, true>(x_args, st)
+                        : launch_expand<SRS_FMT_F16, true>(x_args, st));
 }
 
 extern "C" int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters,

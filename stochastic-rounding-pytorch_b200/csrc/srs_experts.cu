@@ -112,6 +112,7 @@ __device__ __forceinline__ void spread_zeros(char* out, int64_t count, int size,
 }
 
 struct RowSource {
+  static constexpr bool kExtras = false;
   const ExpertProduct& w;
   const GroupPlan& p;
   struct At {
@@ -184,6 +185,7 @@ struct RowSource {
 };
 
 struct SumSource {
+  static constexpr bool kExtras = false;
   const ExpertProduct& w;
   const GroupPlan& p;
   struct At {

@@ -50,14 +50,16 @@ __device__ __forceinline__ void group_span(const int32_t* __restrict__ ends, int
 struct GroupTile {
   int group;      // -1: there is no such tile
   int row0, end;  // first row of the tile, end of its group
+  int start;      // first row of its group
+  int rank;       // groups with rows before it
   int quads;      // 4 * (words of 4 tiles that groups before it take) + tiles before it in its own
 };
 
 // Tile `index` of all groups' tiles in order, found by a warp (the same in all lanes).
 __device__ __forceinline__ GroupTile find_group_tile(const int32_t* __restrict__ ends, int groups,
                                                      int rows, int edge, int index, int lane) {
-  GroupTile r{-1, 0, 0, 0};
-  int carry = 0, tiles_before = 0, quads_before = 0;
+  GroupTile r{-1, 0, 0, 0, 0, 0};
+  int carry = 0, tiles_before = 0, quads_before = 0, rank = 0;
   for (int base = 0; base < groups; base += 32) {
     int start, end;
     group_span(ends, groups, rows, base, lane, &carry, &start, &end);
@@ -65,16 +67,20 @@ __device__ __forceinline__ GroupTile find_group_tile(const int32_t* __restrict__
     const int upto = tiles_before + warp_scan_sum(tiles, lane);
     const int quads_upto = quads_before + warp_scan_sum(quads, lane);
     const unsigned found = __ballot_sync(0xFFFFFFFFu, upto > index);
+    const unsigned some = __ballot_sync(0xFFFFFFFFu, tiles > 0);
     if (found != 0u) {
       const int at = __ffs(found) - 1, inside = index - (upto - tiles);
       r.group = base + at;
       r.row0 = __shfl_sync(0xFFFFFFFFu, start + inside * edge, at);
       r.end = __shfl_sync(0xFFFFFFFFu, end, at);
+      r.start = __shfl_sync(0xFFFFFFFFu, start, at);
+      r.rank = rank + __popc(some & ((1u << at) - 1u));
       r.quads = __shfl_sync(0xFFFFFFFFu, quads_upto - quads + inside, at);
       return r;
     }
     tiles_before = __shfl_sync(0xFFFFFFFFu, upto, 31);
     quads_before = __shfl_sync(0xFFFFFFFFu, quads_upto, 31);
+    rank += __popc(some);
   }
   return r;
 }

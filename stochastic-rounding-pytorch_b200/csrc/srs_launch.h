@@ -77,4 +77,37 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
 int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
                        int64_t k, void* d, int d_format, bool overlap, cudaStream_t stream);
 
+// Low-rank adapters in a large product (srs_adapter_product.cu).  The low part of tokens in their
+// adapters' order enters as pairs of 16-bit numbers, high and what it leaves, in items of
+// `edge` rows: an item is a tile of the product and one adapter that has tokens in it, other rows
+// zero.  Item of tile i and the r-th adapter with tokens: i + r (each step along the tokens
+// raises one of the two, so no two items share a number).  A row has the rank's high parts, in
+// whole 16s, and the others behind them in one slice of 64 for ranks up to 32; else whole
+// slices of 64 of high parts and then as many of the others.
+struct PairShape {
+  int pitch, rest_at;  // elements of a row, first of the second parts
+  int slices;
+};
+inline PairShape pair_shape(int rank) {
+  if (rank <= 32) return {64, (rank + 15) / 16 * 16, 1};
+  const int wide = (rank + 63) / 64 * 64;
+  return {2 * wide, wide, wide / 32};
+}
+inline int64_t pair_items(int64_t tokens, int64_t adapters, int64_t edge) {
+  return (tokens + edge - 1) / edge + (adapters < tokens ? adapters : tokens);
+}
+
+struct AdapterCall {
+  const void* pairs;
+  const void* up;  // rows x rank a matrix, or (rows_inner) rank x rows; `pitch`, `stride` elements
+  int64_t pitch, stride;
+  bool rows_inner;
+  int count, rank, format;
+  const int32_t* order;
+  const int32_t* ends;
+};
+int adapter_edge(int64_t tokens, int64_t n, int64_t k);  // of the tiles: 128 or 256
+int launch_adapter_product(const srs_blocks& rows, const srs_blocks& w, int64_t k,
+                           const AdapterCall& a, int edge, void* d, cudaStream_t stream);
+
 }  // namespace srs

@@ -189,6 +189,7 @@ struct BlockProduct {
 };
 
 struct BlockSource {
+  static constexpr bool kExtras = false;
   const BlockProduct& w;
   __device__ int phases() const { return 1; }
   __device__ uint32_t tiles(int) const { return w.grid.rows * w.grid.cols; }

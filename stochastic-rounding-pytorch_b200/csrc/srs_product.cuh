@@ -61,6 +61,18 @@ struct TileLoad {
   int k0;  // FP8: the first element of k of both operands
 };
 
+// FP8: a product of 16-bit operands added to a tile's sum, 64 of its k at a time (a Source with
+// kExtras gives them): the tile's rows of A from row_a on, its columns' rows of B.
+struct ExtraLoad {
+  const CUtensorMap* map_a;
+  const CUtensorMap* map_b;
+  int row_a, k_a;         // of the slice, in A's map
+  int k_b, batch_b;       // in B's
+  bool b_rows_inner;
+  int steps;              // of 16 of k, A from its column 0 on
+  int again;              // != 0: as many steps more, A from this step of 16 on, B from the start
+};
+
 // What happens to a tile's accumulator.
 struct TileStore {
   int row0, col0;  // in the matrix
@@ -77,6 +89,7 @@ struct TileStore {
   int format;      // SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t pitch;   // elements
   float step, decay;  // update: p' = fma(step, D, p * decay)
+  const int32_t* order;  // row i of D is stored as row order[i] (kScatter)
 };
 
 // Scales of one operand for a warp: rows row0 + lane + 32 j (j < 4), blocks kb ..
@@ -239,6 +252,37 @@ __device__ __forceinline__ uint32_t staged_read(uint32_t addr) {
 
 // Staged piece to rows of elements of SLOTS / 2 bytes: `out` is the piece's first
 // element, `pitch` and `cols` count elements, `rows` <= 32.
+//
+// Scattered (16-bit results): row i of the piece goes to the row that lane i holds in `to`,
+// counted from `out`.
+__device__ __forceinline__ void scatter_piece(uint32_t base, char* out, int64_t pitch, int rows,
+                                              int cols, int lane, int to) {
+  const int64_t step = pitch * 2;
+  const uint64_t align = reinterpret_cast<uint64_t>(out) | (uint64_t)step;
+  const int bytes = min(cols * 2, 64);
+  if ((align & 15) == 0 && (bytes & 15) == 0) {
+    const int slot = lane & 3, row0 = lane >> 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + row0;
+      const int64_t at = __shfl_sync(0xFFFFFFFFu, to, row);
+      const uint4 v = staged_read4(staged_slot<4>(base, row, slot));
+      if (row < rows && 16 * slot < bytes)
+        *reinterpret_cast<uint4*>(out + at * step + 16 * slot) = v;
+    }
+  } else {
+    // by elements
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row) {
+      char* const p = out + (int64_t)__shfl_sync(0xFFFFFFFFu, to, row) * step;
+      const uint32_t v =
+          staged_read(staged_slot<4>(base, row, lane >> 3) + 4 * ((lane >> 1) & 3));
+      if (2 * lane < bytes)
+        *reinterpret_cast<uint16_t*>(p + 2 * lane) = (uint16_t)(v >> (16 * (lane & 1)));
+    }
+  }
+}
+
 template <int SLOTS>
 __device__ __forceinline__ void store_piece(uint32_t base, char* out, int64_t pitch, int rows,
                                             int cols, int lane) {
@@ -385,10 +429,10 @@ __device__ __forceinline__ void add_piece(const uint4 (&add)[4], float beta, uin
 // 32 accumulator columns from col0 on for a warp's 32 rows from row0 on: v[c] is
 // column col0 + c of row row0 + lane.  `add` holds the addend's piece; the next piece's
 // (next_col, -1: none) is requested before this one is stored.
-template <bool NEWTON, bool SPLIT>
+template <bool NEWTON, bool SPLIT, bool SCATTER>
 __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int col0, int lane,
                                               uint32_t staged, uint32_t (&v)[32],
-                                              uint4 (&add)[4], int next_col) {
+                                              uint4 (&add)[4], int next_col, int to) {
   const int row = row0 + lane, rows = min(32, t.m - row0);
   const int64_t at = (int64_t)row0 * t.pitch + col0;
 #pragma unroll
@@ -428,7 +472,10 @@ __device__ __forceinline__ void write_columns(const TileStore& t, int row0, int 
     }
     stage_row<4, 0, 2>(staged, lane, v);
     __syncwarp();
-    store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
+    if (SCATTER)
+      scatter_piece(staged, t.out + 2 * (int64_t)col0, t.pitch, rows, t.n - col0, lane, to);
+    else
+      store_piece<4>(staged, t.out + 2 * at, t.pitch, rows, t.n - col0, lane);
     if (low)
       store_piece<4>(staged + kPieceBytes / 2, t.out + t.low + 2 * at, t.pitch, rows, t.n - col0,
                      lane);
@@ -480,13 +527,18 @@ struct ProductShape {
   static constexpr uint32_t kInstruction = (uint32_t)(kTileCols >> 3) << 17 |
                                            (uint32_t)(kTileRows >> 4) << 24 |
                                            (KIND == kOperandF8 ? 1u << 23 : 1u << 4);
+  // of the 16-bit products added to an FP8 one
+  static constexpr uint32_t kExtraInstruction = (uint32_t)(kTileCols >> 3) << 17 |
+                                                (uint32_t)(kTileRows >> 4) << 24 | 1u << 4;
 };
 
 // The CTA's work.  Source gives: phases(), tiles(phase), load(phase, tile),
 // store(phase, tile), formats() (bits of the instruction descriptor), counter(phase),
 // status() and longest() (slices of a tile, where they can take seconds); for FP8 also
 // scales(tile): the operands' block scales, and spare(lane): work of the warp that has
-// no role (results that are zero without a product).
+// no role (results that are zero without a product).  kExtras: 16-bit products are added to a
+// tile's sum (extras(tile) of them, extra(tile, i), formats in extra_formats()), and rows
+// are stored in another order.
 template <int KIND, int CG, bool NEWTON, bool SPLIT, class Source>
 __device__ __forceinline__ void run_products(const Source& src) {
   using S = ProductShape<KIND, CG>;
@@ -596,6 +648,31 @@ __device__ __forceinline__ void run_products(const Source& src) {
             parity ^= 1u;
           }
         }
+        if constexpr (Source::kExtras) {
+          const int extras = src.extras(t);
+          for (int i = 0; i < extras && ok; ++i) {
+            const ExtraLoad e = src.extra(t, i);
+            ok = barrier_wait(empty(s), parity ^ 1u, status, 1u);
+            if (!ok) break;
+            const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
+            const uint32_t pa = stage0 + s * S::kStageBytes, pb = pa + kPanelBytes;
+            if (leader) {
+              if (rank == 0) barrier_expect(full(s), CG * S::kStageBytes);
+              load_box<CG>(pa, e.map_a, e.k_a, e.row_a + 128 * (int)rank, 0, bar);
+              if (e.b_rows_inner) {
+                load_box<CG>(pb, e.map_b, rb, e.k_b, e.batch_b, bar);
+                load_box<CG>(pb + kPanelBytes / 2, e.map_b, rb + 64, e.k_b, e.batch_b, bar);
+              } else {
+                load_box<CG>(pb, e.map_b, e.k_b, rb, e.batch_b, bar);
+              }
+            }
+            __syncwarp();
+            if (++s == kStages) {
+              s = 0;
+              parity ^= 1u;
+            }
+          }
+        }
       }
     }
     // Every stage given back (its commit has reached this CTA) before leaving.
@@ -700,6 +777,41 @@ __device__ __forceinline__ void run_products(const Source& src) {
           if (++s == kStages) {
             s = 0;
             parity ^= 1u;
+          }
+        }
+        if constexpr (Source::kExtras) {
+          const int extras = src.extras(t);
+          // MMAs of another kind add to this accumulator only behind the last of these: nothing
+          // says that the two kinds keep their order.
+          if (extras > 0 && ok) ok = barrier_wait(empty(done_stage), done_parity, status, 8u);
+          for (int i = 0; i < extras && ok; ++i) {
+            const ExtraLoad e = src.extra(t, i);
+            ok = barrier_wait(full(s), parity, status, 16u);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t pa = stage0 + s * S::kStageBytes;
+            const uint64_t da = operand_descriptor(false) | uint64_t((pa >> 4) & 0x3FFFu);
+            const uint64_t db = operand_descriptor(e.b_rows_inner) |
+                                uint64_t(((pa + kPanelBytes) >> 4) & 0x3FFFu);
+            const uint32_t step_b = (e.b_rows_inner ? 2048u : 32u) >> 4;
+            const uint32_t idesc =
+                S::kExtraInstruction | src.extra_formats() | (e.b_rows_inner ? 1u << 16 : 0u);
+            if (leader) {
+              for (int j = 0; j < e.steps; ++j)
+                mma_f16<CG>(d, da + 2 * j, db + j * step_b, idesc, 1u);
+              if (e.again != 0) {
+                for (int j = 0; j < e.steps; ++j)
+                  mma_f16<CG>(d, da + 2 * (e.again + j), db + j * step_b, idesc, 1u);
+              }
+              mma_commit<CG>(empty(s));
+            }
+            __syncwarp();
+            done_stage = s;  // (the scales' columns: their readers are done then, too)
+            done_parity = parity;
+            if (++s == kStages) {
+              s = 0;
+              parity ^= 1u;
+            }
           }
         }
         if (ok && leader) mma_commit<CG>(acc_full(acc));
@@ -808,6 +920,9 @@ __device__ __forceinline__ void run_products(const Source& src) {
           }
           load_addend(at, row0, at.col0 + 32 * part * kPieces, lane, add);
         }
+        int to = 0;
+        if (Source::kExtras && row0 + lane < at.m)
+          to = min(max(__ldg(at.order + row0 + lane), 0), at.m - 1);
         float late = 1.0f;
         if (NEWTON && at.late != nullptr) late = __ldg(at.late);
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u, patience);
@@ -832,8 +947,9 @@ __device__ __forceinline__ void run_products(const Source& src) {
             if (lane == 0) barrier_arrive_relaxed(map_to_rank(acc_empty(acc), 0));
           }
           if (row0 < at.m && at.col0 + 32 * c < at.n)
-            write_columns<NEWTON, SPLIT>(at, row0, at.col0 + 32 * c, lane, staged, v, add,
-                                  i + 1 < kPieces ? at.col0 + 32 * (c + 1) : -1);
+            write_columns<NEWTON, SPLIT, Source::kExtras>(
+                at, row0, at.col0 + 32 * c, lane, staged, v, add,
+                i + 1 < kPieces ? at.col0 + 32 * (c + 1) : -1, to);
         }
       }
       if (NEWTON && p + 1 < phases && ok) {
