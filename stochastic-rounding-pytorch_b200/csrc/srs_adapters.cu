@@ -31,9 +31,15 @@ __device__ __forceinline__ int64_t token_at(const int32_t* order, int place, int
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+// Rows of SLOTS (2 or 4) 16-byte slots, turned as rows of 8 are.
+template <int SLOTS>
+__device__ __forceinline__ uint32_t narrow_slot(int row, int slot) {
+  return (uint32_t)(row * 16 * SLOTS + ((slot ^ ((row / (8 / SLOTS)) & (SLOTS - 1))) << 4));
+}
+
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
@@ -90,15 +96,29 @@ __device__ __forceinline__ uint32_t encode16(float x) {
 
 // ------------------------------------------------------------------ low part --
 //
-// A CTA takes up to 128 tokens of one adapter (tiles counted from the adapter's first), up to
-// 64 of the rank and a part of the sum; the parts of a cluster's CTAs are added through
+// A CTA takes up to TOKENS tokens of one adapter (tiles counted from the adapter's first), up to
+// 16 RT of the rank and a part of the sum; the parts of a cluster's CTAs are added through
 // distributed shared memory in rank order.  x's bytes, read once, bound it: mma.sync is far
 // faster than they arrive (4096 tokens, 4096 -> 64: 2 GFLOP).  Sums are FP32.
-constexpr int kLowTokens = 128, kLowRank = 64, kLowStep = 64, kLowStages = 4;
-constexpr int kLowWarps = kLowTokens / 16;
-constexpr int kLowX = kLowTokens * kLowStep * 2, kLowW = kLowRank * kLowStep * 2;
-constexpr int kLowSmem = kLowStages * (kLowX + kLowW);
-static_assert(kLowTokens * (kLowRank + 1) * 4 <= kLowSmem, "the sums fit the stages");
+//
+// TOKENS = 128: 8 warps of 16 tokens each.  TOKENS = 16, for calls of few tokens where most
+// adapters have one or two: 4 warps that share a stage's four steps of 16 of k.
+constexpr int kLowStep = 64;  // of k a stage: 128 bytes of a row
+
+template <int TOKENS, int RT>
+struct LowShape {
+  static constexpr int kWarps = TOKENS == 16 ? 4 : TOKENS / 16;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr bool kShared = TOKENS == 16;  // warps share the steps of a stage
+  static constexpr int kRank = 16 * RT;
+  static constexpr int kX = TOKENS * kLowStep * 2, kW = kRank * kLowStep * 2;
+  // bytes on their way: 6 stages for ranks up to 16; two CTAs an SM fit with all of these
+  static constexpr int kStages = TOKENS == 16 ? 8 : RT == 1 ? 6 : RT == 2 ? 5 : 4;
+  static constexpr int kPitch = kRank + 1;
+  static constexpr int kSums = (kShared ? kWarps : 1) * TOKENS * kPitch * 4;
+  static constexpr int kStageBytes = kStages * (kX + kW);
+  static constexpr int kSmem = kStageBytes > kSums ? kStageBytes : kSums;
+};
 
 struct LowArgs {
   const char* x;  // 16-bit, rows of x_pitch elements
@@ -121,30 +141,35 @@ __device__ __forceinline__ uint32_t turned_slot(int row, int slot) {
   return (uint32_t)(row * 128 + ((slot ^ (row & 7)) << 4));
 }
 
-template <int F, bool KINNER>
-__global__ void __launch_bounds__(32 * kLowWarps, 2) low_kernel(const LowArgs a) {
+template <int F, bool KINNER, int TOKENS, int RT>
+__global__ void __launch_bounds__(LowShape<TOKENS, RT>::kThreads, TOKENS == 16 ? 4 : 2)
+low_kernel(const LowArgs a) {
+  using S = LowShape<TOKENS, RT>;
+  // The quantisation behind this kernel reads nothing of it and waits for it at its end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t splits, split;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
-  const GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, kLowTokens,
+  const GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, TOKENS,
                                          (int)(blockIdx.x / splits), lane);
   if (tile.group < 0) return;  // the whole cluster
-  const int count = min(kLowTokens, tile.end - tile.row0);
-  const int rank0 = (int)blockIdx.y * kLowRank, ranks = min(kLowRank, a.rank - rank0);
+  const int count = min(TOKENS, tile.end - tile.row0);
+  const int rank0 = (int)blockIdx.y * S::kRank, ranks = min(S::kRank, a.rank - rank0);
   const int steps = (a.k + kLowStep - 1) / kLowStep;
   const int first = (int)((int64_t)steps * split / splits);
   const int last = (int)((int64_t)steps * (split + 1) / splits);
   const uint32_t base = shared_at(raw);
-  const auto x_at = [&](int s) { return base + (uint32_t)(s * (kLowX + kLowW)); };
+  const auto x_at = [&](int s) { return base + (uint32_t)(s * (S::kX + S::kW)); };
 
-  // this thread's rows of x: threadIdx.x / 8 + 32 i, slot threadIdx.x % 8
+  // this thread's rows of x: threadIdx.x / 8 + kRows i, slot threadIdx.x % 8
+  constexpr int kRows = S::kThreads / 8, kEach = TOKENS / kRows, kOfW = (S::kRank + kRows - 1) / kRows;
   const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
-  const char* from[kLowTokens / 32];
+  const char* from[kEach];
 #pragma unroll
-  for (int i = 0; i < kLowTokens / 32; ++i) {
-    const int r = row + 32 * i;
+  for (int i = 0; i < kEach; ++i) {
+    const int r = row + kRows * i;
     from[i] = a.x + (r < count ? token_at(a.order, tile.row0 + r, a.tokens) : 0) * a.x_pitch * 2;
   }
   const char* const w = a.w + (int64_t)tile.group * a.w_stride * 2;
@@ -152,95 +177,105 @@ __global__ void __launch_bounds__(32 * kLowWarps, 2) low_kernel(const LowArgs a)
     const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
     const uint32_t to = x_at(s);
 #pragma unroll
-    for (int i = 0; i < kLowTokens / 32; ++i) {
-      const int r = row + 32 * i;
-      if (32 * i < count)  // rows that no warp multiplies stay as they are
+    for (int i = 0; i < kEach; ++i) {
+      const int r = row + kRows * i;
+      if (kRows * i < count)  // rows that no warp multiplies stay as they are
         copy16(to + turned_slot(r, slot), bytes > 0 ? from[i] + 2 * k : a.x, r < count ? bytes : 0);
     }
+    if (KINNER) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = row + 32 * i;
-      if (KINNER) {
+      for (int i = 0; i < kOfW; ++i) {
+        const int r = row + kRows * i;
         const bool in = r < ranks && bytes > 0;
-        if (32 * i < ((ranks + 15) & ~15))
-          copy16(to + kLowX + turned_slot(r, slot),
+        if (r < S::kRank)
+          copy16(to + S::kX + turned_slot(r, slot),
                  in ? w + ((int64_t)(rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
-      } else {
-        // rows are k, slots 8 of the rank
-        const int kk = step * kLowStep + r, left = min(max(ranks - 8 * slot, 0) * 2, 16);
+      }
+    } else {
+      // 64 rows of k, 2 RT slots of 8 of the rank each (the others are not read)
+#pragma unroll
+      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += S::kThreads) {
+        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
+        const int left = min(max(ranks - 8 * c, 0) * 2, 16);
         const bool in = kk < a.k && left > 0;
-        copy16(to + kLowX + turned_slot(r, slot),
-               in ? w + ((int64_t)kk * a.w_pitch + rank0 + 8 * slot) * 2 : w, in ? left : 0);
+        copy16(to + S::kX + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)),
+               in ? w + ((int64_t)kk * a.w_pitch + rank0 + 8 * c) * 2 : w, in ? left : 0);
       }
     }
   };
 
-  float sum[kLowRank / 8][4];
+  float sum[2 * RT][4];
 #pragma unroll
-  for (int i = 0; i < kLowRank / 8; ++i) {
+  for (int i = 0; i < 2 * RT; ++i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
   }
-  for (int i = 0; i < kLowStages - 1; ++i) {
+  for (int i = 0; i < S::kStages - 1; ++i) {
     if (first + i < last) load(first + i, i);
     copies_done();
   }
-  const bool busy = 16 * warp < count;
+  const int my_rows = S::kShared ? 0 : 16 * warp;
+  const bool busy = my_rows < count;
+  int s = 0;
   for (int step = first; step < last; ++step) {
-    const int s = (step - first) % kLowStages;
-    copies_wait<kLowStages - 2>();
+    copies_wait<S::kStages - 2>();
     __syncthreads();
-    if (step + kLowStages - 1 < last)
-      load(step + kLowStages - 1, (step - first + kLowStages - 1) % kLowStages);
+    if (step + S::kStages - 1 < last) load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
     copies_done();
+    const uint32_t xs = x_at(s), ws = xs + S::kX;
+    if (++s == S::kStages) s = 0;
     if (!busy) continue;
-    const uint32_t xs = x_at(s), ws = xs + kLowX;
 #pragma unroll
-    for (int kk = 0; kk < kLowStep / 16; ++kk) {
+    for (int q = 0; q < (S::kShared ? 1 : kLowStep / 16); ++q) {
+      const int kk = S::kShared ? warp : q;
       uint32_t m[4];
-      load_matrices<false>(xs + turned_slot(16 * warp + (lane & 15), 2 * kk + (lane >> 4)), m);
+      load_matrices<false>(xs + turned_slot(my_rows + (lane & 15), 2 * kk + (lane >> 4)), m);
 #pragma unroll
-      for (int j = 0; j < kLowRank / 16; ++j) {
-        if (16 * j >= ranks) break;
+      for (int j = 0; j < RT; ++j) {
         uint32_t b[4];
-        if (KINNER)  // ranks 16 j + (0..15) x k 16 kk ..
+        if (KINNER) {  // ranks 16 j + (0..15) x k 16 kk ..
           load_matrices<false>(ws + turned_slot(16 * j + (lane & 7) + ((lane >> 4) << 3),
                                                 2 * kk + ((lane >> 3) & 1)), b);
-        else         // k 16 kk + (0..15) x ranks 16 j ..
-          load_matrices<true>(ws + turned_slot(16 * kk + (lane & 15), 2 * j + (lane >> 4)), b);
+        } else {       // k 16 kk + (0..15) x ranks 16 j ..
+          const int r = 16 * kk + (lane & 15), c = 2 * j + (lane >> 4);
+          load_matrices<true>(ws + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)), b);
+        }
         multiply<F>(sum[2 * j], m, b[0], b[1]);
         multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
       }
     }
   }
-  // sums to shared memory, [token][rank]
+  // sums to shared memory, [token][rank] (of every warp, where they share the steps)
   copies_wait<0>();
   __syncthreads();
   float* const sums = reinterpret_cast<float*>(raw);
-  constexpr int kPitch = kLowRank + 1;
   if (busy) {
+    float* const mine = sums + (S::kShared ? warp * TOKENS * S::kPitch : 0);
 #pragma unroll
-    for (int j = 0; j < kLowRank / 8; ++j) {
+    for (int j = 0; j < 2 * RT; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        sums[(16 * warp + (lane >> 2) + 8 * (i >> 1)) * kPitch + 8 * j + 2 * (lane & 3) + (i & 1)] =
+        mine[(my_rows + (lane >> 2) + 8 * (i >> 1)) * S::kPitch + 8 * j + 2 * (lane & 3) + (i & 1)] =
             sum[j][i];
     }
   }
+  const float factor = a.factor * (a.scale != nullptr ? __ldg(a.scale + tile.group) : 1.0f);
   if (splits > 1) cg::this_cluster().sync();
   else __syncthreads();
-  const float factor = a.factor * (a.scale != nullptr ? __ldg(a.scale + tile.group) : 1.0f);
   float most = 0.0f;
   // token t of the tile by CTA t % splits
   const int whole = (ranks + 15) & ~15;
-  for (int i = threadIdx.x; i < kLowTokens / (int)splits * kLowRank; i += 32 * kLowWarps) {
-    const int t = i / kLowRank * (int)splits + (int)split, r = i % kLowRank;
+  for (int i = threadIdx.x; i < (TOKENS + (int)splits - 1) / (int)splits * S::kRank;
+       i += S::kThreads) {
+    const int t = i / S::kRank * (int)splits + (int)split, r = i % S::kRank;
     if (t >= count || r >= whole) continue;
     float v = 0.0f;
     if (r < ranks) {
       for (uint32_t p = 0; p < splits; ++p) {
-        const float* const theirs = splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums;
-        v += theirs[t * kPitch + r];
+        const float* const theirs =
+            (splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums) + t * S::kPitch + r;
+#pragma unroll
+        for (int q = 0; q < (S::kShared ? S::kWarps : 1); ++q) v += theirs[q * TOKENS * S::kPitch];
       }
       v *= factor;
       if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + rank0 + r] = v;
@@ -259,20 +294,20 @@ __global__ void __launch_bounds__(32 * kLowWarps, 2) low_kernel(const LowArgs a)
   if (a.pairs != nullptr) {
     // zeros in the rows of the adapter's first and last item that are not its own
     const int words = whole / 2;
-    const auto clear = [&](int item, int from, int to) {
-      const int rows = to - from;
-      for (int i = threadIdx.x + 32 * kLowWarps * (int)split; i < rows * words;
-           i += 32 * kLowWarps * (int)splits) {
-        uint16_t* const p = a.pairs + ((int64_t)item * a.edge + from + i / words) * a.pitch +
+    const auto clear = [&](int item, int from_row, int to_row) {
+      const int rows = to_row - from_row;
+      for (int i = threadIdx.x + S::kThreads * (int)split; i < rows * words;
+           i += S::kThreads * (int)splits) {
+        uint16_t* const p = a.pairs + ((int64_t)item * a.edge + from_row + i / words) * a.pitch +
                             rank0 + 2 * (i % words);
         *reinterpret_cast<uint32_t*>(p) = 0u;
         *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
       }
     };
     if (tile.row0 == tile.start) clear(tile.start / a.edge + tile.rank, 0, tile.start % a.edge);
-    const int last = tile.end - 1;
-    if (last - tile.row0 < kLowTokens)
-      clear(last / a.edge + tile.rank, last % a.edge + 1, a.edge);
+    const int final_row = tile.end - 1;
+    if (final_row - tile.row0 < TOKENS)
+      clear(final_row / a.edge + tile.rank, final_row % a.edge + 1, a.edge);
   }
   if (a.largest != nullptr) {
     const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
@@ -283,9 +318,11 @@ __global__ void __launch_bounds__(32 * kLowWarps, 2) low_kernel(const LowArgs a)
 
 // -------------------------------------------------------------- few tokens --
 //
-// d_t = base_t + U_a low_t with the base in FP32: a CTA takes 256 columns of up to 64 tokens of
-// one adapter, a thread a column, whose row of U it keeps in registers 8 of the rank at a time.
-// U's bytes bound it.  The last tiles of the grid hold the tokens of no adapter.
+// d_t = base_t + U_a low_t with the base in FP32: a CTA takes some columns of up to 64 tokens of
+// one adapter, a thread a column at a time, whose row of U it reads once for eight tokens.  U's
+// bytes bound it (rank 16, 14336 columns, 40 adapters: 18 MB).  The kernel starts beside the one that
+// writes the base: what it can, it reads before it waits for that one.  The last tiles of the grid
+// hold the tokens of no adapter.
 constexpr int kExpandTokens = 64, kExpandThreads = 256;
 
 struct ExpandArgs {
@@ -294,14 +331,31 @@ struct ExpandArgs {
   int64_t u_pitch, u_stride;
   const float* low;
   int tokens, n, rank, adapters;
+  int columns;  // of a CTA
   const int32_t* order;
   const int32_t* ends;
   void* out;  // tokens x n
 };
 
+// Elements r .. r + 7 of a column's row of U, as read: 8 16-bit numbers.
+template <bool RINNER>
+__device__ __forceinline__ uint4 up_words(const ExpandArgs& a, const char* u, int col, int r) {
+  if (RINNER) return __ldg(reinterpret_cast<const uint4*>(u + ((int64_t)col * a.u_pitch + r) * 2));
+  uint32_t w[4];
+  const unsigned short* const p =
+      reinterpret_cast<const unsigned short*>(u) + (int64_t)r * a.u_pitch + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = r + 2 * i < a.rank ? __ldg(p + 2 * i * a.u_pitch) : 0u;
+    const uint32_t hi = r + 2 * i + 1 < a.rank ? __ldg(p + (2 * i + 1) * a.u_pitch) : 0u;
+    w[i] = lo | hi << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int F, bool RINNER>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandArgs a) {
-  extern __shared__ float lows[];  // [token][rank, whole 8s]
+  extern __shared__ __align__(16) float lows[];  // [token][rank, whole 8s]
   __shared__ int32_t rows[kExpandTokens];
   const int lane = threadIdx.x & 31, ranks = (a.rank + 7) & ~7;
   GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, kExpandTokens, (int)blockIdx.y,
@@ -313,67 +367,66 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandArgs
       int start, end;
       group_span(a.ends, a.adapters, a.tokens, base, lane, &carry, &start, &end);
     }
-    const int64_t at = carry + (int64_t)kExpandTokens * (gridDim.y - 1 - blockIdx.y);
-    if (at >= a.tokens) return;
-    tile.row0 = (int)at;
+    tile.row0 = carry + kExpandTokens * (int)(gridDim.y - 1 - blockIdx.y);
     tile.end = a.tokens;
   }
   const int count = min(kExpandTokens, tile.end - tile.row0);
-  if (threadIdx.x < count)
+  if ((int)threadIdx.x < count)
     rows[threadIdx.x] = (int32_t)token_at(a.order, tile.row0 + threadIdx.x, a.tokens);
-  if (tile.group >= 0) {
+  const bool some = tile.group >= 0;
+  const int first = (int)blockIdx.x * a.columns + threadIdx.x;
+  const int last = min((int)blockIdx.x * a.columns + a.columns, a.n);
+  const char* const u = a.u + (int64_t)(some ? tile.group : 0) * a.u_stride * 2;
+  uint4 ahead = make_uint4(0u, 0u, 0u, 0u);
+  if (some && first < last) ahead = up_words<RINNER>(a, u, first, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (count <= 0) return;
+  if (some) {
     for (int i = threadIdx.x; i < count * ranks; i += kExpandThreads) {
       const int t = i / ranks, r = i % ranks;
-      lows[i] = r < a.rank ? a.low[(int64_t)(tile.row0 + t) * a.rank + r] : 0.0f;
+      lows[i] = r < a.rank ? __ldcg(a.low + (int64_t)(tile.row0 + t) * a.rank + r) : 0.0f;
     }
   }
   __syncthreads();
-  const int col = (int)blockIdx.x * kExpandThreads + threadIdx.x;
-  if (col >= a.n) return;
-  const char* const u = a.u + (int64_t)(tile.group < 0 ? 0 : tile.group) * a.u_stride * 2;
-  for (int t0 = 0; t0 < count; t0 += 8) {
-    float sum[8];
+  for (int col = first; col < last; col += kExpandThreads) {
+    for (int t0 = 0; t0 < count; t0 += 8) {
+      float sum[8];
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      sum[t] = t0 + t < count ? a.base[(int64_t)rows[t0 + t] * a.n + col] : 0.0f;
-    if (tile.group >= 0) {
-      for (int r = 0; r < ranks; r += 8) {
-        float v[8];
-        if (RINNER) {
-          const uint4 q = __ldg(reinterpret_cast<const uint4*>(u + ((int64_t)col * a.u_pitch + r) * 2));
+      for (int t = 0; t < 8; ++t)
+        sum[t] = t0 + t < count ? __ldcg(a.base + (int64_t)rows[t0 + t] * a.n + col) : 0.0f;
+      if (some) {
+        uint4 q = t0 == 0 ? ahead : up_words<RINNER>(a, u, col, 0);
+        for (int r = 0; r < ranks; r += 8) {
           const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+          if (r + 8 < ranks) q = up_words<RINNER>(a, u, col, r + 8);
+          float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             v[i] = r + i < a.rank ? decode16<F>((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) : 0.0f;
-        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = r + i < a.rank
-                       ? decode16<F>(__ldg(reinterpret_cast<const unsigned short*>(u) +
-                                           (int64_t)(r + i) * a.u_pitch + col))
-                       : 0.0f;
-        }
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          if (t0 + t >= count) break;
-          const float4* const l = reinterpret_cast<const float4*>(lows + (t0 + t) * ranks + r);
-          const float4 p = l[0], q = l[1];
-          sum[t] = fmaf(v[0], p.x, sum[t]);
-          sum[t] = fmaf(v[1], p.y, sum[t]);
-          sum[t] = fmaf(v[2], p.z, sum[t]);
-          sum[t] = fmaf(v[3], p.w, sum[t]);
-          sum[t] = fmaf(v[4], q.x, sum[t]);
-          sum[t] = fmaf(v[5], q.y, sum[t]);
-          sum[t] = fmaf(v[6], q.z, sum[t]);
-          sum[t] = fmaf(v[7], q.w, sum[t]);
+          for (int t = 0; t < 8; ++t) {
+            if (t0 + t >= count) break;
+            const float4* const l = reinterpret_cast<const float4*>(lows + (t0 + t) * ranks + r);
+            const float4 x = l[0], y = l[1];
+            sum[t] = fmaf(v[0], x.x, sum[t]);
+            sum[t] = fmaf(v[1], x.y, sum[t]);
+            sum[t] = fmaf(v[2], x.z, sum[t]);
+            sum[t] = fmaf(v[3], x.w, sum[t]);
+            sum[t] = fmaf(v[4], y.x, sum[t]);
+            sum[t] = fmaf(v[5], y.y, sum[t]);
+            sum[t] = fmaf(v[6], y.z, sum[t]);
+            sum[t] = fmaf(v[7], y.w, sum[t]);
+          }
         }
       }
-    }
+      if (t0 == 0 && some && col + kExpandThreads < last)
+        ahead = up_words<RINNER>(a, u, col + kExpandThreads, 0);
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if (t0 + t < count)
-        static_cast<uint16_t*>(a.out)[(int64_t)rows[t0 + t] * a.n + col] =
-            (uint16_t)encode16<F>(sum[t]);
+      for (int t = 0; t < 8; ++t)
+        if (t0 + t < count)
+          static_cast<uint16_t*>(a.out)[(int64_t)rows[t0 + t] * a.n + col] =
+              (uint16_t)encode16<F>(sum[t]);
+    }
   }
 }
 
@@ -385,10 +438,16 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandArgs
 // order.  z's bytes, read once for every 64 of the rank, bound it.  `low` enters as a pair of
 // 16-bit numbers (high and what it leaves); in FP16 both are scaled by a power of two that
 // brings the adapter's largest to 2^11 .. 2^12, so that small gradients keep their digits.
-constexpr int kSumCols = 128, kSumRank = 64, kSumStep = 64, kSumStages = 3, kSumTokens = 512;
-constexpr int kSumWarps = kSumCols / 16;
-constexpr int kSumZ = kSumStep * kSumCols * 2, kSumLow = kSumStep * kSumRank * 2;
-constexpr int kSumSmem = kSumStages * kSumZ + 2 * 2 * kSumLow;
+constexpr int kSumCols = 128, kSumStep = 64, kSumTokens = 512;
+constexpr int kSumWarps = kSumCols / 16, kSumThreads = 32 * kSumWarps;
+
+template <int RT>  // 16 RT of the rank
+struct SumShape {
+  static constexpr int kRank = 16 * RT;
+  static constexpr int kZ = kSumStep * kSumCols * 2, kLow = kSumStep * kRank * 2;
+  static constexpr int kStages = 5 - RT / 2;  // with them two CTAs an SM fit
+  static constexpr int kSmem = kStages * kZ + 2 * 2 * kLow;
+};
 
 struct SumArgs {
   const char* z;
@@ -415,84 +474,106 @@ __device__ __forceinline__ uint32_t wide_slot(int row, int slot) {  // rows of 2
   return (uint32_t)(row * 256 + ((slot ^ (row & 7)) << 4));
 }
 
-template <int F>
-__global__ void __launch_bounds__(32 * kSumWarps, 2) sum_kernel(const SumArgs a) {
+template <int F, int RT>
+__global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
+  using S = SumShape<RT>;
   extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ int32_t places[kSumTokens];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const GroupTile tile =
       find_group_tile(a.ends, a.adapters, a.tokens, kSumTokens, (int)blockIdx.y, lane);
   if (tile.group < 0) return;
   const int count = min(kSumTokens, tile.end - tile.row0);
-  const int rank0 = (int)blockIdx.z * kSumRank, ranks = min(kSumRank, a.rank - rank0);
+  for (int i = threadIdx.x; i < count; i += kSumThreads)
+    places[i] = (int32_t)token_at(a.order, tile.row0 + i, a.tokens);
+  const int rank0 = (int)blockIdx.z * S::kRank, ranks = min(S::kRank, a.rank - rank0);
   const int col0 = (int)blockIdx.x * kSumCols;
   const float scale = pair_scale(a.largest, tile.group);
-  const uint32_t z0 = shared_at(raw), low0 = z0 + kSumStages * kSumZ;
+  const uint32_t z0 = shared_at(raw), low0 = z0 + S::kStages * S::kZ;
+  __syncthreads();
 
   const int slot = threadIdx.x & 15, row = threadIdx.x >> 4;  // 16 rows at a time
   const int col = col0 + 8 * slot, bytes = min(max(a.cols - col, 0) * 2, 16);
+  const char* const z = a.z + (int64_t)col * 2;
   const auto load = [&](int step, int s) {
 #pragma unroll
     for (int i = 0; i < kSumStep / 16; ++i) {
       const int r = row + 16 * i, t = step * kSumStep + r;
       const bool in = t < count && bytes > 0;
-      const char* from =
-          in ? a.z + (token_at(a.order, tile.row0 + t, a.tokens) * a.z_pitch + col) * 2 : a.z;
-      copy16(z0 + s * kSumZ + wide_slot(r, slot), from, in ? bytes : 0);
+      copy16(z0 + s * S::kZ + wide_slot(r, slot), in ? z + places[t] * a.z_pitch * 2 : a.z,
+             in ? bytes : 0);
     }
   };
-  // low: thread t has 16 of the rank of token t / 4
-  const int low_row = threadIdx.x >> 2, low_col = (threadIdx.x & 3) * 16;
-  float held[16];
+  // low: thread t has ranks 4 (t % 4) + 16 j of token t / 4
+  const int low_row = threadIdx.x >> 2, low_col = (threadIdx.x & 3) * 4;
+  const bool whole = (a.rank & 3) == 0;  // rows of whole 16 bytes
+  float held[RT][4];
   const auto fetch = [&](int step) {
     const int t = step * kSumStep + low_row;
-    const float* from = a.low + (int64_t)(tile.row0 + t) * a.rank + rank0 + low_col;
+    const float* const from = a.low + (int64_t)(tile.row0 + t) * a.rank + rank0 + low_col;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      held[i] = t < count && low_col + i < ranks ? __ldg(from + i) * scale : 0.0f;
+    for (int j = 0; j < RT; ++j) {
+      if (whole && t < count && low_col + 16 * j < ranks) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(from + 16 * j));
+        held[j][0] = v.x;
+        held[j][1] = v.y;
+        held[j][2] = v.z;
+        held[j][3] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          held[j][i] = t < count && low_col + 16 * j + i < ranks ? __ldg(from + 16 * j + i) : 0.0f;
+      }
+    }
+  };
+  const auto low_slot = [](int r, int c) {
+    return RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c);
   };
   const auto split = [&](int b) {
-    const uint32_t to = low0 + b * 2 * kSumLow;
-    if (low_col >= ((ranks + 15) & ~15)) return;
+    const uint32_t to = low0 + b * 2 * S::kLow;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t high[4], rest[4];
+    for (int j = 0; j < RT; ++j) {
+      uint32_t high[2], rest[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = held[8 * h + 2 * i], y = held[8 * h + 2 * i + 1];
+      for (int i = 0; i < 2; ++i) {
+        const float x = held[j][2 * i] * scale, y = held[j][2 * i + 1] * scale;
         const uint32_t hx = encode16<F>(x), hy = encode16<F>(y);
         high[i] = hx | hy << 16;
         rest[i] = encode16<F>(x - decode16<F>(hx)) | encode16<F>(y - decode16<F>(hy)) << 16;
       }
-      const uint32_t at = to + turned_slot(low_row, (low_col >> 3) + h);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(high[0]), "r"(high[1]),
-                   "r"(high[2]), "r"(high[3])
+      // 8 of the 16 bytes of a slot
+      const uint32_t at = to + low_slot(low_row, 2 * j + (low_col >> 3)) + 2 * (low_col & 7);
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(high[0]), "r"(high[1])
                    : "memory");
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + kSumLow), "r"(rest[0]),
-                   "r"(rest[1]), "r"(rest[2]), "r"(rest[3])
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + S::kLow), "r"(rest[0]),
+                   "r"(rest[1])
                    : "memory");
     }
   };
 
-  float sum[kSumRank / 8][4];
+  float sum[2 * RT][4];
 #pragma unroll
-  for (int i = 0; i < kSumRank / 8; ++i) {
+  for (int i = 0; i < 2 * RT; ++i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
   }
   const int steps = (count + kSumStep - 1) / kSumStep;
-  for (int i = 0; i < kSumStages - 1; ++i) {
+  for (int i = 0; i < S::kStages - 1; ++i) {
     if (i < steps) load(i, i);
     copies_done();
   }
   fetch(0);
+  int s = 0;
   for (int step = 0; step < steps; ++step) {
     split(step & 1);
-    copies_wait<kSumStages - 2>();
+    copies_wait<S::kStages - 2>();
     __syncthreads();
-    if (step + kSumStages - 1 < steps) load(step + kSumStages - 1, (step + kSumStages - 1) % kSumStages);
+    if (step + S::kStages - 1 < steps)
+      load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
     copies_done();
     if (step + 1 < steps) fetch(step + 1);
-    const uint32_t zs = z0 + step % kSumStages * kSumZ, ls = low0 + (step & 1) * 2 * kSumLow;
+    const uint32_t zs = z0 + s * S::kZ, ls = low0 + (step & 1) * 2 * S::kLow;
+    if (++s == S::kStages) s = 0;
 #pragma unroll
     for (int kk = 0; kk < kSumStep / 16; ++kk) {
       // columns 16 warp .. by tokens 16 kk ..: matrices of 8 tokens x 8 columns, turned
@@ -500,14 +581,13 @@ __global__ void __launch_bounds__(32 * kSumWarps, 2) sum_kernel(const SumArgs a)
       load_matrices<true>(zs + wide_slot(16 * kk + (lane & 7) + ((lane >> 4) << 3),
                                          2 * warp + ((lane >> 3) & 1)), m);
 #pragma unroll
-      for (int j = 0; j < kSumRank / 16; ++j) {
-        if (16 * j >= ranks) break;
+      for (int j = 0; j < RT; ++j) {
         uint32_t b[4];
-        const uint32_t at = ls + turned_slot(16 * kk + (lane & 15), 2 * j + (lane >> 4));
+        const uint32_t at = ls + low_slot(16 * kk + (lane & 15), 2 * j + (lane >> 4));
         load_matrices<true>(at, b);
         multiply<F>(sum[2 * j], m, b[0], b[1]);
         multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
-        load_matrices<true>(at + kSumLow, b);
+        load_matrices<true>(at + S::kLow, b);
         multiply<F>(sum[2 * j], m, b[0], b[1]);
         multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
       }
@@ -516,7 +596,7 @@ __global__ void __launch_bounds__(32 * kSumWarps, 2) sum_kernel(const SumArgs a)
   copies_wait<0>();
   const float back = 1.0f / scale;  // a power of two: exact
 #pragma unroll
-  for (int j = 0; j < kSumRank / 8; ++j) {
+  for (int j = 0; j < 2 * RT; ++j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int c = col0 + 16 * warp + (lane >> 2) + 8 * (i >> 1);
@@ -558,46 +638,100 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t whole(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
 
-template <int F, bool KINNER>
-int launch_low(const LowArgs& args, cudaStream_t stream) {
-  const auto kernel = &low_kernel<F, KINNER>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLowSmem);
-  if (e != cudaSuccess) return cuda_fail(e, "low part");
+// Opt-in shared memory of a kernel, once a device.
+int allow_shared(const void* kernel, int bytes) {
+  int resident = 0;
+  return prepare_kernel(kernel, 1, 32, bytes, &resident);
+}
+
+template <int F, bool KINNER, int TOKENS, int RT>
+int launch_low_as(const LowArgs& args, cudaStream_t stream) {
+  using S = LowShape<TOKENS, RT>;
+  const auto kernel = &low_kernel<F, KINNER, TOKENS, RT>;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
   const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
-  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, kLowTokens);
-  const int64_t blocks = ceil_div(args.rank, kLowRank), steps = ceil_div(args.k, kLowStep);
-  // Parts of the sum while the tiles that are likely leave SMs idle, at least 4 steps each.
-  const int64_t likely = (args.tokens / kLowTokens + (busy + 1) / 2) * blocks;
-  int splits = 1;
-  while (splits < 8 && likely * splits < 2 * sm_count() && steps >= 8 * splits) splits *= 2;
+  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, TOKENS);
+  const int64_t blocks = ceil_div(args.rank, S::kRank), steps = ceil_div(args.k, kLowStep);
+  // Parts of the sum while all likely CTAs run at once (two an SM; four of the small), at least
+  // four stages each.  A second round costs as much as the first: 16 prompts of 4096 tokens in
+  // all, 4096 -> 64, took 30 us in 384 CTAs.
+  const int64_t likely = (args.tokens / TOKENS + (busy + 1) / 2) * blocks;
+  const int64_t room = (TOKENS == 16 ? 4 : 2) * sm_count();
+  int64_t splits = likely > 0 ? room / likely : 8;
+  if (splits > steps / 4) splits = steps / 4;
+  splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
   cudaLaunchConfig_t config{};
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = (unsigned)splits;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.gridDim = dim3((unsigned)(tiles * splits), (unsigned)blocks);
-  config.blockDim = dim3(32 * kLowWarps);
-  config.dynamicSmemBytes = kLowSmem;
+  config.blockDim = dim3(S::kThreads);
+  config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  e = cudaLaunchKernelEx(&config, kernel, args);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args);
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "low part launch");
 }
 
+template <int F, bool KINNER>
+int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
+  if (args.rank <= 16)
+    return thin ? launch_low_as<F, KINNER, 16, 1>(args, stream)
+                : launch_low_as<F, KINNER, 128, 1>(args, stream);
+  if (args.rank <= 32)
+    return thin ? launch_low_as<F, KINNER, 16, 2>(args, stream)
+                : launch_low_as<F, KINNER, 128, 2>(args, stream);
+  return thin ? launch_low_as<F, KINNER, 16, 4>(args, stream)
+              : launch_low_as<F, KINNER, 128, 4>(args, stream);
+}
+
 template <int F, bool RINNER>
-int launch_expand(const ExpandArgs& args, cudaStream_t stream) {
+int launch_expand(ExpandArgs& args, cudaStream_t stream) {
   const auto kernel = &expand_kernel<F, RINNER>;
-  const int bytes = kExpandTokens * (int)ceil_div(args.rank, 8) * 8 * 4;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kExpandTokens * SRS_ADAPTER_MAX_RANK * 4);
-  if (e != cudaSuccess) return cuda_fail(e, "expansion");
+  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel),
+                            kExpandTokens * SRS_ADAPTER_MAX_RANK * 4))
+    return rc;
+  const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
   // one more tile than adapters' tokens can take: tokens of none in a last, partial one
   const int64_t tiles = most_group_tiles(args.tokens, args.adapters, kExpandTokens) + 1;
-  const dim3 grid((unsigned)ceil_div(args.n, kExpandThreads), (unsigned)tiles);
-  kernel<<<grid, kExpandThreads, bytes, stream>>>(args);
-  e = cudaGetLastError();
+  // columns of a CTA: as many as let all likely CTAs run at once
+  int64_t each = ceil_div(ceil_div(args.n, kExpandThreads) * busy, 6 * sm_count());
+  each = each < 1 ? 1 : each > 16 ? 16 : each;
+  args.columns = (int)each * kExpandThreads;
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  config.gridDim = dim3((unsigned)ceil_div(args.n, args.columns), (unsigned)tiles);
+  config.blockDim = dim3(kExpandThreads);
+  config.dynamicSmemBytes = (size_t)(kExpandTokens * ceil_div(args.rank, 8) * 8 * 4);
+  config.stream = stream;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<const ExpandArgs&>(args));
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "expansion launch");
+}
+
+template <int F, int RT>
+int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
+  using S = SumShape<RT>;
+  const auto kernel = &sum_kernel<F, RT>;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+  const dim3 grid((unsigned)ceil_div(args.cols, kSumCols),
+                  (unsigned)most_group_tiles(args.tokens, args.adapters, kSumTokens),
+                  (unsigned)ceil_div(args.rank, S::kRank));
+  kernel<<<grid, kSumThreads, S::kSmem, stream>>>(args);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "adapter gradient launch");
+}
+
+template <int F>
+int launch_sum(const SumArgs& args, cudaStream_t stream) {
+  if (args.rank <= 16) return launch_sum_as<F, 1>(args, stream);
+  if (args.rank <= 32) return launch_sum_as<F, 2>(args, stream);
+  return launch_sum_as<F, 4>(args, stream);
 }
 
 int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, bool turned) {
@@ -719,10 +853,10 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
     l.pitch = pairs.pitch;
     l.rest_at = pairs.rest_at;
   }
-  if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, st)
-                              : launch_low<SRS_FMT_F16, false>(l, st))
-                      : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, st)
-                              : launch_low<SRS_FMT_F16, true>(l, st)))
+  if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, thin, st)
+                              : launch_low<SRS_FMT_F16, false>(l, thin, st))
+                      : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, thin, st)
+                              : launch_low<SRS_FMT_F16, true>(l, thin, st)))
     return rc;
   if (n == 0 || k == 0) return SRS_OK;
 
@@ -736,6 +870,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   QuantizeCall q{x, a->format, tokens, k, x_pitch, block_format, rule, false, seed, 0u};
   q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
   q.order = thin ? nullptr : l.order;
+  q.overlap = true;  // beside the low part
   if (int rc = quantize(q, st)) return rc;
   const void* const up = reinterpret_cast<const void*>(turned ? a->down : a->up);
   const int64_t up_pitch = turned ? a->down_pitch : a->up_pitch;
@@ -746,7 +881,12 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
     return launch_adapter_product(rows, *w, k, call, edge, d, st);
   }
   float* const base = reinterpret_cast<float*>(at + space.base);
-  if (int rc = srs_matmul_blocks(&rows, w, k, base, SRS_FMT_F32, stream)) return rc;
+  if (w->rows >= tokens) {
+    // beside the quantisation: its weights are streamed first
+    if (int rc = launch_thin(*w, rows, k, base, SRS_FMT_F32, 1, n, true, st)) return rc;
+  } else {
+    if (int rc = launch_thin(rows, *w, k, base, SRS_FMT_F32, n, 1, false, st)) return rc;
+  }
   ExpandArgs x_args{};
   x_args.base = base;
   x_args.u = static_cast<const char*>(up);
@@ -816,19 +956,13 @@ extern "C" int srs_adapter_gradient(const void* z, int format, int64_t tokens, i
   a.out = out;
   a.parts = static_cast<float*>(workspace);
   a.turned = turned != 0;
-  const auto kernel = format == SRS_FMT_BF16 ? &sum_kernel<SRS_FMT_BF16> : &sum_kernel<SRS_FMT_F16>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem);
-  if (e != cudaSuccess) return cuda_fail(e, "adapter gradient");
-  const dim3 grid((unsigned)ceil_div(cols, kSumCols),
-                  (unsigned)most_group_tiles(tokens, adapters, kSumTokens),
-                  (unsigned)ceil_div(rank, kSumRank));
-  kernel<<<grid, 32 * kSumWarps, kSumSmem, st>>>(a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "adapter gradient launch");
+  if (int rc = format == SRS_FMT_BF16 ? launch_sum<SRS_FMT_BF16>(a, st)
+                                      : launch_sum<SRS_FMT_F16>(a, st))
+    return rc;
   const int64_t blocks = ceil_div((int64_t)rank * cols, 1024);
   const dim3 joins((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)adapters);
   if (format == SRS_FMT_BF16) join_kernel<SRS_FMT_BF16><<<joins, 256, 0, st>>>(a);
   else join_kernel<SRS_FMT_F16><<<joins, 256, 0, st>>>(a);
-  e = cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "adapter gradient launch");
 }

@@ -31,6 +31,7 @@ struct QuantizeArgs {
   const int32_t* ends;
   int groups;
   const int32_t* order;  // rows kernel: row i of the copy is row order[i] of x (null: i)
+  bool overlap;          // host: launched beside the kernel ahead
 };
 
 // What a tile kernel's grid covers: one matrix; a stack of them (blockIdx.z), whose counters
@@ -245,6 +246,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
         encode_values<OF>(y, a.ctr + (uint32_t)(from * a.cols + col), a.rule, plain);
     store_bytes(a.data + row * a.data_pitch + col, w, cols_left);
   }
+  // Launched beside the kernel ahead: done only when that one is.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // One CTA quantises one 128 x 128 tile of x, read once into shared memory.  Thread t has
@@ -530,11 +533,22 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool square, int matrices,
                                         stream);
   if (square || a.data_t != nullptr) return launch_tiles<OF, XF, kMatrix>(a, square, tiles, stream);
   const dim3 grid(columns, (unsigned)((a.rows + 16 * kAhead - 1) / (16 * kAhead)));
-  if (a.order != nullptr)
-    quantize_rows_kernel<OF, XF, true><<<grid, kThreads, 0, stream>>>(a);
-  else
-    quantize_rows_kernel<OF, XF, false><<<grid, kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  const auto kernel = a.order != nullptr ? &quantize_rows_kernel<OF, XF, true>
+                                         : &quantize_rows_kernel<OF, XF, false>;
+  if (!a.overlap) {
+    kernel<<<grid, kThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+  }
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.gridDim = grid;
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, a);
 }
 
 template <int OF>
@@ -678,6 +692,7 @@ int srs::quantize(const QuantizeCall& q, cudaStream_t stream) {
   a.ends = q.ends;
   a.groups = q.groups;
   a.order = q.order;
+  a.overlap = q.overlap;
   const cudaError_t e =
       q.out_format == SRS_FMT_E4M3
           ? launch_quantize<SRS_FMT_E4M3>(a, q.x_format, q.square, (int)q.matrices, stream)

@@ -58,6 +58,7 @@ struct QuantizeCall {
   int groups = 0;
   const int32_t* order = nullptr;
   bool for_product = false;
+  bool overlap = false;  // rows alone: may start beside the kernel ahead, which it reads nothing of
 };
 int quantize(const QuantizeCall& q, cudaStream_t stream);
 

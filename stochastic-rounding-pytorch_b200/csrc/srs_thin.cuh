@@ -110,6 +110,8 @@ template <int BN, bool GROUPED>
 __global__ void __launch_bounds__(kThinThreads, 2)
 thin_product_kernel(const __grid_constant__ ThinArgs a) {
   using S = ThinShape<BN>;
+  // A kernel launched to overlap this one may start (and wait for it).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2 * kThinMaxStages + 1 + 2 * kThinSlots];
   __shared__ uint32_t tmem_slot;
