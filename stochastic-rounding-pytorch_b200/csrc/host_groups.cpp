@@ -1,16 +1,22 @@
-// _srs_groups: tensor front end of the operators on rows in groups (a CPython module):
-// checks, allocation and launch in one call, as _srs_blocks does for the FP8 block entry points.
-// A function returns the negative status of an entry point as an int; the caller turns it
-// into the error.
+// _srs_groups: tensor front end of the operators on rows in groups (a CPython module): checks,
+// allocation, launches and the gradients' bookkeeping in one call.  In Python a training call of
+// small matrices took 180 us of the host's time, most of it between the launches.
+#include <torch/csrc/autograd/custom_function.h>
+
 #include "host_blocks.h"
 
 namespace {
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+decltype(&srs_last_error) g_last_error = nullptr;
 decltype(&srs_group_rows) g_group_rows = nullptr;
 decltype(&srs_quantize_stack) g_quantize_stack = nullptr;
 decltype(&srs_quantize_groups) g_quantize_groups = nullptr;
 decltype(&srs_group_columns) g_group_columns = nullptr;
 decltype(&srs_group_scales) g_group_scales = nullptr;
+decltype(&srs_matmul_blocks) g_matmul = nullptr;
 decltype(&srs_expert_matmul) g_expert_matmul = nullptr;
 decltype(&srs_expert_linear) g_expert_linear = nullptr;
 decltype(&srs_expert_gradient) g_expert_gradient = nullptr;
@@ -20,9 +26,18 @@ decltype(&srs_adapter_linear) g_adapter_linear = nullptr;
 decltype(&srs_adapter_gradient_workspace) g_gradient_workspace = nullptr;
 decltype(&srs_adapter_gradient) g_adapter_gradient = nullptr;
 
+// The error of an entry point: ValueError for arguments, RuntimeError else.
+void check(int rc) {
+  if (rc == SRS_OK) return;
+  TORCH_CHECK_VALUE(rc != SRS_ERR_INVALID_ARGUMENT, g_last_error());
+  TORCH_CHECK(false, g_last_error());
+}
+
 void* stream_of(const at::Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
+
+const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 
 // `ends` as int32 on x's device (int64 is converted).
 at::Tensor checked_ends(const at::Tensor& ends, const at::Tensor& x, const char* what) {
@@ -65,7 +80,7 @@ Blocks empty_stack(int64_t matrices, int64_t rows, int64_t cols, int format, boo
 
 // The weights of all groups, (groups, n, k), as one operand of groups * n rows; data or scales
 // laid out otherwise are copied once, `b` keeps the copies alive.
-int stack_operand(const char* name, Blocks* b, srs_blocks* out) {
+srs_blocks stack_operand(const char* name, Blocks* b) {
   at::Tensor &data = b->data, &scale = b->scale;
   const bool e4m3 = data.scalar_type() == at::kFloat8_e4m3fn;
   TORCH_CHECK_TYPE(e4m3 || data.scalar_type() == at::kFloat8_e5m2, name,
@@ -97,9 +112,8 @@ int stack_operand(const char* name, Blocks* b, srs_blocks* out) {
       const at::Tensor flat = data.contiguous();
       data_pitch = ceil_div(k, 16) * 16;
       at::Tensor copy = at::empty({groups, n, data_pitch}, data.options());
-      if (int rc = g_copy_rows(flat.data_ptr(), k, groups * n, k, copy.data_ptr(), data_pitch,
-                               stream_of(data)))
-        return rc;
+      check(g_copy_rows(flat.data_ptr(), k, groups * n, k, copy.data_ptr(), data_pitch,
+                        stream_of(data)));
       data = copy;
     }
     scale_pitch = pitch_of(scale, blocks);
@@ -108,251 +122,15 @@ int stack_operand(const char* name, Blocks* b, srs_blocks* out) {
       scale_pitch = blocks;
     }
   }
-  out->data = reinterpret_cast<uint64_t>(data.data_ptr());
-  out->scale = reinterpret_cast<uint64_t>(scale.data_ptr());
-  out->rows = groups * n;
-  out->pitch = data_pitch;
-  out->scale_pitch = scale_pitch;
-  out->format = e4m3 ? SRS_FMT_E4M3 : SRS_FMT_E5M2;
-  out->square = high != n;
-  return SRS_OK;
-}
-
-PyObject* wrap(std::initializer_list<at::Tensor> tensors) {
-  PyObject* out = PyTuple_New((Py_ssize_t)tensors.size());
-  if (out == nullptr) return nullptr;
-  Py_ssize_t i = 0;
-  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  srs_blocks out{};
+  out.data = reinterpret_cast<uint64_t>(data.data_ptr());
+  out.scale = reinterpret_cast<uint64_t>(scale.data_ptr());
+  out.rows = groups * n;
+  out.pitch = data_pitch;
+  out.scale_pitch = scale_pitch;
+  out.format = e4m3 ? SRS_FMT_E4M3 : SRS_FMT_E5M2;
+  out.square = high != n;
   return out;
-}
-
-template <class F>
-bool bind_one(PyObject* table, const char* name, F* to) {
-  PyObject* address = PyDict_GetItemString(table, name);
-  if (address == nullptr) {
-    PyErr_Format(PyExc_KeyError, "%s", name);
-    return false;
-  }
-  const unsigned long long at = PyLong_AsUnsignedLongLong(address);
-  if (PyErr_Occurred()) return false;
-  *to = reinterpret_cast<F>(static_cast<uintptr_t>(at));
-  return true;
-}
-
-PyObject* py_bind(PyObject*, PyObject* args) {
-  PyObject* t;
-  if (!PyArg_ParseTuple(args, "O!", &PyDict_Type, &t)) return nullptr;
-  if (!bind_one(t, "srs_group_rows", &g_group_rows) ||
-      !bind_one(t, "srs_quantize_stack", &g_quantize_stack) ||
-      !bind_one(t, "srs_quantize_groups", &g_quantize_groups) ||
-      !bind_one(t, "srs_group_columns", &g_group_columns) ||
-      !bind_one(t, "srs_group_scales", &g_group_scales) ||
-      !bind_one(t, "srs_expert_matmul", &g_expert_matmul) ||
-      !bind_one(t, "srs_expert_linear", &g_expert_linear) ||
-      !bind_one(t, "srs_expert_gradient", &g_expert_gradient) ||
-      !bind_one(t, "srs_linear_workspace", &g_linear_workspace) ||
-      !bind_one(t, "srs_adapter_workspace", &g_adapter_workspace) ||
-      !bind_one(t, "srs_adapter_linear", &g_adapter_linear) ||
-      !bind_one(t, "srs_adapter_gradient_workspace", &g_gradient_workspace) ||
-      !bind_one(t, "srs_adapter_gradient", &g_adapter_gradient) ||
-      !bind_one(t, "srs_copy_rows", &g_copy_rows))
-    return nullptr;
-  Py_RETURN_NONE;
-}
-
-PyObject* py_group_rows(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject* obj;
-  int groups;
-  if (!PyArg_ParseTuple(args, "Oi", &obj, &groups)) return nullptr;
-  c10::NoGradGuard no_grad;
-  const at::Tensor& index = tensor(obj, "index");
-  const c10::cuda::OptionalCUDAGuard guard(index.device());
-  TORCH_CHECK_TYPE(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong,
-                   "group_rows: indices are int32 or int64, got ", index.scalar_type());
-  TORCH_CHECK_VALUE(groups > 0, "group_rows: groups must be positive, got ", groups);
-  const at::Tensor flat = index.contiguous();
-  const auto ints = index.options().dtype(at::kInt);
-  at::Tensor order = at::empty({index.numel()}, ints), ends = at::empty({groups}, ints);
-  const int rc = g_group_rows(flat.data_ptr(), (int)index.element_size(), index.numel(), groups,
-                              static_cast<int32_t*>(order.data_ptr()),
-                              static_cast<int32_t*>(ends.data_ptr()), stream_of(index));
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
-  return wrap({order, ends});
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_quantize_stack(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject* obj;
-  int format, rule, square, orientation;
-  unsigned int seed, offset;
-  if (!PyArg_ParseTuple(args, "OiiiIIi", &obj, &format, &rule, &square, &seed, &offset,
-                        &orientation))
-    return nullptr;
-  c10::NoGradGuard no_grad;
-  const at::Tensor& x = tensor(obj, "x");
-  const c10::cuda::OptionalCUDAGuard guard(x.device());
-  const int x_format = source_format(x, "quantize_blocks");
-  TORCH_CHECK_VALUE(x.dim() == 3, "a stack of matrices has three dimensions, got shape ",
-                    x.sizes());
-  const at::Tensor src = x.stride(2) != 1 && x.size(2) > 1 ? x.contiguous() : x;
-  const int64_t matrices = x.size(0), rows = x.size(1), cols = x.size(2);
-  Blocks straight, turned;
-  if (orientation & 1) straight = empty_stack(matrices, rows, cols, format, square != 0, x);
-  if (orientation & 2) turned = empty_stack(matrices, cols, rows, format, square != 0, x);
-  if (x.numel() != 0) {
-    const srs_block_copy copy = copy_of(straight), copy_t = copy_of(turned);
-    const int rc = g_quantize_stack(src.data_ptr(), x_format, matrices, rows, cols, src.stride(1),
-                                    src.stride(0), format, rule, square, seed, offset, &copy,
-                                    &copy_t, stream_of(x));
-    if (rc != SRS_OK) return PyLong_FromLong(rc);
-  }
-  if (orientation == 3) return wrap({straight.data, straight.scale, turned.data, turned.scale});
-  const Blocks& one = orientation == 1 ? straight : turned;
-  return wrap({one.data, one.scale});
-  END_HANDLE_TH_ERRORS
-}
-
-// The transposed copy of a matrix whose rows are in groups; with `rows` the copy by rows, too.
-PyObject* py_quantize_groups(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject *obj, *ends_obj;
-  int format, rule, rows;
-  unsigned int seed;
-  if (!PyArg_ParseTuple(args, "OOiiIi", &obj, &ends_obj, &format, &rule, &seed, &rows))
-    return nullptr;
-  c10::NoGradGuard no_grad;
-  const at::Tensor& x = tensor(obj, "x");
-  const c10::cuda::OptionalCUDAGuard guard(x.device());
-  const int x_format = source_format(x, "quantize_groups");
-  TORCH_CHECK_VALUE(x.dim() == 2, "quantize_groups needs a matrix, got shape ", x.sizes());
-  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), x, "quantize_groups");
-  const at::Tensor src = x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x;
-  const int64_t height = x.size(0), cols = x.size(1);
-  const int groups = (int)ends.numel();
-  Blocks straight, turned;
-  if (rows) straight = empty_blocks(height, cols, format, false, x);
-  turned.data = at::empty({cols, g_group_columns(height, groups)},
-                          x.options().dtype(format == SRS_FMT_E4M3 ? at::kFloat8_e4m3fn
-                                                                   : at::kFloat8_e5m2));
-  turned.scale = at::empty({cols, ceil_div(g_group_scales(height, groups), 4) * 4},
-                           x.options().dtype(at::kFloat8_e8m0fnu));
-  if (x.numel() != 0) {
-    const srs_block_copy copy = copy_of(straight), copy_t = copy_of(turned);
-    const int rc = g_quantize_groups(src.data_ptr(), x_format, height, cols, src.stride(0),
-                                     static_cast<const int32_t*>(ends.data_ptr()), groups, format,
-                                     rule, seed, 0u, &copy, &copy_t, stream_of(x));
-    if (rc != SRS_OK) return PyLong_FromLong(rc);
-  }
-  if (rows) return wrap({straight.data, straight.scale, turned.data, turned.scale});
-  return wrap({turned.data, turned.scale});
-  END_HANDLE_TH_ERRORS
-}
-
-void check_groups(const at::Tensor& ends, const at::Tensor& weight) {
-  TORCH_CHECK_VALUE(weight.dim() != 3 || ends.numel() == weight.size(0), "ends of ", ends.numel(),
-                    " groups do not fit weights of shape ", weight.sizes());
-}
-
-PyObject* py_expert_matmul(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject *a_obj, *a_scale, *w_obj, *w_scale, *ends_obj;
-  int format;
-  if (!PyArg_ParseTuple(args, "OOOOOi", &a_obj, &a_scale, &w_obj, &w_scale, &ends_obj, &format))
-    return nullptr;
-  c10::NoGradGuard no_grad;
-  Blocks a{tensor(a_obj, "a's data"), tensor(a_scale, "a's scale")};
-  Blocks w{tensor(w_obj, "the weight's data"), tensor(w_scale, "the weight's scale")};
-  const c10::cuda::OptionalCUDAGuard guard(a.data.device());
-  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), a.data, "expert_linear");
-  TORCH_CHECK_VALUE(a.data.device() == w.data.device(),
-                    "all tensors must be on the same CUDA device");
-  check_groups(ends, w.data);
-  const int64_t rows = a.data.size(0), n = w.data.size(1), k = w.data.size(2);
-  srs_blocks left{}, right{};
-  int rc = operand("a", &a, &left);
-  if (rc == SRS_OK) rc = stack_operand("weight", &w, &right);
-  at::Tensor out;
-  if (rc == SRS_OK) {
-    out = at::empty({rows, n}, a.data.options().dtype(result_type(format)));
-    left.square = 0;  // (one row: both forms have one scale a block)
-    if (out.numel() != 0)
-      rc = g_expert_matmul(&left, &right, (int)ends.numel(),
-                           static_cast<const int32_t*>(ends.data_ptr()), k, out.data_ptr(), format,
-                           stream_of(out));
-  }
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
-  return THPVariable_Wrap(out);
-  END_HANDLE_TH_ERRORS
-}
-
-// x (rows, k) quantised to nearest in rows, times the blocks of its rows' groups.
-PyObject* py_expert_linear(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject *obj, *w_obj, *w_scale, *ends_obj;
-  int format;
-  if (!PyArg_ParseTuple(args, "OOOOi", &obj, &w_obj, &w_scale, &ends_obj, &format)) return nullptr;
-  c10::NoGradGuard no_grad;
-  const at::Tensor& x = tensor(obj, "x");
-  Blocks w{tensor(w_obj, "the weight's data"), tensor(w_scale, "the weight's scale")};
-  const c10::cuda::OptionalCUDAGuard guard(x.device());
-  const int x_format = source_format(x, "expert_linear");
-  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), x, "expert_linear");
-  TORCH_CHECK_VALUE(x.device() == w.data.device(), "all tensors must be on the same CUDA device");
-  check_groups(ends, w.data);
-  const int64_t rows = x.size(0), k = x.size(1), n = w.data.size(1);
-  const at::Tensor src = x.stride(1) != 1 && k > 1 ? x.contiguous() : x;
-  srs_blocks matrix{};
-  int rc = stack_operand("weight", &w, &matrix);
-  at::Tensor out;
-  if (rc == SRS_OK) {
-    out = at::empty({rows, n}, x.options());
-    const int64_t bytes = g_linear_workspace(rows, k);
-    const at::Tensor space = at::empty({bytes}, x.options().dtype(at::kByte));
-    if (out.numel() != 0)
-      rc = g_expert_linear(src.data_ptr(), x_format, rows, k, src.stride(0), format, &matrix,
-                           (int)ends.numel(), static_cast<const int32_t*>(ends.data_ptr()),
-                           out.data_ptr(), space.data_ptr(), bytes, stream_of(x));
-  }
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
-  return THPVariable_Wrap(out);
-  END_HANDLE_TH_ERRORS
-}
-
-// Transposed copies of two matrices whose `rows` rows are in groups -> (groups, m, n).
-PyObject* py_expert_gradient(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject *a_obj, *a_scale, *b_obj, *b_scale, *ends_obj;
-  long long rows;
-  int format;
-  if (!PyArg_ParseTuple(args, "OOOOLOi", &a_obj, &a_scale, &b_obj, &b_scale, &rows, &ends_obj,
-                        &format))
-    return nullptr;
-  c10::NoGradGuard no_grad;
-  const Blocks a{tensor(a_obj, "a's data"), tensor(a_scale, "a's scale")};
-  const Blocks b{tensor(b_obj, "b's data"), tensor(b_scale, "b's scale")};
-  const c10::cuda::OptionalCUDAGuard guard(a.data.device());
-  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), a.data, "expert_linear");
-  srs_blocks left{}, right{};
-  for (const auto& [from, to] : {std::make_pair(&a, &left), std::make_pair(&b, &right)}) {
-    to->data = reinterpret_cast<uint64_t>(from->data.data_ptr());
-    to->scale = reinterpret_cast<uint64_t>(from->scale.data_ptr());
-    to->rows = from->data.size(0);
-    to->pitch = from->data.stride(0);
-    to->scale_pitch = from->scale.stride(0);
-    to->format = from->data.scalar_type() == at::kFloat8_e4m3fn ? SRS_FMT_E4M3 : SRS_FMT_E5M2;
-  }
-  at::Tensor out = at::empty({ends.numel(), left.rows, right.rows},
-                             a.data.options().dtype(result_type(format)));
-  int rc = SRS_OK;
-  if (out.numel() != 0)
-    rc = g_expert_gradient(&left, &right, rows, (int)ends.numel(),
-                           static_cast<const int32_t*>(ends.data_ptr()), out.data_ptr(), format,
-                           stream_of(out));
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
-  return THPVariable_Wrap(out);
-  END_HANDLE_TH_ERRORS
 }
 
 // A 16-bit matrix, or a stack of them, whose rows start on 16-byte boundaries; one laid out
@@ -381,11 +159,14 @@ struct Adapters {
   srs_adapters c{};
 };
 
-void set_adapters(Adapters* a, const at::Tensor& x, int64_t in, int64_t out, PyObject* down,
-                  PyObject* up, PyObject* scale, double factor, PyObject* order, PyObject* ends) {
+// The adapters of a projection from `in` to `out`; `scale` undefined: `factor` alone.
+Adapters adapters_of(const at::Tensor& x, int64_t in, int64_t out, const at::Tensor& down,
+                     const at::Tensor& up, const at::Tensor& scale, double factor,
+                     const at::Tensor& places, const at::Tensor& ends) {
   const char* what = "adapter_linear";
-  a->down = tensor(down, "down");
-  a->up = tensor(up, "up");
+  Adapters given, *a = &given;
+  a->down = down;
+  a->up = up;
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what,
                    " takes BF16 or FP16, got ", x.scalar_type());
   TORCH_CHECK_TYPE(
@@ -402,10 +183,9 @@ void set_adapters(Adapters* a, const at::Tensor& x, int64_t in, int64_t out, PyO
   const int64_t count = a->down.size(0), rank = a->down.size(1);
   TORCH_CHECK_VALUE(rank > 0 && rank <= SRS_ADAPTER_MAX_RANK, what, ": the rank must be in [1, ",
                     SRS_ADAPTER_MAX_RANK, "], got ", rank);
-  a->ends = checked_ends(tensor(ends, "ends"), x, what);
+  a->ends = checked_ends(ends, x, what);
   TORCH_CHECK_VALUE(a->ends.numel() == count, what, ": ends of ", a->ends.numel(),
                     " groups do not fit ", count, " adapters");
-  const at::Tensor& places = tensor(order, "order");
   TORCH_CHECK_TYPE(places.scalar_type() == at::kInt || places.scalar_type() == at::kLong, what,
                    ": the order is int32 or int64, got ", places.scalar_type());
   TORCH_CHECK_VALUE(places.device() == x.device() && places.dim() == 1 &&
@@ -413,8 +193,8 @@ void set_adapters(Adapters* a, const at::Tensor& x, int64_t in, int64_t out, PyO
                     what, ": order of shape ", places.sizes(), " does not fit ", x.size(0),
                     " tokens on ", x.device());
   a->order = places.to(at::kInt).contiguous();
-  if (scale != Py_None) {
-    a->scale = tensor(scale, "scale");
+  if (scale.defined()) {
+    a->scale = scale;
     TORCH_CHECK_TYPE(a->scale.scalar_type() == at::kFloat, what, ": scales are FP32, got ",
                      a->scale.scalar_type());
     TORCH_CHECK_VALUE(a->scale.device() == x.device() && a->scale.dim() == 1 &&
@@ -439,28 +219,164 @@ void set_adapters(Adapters* a, const at::Tensor& x, int64_t in, int64_t out, PyO
   c.count = (int32_t)count;
   c.rank = (int32_t)rank;
   c.format = x.scalar_type() == at::kBFloat16 ? SRS_FMT_BF16 : SRS_FMT_F16;
+  return given;
 }
 
-// x (tokens, k), blocks of the projection (None: the low part alone) -> (d or None, low,
-// largest).  turned: x is the output's gradient.
-PyObject* py_adapter_linear(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
-  PyObject *x_obj, *w_obj, *w_scale, *down, *up, *scale, *order, *ends;
-  int format, rule, turned, keep;
-  unsigned int seed;
-  double factor;
-  if (!PyArg_ParseTuple(args, "OiiIOOOOOdOOii", &x_obj, &format, &rule, &seed, &w_obj, &w_scale,
-                        &down, &up, &scale, &factor, &order, &ends, &turned, &keep))
-    return nullptr;
-  c10::NoGradGuard no_grad;
-  const at::Tensor& given = tensor(x_obj, "x");
-  const c10::cuda::OptionalCUDAGuard guard(given.device());
+// ---------------------------------------------------------------- operators --
+
+// How a gradient is quantised.
+struct Rounding {
+  int format, rule;
+  uint32_t seed;
+};
+constexpr int kBoth = 3, kRows = 1, kColumns = 2;
+
+// One matrix (two dimensions) or a stack of them in blocks; orientation: kRows, kColumns, kBoth.
+void quantize(const at::Tensor& x, const Rounding& how, bool square, uint32_t offset,
+              int orientation, Blocks* straight, Blocks* turned) {
+  const int x_format = source_format(x, "quantize_blocks");
+  const bool stack = x.dim() == 3;
+  const int64_t last = x.dim() - 1;
+  const at::Tensor src = x.stride(last) != 1 && x.size(last) > 1 ? x.contiguous() : x;
+  const int64_t matrices = stack ? x.size(0) : 1, rows = x.size(last - 1), cols = x.size(last);
+  const auto make = [&](int64_t high, int64_t wide) {
+    return stack ? empty_stack(matrices, high, wide, how.format, square, x)
+                 : empty_blocks(high, wide, how.format, square, x);
+  };
+  if (orientation & kRows) *straight = make(rows, cols);
+  if (orientation & kColumns) *turned = make(cols, rows);
+  if (x.numel() == 0) return;
+  const srs_block_copy copy = straight != nullptr ? copy_of(*straight) : srs_block_copy{};
+  const srs_block_copy copy_t = turned != nullptr ? copy_of(*turned) : srs_block_copy{};
+  check(g_quantize_stack(src.data_ptr(), x_format, matrices, rows, cols, src.stride(last - 1),
+                         stack ? src.stride(0) : 0, how.format, how.rule, square, how.seed, offset,
+                         &copy, &copy_t, stream_of(x)));
+}
+
+// The transposed copy of a matrix whose rows are in groups; beside it the copy by rows.
+void quantize_groups(const at::Tensor& x, const at::Tensor& ends, const Rounding& how,
+                     Blocks* straight, Blocks* turned) {
+  const int x_format = source_format(x, "expert_linear");
+  const at::Tensor src = x.stride(1) != 1 && x.size(1) > 1 ? x.contiguous() : x;
+  const int64_t height = x.size(0), cols = x.size(1);
+  const int groups = (int)ends.numel();
+  if (straight != nullptr) *straight = empty_blocks(height, cols, how.format, false, x);
+  turned->data = at::empty({cols, g_group_columns(height, groups)},
+                           x.options().dtype(how.format == SRS_FMT_E4M3 ? at::kFloat8_e4m3fn
+                                                                        : at::kFloat8_e5m2));
+  turned->scale = at::empty({cols, ceil_div(g_group_scales(height, groups), 4) * 4},
+                            x.options().dtype(at::kFloat8_e8m0fnu));
+  if (x.numel() == 0) return;
+  const srs_block_copy copy = straight != nullptr ? copy_of(*straight) : srs_block_copy{};
+  const srs_block_copy copy_t = copy_of(*turned);
+  check(g_quantize_groups(src.data_ptr(), x_format, height, cols, src.stride(0), ints(ends), groups,
+                          how.format, how.rule, how.seed, 0u, &copy, &copy_t, stream_of(x)));
+}
+
+// a[i] w_e^T for the rows i of group e.
+at::Tensor expert_matmul(Blocks a, Blocks w, const at::Tensor& ends, at::ScalarType type,
+                         int format) {
+  srs_blocks left{};
+  check(operand("a", &a, &left));
+  const srs_blocks right = stack_operand("weight", &w);
+  const int64_t n = w.data.size(1), k = w.data.size(2);
+  at::Tensor out = at::empty({left.rows, n}, a.data.options().dtype(type));
+  left.square = 0;  // (one row: both forms have one scale a block)
+  if (out.numel() != 0)
+    check(g_expert_matmul(&left, &right, (int)ends.numel(), ints(ends), k, out.data_ptr(), format,
+                          stream_of(out)));
+  return out;
+}
+
+srs_blocks turned_operand(const Blocks& b) {
+  srs_blocks o{};
+  o.data = reinterpret_cast<uint64_t>(b.data.data_ptr());
+  o.scale = reinterpret_cast<uint64_t>(b.scale.data_ptr());
+  o.rows = b.data.size(0);
+  o.pitch = b.data.stride(0);
+  o.scale_pitch = b.scale.stride(0);
+  o.format = b.data.scalar_type() == at::kFloat8_e4m3fn ? SRS_FMT_E4M3 : SRS_FMT_E5M2;
+  return o;
+}
+
+// a_e^T b_e of two matrices of `rows` rows from their transposed copies.
+at::Tensor expert_gradient(const Blocks& a, const Blocks& b, int64_t rows, const at::Tensor& ends,
+                           at::ScalarType type, int format) {
+  const srs_blocks left = turned_operand(a), right = turned_operand(b);
+  at::Tensor out =
+      at::empty({ends.numel(), left.rows, right.rows}, a.data.options().dtype(type));
+  if (out.numel() != 0)
+    check(g_expert_gradient(&left, &right, rows, (int)ends.numel(), ints(ends), out.data_ptr(),
+                            format, stream_of(out)));
+  return out;
+}
+
+int format_of(at::ScalarType type) {
+  return type == at::kFloat ? SRS_FMT_F32 : type == at::kBFloat16 ? SRS_FMT_BF16 : SRS_FMT_F16;
+}
+
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what,
+              " has a first derivative only: its backward pass cannot be differentiated");
+}
+
+struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const at::Tensor& ends, int64_t format, int64_t grad_format,
+                            int64_t grad_rule, int64_t seed, bool need_x, bool need_w) {
+    const Rounding nearest{(int)format, SRS_RULE_NEAREST, 0u};
+    Blocks tokens, tokens_t, matrix, matrix_t;
+    if (need_w) quantize_groups(x, ends, nearest, &tokens, &tokens_t);
+    else quantize(x, nearest, false, 0u, kRows, &tokens, nullptr);
+    quantize(weight, nearest, true, 0u, need_x ? kBoth : kRows, &matrix,
+             need_x ? &matrix_t : nullptr);
+    ctx->save_for_backward(
+        {ends, tokens_t.data, tokens_t.scale, matrix_t.data, matrix_t.scale});
+    ctx->saved_data["how"] = std::vector<int64_t>{grad_format, grad_rule, seed, need_x, need_w,
+                                                  (int64_t)x.scalar_type(),
+                                                  (int64_t)weight.scalar_type()};
+    return expert_matmul(tokens, matrix, ends, x.scalar_type(), format_of(x.scalar_type()));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("expert_linear");
+    const std::vector<int64_t> s = ctx->saved_data["how"].toIntVector();
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &dy = grads[0], &ends = saved[0];
+    const c10::cuda::OptionalCUDAGuard guard(dy.device());
+    const Rounding how{(int)s[0], (int)s[1], (uint32_t)s[2]};
+    const bool need_x = s[3] != 0, need_w = s[4] != 0;
+    const auto x_type = (at::ScalarType)s[5], w_type = (at::ScalarType)s[6];
+    Blocks rows, columns;
+    if (need_w) quantize_groups(dy, ends, how, need_x ? &rows : nullptr, &columns);
+    else quantize(dy, how, false, 0u, kRows, &rows, nullptr);
+    variable_list out(9);
+    if (need_x) out[0] = expert_matmul(rows, {saved[3], saved[4]}, ends, x_type, format_of(x_type));
+    if (need_w)
+      out[1] = expert_gradient(columns, {saved[1], saved[2]}, dy.size(0), ends, w_type,
+                               format_of(w_type));
+    return out;
+  }
+};
+
+// ----------------------------------------------------------------- adapters --
+
+struct Low {
+  at::Tensor values, largest;
+};
+
+// x (tokens, k) by the projection's blocks (undefined: the low part alone) and the adapters;
+// turned: x is the result's gradient.
+at::Tensor adapter_product(const at::Tensor& given, const Rounding& how, Blocks blocks,
+                           const at::Tensor& down, const at::Tensor& up, const at::Tensor& scale,
+                           double factor, const at::Tensor& order, const at::Tensor& ends,
+                           bool turned, Low* low) {
   const int64_t tokens = given.size(0), k = given.size(1);
-  Blocks blocks;
-  const bool project = w_obj != Py_None;
-  const int64_t n = tensor(turned ? down : up, "adapters").size(turned ? 2 : 1);
+  const bool project = blocks.data.defined();
+  TORCH_CHECK_VALUE(down.dim() == 3 && up.dim() == 3, "adapter_linear: down of shape ",
+                    down.sizes(), " and up of shape ", up.sizes(), " are not stacks of matrices");
+  const int64_t n = turned ? down.size(2) : up.size(1);
   if (project) {
-    blocks = {tensor(w_obj, "the weight's data"), tensor(w_scale, "the weight's scale")};
     TORCH_CHECK_VALUE(given.device() == blocks.data.device(),
                       "all tensors must be on the same CUDA device");
     TORCH_CHECK_VALUE(blocks.data.dim() == 2 && blocks.data.size(1) == k &&
@@ -468,81 +384,345 @@ PyObject* py_adapter_linear(PyObject*, PyObject* args) {
                       "adapter_linear: a weight of shape ", blocks.data.sizes(),
                       " does not fit a projection from ", k, " to ", n);
   }
-  Adapters a;
-  set_adapters(&a, given, turned ? n : k, turned ? k : n, down, up, scale, factor, order, ends);
+  const Adapters a = adapters_of(given, turned ? n : k, turned ? k : n, down, up, scale, factor,
+                                 order, ends);
   const at::Tensor x = aligned(given, false);
   srs_blocks matrix{};
-  int rc = project ? operand("weight", &blocks, &matrix) : SRS_OK;
-  at::Tensor out, low, largest;
-  if (rc == SRS_OK) {
-    if (project) out = at::empty({tokens, n}, x.options());
-    if (keep) {
-      low = at::empty({tokens, a.c.rank}, x.options().dtype(at::kFloat));
-      // (the sums of FP16 gradients are scaled by it)
-      if (a.c.format == SRS_FMT_F16)
-        largest = at::empty({a.c.count}, x.options().dtype(at::kInt));
-    }
-    const int64_t bytes =
-        g_adapter_workspace(tokens, k, project ? n : 0, a.c.count, a.c.rank);
-    const at::Tensor space = at::empty({bytes}, x.options().dtype(at::kByte));
-    if (tokens != 0)
-      rc = g_adapter_linear(
-          x.data_ptr(), tokens, k, step_of(x, 0, ceil_div(k, 8) * 8), format, rule, seed,
-          project ? &matrix : nullptr, &a.c, turned, project ? out.data_ptr() : nullptr,
-          keep ? static_cast<float*>(low.data_ptr()) : nullptr,
-          largest.defined() ? static_cast<uint32_t*>(largest.data_ptr()) : nullptr,
-          space.data_ptr(), bytes, stream_of(x));
+  if (project) check(operand("weight", &blocks, &matrix));
+  at::Tensor out;
+  if (project) out = at::empty({tokens, n}, x.options());
+  if (low != nullptr) {
+    low->values = at::empty({tokens, a.c.rank}, x.options().dtype(at::kFloat));
+    // (the sums of FP16 gradients are scaled by it)
+    if (a.c.format == SRS_FMT_F16)
+      low->largest = at::empty({a.c.count}, x.options().dtype(at::kInt));
   }
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
-  PyObject* result = PyTuple_New(3);
-  if (result == nullptr) return nullptr;
+  if (tokens == 0) return out;
+  const int64_t bytes = g_adapter_workspace(tokens, k, project ? n : 0, a.c.count, a.c.rank);
+  const at::Tensor space = at::empty({bytes}, x.options().dtype(at::kByte));
+  check(g_adapter_linear(
+      x.data_ptr(), tokens, k, step_of(x, 0, ceil_div(k, 8) * 8), how.format, how.rule, how.seed,
+      project ? &matrix : nullptr, &a.c, turned, project ? out.data_ptr() : nullptr,
+      low != nullptr ? static_cast<float*>(low->values.data_ptr()) : nullptr,
+      low != nullptr && low->largest.defined() ? static_cast<uint32_t*>(low->largest.data_ptr())
+                                               : nullptr,
+      space.data_ptr(), bytes, stream_of(x)));
+  return out;
+}
+
+// Sums over the tokens of each adapter of z (tokens, cols) by low: (adapters, rank, cols) or,
+// turned, (adapters, cols, rank).
+at::Tensor adapter_gradient(const at::Tensor& given, const Low& low, const at::Tensor& order,
+                            const at::Tensor& ends, bool turned) {
+  const at::Tensor z = aligned(given, false);
+  const int64_t tokens = z.size(0), cols = z.size(1), rank = low.values.size(1);
+  const int64_t count = ends.numel();
+  at::Tensor out = turned ? at::empty({count, cols, rank}, z.options())
+                          : at::empty({count, rank, cols}, z.options());
+  if (out.numel() == 0) return out;
+  const int64_t bytes = g_gradient_workspace(tokens, cols, (int)count, (int)rank);
+  const at::Tensor space = at::empty({bytes}, z.options().dtype(at::kByte));
+  check(g_adapter_gradient(
+      z.data_ptr(), format_of(z.scalar_type()), tokens, cols, step_of(z, 0, ceil_div(cols, 8) * 8),
+      static_cast<const float*>(low.values.data_ptr()),
+      low.largest.defined() ? static_cast<const uint32_t*>(low.largest.data_ptr()) : nullptr,
+      (int)count, (int)rank, ints(order), ints(ends), turned, out.data_ptr(), space.data_ptr(),
+      bytes, stream_of(z)));
+  return out;
+}
+
+at::Tensor flat(const at::Tensor& x) {
+  return x.dim() == 2 ? x : x.dim() == 1 ? x.unsqueeze(0) : x.flatten(0, -2);
+}
+
+at::Tensor shaped(const at::Tensor& rows, at::IntArrayRef like) {
+  if (like.size() == 2) return rows;
+  std::vector<int64_t> sizes(like.begin(), like.end());
+  sizes.back() = rows.size(1);
+  return rows.reshape(sizes);
+}
+
+// What of a call is no leaf.
+struct AdapterInputs {
+  Blocks kept, turned;  // undefined: the weight itself is given
+  at::Tensor scale, order, ends;
+  double factor;
+  int format;
+  Rounding grad;
+  std::vector<int64_t> need;  // gradients of x, weight, down, up
+};
+
+struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
+  enum { kX, kDown, kUp, kScale, kOrder, kEnds, kLow, kLargest, kMatrix, kMatrixScale, kTokens,
+         kTokensScale };
+
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x,
+                            const std::optional<at::Tensor>& weight, const at::Tensor& down,
+                            const at::Tensor& up, const AdapterInputs& in) {
+    const Rounding nearest{in.format, SRS_RULE_NEAREST, 0u};
+    const std::vector<int64_t>& need = in.need;
+    Blocks matrix = in.kept, matrix_t = in.turned, tokens_t;
+    const at::Tensor rows = flat(x);
+    if (weight.has_value()) {
+      matrix_t = {};
+      quantize(*weight, nearest, true, 0u, need[0] ? kBoth : kRows, &matrix,
+               need[0] ? &matrix_t : nullptr);
+    }
+    Low low;
+    const at::Tensor y = adapter_product(rows, nearest, matrix, down, up, in.scale, in.factor,
+                                         in.order, in.ends, false, need[3] ? &low : nullptr);
+    if (need[1]) quantize(rows, nearest, false, 0u, kColumns, nullptr, &tokens_t);
+    if (!need[0]) matrix_t = {};
+    ctx->save_for_backward({need[2] ? rows : at::Tensor(), down, up, in.scale, in.order, in.ends,
+                            low.values, low.largest, matrix_t.data, matrix_t.scale, tokens_t.data,
+                            tokens_t.scale});
+    ctx->saved_data["need"] = need;
+    ctx->saved_data["how"] = std::vector<int64_t>{
+        in.grad.format, in.grad.rule, (int64_t)in.grad.seed,
+        (int64_t)(weight.has_value() ? weight->scalar_type() : at::kFloat)};
+    ctx->saved_data["factor"] = in.factor;
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    return shaped(y, x.sizes());
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("adapter_linear");
+    const std::vector<int64_t> need = ctx->saved_data["need"].toIntVector();
+    const std::vector<int64_t> s = ctx->saved_data["how"].toIntVector();
+    const double factor = ctx->saved_data["factor"].toDouble();
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor dy = flat(grads[0]);
+    const c10::cuda::OptionalCUDAGuard guard(dy.device());
+    const Rounding how{(int)s[0], (int)s[1], (uint32_t)s[2]};
+    const at::Tensor &order = saved[kOrder], &ends = saved[kEnds];
+    variable_list out(5);
+    if (need[0] || need[2]) {
+      Low back;
+      const at::Tensor dx =
+          adapter_product(dy, how, {saved[kMatrix], saved[kMatrixScale]}, saved[kDown], saved[kUp],
+                          saved[kScale], factor, order, ends, true, need[2] ? &back : nullptr);
+      if (need[0]) out[0] = shaped(dx, ctx->saved_data["sizes"].toIntVector());
+      if (need[2]) out[2] = adapter_gradient(saved[kX], back, order, ends, false);
+    }
+    if (need[3])
+      out[3] = adapter_gradient(dy, {saved[kLow], saved[kLargest]}, order, ends, true);
+    if (need[1]) {
+      const auto type = (at::ScalarType)s[3];
+      Blocks columns, tokens{saved[kTokens], saved[kTokensScale]};
+      quantize(dy, how, false, 0u, kColumns, nullptr, &columns);
+      srs_blocks left{}, right{};
+      check(operand("a", &columns, &left));
+      check(operand("b", &tokens, &right));
+      out[1] = at::empty({left.rows, right.rows}, dy.options().dtype(type));
+      if (out[1].numel() != 0)
+        check(g_matmul(&left, &right, dy.size(0), out[1].data_ptr(), format_of(type),
+                       stream_of(dy)));
+    }
+    return out;
+  }
+};
+
+// ------------------------------------------------------------------- module --
+
+at::Tensor optional(PyObject* obj, const char* what) {
+  return obj == Py_None ? at::Tensor() : tensor(obj, what);
+}
+
+PyObject* wrap(std::initializer_list<at::Tensor> tensors) {
+  PyObject* out = PyTuple_New((Py_ssize_t)tensors.size());
+  if (out == nullptr) return nullptr;
   Py_ssize_t i = 0;
-  for (const at::Tensor* t : {&out, &low, &largest}) {
-    if (t->defined()) {
-      PyTuple_SET_ITEM(result, i++, THPVariable_Wrap(*t));
-    } else {
-      Py_INCREF(Py_None);
-      PyTuple_SET_ITEM(result, i++, Py_None);
-    }
+  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+
+template <class F>
+bool bind_one(PyObject* table, const char* name, F* to) {
+  PyObject* address = PyDict_GetItemString(table, name);
+  if (address == nullptr) {
+    PyErr_Format(PyExc_KeyError, "%s", name);
+    return false;
   }
-  return result;
+  const unsigned long long at = PyLong_AsUnsignedLongLong(address);
+  if (PyErr_Occurred()) return false;
+  *to = reinterpret_cast<F>(static_cast<uintptr_t>(at));
+  return true;
+}
+
+PyObject* py_bind(PyObject*, PyObject* args) {
+  PyObject* t;
+  if (!PyArg_ParseTuple(args, "O!", &PyDict_Type, &t)) return nullptr;
+  if (!bind_one(t, "srs_last_error", &g_last_error) ||
+      !bind_one(t, "srs_group_rows", &g_group_rows) ||
+      !bind_one(t, "srs_quantize_stack", &g_quantize_stack) ||
+      !bind_one(t, "srs_quantize_groups", &g_quantize_groups) ||
+      !bind_one(t, "srs_group_columns", &g_group_columns) ||
+      !bind_one(t, "srs_group_scales", &g_group_scales) ||
+      !bind_one(t, "srs_matmul_blocks", &g_matmul) ||
+      !bind_one(t, "srs_expert_matmul", &g_expert_matmul) ||
+      !bind_one(t, "srs_expert_linear", &g_expert_linear) ||
+      !bind_one(t, "srs_expert_gradient", &g_expert_gradient) ||
+      !bind_one(t, "srs_linear_workspace", &g_linear_workspace) ||
+      !bind_one(t, "srs_adapter_workspace", &g_adapter_workspace) ||
+      !bind_one(t, "srs_adapter_linear", &g_adapter_linear) ||
+      !bind_one(t, "srs_adapter_gradient_workspace", &g_gradient_workspace) ||
+      !bind_one(t, "srs_adapter_gradient", &g_adapter_gradient) ||
+      !bind_one(t, "srs_copy_rows", &g_copy_rows))
+    return nullptr;
+  Py_RETURN_NONE;
+}
+
+PyObject* py_group_rows(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject* obj;
+  int groups;
+  if (!PyArg_ParseTuple(args, "Oi", &obj, &groups)) return nullptr;
+  c10::NoGradGuard no_grad;
+  const at::Tensor& index = tensor(obj, "index");
+  const c10::cuda::OptionalCUDAGuard guard(index.device());
+  TORCH_CHECK_TYPE(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong,
+                   "group_rows: indices are int32 or int64, got ", index.scalar_type());
+  TORCH_CHECK_VALUE(groups > 0, "group_rows: groups must be positive, got ", groups);
+  const at::Tensor given = index.contiguous();
+  const auto options = index.options().dtype(at::kInt);
+  at::Tensor order = at::empty({index.numel()}, options), ends = at::empty({groups}, options);
+  check(g_group_rows(given.data_ptr(), (int)index.element_size(), index.numel(), groups,
+                     static_cast<int32_t*>(order.data_ptr()),
+                     static_cast<int32_t*>(ends.data_ptr()), stream_of(index)));
+  return wrap({order, ends});
   END_HANDLE_TH_ERRORS
 }
 
-// Sums over the tokens of each adapter of z (tokens, cols) by low: (count, rank, cols) or,
-// turned, (count, cols, rank).
-PyObject* py_adapter_gradient(PyObject*, PyObject* args) {
+PyObject* py_quantize_stack(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
-  PyObject *z_obj, *low_obj, *largest_obj, *order_obj, *ends_obj;
-  int turned;
-  if (!PyArg_ParseTuple(args, "OOOOOi", &z_obj, &low_obj, &largest_obj, &order_obj, &ends_obj,
-                        &turned))
+  PyObject* obj;
+  int format, rule, square, orientation;
+  unsigned int seed, offset;
+  if (!PyArg_ParseTuple(args, "OiiiIIi", &obj, &format, &rule, &square, &seed, &offset,
+                        &orientation))
     return nullptr;
   c10::NoGradGuard no_grad;
-  const at::Tensor& given = tensor(z_obj, "z");
-  const c10::cuda::OptionalCUDAGuard guard(given.device());
-  const at::Tensor &low = tensor(low_obj, "low");
-  const at::Tensor ends = checked_ends(tensor(ends_obj, "ends"), given, "adapter_linear");
-  const at::Tensor order = tensor(order_obj, "order").to(at::kInt).contiguous();
-  const at::Tensor z = aligned(given, false);
-  const int64_t tokens = z.size(0), cols = z.size(1), rank = low.size(1), count = ends.numel();
-  at::Tensor out = turned ? at::empty({count, cols, rank}, z.options())
-                          : at::empty({count, rank, cols}, z.options());
-  const int64_t bytes = g_gradient_workspace(tokens, cols, (int)count, (int)rank);
-  const at::Tensor space = at::empty({bytes}, z.options().dtype(at::kByte));
-  int rc = SRS_OK;
-  if (out.numel() != 0)
-    rc = g_adapter_gradient(
-        z.data_ptr(), z.scalar_type() == at::kBFloat16 ? SRS_FMT_BF16 : SRS_FMT_F16, tokens, cols,
-        step_of(z, 0, ceil_div(cols, 8) * 8), static_cast<const float*>(low.data_ptr()),
-        largest_obj != Py_None
-            ? static_cast<const uint32_t*>(tensor(largest_obj, "largest").data_ptr())
-            : nullptr,
-        (int)count, (int)rank, static_cast<const int32_t*>(order.data_ptr()),
-        static_cast<const int32_t*>(ends.data_ptr()), turned, out.data_ptr(), space.data_ptr(),
-        bytes, stream_of(z));
-  if (rc != SRS_OK) return PyLong_FromLong(rc);
+  const at::Tensor& x = tensor(obj, "x");
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  TORCH_CHECK_VALUE(x.dim() == 3, "a stack of matrices has three dimensions, got shape ",
+                    x.sizes());
+  Blocks straight, turned;
+  quantize(x, {format, rule, seed}, square != 0, offset, orientation, &straight, &turned);
+  if (orientation == kBoth)
+    return wrap({straight.data, straight.scale, turned.data, turned.scale});
+  const Blocks& one = orientation == kRows ? straight : turned;
+  return wrap({one.data, one.scale});
+  END_HANDLE_TH_ERRORS
+}
+
+// weight: the experts' matrices, or (with w_scale) their blocks.
+PyObject* py_expert_linear(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *x_obj, *w_obj, *w_scale, *ends_obj;
+  int format, grad_format, grad_rule;
+  unsigned int seed;
+  if (!PyArg_ParseTuple(args, "OOOOiiiI", &x_obj, &w_obj, &w_scale, &ends_obj, &format,
+                        &grad_format, &grad_rule, &seed))
+    return nullptr;
+  const at::Tensor &x = tensor(x_obj, "x"), &weight = tensor(w_obj, "weight");
+  const bool kept = w_scale != Py_None;
+  TORCH_CHECK_VALUE(x.dim() == 2 && weight.dim() == 3 && x.size(1) == weight.size(2),
+                    "x of shape ", x.sizes(), " does not fit expert weights of shape ",
+                    weight.sizes());
+  const at::Tensor& given = tensor(ends_obj, "ends");
+  TORCH_CHECK_VALUE(given.dim() == 1 && given.size(0) == weight.size(0), "ends of shape ",
+                    given.sizes(), " do not fit ", weight.size(0), " experts");
+  TORCH_CHECK_VALUE(x.device() == weight.device(), "all tensors must be on the same CUDA device");
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const int x_format = source_format(x, "expert_linear");
+  if (!kept) source_format(weight, "expert_linear");
+  const bool grad = at::GradMode::is_enabled();
+  const bool need_x = grad && x.requires_grad(), need_w = grad && !kept && weight.requires_grad();
+  at::Tensor ends;
+  {
+    c10::NoGradGuard no_grad;
+    ends = checked_ends(given, x, "expert_linear");
+  }
+  if (need_x || need_w) {
+    TORCH_CHECK_VALUE(!kept,
+                      "a BlockTensor weight has no backward pass; pass the weight itself or run "
+                      "under torch.no_grad()");
+    return THPVariable_Wrap(ExpertLinear::apply(x, weight, ends, (int64_t)format,
+                                                (int64_t)grad_format, (int64_t)grad_rule,
+                                                (int64_t)seed, need_x, need_w));
+  }
+  c10::NoGradGuard no_grad;
+  Blocks w{weight, kept ? tensor(w_scale, "the weight's scale") : at::Tensor()};
+  if (!kept) quantize(weight, {format, SRS_RULE_NEAREST, 0u}, true, 0u, kRows, &w, nullptr);
+  const srs_blocks matrix = stack_operand("weight", &w);
+  const int64_t rows = x.size(0), k = x.size(1);
+  const at::Tensor src = x.stride(1) != 1 && k > 1 ? x.contiguous() : x;
+  at::Tensor out = at::empty({rows, weight.size(1)}, x.options());
+  if (out.numel() != 0) {
+    const int64_t bytes = g_linear_workspace(rows, k);
+    const at::Tensor space = at::empty({bytes}, x.options().dtype(at::kByte));
+    check(g_expert_linear(src.data_ptr(), x_format, rows, k, src.stride(0), format, &matrix,
+                          (int)ends.numel(), ints(ends), out.data_ptr(), space.data_ptr(), bytes,
+                          stream_of(x)));
+  }
   return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// weight: the projection's matrix, or None with its blocks (and those of its transpose).
+PyObject* py_adapter_linear(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *x_obj, *w_obj, *kept_obj, *kept_scale, *turned_obj, *turned_scale, *down_obj, *up_obj;
+  PyObject *scale_obj, *order_obj, *ends_obj;
+  double factor;
+  int format, grad_format, grad_rule;
+  unsigned int seed;
+  if (!PyArg_ParseTuple(args, "OOOOOOOOOdOOiiiI", &x_obj, &w_obj, &kept_obj, &kept_scale,
+                        &turned_obj, &turned_scale, &down_obj, &up_obj, &scale_obj, &factor,
+                        &order_obj, &ends_obj, &format, &grad_format, &grad_rule, &seed))
+    return nullptr;
+  const at::Tensor &x = tensor(x_obj, "x"), &down = tensor(down_obj, "down");
+  const at::Tensor& up = tensor(up_obj, "up");
+  const at::Tensor weight = optional(w_obj, "weight"), scale = optional(scale_obj, "scale");
+  const at::Tensor &order = tensor(order_obj, "order"), &ends = tensor(ends_obj, "ends");
+  Blocks kept{optional(kept_obj, "the weight's data"), optional(kept_scale, "the weight's scale")};
+  const Blocks turned{optional(turned_obj, "the transpose's data"),
+                      optional(turned_scale, "the transpose's scale")};
+  const at::Tensor& matrix = weight.defined() ? weight : kept.data;
+  TORCH_CHECK_VALUE(x.dim() > 0, "adapter_linear needs at least one dimension");
+  TORCH_CHECK_VALUE(matrix.dim() == 2 && x.size(-1) == matrix.size(1), "x of shape ", x.sizes(),
+                    " does not fit a weight of shape ", matrix.sizes());
+  TORCH_CHECK_VALUE(x.device() == matrix.device(), "all tensors must be on the same CUDA device");
+  if (turned.data.defined())
+    TORCH_CHECK_VALUE(turned.data.dim() == 2 && turned.data.size(0) == matrix.size(1) &&
+                          turned.data.size(1) == matrix.size(0),
+                      "blocks of shapes ", matrix.sizes(), " and ", turned.data.sizes(),
+                      " are not of a matrix and its transpose");
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const bool grad = at::GradMode::is_enabled();
+  const std::vector<int64_t> need{grad && x.requires_grad(),
+                                  grad && weight.defined() && weight.requires_grad(),
+                                  grad && down.requires_grad(), grad && up.requires_grad()};
+  if (need[0] || need[1] || need[2] || need[3]) {
+    TORCH_CHECK_VALUE(!need[0] || weight.defined() || turned.data.defined(),
+                      "a BlockTensor weight has no backward pass; pass the blocks of both "
+                      "orientations or the weight itself, or run under torch.no_grad()");
+    AdapterInputs in{kept, turned, scale, {}, {}, factor, format, {grad_format, grad_rule, seed},
+                     need};
+    {
+      c10::NoGradGuard no_grad;
+      in.order = order.to(at::kInt);
+      in.ends = checked_ends(ends, x, "adapter_linear");
+    }
+    return THPVariable_Wrap(AdapterLinear::apply(
+        x, weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt, down, up, in));
+  }
+  c10::NoGradGuard no_grad;
+  const Rounding nearest{format, SRS_RULE_NEAREST, 0u};
+  if (weight.defined()) quantize(weight, nearest, true, 0u, kRows, &kept, nullptr);
+  const at::Tensor y = adapter_product(flat(x), nearest, kept, down, up, scale, factor, order, ends,
+                                       false, nullptr);
+  return THPVariable_Wrap(shaped(y, x.sizes()));
   END_HANDLE_TH_ERRORS
 }
 
@@ -551,19 +731,11 @@ PyMethodDef kMethods[] = {
     {"group_rows", py_group_rows, METH_VARARGS, "group_rows(index, groups) -> order, ends."},
     {"quantize_stack", py_quantize_stack, METH_VARARGS,
      "quantize_stack(x, format, rule, square, seed, offset, orientation) -> tensors."},
-    {"quantize_groups", py_quantize_groups, METH_VARARGS,
-     "quantize_groups(x, ends, format, rule, seed, rows) -> tensors."},
-    {"expert_matmul", py_expert_matmul, METH_VARARGS,
-     "expert_matmul(a, a_scale, w, w_scale, ends, format) -> tensor."},
     {"expert_linear", py_expert_linear, METH_VARARGS,
-     "expert_linear(x, w, w_scale, ends, format) -> tensor."},
-    {"expert_gradient", py_expert_gradient, METH_VARARGS,
-     "expert_gradient(a_t, a_scale, b_t, b_scale, rows, ends, format) -> tensor."},
+     "expert_linear(x, weight, w_scale, ends, format, grad_format, grad_rule, seed) -> tensor."},
     {"adapter_linear", py_adapter_linear, METH_VARARGS,
-     "adapter_linear(x, format, rule, seed, w, w_scale, down, up, scale, factor, order, ends, "
-     "turned, keep) -> (d, low, largest)."},
-    {"adapter_gradient", py_adapter_gradient, METH_VARARGS,
-     "adapter_gradient(z, low, largest, order, ends, turned) -> tensor."},
+     "adapter_linear(x, weight, kept, kept_scale, turned, turned_scale, down, up, scale, factor, "
+     "order, ends, format, grad_format, grad_rule, seed) -> tensor."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_srs_groups",

@@ -430,43 +430,25 @@ class NativeLauncher:
         got = blocks_module().linear(x, w, w_scale, fmt)
         return got if type(got) is not int else _check(got)
 
+    # The front end of the operators on rows in groups raises the entry points' errors itself.
     def quantize_stack(self, x, fmt, rule, square, seed, offset, orientation):
         """As quantize_blocks, of every matrix of a stack."""
-        got = groups_module().quantize_stack(x, fmt, rule, square, seed, offset, orientation)
-        return got if type(got) is tuple else _check(got)
+        return groups_module().quantize_stack(x, fmt, rule, square, seed, offset, orientation)
 
     def group_rows(self, index, groups):
-        got = groups_module().group_rows(index, groups)
-        return got if type(got) is tuple else _check(got)
+        return groups_module().group_rows(index, groups)
 
-    def quantize_groups(self, x, ends, fmt, rule, seed, rows):
-        """(data, scale) of the transposed copy for expert_gradient, with ``rows`` behind those
-        of the copy by rows."""
-        got = groups_module().quantize_groups(x, ends, fmt, rule, seed, rows)
-        return got if type(got) is tuple else _check(got)
+    def expert_linear(self, x, weight, w_scale, ends, fmt, grad_fmt, grad_rule, seed):
+        """``weight``: the experts' matrices, or (with ``w_scale``) their blocks."""
+        return groups_module().expert_linear(x, weight, w_scale, ends, fmt, grad_fmt, grad_rule,
+                                             seed)
 
-    def expert_matmul(self, a, a_scale, w, w_scale, ends, fmt):
-        got = groups_module().expert_matmul(a, a_scale, w, w_scale, ends, fmt)
-        return got if type(got) is not int else _check(got)
-
-    def expert_linear(self, x, w, w_scale, ends, fmt):
-        got = groups_module().expert_linear(x, w, w_scale, ends, fmt)
-        return got if type(got) is not int else _check(got)
-
-    def expert_gradient(self, a_t, a_scale, b_t, b_scale, rows, ends, fmt):
-        got = groups_module().expert_gradient(a_t, a_scale, b_t, b_scale, rows, ends, fmt)
-        return got if type(got) is not int else _check(got)
-
-    def adapter_linear(self, x, fmt, rule, seed, w, w_scale, down, up, scale, factor, order, ends,
-                       turned, keep):
-        """(result, low part, its largest values); with ``w`` None the low part alone."""
-        got = groups_module().adapter_linear(x, fmt, rule, seed, w, w_scale, down, up, scale,
-                                             factor, order, ends, turned, keep)
-        return got if type(got) is tuple else _check(got)
-
-    def adapter_gradient(self, z, low, largest, order, ends, turned):
-        got = groups_module().adapter_gradient(z, low, largest, order, ends, turned)
-        return got if type(got) is not int else _check(got)
+    def adapter_linear(self, x, weight, kept, turned, down, up, scale, factor, order, ends, fmt,
+                       grad_fmt, grad_rule, seed):
+        """``weight``: the projection's matrix, or None with its blocks ``kept`` (data, scale) and
+        those of its transpose."""
+        return groups_module().adapter_linear(x, weight, *kept, *turned, down, up, scale, factor,
+                                              order, ends, fmt, grad_fmt, grad_rule, seed)
 
     def product_status(self) -> int:
         """Where a bounded wait of a product kernel ran out since the last call (0: nowhere);

@@ -11,45 +11,10 @@ from __future__ import annotations
 import torch
 
 from .blocks import BlockLayer
-from .cuda.blocks import BLOCK, BlockTensor, check_blocks, quantize_blocks, quantize_stack
-from .cuda.groups import expert_blocks, expert_gradient, expert_matmul, quantize_groups
+from .cuda import _native
+from .cuda.blocks import BLOCK, BlockTensor, check_blocks, quantize_stack
 
 __all__ = ["BlockExperts", "expert_linear"]
-
-
-class _ExpertLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, ends, dtype, grad_dtype, grad_rounding, seed, need_x, need_w):
-        tokens_t = matrix_t = None
-        if need_w:
-            tokens, tokens_t = quantize_groups(x, ends, dtype=dtype, rows=True)
-        else:
-            tokens = quantize_blocks(x, dtype=dtype)
-        matrix = quantize_stack(weight, dtype=dtype, block=(BLOCK, BLOCK),
-                                orientation="both" if need_x else "rows")
-        matrix, matrix_t = matrix if need_x else (matrix, None)
-        ctx.save_for_backward(ends, *(tokens_t or ()), *(matrix_t or ()))
-        ctx.settings = (grad_dtype, grad_rounding, seed, x.dtype, weight.dtype, need_x, need_w)
-        return expert_matmul(tokens, matrix, ends, dtype=x.dtype)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        grad_dtype, rounding, seed, x_dtype, w_dtype, need_x, need_w = ctx.settings
-        ends, *saved = ctx.saved_tensors
-        tokens_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_w else None
-        matrix_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_x else None
-        how = {"dtype": grad_dtype, "rounding": rounding, "seed": seed}
-        rows = columns = None
-        if need_w:
-            got = quantize_groups(dy, ends, rows=need_x, **how)
-            rows, columns = got if need_x else (None, got)
-        elif need_x:
-            rows = quantize_blocks(dy, **how)
-        dx = expert_matmul(rows, matrix_t, ends, dtype=x_dtype) if need_x else None
-        dw = (expert_gradient(columns, tokens_t, dy.shape[0], ends, dtype=w_dtype)
-              if need_w else None)
-        return dx, dw, None, None, None, None, None, None, None
 
 
 def expert_linear(x, weight, ends, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float8_e4m3fn,
@@ -63,21 +28,13 @@ def expert_linear(x, weight, ends, *, dtype=torch.float8_e4m3fn, grad_dtype=torc
     differentiable in ``x`` and ``weight``), or a BlockTensor kept from ``quantize_stack``
     (inference).  The rest as for ``block_linear``.  At most 2^22 rows and 2^30 rows of weights.
     """
-    stack = (weight.data if isinstance(weight, BlockTensor) else weight).shape
-    if x.dim() != 2 or len(stack) != 3 or x.shape[1] != stack[2]:
-        raise ValueError(f"x of shape {tuple(x.shape)} does not fit expert weights of shape "
-                         f"{tuple(stack)}")
-    if ends.dim() != 1 or ends.shape[0] != stack[0]:
-        raise ValueError(f"ends of shape {tuple(ends.shape)} do not fit {stack[0]} experts")
-    if isinstance(weight, BlockTensor):
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise ValueError("a BlockTensor weight has no backward pass; pass the weight itself "
-                             "or run under torch.no_grad()")
-        return expert_blocks(x, weight, ends, dtype)
-    check_blocks(grad_dtype, grad_rounding)
-    grad = torch.is_grad_enabled()
-    return _ExpertLinear.apply(x, weight, ends, dtype, grad_dtype, grad_rounding, seed,
-                               grad and x.requires_grad, grad and weight.requires_grad)
+    fmt, _ = check_blocks(dtype, "nearest")
+    grad_fmt, grad_rule = check_blocks(grad_dtype, grad_rounding)
+    launcher = _native.launcher()
+    launcher.check_device(x.device, "expert_linear")
+    weight, scale = weight if isinstance(weight, BlockTensor) else (weight, None)
+    return launcher.expert_linear(x, weight, scale, ends, fmt, grad_fmt, grad_rule,
+                                  int(seed) & 0xFFFFFFFF)
 
 
 class BlockExperts(BlockLayer):
