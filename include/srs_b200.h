@@ -436,8 +436,8 @@ int srs_group_rows(const void* index, int index_bytes, int64_t rows, int groups,
 
 /* FP8 blocks of a matrix whose rows are in groups, for srs_expert_gradient: the transposed copy
  * in blocks of 128 rows counted from each group's first, srs_group_columns(rows, groups)
- * columns of data and srs_group_scales(rows, groups) of scales (a layout of the library's
- * own); beside it, on demand, the copy by rows.  Rows of no group are not written.  Counters are
+ * columns of data and srs_group_scales(rows, groups) scales a row (a layout of the library's
+ * own, at a multiple of 4 bytes); beside it, on demand, the copy by rows.  Rows of no group are not written.  Counters are
  * those of srs_quantize_blocks. */
 int64_t srs_group_columns(int64_t rows, int groups);
 int64_t srs_group_scales(int64_t rows, int groups);

@@ -264,7 +264,7 @@ void quantize_groups(const at::Tensor& x, const at::Tensor& ends, const Rounding
   turned->data = at::empty({cols, g_group_columns(height, groups)},
                            x.options().dtype(how.format == SRS_FMT_E4M3 ? at::kFloat8_e4m3fn
                                                                         : at::kFloat8_e5m2));
-  turned->scale = at::empty({cols, ceil_div(g_group_scales(height, groups), 4) * 4},
+  turned->scale = at::empty({cols, g_group_scales(height, groups)},
                             x.options().dtype(at::kFloat8_e8m0fnu));
   if (x.numel() == 0) return;
   const srs_block_copy copy = straight != nullptr ? copy_of(*straight) : srs_block_copy{};

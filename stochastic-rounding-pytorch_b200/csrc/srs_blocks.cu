@@ -37,8 +37,8 @@ struct QuantizeArgs {
 // What a tile kernel's grid covers: one matrix; a stack of them (blockIdx.z), whose counters
 // go on from one to the next; or the rows of groups, tiles counted from a group's first
 // row.  The transposed copy of groups has the columns of tile i of all groups' tiles at
-// 128 i, zeros behind a group's last row, and a group's scales start at a multiple of 4
-// columns (products read them by words): rows of no group are not written.
+// 128 i, zeros behind a group's last row; its scales are words of 4 blocks, the words of all its
+// rows one after the other, and a group starts with a new word.  Rows of no group are not written.
 enum : int { kMatrix = 0, kStack = 1, kGroups = 2 };
 
 // k of a block whose largest finite |x| has FP32 encoding u: the largest values of
@@ -402,7 +402,9 @@ quantize_tile_kernel(const __grid_constant__ QuantizeArgs args) {
           const int k = block_exponent<OF>(Z::as_f32(col_top[j]));
           col_factor[j] = power_of_two(-k);
           if (group == 0 && col + j < a.cols)
-            a.scale_t[(col + j) * a.scale_t_pitch + scale_t_at] = (uint8_t)(k + 127);
+            a.scale_t[COVER == kGroups
+                          ? ((scale_t_at >> 2) * a.cols + col + j) * 4 + (scale_t_at & 3)
+                          : (col + j) * a.scale_t_pitch + scale_t_at] = (uint8_t)(k + 127);
         }
       }
     }
@@ -734,10 +736,9 @@ extern "C" int64_t srs_group_columns(int64_t rows, int groups) {
 }
 
 extern "C" int64_t srs_group_scales(int64_t rows, int groups) {
-  // every group with rows takes a multiple of 4 columns
-  return rows <= 0 || groups <= 0
-             ? 0
-             : most_group_tiles(rows, groups, kBlock) + 3 * (groups < rows ? groups : rows);
+  // every group with rows takes a multiple of 4
+  if (rows <= 0 || groups <= 0) return 0;
+  return (most_group_tiles(rows, groups, kBlock) + 3 * (groups < rows ? groups : rows) + 3) / 4 * 4;
 }
 
 extern "C" int srs_quantize_groups(const void* x, int x_format, int64_t rows, int64_t cols,
