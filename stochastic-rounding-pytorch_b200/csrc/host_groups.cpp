@@ -144,8 +144,13 @@ at::Tensor aligned(const at::Tensor& t, bool whole) {
   if (good || t.numel() == 0) return t;
   std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
   sizes[last] = ceil_div(cols, 8) * 8;
-  at::Tensor copy = at::empty(sizes, t.options()).narrow(last, 0, cols);
-  copy.copy_(t);
+  const at::Tensor wide = at::empty(sizes, t.options());
+  at::Tensor copy = sizes[last] == cols ? wide : wide.narrow(last, 0, cols);
+  if (t.is_contiguous())
+    check(g_copy_rows(t.data_ptr(), 2 * cols, t.numel() / cols, 2 * cols, wide.data_ptr(),
+                      2 * sizes[last], stream_of(t)));
+  else
+    copy.copy_(t);
   return copy;
 }
 
@@ -469,11 +474,13 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
                need[0] ? &matrix_t : nullptr);
     }
     Low low;
-    const at::Tensor y = adapter_product(rows, nearest, matrix, down, up, in.scale, in.factor,
+    // (a copy that the kernels' alignment asks for is made once for both passes)
+    const at::Tensor x_rows = aligned(rows, false), a = aligned(down, false), b = aligned(up, true);
+    const at::Tensor y = adapter_product(x_rows, nearest, matrix, a, b, in.scale, in.factor,
                                          in.order, in.ends, false, need[3] ? &low : nullptr);
     if (need[1]) quantize(rows, nearest, false, 0u, kColumns, nullptr, &tokens_t);
     if (!need[0]) matrix_t = {};
-    ctx->save_for_backward({need[2] ? rows : at::Tensor(), down, up, in.scale, in.order, in.ends,
+    ctx->save_for_backward({need[2] ? x_rows : at::Tensor(), a, b, in.scale, in.order, in.ends,
                             low.values, low.largest, matrix_t.data, matrix_t.scale, tokens_t.data,
                             tokens_t.scale});
     ctx->saved_data["need"] = need;
@@ -491,7 +498,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     const std::vector<int64_t> s = ctx->saved_data["how"].toIntVector();
     const double factor = ctx->saved_data["factor"].toDouble();
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor dy = flat(grads[0]);
+    const at::Tensor dy = aligned(flat(grads[0]), false);
     const c10::cuda::OptionalCUDAGuard guard(dy.device());
     const Rounding how{(int)s[0], (int)s[1], (uint32_t)s[2]};
     const at::Tensor &order = saved[kOrder], &ends = saved[kEnds];

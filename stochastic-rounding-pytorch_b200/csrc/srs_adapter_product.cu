@@ -46,10 +46,11 @@ struct AdapterPlan {
 __device__ __forceinline__ void plan_adapters(AdapterPlan& p, const int32_t* ends, int adapters,
                                               int rows) {
   const int lane = threadIdx.x & 31;
+  const EndsAhead ahead(ends, adapters, lane);
   int carry = 0, count = 0;
   for (int base = 0; base < adapters; base += 32) {
     int start, end;
-    group_span(ends, adapters, rows, base, lane, &carry, &start, &end);
+    group_span(ends, ahead, adapters, rows, base, lane, &carry, &start, &end);
     const unsigned some = __ballot_sync(0xFFFFFFFFu, end > start);
     if (end > start) {
       const int at = count + __popc(some & ((1u << lane) - 1u));

@@ -132,6 +132,7 @@ struct LowArgs {
   float* low;             // tokens (in order) x rank (null: not wanted)
   uint16_t* pairs;        // items for a large product (null: not wanted)
   int edge, pitch, rest_at;
+  bool spread;            // items of a thin product: rows are the batch's
   unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
 };
 
@@ -283,8 +284,10 @@ low_kernel(const LowArgs a) {
     }
     if (a.pairs != nullptr) {
       const int place = tile.row0 + t;
-      uint16_t* const to = a.pairs + ((int64_t)(place / a.edge + tile.rank) * a.edge +
-                                      place % a.edge) * a.pitch + rank0 + r;
+      const int64_t at =
+          a.spread ? (int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)
+                   : (int64_t)(place / a.edge + tile.rank) * a.edge + place % a.edge;
+      uint16_t* const to = a.pairs + at * a.pitch + rank0 + r;
       const uint32_t high = encode16<F>(v);
       const float left = v - decode16<F>(high);
       to[0] = (uint16_t)high;
@@ -294,6 +297,19 @@ low_kernel(const LowArgs a) {
   if (a.pairs != nullptr) {
     // zeros in the rows of the adapter's first and last item that are not its own
     const int words = whole / 2;
+    // (spread: in those of all tokens that are not this adapter's)
+    if (a.spread && tile.row0 == tile.start) {
+      const int others = a.tokens - (tile.end - tile.start);
+      for (int i = threadIdx.x + S::kThreads * (int)split; i < others * words;
+           i += S::kThreads * (int)splits) {
+        const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
+        uint16_t* const p =
+            a.pairs + ((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)) * a.pitch +
+            rank0 + 2 * (i % words);
+        *reinterpret_cast<uint32_t*>(p) = 0u;
+        *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
+      }
+    }
     const auto clear = [&](int item, int from_row, int to_row) {
       const int rows = to_row - from_row;
       for (int i = threadIdx.x + S::kThreads * (int)split; i < rows * words;
@@ -304,9 +320,9 @@ low_kernel(const LowArgs a) {
         *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
       }
     };
-    if (tile.row0 == tile.start) clear(tile.start / a.edge + tile.rank, 0, tile.start % a.edge);
+    if (!a.spread && tile.row0 == tile.start) clear(tile.start / a.edge + tile.rank, 0, tile.start % a.edge);
     const int final_row = tile.end - 1;
-    if (final_row - tile.row0 < TOKENS)
+    if (!a.spread && final_row - tile.row0 < TOKENS)
       clear(final_row / a.edge + tile.rank, final_row % a.edge + 1, a.edge);
   }
   if (a.largest != nullptr) {
@@ -314,120 +330,6 @@ low_kernel(const LowArgs a) {
     if (lane == 0 && top != 0u) atomicMax(a.largest + tile.group, top);  // the order is no matter
   }
   if (splits > 1) cg::this_cluster().sync();  // the others have read this CTA's sums
-}
-
-// -------------------------------------------------------------- few tokens --
-//
-// d_t = base_t + U_a low_t with the base in FP32: a CTA takes some columns of up to 64 tokens of
-// one adapter, a thread a column at a time, whose row of U it reads once for eight tokens.  U's
-// bytes bound it (rank 16, 14336 columns, 40 adapters: 18 MB).  The kernel starts beside the one that
-// writes the base: what it can, it reads before it waits for that one.  The last tiles of the grid
-// hold the tokens of no adapter.
-constexpr int kExpandTokens = 64, kExpandThreads = 256;
-
-struct ExpandArgs {
-  const float* base;  // tokens x n
-  const char* u;      // RINNER: n x rank a matrix; else rank x n
-  int64_t u_pitch, u_stride;
-  const float* low;
-  int tokens, n, rank, adapters;
-  int columns;  // of a CTA
-  const int32_t* order;
-  const int32_t* ends;
-  void* out;  // tokens x n
-};
-
-// Elements r .. r + 7 of a column's row of U, as read: 8 16-bit numbers.
-template <bool RINNER>
-__device__ __forceinline__ uint4 up_words(const ExpandArgs& a, const char* u, int col, int r) {
-  if (RINNER) return __ldg(reinterpret_cast<const uint4*>(u + ((int64_t)col * a.u_pitch + r) * 2));
-  uint32_t w[4];
-  const unsigned short* const p =
-      reinterpret_cast<const unsigned short*>(u) + (int64_t)r * a.u_pitch + col;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = r + 2 * i < a.rank ? __ldg(p + 2 * i * a.u_pitch) : 0u;
-    const uint32_t hi = r + 2 * i + 1 < a.rank ? __ldg(p + (2 * i + 1) * a.u_pitch) : 0u;
-    w[i] = lo | hi << 16;
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <int F, bool RINNER>
-__global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandArgs a) {
-  extern __shared__ __align__(16) float lows[];  // [token][rank, whole 8s]
-  __shared__ int32_t rows[kExpandTokens];
-  const int lane = threadIdx.x & 31, ranks = (a.rank + 7) & ~7;
-  GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, kExpandTokens, (int)blockIdx.y,
-                                   lane);
-  if (tile.group < 0) {
-    // tokens without an adapter, from the last of the grid's tiles backwards
-    int carry = 0;
-    for (int base = 0; base < a.adapters; base += 32) {
-      int start, end;
-      group_span(a.ends, a.adapters, a.tokens, base, lane, &carry, &start, &end);
-    }
-    tile.row0 = carry + kExpandTokens * (int)(gridDim.y - 1 - blockIdx.y);
-    tile.end = a.tokens;
-  }
-  const int count = min(kExpandTokens, tile.end - tile.row0);
-  if ((int)threadIdx.x < count)
-    rows[threadIdx.x] = (int32_t)token_at(a.order, tile.row0 + threadIdx.x, a.tokens);
-  const bool some = tile.group >= 0;
-  const int first = (int)blockIdx.x * a.columns + threadIdx.x;
-  const int last = min((int)blockIdx.x * a.columns + a.columns, a.n);
-  const char* const u = a.u + (int64_t)(some ? tile.group : 0) * a.u_stride * 2;
-  uint4 ahead = make_uint4(0u, 0u, 0u, 0u);
-  if (some && first < last) ahead = up_words<RINNER>(a, u, first, 0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (count <= 0) return;
-  if (some) {
-    for (int i = threadIdx.x; i < count * ranks; i += kExpandThreads) {
-      const int t = i / ranks, r = i % ranks;
-      lows[i] = r < a.rank ? __ldcg(a.low + (int64_t)(tile.row0 + t) * a.rank + r) : 0.0f;
-    }
-  }
-  __syncthreads();
-  for (int col = first; col < last; col += kExpandThreads) {
-    for (int t0 = 0; t0 < count; t0 += 8) {
-      float sum[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        sum[t] = t0 + t < count ? __ldcg(a.base + (int64_t)rows[t0 + t] * a.n + col) : 0.0f;
-      if (some) {
-        uint4 q = t0 == 0 ? ahead : up_words<RINNER>(a, u, col, 0);
-        for (int r = 0; r < ranks; r += 8) {
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-          if (r + 8 < ranks) q = up_words<RINNER>(a, u, col, r + 8);
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = r + i < a.rank ? decode16<F>((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) : 0.0f;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            if (t0 + t >= count) break;
-            const float4* const l = reinterpret_cast<const float4*>(lows + (t0 + t) * ranks + r);
-            const float4 x = l[0], y = l[1];
-            sum[t] = fmaf(v[0], x.x, sum[t]);
-            sum[t] = fmaf(v[1], x.y, sum[t]);
-            sum[t] = fmaf(v[2], x.z, sum[t]);
-            sum[t] = fmaf(v[3], x.w, sum[t]);
-            sum[t] = fmaf(v[4], y.x, sum[t]);
-            sum[t] = fmaf(v[5], y.y, sum[t]);
-            sum[t] = fmaf(v[6], y.z, sum[t]);
-            sum[t] = fmaf(v[7], y.w, sum[t]);
-          }
-        }
-      }
-      if (t0 == 0 && some && col + kExpandThreads < last)
-        ahead = up_words<RINNER>(a, u, col + kExpandThreads, 0);
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        if (t0 + t < count)
-          static_cast<uint16_t*>(a.out)[(int64_t)rows[t0 + t] * a.n + col] =
-              (uint16_t)encode16<F>(sum[t]);
-    }
-  }
 }
 
 // ---------------------------------------------------------------- gradients --
@@ -611,10 +513,11 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
 template <int F>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
   const int lane = threadIdx.x & 31, group = (int)blockIdx.y;
+  const EndsAhead ahead(a.ends, a.adapters, lane);
   int carry = 0, chunks_before = 0, first = 0, chunks = 0;
   for (int base = 0; base <= group; base += 32) {
     int start, end;
-    group_span(a.ends, a.adapters, a.tokens, base, lane, &carry, &start, &end);
+    group_span(a.ends, ahead, a.adapters, a.tokens, base, lane, &carry, &start, &end);
     const int n = (end - start + kSumTokens - 1) / kSumTokens;
     const int upto = chunks_before + warp_scan_sum(n, lane);
     if (group - base < 32) {
@@ -687,33 +590,6 @@ int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
               : launch_low_as<F, KINNER, 128, 4>(args, stream);
 }
 
-template <int F, bool RINNER>
-int launch_expand(ExpandArgs& args, cudaStream_t stream) {
-  const auto kernel = &expand_kernel<F, RINNER>;
-  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel),
-                            kExpandTokens * SRS_ADAPTER_MAX_RANK * 4))
-    return rc;
-  const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
-  // one more tile than adapters' tokens can take: tokens of none in a last, partial one
-  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, kExpandTokens) + 1;
-  // columns of a CTA: as many as let all likely CTAs run at once
-  int64_t each = ceil_div(ceil_div(args.n, kExpandThreads) * busy, 6 * sm_count());
-  each = each < 1 ? 1 : each > 16 ? 16 : each;
-  args.columns = (int)each * kExpandThreads;
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute overlap{};
-  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  overlap.val.programmaticStreamSerializationAllowed = 1;
-  config.gridDim = dim3((unsigned)ceil_div(args.n, args.columns), (unsigned)tiles);
-  config.blockDim = dim3(kExpandThreads);
-  config.dynamicSmemBytes = (size_t)(kExpandTokens * ceil_div(args.rank, 8) * 8 * 4);
-  config.stream = stream;
-  config.attrs = &overlap;
-  config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<const ExpandArgs&>(args));
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "expansion launch");
-}
-
 template <int F, int RT>
 int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
   using S = SumShape<RT>;
@@ -764,26 +640,24 @@ int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, 
 
 using namespace srs;
 
-// Few tokens: the projection's thin form with an FP32 result and the expansion; else the adapters
-// enter the large product.
+// Few tokens: the projection's thin form.
 static bool few(int64_t tokens) { return tokens <= kThinRows; }
 
 // Parts of a call's workspace, each on a 256-byte boundary.
 struct AdapterSpace {
-  int64_t rows, low, base, total;  // rows: quantised tokens; low: FP32 or pairs; base: FP32
+  int64_t low, total;  // quantised tokens first, then the pairs of the low part
 };
 
 static AdapterSpace adapter_space(int64_t tokens, int64_t k, int64_t n, int adapters, int rank) {
   AdapterSpace s{};
   int64_t at = whole(srs_linear_workspace(tokens, k));
   s.low = at;
-  if (few(tokens)) {
-    at += whole(tokens * rank * 4);
-    s.base = at;
-    at += whole(tokens * n * 4);
-  } else if (n > 0) {
-    const int64_t edge = adapter_edge(tokens, n, k);
-    at += whole(pair_items(tokens, adapters, edge) * edge * pair_shape(rank).pitch * 2);
+  if (n > 0) {
+    const int64_t rows = few(tokens)
+                             ? (adapters < tokens ? adapters : tokens) * thin_columns(tokens)
+                             : pair_items(tokens, adapters, adapter_edge(tokens, n, k)) *
+                                   adapter_edge(tokens, n, k);
+    at += whole(rows * pair_shape(rank).pitch * 2);
   }
   s.total = at;
   return s;
@@ -829,7 +703,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   // without a sum there is neither a projection nor a low part
   if (e == cudaSuccess && n > 0 && k == 0) e = cudaMemsetAsync(d, 0, (size_t)(tokens * n * 2), st);
   if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
-  const int edge = thin || n == 0 ? 0 : adapter_edge(tokens, n, k);
+  const int edge = n == 0 ? 0 : thin ? thin_columns(tokens) : adapter_edge(tokens, n, k);
   const PairShape pairs = pair_shape(a->rank);
   LowArgs l{};
   l.x = static_cast<const char*>(x);
@@ -845,13 +719,14 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.ends = reinterpret_cast<const int32_t*>(a->ends);
   l.scale = reinterpret_cast<const float*>(a->scale);
   l.factor = a->factor;
-  l.low = low != nullptr ? low : thin ? reinterpret_cast<float*>(at + space.low) : nullptr;
+  l.low = low;
   l.largest = largest;
   if (edge != 0) {
     l.pairs = reinterpret_cast<uint16_t*>(at + space.low);
     l.edge = edge;
     l.pitch = pairs.pitch;
     l.rest_at = pairs.rest_at;
+    l.spread = thin;
   }
   if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, thin, st)
                               : launch_low<SRS_FMT_F16, false>(l, thin, st))
@@ -872,38 +747,19 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   q.order = thin ? nullptr : l.order;
   q.overlap = true;  // beside the low part
   if (int rc = quantize(q, st)) return rc;
-  const void* const up = reinterpret_cast<const void*>(turned ? a->down : a->up);
-  const int64_t up_pitch = turned ? a->down_pitch : a->up_pitch;
-  const int64_t up_stride = turned ? a->down_stride : a->up_stride;
-  if (!thin) {
-    const AdapterCall call{l.pairs,  up,       up_pitch,  up_stride, turned != 0,
-                           a->count, a->rank,  a->format, l.order,   l.ends};
-    return launch_adapter_product(rows, *w, k, call, edge, d, st);
-  }
-  float* const base = reinterpret_cast<float*>(at + space.base);
-  if (w->rows >= tokens) {
-    // beside the quantisation: its weights are streamed first
-    if (int rc = launch_thin(*w, rows, k, base, SRS_FMT_F32, 1, n, true, st)) return rc;
-  } else {
-    if (int rc = launch_thin(rows, *w, k, base, SRS_FMT_F32, n, 1, false, st)) return rc;
-  }
-  ExpandArgs x_args{};
-  x_args.base = base;
-  x_args.u = static_cast<const char*>(up);
-  x_args.u_pitch = up_pitch;
-  x_args.u_stride = up_stride;
-  x_args.low = l.low;
-  x_args.tokens = (int)tokens;
-  x_args.n = (int)n;
-  x_args.rank = a->rank;
-  x_args.adapters = a->count;
-  x_args.order = l.order;
-  x_args.ends = l.ends;
-  x_args.out = d;
-  return turned ? (bf16 ? launch_expand<SRS_FMT_BF16, false>(x_args, st)
-                        : launch_expand<SRS_FMT_F16, false>(x_args, st))
-                : (bf16 ? launch_expand<SRS_FMT_BF16, true>(x_args, st)
-                        : launch_expand<SRS_FMT_F16, true>(x_args, st));
+  const AdapterCall call{l.pairs,
+                         reinterpret_cast<const void*>(turned ? a->down : a->up),
+                         turned ? a->down_pitch : a->up_pitch,
+                         turned ? a->down_stride : a->up_stride,
+                         turned != 0,
+                         a->count,
+                         a->rank,
+                         a->format,
+                         l.order,
+                         l.ends};
+  // (with few tokens beside the quantisation: the weights are streamed first)
+  return thin ? launch_thin(*w, rows, k, d, a->format, 1, n, true, st, &call)
+              : launch_adapter_product(rows, *w, k, call, edge, d, st);
 }
 
 extern "C" int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters,

@@ -13,8 +13,7 @@
 // * Ragged sums: blocks of 128 rows are counted from the group's first one as well, so that a
 //   group's sum is a run of whole slices of k of the transposed copies and its scales are its
 //   own.  Those lie in words of four blocks, a word of every row one after the other: a warp then
-//   reads its 128 rows in whole lines (row by row, sums of some 8 slices waited for them: 8192
-//   rows in 8 groups, 14336 x 4096 each, 571 us instead of RESULT).  Groups without rows have no tiles; their zeros are written by the warp that has no role
+//   reads its 128 rows in whole lines.  Groups without rows have no tiles; their zeros are written by the warp that has no role
 //   in a product, as are the zeros of rows without a group.
 //
 // MMA-bound when groups are large (and then by the power limit), by the weights' bytes when they
@@ -63,11 +62,12 @@ template <bool SUMS>
 __device__ __forceinline__ void plan_groups(GroupPlan& p, const int32_t* ends, int groups, int rows,
                                             int edge) {
   const int lane = threadIdx.x & 31;
+  const EndsAhead ahead(ends, groups, lane);
   int carry = 0, tiles_before = 0, quads_before = 0, count = 0;
   for (int base = 0; base < groups; base += 32) {
     const int g = base + lane;
     int start, end;
-    group_span(ends, groups, rows, base, lane, &carry, &start, &end);
+    group_span(ends, ahead, groups, rows, base, lane, &carry, &start, &end);
     const int tiles = (end - start + edge - 1) / edge;
     const int upto = tiles_before + warp_scan_sum(tiles, lane);
     if (g < groups) {
@@ -193,6 +193,9 @@ struct SumSource {
   struct At {
     int expert, row, col;
   };
+  // Group after group: a tile of every group in turn, so that short sums (bound by the bytes of
+  // their results) run beside long ones, was slower (8192 rows in 8 uneven groups, 14336 x 4096
+  // each: 629 us instead of 559), as the groups' operands then share the L2.
   __device__ __forceinline__ At at(uint32_t t) const {
     const uint32_t each = (uint32_t)w.tile_rows * (uint32_t)w.tile_cols, i = t / each;
     const uint32_t j = t - i * each;

@@ -33,13 +33,27 @@ __device__ __forceinline__ int warp_scan_max(int v, int lane) {
   return v;
 }
 
+// The ends of up to 128 groups from the first on, one a lane, asked for together.
+struct EndsAhead {
+  int e[4];
+  __device__ __forceinline__ EndsAhead(const int32_t* __restrict__ ends, int groups, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = 32 * i + lane < groups ? __ldg(ends + 32 * i + lane) : 0;
+  }
+  __device__ __forceinline__ int at(const int32_t* __restrict__ ends, int groups, int base,
+                                    int lane) const {
+    if (base >= 128) return base + lane < groups ? __ldg(ends + base + lane) : 0;
+    return base < 64 ? (base < 32 ? e[0] : e[1]) : (base < 96 ? e[2] : e[3]);
+  }
+};
+
 // Groups base .. base + 31 for a warp, one a lane; `carry`: end of the group before.
 // Groups from `groups` on are empty.
-__device__ __forceinline__ void group_span(const int32_t* __restrict__ ends, int groups, int rows,
-                                           int base, int lane, int* carry, int* start, int* end) {
-  const int g = base + lane;
-  int e = g < groups ? min(max(ends[g], 0), rows) : 0;
-  e = max(warp_scan_max(e, lane), *carry);
+__device__ __forceinline__ void group_span(const int32_t* __restrict__ ends, const EndsAhead& ahead,
+                                           int groups, int rows, int base, int lane, int* carry,
+                                           int* start, int* end) {
+  int e = min(max(ahead.at(ends, groups, base, lane), 0), rows);
+  e = max(warp_scan_max(base + lane < groups ? e : 0, lane), *carry);
   const int before = __shfl_up_sync(0xFFFFFFFFu, e, 1);
   *start = lane == 0 ? *carry : before;
   *end = e;
@@ -60,9 +74,10 @@ __device__ __forceinline__ GroupTile find_group_tile(const int32_t* __restrict__
                                                      int rows, int edge, int index, int lane) {
   GroupTile r{-1, 0, 0, 0, 0, 0};
   int carry = 0, tiles_before = 0, quads_before = 0, rank = 0;
+  const EndsAhead ahead(ends, groups, lane);
   for (int base = 0; base < groups; base += 32) {
     int start, end;
-    group_span(ends, groups, rows, base, lane, &carry, &start, &end);
+    group_span(ends, ahead, groups, rows, base, lane, &carry, &start, &end);
     const int tiles = (end - start + edge - 1) / edge, quads = (tiles + 3) & ~3;
     const int upto = tiles_before + warp_scan_sum(tiles, lane);
     const int quads_upto = quads_before + warp_scan_sum(quads, lane);

@@ -65,6 +65,19 @@ int quantize(const QuantizeCall& q, cudaStream_t stream);
 int check_operand(const char* what, const srs_blocks* b, int64_t k);
 int check_groups(const int32_t* ends, int groups);
 
+// Low-rank adapters beside a product: their low part and its second matrices.
+inline int thin_columns(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : 64; }
+
+struct AdapterCall {
+  const void* pairs;
+  const void* up;  // rows x rank a matrix, or (rows_inner) rank x rows; `pitch`, `stride` elements
+  int64_t pitch, stride;
+  bool rows_inner;
+  int count, rank, format;
+  const int32_t* order;
+  const int32_t* ends;
+};
+
 // FP8 blocks: d = a b^T (operands checked by the caller).  Element (i, j)
 // of d is stored at i * row_stride + j * col_stride; only products with a thin side
 // (at most kThinRows rows) take a col_stride other than 1.  `overlap`: the kernel ahead
@@ -73,7 +86,8 @@ constexpr int kThinRows = 64;
 int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d,
                          int d_format, cudaStream_t stream);
 int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
-                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream);
+                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream,
+                const AdapterCall* adapters = nullptr);
 // The same for rows in groups: a's rows by their group's matrix of w (few rows a group).
 int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
                        int64_t k, void* d, int d_format, bool overlap, cudaStream_t stream);
@@ -84,7 +98,8 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
 // zero.  Item of tile i and the r-th adapter with tokens: i + r (each step along the tokens
 // raises one of the two, so no two items share a number).  A row has the rank's high parts, in
 // whole 16s, and the others behind them in one slice of 64 for ranks up to 32; else whole
-// slices of 64 of high parts and then as many of the others.
+// slices of 64 of high parts and then as many of the others.  A thin product's items have one row
+// a token in the batch's order, one item an adapter with tokens, and thin_columns rows.
 struct PairShape {
   int pitch, rest_at;  // elements of a row, first of the second parts
   int slices;
@@ -98,15 +113,6 @@ inline int64_t pair_items(int64_t tokens, int64_t adapters, int64_t edge) {
   return (tokens + edge - 1) / edge + (adapters < tokens ? adapters : tokens);
 }
 
-struct AdapterCall {
-  const void* pairs;
-  const void* up;  // rows x rank a matrix, or (rows_inner) rank x rows; `pitch`, `stride` elements
-  int64_t pitch, stride;
-  bool rows_inner;
-  int count, rank, format;
-  const int32_t* order;
-  const int32_t* ends;
-};
 int adapter_edge(int64_t tokens, int64_t n, int64_t k);  // of the tiles: 128 or 256
 int launch_adapter_product(const srs_blocks& rows, const srs_blocks& w, int64_t k,
                            const AdapterCall& a, int edge, void* d, cudaStream_t stream);

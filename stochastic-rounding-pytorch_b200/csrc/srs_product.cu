@@ -292,10 +292,10 @@ int launch_block_product(const srs_blocks& a, const srs_blocks& b, int64_t k, vo
 namespace {
 
 // `tiles`: of the grid (clusters of `splits` CTAs).
-template <int BN, bool GROUPED>
+template <int BN, int FORM>
 int launch_thin_as(ThinArgs& args, int64_t tiles, int splits, bool overlap, cudaStream_t stream) {
   using S = ThinShape<BN>;
-  const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN, GROUPED>);
+  const void* kernel = reinterpret_cast<const void*>(&thin_product_kernel<BN, FORM>);
   // As many stages as fit before a whole panel: the MMA reads 128 rows from the start of
   // the last stage's panel, past the end of that stage when its tile has fewer.
   args.panel_bytes = (args.rows + 7) / 8 * 8 * kSliceBytes;
@@ -315,8 +315,9 @@ int launch_thin_as(ThinArgs& args, int64_t tiles, int splits, bool overlap, cuda
 }  // namespace
 
 int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, int d_format,
-                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream) {
-  const int columns = b.rows <= 16 ? 16 : b.rows <= 32 ? 32 : 64;
+                int64_t row_stride, int64_t col_stride, bool overlap, cudaStream_t stream,
+                const AdapterCall* adapters) {
+  const int columns = thin_columns(b.rows);
   ThinArgs args{};
   args.m = (int)a.rows;
   args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
@@ -328,11 +329,19 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
   const int64_t sms = sm_count(), tiles = (a.rows + 127) / 128;
   int splits = 1;
   args.rows = 128;
-  if (tiles > sms) {
+  // (An adapters' matrix with its rows side by side is loaded in boxes of 64 of them.)
+  const bool whole = adapters != nullptr && adapters->rows_inner;
+  if (tiles > sms && !whole) {
     const int64_t rounds = (tiles + 2 * sms - 1) / (2 * sms);
     args.rows = (int)((a.rows + 2 * sms * rounds - 1) / (2 * sms * rounds));
   } else {
     while (splits < 8 && tiles * splits <= sms && args.slices >= 4 * splits) splits *= 2;
+    // More CTAs than SMs, but not two for each: tiles of the size that gives two (14336 x 4096 by
+    // 64 tokens in 2 x 112 tiles of 128 rows 26.9 us, in 2 x 148 of 97 rows 23.1).  Not with
+    // larger clusters: 37 of eight CTAs need two rounds (4096 x 4096: 8.3 -> 13.1 us).
+    const int64_t room = 2 * sms / splits;
+    if (splits <= 2 && tiles * splits > sms && room > tiles && !whole)
+      args.rows = (int)((a.rows + room - 1) / room);
   }
   if (int rc = operand_map(a, k, args.rows, &args.map_a)) return rc;
   if (int rc = operand_map(b, k, columns, &args.map_b)) return rc;
@@ -350,9 +359,29 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
   args.row_stride = row_stride;
   args.col_stride = col_stride;
   const int64_t grid = (args.m + args.rows - 1) / args.rows;
-  if (columns == 16) return launch_thin_as<16, false>(args, grid, splits, overlap, stream);
-  if (columns == 32) return launch_thin_as<32, false>(args, grid, splits, overlap, stream);
-  return launch_thin_as<64, false>(args, grid, splits, overlap, stream);
+  if (adapters != nullptr) {
+    const PairShape pairs = pair_shape(adapters->rank);
+    const int64_t items = adapters->count < b.rows ? adapters->count : b.rows;
+    const ProductOperand low{adapters->pairs, items * columns, pairs.pitch, pairs.pitch, 0, false};
+    const ProductOperand up{adapters->up,    a.rows, adapters->rank, adapters->pitch,
+                            adapters->stride, adapters->rows_inner};
+    if (int rc = encode_operand(low, 2, 1, columns, &args.map_h)) return rc;
+    if (int rc = encode_operand(up, 2, adapters->count, args.rows, &args.map_u)) return rc;
+    args.ends = adapters->ends;
+    args.groups = adapters->count;
+    args.rank = adapters->rank;
+    args.item_slices = pairs.slices;
+    args.rest_at = pairs.rest_at;
+    args.up_rows_inner = adapters->rows_inner;
+    args.extra_idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
+                       (d_format == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u);
+    if (columns == 16) return launch_thin_as<16, kThinAdapters>(args, grid, splits, overlap, stream);
+    if (columns == 32) return launch_thin_as<32, kThinAdapters>(args, grid, splits, overlap, stream);
+    return launch_thin_as<64, kThinAdapters>(args, grid, splits, overlap, stream);
+  }
+  if (columns == 16) return launch_thin_as<16, kThinPlain>(args, grid, splits, overlap, stream);
+  if (columns == 32) return launch_thin_as<32, kThinPlain>(args, grid, splits, overlap, stream);
+  return launch_thin_as<64, kThinPlain>(args, grid, splits, overlap, stream);
 }
 
 int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
@@ -366,8 +395,7 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
   args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
   args.rows = 128;
   // As for one weight: k split while few tiles are likely; with many, tiles of a size that fills
-  // whole rounds of two CTAs an SM (2 x (14336 x 4096): 224 tiles of 128 rows 26.6 us, 296
-  // of 97 RESULT us).
+  // whole rounds of two CTAs an SM.
   const int64_t sms = sm_count();
   int64_t tiles = (n + 127) / 128;
   int splits = 1;
@@ -401,9 +429,9 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
   args.col_stride = n;
   args.ends = ends;
   args.groups = experts;
-  if (columns == 16) return launch_thin_as<16, true>(args, most, splits, overlap, stream);
-  if (columns == 32) return launch_thin_as<32, true>(args, most, splits, overlap, stream);
-  return launch_thin_as<64, true>(args, most, splits, overlap, stream);
+  if (columns == 16) return launch_thin_as<16, kThinGrouped>(args, most, splits, overlap, stream);
+  if (columns == 32) return launch_thin_as<32, kThinGrouped>(args, most, splits, overlap, stream);
+  return launch_thin_as<64, kThinGrouped>(args, most, splits, overlap, stream);
 }
 
 }  // namespace srs

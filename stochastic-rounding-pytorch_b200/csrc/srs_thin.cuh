@@ -21,6 +21,12 @@
 // rows of one group's A by up to BN of its rows; which, it finds from the ends (all its warps
 // do, so that nothing waits for a barrier).  Grids are sized by a bound: the CTAs left over write
 // zeros for the rows of no group, as the others do behind their tile, and leave.
+//
+// ADAPTERS: B's rows are tokens, and token t of adapter a gets U_a low_t more, as MMAs of 16-bit
+// operands on the same sums (see the large product with adapters): an item of low parts, zero but
+// for its adapter's tokens, by the adapter's U; the CTAs of a cluster take the adapters in turn.
+// (In a kernel of its own behind this one that part took 5 us for one token and 10 for 64 with
+// 41 adapters, nearly all of it launch and dependent loads; in this one's epilogue as much.)
 #pragma once
 
 #include "srs_groups.cuh"
@@ -33,6 +39,9 @@ constexpr int kThinThreads = 256;
 constexpr int kThinMaxStages = 12;
 constexpr int kThinSlots = 8;    // scale groups on their way
 constexpr int kThinLoaders = 6;  // warps that bring them
+
+// What else a thin product does.
+enum : int { kThinPlain = 0, kThinGrouped = 1, kThinAdapters = 2 };
 
 struct ThinArgs {
   CUtensorMap map_a, map_b;
@@ -54,6 +63,11 @@ struct ThinArgs {
   const int32_t* ends;
   int groups;
   int64_t scale_a_group;  // bytes of scales from one group's A to the next
+  // ADAPTERS (`ends`, `groups`: those of the tokens' adapters)
+  CUtensorMap map_h, map_u;
+  int rank, item_slices, rest_at;
+  bool up_rows_inner;  // U is stored rank x rows
+  uint32_t extra_idesc;
 };
 
 template <int BN>
@@ -95,10 +109,12 @@ __device__ __forceinline__ void store_value(void* out, int format, int64_t at, f
 // Zeros in the rows of D (B's rows) that belong to no group, by all threads of the grid.
 __device__ __forceinline__ void zero_ungrouped(const ThinArgs& a) {
   // the last end as the groups' own reading of them has it
+  const int lane = threadIdx.x & 31;
+  const EndsAhead ahead(a.ends, a.groups, lane);
   int carry = 0;
   for (int base = 0; base < a.groups; base += 32) {
     int start, end;
-    group_span(a.ends, a.groups, a.n, base, (int)(threadIdx.x & 31), &carry, &start, &end);
+    group_span(a.ends, ahead, a.groups, a.n, base, lane, &carry, &start, &end);
   }
   const int64_t last = (int64_t)a.n * a.m;
   for (int64_t i = (int64_t)carry * a.m + (int64_t)blockIdx.x * kThinThreads + threadIdx.x;
@@ -106,10 +122,13 @@ __device__ __forceinline__ void zero_ungrouped(const ThinArgs& a) {
     store_value(a.out, a.out_format, i, 0.0f);
 }
 
-template <int BN, bool GROUPED>
+template <int BN, int FORM>
 __global__ void __launch_bounds__(kThinThreads, 2)
 thin_product_kernel(const __grid_constant__ ThinArgs a) {
+  constexpr bool GROUPED = FORM == kThinGrouped;
+  constexpr bool ADAPTERS = FORM == kThinAdapters;
   using S = ThinShape<BN>;
+  __shared__ int active[kThinRows], actives;  // ADAPTERS: those with tokens, in order
   // A kernel launched to overlap this one may start (and wait for it).
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t raw[];
@@ -187,7 +206,6 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   bool ok = true;
-
   if (warp == 4) {
     const bool leader = elect_lane();
     // B may come from the kernel this one overlaps.
@@ -210,6 +228,33 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       if (++s == stages) {
         s = 0;
         phase ^= 1u;
+      }
+    }
+    if constexpr (ADAPTERS) {
+      asm volatile("bar.sync 1, 96;" ::: "memory");  // the list of adapters
+      const int slices = a.item_slices, chunks = (slices + 1) / 2;
+      for (int e = (int)rank; e < actives && ok; e += (int)splits) {
+        for (int q = 0; q < slices && ok; ++q) {
+          const uint32_t pa = stage0 + s * stage_bytes;
+          ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
+          if (!ok) break;
+          if (leader) {
+            const int k = 64 * (q < chunks ? q : q - chunks);
+            barrier_expect(full(s), load_bytes);
+            if (a.up_rows_inner) {
+              load_box<1>(pa, &a.map_u, row0, k, active[e], full(s));
+              load_box<1>(pa + kPanelBytes / 2, &a.map_u, row0 + 64, k, active[e], full(s));
+            } else {
+              load_box<1>(pa, &a.map_u, k, row0, active[e], full(s));
+            }
+            load_box<1>(pa + panel_bytes, &a.map_h, 64 * q, e * BN, 0, full(s));
+          }
+          __syncwarp();
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
       }
     }
     // Every stage given back before the CTA can leave.
@@ -269,6 +314,44 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       }
       if ((j0 & 3) == 3) ++group;
     }
+    if constexpr (ADAPTERS) {
+      asm volatile("bar.sync 1, 96;" ::: "memory");
+      const int slices = a.item_slices, chunks = (slices + 1) / 2;
+      // Behind the MMAs of the other kind: nothing says that the two keep their order.
+      if (ok && (int)rank < actives)
+        ok = barrier_wait(empty(s == 0 ? stages - 1 : s - 1), s == 0 ? phase ^ 1u : phase, a.status,
+                          1u << 9);
+      const bool inner = a.up_rows_inner;
+      const uint64_t desc_u = operand_descriptor(inner);
+      const uint32_t step_u = (inner ? 2048u : 32u) >> 4;
+      const uint32_t idesc = a.extra_idesc | (inner ? 1u << 15 : 0u);
+      for (int e = (int)rank; e < actives && ok; e += (int)splits) {
+        for (int q = 0; q < slices && ok; ++q) {
+          ok = barrier_wait(full(s), phase, a.status, 1u << 11);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint32_t pa = stage0 + s * stage_bytes;
+          const uint64_t du = desc_u | uint64_t((pa >> 4) & 0x3FFFu);
+          const uint64_t dh = desc | uint64_t(((pa + panel_bytes) >> 4) & 0x3FFFu);
+          const int chunk = q < chunks ? q : q - chunks;
+          const int steps = (min(a.rank - 64 * chunk, 64) + 15) / 16;
+          if (leader) {
+            for (int j = 0; j < steps; ++j)
+              mma_f16<1>(tmem, du + j * step_u, dh + 2 * j, idesc, 1u);
+            if (slices == 1) {
+              for (int j = 0; j < steps; ++j)
+                mma_f16<1>(tmem, du + j * step_u, dh + 2 * (a.rest_at / 16 + j), idesc, 1u);
+            }
+            mma_commit<1>(empty(s));
+          }
+          __syncwarp();
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
     if (ok && leader) mma_commit<1>(done);
     __syncwarp();
   } else {
@@ -280,6 +363,23 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     ScaleRows from_a, from_b;
     from_a.at(scale_a, a.scale_a_pitch, a.scale_a_shift, row0, a.m, lane);
     from_b.at(a.scale_b, a.scale_b_pitch, a.scale_b_shift, b_row0, a.n, lane);
+    if constexpr (ADAPTERS) {
+      if (warp == 7) {
+        // the adapters with tokens, for the loads and MMAs (at most as many as tokens)
+        const EndsAhead ahead(a.ends, a.groups, lane);
+        int carry = 0, count = 0;
+        for (int base = 0; base < a.groups; base += 32) {
+          int start, end;
+          group_span(a.ends, ahead, a.groups, a.n, base, lane, &carry, &start, &end);
+          const unsigned some = __ballot_sync(0xFFFFFFFFu, end > start);
+          if (end > start) active[count + __popc(some & ((1u << lane) - 1u))] = base + lane;
+          count += __popc(some);
+        }
+        if (lane == 0) actives = count;
+        __syncwarp();
+        asm volatile("bar.arrive 1, 96;" ::: "memory");
+      }
+    }
     const int groups = (last - first + 3) >> 2;
     bool waited = false;
     for (int g = warp < 4 ? warp : warp - 2; g < groups; g += kThinLoaders) {

@@ -131,7 +131,7 @@ def indices(tokens, adapters, how, device, seed=0):
 SIZES = [(1, 1, 16, 128, 128), (3, 2, 1, 77, 333), (64, 48, 16, 256, 300), (65, 3, 8, 64, 64),
          (200, 7, 12, 300, 129), (500, 5, 64, 128, 520), (300, 4, 33, 1000, 96),
          (700, 2, 128, 264, 136), (130, 2, 200, 130, 72), (1500, 3, 24, 72, 40),
-         (40, 300, 4, 64, 48)]
+         (40, 300, 4, 64, 48), (60, 3, 256, 128, 136), (64, 5, 128, 128, 1000), (17, 1024, 20, 96, 24)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
