@@ -10,27 +10,30 @@
 // CTAs through distributed shared memory), and the warp then places its rows one batch of
 // 32 after the other, a row's rank in its batch from a vote over equal groups.  No atomic
 // decides an order, so the result does not depend on timing.
+//
+// In a cluster, up to 4096 rows of a CTA are put in order in shared memory first and leave in runs.
 #include <cooperative_groups.h>
 
 #include "srs_groups.cuh"
 #include "srs_host.h"
+#include "srs_launch.h"
 
 namespace srs {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kSortAhead = 4;     // batches of a warp loaded together
-constexpr int kSortCluster = 8;   // CTAs of a large sort
-// One CTA places 65536 rows in 64 batches a warp; from 4096 rows (4 batches) on eight CTAs
-// are used.
+constexpr int kSortAhead = 8;     // batches of a warp loaded together
+// Rows up to kSortSmall: one CTA of 32 warps, 128 rows each.  More: a cluster of 16 CTAs of 16
+// warps (its meetings and remote counts cost about 2 us).  The instructions of 200 a batch bound
+// it: 65536 rows took 11.8 us on eight SMs.
+constexpr int kSortCluster = 16;
 constexpr int64_t kSortSmall = 4096;
 
 struct SortArgs {
   const void* index;
   int64_t rows, segment;  // rows of a warp
-  int groups;
+  int groups, bits;  // bits: of groups + 1
   int32_t* order;
   int32_t* ends;
 };
@@ -42,8 +45,63 @@ __device__ __forceinline__ int group_of(const SortArgs& a, int64_t row, int64_t 
   return g >= 0 && g < (I)a.groups ? (int)g : a.groups;
 }
 
+// Lanes whose value of `bits` bits is this lane's: a vote a bit (match.any takes longer the more
+// values differ: with it 65536 rows in 64 groups took 2 us more).
+__device__ __forceinline__ unsigned equal_lanes(int value, int bits) {
+  unsigned same = 0xFFFFFFFFu;
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (value >> b & 1) != 0;
+    const unsigned vote = __ballot_sync(0xFFFFFFFFu, set);
+    same &= set ? vote : ~vote;
+  }
+  return same;
+}
+
+// values[0 .. wide): their sums before each, by the whole CTA (at most 1025 values).
+template <int THREADS>
+__device__ __forceinline__ void sums_before(int* values, int wide, int* warp_sums) {
+  constexpr int kEach = (kMaxGroups + THREADS) / THREADS;  // values a thread
+  const int at = kEach * threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int n[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    n[i] = at + i < wide ? values[at + i] : 0;
+    sum += n[i];
+  }
+  const int upto = warp_scan_sum(sum, lane);
+  __syncthreads();  // (warp_sums may still be read)
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  int start = upto - sum;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) start += w < warp ? warp_sums[w] : 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (at + i < wide) values[at + i] = start;
+    start += n[i];
+  }
+  __syncthreads();
+}
+
+// `totals` again in `to`, for their sums.
+__device__ __forceinline__ int* totals_copy(const int* totals, int* to, int wide) {
+  __syncthreads();
+  for (int q = threadIdx.x; q < wide; q += blockDim.x) to[q] = totals[q];
+  __syncthreads();
+  return to;
+}
+
+template <int C>
+struct SortShape {
+  static constexpr int kWarps = C > 1 ? 16 : 32, kThreads = 32 * kWarps;
+  static constexpr int kLocal = kWarps * 32 * kSortAhead;  // rows of a CTA put in order locally
+  static constexpr int kMostBytes = (kWarps + 3) * (kMaxGroups + 1) * 4 + kLocal * 6;
+};
+
 template <class I, int C>
-__global__ void __launch_bounds__(kSortThreads, 1) sort_rows_kernel(const SortArgs a) {
+__global__ void __launch_bounds__(SortShape<C>::kThreads, 1) sort_rows_kernel(const SortArgs a) {
+  constexpr int kSortWarps = SortShape<C>::kWarps, kSortThreads = SortShape<C>::kThreads;
+  constexpr int kSortLocal = SortShape<C>::kLocal;
   extern __shared__ int counts[];  // [warp][group], group `groups`: rows of none
   __shared__ int sums[kSortWarps];
   const int wide = a.groups + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -57,8 +115,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_rows_kernel(const SortAr
 
   const int64_t first = min(((int64_t)rank * kSortWarps + warp) * a.segment, a.rows);
   const int64_t end = min(first + a.segment, a.rows);
+  int g[kSortAhead];  // the groups of the batches at hand: for short segments, of all
   for (int64_t r = first; r < end; r += 32 * kSortAhead) {
-    int g[kSortAhead];
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i) g[i] = group_of<I>(a, r + 32 * i + lane, end);
 #pragma unroll
@@ -66,101 +124,125 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_rows_kernel(const SortAr
       if (g[i] < wide) atomicAdd(mine + g[i], 1);
   }
   __syncthreads();
-  for (int g = threadIdx.x; g < wide; g += kSortThreads) {
-    int sum = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int n = counts[w * wide + g];
-      counts[w * wide + g] = sum;
-      sum += n;
-    }
-    totals[g] = sum;
+  // counts of the warps before, a warp to a group
+  for (int q = warp; q < wide; q += kSortWarps) {
+    int* const at = counts + (lane < kSortWarps ? lane : 0) * wide + q;
+    const int n = lane < kSortWarps ? *at : 0, upto = warp_scan_sum(n, lane);
+    __syncwarp();
+    if (lane < kSortWarps) *at = upto - n;
+    if (lane == 31) totals[q] = upto;
   }
   if constexpr (C > 1) {
     cg::this_cluster().sync();
-    for (int g = threadIdx.x; g < wide; g += kSortThreads) {
+    for (int q = threadIdx.x; q < wide; q += kSortThreads) {
       int sum = 0, prior = 0;
 #pragma unroll
       for (int r = 0; r < C; ++r) {
-        const int n = cg::this_cluster().map_shared_rank(totals, r)[g];
+        const int n = cg::this_cluster().map_shared_rank(totals, r)[q];
         if (r < rank) prior += n;
         sum += n;
       }
-      before[g] = prior;
-      all[g] = sum;
+      before[q] = prior;
+      all[q] = sum;
     }
   } else {
     __syncthreads();
-    for (int g = threadIdx.x; g < wide; g += kSortThreads) {
-      before[g] = 0;
-      all[g] = totals[g];
+    for (int q = threadIdx.x; q < wide; q += kSortThreads) {
+      before[q] = 0;
+      all[q] = totals[q];
     }
   }
   __syncthreads();
-  // the first place of every group: at most 1025 numbers, two a thread
-  const int at = 2 * threadIdx.x;
-  const int n0 = at < wide ? all[at] : 0, n1 = at + 1 < wide ? all[at + 1] : 0;
-  const int pair = warp_scan_sum(n0 + n1, lane);
-  if (lane == 31) sums[warp] = pair;
-  __syncthreads();
-  if (warp == 0) sums[lane] = warp_scan_sum(sums[lane], lane);
-  __syncthreads();
-  const int start = pair - n0 - n1 + (warp > 0 ? sums[warp - 1] : 0);
-  if (at < wide) all[at] = start;
-  if (at + 1 < wide) all[at + 1] = start + n0;
+  // the first place of every group
+  sums_before<kSortThreads>(all, wide, sums);
   if (rank == 0) {
-    if (at < a.groups) a.ends[at] = start + n0;
-    if (at + 1 < a.groups) a.ends[at + 1] = start + n0 + n1;
+    for (int q = threadIdx.x; q < a.groups; q += kSortThreads) a.ends[q] = all[q + 1];
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kSortWarps * wide; i += kSortThreads)
-    counts[i] += all[i % wide] + before[i % wide];
+  // (few rows go straight to their places)
+  const bool at_hand = a.segment <= 32 * kSortAhead, local = C > 1 && at_hand;
+  int* const rows = all + wide;  // local: the CTA's rows in order, and their groups
+  uint16_t* const groups = reinterpret_cast<uint16_t*>(rows + kSortLocal);
+  if (local) {
+    // `before`: from a place among the CTA's rows to the place among all
+    for (int q = threadIdx.x; q < wide; q += kSortThreads) before[q] += all[q];
+    sums_before<kSortThreads>(totals_copy(totals, all, wide), wide, sums);
+    for (int q = threadIdx.x; q < wide; q += kSortThreads) before[q] -= all[q];
+    for (int q = warp; q < wide; q += kSortWarps)
+      if (lane < kSortWarps) counts[lane * wide + q] += all[q];
+  } else {
+    for (int q = warp; q < wide; q += kSortWarps)
+      if (lane < kSortWarps) counts[lane * wide + q] += all[q] + before[q];
+  }
   __syncthreads();
 
   for (int64_t r = first; r < end; r += 32 * kSortAhead) {
-    int g[kSortAhead];
+    if (!at_hand) {
 #pragma unroll
-    for (int i = 0; i < kSortAhead; ++i) g[i] = group_of<I>(a, r + 32 * i + lane, end);
+      for (int i = 0; i < kSortAhead; ++i) g[i] = group_of<I>(a, r + 32 * i + lane, end);
+    }
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i) {
-      const unsigned same = __match_any_sync(0xFFFFFFFFu, g[i]);
+      if (r + 32 * i >= end) break;
+      const unsigned same = equal_lanes(g[i], a.bits);
       const int place = __popc(same & ((1u << lane) - 1u));
       const bool is_row = g[i] < wide;
       const int base = is_row ? mine[g[i]] : 0;
       __syncwarp();
       if (is_row) {
-        a.order[base + place] = (int32_t)(r + 32 * i + lane);
+        const int32_t at = (int32_t)(r + 32 * i + lane);
+        if (local) {
+          rows[base + place] = at;
+          groups[base + place] = (uint16_t)g[i];
+        } else {
+          a.order[base + place] = at;
+        }
         if (place == 0) mine[g[i]] = base + __popc(same);
       }
       __syncwarp();
     }
+  }
+  if (local) {
+    __syncthreads();
+    const int64_t mine0 = min((int64_t)rank * kSortWarps * a.segment, a.rows);
+    const int count = (int)(min(mine0 + kSortWarps * a.segment, a.rows) - mine0);
+    for (int i = threadIdx.x; i < count; i += kSortThreads) a.order[i + before[groups[i]]] = rows[i];
   }
   // no CTA leaves while others may still read its totals
   if constexpr (C > 1) cg::this_cluster().sync();
 }
 
 template <class I, int C>
-cudaError_t launch_sort(SortArgs& a, cudaStream_t stream) {
+int launch_sort(SortArgs& a, cudaStream_t stream) {
   const auto kernel = &sort_rows_kernel<I, C>;
-  const int64_t warps = (int64_t)C * kSortWarps;
-  a.segment = ((a.rows + warps - 1) / warps + 31) / 32 * 32;
-  const size_t bytes = (size_t)(kSortWarps + 3) * (a.groups + 1) * sizeof(int);
-  if (bytes > 40 * 1024) {
+  using S = SortShape<C>;
+  int resident = 0;
+  if (int rc = prepare_kernel(reinterpret_cast<const void*>(kernel), 1, S::kThreads, S::kMostBytes,
+                              &resident))
+    return rc;
+  if (C > 8) {
+    // (an attribute of the kernel; set again it costs half a microsecond)
     const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess) return e;
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return cuda_fail(e, "srs_group_rows");
   }
+  const int64_t warps = (int64_t)C * S::kWarps;
+  a.segment = ((a.rows + warps - 1) / warps + 31) / 32 * 32;
+  const bool local = C > 1 && a.segment <= 32 * kSortAhead;
+  const size_t bytes =
+      (size_t)(S::kWarps + 3) * (a.groups + 1) * sizeof(int) + (local ? S::kLocal * 6 : 0);
   cudaLaunchConfig_t config{};
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = C;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.gridDim = dim3(C);
-  config.blockDim = dim3(kSortThreads);
+  config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = bytes;
   config.stream = stream;
   config.attrs = &cluster;
   config.numAttrs = C > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&config, kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<const SortArgs&>(a));
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_group_rows launch");
 }
 
 }  // namespace
@@ -183,11 +265,10 @@ extern "C" int srs_group_rows(const void* index, int index_bytes, int64_t rows, 
     return fail(SRS_ERR_INVALID_ARGUMENT, "index, order or ends is not element aligned");
   if (int rc = check_device()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SortArgs a{index, rows, 0, groups, order, ends};
+  SortArgs a{index, rows, 0, groups, 1, order, ends};
+  while ((groups + 1) >> a.bits != 0) ++a.bits;
   const bool small = rows <= kSortSmall;
-  const cudaError_t e =
-      index_bytes == 4
-          ? (small ? launch_sort<int32_t, 1>(a, st) : launch_sort<int32_t, kSortCluster>(a, st))
-          : (small ? launch_sort<int64_t, 1>(a, st) : launch_sort<int64_t, kSortCluster>(a, st));
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_group_rows launch");
+  return index_bytes == 4
+             ? (small ? launch_sort<int32_t, 1>(a, st) : launch_sort<int32_t, kSortCluster>(a, st))
+             : (small ? launch_sort<int64_t, 1>(a, st) : launch_sort<int64_t, kSortCluster>(a, st));
 }
