@@ -19,6 +19,7 @@
 #include "srs_groups.cuh"
 #include "srs_host.h"
 #include "srs_launch.h"
+#include "srs_tcgen05.cuh"
 
 namespace srs {
 namespace {
@@ -44,10 +45,6 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint32_t shared_at(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
 template <bool TURN>
@@ -96,29 +93,10 @@ __device__ __forceinline__ uint32_t encode16(float x) {
 
 // ------------------------------------------------------------------ low part --
 //
-// A CTA takes up to TOKENS tokens of one adapter (tiles counted from the adapter's first), up to
-// 16 RT of the rank and a part of the sum; the parts of a cluster's CTAs are added through
-// distributed shared memory in rank order.  x's bytes, read once, bound it: mma.sync is far
-// faster than they arrive (4096 tokens, 4096 -> 64: 2 GFLOP).  Sums are FP32.
-//
-// TOKENS = 128: 8 warps of 16 tokens each.  TOKENS = 16, for calls of few tokens where most
-// adapters have one or two: 4 warps that share a stage's four steps of 16 of k.
+// A CTA takes up to 128 (or 16) tokens of one adapter (tiles counted from the adapter's first), up
+// to 16 RT of the rank and a part of the sum; the parts of a cluster's CTAs are added through
+// distributed shared memory in rank order.  x's bytes, read once, bound it.  Sums are FP32.
 constexpr int kLowStep = 64;  // of k a stage: 128 bytes of a row
-
-template <int TOKENS, int RT>
-struct LowShape {
-  static constexpr int kWarps = TOKENS == 16 ? 4 : TOKENS / 16;
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr bool kShared = TOKENS == 16;  // warps share the steps of a stage
-  static constexpr int kRank = 16 * RT;
-  static constexpr int kX = TOKENS * kLowStep * 2, kW = kRank * kLowStep * 2;
-  // bytes on their way: 6 stages for ranks up to 16; two CTAs an SM fit with all of these
-  static constexpr int kStages = TOKENS == 16 ? 8 : RT == 1 ? 6 : RT == 2 ? 5 : 4;
-  static constexpr int kPitch = kRank + 1;
-  static constexpr int kSums = (kShared ? kWarps : 1) * TOKENS * kPitch * 4;
-  static constexpr int kStageBytes = kStages * (kX + kW);
-  static constexpr int kSmem = kStageBytes > kSums ? kStageBytes : kSums;
-};
 
 struct LowArgs {
   const char* x;  // 16-bit, rows of x_pitch elements
@@ -130,164 +108,73 @@ struct LowArgs {
   const float* scale;  // null: `factor` alone
   float factor;
   float* low;             // tokens (in order) x rank (null: not wanted)
-  uint16_t* pairs;        // items for a large product (null: not wanted)
+  uint16_t* pairs;        // items for a product (null: not wanted)
   int edge, pitch, rest_at;
   bool spread;            // items of a thin product: rows are the batch's
   unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
+  unsigned int* status;
 };
 
 // 16-byte slot `slot` of a row of 128 bytes, turned so that 8 rows at one slot and 8 slots of a
-// row both reach all banks.
+// row both reach all banks: the order of 128-byte swizzled boxes.
 __device__ __forceinline__ uint32_t turned_slot(int row, int slot) {
   return (uint32_t)(row * 128 + ((slot ^ (row & 7)) << 4));
 }
 
-template <int F, bool KINNER, int TOKENS, int RT>
-__global__ void __launch_bounds__(LowShape<TOKENS, RT>::kThreads, TOKENS == 16 ? 4 : 2)
-low_kernel(const LowArgs a) {
-  using S = LowShape<TOKENS, RT>;
-  // The quantisation behind this kernel reads nothing of it and waits for it at its end.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  extern __shared__ __align__(128) uint8_t raw[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The CTA's part of a sum.
+struct LowTile {
+  GroupTile tile;
+  int count, rank0, ranks, first, last;  // tokens, ranks, stages of k
   uint32_t splits, split;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
-  const GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, TOKENS,
-                                         (int)(blockIdx.x / splits), lane);
-  if (tile.group < 0) return;  // the whole cluster
-  const int count = min(TOKENS, tile.end - tile.row0);
-  const int rank0 = (int)blockIdx.y * S::kRank, ranks = min(S::kRank, a.rank - rank0);
+};
+
+__device__ __forceinline__ LowTile low_tile(const LowArgs& a, int most, int rank_block, int lane) {
+  LowTile t;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(t.splits));
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(t.split));
+  t.tile = find_group_tile(a.ends, a.adapters, a.tokens, most, (int)(blockIdx.x / t.splits), lane);
+  t.count = min(most, t.tile.end - t.tile.row0);
+  t.rank0 = (int)blockIdx.y * rank_block;
+  t.ranks = min(rank_block, a.rank - t.rank0);
   const int steps = (a.k + kLowStep - 1) / kLowStep;
-  const int first = (int)((int64_t)steps * split / splits);
-  const int last = (int)((int64_t)steps * (split + 1) / splits);
-  const uint32_t base = shared_at(raw);
-  const auto x_at = [&](int s) { return base + (uint32_t)(s * (S::kX + S::kW)); };
+  t.first = (int)((int64_t)steps * t.split / t.splits);
+  t.last = (int)((int64_t)steps * (t.split + 1) / t.splits);
+  return t;
+}
 
-  // this thread's rows of x: threadIdx.x / 8 + kRows i, slot threadIdx.x % 8
-  constexpr int kRows = S::kThreads / 8, kEach = TOKENS / kRows, kOfW = (S::kRank + kRows - 1) / kRows;
-  const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
-  const char* from[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int r = row + kRows * i;
-    from[i] = a.x + (r < count ? token_at(a.order, tile.row0 + r, a.tokens) : 0) * a.x_pitch * 2;
-  }
-  const char* const w = a.w + (int64_t)tile.group * a.w_stride * 2;
-  const auto load = [&](int step, int s) {
-    const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
-    const uint32_t to = x_at(s);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int r = row + kRows * i;
-      if (kRows * i < count)  // rows that no warp multiplies stay as they are
-        copy16(to + turned_slot(r, slot), bytes > 0 ? from[i] + 2 * k : a.x, r < count ? bytes : 0);
-    }
-    if (KINNER) {
-#pragma unroll
-      for (int i = 0; i < kOfW; ++i) {
-        const int r = row + kRows * i;
-        const bool in = r < ranks && bytes > 0;
-        if (r < S::kRank)
-          copy16(to + S::kX + turned_slot(r, slot),
-                 in ? w + ((int64_t)(rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
-      }
-    } else {
-      // 64 rows of k, 2 RT slots of 8 of the rank each (the others are not read)
-#pragma unroll
-      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += S::kThreads) {
-        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
-        const int left = min(max(ranks - 8 * c, 0) * 2, 16);
-        const bool in = kk < a.k && left > 0;
-        copy16(to + S::kX + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)),
-               in ? w + ((int64_t)kk * a.w_pitch + rank0 + 8 * c) * 2 : w, in ? left : 0);
-      }
-    }
-  };
-
-  float sum[2 * RT][4];
-#pragma unroll
-  for (int i = 0; i < 2 * RT; ++i) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
-  }
-  for (int i = 0; i < S::kStages - 1; ++i) {
-    if (first + i < last) load(first + i, i);
-    copies_done();
-  }
-  const int my_rows = S::kShared ? 0 : 16 * warp;
-  const bool busy = my_rows < count;
-  int s = 0;
-  for (int step = first; step < last; ++step) {
-    copies_wait<S::kStages - 2>();
-    __syncthreads();
-    if (step + S::kStages - 1 < last) load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
-    copies_done();
-    const uint32_t xs = x_at(s), ws = xs + S::kX;
-    if (++s == S::kStages) s = 0;
-    if (!busy) continue;
-#pragma unroll
-    for (int q = 0; q < (S::kShared ? 1 : kLowStep / 16); ++q) {
-      const int kk = S::kShared ? warp : q;
-      uint32_t m[4];
-      load_matrices<false>(xs + turned_slot(my_rows + (lane & 15), 2 * kk + (lane >> 4)), m);
-#pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        uint32_t b[4];
-        if (KINNER) {  // ranks 16 j + (0..15) x k 16 kk ..
-          load_matrices<false>(ws + turned_slot(16 * j + (lane & 7) + ((lane >> 4) << 3),
-                                                2 * kk + ((lane >> 3) & 1)), b);
-        } else {       // k 16 kk + (0..15) x ranks 16 j ..
-          const int r = 16 * kk + (lane & 15), c = 2 * j + (lane >> 4);
-          load_matrices<true>(ws + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)), b);
-        }
-        multiply<F>(sum[2 * j], m, b[0], b[1]);
-        multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
-      }
-    }
-  }
-  // sums to shared memory, [token][rank] (of every warp, where they share the steps)
-  copies_wait<0>();
-  __syncthreads();
-  float* const sums = reinterpret_cast<float*>(raw);
-  if (busy) {
-    float* const mine = sums + (S::kShared ? warp * TOKENS * S::kPitch : 0);
-#pragma unroll
-    for (int j = 0; j < 2 * RT; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mine[(my_rows + (lane >> 2) + 8 * (i >> 1)) * S::kPitch + 8 * j + 2 * (lane & 3) + (i & 1)] =
-            sum[j][i];
-    }
-  }
+// Sums of the cluster's CTAs (`sums`: [token][rank], rows of `pitch`, PARTS of them `part` apart
+// in every CTA) added, scaled and written: token t of the tile by CTA t % splits.
+template <int F, int RANK, int PARTS>
+__device__ __forceinline__ void write_low(const LowArgs& a, const LowTile& l, float* sums, int pitch,
+                                          int part, int most, int threads) {
+  const GroupTile& tile = l.tile;
+  const int splits = (int)l.splits, split = (int)l.split;
   const float factor = a.factor * (a.scale != nullptr ? __ldg(a.scale + tile.group) : 1.0f);
   if (splits > 1) cg::this_cluster().sync();
   else __syncthreads();
-  float most = 0.0f;
-  // token t of the tile by CTA t % splits
-  const int whole = (ranks + 15) & ~15;
-  for (int i = threadIdx.x; i < (TOKENS + (int)splits - 1) / (int)splits * S::kRank;
-       i += S::kThreads) {
-    const int t = i / S::kRank * (int)splits + (int)split, r = i % S::kRank;
-    if (t >= count || r >= whole) continue;
+  float top_size = 0.0f;
+  const int whole = (l.ranks + 15) & ~15;
+  for (int i = threadIdx.x; i < (most + splits - 1) / splits * RANK; i += threads) {
+    const int t = i / RANK * splits + split, r = i % RANK;
+    if (t >= l.count || r >= whole) continue;
     float v = 0.0f;
-    if (r < ranks) {
-      for (uint32_t p = 0; p < splits; ++p) {
+    if (r < l.ranks) {
+      for (int p = 0; p < splits; ++p) {
         const float* const theirs =
-            (splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums) + t * S::kPitch + r;
+            (splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums) + t * pitch + r;
 #pragma unroll
-        for (int q = 0; q < (S::kShared ? S::kWarps : 1); ++q) v += theirs[q * TOKENS * S::kPitch];
+        for (int q = 0; q < PARTS; ++q) v += theirs[q * part];
       }
       v *= factor;
-      if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + rank0 + r] = v;
-      most = fmaxf(most, isfinite(v) ? fabsf(v) : 0.0f);
+      if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + l.rank0 + r] = v;
+      top_size = fmaxf(top_size, isfinite(v) ? fabsf(v) : 0.0f);
     }
     if (a.pairs != nullptr) {
       const int place = tile.row0 + t;
       const int64_t at =
           a.spread ? (int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)
                    : (int64_t)(place / a.edge + tile.rank) * a.edge + place % a.edge;
-      uint16_t* const to = a.pairs + at * a.pitch + rank0 + r;
+      uint16_t* const to = a.pairs + at * a.pitch + l.rank0 + r;
       const uint32_t high = encode16<F>(v);
       const float left = v - decode16<F>(high);
       to[0] = (uint16_t)high;
@@ -295,61 +182,294 @@ low_kernel(const LowArgs a) {
     }
   }
   if (a.pairs != nullptr) {
-    // zeros in the rows of the adapter's first and last item that are not its own
+    // zeros in the rows of the adapter's items that are not its own
     const int words = whole / 2;
-    // (spread: in those of all tokens that are not this adapter's)
-    if (a.spread && tile.row0 == tile.start) {
-      const int others = a.tokens - (tile.end - tile.start);
-      for (int i = threadIdx.x + S::kThreads * (int)split; i < others * words;
-           i += S::kThreads * (int)splits) {
-        const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
-        uint16_t* const p =
-            a.pairs + ((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)) * a.pitch +
-            rank0 + 2 * (i % words);
-        *reinterpret_cast<uint32_t*>(p) = 0u;
-        *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
-      }
-    }
-    const auto clear = [&](int item, int from_row, int to_row) {
-      const int rows = to_row - from_row;
-      for (int i = threadIdx.x + S::kThreads * (int)split; i < rows * words;
-           i += S::kThreads * (int)splits) {
-        uint16_t* const p = a.pairs + ((int64_t)item * a.edge + from_row + i / words) * a.pitch +
-                            rank0 + 2 * (i % words);
-        *reinterpret_cast<uint32_t*>(p) = 0u;
-        *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
-      }
+    const auto zero = [&](int64_t row, int word) {
+      uint16_t* const p = a.pairs + row * a.pitch + l.rank0 + 2 * word;
+      *reinterpret_cast<uint32_t*>(p) = 0u;
+      *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
     };
-    if (!a.spread && tile.row0 == tile.start) clear(tile.start / a.edge + tile.rank, 0, tile.start % a.edge);
-    const int final_row = tile.end - 1;
-    if (!a.spread && final_row - tile.row0 < TOKENS)
-      clear(final_row / a.edge + tile.rank, final_row % a.edge + 1, a.edge);
+    const int from = threadIdx.x + threads * split, step = threads * splits;
+    if (a.spread) {
+      if (tile.row0 == tile.start) {
+        const int others = a.tokens - (tile.end - tile.start);
+        for (int i = from; i < others * words; i += step) {
+          const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
+          zero((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens), i % words);
+        }
+      }
+    } else {
+      // before its first row in its first item, behind its last in the last
+      if (tile.row0 == tile.start)
+        for (int i = from; i < tile.start % a.edge * words; i += step)
+          zero((int64_t)(tile.start / a.edge + tile.rank) * a.edge + i / words, i % words);
+      const int final_row = tile.end - 1, behind = final_row % a.edge + 1;
+      if (final_row - tile.row0 < most)
+        for (int i = from; i < (a.edge - behind) * words; i += step)
+          zero((int64_t)(final_row / a.edge + tile.rank) * a.edge + behind + i / words, i % words);
+    }
   }
   if (a.largest != nullptr) {
-    const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
-    if (lane == 0 && top != 0u) atomicMax(a.largest + tile.group, top);  // the order is no matter
+    const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_size));
+    if ((threadIdx.x & 31) == 0 && top != 0u)
+      atomicMax(a.largest + tile.group, top);  // the order is no matter
   }
   if (splits > 1) cg::this_cluster().sync();  // the others have read this CTA's sums
 }
 
+// Calls of few tokens, where most adapters have one or two: 16 tokens, and 4 warps that share a
+// stage's four steps of 16 of k with mma.sync.  Latency bounds them: launch, the ends, the order and
+// the first bytes one after the other, and the cluster's meeting.
+template <int RT>
+struct FewShape {
+  static constexpr int kTokens = 16, kWarps = 4, kThreads = 128, kRank = 16 * RT, kStages = 8;
+  static constexpr int kX = kTokens * kLowStep * 2, kW = kRank * kLowStep * 2;
+  static constexpr int kPitch = kRank + 1;
+  static constexpr int kSums = kWarps * kTokens * kPitch * 4;
+  static constexpr int kSmem = kStages * (kX + kW) > kSums ? kStages * (kX + kW) : kSums;
+};
+
+template <int F, bool KINNER, int RT>
+__global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(const LowArgs a) {
+  using S = FewShape<RT>;
+  // The quantisation behind this kernel reads nothing of it and waits for it at its end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(128) uint8_t raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const LowTile l = low_tile(a, S::kTokens, S::kRank, lane);
+  if (l.tile.group < 0) return;  // the whole cluster
+  const uint32_t base = smem_address(raw);
+  const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const char* const from =
+      a.x + (row < l.count ? token_at(a.order, l.tile.row0 + row, a.tokens) : 0) * a.x_pitch * 2;
+  const char* const w = a.w + (int64_t)l.tile.group * a.w_stride * 2;
+  const auto load = [&](int step, int s) {
+    const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
+    const uint32_t to = base + (uint32_t)(s * (S::kX + S::kW));
+    copy16(to + turned_slot(row, slot), bytes > 0 ? from + 2 * k : a.x, row < l.count ? bytes : 0);
+    if (KINNER) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = row + 16 * i;
+        const bool in = r < l.ranks && bytes > 0;
+        copy16(to + S::kX + turned_slot(r, slot),
+               in ? w + ((int64_t)(l.rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
+      }
+    } else {
+      // 64 rows of k, 2 RT slots of 8 of the rank each
+#pragma unroll
+      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += S::kThreads) {
+        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
+        const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
+        const bool in = kk < a.k && left > 0;
+        copy16(to + S::kX + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)),
+               in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
+      }
+    }
+  };
+  float sum[2 * RT][4];
+#pragma unroll
+  for (int i = 0; i < 2 * RT; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
+  }
+  for (int i = 0; i < S::kStages - 1; ++i) {
+    if (l.first + i < l.last) load(l.first + i, i);
+    copies_done();
+  }
+  int s = 0;
+  for (int step = l.first; step < l.last; ++step) {
+    copies_wait<S::kStages - 2>();
+    __syncthreads();
+    if (step + S::kStages - 1 < l.last) load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
+    copies_done();
+    const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW)), ws = xs + S::kX;
+    if (++s == S::kStages) s = 0;
+    uint32_t m[4];
+    load_matrices<false>(xs + turned_slot(lane & 15, 2 * warp + (lane >> 4)), m);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      uint32_t b[4];
+      if (KINNER) {  // ranks 16 j + (0..15) x k 16 warp ..
+        load_matrices<false>(ws + turned_slot(16 * j + (lane & 7) + ((lane >> 4) << 3),
+                                              2 * warp + ((lane >> 3) & 1)), b);
+      } else {       // k 16 warp + (0..15) x ranks 16 j ..
+        const int r = 16 * warp + (lane & 15), c = 2 * j + (lane >> 4);
+        load_matrices<true>(ws + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)), b);
+      }
+      multiply<F>(sum[2 * j], m, b[0], b[1]);
+      multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
+    }
+  }
+  // every warp's sums to shared memory
+  copies_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(raw);
+  float* const mine = sums + warp * S::kTokens * S::kPitch;
+#pragma unroll
+  for (int j = 0; j < 2 * RT; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mine[((lane >> 2) + 8 * (i >> 1)) * S::kPitch + 8 * j + 2 * (lane & 3) + (i & 1)] = sum[j][i];
+  }
+  write_low<F, S::kRank, S::kWarps>(a, l, sums, S::kPitch, S::kTokens * S::kPitch, S::kTokens,
+                                    S::kThreads);
+}
+
+// Many tokens: 128 of one adapter (the rows of an MMA), gathered with cp.async into the layout that
+// the tensor core reads, so that a stage's four MMAs need nothing of the warps.  A stage is loaded
+// again once the MMAs of two stages before have read theirs.  (With ldmatrix and mma.sync in 8
+// warps shared memory was read five times as often: 4096 tokens, 4096 -> 64: 25 us; so RESULT.)
+constexpr int kManyTokens = 128, kManyThreads = 256;
+
+template <int RT>
+struct ManyShape {
+  static constexpr int kRank = 16 * RT;
+  static constexpr int kX = kManyTokens * 128, kW = kLowStep * 128;
+  static constexpr int kStages = 4;  // two CTAs an SM fit
+  static constexpr int kPitch = kRank + 1;
+  static constexpr int kSmem = 1024 + kStages * (kX + kW);
+  static constexpr uint32_t kColumns = RT == 4 ? 64 : 32;  // of TMEM
+  static_assert(kManyTokens * kPitch * 4 <= kStages * (kX + kW), "the sums fit the stages");
+};
+
+template <int F, bool KINNER, int RT>
+__global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs a) {
+  using S = ManyShape<RT>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[S::kStages];
+  __shared__ uint32_t tmem_slot;
+  const int lane = threadIdx.x & 31, warp = warp_index();
+  const LowTile l = low_tile(a, kManyTokens, S::kRank, lane);
+  if (l.tile.group < 0) return;  // the whole cluster
+  const uint32_t base = (smem_address(raw) + 1023u) & ~1023u, bar0 = smem_address(bars);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) barrier_init(bar0 + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
+
+  // this thread's rows of x: threadIdx.x / 8 + 32 i, slot threadIdx.x % 8
+  const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const char* from[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row + 32 * i;
+    from[i] = a.x + (r < l.count ? token_at(a.order, l.tile.row0 + r, a.tokens) : 0) * a.x_pitch * 2;
+  }
+  const char* const w = a.w + (int64_t)l.tile.group * a.w_stride * 2;
+  const auto load = [&](int step, int s) {
+    const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
+    const uint32_t to = base + (uint32_t)(s * (S::kX + S::kW));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 32 * i;
+      if (32 * i < l.count)  // sums of the rows behind are not read
+        copy16(to + turned_slot(r, slot), bytes > 0 ? from[i] + 2 * k : a.x,
+               r < l.count ? bytes : 0);
+    }
+    if (KINNER) {
+#pragma unroll
+      for (int i = 0; i < (S::kRank + 31) / 32; ++i) {
+        const int r = row + 32 * i;
+        const bool in = r < l.ranks && bytes > 0;
+        if (r < S::kRank)
+          copy16(to + S::kX + turned_slot(r, slot),
+                 in ? w + ((int64_t)(l.rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
+      }
+    } else {
+      // 64 rows of k, of which 2 RT slots of 8 of the rank are read
+#pragma unroll
+      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += kManyThreads) {
+        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
+        const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
+        const bool in = kk < a.k && left > 0;
+        copy16(to + S::kX + turned_slot(r, c),
+               in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
+      }
+    }
+  };
+  for (int i = 0; i < S::kStages - 2; ++i) {
+    if (l.first + i < l.last) load(l.first + i, i);
+    copies_done();
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t kInstruction = (uint32_t)(S::kRank >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
+                                    (F == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u) |
+                                    (KINNER ? 0u : 1u << 16);
+  bool ok = true;
+  const int steps = l.last - l.first;
+  for (int i = 0; i < steps; ++i) {
+    const int s = i % S::kStages;
+    // what the threads have copied, for the tensor core
+    copies_wait<S::kStages - 3>();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+      if (elect_lane()) {
+        const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW));
+        const uint64_t dx = operand_descriptor(false) | uint64_t((xs >> 4) & 0x3FFFu);
+        const uint64_t dw = operand_descriptor(!KINNER) | uint64_t(((xs + S::kX) >> 4) & 0x3FFFu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_f16<1>(tmem, dx + 2 * j, dw + j * (KINNER ? 2u : 128u), kInstruction,
+                     (i | j) != 0 ? 1u : 0u);
+        mma_commit<1>(bar0 + 8 * s);
+      }
+      __syncwarp();
+    }
+    // stage s - 2 for step i + kStages - 2
+    if (i + S::kStages - 2 < steps) {
+      if (ok && i >= 2)
+        ok = barrier_wait(bar0 + 8 * ((i - 2) % S::kStages), ((i - 2) / S::kStages) & 1, a.status,
+                          1u << 18);
+      if (ok) load(l.first + i + S::kStages - 2, (i + S::kStages - 2) % S::kStages);
+    }
+    copies_done();
+  }
+  copies_wait<0>();
+  // the last MMAs (those before are done with them)
+  if (ok && steps > 0)
+    barrier_wait(bar0 + 8 * ((steps - 1) % S::kStages), ((steps - 1) / S::kStages) & 1, a.status,
+                 1u << 18);
+  tmem_fence_after();
+  __syncthreads();  // no thread still copies or reads a stage
+  float* const sums = reinterpret_cast<float*>(raw + (base - smem_address(raw)));
+  if (warp < 4) {
+    const int t = 32 * warp + lane;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      uint32_t v[16];
+      tmem_load16(tmem + ((uint32_t)(32 * warp) << 16) + 16 * j, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sums[t * S::kPitch + 16 * j + i] = steps > 0 ? __uint_as_float(v[i]) : 0.0f;
+    }
+  }
+  tmem_fence_before();
+  write_low<F, S::kRank, 1>(a, l, sums, S::kPitch, 0, kManyTokens, kManyThreads);
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 1) tmem_free<1>(tmem, S::kColumns);
+}
+
 // ---------------------------------------------------------------- gradients --
 //
-// out_a = sum over an adapter's tokens of z_t (cols) by low_t (rank).  A CTA takes 128 columns,
-// up to 64 of the rank and a chunk of up to kSumTokens tokens of one adapter (counted from
-// its first); adapters of several chunks leave FP32 parts, which another kernel adds in
-// order.  z's bytes, read once for every 64 of the rank, bound it.  `low` enters as a pair of
-// 16-bit numbers (high and what it leaves); in FP16 both are scaled by a power of two that
+// out_a = sum over an adapter's tokens of z_t (cols) by low_t (rank).  A CTA takes 128 columns (the
+// rows of an MMA), up to 16 RT of the rank and a chunk of tokens of one adapter (counted from its
+// first); an adapter of one chunk is finished here, one of several leaves FP32 parts, which another
+// kernel adds in order.  z's bytes, read once for every 64 of the rank, bound it: rows are gathered
+// with cp.async into the layout in which the tensor core reads tokens as k.  `low` enters as a
+// pair of 16-bit numbers (high and what it leaves); in FP16 both are scaled by a power of two that
 // brings the adapter's largest to 2^11 .. 2^12, so that small gradients keep their digits.
-constexpr int kSumCols = 128, kSumStep = 64, kSumTokens = 512;
-constexpr int kSumWarps = kSumCols / 16, kSumThreads = 32 * kSumWarps;
-
-template <int RT>  // 16 RT of the rank
-struct SumShape {
-  static constexpr int kRank = 16 * RT;
-  static constexpr int kZ = kSumStep * kSumCols * 2, kLow = kSumStep * kRank * 2;
-  static constexpr int kStages = 5 - RT / 2;  // with them two CTAs an SM fit
-  static constexpr int kSmem = kStages * kZ + 2 * 2 * kLow;
-};
+constexpr int kSumCols = 128, kSumStep = 64, kSumThreads = 256, kSumStages = 4;
+constexpr int kSumChunk = 1024;  // most tokens of a chunk
+constexpr int kSumZ = kSumStep * kSumCols * 2, kSumLow = kSumStep * 128;
+constexpr int kSumSmem = 1024 + kSumStages * kSumZ + 2 * 2 * kSumLow;  // two CTAs an SM fit
 
 struct SumArgs {
   const char* z;
@@ -357,11 +477,13 @@ struct SumArgs {
   const float* low;
   const unsigned int* largest;
   int tokens, cols, rank, adapters;
+  int chunk;  // tokens
   const int32_t* order;
   const int32_t* ends;
   void* out;
   float* parts;  // [chunk][rank][cols]
   int turned;    // out: cols x rank instead of rank x cols
+  unsigned int* status;
 };
 
 __device__ __forceinline__ float pair_scale(const unsigned int* largest, int group) {
@@ -372,38 +494,48 @@ __device__ __forceinline__ float pair_scale(const unsigned int* largest, int gro
   return __uint_as_float((uint32_t)(min(max(k, -126), 126) + 127) << 23);
 }
 
-__device__ __forceinline__ uint32_t wide_slot(int row, int slot) {  // rows of 256 bytes
-  return (uint32_t)(row * 256 + ((slot ^ (row & 7)) << 4));
-}
-
 template <int F, int RT>
 __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
-  using S = SumShape<RT>;
-  extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ int32_t places[kSumTokens];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kRank = 16 * RT;
+  constexpr uint32_t kColumns = RT == 4 ? 64 : 32;
+  extern __shared__ uint8_t raw[];
+  __shared__ int32_t places[kSumChunk];
+  __shared__ __align__(8) uint64_t bars[kSumStages];
+  __shared__ uint32_t tmem_slot;
+  const int lane = threadIdx.x & 31, warp = warp_index();
   const GroupTile tile =
-      find_group_tile(a.ends, a.adapters, a.tokens, kSumTokens, (int)blockIdx.y, lane);
+      find_group_tile(a.ends, a.adapters, a.tokens, a.chunk, (int)blockIdx.y, lane);
   if (tile.group < 0) return;
-  const int count = min(kSumTokens, tile.end - tile.row0);
+  const int count = min(a.chunk, tile.end - tile.row0);
   for (int i = threadIdx.x; i < count; i += kSumThreads)
     places[i] = (int32_t)token_at(a.order, tile.row0 + i, a.tokens);
-  const int rank0 = (int)blockIdx.z * S::kRank, ranks = min(S::kRank, a.rank - rank0);
+  const int rank0 = (int)blockIdx.z * kRank, ranks = min(kRank, a.rank - rank0);
   const int col0 = (int)blockIdx.x * kSumCols;
   const float scale = pair_scale(a.largest, tile.group);
-  const uint32_t z0 = shared_at(raw), low0 = z0 + S::kStages * S::kZ;
+  const uint32_t z0 = (smem_address(raw) + 1023u) & ~1023u, low0 = z0 + kSumStages * kSumZ;
+  const uint32_t bar0 = smem_address(bars);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSumStages; ++i) barrier_init(bar0 + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<1>(smem_address(&tmem_slot), kColumns);
+  tmem_fence_before();
   __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
 
-  const int slot = threadIdx.x & 15, row = threadIdx.x >> 4;  // 16 rows at a time
+  // z: two boxes of 64 columns, a token's 128 bytes a row; 16 tokens at a time
+  const int slot = threadIdx.x & 15, row = threadIdx.x >> 4;
   const int col = col0 + 8 * slot, bytes = min(max(a.cols - col, 0) * 2, 16);
   const char* const z = a.z + (int64_t)col * 2;
+  const uint32_t box = (uint32_t)(slot >> 3) * (kSumZ / 2);
   const auto load = [&](int step, int s) {
 #pragma unroll
     for (int i = 0; i < kSumStep / 16; ++i) {
       const int r = row + 16 * i, t = step * kSumStep + r;
       const bool in = t < count && bytes > 0;
-      copy16(z0 + s * S::kZ + wide_slot(r, slot), in ? z + places[t] * a.z_pitch * 2 : a.z,
-             in ? bytes : 0);
+      copy16(z0 + s * kSumZ + box + turned_slot(r, slot & 7),
+             in ? z + places[t] * a.z_pitch * 2 : a.z, in ? bytes : 0);
     }
   };
   // low: thread t has ranks 4 (t % 4) + 16 j of token t / 4
@@ -428,11 +560,8 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
       }
     }
   };
-  const auto low_slot = [](int r, int c) {
-    return RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c);
-  };
   const auto split = [&](int b) {
-    const uint32_t to = low0 + b * 2 * S::kLow;
+    const uint32_t to = low0 + b * 2 * kSumLow;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       uint32_t high[2], rest[2];
@@ -444,72 +573,90 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
         rest[i] = encode16<F>(x - decode16<F>(hx)) | encode16<F>(y - decode16<F>(hy)) << 16;
       }
       // 8 of the 16 bytes of a slot
-      const uint32_t at = to + low_slot(low_row, 2 * j + (low_col >> 3)) + 2 * (low_col & 7);
+      const uint32_t at = to + turned_slot(low_row, 2 * j + (low_col >> 3)) + 2 * (low_col & 7);
       asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(high[0]), "r"(high[1])
                    : "memory");
-      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + S::kLow), "r"(rest[0]),
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + kSumLow), "r"(rest[0]),
                    "r"(rest[1])
                    : "memory");
     }
   };
-
-  float sum[2 * RT][4];
-#pragma unroll
-  for (int i = 0; i < 2 * RT; ++i) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
-  }
+  // both operands have their rows (columns of z, ranks) side by side
+  constexpr uint32_t kInstruction = (uint32_t)(kRank >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
+                                    (F == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u) | 1u << 15 |
+                                    1u << 16;
   const int steps = (count + kSumStep - 1) / kSumStep;
-  for (int i = 0; i < S::kStages - 1; ++i) {
+  for (int i = 0; i < kSumStages - 2; ++i) {
     if (i < steps) load(i, i);
     copies_done();
   }
   fetch(0);
-  int s = 0;
-  for (int step = 0; step < steps; ++step) {
-    split(step & 1);
-    copies_wait<S::kStages - 2>();
+  bool ok = true;
+  for (int i = 0; i < steps; ++i) {
+    const int s = i % kSumStages;
+    // the MMAs of step i - 2 have read this step's buffer of low, and the stage of step i + 2
+    if (ok && i >= 2)
+      ok = barrier_wait(bar0 + 8 * ((i - 2) % kSumStages), ((i - 2) / kSumStages) & 1, a.status,
+                        1u << 19);
+    split(i & 1);
+    copies_wait<kSumStages - 3>();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    if (step + S::kStages - 1 < steps)
-      load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
+    if (warp == 0) {
+      if (elect_lane()) {
+        const uint32_t zs = z0 + s * kSumZ, ls = low0 + (i & 1) * 2 * kSumLow;
+        const uint64_t dz = operand_descriptor(true) | uint64_t((zs >> 4) & 0x3FFFu);
+        const uint64_t dl = operand_descriptor(true) | uint64_t((ls >> 4) & 0x3FFFu);
+        const uint64_t dr = operand_descriptor(true) | uint64_t(((ls + kSumLow) >> 4) & 0x3FFFu);
+#pragma unroll
+        for (int j = 0; j < kSumStep / 16; ++j) {
+          mma_f16<1>(tmem, dz + 128 * j, dr + 128 * j, kInstruction, (i | j) != 0 ? 1u : 0u);
+          mma_f16<1>(tmem, dz + 128 * j, dl + 128 * j, kInstruction, 1u);
+        }
+        mma_commit<1>(bar0 + 8 * s);
+      }
+      __syncwarp();
+    }
+    if (i + kSumStages - 2 < steps && ok)
+      load(i + kSumStages - 2, (i + kSumStages - 2) % kSumStages);
     copies_done();
-    if (step + 1 < steps) fetch(step + 1);
-    const uint32_t zs = z0 + s * S::kZ, ls = low0 + (step & 1) * 2 * S::kLow;
-    if (++s == S::kStages) s = 0;
+    if (i + 1 < steps) fetch(i + 1);
+  }
+  copies_wait<0>();
+  if (ok)
+    barrier_wait(bar0 + 8 * ((steps - 1) % kSumStages), ((steps - 1) / kSumStages) & 1, a.status,
+                 1u << 19);
+  tmem_fence_after();
+  if (warp < 4) {
+    const float back = 1.0f / scale;  // a power of two: exact
+    const int c = col0 + 32 * warp + lane;
+    const bool alone = tile.end - tile.start <= a.chunk;
 #pragma unroll
-    for (int kk = 0; kk < kSumStep / 16; ++kk) {
-      // columns 16 warp .. by tokens 16 kk ..: matrices of 8 tokens x 8 columns, turned
-      uint32_t m[4];
-      load_matrices<true>(zs + wide_slot(16 * kk + (lane & 7) + ((lane >> 4) << 3),
-                                         2 * warp + ((lane >> 3) & 1)), m);
+    for (int j = 0; j < RT; ++j) {
+      uint32_t v[16];
+      tmem_load16(tmem + ((uint32_t)(32 * warp) << 16) + 16 * j, v);
 #pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        uint32_t b[4];
-        const uint32_t at = ls + low_slot(16 * kk + (lane & 15), 2 * j + (lane >> 4));
-        load_matrices<true>(at, b);
-        multiply<F>(sum[2 * j], m, b[0], b[1]);
-        multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
-        load_matrices<true>(at + S::kLow, b);
-        multiply<F>(sum[2 * j], m, b[0], b[1]);
-        multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
+      for (int i = 0; i < 16; ++i) {
+        const int r = 16 * j + i;
+        if (c >= a.cols || r >= ranks) continue;
+        const float value = __uint_as_float(v[i]) * back;
+        if (!alone)
+          a.parts[((int64_t)blockIdx.y * a.rank + rank0 + r) * a.cols + c] = value;
+        else
+          static_cast<uint16_t*>(a.out)[(int64_t)tile.group * a.rank * a.cols +
+                                        (a.turned ? (int64_t)c * a.rank + rank0 + r
+                                                  : (int64_t)(rank0 + r) * a.cols + c)] =
+              (uint16_t)encode16<F>(value);
       }
     }
   }
-  copies_wait<0>();
-  const float back = 1.0f / scale;  // a power of two: exact
-#pragma unroll
-  for (int j = 0; j < 2 * RT; ++j) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = col0 + 16 * warp + (lane >> 2) + 8 * (i >> 1);
-      const int r = 8 * j + 2 * (lane & 3) + (i & 1);
-      if (c >= a.cols || r >= ranks) continue;
-      a.parts[((int64_t)blockIdx.y * a.rank + rank0 + r) * a.cols + c] = sum[j][i] * back;
-    }
-  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 1) tmem_free<1>(tmem, kColumns);
 }
 
-// out_a = the sum of its chunks' parts, in order; zeros without tokens.
+// out_a = the sum of its chunks' parts, in order, where there are several; zeros without tokens.
 template <int F>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
   const int lane = threadIdx.x & 31, group = (int)blockIdx.y;
@@ -518,7 +665,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
   for (int base = 0; base <= group; base += 32) {
     int start, end;
     group_span(a.ends, ahead, a.adapters, a.tokens, base, lane, &carry, &start, &end);
-    const int n = (end - start + kSumTokens - 1) / kSumTokens;
+    const int n = (end - start + a.chunk - 1) / a.chunk;
     const int upto = chunks_before + warp_scan_sum(n, lane);
     if (group - base < 32) {
       first = __shfl_sync(0xFFFFFFFFu, upto - n, group - base);
@@ -526,6 +673,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
     }
     chunks_before = __shfl_sync(0xFFFFFFFFu, upto, 31);
   }
+  if (chunks == 1) return;
   const int64_t each = (int64_t)a.rank * a.cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < each; i += (int64_t)gridDim.x * 256) {
     // i runs over the result's order
@@ -547,19 +695,16 @@ int allow_shared(const void* kernel, int bytes) {
   return prepare_kernel(kernel, 1, 32, bytes, &resident);
 }
 
-template <int F, bool KINNER, int TOKENS, int RT>
-int launch_low_as(const LowArgs& args, cudaStream_t stream) {
-  using S = LowShape<TOKENS, RT>;
-  const auto kernel = &low_kernel<F, KINNER, TOKENS, RT>;
-  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+// `room`: CTAs that run at once.
+int launch_low_kernel(const void* kernel, const LowArgs& args, int most, int rank_block, int threads,
+                      int smem, int64_t room, cudaStream_t stream) {
+  if (int rc = allow_shared(kernel, smem)) return rc;
   const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
-  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, TOKENS);
-  const int64_t blocks = ceil_div(args.rank, S::kRank), steps = ceil_div(args.k, kLowStep);
-  // Parts of the sum while all likely CTAs run at once (two an SM; four of the small), at least
-  // four stages each.  A second round costs as much as the first: 16 prompts of 4096 tokens in
-  // all, 4096 -> 64, took 30 us in 384 CTAs.
-  const int64_t likely = (args.tokens / TOKENS + (busy + 1) / 2) * blocks;
-  const int64_t room = (TOKENS == 16 ? 4 : 2) * sm_count();
+  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, most);
+  const int64_t blocks = ceil_div(args.rank, rank_block), steps = ceil_div(args.k, kLowStep);
+  // Parts of the sum while all likely CTAs run at once, at least four stages each.  A second round
+  // costs as much as the first: 16 prompts of 4096 tokens in all, 4096 -> 64, took 30 us in 384 CTAs.
+  const int64_t likely = (args.tokens / most + (busy + 1) / 2) * blocks;
   int64_t splits = likely > 0 ? room / likely : 8;
   if (splits > steps / 4) splits = steps / 4;
   splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
@@ -569,36 +714,44 @@ int launch_low_as(const LowArgs& args, cudaStream_t stream) {
   cluster.val.clusterDim.x = (unsigned)splits;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.gridDim = dim3((unsigned)(tiles * splits), (unsigned)blocks);
-  config.blockDim = dim3(S::kThreads);
-  config.dynamicSmemBytes = S::kSmem;
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = (size_t)smem;
   config.stream = stream;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args);
+  LowArgs copy = args;
+  void* arguments[1] = {&copy};
+  const cudaError_t e = cudaLaunchKernelExC(&config, kernel, arguments);
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "low part launch");
+}
+
+template <int F, bool KINNER, int RT>
+int launch_low_as(const LowArgs& args, bool thin, cudaStream_t stream) {
+  const int64_t sms = sm_count();
+  if (thin)
+    return launch_low_kernel(reinterpret_cast<const void*>(&low_few_kernel<F, KINNER, RT>), args,
+                             FewShape<RT>::kTokens, FewShape<RT>::kRank, FewShape<RT>::kThreads,
+                             FewShape<RT>::kSmem, (RT == 4 ? 2 : 4) * sms, stream);
+  return launch_low_kernel(reinterpret_cast<const void*>(&low_many_kernel<F, KINNER, RT>), args,
+                           kManyTokens, ManyShape<RT>::kRank, kManyThreads, ManyShape<RT>::kSmem,
+                           2 * sms, stream);
 }
 
 template <int F, bool KINNER>
 int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
-  if (args.rank <= 16)
-    return thin ? launch_low_as<F, KINNER, 16, 1>(args, stream)
-                : launch_low_as<F, KINNER, 128, 1>(args, stream);
-  if (args.rank <= 32)
-    return thin ? launch_low_as<F, KINNER, 16, 2>(args, stream)
-                : launch_low_as<F, KINNER, 128, 2>(args, stream);
-  return thin ? launch_low_as<F, KINNER, 16, 4>(args, stream)
-              : launch_low_as<F, KINNER, 128, 4>(args, stream);
+  if (args.rank <= 16) return launch_low_as<F, KINNER, 1>(args, thin, stream);
+  if (args.rank <= 32) return launch_low_as<F, KINNER, 2>(args, thin, stream);
+  return launch_low_as<F, KINNER, 4>(args, thin, stream);
 }
 
 template <int F, int RT>
 int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
-  using S = SumShape<RT>;
   const auto kernel = &sum_kernel<F, RT>;
-  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSumSmem)) return rc;
   const dim3 grid((unsigned)ceil_div(args.cols, kSumCols),
-                  (unsigned)most_group_tiles(args.tokens, args.adapters, kSumTokens),
-                  (unsigned)ceil_div(args.rank, S::kRank));
-  kernel<<<grid, kSumThreads, S::kSmem, stream>>>(args);
+                  (unsigned)most_group_tiles(args.tokens, args.adapters, args.chunk),
+                  (unsigned)ceil_div(args.rank, 16 * RT));
+  kernel<<<grid, kSumThreads, kSumSmem, stream>>>(args);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "adapter gradient launch");
 }
@@ -721,6 +874,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.factor = a->factor;
   l.low = low;
   l.largest = largest;
+  if (int rc = status_word(&l.status)) return rc;
   if (edge != 0) {
     l.pairs = reinterpret_cast<uint16_t*>(at + space.low);
     l.edge = edge;
@@ -762,10 +916,18 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
               : launch_adapter_product(rows, *w, k, call, edge, d, st);
 }
 
+// Tokens of a chunk: long ones leave fewer parts, short ones keep the SMs busy (two CTAs each).
+static int sum_chunk(int64_t tokens, int64_t cols, int rank) {
+  const int64_t each = ceil_div(cols, kSumCols) * ceil_div(rank, 64);
+  int64_t chunk = tokens * each / (2 * sm_count());
+  chunk = ceil_div(chunk < 256 ? 256 : chunk, kSumStep) * kSumStep;
+  return (int)(chunk > kSumChunk ? kSumChunk : chunk);
+}
+
 extern "C" int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters,
                                                   int rank) {
   if (tokens <= 0 || cols <= 0 || adapters < 1 || rank < 1) return 0;
-  return most_group_tiles(tokens, adapters, kSumTokens) * rank * cols * 4;
+  return most_group_tiles(tokens, adapters, sum_chunk(tokens, cols, rank)) * rank * cols * 4;
 }
 
 extern "C" int srs_adapter_gradient(const void* z, int format, int64_t tokens, int64_t cols,
@@ -812,6 +974,9 @@ extern "C" int srs_adapter_gradient(const void* z, int format, int64_t tokens, i
   a.out = out;
   a.parts = static_cast<float*>(workspace);
   a.turned = turned != 0;
+  a.chunk = sum_chunk(tokens, cols, rank);
+  if (int rc = check_products()) return rc;
+  if (int rc = status_word(&a.status)) return rc;
   if (int rc = format == SRS_FMT_BF16 ? launch_sum<SRS_FMT_BF16>(a, st)
                                       : launch_sum<SRS_FMT_F16>(a, st))
     return rc;
