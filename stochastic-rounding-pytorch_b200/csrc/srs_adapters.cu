@@ -19,7 +19,6 @@
 #include "srs_groups.cuh"
 #include "srs_host.h"
 #include "srs_launch.h"
-#include "srs_quantize.cuh"
 #include "srs_tcgen05.cuh"
 
 namespace srs {
@@ -36,10 +35,48 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+// Rows of SLOTS (2 or 4) 16-byte slots, turned as rows of 8 are.
+template <int SLOTS>
+__device__ __forceinline__ uint32_t narrow_slot(int row, int slot) {
+  return (uint32_t)(row * 16 * SLOTS + ((slot ^ ((row / (8 / SLOTS)) & (SLOTS - 1))) << 4));
+}
+
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <bool TURN>
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&r)[4]) {
+  if constexpr (TURN)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+// c += a b: 16 x 8 += (16 x 16) (16 x 8)
+template <int F>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (F == SRS_FMT_BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <int F>
@@ -54,22 +91,14 @@ __device__ __forceinline__ uint32_t encode16(float x) {
   return __half_as_ushort(__float2half_rn(x));
 }
 
-// ------------------------------------------------- quantisation and low part --
+// ------------------------------------------------------------------ low part --
 //
-// One pass over the tokens: their rows in FP8 blocks for the projection, and the low part.
-//
-// A CTA takes up to TOKENS tokens of one adapter (tiles counted from the adapter's first; tokens of
-// none come in tiles of their own), up to 16 RT of the rank and a part of k.  Rows are gathered
-// with cp.async, 128 of k a stage, into the layout that the tensor core reads; a stage's MMAs then run
-// while the warps quantise the same bytes from shared memory, half a warp to a block of 128.
-// The parts of a cluster's CTAs are added through distributed shared memory in rank order (FP32).
-// Nearest: bound by x's bytes, read once; stochastic: by the integer units (hashes), behind
-// which the low part disappears.  As two kernels side by side, x read twice: 4096 tokens x 4096,
-// rank 64, nearest 33 us, 4096 x 14336, rank 16, stochastic 114 us; as one: RESULT.
-constexpr int kTakeStep = 128;  // of k a stage: one block, 256 bytes of a row in two boxes
-constexpr int kTakeStages = 3;
+// A CTA takes up to 128 (or 16) tokens of one adapter (tiles counted from the adapter's first), up
+// to 16 RT of the rank and a part of the sum; the parts of a cluster's CTAs are added through
+// distributed shared memory in rank order.  x's bytes, read once, bound it.  Sums are FP32.
+constexpr int kLowStep = 64;  // of k a stage: 128 bytes of a row
 
-struct TakeArgs {
+struct LowArgs {
   const char* x;  // 16-bit, rows of x_pitch elements
   const char* w;  // KINNER: rank x k a matrix; else k x rank
   int64_t x_pitch, w_pitch, w_stride;  // elements
@@ -78,33 +107,12 @@ struct TakeArgs {
   const int32_t* ends;
   const float* scale;  // null: `factor` alone
   float factor;
-  // the rows in blocks (data null: not wanted), in the adapters' order, or (spread) the batch's
-  uint8_t* data;
-  uint8_t* block_scale;
-  int64_t data_pitch, scale_pitch;
-  uint32_t counter;
-  int rule;
-  bool spread;
-  float* low;       // tokens (in order) x rank (null: not wanted)
-  uint16_t* pairs;  // items for a product (null: not wanted); spread: rows are the batch's
+  float* low;             // tokens (in order) x rank (null: not wanted)
+  uint16_t* pairs;        // items for a product (null: not wanted)
   int edge, pitch, rest_at;
+  bool spread;            // items of a thin product: rows are the batch's
   unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
   unsigned int* status;
-};
-
-template <int TOKENS, int RT>
-struct TakeShape {
-  static constexpr int kThreads = TOKENS == 16 ? 128 : 256, kRank = 16 * RT;
-  static constexpr int kBox = TOKENS * 128;           // 64 of k of all tokens
-  static constexpr int kX = 2 * kBox, kW = kTakeStep * kRank * 2;
-  static constexpr int kPitch = kRank + 1;
-  static constexpr int kSums = TOKENS * kPitch * 4;
-  // The MMA reads 128 rows of a box whatever the tile has: behind the last stage there is room for
-  // them.  What lies there reaches rows that are not read.
-  static constexpr int kSlack = kBox + kW < 128 * 128 ? 128 * 128 - kBox - kW : 0;
-  static constexpr int kSmem = 1024 + kTakeStages * (kX + kW) + kSlack;
-  static constexpr uint32_t kColumns = RT == 4 ? 64 : 32;  // of TMEM
-  static_assert(kSums <= kTakeStages * (kX + kW), "the sums fit the stages");
 };
 
 // 16-byte slot `slot` of a row of 128 bytes, turned so that 8 rows at one slot and 8 slots of a
@@ -113,40 +121,52 @@ __device__ __forceinline__ uint32_t turned_slot(int row, int slot) {
   return (uint32_t)(row * 128 + ((slot ^ (row & 7)) << 4));
 }
 
-// Rows of SLOTS (2, 4 or 8) 16-byte slots: the order of 32-, 64- and 128-byte swizzled boxes.
-template <int SLOTS>
-__device__ __forceinline__ uint32_t narrow_slot(int row, int slot) {
-  return (uint32_t)(row * 16 * SLOTS + ((slot ^ ((row / (8 / SLOTS)) & (SLOTS - 1))) << 4));
+// The CTA's part of a sum.
+struct LowTile {
+  GroupTile tile;
+  int count, rank0, ranks, first, last;  // tokens, ranks, stages of k
+  uint32_t splits, split;
+};
+
+__device__ __forceinline__ LowTile low_tile(const LowArgs& a, int most, int rank_block, int lane) {
+  LowTile t;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(t.splits));
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(t.split));
+  t.tile = find_group_tile(a.ends, a.adapters, a.tokens, most, (int)(blockIdx.x / t.splits), lane);
+  t.count = min(most, t.tile.end - t.tile.row0);
+  t.rank0 = (int)blockIdx.y * rank_block;
+  t.ranks = min(rank_block, a.rank - t.rank0);
+  const int steps = (a.k + kLowStep - 1) / kLowStep;
+  t.first = (int)((int64_t)steps * t.split / t.splits);
+  t.last = (int)((int64_t)steps * (t.split + 1) / t.splits);
+  return t;
 }
 
-// Descriptor of an operand whose rows lie side by side, 16 RT of them (one box): groups of 8 of k
-// are 256 RT bytes apart.
-template <int RT>
-__device__ __forceinline__ uint64_t narrow_descriptor() {
-  constexpr uint64_t kMode = RT == 4 ? 2 : RT == 2 ? 4 : 6;  // 128-, 64-, 32-byte swizzle
-  return (1ull << 16) | (uint64_t((256u * RT) >> 4) << 32) | (1ull << 46) | (kMode << 61);
-}
-
-// Sums of the cluster's CTAs (`sums`: [token][rank], rows of `pitch`) added, scaled and written:
-// token t of the tile by CTA t % splits.
-template <int F, int TOKENS, int RT>
-__device__ __forceinline__ void write_low(const TakeArgs& a, const GroupTile& tile, int count,
-                                          int rank0, int ranks, int splits, int split, float* sums) {
-  using S = TakeShape<TOKENS, RT>;
+// Sums of the cluster's CTAs (`sums`: [token][rank], rows of `pitch`, PARTS of them `part` apart
+// in every CTA) added, scaled and written: token t of the tile by CTA t % splits.
+template <int F, int RANK, int PARTS>
+__device__ __forceinline__ void write_low(const LowArgs& a, const LowTile& l, float* sums, int pitch,
+                                          int part, int most, int threads) {
+  const GroupTile& tile = l.tile;
+  const int splits = (int)l.splits, split = (int)l.split;
   const float factor = a.factor * (a.scale != nullptr ? __ldg(a.scale + tile.group) : 1.0f);
   if (splits > 1) cg::this_cluster().sync();
   else __syncthreads();
   float top_size = 0.0f;
-  const int whole = (ranks + 15) & ~15;
-  for (int i = threadIdx.x; i < (TOKENS + splits - 1) / splits * S::kRank; i += S::kThreads) {
-    const int t = i / S::kRank * splits + split, r = i % S::kRank;
-    if (t >= count || r >= whole) continue;
+  const int whole = (l.ranks + 15) & ~15;
+  for (int i = threadIdx.x; i < (most + splits - 1) / splits * RANK; i += threads) {
+    const int t = i / RANK * splits + split, r = i % RANK;
+    if (t >= l.count || r >= whole) continue;
     float v = 0.0f;
-    if (r < ranks) {
-      for (int p = 0; p < splits; ++p)
-        v += (splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums)[t * S::kPitch + r];
+    if (r < l.ranks) {
+      for (int p = 0; p < splits; ++p) {
+        const float* const theirs =
+            (splits > 1 ? cg::this_cluster().map_shared_rank(sums, p) : sums) + t * pitch + r;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) v += theirs[q * part];
+      }
       v *= factor;
-      if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + rank0 + r] = v;
+      if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + l.rank0 + r] = v;
       top_size = fmaxf(top_size, isfinite(v) ? fabsf(v) : 0.0f);
     }
     if (a.pairs != nullptr) {
@@ -154,7 +174,7 @@ __device__ __forceinline__ void write_low(const TakeArgs& a, const GroupTile& ti
       const int64_t at =
           a.spread ? (int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)
                    : (int64_t)(place / a.edge + tile.rank) * a.edge + place % a.edge;
-      uint16_t* const to = a.pairs + at * a.pitch + rank0 + r;
+      uint16_t* const to = a.pairs + at * a.pitch + l.rank0 + r;
       const uint32_t high = encode16<F>(v);
       const float left = v - decode16<F>(high);
       to[0] = (uint16_t)high;
@@ -165,11 +185,11 @@ __device__ __forceinline__ void write_low(const TakeArgs& a, const GroupTile& ti
     // zeros in the rows of the adapter's items that are not its own
     const int words = whole / 2;
     const auto zero = [&](int64_t row, int word) {
-      uint16_t* const p = a.pairs + row * a.pitch + rank0 + 2 * word;
+      uint16_t* const p = a.pairs + row * a.pitch + l.rank0 + 2 * word;
       *reinterpret_cast<uint32_t*>(p) = 0u;
       *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
     };
-    const int from = threadIdx.x + S::kThreads * split, step = S::kThreads * splits;
+    const int from = threadIdx.x + threads * split, step = threads * splits;
     if (a.spread) {
       if (tile.row0 == tile.start) {
         const int others = a.tokens - (tile.end - tile.start);
@@ -184,7 +204,7 @@ __device__ __forceinline__ void write_low(const TakeArgs& a, const GroupTile& ti
         for (int i = from; i < tile.start % a.edge * words; i += step)
           zero((int64_t)(tile.start / a.edge + tile.rank) * a.edge + i / words, i % words);
       const int final_row = tile.end - 1, behind = final_row % a.edge + 1;
-      if (final_row - tile.row0 < TOKENS)
+      if (final_row - tile.row0 < most)
         for (int i = from; i < (a.edge - behind) * words; i += step)
           zero((int64_t)(final_row / a.edge + tile.rank) * a.edge + behind + i / words, i % words);
     }
@@ -197,189 +217,229 @@ __device__ __forceinline__ void write_low(const TakeArgs& a, const GroupTile& ti
   if (splits > 1) cg::this_cluster().sync();  // the others have read this CTA's sums
 }
 
-template <int F, int OF, bool KINNER, int TOKENS, int RT>
-__global__ void __launch_bounds__(TakeShape<TOKENS, RT>::kThreads, 2) take_kernel(const TakeArgs a) {
-  using S = TakeShape<TOKENS, RT>;
-  // A thin product launched to overlap this kernel may start.
+// Calls of few tokens, where most adapters have one or two: 16 tokens, and 4 warps that share a
+// stage's four steps of 16 of k with mma.sync.  Latency bounds them: launch, the ends, the order and
+// the first bytes one after the other, and the cluster's meeting.
+template <int RT>
+struct FewShape {
+  static constexpr int kTokens = 16, kWarps = 4, kThreads = 128, kRank = 16 * RT, kStages = 8;
+  static constexpr int kX = kTokens * kLowStep * 2, kW = kRank * kLowStep * 2;
+  static constexpr int kPitch = kRank + 1;
+  static constexpr int kSums = kWarps * kTokens * kPitch * 4;
+  static constexpr int kSmem = kStages * (kX + kW) > kSums ? kStages * (kX + kW) : kSums;
+};
+
+template <int F, bool KINNER, int RT>
+__global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(const LowArgs a) {
+  using S = FewShape<RT>;
+  // The quantisation behind this kernel reads nothing of it and waits for it at its end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(128) uint8_t raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const LowTile l = low_tile(a, S::kTokens, S::kRank, lane);
+  if (l.tile.group < 0) return;  // the whole cluster
+  const uint32_t base = smem_address(raw);
+  const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const char* const from =
+      a.x + (row < l.count ? token_at(a.order, l.tile.row0 + row, a.tokens) : 0) * a.x_pitch * 2;
+  const char* const w = a.w + (int64_t)l.tile.group * a.w_stride * 2;
+  const auto load = [&](int step, int s) {
+    const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
+    const uint32_t to = base + (uint32_t)(s * (S::kX + S::kW));
+    copy16(to + turned_slot(row, slot), bytes > 0 ? from + 2 * k : a.x, row < l.count ? bytes : 0);
+    if (KINNER) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = row + 16 * i;
+        const bool in = r < l.ranks && bytes > 0;
+        copy16(to + S::kX + turned_slot(r, slot),
+               in ? w + ((int64_t)(l.rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
+      }
+    } else {
+      // 64 rows of k, 2 RT slots of 8 of the rank each
+#pragma unroll
+      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += S::kThreads) {
+        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
+        const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
+        const bool in = kk < a.k && left > 0;
+        copy16(to + S::kX + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)),
+               in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
+      }
+    }
+  };
+  float sum[2 * RT][4];
+#pragma unroll
+  for (int i = 0; i < 2 * RT; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
+  }
+  for (int i = 0; i < S::kStages - 1; ++i) {
+    if (l.first + i < l.last) load(l.first + i, i);
+    copies_done();
+  }
+  int s = 0;
+  for (int step = l.first; step < l.last; ++step) {
+    copies_wait<S::kStages - 2>();
+    __syncthreads();
+    if (step + S::kStages - 1 < l.last) load(step + S::kStages - 1, s == 0 ? S::kStages - 1 : s - 1);
+    copies_done();
+    const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW)), ws = xs + S::kX;
+    if (++s == S::kStages) s = 0;
+    uint32_t m[4];
+    load_matrices<false>(xs + turned_slot(lane & 15, 2 * warp + (lane >> 4)), m);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      uint32_t b[4];
+      if (KINNER) {  // ranks 16 j + (0..15) x k 16 warp ..
+        load_matrices<false>(ws + turned_slot(16 * j + (lane & 7) + ((lane >> 4) << 3),
+                                              2 * warp + ((lane >> 3) & 1)), b);
+      } else {       // k 16 warp + (0..15) x ranks 16 j ..
+        const int r = 16 * warp + (lane & 15), c = 2 * j + (lane >> 4);
+        load_matrices<true>(ws + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)), b);
+      }
+      multiply<F>(sum[2 * j], m, b[0], b[1]);
+      multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
+    }
+  }
+  // every warp's sums to shared memory
+  copies_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(raw);
+  float* const mine = sums + warp * S::kTokens * S::kPitch;
+#pragma unroll
+  for (int j = 0; j < 2 * RT; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mine[((lane >> 2) + 8 * (i >> 1)) * S::kPitch + 8 * j + 2 * (lane & 3) + (i & 1)] = sum[j][i];
+  }
+  write_low<F, S::kRank, S::kWarps>(a, l, sums, S::kPitch, S::kTokens * S::kPitch, S::kTokens,
+                                    S::kThreads);
+}
+
+// Many tokens: 128 of one adapter (the rows of an MMA), gathered with cp.async into the layout that
+// the tensor core reads, so that a stage's four MMAs need nothing of the warps.  A stage is loaded
+// again once the MMAs of two stages before have read theirs.  (With ldmatrix and mma.sync in 8
+// warps shared memory was read five times as often: 4096 tokens, 4096 -> 64: 25 us; so RESULT.)
+constexpr int kManyTokens = 128, kManyThreads = 256;
+
+template <int RT>
+struct ManyShape {
+  static constexpr int kRank = 16 * RT;
+  static constexpr int kX = kManyTokens * 128, kW = kLowStep * 128;
+  static constexpr int kStages = 4;  // two CTAs an SM fit
+  static constexpr int kPitch = kRank + 1;
+  static constexpr int kSmem = 1024 + kStages * (kX + kW);
+  static constexpr uint32_t kColumns = RT == 4 ? 64 : 32;  // of TMEM
+  static_assert(kManyTokens * kPitch * 4 <= kStages * (kX + kW), "the sums fit the stages");
+};
+
+template <int F, bool KINNER, int RT>
+__global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs a) {
+  using S = ManyShape<RT>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t raw[];
-  __shared__ int32_t places[TOKENS];
-  __shared__ __align__(8) uint64_t bars[kTakeStages];
+  __shared__ __align__(8) uint64_t bars[S::kStages];
   __shared__ uint32_t tmem_slot;
   const int lane = threadIdx.x & 31, warp = warp_index();
-  uint32_t splits, split;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
-  GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, TOKENS,
-                                   (int)(blockIdx.x / splits), lane);
-  const bool some = tile.group >= 0;
-  if (!some) {
-    // tokens of no adapter, from the last of the grid's tiles backwards
-    const int back = (int)(gridDim.x / splits) - 1 - (int)(blockIdx.x / splits);
-    tile.row0 = tile.end + TOKENS * back;
-    tile.end = a.tokens;
-  }
-  const bool quantise = a.data != nullptr && blockIdx.y == 0;
-  // (the whole cluster)
-  if (tile.row0 >= tile.end || (!some && !quantise)) return;
-  const int count = min(TOKENS, tile.end - tile.row0);
-  const int rank0 = (int)blockIdx.y * S::kRank, ranks = min(S::kRank, a.rank - rank0);
-  const int blocks = (a.k + kTakeStep - 1) / kTakeStep;
-  const int first = (int)((int64_t)blocks * split / splits);
-  const int steps = (int)((int64_t)blocks * (split + 1) / splits) - first;
-
+  const LowTile l = low_tile(a, kManyTokens, S::kRank, lane);
+  if (l.tile.group < 0) return;  // the whole cluster
   const uint32_t base = (smem_address(raw) + 1023u) & ~1023u, bar0 = smem_address(bars);
-  if (threadIdx.x < TOKENS)
-    places[threadIdx.x] = (int)threadIdx.x < count
-                              ? (int32_t)token_at(a.order, tile.row0 + threadIdx.x, a.tokens) : 0;
-  if (threadIdx.x == S::kThreads - 1) {
-    for (int i = 0; i < kTakeStages; ++i) barrier_init(bar0 + 8 * i, 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) barrier_init(bar0 + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (some && warp == 1) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
+  if (warp == 1) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
+
+  // this thread's rows of x: threadIdx.x / 8 + 32 i, slot threadIdx.x % 8
+  const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const char* from[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row + 32 * i;
+    from[i] = a.x + (r < l.count ? token_at(a.order, l.tile.row0 + r, a.tokens) : 0) * a.x_pitch * 2;
+  }
+  const char* const w = a.w + (int64_t)l.tile.group * a.w_stride * 2;
+  const auto load = [&](int step, int s) {
+    const int k = step * kLowStep + 8 * slot, bytes = min(max(a.k - k, 0) * 2, 16);
+    const uint32_t to = base + (uint32_t)(s * (S::kX + S::kW));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 32 * i;
+      if (32 * i < l.count)  // sums of the rows behind are not read
+        copy16(to + turned_slot(r, slot), bytes > 0 ? from[i] + 2 * k : a.x,
+               r < l.count ? bytes : 0);
+    }
+    if (KINNER) {
+#pragma unroll
+      for (int i = 0; i < (S::kRank + 31) / 32; ++i) {
+        const int r = row + 32 * i;
+        const bool in = r < l.ranks && bytes > 0;
+        if (r < S::kRank)
+          copy16(to + S::kX + turned_slot(r, slot),
+                 in ? w + ((int64_t)(l.rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
+      }
+    } else {
+      // 64 rows of k, of which 2 RT slots of 8 of the rank are read
+#pragma unroll
+      for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += kManyThreads) {
+        const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
+        const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
+        const bool in = kk < a.k && left > 0;
+        copy16(to + S::kX + turned_slot(r, c),
+               in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
+      }
+    }
+  };
+  for (int i = 0; i < S::kStages - 2; ++i) {
+    if (l.first + i < l.last) load(l.first + i, i);
+    copies_done();
+  }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
-
-  const char* const w = a.w + (int64_t)(some ? tile.group : 0) * a.w_stride * 2;
-  const auto load = [&](int step, int s) {
-    const uint32_t to = base + (uint32_t)(s * (S::kX + S::kW));
-    const int k0 = (first + step) * kTakeStep;
-    {
-      const int slot = threadIdx.x & 15, row = threadIdx.x >> 4, k = k0 + 8 * slot;
-      const int bytes = min(max(a.k - k, 0) * 2, 16);
-#pragma unroll
-      for (int i = 0; i < TOKENS * 16 / S::kThreads; ++i) {
-        const int r = row + i * (S::kThreads / 16);
-        copy16(to + (slot >> 3) * S::kBox + turned_slot(r, slot & 7),
-               r < count && bytes > 0 ? a.x + (places[r] * a.x_pitch + k) * 2 : a.x,
-               r < count ? bytes : 0);
-      }
-    }
-    if (!some) return;
-    if (KINNER) {
-      // two boxes of 64 of k, the rank's rows
-#pragma unroll
-      for (int i = threadIdx.x; i < S::kRank * 16; i += S::kThreads) {
-        const int r = i >> 4, slot = i & 15, k = k0 + 8 * slot;
-        const int bytes = r < ranks ? min(max(a.k - k, 0) * 2, 16) : 0;
-        copy16(to + S::kX + (slot >> 3) * (S::kRank * 128) + turned_slot(r, slot & 7),
-               bytes > 0 ? w + ((int64_t)(rank0 + r) * a.w_pitch + k) * 2 : w, bytes);
-      }
-    } else {
-      // rows of k, ranks side by side
-#pragma unroll
-      for (int i = threadIdx.x; i < kTakeStep * 2 * RT; i += S::kThreads) {
-        const int r = i / (2 * RT), c = i % (2 * RT), k = k0 + r;
-        const int bytes = k < a.k ? min(max(ranks - 8 * c, 0) * 2, 16) : 0;
-        copy16(to + S::kX + narrow_slot<2 * RT>(r, c),
-               bytes > 0 ? w + ((int64_t)k * a.w_pitch + rank0 + 8 * c) * 2 : w, bytes);
-      }
-    }
-  };
-
-  // half a warp to a block of 128; kRows rows at a time, as far apart as there are half-warps
-  constexpr int kHalves = S::kThreads / 16, kRows = TOKENS / kHalves < 4 ? TOKENS / kHalves : 4;
-  const int lane16 = threadIdx.x & 15;
-  const auto quantise_stage = [&](int step, int s) {
-    const uint32_t from = base + (uint32_t)(s * (S::kX + S::kW)) + (lane16 >> 3) * S::kBox;
-    const int block = first + step, col = block * kTakeStep + 8 * lane16;
-    const int cols_left = min(a.k - col, kVec);
-#pragma unroll 1
-    for (int q0 = 2 * warp; q0 < count; q0 += kRows * kHalves) {  // the same for the whole warp
-      const int r0 = q0 + (lane >> 4);
-      uint32_t words[kRows][4];
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int r = r0 + i * kHalves;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(words[i][0]), "=r"(words[i][1]), "=r"(words[i][2]), "=r"(words[i][3])
-                     : "r"(from + turned_slot(r < TOKENS ? r : 0, lane16 & 7))
-                     : "memory");
-      }
-      uint32_t top = row_sizes<F, kRows>(words, lane16);
-      bool plain = !__any_sync(0xFFFFFFFFu, top >= Size<F>::kInfinite);
-      if (!plain) {
-        uint32_t sizes[kRows][4];
-        only_finite<F>(words, sizes);
-        top = row_sizes<F, kRows>(sizes, lane16);
-      }
-      const int own_k = block_exponent<OF>(Size<F>::as_f32(top));
-      if (lane16 < kRows) {
-        const int r = r0 + lane16 * kHalves;
-        if (r < count)
-          a.block_scale[(a.spread ? places[r] : (int64_t)(tile.row0 + r)) * a.scale_pitch + block] =
-              (uint8_t)(own_k + 127);
-      }
-      const float own_factor = power_of_two(-own_k);
-      plain = plain && a.rule != SRS_RULE_TOWARD_ZERO;
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int r = r0 + i * kHalves;
-        const float factor = __shfl_sync(0xFFFFFFFFu, own_factor, i, 16);
-        if (r >= count) continue;
-        float y[kVec];
-        decode8<F>(words[i], y);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) y[j] *= factor;
-        const int64_t token = places[r], to = a.spread ? token : tile.row0 + r;
-        const uint2 q = encode_values<OF>(y, a.counter + (uint32_t)(token * a.k + col), a.rule, plain);
-        store_bytes(a.data + to * a.data_pitch + col, q, cols_left);
-      }
-    }
-  };
-
   constexpr uint32_t kInstruction = (uint32_t)(S::kRank >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
                                     (F == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u) |
                                     (KINNER ? 0u : 1u << 16);
-  for (int i = 0; i < kTakeStages - 1; ++i) {
-    if (i < steps) load(i, i);
-    copies_done();
-  }
   bool ok = true;
+  const int steps = l.last - l.first;
   for (int i = 0; i < steps; ++i) {
-    const int s = i % kTakeStages;
-    // what the threads have copied, for the tensor core; all are done with step i - 1's stage
-    copies_wait<kTakeStages - 2>();
+    const int s = i % S::kStages;
+    // what the threads have copied, for the tensor core
+    copies_wait<S::kStages - 3>();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    if (some && warp == 0) {
+    if (warp == 0) {
       if (elect_lane()) {
-        const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW)), ws = xs + S::kX;
+        const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW));
+        const uint64_t dx = operand_descriptor(false) | uint64_t((xs >> 4) & 0x3FFFu);
+        const uint64_t dw = operand_descriptor(!KINNER) | uint64_t(((xs + S::kX) >> 4) & 0x3FFFu);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t xj = xs + (j >> 2) * S::kBox + 32 * (j & 3);
-          const uint32_t wj = KINNER ? ws + (j >> 2) * (S::kRank * 128) + 32 * (j & 3)
-                                     : ws + j * 512 * RT;
-          const uint64_t dx = operand_descriptor(false) | uint64_t((xj >> 4) & 0x3FFFu);
-          const uint64_t dw = (KINNER ? operand_descriptor(false) : narrow_descriptor<RT>()) |
-                              uint64_t((wj >> 4) & 0x3FFFu);
-          mma_f16<1>(tmem, dx, dw, kInstruction, (i | j) != 0 ? 1u : 0u);
-        }
+        for (int j = 0; j < 4; ++j)
+          mma_f16<1>(tmem, dx + 2 * j, dw + j * (KINNER ? 2u : 128u), kInstruction,
+                     (i | j) != 0 ? 1u : 0u);
         mma_commit<1>(bar0 + 8 * s);
       }
       __syncwarp();
     }
-    if (i + kTakeStages - 1 < steps) {
-      if (some && ok && i >= 1)
-        ok = barrier_wait(bar0 + 8 * ((i - 1) % kTakeStages), ((i - 1) / kTakeStages) & 1, a.status,
+    // stage s - 2 for step i + kStages - 2
+    if (i + S::kStages - 2 < steps) {
+      if (ok && i >= 2)
+        ok = barrier_wait(bar0 + 8 * ((i - 2) % S::kStages), ((i - 2) / S::kStages) & 1, a.status,
                           1u << 18);
-      if (ok) load(i + kTakeStages - 1, (i + kTakeStages - 1) % kTakeStages);
+      if (ok) load(l.first + i + S::kStages - 2, (i + S::kStages - 2) % S::kStages);
     }
     copies_done();
-    if (quantise) quantise_stage(i, s);
   }
   copies_wait<0>();
-  if (!some) return;
   // the last MMAs (those before are done with them)
   if (ok && steps > 0)
-    barrier_wait(bar0 + 8 * ((steps - 1) % kTakeStages), ((steps - 1) / kTakeStages) & 1, a.status,
+    barrier_wait(bar0 + 8 * ((steps - 1) % S::kStages), ((steps - 1) / S::kStages) & 1, a.status,
                  1u << 18);
   tmem_fence_after();
   __syncthreads();  // no thread still copies or reads a stage
   float* const sums = reinterpret_cast<float*>(raw + (base - smem_address(raw)));
-  if (warp < 4 && 32 * warp < TOKENS) {
+  if (warp < 4) {
     const int t = 32 * warp + lane;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
@@ -387,11 +447,11 @@ __global__ void __launch_bounds__(TakeShape<TOKENS, RT>::kThreads, 2) take_kerne
       tmem_load16(tmem + ((uint32_t)(32 * warp) << 16) + 16 * j, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (t < TOKENS) sums[t * S::kPitch + 16 * j + i] = steps > 0 ? __uint_as_float(v[i]) : 0.0f;
+        sums[t * S::kPitch + 16 * j + i] = steps > 0 ? __uint_as_float(v[i]) : 0.0f;
     }
   }
   tmem_fence_before();
-  write_low<F, TOKENS, RT>(a, tile, count, rank0, ranks, (int)splits, (int)split, sums);
+  write_low<F, S::kRank, 1>(a, l, sums, S::kPitch, 0, kManyTokens, kManyThreads);
   __syncthreads();
   tmem_fence_after();
   if (warp == 1) tmem_free<1>(tmem, S::kColumns);
@@ -635,21 +695,18 @@ int allow_shared(const void* kernel, int bytes) {
   return prepare_kernel(kernel, 1, 32, bytes, &resident);
 }
 
-template <int F, int OF, bool KINNER, int TOKENS, int RT>
-int launch_take_as(const TakeArgs& args, cudaStream_t stream) {
-  using S = TakeShape<TOKENS, RT>;
-  const auto kernel = &take_kernel<F, OF, KINNER, TOKENS, RT>;
-  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+// `room`: CTAs that run at once.
+int launch_low_kernel(const void* kernel, const LowArgs& args, int most, int rank_block, int threads,
+                      int smem, int64_t room, cudaStream_t stream) {
+  if (int rc = allow_shared(kernel, smem)) return rc;
   const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
-  // one more tile than adapters' tokens can take: tokens of none in a last, partial one
-  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, TOKENS) + 1;
-  const int64_t blocks = ceil_div(args.rank, S::kRank), steps = ceil_div(args.k, kTakeStep);
-  // Parts of k while all likely CTAs run at once, at least two stages each.  A second round costs
-  // as much as the first.
-  const int64_t likely = (args.tokens / TOKENS + (busy + 1) / 2) * blocks;
-  const int64_t room = sm_count() * (S::kThreads == 256 ? 2 : RT == 4 ? 3 : 4);
+  const int64_t tiles = most_group_tiles(args.tokens, args.adapters, most);
+  const int64_t blocks = ceil_div(args.rank, rank_block), steps = ceil_div(args.k, kLowStep);
+  // Parts of the sum while all likely CTAs run at once, at least four stages each.  A second round
+  // costs as much as the first: 16 prompts of 4096 tokens in all, 4096 -> 64, took 30 us in 384 CTAs.
+  const int64_t likely = (args.tokens / most + (busy + 1) / 2) * blocks;
   int64_t splits = likely > 0 ? room / likely : 8;
-  if (splits > steps / 2) splits = steps / 2;
+  if (splits > steps / 4) splits = steps / 4;
   splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
   cudaLaunchConfig_t config{};
   cudaLaunchAttribute cluster{};
@@ -657,37 +714,34 @@ int launch_take_as(const TakeArgs& args, cudaStream_t stream) {
   cluster.val.clusterDim.x = (unsigned)splits;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.gridDim = dim3((unsigned)(tiles * splits), (unsigned)blocks);
-  config.blockDim = dim3(S::kThreads);
-  config.dynamicSmemBytes = S::kSmem;
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = (size_t)smem;
   config.stream = stream;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args);
-  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "quantisation and low part launch");
+  LowArgs copy = args;
+  void* arguments[1] = {&copy};
+  const cudaError_t e = cudaLaunchKernelExC(&config, kernel, arguments);
+  return e == cudaSuccess ? SRS_OK : cuda_fail(e, "low part launch");
 }
 
-// 16 tokens a tile for calls of few tokens, where most adapters have one or two; else 128, or 64
-// where wider ranks leave less shared memory.
-template <int F, int OF, bool KINNER>
-int launch_take(const TakeArgs& args, bool thin, cudaStream_t stream) {
-  if (args.rank <= 16)
-    return thin ? launch_take_as<F, OF, KINNER, 16, 1>(args, stream)
-                : launch_take_as<F, OF, KINNER, 128, 1>(args, stream);
-  if (args.rank <= 32)
-    return thin ? launch_take_as<F, OF, KINNER, 16, 2>(args, stream)
-                : launch_take_as<F, OF, KINNER, 64, 2>(args, stream);
-  return thin ? launch_take_as<F, OF, KINNER, 16, 4>(args, stream)
-              : launch_take_as<F, OF, KINNER, 64, 4>(args, stream);
+template <int F, bool KINNER, int RT>
+int launch_low_as(const LowArgs& args, bool thin, cudaStream_t stream) {
+  const int64_t sms = sm_count();
+  if (thin)
+    return launch_low_kernel(reinterpret_cast<const void*>(&low_few_kernel<F, KINNER, RT>), args,
+                             FewShape<RT>::kTokens, FewShape<RT>::kRank, FewShape<RT>::kThreads,
+                             FewShape<RT>::kSmem, (RT == 4 ? 2 : 4) * sms, stream);
+  return launch_low_kernel(reinterpret_cast<const void*>(&low_many_kernel<F, KINNER, RT>), args,
+                           kManyTokens, ManyShape<RT>::kRank, kManyThreads, ManyShape<RT>::kSmem,
+                           2 * sms, stream);
 }
 
-template <int F>
-int launch_take(const TakeArgs& args, int block_format, bool turned, bool thin,
-                cudaStream_t stream) {
-  if (block_format == SRS_FMT_E4M3)
-    return turned ? launch_take<F, SRS_FMT_E4M3, false>(args, thin, stream)
-                  : launch_take<F, SRS_FMT_E4M3, true>(args, thin, stream);
-  return turned ? launch_take<F, SRS_FMT_E5M2, false>(args, thin, stream)
-                : launch_take<F, SRS_FMT_E5M2, true>(args, thin, stream);
+template <int F, bool KINNER>
+int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
+  if (args.rank <= 16) return launch_low_as<F, KINNER, 1>(args, thin, stream);
+  if (args.rank <= 32) return launch_low_as<F, KINNER, 2>(args, thin, stream);
+  return launch_low_as<F, KINNER, 4>(args, thin, stream);
 }
 
 template <int F, int RT>
@@ -782,9 +836,6 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   if (k > 0 && (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0 || x_pitch % 8 != 0 ||
                 x_pitch < k))
     return fail(SRS_ERR_INVALID_ARGUMENT, "x needs a 16-byte aligned address and row pitch");
-  if ((block_format != SRS_FMT_E4M3 && block_format != SRS_FMT_E5M2) || !valid_rule(rule))
-    return fail(SRS_ERR_INVALID_ARGUMENT, "unknown block format %d or rounding rule %d",
-                block_format, rule);
   if (n > 0 && reinterpret_cast<uintptr_t>(d) % 2 != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "misaligned result pointer");
   const AdapterSpace space = adapter_space(tokens, k, n, a->count, a->rank);
@@ -807,7 +858,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
   const int edge = n == 0 ? 0 : thin ? thin_columns(tokens) : adapter_edge(tokens, n, k);
   const PairShape pairs = pair_shape(a->rank);
-  TakeArgs l{};
+  LowArgs l{};
   l.x = static_cast<const char*>(x);
   l.w = reinterpret_cast<const char*>(turned ? a->up : a->down);
   l.x_pitch = x_pitch;
@@ -824,30 +875,32 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.low = low;
   l.largest = largest;
   if (int rc = status_word(&l.status)) return rc;
-  srs_blocks rows{};
-  if (n > 0) {
+  if (edge != 0) {
     l.pairs = reinterpret_cast<uint16_t*>(at + space.low);
     l.edge = edge;
     l.pitch = pairs.pitch;
     l.rest_at = pairs.rest_at;
     l.spread = thin;
-    rows.data = reinterpret_cast<uint64_t>(workspace);
-    rows.rows = tokens;
-    rows.pitch = ceil_div(k, 16) * 16;
-    rows.scale = rows.data + (uint64_t)(tokens * rows.pitch);
-    rows.scale_pitch = ceil_div(k, 128);
-    rows.format = block_format;
-    l.data = reinterpret_cast<uint8_t*>(rows.data);
-    l.block_scale = reinterpret_cast<uint8_t*>(rows.scale);
-    l.data_pitch = rows.pitch;
-    l.scale_pitch = rows.scale_pitch;
-    l.counter = block_counter(seed, 0u, 0u);
-    l.rule = rule;
   }
-  if (int rc = bf16 ? launch_take<SRS_FMT_BF16>(l, block_format, turned != 0, thin, st)
-                    : launch_take<SRS_FMT_F16>(l, block_format, turned != 0, thin, st))
+  if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, thin, st)
+                              : launch_low<SRS_FMT_F16, false>(l, thin, st))
+                      : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, thin, st)
+                              : launch_low<SRS_FMT_F16, true>(l, thin, st)))
     return rc;
   if (n == 0 || k == 0) return SRS_OK;
+
+  srs_blocks rows{};
+  rows.data = reinterpret_cast<uint64_t>(workspace);
+  rows.rows = tokens;
+  rows.pitch = ceil_div(k, 16) * 16;
+  rows.scale = rows.data + (uint64_t)(tokens * rows.pitch);
+  rows.scale_pitch = ceil_div(k, 128);
+  rows.format = block_format;
+  QuantizeCall q{x, a->format, tokens, k, x_pitch, block_format, rule, false, seed, 0u};
+  q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
+  q.order = thin ? nullptr : l.order;
+  q.overlap = true;  // beside the low part
+  if (int rc = quantize(q, st)) return rc;
   const AdapterCall call{l.pairs,
                          reinterpret_cast<const void*>(turned ? a->down : a->up),
                          turned ? a->down_pitch : a->up_pitch,
@@ -858,7 +911,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
                          a->format,
                          l.order,
                          l.ends};
-  // (with few tokens beside the kernel ahead: the weights are streamed first)
+  // (with few tokens beside the quantisation: the weights are streamed first)
   return thin ? launch_thin(*w, rows, k, d, a->format, 1, n, true, st, &call)
               : launch_adapter_product(rows, *w, k, call, edge, d, st);
 }

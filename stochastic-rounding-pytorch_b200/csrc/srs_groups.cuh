@@ -62,7 +62,7 @@ __device__ __forceinline__ void group_span(const int32_t* __restrict__ ends, con
 
 // One tile of `edge` rows at most, counted from its group's first row.
 struct GroupTile {
-  int group;      // -1: there is no such tile (`end` is then the last group's end)
+  int group;      // -1: there is no such tile
   int row0, end;  // first row of the tile, end of its group
   int start;      // first row of its group
   int rank;       // groups with rows before it
@@ -97,7 +97,6 @@ __device__ __forceinline__ GroupTile find_group_tile(const int32_t* __restrict__
     quads_before = __shfl_sync(0xFFFFFFFFu, quads_upto, 31);
     rank += __popc(some);
   }
-  r.end = carry;
   return r;
 }
 

@@ -42,8 +42,9 @@ int launch_groups(const void* kernel, int64_t groups, int group, int threads, in
                   bool overlap = false);
 
 // What is quantised to FP8 blocks, and where to (srs_quantize_blocks, _stack and _groups):
-// one matrix, a stack of them (`matrices`, `x_stride` elements apart), or rows of groups (`ends`;
-// the transposed copy in the products' form).  `for_product`: ahead of a product of the same call.
+// one matrix, a stack of them (`matrices`, `x_stride` elements apart), rows of groups (`ends`;
+// the transposed copy in the products' form), or rows in another order (`order`: row i of
+// the copy is row order[i] of x; rows alone).  `for_product`: ahead of a product of the same call.
 struct QuantizeCall {
   const void* x;
   int x_format;
@@ -55,7 +56,9 @@ struct QuantizeCall {
   int64_t matrices = 1, x_stride = 0;
   const int32_t* ends = nullptr;
   int groups = 0;
+  const int32_t* order = nullptr;
   bool for_product = false;
+  bool overlap = false;  // rows alone: may start beside the kernel ahead, which it reads nothing of
 };
 int quantize(const QuantizeCall& q, cudaStream_t stream);
 
