@@ -35,10 +35,19 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
-// Rows of SLOTS (2 or 4) 16-byte slots, turned as rows of 8 are.
+// Rows of SLOTS (2, 4 or 8) 16-byte slots, turned so that 8 rows at one slot reach all banks: the
+// order of 32-, 64- and 128-byte swizzled boxes.
 template <int SLOTS>
 __device__ __forceinline__ uint32_t narrow_slot(int row, int slot) {
   return (uint32_t)(row * 16 * SLOTS + ((slot ^ ((row / (8 / SLOTS)) & (SLOTS - 1))) << 4));
+}
+
+// Descriptor of such an operand with 16 RT rows side by side: groups of 8 of k are 256 RT bytes
+// apart.
+template <int RT>
+__device__ __forceinline__ uint64_t narrow_descriptor() {
+  constexpr uint64_t kMode = RT == 4 ? 2 : RT == 2 ? 4 : 6;  // 128-, 64-, 32-byte swizzle
+  return (1ull << 16) | (uint64_t((256u * RT) >> 4) << 32) | (1ull << 46) | (kMode << 61);
 }
 
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(cons
         const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
         const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
         const bool in = kk < a.k && left > 0;
-        copy16(to + S::kX + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)),
+        copy16(to + S::kX + narrow_slot<2 * RT>(r, c),
                in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
       }
     }
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(cons
                                               2 * warp + ((lane >> 3) & 1)), b);
       } else {       // k 16 warp + (0..15) x ranks 16 j ..
         const int r = 16 * warp + (lane & 15), c = 2 * j + (lane >> 4);
-        load_matrices<true>(ws + (RT == 4 ? turned_slot(r, c) : narrow_slot<2 * RT>(r, c)), b);
+        load_matrices<true>(ws + narrow_slot<2 * RT>(r, c), b);
       }
       multiply<F>(sum[2 * j], m, b[0], b[1]);
       multiply<F>(sum[2 * j + 1], m, b[2], b[3]);
@@ -325,8 +334,8 @@ constexpr int kManyTokens = 128, kManyThreads = 256;
 template <int RT>
 struct ManyShape {
   static constexpr int kRank = 16 * RT;
-  static constexpr int kX = kManyTokens * 128, kW = kLowStep * 128;
-  static constexpr int kStages = 4;  // two CTAs an SM fit
+  static constexpr int kX = kManyTokens * 128, kW = kLowStep * kRank * 2;
+  static constexpr int kStages = RT == 1 ? 6 : RT == 2 ? 5 : 4;  // two CTAs an SM fit
   static constexpr int kPitch = kRank + 1;
   static constexpr int kSmem = 1024 + kStages * (kX + kW);
   static constexpr uint32_t kColumns = RT == 4 ? 64 : 32;  // of TMEM
@@ -379,13 +388,13 @@ __global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs
                  in ? w + ((int64_t)(l.rank0 + r) * a.w_pitch + k) * 2 : w, in ? bytes : 0);
       }
     } else {
-      // 64 rows of k, of which 2 RT slots of 8 of the rank are read
+      // 64 rows of k, 2 RT slots of 8 of the rank each
 #pragma unroll
       for (int i = threadIdx.x; i < kLowStep * 2 * RT; i += kManyThreads) {
         const int r = i / (2 * RT), c = i % (2 * RT), kk = step * kLowStep + r;
         const int left = min(max(l.ranks - 8 * c, 0) * 2, 16);
         const bool in = kk < a.k && left > 0;
-        copy16(to + S::kX + turned_slot(r, c),
+        copy16(to + S::kX + narrow_slot<2 * RT>(r, c),
                in ? w + ((int64_t)kk * a.w_pitch + l.rank0 + 8 * c) * 2 : w, in ? left : 0);
       }
     }
@@ -413,10 +422,11 @@ __global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs
       if (elect_lane()) {
         const uint32_t xs = base + (uint32_t)(s * (S::kX + S::kW));
         const uint64_t dx = operand_descriptor(false) | uint64_t((xs >> 4) & 0x3FFFu);
-        const uint64_t dw = operand_descriptor(!KINNER) | uint64_t(((xs + S::kX) >> 4) & 0x3FFFu);
+        const uint64_t dw = (KINNER ? operand_descriptor(false) : narrow_descriptor<RT>()) |
+                            uint64_t(((xs + S::kX) >> 4) & 0x3FFFu);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          mma_f16<1>(tmem, dx + 2 * j, dw + j * (KINNER ? 2u : 128u), kInstruction,
+          mma_f16<1>(tmem, dx + 2 * j, dw + j * (KINNER ? 2u : 32u * RT), kInstruction,
                      (i | j) != 0 ? 1u : 0u);
         mma_commit<1>(bar0 + 8 * s);
       }
@@ -466,10 +476,16 @@ __global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs
 // with cp.async into the layout in which the tensor core reads tokens as k.  `low` enters as a
 // pair of 16-bit numbers (high and what it leaves); in FP16 both are scaled by a power of two that
 // brings the adapter's largest to 2^11 .. 2^12, so that small gradients keep their digits.
-constexpr int kSumCols = 128, kSumStep = 64, kSumThreads = 256, kSumStages = 4;
+constexpr int kSumCols = 128, kSumStep = 64, kSumThreads = 256;
 constexpr int kSumChunk = 1024;  // most tokens of a chunk
-constexpr int kSumZ = kSumStep * kSumCols * 2, kSumLow = kSumStep * 128;
-constexpr int kSumSmem = 1024 + kSumStages * kSumZ + 2 * 2 * kSumLow;  // two CTAs an SM fit
+constexpr int kSumZ = kSumStep * kSumCols * 2;
+
+template <int RT>
+struct SumShape {
+  static constexpr int kRank = 16 * RT, kLow = kSumStep * kRank * 2;
+  static constexpr int kStages = RT == 1 ? 6 : RT == 2 ? 5 : 4;  // two CTAs an SM fit
+  static constexpr int kSmem = 1024 + kStages * kSumZ + 2 * 2 * kLow;
+};
 
 struct SumArgs {
   const char* z;
@@ -496,7 +512,7 @@ __device__ __forceinline__ float pair_scale(const unsigned int* largest, int gro
 
 template <int F, int RT>
 __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
-  constexpr int kRank = 16 * RT;
+  constexpr int kRank = 16 * RT, kSumStages = SumShape<RT>::kStages, kSumLow = SumShape<RT>::kLow;
   constexpr uint32_t kColumns = RT == 4 ? 64 : 32;
   extern __shared__ uint8_t raw[];
   __shared__ int32_t places[kSumChunk];
@@ -573,7 +589,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
         rest[i] = encode16<F>(x - decode16<F>(hx)) | encode16<F>(y - decode16<F>(hy)) << 16;
       }
       // 8 of the 16 bytes of a slot
-      const uint32_t at = to + turned_slot(low_row, 2 * j + (low_col >> 3)) + 2 * (low_col & 7);
+      const uint32_t at = to + narrow_slot<2 * RT>(low_row, 2 * j + (low_col >> 3)) + 2 * (low_col & 7);
       asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(high[0]), "r"(high[1])
                    : "memory");
       asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + kSumLow), "r"(rest[0]),
@@ -594,7 +610,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
   bool ok = true;
   for (int i = 0; i < steps; ++i) {
     const int s = i % kSumStages;
-    // the MMAs of step i - 2 have read this step's buffer of low, and the stage of step i + 2
+    // the MMAs of step i - 2 have read this step's buffer of low, and the stage loaded below
     if (ok && i >= 2)
       ok = barrier_wait(bar0 + 8 * ((i - 2) % kSumStages), ((i - 2) / kSumStages) & 1, a.status,
                         1u << 19);
@@ -606,12 +622,12 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
       if (elect_lane()) {
         const uint32_t zs = z0 + s * kSumZ, ls = low0 + (i & 1) * 2 * kSumLow;
         const uint64_t dz = operand_descriptor(true) | uint64_t((zs >> 4) & 0x3FFFu);
-        const uint64_t dl = operand_descriptor(true) | uint64_t((ls >> 4) & 0x3FFFu);
-        const uint64_t dr = operand_descriptor(true) | uint64_t(((ls + kSumLow) >> 4) & 0x3FFFu);
+        const uint64_t dl = narrow_descriptor<RT>() | uint64_t((ls >> 4) & 0x3FFFu);
+        const uint64_t dr = narrow_descriptor<RT>() | uint64_t(((ls + kSumLow) >> 4) & 0x3FFFu);
 #pragma unroll
         for (int j = 0; j < kSumStep / 16; ++j) {
-          mma_f16<1>(tmem, dz + 128 * j, dr + 128 * j, kInstruction, (i | j) != 0 ? 1u : 0u);
-          mma_f16<1>(tmem, dz + 128 * j, dl + 128 * j, kInstruction, 1u);
+          mma_f16<1>(tmem, dz + 128 * j, dr + 32 * RT * j, kInstruction, (i | j) != 0 ? 1u : 0u);
+          mma_f16<1>(tmem, dz + 128 * j, dl + 32 * RT * j, kInstruction, 1u);
         }
         mma_commit<1>(bar0 + 8 * s);
       }
@@ -747,11 +763,11 @@ int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
 template <int F, int RT>
 int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
   const auto kernel = &sum_kernel<F, RT>;
-  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSumSmem)) return rc;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), SumShape<RT>::kSmem)) return rc;
   const dim3 grid((unsigned)ceil_div(args.cols, kSumCols),
                   (unsigned)most_group_tiles(args.tokens, args.adapters, args.chunk),
                   (unsigned)ceil_div(args.rank, 16 * RT));
-  kernel<<<grid, kSumThreads, kSumSmem, stream>>>(args);
+  kernel<<<grid, kSumThreads, SumShape<RT>::kSmem, stream>>>(args);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SRS_OK : cuda_fail(e, "adapter gradient launch");
 }
