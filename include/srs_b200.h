@@ -480,8 +480,9 @@ int srs_expert_gradient(const srs_blocks* a_t, const srs_blocks* b_t, int64_t ro
  * not written.  largest: encodings of max |low| an adapter, or NULL.  d == NULL: `low` alone.
  * An FP16 |low| above 65504 does not fit the second product.
  *
- * srs_adapter_gradient: out_a = sum over its tokens of low_t z_t^T (rank x cols) or, turned, z_t
- * low_t^T (cols x rank), in z's format; zeros without tokens.  `largest` as given above (FP16).
+ * srs_adapter_gradient: one or two sums over the tokens of every adapter, out_a = sum of low_t
+ * z_t^T (rank x cols) or, turned, z_t low_t^T (cols x rank), in z's format; zeros without tokens.
+ * `largest` as given above (FP16).  The workspace is that of all sums' columns together.
  *
  * `workspace`: 256-byte aligned, not used by any other call that can overlap in time. */
 #define SRS_ADAPTER_MAX_RANK 256
@@ -499,9 +500,14 @@ int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int64_t x_pitch
                        void* workspace, int64_t workspace_bytes, void* stream);
 
 int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters, int rank);
-int srs_adapter_gradient(const void* z, int format, int64_t tokens, int64_t cols, int64_t z_pitch,
-                         const float* low, const uint32_t* largest, int adapters, int rank,
-                         const int32_t* order, const int32_t* ends, int turned, void* out,
+typedef struct srs_adapter_sum {
+  uint64_t z; /* tokens x cols, 16-byte aligned, row pitch z_pitch elements */
+  int64_t z_pitch, cols;
+  uint64_t low, largest, out;
+  int64_t turned;
+} srs_adapter_sum;
+int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int format, int64_t tokens,
+                         int adapters, int rank, const int32_t* order, const int32_t* ends,
                          void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Rows of `cols` bytes at src_pitch copied to rows at dst_pitch (zeros behind them up to

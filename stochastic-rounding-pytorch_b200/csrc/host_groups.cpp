@@ -415,25 +415,45 @@ at::Tensor adapter_product(const at::Tensor& given, const Rounding& how, Blocks 
   return out;
 }
 
-// Sums over the tokens of each adapter of z (tokens, cols) by low: (adapters, rank, cols) or,
+// A sum over the tokens of each adapter of z (tokens, cols) by low: (adapters, rank, cols) or,
 // turned, (adapters, cols, rank).
-at::Tensor adapter_gradient(const at::Tensor& given, const Low& low, const at::Tensor& order,
-                            const at::Tensor& ends, bool turned) {
-  const at::Tensor z = aligned(given, false);
-  const int64_t tokens = z.size(0), cols = z.size(1), rank = low.values.size(1);
+struct Sum {
+  at::Tensor z;
+  const Low* low;
+  bool turned;
+  at::Tensor out;
+};
+
+// One or two sums in one call.
+void adapter_gradients(std::vector<Sum>& sums, const at::Tensor& order, const at::Tensor& ends) {
+  srs_adapter_sum jobs[2] = {};
+  int64_t cols = 0, filled = 0;
+  int n = 0;
   const int64_t count = ends.numel();
-  at::Tensor out = turned ? at::empty({count, cols, rank}, z.options())
-                          : at::empty({count, rank, cols}, z.options());
-  if (out.numel() == 0) return out;
+  for (Sum& sum : sums) {
+    sum.z = aligned(sum.z, false);
+    const int64_t wide = sum.z.size(1), rank = sum.low->values.size(1);
+    sum.out = sum.turned ? at::empty({count, wide, rank}, sum.z.options())
+                         : at::empty({count, rank, wide}, sum.z.options());
+    srs_adapter_sum& job = jobs[n++];
+    job.z = reinterpret_cast<uint64_t>(sum.z.data_ptr());
+    job.z_pitch = step_of(sum.z, 0, ceil_div(wide, 8) * 8);
+    job.cols = wide;
+    job.low = reinterpret_cast<uint64_t>(sum.low->values.data_ptr());
+    if (sum.low->largest.defined())
+      job.largest = reinterpret_cast<uint64_t>(sum.low->largest.data_ptr());
+    job.out = reinterpret_cast<uint64_t>(sum.out.data_ptr());
+    job.turned = sum.turned;
+    cols += wide;
+    filled += sum.out.numel();
+  }
+  if (filled == 0) return;
+  const at::Tensor& z = sums[0].z;
+  const int64_t tokens = z.size(0), rank = sums[0].low->values.size(1);
   const int64_t bytes = g_gradient_workspace(tokens, cols, (int)count, (int)rank);
   const at::Tensor space = at::empty({bytes}, z.options().dtype(at::kByte));
-  check(g_adapter_gradient(
-      z.data_ptr(), format_of(z.scalar_type()), tokens, cols, step_of(z, 0, ceil_div(cols, 8) * 8),
-      static_cast<const float*>(low.values.data_ptr()),
-      low.largest.defined() ? static_cast<const uint32_t*>(low.largest.data_ptr()) : nullptr,
-      (int)count, (int)rank, ints(order), ints(ends), turned, out.data_ptr(), space.data_ptr(),
-      bytes, stream_of(z)));
-  return out;
+  check(g_adapter_gradient(jobs, n, format_of(z.scalar_type()), tokens, (int)count, (int)rank,
+                           ints(order), ints(ends), space.data_ptr(), bytes, stream_of(z)));
 }
 
 at::Tensor flat(const at::Tensor& x) {
@@ -503,16 +523,21 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     const Rounding how{(int)s[0], (int)s[1], (uint32_t)s[2]};
     const at::Tensor &order = saved[kOrder], &ends = saved[kEnds];
     variable_list out(5);
+    std::vector<Sum> sums;
+    Low back;
+    const Low low{saved[kLow], saved[kLargest]};
     if (need[0] || need[2]) {
-      Low back;
       const at::Tensor dx =
           adapter_product(dy, how, {saved[kMatrix], saved[kMatrixScale]}, saved[kDown], saved[kUp],
                           saved[kScale], factor, order, ends, true, need[2] ? &back : nullptr);
       if (need[0]) out[0] = shaped(dx, ctx->saved_data["sizes"].toIntVector());
-      if (need[2]) out[2] = adapter_gradient(saved[kX], back, order, ends, false);
+      if (need[2]) sums.push_back({saved[kX], &back, false, {}});
     }
-    if (need[3])
-      out[3] = adapter_gradient(dy, {saved[kLow], saved[kLargest]}, order, ends, true);
+    if (need[3]) sums.push_back({dy, &low, true, {}});
+    if (!sums.empty()) {
+      adapter_gradients(sums, order, ends);
+      for (const Sum& sum : sums) out[sum.turned ? 3 : 2] = sum.out;
+    }
     if (need[1]) {
       const auto type = (at::ScalarType)s[3];
       Blocks columns, tokens{saved[kTokens], saved[kTokensScale]};

@@ -483,22 +483,29 @@ constexpr int kSumZ = kSumStep * kSumCols * 2;
 template <int RT>
 struct SumShape {
   static constexpr int kRank = 16 * RT, kLow = kSumStep * kRank * 2;
-  static constexpr int kStages = RT == 1 ? 6 : RT == 2 ? 5 : 4;  // two CTAs an SM fit
+  // more CTAs an SM rather than deeper stages: three, three and two
+  static constexpr int kStages = RT == 2 ? 3 : 4, kResident = RT == 4 ? 2 : 3;
   static constexpr int kSmem = 1024 + kStages * kSumZ + 2 * 2 * kLow;
 };
 
-struct SumArgs {
+struct SumJob {
   const char* z;
   int64_t z_pitch;
   const float* low;
   const unsigned int* largest;
-  int tokens, cols, rank, adapters;
+  int cols, turned;  // turned: out is cols x rank instead of rank x cols
+  void* out;
+  float* parts;  // [chunk][rank][cols]
+  int blocks;    // of the grid's width (of sums; of joins)
+};
+
+// Both gradients of a call in one launch: their CTAs fill the SMs' last round together.
+struct SumArgs {
+  SumJob job[2];
+  int tokens, rank, adapters;
   int chunk;  // tokens
   const int32_t* order;
   const int32_t* ends;
-  void* out;
-  float* parts;  // [chunk][rank][cols]
-  int turned;    // out: cols x rank instead of rank x cols
   unsigned int* status;
 };
 
@@ -511,7 +518,8 @@ __device__ __forceinline__ float pair_scale(const unsigned int* largest, int gro
 }
 
 template <int F, int RT>
-__global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
+__global__ void __launch_bounds__(kSumThreads, SumShape<RT>::kResident)
+sum_kernel(const __grid_constant__ SumArgs a) {
   constexpr int kRank = 16 * RT, kSumStages = SumShape<RT>::kStages, kSumLow = SumShape<RT>::kLow;
   constexpr uint32_t kColumns = RT == 4 ? 64 : 32;
   extern __shared__ uint8_t raw[];
@@ -525,9 +533,11 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
   const int count = min(a.chunk, tile.end - tile.row0);
   for (int i = threadIdx.x; i < count; i += kSumThreads)
     places[i] = (int32_t)token_at(a.order, tile.row0 + i, a.tokens);
+  const bool second = (int)blockIdx.x >= a.job[0].blocks;
+  const SumJob& job = a.job[second ? 1 : 0];
   const int rank0 = (int)blockIdx.z * kRank, ranks = min(kRank, a.rank - rank0);
-  const int col0 = (int)blockIdx.x * kSumCols;
-  const float scale = pair_scale(a.largest, tile.group);
+  const int col0 = ((int)blockIdx.x - (second ? a.job[0].blocks : 0)) * kSumCols;
+  const float scale = pair_scale(job.largest, tile.group);
   const uint32_t z0 = (smem_address(raw) + 1023u) & ~1023u, low0 = z0 + kSumStages * kSumZ;
   const uint32_t bar0 = smem_address(bars);
   if (threadIdx.x == 0) {
@@ -542,8 +552,9 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
 
   // z: two boxes of 64 columns, a token's 128 bytes a row; 16 tokens at a time
   const int slot = threadIdx.x & 15, row = threadIdx.x >> 4;
-  const int col = col0 + 8 * slot, bytes = min(max(a.cols - col, 0) * 2, 16);
-  const char* const z = a.z + (int64_t)col * 2;
+  const int col = col0 + 8 * slot, bytes = min(max(job.cols - col, 0) * 2, 16);
+  const char* const z = job.z + (int64_t)col * 2;
+  const int64_t z_step = job.z_pitch * 2;
   const uint32_t box = (uint32_t)(slot >> 3) * (kSumZ / 2);
   const auto load = [&](int step, int s) {
 #pragma unroll
@@ -551,16 +562,17 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
       const int r = row + 16 * i, t = step * kSumStep + r;
       const bool in = t < count && bytes > 0;
       copy16(z0 + s * kSumZ + box + turned_slot(r, slot & 7),
-             in ? z + places[t] * a.z_pitch * 2 : a.z, in ? bytes : 0);
+             in ? z + places[t] * z_step : job.z, in ? bytes : 0);
     }
   };
   // low: thread t has ranks 4 (t % 4) + 16 j of token t / 4
   const int low_row = threadIdx.x >> 2, low_col = (threadIdx.x & 3) * 4;
   const bool whole = (a.rank & 3) == 0;  // rows of whole 16 bytes
+  const float* const low = job.low;
   float held[RT][4];
   const auto fetch = [&](int step) {
     const int t = step * kSumStep + low_row;
-    const float* const from = a.low + (int64_t)(tile.row0 + t) * a.rank + rank0 + low_col;
+    const float* const from = low + (int64_t)(tile.row0 + t) * a.rank + rank0 + low_col;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       if (whole && t < count && low_col + 16 * j < ranks) {
@@ -654,14 +666,14 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = 16 * j + i;
-        if (c >= a.cols || r >= ranks) continue;
+        if (c >= job.cols || r >= ranks) continue;
         const float value = __uint_as_float(v[i]) * back;
         if (!alone)
-          a.parts[((int64_t)blockIdx.y * a.rank + rank0 + r) * a.cols + c] = value;
+          job.parts[((int64_t)blockIdx.y * a.rank + rank0 + r) * job.cols + c] = value;
         else
-          static_cast<uint16_t*>(a.out)[(int64_t)tile.group * a.rank * a.cols +
-                                        (a.turned ? (int64_t)c * a.rank + rank0 + r
-                                                  : (int64_t)(rank0 + r) * a.cols + c)] =
+          static_cast<uint16_t*>(job.out)[(int64_t)tile.group * a.rank * job.cols +
+                                          (job.turned ? (int64_t)c * a.rank + rank0 + r
+                                                      : (int64_t)(rank0 + r) * job.cols + c)] =
               (uint16_t)encode16<F>(value);
       }
     }
@@ -674,7 +686,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const SumArgs a) {
 
 // out_a = the sum of its chunks' parts, in order, where there are several; zeros without tokens.
 template <int F>
-__global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumArgs a) {
   const int lane = threadIdx.x & 31, group = (int)blockIdx.y;
   const EndsAhead ahead(a.ends, a.adapters, lane);
   int carry = 0, chunks_before = 0, first = 0, chunks = 0;
@@ -690,13 +702,16 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
     chunks_before = __shfl_sync(0xFFFFFFFFu, upto, 31);
   }
   if (chunks == 1) return;
-  const int64_t each = (int64_t)a.rank * a.cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < each; i += (int64_t)gridDim.x * 256) {
+  const bool second = (int)blockIdx.x >= a.job[0].blocks;
+  const SumJob& job = a.job[second ? 1 : 0];
+  const int block = (int)blockIdx.x - (second ? a.job[0].blocks : 0);
+  const int64_t each = (int64_t)a.rank * job.cols;
+  for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < each; i += (int64_t)job.blocks * 256) {
     // i runs over the result's order
-    const int64_t at = a.turned ? i % a.rank * a.cols + i / a.rank : i;
+    const int64_t at = job.turned ? i % a.rank * job.cols + i / a.rank : i;
     float v = 0.0f;
-    for (int c = 0; c < chunks; ++c) v += a.parts[(first + c) * each + at];
-    static_cast<uint16_t*>(a.out)[group * each + i] = (uint16_t)encode16<F>(v);
+    for (int c = 0; c < chunks; ++c) v += job.parts[(first + c) * each + at];
+    static_cast<uint16_t*>(job.out)[group * each + i] = (uint16_t)encode16<F>(v);
   }
 }
 
@@ -761,10 +776,11 @@ int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
 }
 
 template <int F, int RT>
-int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
+int launch_sum_as(SumArgs& args, cudaStream_t stream) {
   const auto kernel = &sum_kernel<F, RT>;
   if (int rc = allow_shared(reinterpret_cast<const void*>(kernel), SumShape<RT>::kSmem)) return rc;
-  const dim3 grid((unsigned)ceil_div(args.cols, kSumCols),
+  for (SumJob& job : args.job) job.blocks = (int)ceil_div(job.cols, kSumCols);
+  const dim3 grid((unsigned)(args.job[0].blocks + args.job[1].blocks),
                   (unsigned)most_group_tiles(args.tokens, args.adapters, args.chunk),
                   (unsigned)ceil_div(args.rank, 16 * RT));
   kernel<<<grid, kSumThreads, SumShape<RT>::kSmem, stream>>>(args);
@@ -773,7 +789,7 @@ int launch_sum_as(const SumArgs& args, cudaStream_t stream) {
 }
 
 template <int F>
-int launch_sum(const SumArgs& args, cudaStream_t stream) {
+int launch_sum(SumArgs& args, cudaStream_t stream) {
   if (args.rank <= 16) return launch_sum_as<F, 1>(args, stream);
   if (args.rank <= 32) return launch_sum_as<F, 2>(args, stream);
   return launch_sum_as<F, 4>(args, stream);
@@ -932,10 +948,11 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
               : launch_adapter_product(rows, *w, k, call, edge, d, st);
 }
 
-// Tokens of a chunk: long ones leave fewer parts, short ones keep the SMs busy (two CTAs each).
+// Tokens of a chunk for `cols` columns in all: long ones leave fewer parts, short ones keep the SMs
+// busy (with three CTAs each).
 static int sum_chunk(int64_t tokens, int64_t cols, int rank) {
   const int64_t each = ceil_div(cols, kSumCols) * ceil_div(rank, 64);
-  int64_t chunk = tokens * each / (2 * sm_count());
+  int64_t chunk = tokens * each / (3 * sm_count());
   chunk = ceil_div(chunk < 256 ? 256 : chunk, kSumStep) * kSumStep;
   return (int)(chunk > kSumChunk ? kSumChunk : chunk);
 }
@@ -946,58 +963,78 @@ extern "C" int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, 
   return most_group_tiles(tokens, adapters, sum_chunk(tokens, cols, rank)) * rank * cols * 4;
 }
 
-extern "C" int srs_adapter_gradient(const void* z, int format, int64_t tokens, int64_t cols,
-                                    int64_t z_pitch, const float* low, const uint32_t* largest,
-                                    int adapters, int rank, const int32_t* order,
-                                    const int32_t* ends, int turned, void* out, void* workspace,
-                                    int64_t workspace_bytes, void* stream) {
+extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int format,
+                                    int64_t tokens, int adapters, int rank, const int32_t* order,
+                                    const int32_t* ends, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
   clear_error();
   if (int rc = check_groups(ends, adapters)) return rc;
+  if (sums == nullptr || n_sums < 1 || n_sums > 2)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "one or two sums a call, got %d", n_sums);
   if (format != SRS_FMT_BF16 && format != SRS_FMT_F16)
     return fail(SRS_ERR_INVALID_ARGUMENT, "adapters are BF16 or FP16, got format %d", format);
-  if (rank < 1 || rank > SRS_ADAPTER_MAX_RANK || tokens < 0 || tokens > (1ll << 22) || cols < 0 ||
-      cols > (1ll << 30))
-    return fail(SRS_ERR_INVALID_ARGUMENT, "sizes out of range (%lld tokens, %lld columns, rank %d)",
-                (long long)tokens, (long long)cols, rank);
-  if (cols == 0) return SRS_OK;
-  if (out == nullptr || reinterpret_cast<uintptr_t>(out) % 2 != 0)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
+  if (rank < 1 || rank > SRS_ADAPTER_MAX_RANK || tokens < 0 || tokens > (1ll << 22))
+    return fail(SRS_ERR_INVALID_ARGUMENT, "sizes out of range (%lld tokens, rank %d)",
+                (long long)tokens, rank);
+  SumArgs a{};
+  int64_t cols = 0;
+  int jobs = 0;
+  for (int i = 0; i < n_sums; ++i) {
+    const srs_adapter_sum& s = sums[i];
+    if (s.cols < 0 || s.cols > (1ll << 30))
+      return fail(SRS_ERR_INVALID_ARGUMENT, "%lld columns are out of range", (long long)s.cols);
+    if (s.cols == 0) continue;
+    if (s.out == 0 || s.out % 2 != 0)
+      return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
+    if (tokens > 0 && (s.z == 0 || s.low == 0 || order == nullptr || s.z_pitch < s.cols ||
+                       s.z_pitch % 8 != 0 || s.z % 16 != 0))
+      return fail(SRS_ERR_INVALID_ARGUMENT, "z needs a 16-byte aligned address and row pitch");
+    SumJob& job = a.job[jobs++];
+    job.z = reinterpret_cast<const char*>(s.z);
+    job.z_pitch = s.z_pitch;
+    job.low = reinterpret_cast<const float*>(s.low);
+    job.largest =
+        format == SRS_FMT_F16 ? reinterpret_cast<const unsigned int*>(s.largest) : nullptr;
+    job.cols = (int)s.cols;
+    job.turned = s.turned != 0;
+    job.out = reinterpret_cast<void*>(s.out);
+    cols += s.cols;
+  }
+  if (jobs == 0) return SRS_OK;
   if (int rc = check_device()) return rc;
+  if (int rc = check_products()) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (tokens == 0) {
-    const cudaError_t e = cudaMemsetAsync(out, 0, (size_t)(2 * cols * rank * adapters), st);
-    return e == cudaSuccess ? SRS_OK : cuda_fail(e, "srs_adapter_gradient");
+    for (int i = 0; i < jobs; ++i) {
+      const cudaError_t e = cudaMemsetAsync(
+          a.job[i].out, 0, (size_t)(2ll * a.job[i].cols * rank * adapters), st);
+      if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_gradient");
+    }
+    return SRS_OK;
   }
-  if (z == nullptr || low == nullptr || order == nullptr || z_pitch < cols || z_pitch % 8 != 0 ||
-      reinterpret_cast<uintptr_t>(z) % 16 != 0)
-    return fail(SRS_ERR_INVALID_ARGUMENT, "z needs a 16-byte aligned address and row pitch");
+  const int64_t least = srs_adapter_gradient_workspace(tokens, cols, adapters, rank);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-      workspace_bytes < srs_adapter_gradient_workspace(tokens, cols, adapters, rank))
+      workspace_bytes < least)
     return fail(SRS_ERR_INVALID_ARGUMENT, "workspace of %lld bytes, %lld needed",
-                (long long)workspace_bytes,
-                (long long)srs_adapter_gradient_workspace(tokens, cols, adapters, rank));
-  SumArgs a{};
-  a.z = static_cast<const char*>(z);
-  a.z_pitch = z_pitch;
-  a.low = low;
-  a.largest = format == SRS_FMT_F16 ? largest : nullptr;
+                (long long)workspace_bytes, (long long)least);
   a.tokens = (int)tokens;
-  a.cols = (int)cols;
   a.rank = rank;
   a.adapters = adapters;
   a.order = order;
   a.ends = ends;
-  a.out = out;
-  a.parts = static_cast<float*>(workspace);
-  a.turned = turned != 0;
   a.chunk = sum_chunk(tokens, cols, rank);
-  if (int rc = check_products()) return rc;
   if (int rc = status_word(&a.status)) return rc;
+  const int64_t chunks = most_group_tiles(tokens, adapters, a.chunk);
+  a.job[0].parts = static_cast<float*>(workspace);
+  a.job[1].parts = a.job[0].parts + chunks * rank * a.job[0].cols;
   if (int rc = format == SRS_FMT_BF16 ? launch_sum<SRS_FMT_BF16>(a, st)
                                       : launch_sum<SRS_FMT_F16>(a, st))
     return rc;
-  const int64_t blocks = ceil_div((int64_t)rank * cols, 1024);
-  const dim3 joins((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)adapters);
+  for (SumJob& job : a.job) {
+    const int64_t blocks = ceil_div((int64_t)rank * job.cols, 1024);
+    job.blocks = (int)(blocks < 512 ? blocks : 512);
+  }
+  const dim3 joins((unsigned)(a.job[0].blocks + a.job[1].blocks), (unsigned)adapters);
   if (format == SRS_FMT_BF16) join_kernel<SRS_FMT_BF16><<<joins, 256, 0, st>>>(a);
   else join_kernel<SRS_FMT_F16><<<joins, 256, 0, st>>>(a);
   const cudaError_t e = cudaGetLastError();

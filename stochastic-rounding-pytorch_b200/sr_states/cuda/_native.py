@@ -200,9 +200,8 @@ _SIGNATURES = {
                             ctypes.c_int64, _P], ctypes.c_int),
     "srs_adapter_gradient_workspace": ([*[ctypes.c_int64] * 2, ctypes.c_int, ctypes.c_int],
                                        ctypes.c_int64),
-    "srs_adapter_gradient": ([_P, ctypes.c_int, *[ctypes.c_int64] * 3, _P, _P, ctypes.c_int,
-                              ctypes.c_int, _P, _P, ctypes.c_int, _P, _P, ctypes.c_int64, _P],
-                             ctypes.c_int),
+    "srs_adapter_gradient": ([_P, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int,
+                              ctypes.c_int, _P, _P, _P, ctypes.c_int64, _P], ctypes.c_int),
     "srs_product_status": ([ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "srs_product_status_word": ([ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32))], ctypes.c_int),
 }
