@@ -31,10 +31,12 @@ __device__ __forceinline__ int64_t token_at(const int32_t* order, int place, int
   return t >= 0 && t < tokens ? t : 0;  // an entry that names no token reads the first
 }
 
+// 16 bytes to shared memory, those behind the first `bytes` zero.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+
 // Rows of SLOTS (2, 4 or 8) 16-byte slots, turned so that 8 rows at one slot reach all banks: the
 // order of 32-, 64- and 128-byte swizzled boxes.
 template <int SLOTS>
@@ -327,8 +329,12 @@ __global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(cons
 
 // Many tokens: 128 of one adapter (the rows of an MMA), gathered with cp.async into the layout that
 // the tensor core reads, so that a stage's four MMAs need nothing of the warps.  A stage is loaded
-// again once the MMAs of two stages before have read theirs.  (With ldmatrix and mma.sync in 8
-// warps shared memory was read five times as often: 4096 tokens, 4096 -> 64: 25 us; so RESULT.)
+// again once the MMAs of two stages before have read theirs.  4096 tokens, 4096 -> 64, 16 adapters,
+// beside the quantisation: 24 us; x's bytes would take 5, some 9 are launch, dependent first loads and
+// the cluster's meeting.  4096 tokens, 14336 -> 16, behind a kernel that left 117 MB to write back:
+// 49 us for 117 MB.  (ldmatrix and mma.sync in 8 warps read shared memory five times as often and
+// took as long, 25 and 44 us; one kernel for this and the quantisation, x read once, took 36 and
+// 113 us, these two side by side 33 and 112.)
 constexpr int kManyTokens = 128, kManyThreads = 256;
 
 template <int RT>
@@ -473,7 +479,8 @@ __global__ void __launch_bounds__(kManyThreads, 2) low_many_kernel(const LowArgs
 // rows of an MMA), up to 16 RT of the rank and a chunk of tokens of one adapter (counted from its
 // first); an adapter of one chunk is finished here, one of several leaves FP32 parts, which another
 // kernel adds in order.  z's bytes, read once for every 64 of the rank, bound it: rows are gathered
-// with cp.async into the layout in which the tensor core reads tokens as k.  `low` enters as a
+// with cp.async into the layout in which the tensor core reads tokens as k (4096 tokens, 4096 + 14336
+// columns, rank 16: 61 us for 151 MB, and 9 to join).  `low` enters as a
 // pair of 16-bit numbers (high and what it leaves); in FP16 both are scaled by a power of two that
 // brings the adapter's largest to 2^11 .. 2^12, so that small gradients keep their digits.
 constexpr int kSumCols = 128, kSumStep = 64, kSumThreads = 256;
