@@ -19,7 +19,7 @@
 #include "srs_groups.cuh"
 #include "srs_host.h"
 #include "srs_launch.h"
-#include "srs_tcgen05.cuh"
+#include "srs_product.cuh"
 
 namespace srs {
 namespace {
@@ -122,7 +122,7 @@ struct LowArgs {
   uint16_t* pairs;        // items for a product (null: not wanted)
   int edge, pitch, rest_at;
   bool spread;            // items of a thin product: rows are the batch's
-  unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
+  unsigned int* largest;  // of an adapter's |low|, behind them of all, as encodings (null: not wanted)
   unsigned int* status;
 };
 
@@ -153,6 +153,49 @@ __device__ __forceinline__ LowTile low_tile(const LowArgs& a, int most, int rank
   return t;
 }
 
+// Token at place `place`, rank r of the low part as a pair.
+template <int F>
+__device__ __forceinline__ void write_pair(const LowArgs& a, const GroupTile& tile, int place, int r,
+                                           float v) {
+  const int64_t at = a.spread ? (int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)
+                              : (int64_t)(place / a.edge + tile.rank) * a.edge + place % a.edge;
+  uint16_t* const to = a.pairs + at * a.pitch + r;
+  const uint32_t high = encode16<F>(v);
+  const float left = v - decode16<F>(high);
+  to[0] = (uint16_t)high;
+  to[a.rest_at] = (uint16_t)encode16<F>(isfinite(left) ? left : 0.0f);
+}
+
+// Zeros in the rows of the adapter's items that are not its own (`whole` of the rank from rank0 on),
+// by the threads from, from + step, .. of those that have its first and its last tile of `most`.
+__device__ __forceinline__ void clear_items(const LowArgs& a, const GroupTile& tile, int most,
+                                            int rank0, int whole, int from, int step) {
+  const int words = whole / 2;
+  const auto zero = [&](int64_t row, int word) {
+    uint16_t* const p = a.pairs + row * a.pitch + rank0 + 2 * word;
+    *reinterpret_cast<uint32_t*>(p) = 0u;
+    *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
+  };
+  if (a.spread) {
+    if (tile.row0 == tile.start) {
+      const int others = a.tokens - (tile.end - tile.start);
+      for (int i = from; i < others * words; i += step) {
+        const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
+        zero((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens), i % words);
+      }
+    }
+  } else {
+    // before its first row in its first item, behind its last in the last
+    if (tile.row0 == tile.start)
+      for (int i = from; i < tile.start % a.edge * words; i += step)
+        zero((int64_t)(tile.start / a.edge + tile.rank) * a.edge + i / words, i % words);
+    const int final_row = tile.end - 1, behind = final_row % a.edge + 1;
+    if (final_row - tile.row0 < most)
+      for (int i = from; i < (a.edge - behind) * words; i += step)
+        zero((int64_t)(final_row / a.edge + tile.rank) * a.edge + behind + i / words, i % words);
+  }
+}
+
 // Sums of the cluster's CTAs (`sums`: [token][rank], rows of `pitch`, PARTS of them `part` apart
 // in every CTA) added, scaled and written: token t of the tile by CTA t % splits.
 template <int F, int RANK, int PARTS>
@@ -180,52 +223,37 @@ __device__ __forceinline__ void write_low(const LowArgs& a, const LowTile& l, fl
       if (a.low != nullptr) a.low[(int64_t)(tile.row0 + t) * a.rank + l.rank0 + r] = v;
       top_size = fmaxf(top_size, isfinite(v) ? fabsf(v) : 0.0f);
     }
-    if (a.pairs != nullptr) {
-      const int place = tile.row0 + t;
-      const int64_t at =
-          a.spread ? (int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)
-                   : (int64_t)(place / a.edge + tile.rank) * a.edge + place % a.edge;
-      uint16_t* const to = a.pairs + at * a.pitch + l.rank0 + r;
-      const uint32_t high = encode16<F>(v);
-      const float left = v - decode16<F>(high);
-      to[0] = (uint16_t)high;
-      to[a.rest_at] = (uint16_t)encode16<F>(isfinite(left) ? left : 0.0f);
-    }
+    if (a.pairs != nullptr) write_pair<F>(a, tile, tile.row0 + t, l.rank0 + r, v);
   }
-  if (a.pairs != nullptr) {
-    // zeros in the rows of the adapter's items that are not its own
-    const int words = whole / 2;
-    const auto zero = [&](int64_t row, int word) {
-      uint16_t* const p = a.pairs + row * a.pitch + l.rank0 + 2 * word;
-      *reinterpret_cast<uint32_t*>(p) = 0u;
-      *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
-    };
-    const int from = threadIdx.x + threads * split, step = threads * splits;
-    if (a.spread) {
-      if (tile.row0 == tile.start) {
-        const int others = a.tokens - (tile.end - tile.start);
-        for (int i = from; i < others * words; i += step) {
-          const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
-          zero((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens), i % words);
-        }
-      }
-    } else {
-      // before its first row in its first item, behind its last in the last
-      if (tile.row0 == tile.start)
-        for (int i = from; i < tile.start % a.edge * words; i += step)
-          zero((int64_t)(tile.start / a.edge + tile.rank) * a.edge + i / words, i % words);
-      const int final_row = tile.end - 1, behind = final_row % a.edge + 1;
-      if (final_row - tile.row0 < most)
-        for (int i = from; i < (a.edge - behind) * words; i += step)
-          zero((int64_t)(final_row / a.edge + tile.rank) * a.edge + behind + i / words, i % words);
-    }
-  }
+  if (a.pairs != nullptr)
+    clear_items(a, tile, most, l.rank0, whole, (int)threadIdx.x + threads * split, threads * splits);
   if (a.largest != nullptr) {
     const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_size));
-    if ((threadIdx.x & 31) == 0 && top != 0u)
-      atomicMax(a.largest + tile.group, top);  // the order is no matter
+    if ((threadIdx.x & 31) == 0 && top != 0u) {  // (the order is no matter)
+      atomicMax(a.largest + tile.group, top);
+      atomicMax(a.largest + a.adapters, top);
+    }
   }
   if (splits > 1) cg::this_cluster().sync();  // the others have read this CTA's sums
+}
+
+// FP16 pairs, of the finished FP32 low part: what they are scaled by depends on all of it.
+constexpr int kPairTokens = 128, kPairThreads = 256;
+
+__global__ void __launch_bounds__(kPairThreads) pairs_kernel(const LowArgs a) {
+  // A thin product launched to overlap this kernel may start.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, kPairTokens,
+                                         (int)blockIdx.x, (int)(threadIdx.x & 31));
+  if (tile.group < 0) return;
+  const int count = min(kPairTokens, tile.end - tile.row0), whole = (a.rank + 15) & ~15;
+  const float factor = two_to(pair_exponent(__ldcg(a.largest + a.adapters)));
+  for (int i = threadIdx.x; i < count * whole; i += kPairThreads) {
+    const int place = tile.row0 + i / whole, r = i % whole;
+    const float v = r < a.rank ? __ldcg(a.low + (int64_t)place * a.rank + r) * factor : 0.0f;
+    write_pair<SRS_FMT_F16>(a, tile, place, r, v);
+  }
+  clear_items(a, tile, kPairTokens, 0, whole, (int)threadIdx.x, kPairThreads);
 }
 
 // Calls of few tokens, where most adapters have one or two: 16 tokens, and 4 warps that share a
@@ -835,23 +863,23 @@ using namespace srs;
 // Few tokens: the projection's thin form.
 static bool few(int64_t tokens) { return tokens <= kThinRows; }
 
-// Parts of a call's workspace, each on a 256-byte boundary.
+// Parts of a call's workspace, each on a 256-byte boundary: the quantised tokens first; FP16 alone
+// needs `low` and `largest` (for both formats there is room).
 struct AdapterSpace {
-  int64_t low, total;  // quantised tokens first, then the pairs of the low part
+  int64_t pairs, low, largest, total;
 };
 
 static AdapterSpace adapter_space(int64_t tokens, int64_t k, int64_t n, int adapters, int rank) {
   AdapterSpace s{};
-  int64_t at = whole(srs_linear_workspace(tokens, k));
-  s.low = at;
-  if (n > 0) {
-    const int64_t rows = few(tokens)
-                             ? (adapters < tokens ? adapters : tokens) * thin_columns(tokens)
-                             : pair_items(tokens, adapters, adapter_edge(tokens, n, k)) *
-                                   adapter_edge(tokens, n, k);
-    at += whole(rows * pair_shape(rank).pitch * 2);
-  }
-  s.total = at;
+  s.pairs = whole(srs_linear_workspace(tokens, k));
+  int64_t rows = 0;
+  if (n > 0)
+    rows = few(tokens) ? (adapters < tokens ? adapters : tokens) * thin_columns(tokens)
+                       : pair_items(tokens, adapters, adapter_edge(tokens, n, k)) *
+                             adapter_edge(tokens, n, k);
+  s.low = s.pairs + whole(rows * pair_shape(rank).pitch * 2);
+  s.largest = s.low + (n > 0 ? whole(tokens * rank * 4) : 0);
+  s.total = s.largest + whole((adapters + 1) * 4);
   return s;
 }
 
@@ -891,7 +919,10 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   const bool bf16 = a->format == SRS_FMT_BF16, thin = few(tokens);
 
   cudaError_t e = cudaSuccess;
-  if (largest != nullptr) e = cudaMemsetAsync(largest, 0, (size_t)a->count * 4, st);
+  unsigned int* const sizes =
+      bf16 ? nullptr : largest != nullptr ? largest
+                                          : reinterpret_cast<unsigned int*>(at + space.largest);
+  if (sizes != nullptr) e = cudaMemsetAsync(sizes, 0, ((size_t)a->count + 1) * 4, st);
   // without a sum there is neither a projection nor a low part
   if (e == cudaSuccess && n > 0 && k == 0) e = cudaMemsetAsync(d, 0, (size_t)(tokens * n * 2), st);
   if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
@@ -911,11 +942,11 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.ends = reinterpret_cast<const int32_t*>(a->ends);
   l.scale = reinterpret_cast<const float*>(a->scale);
   l.factor = a->factor;
-  l.low = low;
-  l.largest = largest;
+  l.low = low != nullptr ? low : bf16 ? nullptr : reinterpret_cast<float*>(at + space.low);
+  l.largest = sizes;
   if (int rc = status_word(&l.status)) return rc;
   if (edge != 0) {
-    l.pairs = reinterpret_cast<uint16_t*>(at + space.low);
+    if (bf16) l.pairs = reinterpret_cast<uint16_t*>(at + space.pairs);
     l.edge = edge;
     l.pitch = pairs.pitch;
     l.rest_at = pairs.rest_at;
@@ -940,6 +971,12 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   q.order = thin ? nullptr : l.order;
   q.overlap = true;  // beside the low part
   if (int rc = quantize(q, st)) return rc;
+  if (!bf16) {
+    l.pairs = reinterpret_cast<uint16_t*>(at + space.pairs);
+    pairs_kernel<<<(unsigned)most_group_tiles(tokens, a->count, kPairTokens), kPairThreads, 0, st>>>(l);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "pairs of the low part");
+  }
   const AdapterCall call{l.pairs,
                          reinterpret_cast<const void*>(turned ? a->down : a->up),
                          turned ? a->down_pitch : a->up_pitch,
@@ -949,7 +986,8 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
                          a->rank,
                          a->format,
                          l.order,
-                         l.ends};
+                         l.ends,
+                         bf16 ? nullptr : sizes + a->count};
   // (with few tokens beside the quantisation: the weights are streamed first)
   return thin ? launch_thin(*w, rows, k, d, a->format, 1, n, true, st, &call)
               : launch_adapter_product(rows, *w, k, call, edge, d, st);

@@ -76,6 +76,7 @@ struct AdapterCall {
   int count, rank, format;
   const int32_t* order;
   const int32_t* ends;
+  const unsigned int* top;  // FP16: encoding of the largest |low|, by which the pairs are scaled
 };
 
 // FP8 blocks: d = a b^T (operands checked by the caller).  Element (i, j)

@@ -150,7 +150,23 @@ struct BlockScales {
   int row0, col0, m, n, slices;
   int64_t a_quad = 4, b_quad = 4;  // see ScaleRows
   bool padded = false;
+  uint32_t a_more = 0;  // added to every byte of a's scales
 };
+
+// FP16 pairs of a low part are held times 2^k, so that small gradients keep their digits and large
+// values fit: k brings the largest of all to 2^13 .. 2^14.  The FP8 product they are added to gets the
+// same factor through its block scales (bytes of FP16 values' blocks lie in 88 .. 135), and the
+// results lose it again.  `top`: encoding of the largest; 0: none.  (Up to 2^30: then a pair's
+// last digit is far below that of any FP16 result, and no sum leaves FP32's range.)
+__device__ __forceinline__ int pair_exponent(uint32_t top) {
+  return top == 0u ? 0 : min(max(13 - ((int)(top >> 23) - 127), -60), 30);
+}
+__device__ __forceinline__ float two_to(int k) {  // -126 <= k <= 127
+  return __uint_as_float((uint32_t)(k + 127) << 23);
+}
+__device__ __forceinline__ uint32_t in_every_byte(int k) {
+  return ((uint32_t)k & 0xFFu) * 0x01010101u;
+}
 
 __device__ __forceinline__ bool scale_words(const uint8_t* scale, int64_t pitch, int kb) {
   return ((reinterpret_cast<uint64_t>(scale) | (uint64_t)pitch | (uint64_t)kb) & 3) == 0;
@@ -838,6 +854,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
       uint32_t t = first;
       int kb = 0, slices = 0;
       bool a_words = false, b_words = false, padded = false;
+      uint32_t a_more = 0;
       int64_t a_quad = 4, b_quad = 4;
       ScaleRows from[1 + CG];
       uint32_t next[1 + CG][4];
@@ -849,6 +866,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
           a_quad = scales.a_quad;
           b_quad = scales.b_quad;
           padded = scales.padded;
+          a_more = scales.a_more;
           a_words = scale_words(scales.a, scales.a_pitch, 0);
           b_words = scale_words(scales.b, scales.b_pitch, 0);
           from[0].at(scales.a, scales.a_pitch, scales.a_shift, scales.row0 + 128 * (int)rank,
@@ -859,6 +877,10 @@ __device__ __forceinline__ void run_products(const Source& src) {
                            scales.n, lane);
         }
         from[0].read(kb, slices, a_words, next[0], a_quad, padded);
+        if (Source::kExtras) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) next[0][j] = __vadd4(next[0][j], a_more);
+        }
 #pragma unroll
         for (int c = 0; c < CG; ++c)
           from[1 + c].read(kb, slices, b_words, next[1 + c], b_quad, padded);

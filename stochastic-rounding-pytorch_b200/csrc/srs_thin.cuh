@@ -67,6 +67,7 @@ struct ThinArgs {
   CUtensorMap map_h, map_u;
   int rank, item_slices, rest_at;
   bool up_rows_inner;  // U is stored rank x rows
+  const unsigned int* top;  // of FP16 pairs (null: BF16)
   uint32_t extra_idesc;
 };
 
@@ -373,6 +374,14 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
       waited = true;
       from_b.read<true>(kb, last, words_b, w[1]);
+      if constexpr (ADAPTERS) {
+        // (written ahead of this kernel, as B is)
+        if (a.top != nullptr) {
+          const uint32_t more = in_every_byte(pair_exponent(__ldcg(a.top)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[1][j] = __vadd4(w[1][j], more);
+        }
+      }
       ok = barrier_wait(scale_empty(slot), ((uint32_t)(g / kThinSlots) & 1u) ^ 1u, a.status,
                         1u << 12);
       ok = __all_sync(0xFFFFFFFFu, ok);
@@ -409,6 +418,11 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_after();
   const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
   const int row = row0 + 32 * warp + lane, row_end = min(a.m, row0 + a.rows);
+  float factor = 1.0f;  // FP16 pairs': a power of two
+  if constexpr (ADAPTERS) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.top != nullptr) factor = two_to(-pair_exponent(__ldcg(a.top)));
+  }
   if (splits == 1) {
     if (warp < 4 && ok) {
 #pragma unroll
@@ -421,7 +435,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           if (row < row_end && c0 + c < n)
             store_value(a.out, a.out_format,
                         row * a.row_stride + (b_row0 + c0 + c) * a.col_stride,
-                        __uint_as_float(v[c]));
+                        ADAPTERS ? __uint_as_float(v[c]) * factor : __uint_as_float(v[c]));
       }
     }
   } else {
@@ -461,7 +475,8 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
         if (r < (int)splits) sum = __fadd_rn(sum, part[r]);
       if (out_row < row_end && ok)
         store_value(a.out, a.out_format,
-                    out_row * a.row_stride + (b_row0 + c) * a.col_stride, sum);
+                    out_row * a.row_stride + (b_row0 + c) * a.col_stride,
+                    ADAPTERS ? sum * factor : sum);
     }
     cluster_sync();  // the others have read this CTA's sums
   }

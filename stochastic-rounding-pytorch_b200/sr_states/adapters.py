@@ -27,8 +27,7 @@ def adapter_linear(x, weight, down, up, groups, *, scale=1.0, dtype=torch.float8
     ``weight``: a BlockTensor (inference), a pair of BlockTensors
     ``quantize_blocks(w, block=(128, 128), orientation="both")`` (a frozen projection:
     differentiable in ``x``, ``down`` and ``up``), or an (N, K) tensor (quantised in the call,
-    differentiable too).  The rest as for ``block_linear``.  At most 2^22 tokens.  With FP16
-    the inner products must stay below 65504.
+    differentiable too).  The rest as for ``block_linear``.  At most 2^22 tokens.
     """
     kept = turned = (None, None)
     if isinstance(weight, BlockTensor):

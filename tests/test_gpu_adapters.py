@@ -6,7 +6,9 @@ at each addition):
 * the projection, as for ``matmul_blocks``: (K + 2) u sum |x||w|;
 * the low part h = s A x: (K + 16) u |s| sum |A||x| (K terms, up to 8 parts of the sum, the
   scale); where a tensor core takes it as a pair of 16-bit numbers, 2^-17 |h| more in BF16 (each
-  rounding is off by 2^-9 of what it rounds) and 2^-22 |h| + 2^-25 in FP16;
+  rounding is off by 2^-9 of what it rounds), and in FP16, whose pairs are scaled to the call's
+  largest |h|, 2^-22 |h| + 2^-37 of that largest (2^-25 at 2^13 and above, or 2^-55 if the factor has
+  reached its limit);
 * B h: that error through |B|, and (2 rank + 8) u sum |B||h|;
 * a gradient sum_t z h: the error of h through |z|, the pair's, and (2 n + 8) u sum |z||h| over
   n tokens; FP16 pairs are scaled to the adapter's largest, which leaves 2^-35 of it;
@@ -38,11 +40,11 @@ def held(x, **how):
     return quantize_blocks(x, **how).dequantize().double()
 
 
-def pair(h, dtype, largest=None):
+def pair(h, dtype, largest):
     """What a pair of 16-bit numbers loses of h."""
     if dtype == torch.bfloat16:
         return 2.0**-17 * h.abs()
-    return 2.0**-22 * h.abs() + (2.0**-25 if largest is None else 2.0**-35 * largest)
+    return 2.0**-22 * h.abs() + 2.0**-35 * largest + 2.0**-55
 
 
 def low_of(x, a, s, dtype):
@@ -65,10 +67,12 @@ def expected(x, w, a, b, s, index, dtype):
     inside, given = x
     exact = inside @ w.mT
     error = (w.shape[1] + 2) * U * (inside.abs() @ w.abs().mT)
+    lows = [low_of(given[index == i], a[i], s[i], dtype)[0] for i in range(a.shape[0])]
+    largest = max([h.abs().max() for h in lows if h.numel()], default=torch.zeros(()))
     for i in range(a.shape[0]):
         rows = index == i
         h, off = low_of(given[rows], a[i], s[i], dtype)
-        off = off + pair(h, dtype)
+        off = off + pair(h, dtype, largest)
         exact[rows] += h @ b[i].mT
         error[rows] += off @ b[i].abs().mT + (2 * a.shape[1] + 8) * U * (h.abs() @ b[i].abs().mT)
     return exact, error + 4 * U * exact.abs()
@@ -145,9 +149,25 @@ def test_result_and_gradients(size, how, dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
-def test_small_gradients_keep_their_digits(dtype, cuda_device):
-    run_case(300, 3, 16, 256, 200, dtype, cuda_device, indices(300, 3, "mixed", cuda_device),
-             size=1e-4)
+@pytest.mark.parametrize("tokens", [50, 300])
+@pytest.mark.parametrize("size", [1e-6, 1e-4, 300.0])
+def test_small_and_large_gradients_keep_their_digits(dtype, tokens, size, cuda_device):
+    run_case(tokens, 3, 16, 256, 200, dtype, cuda_device,
+             indices(tokens, 3, "mixed", cuda_device), size=size)
+
+
+def test_low_parts_beyond_fp16_fit(cuda_device):
+    """An FP16 result that fits, by inner products that do not."""
+    x = torch.full((70, 64), 256.0, device=cuda_device, dtype=torch.float16)
+    w = torch.zeros((32, 64), device=cuda_device, dtype=torch.float16)
+    down = torch.full((1, 8, 64), 16.0, device=cuda_device, dtype=torch.float16)
+    up = torch.full((1, 32, 8), 2.0**-10, device=cuda_device, dtype=torch.float16)
+    groups = group_rows(torch.zeros(70, dtype=torch.int32, device=cuda_device), 1)
+    for tokens in (70, 9):
+        plan = RowGroups(groups.order[:tokens], (groups.ends * 0 + tokens))
+        with torch.no_grad():
+            y = adapter_linear(x[:tokens], w, down, up, plan)
+        assert (y == 256 * 16 * 64 * 8 * 2.0**-10).all()  # 2^18 inside, 2^11 out
 
 
 def test_other_forms_of_the_weight(cuda_device):
