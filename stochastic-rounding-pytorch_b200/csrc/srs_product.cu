@@ -336,12 +336,6 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
     args.rows = (int)((a.rows + 2 * sms * rounds - 1) / (2 * sms * rounds));
   } else {
     while (splits < 8 && tiles * splits <= sms && args.slices >= 4 * splits) splits *= 2;
-    // More CTAs than SMs, but not two for each: tiles of the size that gives two (14336 x 4096 by
-    // 64 tokens in 2 x 112 tiles of 128 rows 26.9 us, in 2 x 148 of 97 rows 23.1).  Not with
-    // larger clusters: 37 of eight CTAs need two rounds (4096 x 4096: 8.3 -> 13.1 us).
-    const int64_t room = 2 * sms / splits;
-    if (splits <= 2 && tiles * splits > sms && room > tiles && !whole)
-      args.rows = (int)((a.rows + room - 1) / room);
   }
   if (int rc = operand_map(a, k, args.rows, &args.map_a)) return rc;
   if (int rc = operand_map(b, k, columns, &args.map_b)) return rc;
