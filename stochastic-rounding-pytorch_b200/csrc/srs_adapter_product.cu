@@ -67,7 +67,7 @@ __device__ __forceinline__ void plan_adapters(AdapterPlan& p, const int32_t* end
 }
 
 struct AdapterSource {
-  static constexpr bool kExtras = true;
+  static constexpr bool kExtras = true, kPadded = false;
   const AdapterProduct& w;
   const AdapterPlan& p;
   __device__ int phases() const { return 1; }

@@ -114,7 +114,7 @@ __device__ __forceinline__ void spread_zeros(char* out, int64_t count, int size,
 }
 
 struct RowSource {
-  static constexpr bool kExtras = false;
+  static constexpr bool kExtras = false, kPadded = false;
   const ExpertProduct& w;
   const GroupPlan& p;
   struct At {
@@ -187,7 +187,7 @@ struct RowSource {
 };
 
 struct SumSource {
-  static constexpr bool kExtras = false;
+  static constexpr bool kExtras = false, kPadded = true;
   const ExpertProduct& w;
   const GroupPlan& p;
   struct At {
@@ -255,8 +255,7 @@ struct SumSource {
             w.n,
             slices(i.expert),
             a_quad,
-            b_quad,
-            true};
+            b_quad};
   }
   __device__ void spare(int lane) const {
     const int size = w.format == SRS_FMT_F32 ? 4 : 2;

@@ -189,7 +189,7 @@ struct BlockProduct {
 };
 
 struct BlockSource {
-  static constexpr bool kExtras = false;
+  static constexpr bool kExtras = false, kPadded = false;
   const BlockProduct& w;
   __device__ int phases() const { return 1; }
   __device__ uint32_t tiles(int) const { return w.grid.rows * w.grid.cols; }

@@ -96,8 +96,7 @@ struct TileStore {
 // kb + 3 of each, one byte a block.  Rows outside the matrix read its last row
 // instead (their data are zeros and their results are not stored); blocks from
 // `last` on give 1 (127).  Rows on 4-byte boundaries are read a word at a time.
-// `quad`: bytes from a word of four scales to the row's next (4: rows one after the other);
-// `padded`: whole words may be read behind `last`.
+// PADDED: whole words may be read behind `last`, `quad` bytes from one to the row's next.
 //
 // FRESH: the kernel ahead in the stream may write the scales while this one runs; they are
 // then read (behind the wait for that kernel) through L2, never through the non-coherent
@@ -115,17 +114,20 @@ struct ScaleRows {
     if constexpr (FRESH) return __ldcg(p);
     return __ldg(p);
   }
-  template <bool FRESH = false>
+  template <bool FRESH = false, bool PADDED = false>
   __device__ __forceinline__ void read(int kb, int last, bool words, uint32_t (&w)[4],
-                                       int64_t quad = 4, bool padded = false) const {
-    const int64_t at = (int64_t)(kb >> 2) * quad + (kb & 3);
-    if (words && (padded || kb + 4 <= last)) {
+                                       int64_t quad = 4) const {
+    if (PADDED) {  // kb is a multiple of 4
       const uint32_t behind = kb + 4 <= last ? 0u : 0xFFFFFFFFu << (8 * (last - kb));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        w[j] = load<FRESH>(reinterpret_cast<const uint32_t*>(row[j] + at));
+        w[j] = load<FRESH>(reinterpret_cast<const uint32_t*>(row[j] + (int64_t)(kb >> 2) * quad));
         w[j] = (w[j] & ~behind) | (0x7F7F7F7Fu & behind);
       }
+    } else if (words && kb + 4 <= last) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = load<FRESH>(reinterpret_cast<const uint32_t*>(row[j] + kb));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -134,7 +136,7 @@ struct ScaleRows {
         for (int i = 0; i < 4; ++i)
           if (kb + i < last)
             w[j] = (w[j] & ~(0xFFu << (8 * i))) |
-                   ((uint32_t)load<FRESH>(row[j] + at + i) << (8 * i));
+                   ((uint32_t)load<FRESH>(row[j] + kb + i) << (8 * i));
       }
     }
   }
@@ -148,8 +150,7 @@ struct BlockScales {
   int64_t a_pitch, b_pitch;
   int a_shift, b_shift;  // 7 when one scale covers 128 rows
   int row0, col0, m, n, slices;
-  int64_t a_quad = 4, b_quad = 4;  // see ScaleRows
-  bool padded = false;
+  int64_t a_quad = 4, b_quad = 4;  // see ScaleRows (a Source with kPadded)
   uint32_t a_more = 0;  // added to every byte of a's scales
 };
 
@@ -853,7 +854,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
       uint32_t parity = 0;
       uint32_t t = first;
       int kb = 0, slices = 0;
-      bool a_words = false, b_words = false, padded = false;
+      bool a_words = false, b_words = false;
       uint32_t a_more = 0;
       int64_t a_quad = 4, b_quad = 4;
       ScaleRows from[1 + CG];
@@ -865,7 +866,6 @@ __device__ __forceinline__ void run_products(const Source& src) {
           slices = scales.slices;
           a_quad = scales.a_quad;
           b_quad = scales.b_quad;
-          padded = scales.padded;
           a_more = scales.a_more;
           a_words = scale_words(scales.a, scales.a_pitch, 0);
           b_words = scale_words(scales.b, scales.b_pitch, 0);
@@ -876,14 +876,14 @@ __device__ __forceinline__ void run_products(const Source& src) {
             from[1 + c].at(scales.b, scales.b_pitch, scales.b_shift, scales.col0 + 128 * c,
                            scales.n, lane);
         }
-        from[0].read(kb, slices, a_words, next[0], a_quad, padded);
+        from[0].template read<false, Source::kPadded>(kb, slices, a_words, next[0], a_quad);
         if (Source::kExtras) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) next[0][j] = __vadd4(next[0][j], a_more);
         }
 #pragma unroll
         for (int c = 0; c < CG; ++c)
-          from[1 + c].read(kb, slices, b_words, next[1 + c], b_quad, padded);
+          from[1 + c].template read<false, Source::kPadded>(kb, slices, b_words, next[1 + c], b_quad);
         kb += 4;
         if (kb >= slices) {
           kb = 0;

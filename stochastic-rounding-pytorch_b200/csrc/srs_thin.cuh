@@ -40,6 +40,11 @@ constexpr int kThinMaxStages = 12;
 constexpr int kThinSlots = 8;    // scale groups on their way
 constexpr int kThinLoaders = 6;  // warps that bring them
 
+template <int N>
+struct Constant {
+  static constexpr int value = N;
+};
+
 // What else a thin product does.
 enum : int { kThinPlain = 0, kThinGrouped = 1, kThinAdapters = 2 };
 
@@ -458,26 +463,39 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     // columns rank, rank + splits, ...: half of the CTA's threads a column
     const int half = threadIdx.x >> 7, at = threadIdx.x & 127;
     const int out_row = row0 + at;
-    for (int c = (int)rank + half * (int)splits; c < n; c += 2 * (int)splits) {
-      float part[8];
+    const bool write = out_row < row_end && ok;
+    // `columns` of `parts` words in flight, then their stores: one column after the other took a
+    // microsecond more for 64 columns of two parts.
+    const auto join = [&](auto parts, auto columns) {
+      constexpr int P = decltype(parts)::value, C = decltype(columns)::value;
+      for (int c0 = (int)rank + half * P; c0 < n; c0 += 2 * P * C) {
+        float part[C][P];
 #pragma unroll
-      for (uint32_t r = 0; r < 8; ++r) {
-        part[r] = 0.0f;
-        if (r < splits)
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(part[r])
-                       : "r"(map_to_rank(stage0 + 512 * c + 4 * at, r))
-                       : "memory");
+        for (int i = 0; i < C; ++i) {
+          const int c = min(c0 + 2 * P * i, n - 1);
+#pragma unroll
+          for (int r = 0; r < P; ++r)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(part[i][r])
+                         : "r"(map_to_rank(stage0 + 512 * c + 4 * at, (uint32_t)r))
+                         : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int c = c0 + 2 * P * i;
+          float sum = part[i][0];
+#pragma unroll
+          for (int r = 1; r < P; ++r) sum = __fadd_rn(sum, part[i][r]);
+          if (write && c < n)
+            store_value(a.out, a.out_format,
+                        out_row * a.row_stride + (b_row0 + c) * a.col_stride,
+                        ADAPTERS ? sum * factor : sum);
+        }
       }
-      float sum = part[0];
-#pragma unroll
-      for (int r = 1; r < 8; ++r)
-        if (r < (int)splits) sum = __fadd_rn(sum, part[r]);
-      if (out_row < row_end && ok)
-        store_value(a.out, a.out_format,
-                    out_row * a.row_stride + (b_row0 + c) * a.col_stride,
-                    ADAPTERS ? sum * factor : sum);
-    }
+    };
+    if (splits == 2) join(Constant<2>{}, Constant<4>{});
+    else if (splits == 4) join(Constant<4>{}, Constant<4>{});
+    else join(Constant<8>{}, Constant<1>{});
     cluster_sync();  // the others have read this CTA's sums
   }
   tmem_fence_before();
