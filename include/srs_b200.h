@@ -477,8 +477,8 @@ int srs_expert_gradient(const srs_blocks* a_t, const srs_blocks* b_t, int64_t ro
  *   turned == 1:  low_t = s_a up_a^T x_t;    d_t = w x_t + down_a^T low_t    (k = out, w->rows = in)
  * Sums of both parts in FP32, d (tokens x w->rows, in the adapters' format) rounded once.  low:
  * FP32, tokens (in the order of `order`) x rank, or NULL; rows of tokens without an adapter are
- * not written.  largest (FP16 alone): count + 1 words, encodings of max |low| of every adapter and of
- * all, or NULL.  d == NULL: `low` alone.
+ * not written.  largest (FP16 alone): `count` words, encodings of max |low| of every adapter, or
+ * NULL.  d == NULL: `low` alone.
  *
  * srs_adapter_gradient: one or two sums over the tokens of every adapter, out_a = sum of low_t
  * z_t^T (rank x cols) or, turned, z_t low_t^T (cols x rank), in z's format; zeros without tokens.

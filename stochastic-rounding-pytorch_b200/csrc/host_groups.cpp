@@ -400,7 +400,7 @@ at::Tensor adapter_product(const at::Tensor& given, const Rounding& how, Blocks 
     low->values = at::empty({tokens, a.c.rank}, x.options().dtype(at::kFloat));
     // (the sums of FP16 gradients are scaled by it)
     if (a.c.format == SRS_FMT_F16)
-      low->largest = at::empty({a.c.count + 1}, x.options().dtype(at::kInt));
+      low->largest = at::empty({a.c.count}, x.options().dtype(at::kInt));
   }
   if (tokens == 0) return out;
   const int64_t bytes = g_adapter_workspace(tokens, k, project ? n : 0, a.c.count, a.c.rank);

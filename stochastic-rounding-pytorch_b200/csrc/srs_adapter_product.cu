@@ -32,7 +32,7 @@ struct AdapterProduct {
   char* out;
   int format;
   int rank, extra_slices, rest_at;
-  const unsigned int* top;  // of FP16 pairs (null: BF16)
+  const int32_t* exponents;  // of FP16 pairs, one a row (null: BF16)
   bool rows_inner;
   unsigned int* status_at;
 };
@@ -96,11 +96,12 @@ struct AdapterSource {
     s.col0 = col * w.edge;
     s.m = w.m;
     s.n = w.n;
-    s.factor = two_to(-exponent());
+    s.factor = 1.0f;
     s.out = w.out;
     s.format = w.format;
     s.pitch = w.n;
     s.order = w.order;
+    s.exponents = w.exponents;
     return s;
   }
   __device__ BlockScales scales(uint32_t t) const {
@@ -108,13 +109,9 @@ struct AdapterSource {
     w.grid.at(t, &row, &col);
     return {w.scale_a,        w.scale_b,    w.scale_a_pitch, w.scale_b_pitch, 0,
             w.scale_b_shift,  row * w.edge, col * w.edge,    w.m,             w.n,
-            w.slices,         4,            4,               false,
-            in_every_byte(exponent())};
+            w.slices,         4,            4,               w.exponents};
   }
   __device__ void spare(int) const {}
-  __device__ __forceinline__ int exponent() const {
-    return w.top == nullptr ? 0 : pair_exponent(__ldg(w.top));
-  }
   // The first adapter whose rows reach past `row`.
   __device__ __forceinline__ int first_past(int row) const {
     int lo = 0, hi = p.count;
@@ -223,7 +220,7 @@ int launch_adapter_product(const srs_blocks& rows, const srs_blocks& w, int64_t 
   p.out = static_cast<char*>(d);
   p.format = a.format;
   p.rank = a.rank;
-  p.top = a.top;
+  p.exponents = a.exponents;
   p.extra_slices = pairs.slices;
   p.rest_at = pairs.rest_at;
   p.rows_inner = a.rows_inner;

@@ -122,7 +122,8 @@ struct LowArgs {
   uint16_t* pairs;        // items for a product (null: not wanted)
   int edge, pitch, rest_at;
   bool spread;            // items of a thin product: rows are the batch's
-  unsigned int* largest;  // of an adapter's |low|, behind them of all, as encodings (null: not wanted)
+  unsigned int* largest;  // of an adapter's |low|, as encodings (null: not wanted)
+  int32_t* exponents;     // of the tokens' pairs (FP16)
   unsigned int* status;
 };
 
@@ -229,29 +230,53 @@ __device__ __forceinline__ void write_low(const LowArgs& a, const LowTile& l, fl
     clear_items(a, tile, most, l.rank0, whole, (int)threadIdx.x + threads * split, threads * splits);
   if (a.largest != nullptr) {
     const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_size));
-    if ((threadIdx.x & 31) == 0 && top != 0u) {  // (the order is no matter)
-      atomicMax(a.largest + tile.group, top);
-      atomicMax(a.largest + a.adapters, top);
-    }
+    // (the order is no matter)
+    if ((threadIdx.x & 31) == 0 && top != 0u) atomicMax(a.largest + tile.group, top);
   }
   if (splits > 1) cg::this_cluster().sync();  // the others have read this CTA's sums
 }
 
-// FP16 pairs, of the finished FP32 low part: what they are scaled by depends on all of it.
-constexpr int kPairTokens = 128, kPairThreads = 256;
+// FP16 pairs, of the finished FP32 low part: what they are scaled by depends on all of a token's.  A
+// warp a token.
+constexpr int kPairTokens = 32, kPairThreads = 256;
 
 __global__ void __launch_bounds__(kPairThreads) pairs_kernel(const LowArgs a) {
   // A thin product launched to overlap this kernel may start.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const GroupTile tile = find_group_tile(a.ends, a.adapters, a.tokens, kPairTokens,
                                          (int)blockIdx.x, (int)(threadIdx.x & 31));
+  const int lane = threadIdx.x & 31;
+  const auto exponent_of = [&](int place) {
+    return a.exponents + (a.spread ? token_at(a.order, place, a.tokens) : place);
+  };
+  {
+    // tokens of no adapter, by all threads of the grid
+    const EndsAhead ahead(a.ends, a.adapters, lane);
+    int last = 0;
+    for (int base = 0; base < a.adapters; base += 32) {
+      int start, end;
+      group_span(a.ends, ahead, a.adapters, a.tokens, base, lane, &last, &start, &end);
+    }
+    for (int i = last + (int)(blockIdx.x * kPairThreads + threadIdx.x); i < a.tokens;
+         i += (int)gridDim.x * kPairThreads)
+      *exponent_of(i) = 0;
+  }
   if (tile.group < 0) return;
   const int count = min(kPairTokens, tile.end - tile.row0), whole = (a.rank + 15) & ~15;
-  const float factor = two_to(pair_exponent(__ldcg(a.largest + a.adapters)));
-  for (int i = threadIdx.x; i < count * whole; i += kPairThreads) {
-    const int place = tile.row0 + i / whole, r = i % whole;
-    const float v = r < a.rank ? __ldcg(a.low + (int64_t)place * a.rank + r) * factor : 0.0f;
-    write_pair<SRS_FMT_F16>(a, tile, place, r, v);
+  for (int t = threadIdx.x >> 5; t < count; t += kPairThreads / 32) {
+    const int place = tile.row0 + t;
+    const float* const from = a.low + (int64_t)place * a.rank;
+    float top_size = 0.0f;
+    for (int r = lane; r < a.rank; r += 32) {
+      const float size = fabsf(__ldcg(from + r));
+      top_size = fmaxf(top_size, isfinite(size) ? size : 0.0f);
+    }
+    const int k =
+        pair_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_size)));
+    const float factor = two_to(k);
+    for (int r = lane; r < whole; r += 32)
+      write_pair<SRS_FMT_F16>(a, tile, place, r, r < a.rank ? __ldcg(from + r) * factor : 0.0f);
+    if (lane == 0) *exponent_of(place) = k;
   }
   clear_items(a, tile, kPairTokens, 0, whole, (int)threadIdx.x, kPairThreads);
 }
@@ -864,9 +889,9 @@ using namespace srs;
 static bool few(int64_t tokens) { return tokens <= kThinRows; }
 
 // Parts of a call's workspace, each on a 256-byte boundary: the quantised tokens first; FP16 alone
-// needs `low` and `largest` (for both formats there is room).
+// needs `low` and `exponents` (for both formats there is room).
 struct AdapterSpace {
-  int64_t pairs, low, largest, total;
+  int64_t pairs, low, exponents, total;
 };
 
 static AdapterSpace adapter_space(int64_t tokens, int64_t k, int64_t n, int adapters, int rank) {
@@ -878,8 +903,8 @@ static AdapterSpace adapter_space(int64_t tokens, int64_t k, int64_t n, int adap
                        : pair_items(tokens, adapters, adapter_edge(tokens, n, k)) *
                              adapter_edge(tokens, n, k);
   s.low = s.pairs + whole(rows * pair_shape(rank).pitch * 2);
-  s.largest = s.low + (n > 0 ? whole(tokens * rank * 4) : 0);
-  s.total = s.largest + whole((adapters + 1) * 4);
+  s.exponents = s.low + (n > 0 ? whole(tokens * rank * 4) : 0);
+  s.total = s.exponents + (n > 0 ? whole(tokens * 4) : 0);
   return s;
 }
 
@@ -919,10 +944,8 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   const bool bf16 = a->format == SRS_FMT_BF16, thin = few(tokens);
 
   cudaError_t e = cudaSuccess;
-  unsigned int* const sizes =
-      bf16 ? nullptr : largest != nullptr ? largest
-                                          : reinterpret_cast<unsigned int*>(at + space.largest);
-  if (sizes != nullptr) e = cudaMemsetAsync(sizes, 0, ((size_t)a->count + 1) * 4, st);
+  if (bf16) largest = nullptr;
+  if (largest != nullptr) e = cudaMemsetAsync(largest, 0, (size_t)a->count * 4, st);
   // without a sum there is neither a projection nor a low part
   if (e == cudaSuccess && n > 0 && k == 0) e = cudaMemsetAsync(d, 0, (size_t)(tokens * n * 2), st);
   if (e != cudaSuccess) return cuda_fail(e, "srs_adapter_linear");
@@ -943,7 +966,8 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   l.scale = reinterpret_cast<const float*>(a->scale);
   l.factor = a->factor;
   l.low = low != nullptr ? low : bf16 ? nullptr : reinterpret_cast<float*>(at + space.low);
-  l.largest = sizes;
+  l.largest = largest;
+  l.exponents = reinterpret_cast<int32_t*>(at + space.exponents);
   if (int rc = status_word(&l.status)) return rc;
   if (edge != 0) {
     if (bf16) l.pairs = reinterpret_cast<uint16_t*>(at + space.pairs);
@@ -987,7 +1011,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
                          a->format,
                          l.order,
                          l.ends,
-                         bf16 ? nullptr : sizes + a->count};
+                         bf16 ? nullptr : l.exponents};
   // (with few tokens beside the quantisation: the weights are streamed first)
   return thin ? launch_thin(*w, rows, k, d, a->format, 1, n, true, st, &call)
               : launch_adapter_product(rows, *w, k, call, edge, d, st);

@@ -76,7 +76,8 @@ struct AdapterCall {
   int count, rank, format;
   const int32_t* order;
   const int32_t* ends;
-  const unsigned int* top;  // FP16: encoding of the largest |low|, by which the pairs are scaled
+  // FP16: powers of two of the tokens' pairs (thin: in the batch's order, else the adapters')
+  const int32_t* exponents;
 };
 
 // FP8 blocks: d = a b^T (operands checked by the caller).  Element (i, j)

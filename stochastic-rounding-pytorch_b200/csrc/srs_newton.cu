@@ -330,7 +330,7 @@ struct NewtonWork {
 // itself, so that P has no a I, except in the last step, whose result is not in FP16.)
 template <bool SPLIT>
 struct NewtonProducts {
-  static constexpr bool kExtras = false, kPadded = false;
+  static constexpr bool kExtras = false;
   const NewtonWork<SPLIT>& w;
   struct Place {
     int shape, batch, row, col;

@@ -366,7 +366,7 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
     args.rank = adapters->rank;
     args.item_slices = pairs.slices;
     args.rest_at = pairs.rest_at;
-    args.top = adapters->top;
+    args.exponents = adapters->exponents;
     args.up_rows_inner = adapters->rows_inner;
     args.extra_idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
                        (d_format == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u);

@@ -89,7 +89,8 @@ struct TileStore {
   int format;      // SRS_FMT_F32, SRS_FMT_BF16 or SRS_FMT_F16
   int64_t pitch;   // elements
   float step, decay;  // update: p' = fma(step, D, p * decay)
-  const int32_t* order;  // row i of D is stored as row order[i] (kScatter)
+  const int32_t* order;      // kExtras: row i of D is stored as row order[i],
+  const int32_t* exponents;  // times 2^-exponents[i] (null: as it is)
 };
 
 // Scales of one operand for a warp: rows row0 + lane + 32 j (j < 4), blocks kb ..
@@ -151,12 +152,13 @@ struct BlockScales {
   int a_shift, b_shift;  // 7 when one scale covers 128 rows
   int row0, col0, m, n, slices;
   int64_t a_quad = 4, b_quad = 4;  // see ScaleRows (a Source with kPadded)
-  uint32_t a_more = 0;  // added to every byte of a's scales
+  const int32_t* a_exponents = nullptr;  // added to a's scales, one a row (null: none)
 };
 
 // FP16 pairs of a low part are held times 2^k, so that small gradients keep their digits and large
-// values fit: k brings the largest of all to 2^13 .. 2^14.  The FP8 product they are added to gets the
-// same factor through its block scales (bytes of FP16 values' blocks lie in 88 .. 135), and the
+// values fit: k brings a token's largest to 2^13 .. 2^14 (the token's own, so that its results do not
+// depend on what else is in the batch).  The FP8 product they are added to gets the same factor
+// through the token's block scales (bytes of FP16 values' blocks lie in 88 .. 135), and the
 // results lose it again.  `top`: encoding of the largest; 0: none.  (Up to 2^30: then a pair's
 // last digit is far below that of any FP16 result, and no sum leaves FP32's range.)
 __device__ __forceinline__ int pair_exponent(uint32_t top) {
@@ -855,7 +857,7 @@ __device__ __forceinline__ void run_products(const Source& src) {
       uint32_t t = first;
       int kb = 0, slices = 0;
       bool a_words = false, b_words = false;
-      uint32_t a_more = 0;
+      uint32_t more[4] = {0u, 0u, 0u, 0u};  // kExtras: for a's scales of the tile
       int64_t a_quad = 4, b_quad = 4;
       ScaleRows from[1 + CG];
       uint32_t next[1 + CG][4];
@@ -866,7 +868,6 @@ __device__ __forceinline__ void run_products(const Source& src) {
           slices = scales.slices;
           a_quad = scales.a_quad;
           b_quad = scales.b_quad;
-          a_more = scales.a_more;
           a_words = scale_words(scales.a, scales.a_pitch, 0);
           b_words = scale_words(scales.b, scales.b_pitch, 0);
           from[0].at(scales.a, scales.a_pitch, scales.a_shift, scales.row0 + 128 * (int)rank,
@@ -875,12 +876,14 @@ __device__ __forceinline__ void run_products(const Source& src) {
           for (int c = 0; c < CG; ++c)
             from[1 + c].at(scales.b, scales.b_pitch, scales.b_shift, scales.col0 + 128 * c,
                            scales.n, lane);
+          if (Source::kExtras && scales.a_exponents != nullptr) {
+            const int row = scales.row0 + 128 * (int)rank + lane;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              more[j] = in_every_byte(__ldg(scales.a_exponents + min(row + 32 * j, scales.m - 1)));
+          }
         }
         from[0].template read<false, Source::kPadded>(kb, slices, a_words, next[0], a_quad);
-        if (Source::kExtras) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) next[0][j] = __vadd4(next[0][j], a_more);
-        }
 #pragma unroll
         for (int c = 0; c < CG; ++c)
           from[1 + c].template read<false, Source::kPadded>(kb, slices, b_words, next[1 + c], b_quad);
@@ -890,17 +893,21 @@ __device__ __forceinline__ void run_products(const Source& src) {
           t += step;
         }
       };
-      bool more = t < tiles;
-      if (more) request();
-      while (more) {
+      bool left = t < tiles;
+      if (left) request();
+      while (left) {
         uint32_t w[1 + CG][4];
 #pragma unroll
         for (int c = 0; c < 1 + CG; ++c) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[c][j] = next[c][j];
         }
-        more = t < tiles;
-        if (more) request();
+        if (Source::kExtras) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[0][j] = __vadd4(w[0][j], more[j]);
+        }
+        left = t < tiles;
+        if (left) request();
         ok = barrier_wait(scale_empty(slot), parity ^ 1u, status, 32u);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
@@ -957,8 +964,10 @@ __device__ __forceinline__ void run_products(const Source& src) {
           load_addend(at, row0, at.col0 + 32 * part * kPieces, lane, add);
         }
         int to = 0;
-        if (Source::kExtras && row0 + lane < at.m)
+        if (Source::kExtras && row0 + lane < at.m) {
           to = min(max(__ldg(at.order + row0 + lane), 0), at.m - 1);
+          if (at.exponents != nullptr) at.factor = two_to(-__ldg(at.exponents + row0 + lane));
+        }
         float late = 1.0f;
         if (NEWTON && at.late != nullptr) late = __ldg(at.late);
         ok = barrier_wait(acc_full(acc), (count >> 1) & 1u, status, 128u, patience);

@@ -72,7 +72,7 @@ struct ThinArgs {
   CUtensorMap map_h, map_u;
   int rank, item_slices, rest_at;
   bool up_rows_inner;  // U is stored rank x rows
-  const unsigned int* top;  // of FP16 pairs (null: BF16)
+  const int32_t* exponents;  // of FP16 pairs, one a token (null: BF16)
   uint32_t extra_idesc;
 };
 
@@ -372,20 +372,27 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     }
     const int groups = (last - first + 3) >> 2;
     bool waited = false;
+    uint32_t more[4] = {0u, 0u, 0u, 0u};  // ADAPTERS: for B's scales
     for (int g = warp < 4 ? warp : warp - 2; g < groups; g += kThinLoaders) {
       const int slot = g % kThinSlots, kb = first + 4 * g;
       uint32_t w[2][4];
       from_a.read(kb, last, words_a, w[0]);
-      if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (!waited) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if constexpr (ADAPTERS) {
+          // (written ahead of this kernel, as B is)
+          if (a.exponents != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              more[j] = in_every_byte(__ldcg(a.exponents + min(lane + 32 * j, a.n - 1)));
+          }
+        }
+      }
       waited = true;
       from_b.read<true>(kb, last, words_b, w[1]);
       if constexpr (ADAPTERS) {
-        // (written ahead of this kernel, as B is)
-        if (a.top != nullptr) {
-          const uint32_t more = in_every_byte(pair_exponent(__ldcg(a.top)));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[1][j] = __vadd4(w[1][j], more);
-        }
+        for (int j = 0; j < 4; ++j) w[1][j] = __vadd4(w[1][j], more[j]);
       }
       ok = barrier_wait(scale_empty(slot), ((uint32_t)(g / kThinSlots) & 1u) ^ 1u, a.status,
                         1u << 12);
@@ -423,11 +430,14 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_after();
   const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
   const int row = row0 + 32 * warp + lane, row_end = min(a.m, row0 + a.rows);
-  float factor = 1.0f;  // FP16 pairs': a power of two
-  if constexpr (ADAPTERS) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (a.top != nullptr) factor = two_to(-pair_exponent(__ldcg(a.top)));
-  }
+  if constexpr (ADAPTERS) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // A sum of column c without the power of two of its FP16 pairs.
+  const auto result = [&](float sum, int c) {
+    if constexpr (ADAPTERS) {
+      if (a.exponents != nullptr) return sum * two_to(-__ldcg(a.exponents + c));
+    }
+    return sum;
+  };
   if (splits == 1) {
     if (warp < 4 && ok) {
 #pragma unroll
@@ -440,7 +450,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           if (row < row_end && c0 + c < n)
             store_value(a.out, a.out_format,
                         row * a.row_stride + (b_row0 + c0 + c) * a.col_stride,
-                        ADAPTERS ? __uint_as_float(v[c]) * factor : __uint_as_float(v[c]));
+                        result(__uint_as_float(v[c]), c0 + c));
       }
     }
   } else {
@@ -489,7 +499,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           if (write && c < n)
             store_value(a.out, a.out_format,
                         out_row * a.row_stride + (b_row0 + c) * a.col_stride,
-                        ADAPTERS ? sum * factor : sum);
+                        result(sum, c));
         }
       }
     };

@@ -241,6 +241,30 @@ def test_tokens_of_other_adapters_do_not_matter(cuda_device):
     assert got[1][1].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40, 200, 700])
+def test_large_low_parts_of_one_adapter_leave_the_others_alone(tokens, dtype, cuda_device):
+    k, n, rank = 320, 400, 20
+    x = values((tokens + 5, k), 1, cuda_device, dtype)
+    down = values((2, rank, k), 2, cuda_device, dtype, k**-0.5)
+    up = values((2, n, rank), 3, cuda_device, dtype, 0.1)
+    w = quantize_blocks(values((n, k), 4, cuda_device, dtype, 0.1), block=(128, 128),
+                        orientation="both")
+    index = torch.zeros(tokens + 5, dtype=torch.int32, device=cuda_device)
+    index[tokens // 2:tokens // 2 + 5] = 1
+    dy = values((tokens + 5, n), 5, cuda_device, dtype)
+    groups, results = group_rows(index, 2), []
+    for size in (1.0, 2.0**40):
+        scale = torch.tensor([0.7, size], device=cuda_device)
+        a, b, v = (t.clone().requires_grad_() for t in (down, up, x))
+        y = adapter_linear(v, w, a, b, groups, scale=scale)
+        results.append((y.detach(), *torch.autograd.grad(y, (v, a, b), dy)))
+    others = index == 0
+    for one, two in zip(*results):
+        rows = others if one.shape[0] == tokens + 5 else 0
+        assert torch.equal(one[rows], two[rows])
+
+
 @pytest.mark.parametrize("tokens", [40, 200])
 def test_plans_that_make_no_sense_stay_inside(tokens, cuda_device):
     """Entries of the order outside the tokens, ends that fall or pass them: results are those of
