@@ -134,14 +134,19 @@ srs_blocks stack_operand(const char* name, Blocks* b) {
 }
 
 // A 16-bit matrix, or a stack of them, whose rows start on 16-byte boundaries; one laid out
-// otherwise is copied once.  `whole`: rows of whole 16 bytes as well.
+// otherwise is copied once.  `whole`: with memory up to 16 bytes behind the last row, too.
 at::Tensor aligned(const at::Tensor& t, bool whole) {
   const int64_t last = t.dim() - 1, cols = t.size(last);
+  if (t.numel() == 0) return t;
   bool good = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-              (cols <= 1 || t.stride(last) == 1) && (!whole || cols % 8 == 0);
-  for (int64_t d = 0; d < last; ++d)
+              (cols <= 1 || t.stride(last) == 1);
+  int64_t end = t.storage_offset() + ceil_div(cols, 8) * 8;
+  for (int64_t d = 0; d < last; ++d) {
     good = good && (t.size(d) <= 1 || (t.stride(d) % 8 == 0 && (d != last - 1 || t.stride(d) >= cols)));
-  if (good || t.numel() == 0) return t;
+    end += (t.size(d) - 1) * t.stride(d);
+  }
+  good = good && (!whole || 2 * end <= (int64_t)t.storage().nbytes());
+  if (good) return t;
   std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
   sizes[last] = ceil_div(cols, 8) * 8;
   const at::Tensor wide = at::empty(sizes, t.options());
