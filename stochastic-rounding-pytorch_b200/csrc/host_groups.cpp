@@ -39,7 +39,7 @@ void* stream_of(const at::Tensor& t) {
 
 const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 
-// `ends` as int32 on x's device (int64 is converted).
+// `ends` as int32 on x's device (int64 is converted, what is too large for int32 to its largest).
 at::Tensor checked_ends(const at::Tensor& ends, const at::Tensor& x, const char* what) {
   TORCH_CHECK_TYPE(ends.scalar_type() == at::kInt || ends.scalar_type() == at::kLong, what,
                    ": ends are int32 or int64, got ", ends.scalar_type());
@@ -47,7 +47,8 @@ at::Tensor checked_ends(const at::Tensor& ends, const at::Tensor& x, const char*
                     ": ends must have one dimension and one entry a group, got shape ",
                     ends.sizes());
   TORCH_CHECK_VALUE(ends.device() == x.device(), "all tensors must be on the same CUDA device");
-  return ends.to(at::kInt).contiguous();
+  if (ends.scalar_type() == at::kLong) return ends.clamp(0, INT32_MAX).to(at::kInt).contiguous();
+  return ends.contiguous();
 }
 
 srs_block_copy copy_of(const Blocks& b) {

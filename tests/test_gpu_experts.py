@@ -154,12 +154,14 @@ def test_ends_that_make_no_sense_stay_inside(cuda_device):
     w = values((4, n, k), 2, cuda_device, torch.bfloat16).requires_grad_()
     dy = values((100, n), 3, cuda_device, torch.bfloat16)
     results = []
-    for ends in ([40, 10, 2000, -5], [40, 40, 100, 100]):
-        ends = torch.tensor(ends, dtype=torch.int32, device=cuda_device)
+    for ends, dtype in (([40, 40, 100, 100], torch.int32), ([40, 10, 2000, -5], torch.int32),
+                        ([40, 10, 2**40, -2**40], torch.int64)):
+        ends = torch.tensor(ends, dtype=dtype, device=cuda_device)
         y = expert_linear(x, w, ends, seed=2)
         results.append((y.detach(), *torch.autograd.grad(y, (x, w), dy)))
-    for got, want in zip(*results):
-        assert torch.equal(got, want)
+    for result in results[1:]:
+        for got, want in zip(result, results[0]):
+            assert torch.equal(got, want)
 
 
 def test_strides_and_layouts(cuda_device):
