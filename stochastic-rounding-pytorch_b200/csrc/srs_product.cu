@@ -47,7 +47,7 @@ int find_encode(EncodeTiled* out) {
 }  // namespace
 
 int encode_operand(const ProductOperand& o, int element_bytes, int64_t batch, int box_rows,
-                   CUtensorMap* map) {
+                   CUtensorMap* map, int box_bytes) {
   EncodeTiled encode = nullptr;
   if (int rc = find_encode(&encode)) return rc;
   const uint64_t size = (uint64_t)element_bytes;
@@ -55,13 +55,16 @@ int encode_operand(const ProductOperand& o, int element_bytes, int64_t batch, in
                               (cuuint64_t)(o.rows_inner ? o.k : o.rows), (cuuint64_t)batch};
   const uint64_t entry = batch > 1 ? (uint64_t)o.batch_stride : (uint64_t)o.pitch * dims[1];
   const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * size, entry * size};
-  const cuuint32_t box[3] = {(cuuint32_t)(kSliceBytes / size),
+  const cuuint32_t box[3] = {(cuuint32_t)(box_bytes / size),
                              o.rows_inner ? 64u : (cuuint32_t)box_rows, 1u};
   const cuuint32_t ones[3] = {1, 1, 1};
   const CUresult r = encode(
       map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
       const_cast<void*>(o.base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      box_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+      : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                        : CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(SRS_ERR_CUDA,
@@ -359,8 +362,19 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
     const ProductOperand low{adapters->pairs, items * columns, pairs.pitch, pairs.pitch, 0, false};
     const ProductOperand up{adapters->up,    a.rows, adapters->rank, adapters->pitch,
                             adapters->stride, adapters->rows_inner};
-    if (int rc = encode_operand(low, 2, 1, columns, &args.map_h)) return rc;
-    if (int rc = encode_operand(up, 2, adapters->count, args.rows, &args.map_u)) return rc;
+    // Ranks up to 16: as many adapters' narrow boxes a stage as fit, U's and behind them the pairs'.
+    if (adapters->rank <= 16 && !adapters->rows_inner) {
+      const int high = (args.rows + 7) / 8 * 8, stage = (high + columns) * kSliceBytes;
+      for (args.pack = 4; args.pack > 1; --args.pack) {
+        args.pack_at = (args.pack * high * 32 + 1023) / 1024 * 1024;
+        if (args.pack_at + args.pack * columns * 64 <= stage) break;
+      }
+      if (args.pack == 1) args.pack_at = (high * 32 + 1023) / 1024 * 1024;
+    }
+    const bool narrow = args.pack != 0;
+    if (int rc = encode_operand(low, 2, 1, columns, &args.map_h, narrow ? 64 : 128)) return rc;
+    if (int rc = encode_operand(up, 2, adapters->count, args.rows, &args.map_u, narrow ? 32 : 128))
+      return rc;
     args.ends = adapters->ends;
     args.groups = adapters->count;
     args.rank = adapters->rank;

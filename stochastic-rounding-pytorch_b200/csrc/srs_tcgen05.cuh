@@ -282,6 +282,11 @@ __device__ __forceinline__ uint64_t operand_descriptor(bool rows_inner) {
   const uint64_t lead = rows_inner ? 8192u >> 4 : 1u;
   return (lead << 16) | (uint64_t(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+// k contiguous in rows of 32 or 64 bytes, swizzled over as many.
+__device__ __forceinline__ uint64_t narrow_descriptor(int row_bytes) {
+  return (1ull << 16) | (uint64_t(row_bytes * 8) >> 4 << 32) | (1ull << 46) |
+         ((row_bytes == 32 ? 6ull : 4ull) << 61);
+}
 // Scale blocks: unswizzled 8 x 16-byte core matrices, 128 bytes apart.
 __device__ __forceinline__ uint64_t scale_descriptor(uint32_t addr) {
   return uint64_t((addr >> 4) & 0x3FFFu) | (1ull << 16) | (uint64_t(128u >> 4) << 32) |

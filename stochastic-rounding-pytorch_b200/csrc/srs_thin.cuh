@@ -27,6 +27,9 @@
 // for its adapter's tokens, by the adapter's U; the CTAs of a cluster take the adapters in turn.
 // (In a kernel of its own behind this one that part took 5 us for one token and 10 for 64 with
 // 41 adapters, nearly all of it launch and dependent loads; in this one's epilogue as much.)
+// Ranks up to 16 take narrow boxes, three adapters a stage: with one a stage, of boxes of 128 bytes
+// that were mostly fill, 64 tokens of 40 adapters waited for four loads in flight (14336 x 4096:
+// 34 us a call in a graph, now 30.8; of one adapter 24.6, without any 17.6).
 #pragma once
 
 #include "srs_groups.cuh"
@@ -72,6 +75,9 @@ struct ThinArgs {
   CUtensorMap map_h, map_u;
   int rank, item_slices, rest_at;
   bool up_rows_inner;  // U is stored rank x rows
+  // Ranks up to 16: adapters a stage (0: see item_slices), boxes of 32 bytes a row of U, and behind
+  // them, from pack_at on, of 64 bytes a token of the pairs.
+  int pack, pack_at;
   const int32_t* exponents;  // of FP16 pairs, one a token (null: BF16)
   uint32_t extra_idesc;
 };
@@ -222,7 +228,26 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     }
     if constexpr (ADAPTERS) {
       asm volatile("bar.sync 1, 96;" ::: "memory");  // the list of adapters
-      const int slices = a.item_slices, chunks = (slices + 1) / 2;
+      const int slices = a.pack != 0 ? 0 : a.item_slices, chunks = (slices + 1) / 2;
+      for (int e0 = (int)rank; a.pack != 0 && e0 < actives && ok; e0 += (int)splits * a.pack) {
+        const uint32_t pa = stage0 + s * stage_bytes;
+        ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
+        if (!ok) break;
+        if (leader) {
+          const int count = min(a.pack, (actives - e0 + (int)splits - 1) / (int)splits);
+          barrier_expect(full(s), (uint32_t)(count * (a.rows * 32 + BN * 64)));
+          for (int i = 0; i < count; ++i) {
+            const int e = e0 + i * (int)splits;
+            load_box<1>(pa + i * (panel_bytes / 4), &a.map_u, 0, row0, active[e], full(s));
+            load_box<1>(pa + a.pack_at + i * (BN * 64), &a.map_h, 0, e * BN, 0, full(s));
+          }
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
       for (int e = (int)rank; e < actives && ok; e += (int)splits) {
         for (int q = 0; q < slices && ok; ++q) {
           const uint32_t pa = stage0 + s * stage_bytes;
@@ -306,7 +331,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     }
     if constexpr (ADAPTERS) {
       asm volatile("bar.sync 1, 96;" ::: "memory");
-      const int slices = a.item_slices, chunks = (slices + 1) / 2;
+      const int slices = a.pack != 0 ? 0 : a.item_slices, chunks = (slices + 1) / 2;
       // Behind the MMAs of the other kind: nothing says that the two keep their order.
       if (ok && (int)rank < actives)
         ok = barrier_wait(empty(s == 0 ? stages - 1 : s - 1), s == 0 ? phase ^ 1u : phase, a.status,
@@ -315,6 +340,29 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       const uint64_t desc_u = operand_descriptor(inner);
       const uint32_t step_u = (inner ? 2048u : 32u) >> 4;
       const uint32_t idesc = a.extra_idesc | (inner ? 1u << 15 : 0u);
+      for (int e0 = (int)rank; a.pack != 0 && e0 < actives && ok; e0 += (int)splits * a.pack) {
+        ok = barrier_wait(full(s), phase, a.status, 1u << 11);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t pa = stage0 + s * stage_bytes;
+        if (leader) {
+          const int count = min(a.pack, (actives - e0 + (int)splits - 1) / (int)splits);
+          for (int i = 0; i < count; ++i) {
+            const uint64_t du = narrow_descriptor(32) |
+                                uint64_t(((pa + i * (panel_bytes / 4)) >> 4) & 0x3FFFu);
+            const uint64_t dh = narrow_descriptor(64) |
+                                uint64_t(((pa + a.pack_at + i * (BN * 64)) >> 4) & 0x3FFFu);
+            mma_f16<1>(tmem, du, dh, idesc, 1u);
+            mma_f16<1>(tmem, du, dh + 2, idesc, 1u);  // the pairs' second parts
+          }
+          mma_commit<1>(empty(s));
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
       for (int e = (int)rank; e < actives && ok; e += (int)splits) {
         for (int q = 0; q < slices && ok; ++q) {
           ok = barrier_wait(full(s), phase, a.status, 1u << 11);
