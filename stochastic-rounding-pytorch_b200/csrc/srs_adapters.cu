@@ -296,12 +296,16 @@ struct FewShape {
 template <int F, bool KINNER, int RT>
 __global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(const LowArgs a) {
   using S = FewShape<RT>;
-  // The quantisation behind this kernel reads nothing of it and waits for it at its end.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const LowTile l = low_tile(a, S::kTokens, S::kRank, lane);
-  if (l.tile.group < 0) return;  // the whole cluster
+  // This kernel runs beside the quantisation, of which it reads nothing, but no CTA of it lets the
+  // product behind start, or leaves, before that is done: the product starts with the tokens'
+  // blocks there and waits for the low part alone, when it comes to the adapters.
+  if (l.tile.group < 0) {  // the whole cluster
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const uint32_t base = smem_address(raw);
   const int slot = threadIdx.x & 7, row = threadIdx.x >> 3;
   const char* const from =
@@ -341,6 +345,8 @@ __global__ void __launch_bounds__(FewShape<RT>::kThreads, 4) low_few_kernel(cons
     if (l.first + i < l.last) load(l.first + i, i);
     copies_done();
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int s = 0;
   for (int step = l.first; step < l.last; ++step) {
     copies_wait<S::kStages - 2>();
@@ -786,9 +792,9 @@ int allow_shared(const void* kernel, int bytes) {
   return prepare_kernel(kernel, 1, 32, bytes, &resident);
 }
 
-// `room`: CTAs that run at once.
+// `room`: CTAs that run at once.  `overlap`: may start beside the kernel ahead.
 int launch_low_kernel(const void* kernel, const LowArgs& args, int most, int rank_block, int threads,
-                      int smem, int64_t room, cudaStream_t stream) {
+                      int smem, int64_t room, bool overlap, cudaStream_t stream) {
   if (int rc = allow_shared(kernel, smem)) return rc;
   const int64_t busy = args.adapters < args.tokens ? args.adapters : args.tokens;
   const int64_t tiles = most_group_tiles(args.tokens, args.adapters, most);
@@ -800,16 +806,18 @@ int launch_low_kernel(const void* kernel, const LowArgs& args, int most, int ran
   if (splits > steps / 4) splits = steps / 4;
   splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
   cudaLaunchConfig_t config{};
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = (unsigned)splits;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = (unsigned)splits;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.gridDim = dim3((unsigned)(tiles * splits), (unsigned)blocks);
   config.blockDim = dim3((unsigned)threads);
   config.dynamicSmemBytes = (size_t)smem;
   config.stream = stream;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = overlap ? 2 : 1;
   LowArgs copy = args;
   void* arguments[1] = {&copy};
   const cudaError_t e = cudaLaunchKernelExC(&config, kernel, arguments);
@@ -817,22 +825,22 @@ int launch_low_kernel(const void* kernel, const LowArgs& args, int most, int ran
 }
 
 template <int F, bool KINNER, int RT>
-int launch_low_as(const LowArgs& args, bool thin, cudaStream_t stream) {
+int launch_low_as(const LowArgs& args, bool thin, bool overlap, cudaStream_t stream) {
   const int64_t sms = sm_count();
   if (thin)
     return launch_low_kernel(reinterpret_cast<const void*>(&low_few_kernel<F, KINNER, RT>), args,
                              FewShape<RT>::kTokens, FewShape<RT>::kRank, FewShape<RT>::kThreads,
-                             FewShape<RT>::kSmem, (RT == 4 ? 2 : 4) * sms, stream);
+                             FewShape<RT>::kSmem, (RT == 4 ? 2 : 4) * sms, overlap, stream);
   return launch_low_kernel(reinterpret_cast<const void*>(&low_many_kernel<F, KINNER, RT>), args,
                            kManyTokens, ManyShape<RT>::kRank, kManyThreads, ManyShape<RT>::kSmem,
-                           2 * sms, stream);
+                           2 * sms, overlap, stream);
 }
 
 template <int F, bool KINNER>
-int launch_low(const LowArgs& args, bool thin, cudaStream_t stream) {
-  if (args.rank <= 16) return launch_low_as<F, KINNER, 1>(args, thin, stream);
-  if (args.rank <= 32) return launch_low_as<F, KINNER, 2>(args, thin, stream);
-  return launch_low_as<F, KINNER, 4>(args, thin, stream);
+int launch_low(const LowArgs& args, bool thin, bool overlap, cudaStream_t stream) {
+  if (args.rank <= 16) return launch_low_as<F, KINNER, 1>(args, thin, overlap, stream);
+  if (args.rank <= 32) return launch_low_as<F, KINNER, 2>(args, thin, overlap, stream);
+  return launch_low_as<F, KINNER, 4>(args, thin, overlap, stream);
 }
 
 template <int F, int RT>
@@ -976,12 +984,18 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
     l.rest_at = pairs.rest_at;
     l.spread = thin;
   }
-  if (int rc = turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, thin, st)
-                              : launch_low<SRS_FMT_F16, false>(l, thin, st))
-                      : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, thin, st)
-                              : launch_low<SRS_FMT_F16, true>(l, thin, st)))
-    return rc;
-  if (n == 0 || k == 0) return SRS_OK;
+  // Quantisation and low part run beside each other: with few tokens the quantisation first, as the
+  // product waits for the low part only when it comes to the adapters; with many the longer one.
+  const bool project = n > 0 && k > 0;
+  const auto low_part = [&](bool overlap) {
+    return turned ? (bf16 ? launch_low<SRS_FMT_BF16, false>(l, thin, overlap, st)
+                          : launch_low<SRS_FMT_F16, false>(l, thin, overlap, st))
+                  : (bf16 ? launch_low<SRS_FMT_BF16, true>(l, thin, overlap, st)
+                          : launch_low<SRS_FMT_F16, true>(l, thin, overlap, st));
+  };
+  if (!thin || !project)
+    if (int rc = low_part(false)) return rc;
+  if (!project) return SRS_OK;
 
   srs_blocks rows{};
   rows.data = reinterpret_cast<uint64_t>(workspace);
@@ -993,8 +1007,10 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   QuantizeCall q{x, a->format, tokens, k, x_pitch, block_format, rule, false, seed, 0u};
   q.copy = {rows.data, rows.scale, rows.pitch, rows.scale_pitch, 0, 0};
   q.order = thin ? nullptr : l.order;
-  q.overlap = true;  // beside the low part
+  q.overlap = !thin;
   if (int rc = quantize(q, st)) return rc;
+  if (thin)
+    if (int rc = low_part(true)) return rc;
   if (!bf16) {
     l.pairs = reinterpret_cast<uint16_t*>(at + space.pairs);
     pairs_kernel<<<(unsigned)most_group_tiles(tokens, a->count, kPairTokens), kPairThreads, 0, st>>>(l);
@@ -1012,7 +1028,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
                          l.order,
                          l.ends,
                          bf16 ? nullptr : l.exponents};
-  // (with few tokens beside the quantisation: the weights are streamed first)
+  // (with few tokens beside the low part or its pairs: weights and tokens' blocks are streamed first)
   return thin ? launch_thin(*w, rows, k, d, a->format, 1, n, true, st, &call)
               : launch_adapter_product(rows, *w, k, call, edge, d, st);
 }

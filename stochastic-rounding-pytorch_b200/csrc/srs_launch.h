@@ -18,10 +18,10 @@ struct ProductOperand {
   bool rows_inner;
 };
 
-// Tensor map of an operand: boxes of `box_rows` rows x 128 bytes of k, or of 64 rows x
+// Tensor map of an operand: boxes of `box_rows` rows x `box_bytes` (32, 64, 128) of k, or of 64 rows x
 // 64 k when the row index is contiguous; elements outside the operand read as zero.
 int encode_operand(const ProductOperand& o, int element_bytes, int64_t batch, int box_rows,
-                   CUtensorMap* map, int box_bytes = 128);  // (bytes of k in a box)
+                   CUtensorMap* map, int box_bytes = 128);
 
 // The word of the current device in which bounded waits record where they ran out.
 int status_word(unsigned int** word);

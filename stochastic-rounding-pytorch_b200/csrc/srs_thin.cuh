@@ -29,7 +29,9 @@
 // 41 adapters, nearly all of it launch and dependent loads; in this one's epilogue as much.)
 // Ranks up to 16 take narrow boxes, three adapters a stage: with one a stage, of boxes of 128 bytes
 // that were mostly fill, 64 tokens of 40 adapters waited for four loads in flight (14336 x 4096:
-// 34 us a call in a graph, now 30.8; of one adapter 24.6, without any 17.6).
+// 34 us a call in a graph, 30.8 with three).  The product of the projection does not wait for the low
+// part, which the kernels ahead arrange: 29.7 us, and of one adapter 24.6 -> 22.1; without any 17.6.
+// What is left is mostly the items: 40 of 64 tokens a CTA's tile, of which one or two are not zero.
 #pragma once
 
 #include "srs_groups.cuh"
@@ -204,8 +206,9 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   bool ok = true;
   if (warp == 4) {
     const bool leader = elect_lane();
-    // B may come from the kernel this one overlaps.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // B may come from the kernel this one overlaps (of adapters: only from the one ahead of that,
+    // which was done before this kernel could start).
+    if constexpr (!ADAPTERS) asm volatile("griddepcontrol.wait;" ::: "memory");
     int s = 0;
     uint32_t phase = 0;
     for (int i = first; i < last; ++i) {
@@ -227,7 +230,8 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       }
     }
     if constexpr (ADAPTERS) {
-      asm volatile("bar.sync 1, 96;" ::: "memory");  // the list of adapters
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the low part
+      asm volatile("bar.sync 1, 96;" ::: "memory");       // the list of adapters
       const int slices = a.pack != 0 ? 0 : a.item_slices, chunks = (slices + 1) / 2;
       for (int e0 = (int)rank; a.pack != 0 && e0 < actives && ok; e0 += (int)splits * a.pack) {
         const uint32_t pa = stage0 + s * stage_bytes;
@@ -425,15 +429,13 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       const int slot = g % kThinSlots, kb = first + 4 * g;
       uint32_t w[2][4];
       from_a.read(kb, last, words_a, w[0]);
-      if (!waited) {
+      if (!waited && (!ADAPTERS || a.exponents != nullptr)) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         if constexpr (ADAPTERS) {
-          // (written ahead of this kernel, as B is)
-          if (a.exponents != nullptr) {
+          // (written ahead of this kernel, as the pairs are)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              more[j] = in_every_byte(__ldcg(a.exponents + min(lane + 32 * j, a.n - 1)));
-          }
+          for (int j = 0; j < 4; ++j)
+            more[j] = in_every_byte(__ldcg(a.exponents + min(lane + 32 * j, a.n - 1)));
         }
       }
       waited = true;
