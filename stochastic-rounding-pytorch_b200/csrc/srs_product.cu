@@ -402,20 +402,13 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
   ThinArgs args{};
   args.m = (int)n;
   args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
-  args.rows = 128;
-  // As for one weight: k split while few tiles are likely; with many, tiles of a size that fills
-  // whole rounds of two CTAs an SM.
-  const int64_t sms = sm_count();
-  int64_t tiles = (n + 127) / 128;
+  // k is split while few tiles are likely, as for one weight.  Tiles of a size that fills whole rounds of
+  // two CTAs an SM are no gain here (256 rows of 62 groups, 2048 -> 1024: 31.2 us, so 30.1; two
+  // rows, 4096 -> 14336: 25.3 and 24.7).
+  const int64_t sms = sm_count(), tiles = (n + 127) / 128;
+  args.rows = (int)((n + tiles - 1) / tiles);
   int splits = 1;
-  if (tiles * busy > sms) {
-    const int64_t rounds = (tiles * busy + 2 * sms - 1) / (2 * sms);
-    tiles = 2 * sms * rounds / busy > tiles ? 2 * sms * rounds / busy : tiles;
-    args.rows = (int)((n + tiles - 1) / tiles);
-    tiles = (n + args.rows - 1) / args.rows;
-  } else {
-    while (splits < 8 && tiles * busy * splits <= sms && args.slices >= 4 * splits) splits *= 2;
-  }
+  while (splits < 8 && tiles * busy * splits <= sms && args.slices >= 4 * splits) splits *= 2;
   const int64_t most = tiles * most_group_tiles(a.rows, experts, columns);
   if (most * splits >= (1ll << 31))
     return fail(SRS_ERR_INVALID_ARGUMENT, "a result of %lld x %lld is too large",
