@@ -503,7 +503,7 @@ int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapter
 typedef struct srs_adapter_sum {
   uint64_t z; /* tokens x cols, 16-byte aligned, row pitch z_pitch elements */
   int64_t z_pitch, cols;
-  uint64_t low, largest, out;
+  uint64_t low, largest, out; /* low: 16-byte aligned */
   int64_t turned;
 } srs_adapter_sum;
 int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int format, int64_t tokens,

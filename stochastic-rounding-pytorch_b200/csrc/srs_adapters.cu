@@ -877,6 +877,7 @@ int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, 
   if (tokens == 0) return SRS_OK;
   if (a->order == 0 || a->order % 4 != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned order");
+  if (a->scale % 4 != 0) return fail(SRS_ERR_INVALID_ARGUMENT, "misaligned scales");
   const int64_t in = turned ? n : k, out = turned ? k : n;  // of the adapters
   const auto bad = [](uint64_t at, int64_t pitch, int64_t stride, int64_t least) {
     return at == 0 || at % 16 != 0 || pitch % 8 != 0 || stride % 8 != 0 || pitch < least;
@@ -936,7 +937,8 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
   if (k > 0 && (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0 || x_pitch % 8 != 0 ||
                 x_pitch < k))
     return fail(SRS_ERR_INVALID_ARGUMENT, "x needs a 16-byte aligned address and row pitch");
-  if (n > 0 && reinterpret_cast<uintptr_t>(d) % 2 != 0)
+  if ((n > 0 && reinterpret_cast<uintptr_t>(d) % 2 != 0) ||
+      reinterpret_cast<uintptr_t>(low) % 4 != 0 || reinterpret_cast<uintptr_t>(largest) % 4 != 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "misaligned result pointer");
   const AdapterSpace space = adapter_space(tokens, k, n, a->count, a->rank);
   if (workspace_bytes < space.total ||
@@ -1071,9 +1073,13 @@ extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int
     if (s.cols == 0) continue;
     if (s.out == 0 || s.out % 2 != 0)
       return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned result pointer");
-    if (tokens > 0 && (s.z == 0 || s.low == 0 || order == nullptr || s.z_pitch < s.cols ||
-                       s.z_pitch % 8 != 0 || s.z % 16 != 0))
+    if (tokens > 0 && (s.z == 0 || s.z_pitch < s.cols || s.z_pitch % 8 != 0 || s.z % 16 != 0))
       return fail(SRS_ERR_INVALID_ARGUMENT, "z needs a 16-byte aligned address and row pitch");
+    if (tokens > 0 && (s.low == 0 || s.low % 16 != 0 || s.largest % 4 != 0))
+      return fail(SRS_ERR_INVALID_ARGUMENT,
+                  "low needs a 16-byte aligned address, the largest a multiple of 4");
+    if (tokens > 0 && (order == nullptr || reinterpret_cast<uintptr_t>(order) % 4 != 0))
+      return fail(SRS_ERR_INVALID_ARGUMENT, "null or misaligned order");
     SumJob& job = a.job[jobs++];
     job.z = reinterpret_cast<const char*>(s.z);
     job.z_pitch = s.z_pitch;

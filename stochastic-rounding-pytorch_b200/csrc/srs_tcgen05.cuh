@@ -283,7 +283,7 @@ __device__ __forceinline__ uint64_t operand_descriptor(bool rows_inner) {
   return (lead << 16) | (uint64_t(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // k contiguous in rows of 32 or 64 bytes, swizzled over as many.
-__device__ __forceinline__ uint64_t narrow_descriptor(int row_bytes) {
+__device__ __forceinline__ uint64_t short_row_descriptor(int row_bytes) {
   return (1ull << 16) | (uint64_t(row_bytes * 8) >> 4 << 32) | (1ull << 46) |
          ((row_bytes == 32 ? 6ull : 4ull) << 61);
 }

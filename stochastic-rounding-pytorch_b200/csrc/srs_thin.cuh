@@ -352,9 +352,9 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
         if (leader) {
           const int count = min(a.pack, (actives - e0 + (int)splits - 1) / (int)splits);
           for (int i = 0; i < count; ++i) {
-            const uint64_t du = narrow_descriptor(32) |
+            const uint64_t du = short_row_descriptor(32) |
                                 uint64_t(((pa + i * (panel_bytes / 4)) >> 4) & 0x3FFFu);
-            const uint64_t dh = narrow_descriptor(64) |
+            const uint64_t dh = short_row_descriptor(64) |
                                 uint64_t(((pa + a.pack_at + i * (BN * 64)) >> 4) & 0x3FFFu);
             mma_f16<1>(tmem, du, dh, idesc, 1u);
             mma_f16<1>(tmem, du, dh + 2, idesc, 1u);  // the pairs' second parts

@@ -179,6 +179,13 @@ def test_adapter_refusals():
     refused(gradient(z=A + 8), "16-byte")
     refused(gradient(z_pitch=64), "16-byte")
     refused(gradient(out=0), "result pointer")
+    refused(gradient(low=A + 8), "low needs a 16-byte")
+    refused(gradient(low=0), "low needs a 16-byte")
+    refused(gradient(largest=A + 2), "multiple of 4")
+    refused(linear(a=adapters(scale=A + 2)), "scales")
+    for low, largest in ((A + 2, None), (A, A + 1)):
+        refused(lib.srs_adapter_linear(A, 100, 128, 128, 3, 0, 0, blocks(), adapters(), 0, A, low,
+                                       largest, A, 1 << 30, None), "result pointer")
 
 
 def test_struct_layouts():
