@@ -4,8 +4,9 @@
 //
 // A and H have the tokens in their adapters' order, D in the batch's.  A tile runs its FP8 slices
 // and then, for every adapter with rows in it, one slice of 16-bit products for ranks up to 32
-// (two for every 64 above): H in items whose other rows are zero, as a pair of 16-bit numbers, so
-// that the sum stays FP32 all through and the result is rounded once.  At rank 16 that is 2 to 3
+// (two for every 64 above), H as a pair of 16-bit numbers, so that the sum stays FP32 all through
+// and the result is rounded once.  These MMAs write the adapter's own rows of the accumulator alone:
+// what other adapters' matrices hold, infinities and NaN too, never reaches a token.  At rank 16 that is 2 to 3
 // slices beside the 32 of k = 4096; adding the adapters' part in a pass of its own took as long
 // as the product (4096 tokens, 4096 -> 14336, rank 16: 147 us beside 178).  MMA-bound, then by
 // the power limit.
@@ -133,7 +134,8 @@ struct AdapterSource {
   __device__ ExtraLoad extra(uint32_t t, int i) const {
     int row, col;
     w.grid.at(t, &row, &col);
-    const int adapter = first_past(row * w.edge) + i / w.extra_slices, slice = i % w.extra_slices;
+    const int row0 = row * w.edge;
+    const int adapter = first_past(row0) + i / w.extra_slices, slice = i % w.extra_slices;
     ExtraLoad e;
     e.map_a = &w.map_h;
     e.map_b = &w.map_u;
@@ -145,6 +147,8 @@ struct AdapterSource {
     e.k_b = 64 * chunk;
     e.steps = (min(w.rank - 64 * chunk, 64) + 15) / 16;
     e.again = w.extra_slices == 1 ? w.rest_at / 16 : 0;
+    e.first = p.start[adapter] - row0;
+    e.end = p.start[adapter + 1] - row0;
     return e;
   }
 };

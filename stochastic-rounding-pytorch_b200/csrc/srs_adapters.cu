@@ -167,33 +167,19 @@ __device__ __forceinline__ void write_pair(const LowArgs& a, const GroupTile& ti
   to[a.rest_at] = (uint16_t)encode16<F>(isfinite(left) ? left : 0.0f);
 }
 
-// Zeros in the rows of the adapter's items that are not its own (`whole` of the rank from rank0 on),
-// by the threads from, from + step, .. of those that have its first and its last tile of `most`.
-__device__ __forceinline__ void clear_items(const LowArgs& a, const GroupTile& tile, int most,
-                                            int rank0, int whole, int from, int step) {
-  const int words = whole / 2;
-  const auto zero = [&](int64_t row, int word) {
-    uint16_t* const p = a.pairs + row * a.pitch + rank0 + 2 * word;
+// Zeros in the rows of a thin product's item that are not its adapter's (`whole` of the rank from
+// rank0 on), by the threads from, from + step, .. of those that have the adapter's first tile.
+__device__ __forceinline__ void clear_item(const LowArgs& a, const GroupTile& tile, int rank0,
+                                           int whole, int from, int step) {
+  if (tile.row0 != tile.start) return;
+  const int words = whole / 2, others = a.tokens - (tile.end - tile.start);
+  for (int i = from; i < others * words; i += step) {
+    const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
+    uint16_t* const p =
+        a.pairs + ((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens)) * a.pitch +
+        rank0 + 2 * (i % words);
     *reinterpret_cast<uint32_t*>(p) = 0u;
     *reinterpret_cast<uint32_t*>(p + a.rest_at) = 0u;
-  };
-  if (a.spread) {
-    if (tile.row0 == tile.start) {
-      const int others = a.tokens - (tile.end - tile.start);
-      for (int i = from; i < others * words; i += step) {
-        const int o = i / words, place = o < tile.start ? o : o + tile.end - tile.start;
-        zero((int64_t)tile.rank * a.edge + token_at(a.order, place, a.tokens), i % words);
-      }
-    }
-  } else {
-    // before its first row in its first item, behind its last in the last
-    if (tile.row0 == tile.start)
-      for (int i = from; i < tile.start % a.edge * words; i += step)
-        zero((int64_t)(tile.start / a.edge + tile.rank) * a.edge + i / words, i % words);
-    const int final_row = tile.end - 1, behind = final_row % a.edge + 1;
-    if (final_row - tile.row0 < most)
-      for (int i = from; i < (a.edge - behind) * words; i += step)
-        zero((int64_t)(final_row / a.edge + tile.rank) * a.edge + behind + i / words, i % words);
   }
 }
 
@@ -226,8 +212,8 @@ __device__ __forceinline__ void write_low(const LowArgs& a, const LowTile& l, fl
     }
     if (a.pairs != nullptr) write_pair<F>(a, tile, tile.row0 + t, l.rank0 + r, v);
   }
-  if (a.pairs != nullptr)
-    clear_items(a, tile, most, l.rank0, whole, (int)threadIdx.x + threads * split, threads * splits);
+  if (a.pairs != nullptr && a.spread)
+    clear_item(a, tile, l.rank0, whole, (int)threadIdx.x + threads * split, threads * splits);
   if (a.largest != nullptr) {
     const unsigned int top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_size));
     // (the order is no matter)
@@ -278,7 +264,7 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(const LowArgs a) {
       write_pair<SRS_FMT_F16>(a, tile, place, r, r < a.rank ? __ldcg(from + r) * factor : 0.0f);
     if (lane == 0) *exponent_of(place) = k;
   }
-  clear_items(a, tile, kPairTokens, 0, whole, (int)threadIdx.x, kPairThreads);
+  if (a.spread) clear_item(a, tile, 0, whole, (int)threadIdx.x, kPairThreads);
 }
 
 // Calls of few tokens, where most adapters have one or two: 16 tokens, and 4 warps that share a

@@ -97,11 +97,12 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
 // Low-rank adapters in a large product (srs_adapter_product.cu).  The low part of tokens in their
 // adapters' order enters as pairs of 16-bit numbers, high and what it leaves, in items of
 // `edge` rows: an item is a tile of the product and one adapter that has tokens in it, other rows
-// zero.  Item of tile i and the r-th adapter with tokens: i + r (each step along the tokens
+// not written.  Item of tile i and the r-th adapter with tokens: i + r (each step along the tokens
 // raises one of the two, so no two items share a number).  A row has the rank's high parts, in
 // whole 16s, and the others behind them in one slice of 64 for ranks up to 32; else whole
 // slices of 64 of high parts and then as many of the others.  A thin product's items have one row
-// a token in the batch's order, one item an adapter with tokens, and thin_columns rows.
+// a token in the batch's order (zero but for the adapter's own), one item an adapter with tokens,
+// and thin_columns rows.
 struct PairShape {
   int pitch, rest_at;  // elements of a row, first of the second parts
   int slices;

@@ -189,6 +189,28 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   }
 }
 
+// The same for some rows of D: bit i % 32 of off[i / 32] leaves row i (of 128 CG) as it is, whatever
+// A and B hold.
+__device__ __forceinline__ void mma_f16_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate, const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(off[0]), "r"(off[1]), "r"(off[2]),
+      "r"(off[3])
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate, const uint32_t (&off)[8]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, "
+      "{%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(off[0]), "r"(off[1]), "r"(off[2]),
+      "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
+      : "memory");
+}
+
 template <int CG>
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
