@@ -26,11 +26,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-__device__ __forceinline__ int64_t token_at(const int32_t* order, int place, int tokens) {
-  const int t = __ldg(order + place);
-  return t >= 0 && t < tokens ? t : 0;  // an entry that names no token reads the first
-}
-
 // 16 bytes to shared memory, those behind the first `bytes` zero.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)

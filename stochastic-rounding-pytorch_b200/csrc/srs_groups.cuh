@@ -15,6 +15,11 @@ namespace srs {
 
 constexpr int kMaxGroups = 1024;
 
+__device__ __forceinline__ int64_t token_at(const int32_t* order, int place, int tokens) {
+  const int t = __ldg(order + place);
+  return t >= 0 && t < tokens ? t : 0;  // an entry that names no token reads the first
+}
+
 __device__ __forceinline__ int warp_scan_sum(int v, int lane) {
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {

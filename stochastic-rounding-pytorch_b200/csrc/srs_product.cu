@@ -382,6 +382,12 @@ int launch_thin(const srs_blocks& a, const srs_blocks& b, int64_t k, void* d, in
     args.rest_at = pairs.rest_at;
     args.exponents = adapters->exponents;
     args.up_rows_inner = adapters->rows_inner;
+    args.pairs = static_cast<const uint16_t*>(adapters->pairs);
+    args.pair_pitch = pairs.pitch;
+    args.up = static_cast<const uint16_t*>(adapters->up);
+    args.up_pitch = adapters->pitch;
+    args.up_stride = adapters->stride;
+    args.order = adapters->order;
     args.extra_idesc = (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24 | 1u << 4 |
                        (d_format == SRS_FMT_BF16 ? 1u << 7 | 1u << 10 : 0u);
     if (columns == 16) return launch_thin_as<16, kThinAdapters>(args, grid, splits, overlap, stream);

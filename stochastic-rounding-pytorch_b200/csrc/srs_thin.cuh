@@ -23,8 +23,13 @@
 // zeros for the rows of no group, as the others do behind their tile, and leave.
 //
 // ADAPTERS: B's rows are tokens, and token t of adapter a gets U_a low_t more, as MMAs of 16-bit
-// operands on the same sums (see the large product with adapters): an item of low parts, zero but
-// for its adapter's tokens, by the adapter's U; the CTAs of a cluster take the adapters in turn.
+// operands (see the large product with adapters): an item of low parts, zero but for its adapter's
+// tokens, by the adapter's U; the CTAs of a cluster take the adapters in turn.  Their sums are apart
+// from the projection's, as zero times an infinity is NaN and an item's zeros are in other tokens'
+// columns, which an MMA cannot leave out: a row where an adapter's U is not finite has such sums in
+// every column.  The epilogue computes the adapters' part of a sum that is not finite again, of the
+// token's own adapter alone.  (For 64 tokens of 40 adapters, 14336 x 4096: 29.3 us a call; with all
+// sums in one accumulator 28.8; with a look at U in shared memory ahead of its MMAs 31.5.)
 // (In a kernel of its own behind this one that part took 5 us for one token and 10 for 64 with
 // 41 adapters, nearly all of it launch and dependent loads; in this one's epilogue as much.)
 // Ranks up to 16 take narrow boxes, three adapters a stage: with one a stage, of boxes of 128 bytes
@@ -82,19 +87,28 @@ struct ThinArgs {
   int pack, pack_at;
   const int32_t* exponents;  // of FP16 pairs, one a token (null: BF16)
   uint32_t extra_idesc;
+  // for own_part: low parts and U as the maps have them, and the tokens' order
+  const uint16_t* pairs;
+  const uint16_t* up;
+  int64_t up_pitch, up_stride;  // elements
+  int pair_pitch;
+  const int32_t* order;
 };
 
 template <int BN>
 struct ThinShape {
   static constexpr int kColumns = BN <= 16 ? 32 : BN <= 32 ? 64 : 128;  // TMEM
   static constexpr int kScaleColumn = BN;  // two groups of 8 columns (A, B)
+  // ADAPTERS: their sums behind the scales (two CTAs an SM still fit its 512 columns)
+  static constexpr int kAdapterColumn = BN + 16;
+  static constexpr int kAllColumns = BN <= 16 ? 64 : BN <= 32 ? 128 : 256;
   static constexpr int kScaleBytes = 1024;
   static constexpr int kFixed = 1024 + kThinSlots * kScaleBytes;  // alignment, scales
   // Two CTAs fit an SM.  The MMA reads 128 rows of A whatever the tile has: behind the
   // last stage's panel a whole one stays inside the CTA's memory.
   static constexpr int kBudget = 110 * 1024 - kFixed;
   static constexpr int kSums = 128 * BN * 4;  // split sums, in the stages' place
-  static_assert(BN + 16 <= kColumns, "accumulator and scales fit");
+  static_assert(BN + 16 <= kColumns && 2 * BN + 16 <= kAllColumns, "accumulators and scales fit");
   static_assert(kSums <= kBudget, "split sums fit the stages");
 };
 
@@ -120,13 +134,47 @@ __device__ __forceinline__ void zero_ungrouped(const ThinArgs& a) {
     store_value(a.out, a.out_format, i, 0.0f);
 }
 
+// ADAPTERS: those with tokens, in order; active[e] has the places first[e] .. first[e + 1] - 1.
+struct ThinAdapters {
+  int active[kThinRows], actives;
+  int first[kThinRows + 1];
+};
+
+// Row `row` of U low for one token (its pairs are held times a power of two), if its adapter is one
+// of every `step`-th from e on; else 0.
+template <int BN>
+__device__ __noinline__ float own_part(const ThinArgs& a, const ThinAdapters& given, int e, int step,
+                                       int token, int row) {
+  for (; e < given.actives; e += step) {
+    int p = given.first[e];
+    while (p < given.first[e + 1] && token_at(a.order, p, a.n) != token) ++p;
+    if (p < given.first[e + 1]) break;
+  }
+  if (e >= given.actives) return 0.0f;
+  const uint16_t* const low = a.pairs + ((int64_t)e * BN + token) * a.pair_pitch;
+  const uint16_t* const up = a.up + given.active[e] * a.up_stride +
+                             (a.up_rows_inner ? row : row * a.up_pitch);
+  const int64_t up_step = a.up_rows_inner ? a.up_pitch : 1;
+  const auto decode = [&](uint16_t v) {
+    return a.out_format == SRS_FMT_BF16 ? __uint_as_float((uint32_t)v << 16)
+                                        : __half2float(__ushort_as_half(v));
+  };
+  float sum = 0.0f;
+  for (int r = 0; r < a.rank; ++r) {
+    const float h = decode(__ldcg(low + r)) + decode(__ldcg(low + a.rest_at + r));
+    sum = fmaf(h, decode(__ldg(up + r * up_step)), sum);
+  }
+  return sum;
+}
+
 template <int BN, int FORM>
 __global__ void __launch_bounds__(kThinThreads, 2)
 thin_product_kernel(const __grid_constant__ ThinArgs a) {
   constexpr bool GROUPED = FORM == kThinGrouped;
   constexpr bool ADAPTERS = FORM == kThinAdapters;
   using S = ThinShape<BN>;
-  __shared__ int active[kThinRows], actives;  // ADAPTERS: those with tokens, in order
+  constexpr uint32_t kColumns = ADAPTERS ? S::kAllColumns : S::kColumns;
+  __shared__ ThinAdapters given;
   // A kernel launched to overlap this one may start (and wait for it).
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t raw[];
@@ -198,7 +246,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     }
     __syncwarp();
   }
-  if (warp == 5) tmem_alloc<1>(smem_address(&tmem_slot), S::kColumns);
+  if (warp == 5) tmem_alloc<1>(smem_address(&tmem_slot), kColumns);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -233,6 +281,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the low part
       asm volatile("bar.sync 1, 96;" ::: "memory");       // the list of adapters
       const int slices = a.pack != 0 ? 0 : a.item_slices, chunks = (slices + 1) / 2;
+      const int actives = given.actives;
       for (int e0 = (int)rank; a.pack != 0 && e0 < actives && ok; e0 += (int)splits * a.pack) {
         const uint32_t pa = stage0 + s * stage_bytes;
         ok = barrier_wait(empty(s), phase ^ 1u, a.status, 1u << 8);
@@ -242,7 +291,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           barrier_expect(full(s), (uint32_t)(count * (a.rows * 32 + BN * 64)));
           for (int i = 0; i < count; ++i) {
             const int e = e0 + i * (int)splits;
-            load_box<1>(pa + i * (panel_bytes / 4), &a.map_u, 0, row0, active[e], full(s));
+            load_box<1>(pa + i * (panel_bytes / 4), &a.map_u, 0, row0, given.active[e], full(s));
             load_box<1>(pa + a.pack_at + i * (BN * 64), &a.map_h, 0, e * BN, 0, full(s));
           }
         }
@@ -261,10 +310,10 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
             const int k = 64 * (q < chunks ? q : q - chunks);
             barrier_expect(full(s), load_bytes);
             if (a.up_rows_inner) {
-              load_box<1>(pa, &a.map_u, row0, k, active[e], full(s));
-              load_box<1>(pa + kPanelBytes / 2, &a.map_u, row0 + 64, k, active[e], full(s));
+              load_box<1>(pa, &a.map_u, row0, k, given.active[e], full(s));
+              load_box<1>(pa + kPanelBytes / 2, &a.map_u, row0 + 64, k, given.active[e], full(s));
             } else {
-              load_box<1>(pa, &a.map_u, k, row0, active[e], full(s));
+              load_box<1>(pa, &a.map_u, k, row0, given.active[e], full(s));
             }
             load_box<1>(pa + panel_bytes, &a.map_h, 64 * q, e * BN, 0, full(s));
           }
@@ -336,10 +385,9 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
     if constexpr (ADAPTERS) {
       asm volatile("bar.sync 1, 96;" ::: "memory");
       const int slices = a.pack != 0 ? 0 : a.item_slices, chunks = (slices + 1) / 2;
-      // Behind the MMAs of the other kind: nothing says that the two keep their order.
-      if (ok && (int)rank < actives)
-        ok = barrier_wait(empty(s == 0 ? stages - 1 : s - 1), s == 0 ? phase ^ 1u : phase, a.status,
-                          1u << 9);
+      const int actives = given.actives;
+      const uint32_t sums = tmem + S::kAdapterColumn;
+      uint32_t more = 0u;  // 0: the first MMA writes the sums
       const bool inner = a.up_rows_inner;
       const uint64_t desc_u = operand_descriptor(inner);
       const uint32_t step_u = (inner ? 2048u : 32u) >> 4;
@@ -356,12 +404,13 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
                                 uint64_t(((pa + i * (panel_bytes / 4)) >> 4) & 0x3FFFu);
             const uint64_t dh = short_row_descriptor(64) |
                                 uint64_t(((pa + a.pack_at + i * (BN * 64)) >> 4) & 0x3FFFu);
-            mma_f16<1>(tmem, du, dh, idesc, 1u);
-            mma_f16<1>(tmem, du, dh + 2, idesc, 1u);  // the pairs' second parts
+            mma_f16<1>(sums, du, dh, idesc, more | (uint32_t)i);
+            mma_f16<1>(sums, du, dh + 2, idesc, 1u);  // the pairs' second parts
           }
           mma_commit<1>(empty(s));
         }
         __syncwarp();
+        more = 1u;
         if (++s == stages) {
           s = 0;
           phase ^= 1u;
@@ -379,14 +428,15 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           const int steps = (min(a.rank - 64 * chunk, 64) + 15) / 16;
           if (leader) {
             for (int j = 0; j < steps; ++j)
-              mma_f16<1>(tmem, du + j * step_u, dh + 2 * j, idesc, 1u);
+              mma_f16<1>(sums, du + j * step_u, dh + 2 * j, idesc, more | (uint32_t)j);
             if (slices == 1) {
               for (int j = 0; j < steps; ++j)
-                mma_f16<1>(tmem, du + j * step_u, dh + 2 * (a.rest_at / 16 + j), idesc, 1u);
+                mma_f16<1>(sums, du + j * step_u, dh + 2 * (a.rest_at / 16 + j), idesc, 1u);
             }
             mma_commit<1>(empty(s));
           }
           __syncwarp();
+          more = 1u;
           if (++s == stages) {
             s = 0;
             phase ^= 1u;
@@ -414,10 +464,17 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
           int start, end;
           group_span(a.ends, ahead, a.groups, a.n, base, lane, &carry, &start, &end);
           const unsigned some = __ballot_sync(0xFFFFFFFFu, end > start);
-          if (end > start) active[count + __popc(some & ((1u << lane) - 1u))] = base + lane;
+          if (end > start) {
+            const int e = count + __popc(some & ((1u << lane) - 1u));
+            given.active[e] = base + lane;
+            given.first[e] = start;
+          }
           count += __popc(some);
         }
-        if (lane == 0) actives = count;
+        if (lane == 0) {
+          given.actives = count;
+          given.first[count] = carry;
+        }
         __syncwarp();
         asm volatile("bar.arrive 1, 96;" ::: "memory");
       }
@@ -480,7 +537,44 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_after();
   const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
   const int row = row0 + 32 * warp + lane, row_end = min(a.m, row0 + a.rows);
-  if constexpr (ADAPTERS) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (ADAPTERS) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __syncthreads();  // (the list of adapters)
+  }
+  // 16 columns of this thread's row; which of them still want their adapters' part (own_part).
+  const auto sums_of = [&](int c0, uint32_t (&v)[16]) {
+    unsigned odd = 0u;
+    tmem_load16(acc + c0, v);
+    if constexpr (ADAPTERS) {
+      if ((int)rank < given.actives) {
+        uint32_t u[16];
+        tmem_load16(acc + S::kAdapterColumn + c0, u);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const bool finite = (u[c] & 0x7F800000u) != 0x7F800000u;
+          if (finite) v[c] = __float_as_uint(__uint_as_float(v[c]) + __uint_as_float(u[c]));
+          else if (row < row_end && c0 + c < n) odd |= 1u << c;
+        }
+      }
+    }
+    return odd;
+  };
+  // Column c of this thread's row among sums in shared memory (512 bytes a column, one word a row).
+  const auto word_of = [&](int c) { return stage0 + 512 * c + 128 * warp + 4 * lane; };
+  const auto stage_sums = [&](int c0, const uint32_t (&v)[16], unsigned odd) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(word_of(c0 + c)), "r"(v[c]) : "memory");
+    if constexpr (ADAPTERS) {
+      for (; odd != 0u; odd &= odd - 1u) {
+        const int c = c0 + __ffs(odd) - 1;
+        const float part = own_part<BN>(a, given, (int)rank, (int)splits, c, row);
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(word_of(c)),
+                     "f"(__uint_as_float(staged_read(word_of(c))) + part)
+                     : "memory");
+      }
+    }
+  };
   // A sum of column c without the power of two of its FP16 pairs.
   const auto result = [&](float sum, int c) {
     if constexpr (ADAPTERS) {
@@ -494,29 +588,26 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       for (int c0 = 0; c0 < BN; c0 += 16) {
         if (c0 >= n) break;
         uint32_t v[16];
-        tmem_load16(acc + c0, v);
+        const unsigned odd = sums_of(c0, v);
+        if (ADAPTERS && odd != 0u) stage_sums(c0, v, odd);
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          if (row < row_end && c0 + c < n)
+          if (row < row_end && c0 + c < n) {
+            if (ADAPTERS && odd != 0u) v[c] = staged_read(word_of(c0 + c));
             store_value(a.out, a.out_format,
                         row * a.row_stride + (b_row0 + c0 + c) * a.col_stride,
                         result(__uint_as_float(v[c]), c0 + c));
+          }
       }
     }
   } else {
-    // column c of this CTA's sum at 512 * c bytes, one word a row
     if (warp < 4) {
 #pragma unroll
       for (int c0 = 0; c0 < BN; c0 += 16) {
         if (c0 >= n) break;
         uint32_t v[16];
-        tmem_load16(acc + c0, v);
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(stage0 + 512 * (c0 + c) + 128 * warp +
-                                                       4 * lane),
-                       "r"(v[c])
-                       : "memory");
+        const unsigned odd = sums_of(c0, v);
+        stage_sums(c0, v, odd);
       }
     }
     cluster_sync();
@@ -561,7 +652,7 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  if (warp == 5) tmem_free<1>(tmem, S::kColumns);
+  if (warp == 5) tmem_free<1>(tmem, kColumns);
   if constexpr (GROUPED) zero_ungrouped(a);
 }
 

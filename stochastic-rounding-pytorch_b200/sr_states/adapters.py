@@ -22,7 +22,8 @@ def adapter_linear(x, weight, down, up, groups, *, scale=1.0, dtype=torch.float8
     ``x``: (..., K) in BF16 or FP16; ``down``: (adapters, rank, K) and ``up``: (adapters, N,
     rank) in x's dtype, rank at most 256; ``groups``: the tokens (x's rows taken flat) by adapter, from
     ``group_rows(index, adapters)``: made once a batch, for all its layers.  Tokens of no group
-    have the projection alone.  ``scale``: a number, or FP32, one an adapter (no gradient).
+    have the projection alone.  Infinities and NaN in an adapter's matrices reach its own tokens
+    alone (as either).  ``scale``: a number, or FP32, one an adapter (no gradient).
 
     ``weight``: a BlockTensor (inference), a pair of BlockTensors
     ``quantize_blocks(w, block=(128, 128), orientation="both")`` (a frozen projection:

@@ -88,3 +88,49 @@ def test_all_matrices_but_one(tokens, dtype, cuda_device):
         assert not got[i][~kept].isfinite().any()
     for i in (2, 3):
         assert torch.equal(got[i][1], clean[i][1])
+
+
+@FORMATS
+@pytest.mark.parametrize("rank", [8, 20, 64, 130])
+@pytest.mark.parametrize("tokens", [1, 5, 30, 64])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_few_tokens_and_matrices_that_are_not_finite(tokens, rank, bad, dtype, cuda_device):
+    case = make(tokens, 4, rank, 1333, 410, dtype, cuda_device)
+    for row, r, col in ((0, 0, 1332), (409, rank - 1, 130)):
+        check_apart(case, bad, (row, r), (r, col))
+
+
+@FORMATS
+@pytest.mark.parametrize("tokens", [3, 30, 64])
+def test_few_tokens_and_all_matrices_but_one(tokens, dtype, cuda_device):
+    test_all_matrices_but_one(tokens, dtype, cuda_device)
+
+
+@FORMATS
+@pytest.mark.parametrize("rank", [12, 40])
+@pytest.mark.parametrize("k,n", [(130, 19001), (19001, 130)])
+def test_wide_products_and_matrices_that_are_not_finite(k, n, rank, dtype, cuda_device):
+    """More tiles than SMs: a CTA has all of k, and stores what it has added by itself."""
+    case = make(40, 6, rank, k, n, dtype, cuda_device)
+    check_apart(case, float("nan"), (n - 1, rank - 1), (rank - 1, k - 1))
+
+
+@FORMATS
+def test_a_chunk_apart_is_the_chunk(dtype, cuda_device):
+    """An infinity that the low part multiplies by zero's neighbours alone: with tokens whose low
+    part there is zero, nothing else of adapter 1's part is lost.  (Zero times it is NaN, in its
+    column.)  The other columns of its tokens are the sum of both parts."""
+    case = make(20, 3, 130, 256, 300, dtype, cuda_device)
+    case["up"][1, 7, 100] = float("inf")
+    h = case["scale"][1].double() * (case["x"].double() @ case["down"][1].double().mT)
+    with torch.no_grad():
+        y = adapter_linear(case["x"], case["w"], case["down"], case["up"], case["groups"],
+                           scale=case["scale"]).double()
+        none = adapter_linear(case["x"], case["w"], case["down"], torch.zeros_like(case["up"]), case["groups"]).double()
+    own = case["index"] == 1
+    part = h[own] @ case["up"][1].double().mT
+    columns = [c for c in range(300) if c != 7]
+    exact = (none[own] + part)[:, columns]
+    limit = 2 * torch.finfo(dtype).eps * (exact.abs() + none[own][:, columns].abs()) + 1e-4
+    assert ((y[own][:, columns] - exact).abs() <= limit).all()
+    assert torch.equal(y[own][:, 7], torch.sign(h[own][:, 100]) * float("inf"))
