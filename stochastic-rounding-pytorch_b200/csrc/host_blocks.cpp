@@ -104,6 +104,7 @@ PyObject* py_linear(PyObject*, PyObject* args) {
   c10::NoGradGuard no_grad;
   const at::Tensor& t = tensor(x, "x");
   const at::Tensor& weight = tensor(w, "the weight's data");
+  refuse_tangents("block_linear", {&t});
   const c10::cuda::OptionalCUDAGuard guard(t.device());
   const int x_format = source_format(t, "block_linear");
   TORCH_CHECK_VALUE(t.device() == weight.device(), "all tensors must be on the same CUDA device");

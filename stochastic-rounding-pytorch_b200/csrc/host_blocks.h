@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -104,6 +105,14 @@ int operand(const char* name, Blocks* b, srs_blocks* out) {
 const at::Tensor& tensor(PyObject* obj, const char* what) {
   TORCH_CHECK_TYPE(THPVariable_Check(obj), what, " must be a tensor");
   return THPVariable_Unpack(obj);
+}
+
+// Nothing here has a rule for forward-mode differentiation: a tangent would be lost without a word.
+void refuse_tangents(const char* what, std::initializer_list<const at::Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
+                                " has no forward-mode derivative");
 }
 
 PyObject* pack(const Blocks& straight, const Blocks& turned, int orientation) {

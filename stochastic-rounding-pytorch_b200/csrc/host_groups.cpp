@@ -664,6 +664,7 @@ PyObject* py_expert_linear(PyObject*, PyObject* args) {
     return nullptr;
   const at::Tensor &x = tensor(x_obj, "x"), &weight = tensor(w_obj, "weight");
   const bool kept = w_scale != Py_None;
+  refuse_tangents("expert_linear", {&x, &weight});
   TORCH_CHECK_VALUE(x.dim() == 2 && weight.dim() == 3 && x.size(1) == weight.size(2),
                     "x of shape ", x.sizes(), " does not fit expert weights of shape ",
                     weight.sizes());
@@ -726,6 +727,7 @@ PyObject* py_adapter_linear(PyObject*, PyObject* args) {
   Blocks kept{optional(kept_obj, "the weight's data"), optional(kept_scale, "the weight's scale")};
   const Blocks turned{optional(turned_obj, "the transpose's data"),
                       optional(turned_scale, "the transpose's scale")};
+  refuse_tangents("adapter_linear", {&x, &weight, &down, &up, &scale});
   const at::Tensor& matrix = weight.defined() ? weight : kept.data;
   TORCH_CHECK_VALUE(x.dim() > 0, "adapter_linear needs at least one dimension");
   TORCH_CHECK_VALUE(matrix.dim() == 2 && x.size(-1) == matrix.size(1), "x of shape ", x.sizes(),
