@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from sr_states import adapter_linear, expert_linear, group_rows, quantize_blocks
+from sr_states import adapter_linear, block_linear, expert_linear, group_rows, quantize_blocks
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,10 @@ def test_experts(cuda_device):
     w = values((2, 48, 64), 2, cuda_device).requires_grad_()
     ends = torch.tensor([2, 5], device=cuda_device)
     check(lambda: expert_linear(x, w, ends, seed=3), x, (x, w))
+
+
+@SHAPES
+def test_one_weight(shape, cuda_device):
+    x = values(shape, 1, cuda_device).requires_grad_()
+    w = values((48, 64), 2, cuda_device).requires_grad_()
+    check(lambda: block_linear(x, w, seed=3), x, (x, w))
