@@ -542,7 +542,7 @@ struct SumJob {
   const unsigned int* largest;
   int cols, turned;  // turned: out is cols x rank instead of rank x cols
   void* out;
-  float* parts;  // [chunk][rank][cols]
+  float* parts;  // [part][rank][cols]: the chunks of the adapters that have several, in order
   int blocks;    // of the grid's width (of sums; of joins)
 };
 
@@ -555,6 +555,29 @@ struct SumArgs {
   const int32_t* ends;
   unsigned int* status;
 };
+
+// An adapter's chunks, and the parts ahead of its own; by a warp.
+struct SumParts {
+  int first, chunks;
+};
+
+__device__ __forceinline__ SumParts parts_of(const SumArgs& a, int group, int lane) {
+  const EndsAhead ahead(a.ends, a.adapters, lane);
+  SumParts p{0, 0};
+  int carry = 0, before = 0;
+  for (int base = 0; base <= group; base += 32) {
+    int start, end;
+    group_span(a.ends, ahead, a.adapters, a.tokens, base, lane, &carry, &start, &end);
+    const int n = (end - start + a.chunk - 1) / a.chunk, parts = n > 1 ? n : 0;
+    const int upto = before + warp_scan_sum(parts, lane);
+    if (group - base < 32) {
+      p.first = __shfl_sync(0xFFFFFFFFu, upto - parts, group - base);
+      p.chunks = __shfl_sync(0xFFFFFFFFu, n, group - base);
+    }
+    before = __shfl_sync(0xFFFFFFFFu, upto, 31);
+  }
+  return p;
+}
 
 __device__ __forceinline__ float pair_scale(const unsigned int* largest, int group) {
   if (largest == nullptr) return 1.0f;
@@ -666,6 +689,8 @@ sum_kernel(const __grid_constant__ SumArgs a) {
     copies_done();
   }
   fetch(0);
+  const bool alone = tile.end - tile.start <= a.chunk;
+  const int part = alone ? 0 : parts_of(a, tile.group, lane).first + (tile.row0 - tile.start) / a.chunk;
   bool ok = true;
   for (int i = 0; i < steps; ++i) {
     const int s = i % kSumStages;
@@ -705,7 +730,6 @@ sum_kernel(const __grid_constant__ SumArgs a) {
   if (warp < 4) {
     const float back = 1.0f / scale;  // a power of two: exact
     const int c = col0 + 32 * warp + lane;
-    const bool alone = tile.end - tile.start <= a.chunk;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       uint32_t v[16];
@@ -716,7 +740,7 @@ sum_kernel(const __grid_constant__ SumArgs a) {
         if (c >= job.cols || r >= ranks) continue;
         const float value = __uint_as_float(v[i]) * back;
         if (!alone)
-          job.parts[((int64_t)blockIdx.y * a.rank + rank0 + r) * job.cols + c] = value;
+          job.parts[((int64_t)part * a.rank + rank0 + r) * job.cols + c] = value;
         else
           static_cast<uint16_t*>(job.out)[(int64_t)tile.group * a.rank * job.cols +
                                           (job.turned ? (int64_t)c * a.rank + rank0 + r
@@ -735,20 +759,8 @@ sum_kernel(const __grid_constant__ SumArgs a) {
 template <int F>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumArgs a) {
   const int lane = threadIdx.x & 31, group = (int)blockIdx.y;
-  const EndsAhead ahead(a.ends, a.adapters, lane);
-  int carry = 0, chunks_before = 0, first = 0, chunks = 0;
-  for (int base = 0; base <= group; base += 32) {
-    int start, end;
-    group_span(a.ends, ahead, a.adapters, a.tokens, base, lane, &carry, &start, &end);
-    const int n = (end - start + a.chunk - 1) / a.chunk;
-    const int upto = chunks_before + warp_scan_sum(n, lane);
-    if (group - base < 32) {
-      first = __shfl_sync(0xFFFFFFFFu, upto - n, group - base);
-      chunks = __shfl_sync(0xFFFFFFFFu, n, group - base);
-    }
-    chunks_before = __shfl_sync(0xFFFFFFFFu, upto, 31);
-  }
-  if (chunks == 1) return;
+  const SumParts own = parts_of(a, group, lane);
+  if (own.chunks == 1) return;
   const bool second = (int)blockIdx.x >= a.job[0].blocks;
   const SumJob& job = a.job[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? a.job[0].blocks : 0);
@@ -757,7 +769,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumAr
     // i runs over the result's order
     const int64_t at = job.turned ? i % a.rank * job.cols + i / a.rank : i;
     float v = 0.0f;
-    for (int c = 0; c < chunks; ++c) v += job.parts[(first + c) * each + at];
+    for (int c = 0; c < own.chunks; ++c) v += job.parts[(own.first + c) * each + at];
     static_cast<uint16_t*>(job.out)[group * each + i] = (uint16_t)encode16<F>(v);
   }
 }
@@ -1025,10 +1037,17 @@ static int sum_chunk(int64_t tokens, int64_t cols, int rank) {
   return (int)(chunk > kSumChunk ? kSumChunk : chunk);
 }
 
+// Most chunks of the adapters that have more than one: two of every chunk + 1 tokens, as many such
+// adapters as there can be, and one more of a chunk that is left.
+static int64_t sum_parts(int64_t tokens, int64_t chunk) {
+  const int64_t adapters = tokens / (chunk + 1);
+  return adapters == 0 ? 0 : 2 * adapters + (tokens - adapters * (chunk + 1)) / chunk;
+}
+
 extern "C" int64_t srs_adapter_gradient_workspace(int64_t tokens, int64_t cols, int adapters,
                                                   int rank) {
   if (tokens <= 0 || cols <= 0 || adapters < 1 || rank < 1) return 0;
-  return most_group_tiles(tokens, adapters, sum_chunk(tokens, cols, rank)) * rank * cols * 4;
+  return sum_parts(tokens, sum_chunk(tokens, cols, rank)) * rank * cols * 4;
 }
 
 extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int format,
@@ -1085,8 +1104,8 @@ extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int
     return SRS_OK;
   }
   const int64_t least = srs_adapter_gradient_workspace(tokens, cols, adapters, rank);
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-      workspace_bytes < least)
+  if (workspace_bytes < least ||
+      (least > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
     return fail(SRS_ERR_INVALID_ARGUMENT, "workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)least);
   a.tokens = (int)tokens;
@@ -1096,9 +1115,8 @@ extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int
   a.ends = ends;
   a.chunk = sum_chunk(tokens, cols, rank);
   if (int rc = status_word(&a.status)) return rc;
-  const int64_t chunks = most_group_tiles(tokens, adapters, a.chunk);
   a.job[0].parts = static_cast<float*>(workspace);
-  a.job[1].parts = a.job[0].parts + chunks * rank * a.job[0].cols;
+  a.job[1].parts = a.job[0].parts + sum_parts(tokens, a.chunk) * rank * a.job[0].cols;
   if (int rc = format == SRS_FMT_BF16 ? launch_sum<SRS_FMT_BF16>(a, st)
                                       : launch_sum<SRS_FMT_F16>(a, st))
     return rc;
