@@ -864,7 +864,8 @@ int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, 
   if (a->rank < 1 || a->rank > SRS_ADAPTER_MAX_RANK)
     return fail(SRS_ERR_INVALID_ARGUMENT, "the rank must be in [1, %d], got %d",
                 SRS_ADAPTER_MAX_RANK, a->rank);
-  if (tokens < 0 || tokens > (1ll << 22) || k < 0 || n < 0 || k > (1ll << 30) || n > (1ll << 30))
+  if (tokens < 0 || tokens > kMaxQuantizedRows || k < 0 || n < 0 || k > (1ll << 30) ||
+      n > (1ll << 30))
     return fail(SRS_ERR_INVALID_ARGUMENT, "sizes out of range (%lld tokens, %lld -> %lld)",
                 (long long)tokens, (long long)k, (long long)n);
   if (tokens == 0) return SRS_OK;
@@ -1060,7 +1061,7 @@ extern "C" int srs_adapter_gradient(const srs_adapter_sum* sums, int n_sums, int
     return fail(SRS_ERR_INVALID_ARGUMENT, "one or two sums a call, got %d", n_sums);
   if (format != SRS_FMT_BF16 && format != SRS_FMT_F16)
     return fail(SRS_ERR_INVALID_ARGUMENT, "adapters are BF16 or FP16, got format %d", format);
-  if (rank < 1 || rank > SRS_ADAPTER_MAX_RANK || tokens < 0 || tokens > (1ll << 22))
+  if (rank < 1 || rank > SRS_ADAPTER_MAX_RANK || tokens < 0 || tokens > kMaxQuantizedRows)
     return fail(SRS_ERR_INVALID_ARGUMENT, "sizes out of range (%lld tokens, rank %d)",
                 (long long)tokens, rank);
   SumArgs a{};

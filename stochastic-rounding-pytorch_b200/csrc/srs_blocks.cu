@@ -198,6 +198,7 @@ __device__ __forceinline__ void store_bytes(uint8_t* out, uint2 w, int left) {
 // 4096: 20.5 us a call among others; 3 bytes an element at 6.5 TB/s would be 15), by the
 // integer units for the stochastic rule's hashes (37 us).
 constexpr int kAhead = 4;
+static_assert(kMaxQuantizedRows <= 65535ll * 16 * kAhead, "the rows fit a grid's height");
 
 __device__ __forceinline__ int64_t ordered_row(const QuantizeArgs& a, int64_t row) {
   const int64_t from = __ldg(a.order + row);
@@ -648,7 +649,7 @@ int srs::quantize(const QuantizeCall& q, cudaStream_t stream) {
   if (!valid_rule(q.rule)) return fail(SRS_ERR_INVALID_ARGUMENT, "unknown rounding rule %d", q.rule);
   if (q.rows < 0 || q.cols < 0 || q.x_pitch < 0 || q.matrices < 0)
     return fail(SRS_ERR_INVALID_ARGUMENT, "negative size or pitch");
-  if (q.rows > 65535ll * 16 * kAhead || q.cols > (1ll << 30) || q.matrices > 65535)
+  if (q.rows > kMaxQuantizedRows || q.cols > (1ll << 30) || q.matrices > 65535)
     return fail(SRS_ERR_INVALID_ARGUMENT, "%lld x %lld is too large", (long long)q.rows,
                 (long long)q.cols);
   const srs_block_copy &copy = q.copy, &turned = q.turned;

@@ -434,8 +434,9 @@ extern "C" int srs_expert_gradient(const srs_blocks* a_t, const srs_blocks* b_t,
                                    void* stream) {
   clear_error();
   if (int rc = check_groups(ends, experts)) return rc;
-  if (rows < 0 || rows > (1ll << 22))
-    return fail(SRS_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^22], got %lld", (long long)rows);
+  if (rows < 0 || rows > kMaxQuantizedRows)
+    return fail(SRS_ERR_INVALID_ARGUMENT, "rows must be in [0, %lld], got %lld",
+                (long long)kMaxQuantizedRows, (long long)rows);
   const int64_t columns = srs_group_columns(rows, experts);
   for (const srs_blocks* b : {a_t, b_t}) {
     if (int rc = check_operand(b == a_t ? "a_t" : "b_t", b, columns)) return rc;

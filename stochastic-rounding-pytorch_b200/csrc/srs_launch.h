@@ -61,6 +61,7 @@ struct QuantizeCall {
   bool overlap = false;  // rows alone: may start beside the kernel ahead, which it reads nothing of
 };
 int quantize(const QuantizeCall& q, cudaStream_t stream);
+constexpr int64_t kMaxQuantizedRows = 65535ll * 64;
 
 int check_operand(const char* what, const srs_blocks* b, int64_t k);
 int check_groups(const int32_t* ends, int groups);

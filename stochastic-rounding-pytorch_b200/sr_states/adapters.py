@@ -28,7 +28,7 @@ def adapter_linear(x, weight, down, up, groups, *, scale=1.0, dtype=torch.float8
     ``weight``: a BlockTensor (inference), a pair of BlockTensors
     ``quantize_blocks(w, block=(128, 128), orientation="both")`` (a frozen projection:
     differentiable in ``x``, ``down`` and ``up``), or an (N, K) tensor (quantised in the call,
-    differentiable too).  The rest as for ``block_linear``.  At most 2^22 tokens.
+    differentiable too).  The rest as for ``block_linear``.  At most 4194240 tokens.
     """
     kept = turned = (None, None)
     if isinstance(weight, BlockTensor):

@@ -26,7 +26,8 @@ def expert_linear(x, weight, ends, *, dtype=torch.float8_e4m3fn, grad_dtype=torc
     same GPU, one entry an expert (at most 1024), rising, as ``group_rows`` gives them (the host
     does not read it).  ``weight``: an (experts, N, K) tensor (quantised in the call;
     differentiable in ``x`` and ``weight``), or a BlockTensor kept from ``quantize_stack``
-    (inference).  The rest as for ``block_linear``.  At most 2^22 rows and 2^30 rows of weights.
+    (inference).  The rest as for ``block_linear``.  At most 4194240 rows and 2^30 rows of
+    weights.
     """
     fmt, _ = check_blocks(dtype, "nearest")
     grad_fmt, grad_rule = check_blocks(grad_dtype, grad_rounding)
