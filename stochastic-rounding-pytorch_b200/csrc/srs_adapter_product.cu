@@ -123,19 +123,18 @@ struct AdapterSource {
     }
     return lo;
   }
-  __device__ int extras(uint32_t t) const {
+  __device__ ExtraSet extras(uint32_t t) const {
     int row, col;
     w.grid.at(t, &row, &col);
-    if (row * w.edge >= p.start[p.count]) return 0;
+    if (row * w.edge >= p.start[p.count]) return {row, 0, 0};
     const int first = first_past(row * w.edge);
     const int last = first_past(min((row + 1) * w.edge, p.start[p.count]) - 1);
-    return (last - first + 1) * w.extra_slices;
+    return {row, first, (last - first + 1) * w.extra_slices};
   }
-  __device__ ExtraLoad extra(uint32_t t, int i) const {
-    int row, col;
-    w.grid.at(t, &row, &col);
-    const int row0 = row * w.edge;
-    const int adapter = first_past(row0) + i / w.extra_slices, slice = i % w.extra_slices;
+  __device__ ExtraLoad extra(const ExtraSet& set, int i) const {
+    const int row = set.row, row0 = row * w.edge;
+    const int ahead = w.extra_slices == 1 ? i : i / w.extra_slices;
+    const int adapter = set.first + ahead, slice = i - ahead * w.extra_slices;
     ExtraLoad e;
     e.map_a = &w.map_h;
     e.map_b = &w.map_u;

@@ -74,6 +74,12 @@ struct ExtraLoad {
   int first, end;         // the tile's rows that it is added to; A's other rows may hold anything
 };
 
+// The products that a tile has of these.
+struct ExtraSet {
+  int row, first;  // the Source's own: tile row, first of what is added
+  int count;
+};
+
 // What happens to a tile's accumulator.
 struct TileStore {
   int row0, col0;  // in the matrix
@@ -678,9 +684,9 @@ __device__ __forceinline__ void run_products(const Source& src) {
           }
         }
         if constexpr (Source::kExtras) {
-          const int extras = src.extras(t);
-          for (int i = 0; i < extras && ok; ++i) {
-            const ExtraLoad e = src.extra(t, i);
+          const ExtraSet extras = src.extras(t);
+          for (int i = 0; i < extras.count && ok; ++i) {
+            const ExtraLoad e = src.extra(extras, i);
             ok = barrier_wait(empty(s), parity ^ 1u, status, 1u);
             if (!ok) break;
             const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
@@ -809,12 +815,12 @@ __device__ __forceinline__ void run_products(const Source& src) {
           }
         }
         if constexpr (Source::kExtras) {
-          const int extras = src.extras(t);
+          const ExtraSet extras = src.extras(t);
           // MMAs of another kind add to this accumulator only behind the last of these: nothing
           // says that the two kinds keep their order.
-          if (extras > 0 && ok) ok = barrier_wait(empty(done_stage), done_parity, status, 8u);
-          for (int i = 0; i < extras && ok; ++i) {
-            const ExtraLoad e = src.extra(t, i);
+          if (extras.count > 0 && ok) ok = barrier_wait(empty(done_stage), done_parity, status, 8u);
+          for (int i = 0; i < extras.count && ok; ++i) {
+            const ExtraLoad e = src.extra(extras, i);
             // Rows that are not the adapter's.  By votes, which leave the words in uniform registers,
             // and with the MMAs unrolled: made from e's numbers by each lane, the words were moved
             // there for every MMA (4096 tokens, 4096 -> 4096, rank 64: 95.9 us instead of 93.1).
