@@ -27,9 +27,9 @@
 // tokens, by the adapter's U; the CTAs of a cluster take the adapters in turn.  Their sums are apart
 // from the projection's, as zero times an infinity is NaN and an item's zeros are in other tokens'
 // columns, which an MMA cannot leave out: a row where an adapter's U is not finite has such sums in
-// every column.  The epilogue computes the adapters' part of a sum that is not finite again, of the
-// token's own adapter alone.  (For 64 tokens of 40 adapters, 14336 x 4096: 29.3 us a call; with all
-// sums in one accumulator 28.8; with a look at U in shared memory ahead of its MMAs 31.5.)
+// every column.  The adapters' part of a sum that is not finite is computed again, from the token's
+// own adapter alone (sums_again, out of line: in the epilogue's own code it took a microsecond for 64
+// tokens, used or not; a look at U in shared memory ahead of the MMAs took three).
 // (In a kernel of its own behind this one that part took 5 us for one token and 10 for 64 with
 // 41 adapters, nearly all of it launch and dependent loads; in this one's epilogue as much.)
 // Ranks up to 16 take narrow boxes, three adapters a stage: with one a stage, of boxes of 128 bytes
@@ -165,6 +165,40 @@ __device__ __noinline__ float own_part(const ThinArgs& a, const ThinAdapters& gi
     sum = fmaf(h, decode(__ldg(up + r * up_step)), sum);
   }
   return sum;
+}
+
+// Times the power of two that a token's FP16 pairs, and with them its sums, do not have.
+__device__ __forceinline__ float unscaled(const ThinArgs& a, float sum, int token) {
+  return a.exponents != nullptr ? sum * two_to(-__ldcg(a.exponents + token)) : sum;
+}
+
+// The sums of this thread's row whose adapters' part is not finite, with their own adapter's part
+// instead: to D (`last`), or to `words` in shared memory, 512 bytes a column.  By whole warps.
+template <int BN>
+__device__ __noinline__ void sums_again(const ThinArgs& a, const ThinAdapters& given, uint32_t acc,
+                                        uint32_t words, int e, int step, int row, bool last) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < a.n; c0 += 16) {
+    uint32_t v[16], u[16];
+    tmem_load16(acc + c0, v, acc + ThinShape<BN>::kAdapterColumn + c0, u);
+    unsigned odd = 0u;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      if (row < 0 || c0 + c >= a.n || (u[c] & 0x7F800000u) != 0x7F800000u) continue;
+      odd |= 1u << c;
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(words + 512 * (c0 + c)), "r"(v[c]) : "memory");
+    }
+    for (; odd != 0u; odd &= odd - 1u) {
+      const int c = c0 + __ffs(odd) - 1;
+      const float sum = __uint_as_float(staged_read(words + 512 * c)) +
+                        own_part<BN>(a, given, e, step, c, row);
+      if (last)
+        store_value(a.out, a.out_format, row * a.row_stride + c * a.col_stride, unscaled(a, sum, c));
+      else
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(words + 512 * c), "f"(sum) : "memory");
+    }
+    __syncwarp();
+  }
 }
 
 template <int BN, int FORM>
@@ -537,50 +571,39 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
   tmem_fence_after();
   const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
   const int row = row0 + 32 * warp + lane, row_end = min(a.m, row0 + a.rows);
+  bool with = false;  // this CTA has adapters' sums
   if constexpr (ADAPTERS) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();  // (the list of adapters)
+    with = (int)rank < given.actives;
   }
-  // 16 columns of this thread's row; which of them still want their adapters' part (own_part).
+  // This thread's row among sums in shared memory: column c at 512 * c bytes, one word a row.
+  const uint32_t words = stage0 + 128 * warp + 4 * lane;
+  // 16 columns of this thread's row.
+  uint32_t top = 0u;  // largest size of the adapters' sums among them
   const auto sums_of = [&](int c0, uint32_t (&v)[16]) {
-    unsigned odd = 0u;
-    tmem_load16(acc + c0, v);
-    if constexpr (ADAPTERS) {
-      if ((int)rank < given.actives) {
-        uint32_t u[16];
-        tmem_load16(acc + S::kAdapterColumn + c0, u);
+    if (!ADAPTERS || !with) {
+      tmem_load16(acc + c0, v);
+    } else {
+      uint32_t u[16];
+      tmem_load16(acc + c0, v, acc + S::kAdapterColumn + c0, u);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const bool finite = (u[c] & 0x7F800000u) != 0x7F800000u;
-          if (finite) v[c] = __float_as_uint(__uint_as_float(v[c]) + __uint_as_float(u[c]));
-          else if (row < row_end && c0 + c < n) odd |= 1u << c;
-        }
-      }
-    }
-    return odd;
-  };
-  // Column c of this thread's row among sums in shared memory (512 bytes a column, one word a row).
-  const auto word_of = [&](int c) { return stage0 + 512 * c + 128 * warp + 4 * lane; };
-  const auto stage_sums = [&](int c0, const uint32_t (&v)[16], unsigned odd) {
-#pragma unroll
-    for (int c = 0; c < 16; ++c)
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(word_of(c0 + c)), "r"(v[c]) : "memory");
-    if constexpr (ADAPTERS) {
-      for (; odd != 0u; odd &= odd - 1u) {
-        const int c = c0 + __ffs(odd) - 1;
-        const float part = own_part<BN>(a, given, (int)rank, (int)splits, c, row);
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(word_of(c)),
-                     "f"(__uint_as_float(staged_read(word_of(c))) + part)
-                     : "memory");
+      for (int c = 0; c < 16; ++c) {
+        v[c] = __float_as_uint(__uint_as_float(v[c]) + __uint_as_float(u[c]));
+        top = max(top, c0 + c < n ? u[c] & 0x7FFFFFFFu : 0u);
       }
     }
   };
-  // A sum of column c without the power of two of its FP16 pairs.
   const auto result = [&](float sum, int c) {
-    if constexpr (ADAPTERS) {
-      if (a.exponents != nullptr) return sum * two_to(-__ldcg(a.exponents + c));
-    }
+    if constexpr (ADAPTERS) return unscaled(a, sum, c);
     return sum;
+  };
+  const auto look_again = [&]() {
+    if constexpr (ADAPTERS) {
+      if (__any_sync(0xFFFFFFFFu, top >= 0x7F800000u && row < row_end))
+        sums_again<BN>(a, given, acc, words, (int)rank, (int)splits, row < row_end ? row : -1,
+                       splits == 1);
+    }
   };
   if (splits == 1) {
     if (warp < 4 && ok) {
@@ -588,17 +611,15 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       for (int c0 = 0; c0 < BN; c0 += 16) {
         if (c0 >= n) break;
         uint32_t v[16];
-        const unsigned odd = sums_of(c0, v);
-        if (ADAPTERS && odd != 0u) stage_sums(c0, v, odd);
+        sums_of(c0, v);
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          if (row < row_end && c0 + c < n) {
-            if (ADAPTERS && odd != 0u) v[c] = staged_read(word_of(c0 + c));
+          if (row < row_end && c0 + c < n)
             store_value(a.out, a.out_format,
                         row * a.row_stride + (b_row0 + c0 + c) * a.col_stride,
                         result(__uint_as_float(v[c]), c0 + c));
-          }
       }
+      look_again();
     }
   } else {
     if (warp < 4) {
@@ -606,9 +627,13 @@ thin_product_kernel(const __grid_constant__ ThinArgs a) {
       for (int c0 = 0; c0 < BN; c0 += 16) {
         if (c0 >= n) break;
         uint32_t v[16];
-        const unsigned odd = sums_of(c0, v);
-        stage_sums(c0, v, odd);
+        sums_of(c0, v);
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(words + 512 * (c0 + c)), "r"(v[c])
+                       : "memory");
       }
+      look_again();
     }
     cluster_sync();
     // columns rank, rank + splits, ...: half of the CTA's threads a column
