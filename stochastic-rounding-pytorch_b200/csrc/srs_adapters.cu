@@ -12,7 +12,10 @@
 //
 // Tokens are taken in the order of their adapters (srs_group_rows), gathered where they are
 // read and scattered where results are written.  h and g are FP32; where a tensor core takes them
-// they are split into a pair of 16-bit numbers, so that only the results are rounded.
+// they are split into a pair of 16-bit numbers.  A pair loses 2^-17 of them in BF16 and 2^-22 in
+// FP16, a 256th and a 1024th of what the result's own rounding may: with three BF16 numbers in the
+// gradients' sums the results' distance from FP64 was the same to five digits (0.001654 of their
+// size), and calls were 1 to 4 % slower.
 #include <cooperative_groups.h>
 
 #include "srs_common.cuh"
@@ -530,8 +533,8 @@ constexpr int kSumZ = kSumStep * kSumCols * 2;
 template <int RT>
 struct SumShape {
   static constexpr int kRank = 16 * RT, kLow = kSumStep * kRank * 2;
-  // more CTAs an SM rather than deeper stages: three, three and two
-  static constexpr int kStages = RT == 2 ? 3 : 4, kResident = RT == 4 ? 2 : 3;
+  // two CTAs an SM for ranks up to 16 and above 32 (what shared memory has room for), else three
+  static constexpr int kStages = RT == 2 ? 3 : 4, kResident = RT == 2 ? 3 : 2;
   static constexpr int kSmem = 1024 + kStages * kSumZ + 2 * 2 * kLow;
 };
 
@@ -888,7 +891,9 @@ int check_adapters(const srs_adapters* a, int64_t tokens, int64_t k, int64_t n, 
 
 using namespace srs;
 
-// Few tokens: the projection's thin form.
+// Few tokens: the projection's thin form.  (4096 -> 4096, rank 16, 5 adapters for every 8 tokens: 64
+// tokens 25 us a call, 65 in the large form 43: nothing splits k there, and a tile has as many
+// adapters as a thin one.)
 static bool few(int64_t tokens) { return tokens <= kThinRows; }
 
 // Parts of a call's workspace, each on a 256-byte boundary: the quantised tokens first; FP16 alone
@@ -1030,7 +1035,7 @@ extern "C" int srs_adapter_linear(const void* x, int64_t tokens, int64_t k, int6
 }
 
 // Tokens of a chunk for `cols` columns in all: long ones leave fewer parts, short ones keep the SMs
-// busy (with three CTAs each).
+// busy (as if with three CTAs each).
 static int sum_chunk(int64_t tokens, int64_t cols, int rank) {
   const int64_t each = ceil_div(cols, kSumCols) * ceil_div(rank, 64);
   int64_t chunk = tokens * each / (3 * sm_count());

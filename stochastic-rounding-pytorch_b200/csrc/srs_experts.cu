@@ -369,7 +369,9 @@ int zeros(void* d, int64_t count, int format, cudaStream_t stream) {
 int expert_matmul(const srs_blocks& a, const srs_blocks& w, int experts, const int32_t* ends,
                   int64_t k, void* d, int d_format, bool overlap, cudaStream_t stream) {
   const int64_t busy = experts < a.rows ? experts : a.rows;
-  // Up to 32 rows a group in the mean the weights' bytes bound the product.
+  // Up to 32 rows a group in the mean the weights' bytes bound the product.  Both forms, thin first, us
+  // a call: 64 experts, 2048 -> 1024, of 16 rows each 37 and 43, of 32 43.3 and 44.0, of 40 47.4 and
+  // 45.5, of 64 57 and 49; 8 experts, 4096 -> 14336, 91 and 107, 98 and 109, 103 and 110, 124 and 111.
   if (a.rows <= 32 * busy)
     return launch_expert_thin(a, w, experts, ends, k, d, d_format, overlap, stream);
   return launch_ragged_rows(a, w, experts, ends, k, d, d_format, stream);

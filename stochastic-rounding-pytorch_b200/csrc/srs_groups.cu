@@ -26,7 +26,9 @@ namespace cg = cooperative_groups;
 constexpr int kSortAhead = 8;     // batches of a warp loaded together
 // Rows up to kSortSmall: one CTA of 32 warps, 128 rows each.  More: a cluster of 16 CTAs of 16
 // warps (its meetings and remote counts cost about 2 us).  The instructions of 200 a batch bound
-// it: 65536 rows took 11.8 us on eight SMs.
+// it: 65536 rows took 12.2 us on eight SMs, 9.6 on these.  Beyond 65536 rows (16 x 4096) they do not
+// fit the registers and shared memory: the index is read twice and rows leave one by one, 14.6 us a
+// call for 2^17 rows, 21.9 for 2^18, 66 for 2^20, 240 for 2^22.
 constexpr int kSortCluster = 16;
 constexpr int64_t kSortSmall = 4096;
 

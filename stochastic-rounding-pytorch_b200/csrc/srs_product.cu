@@ -409,8 +409,8 @@ int launch_expert_thin(const srs_blocks& a, const srs_blocks& w, int experts, co
   args.m = (int)n;
   args.slices = (int)((k + kSliceBytes - 1) / kSliceBytes);
   // k is split while few tiles are likely, as for one weight.  Tiles of a size that fills whole rounds of
-  // two CTAs an SM are no gain here (256 rows of 62 groups, 2048 -> 1024: 31.2 us, so 30.1; two
-  // rows, 4096 -> 14336: 25.3 and 24.7).
+  // two CTAs an SM are no gain here (256 rows of 62 groups, 2048 -> 1024: 31.2 us with them, 30.1
+  // without; two rows, 4096 -> 14336: 25.3 and 24.7).
   const int64_t sms = sm_count(), tiles = (n + 127) / 128;
   args.rows = (int)((n + tiles - 1) / tiles);
   int splits = 1;
