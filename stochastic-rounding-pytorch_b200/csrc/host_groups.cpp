@@ -466,11 +466,12 @@ at::Tensor flat(const at::Tensor& x) {
   return x.dim() == 2 ? x : x.dim() == 1 ? x.unsqueeze(0) : x.flatten(0, -2);
 }
 
+// (no view: autograd refuses to change one in place that was made inside a function)
 at::Tensor shaped(const at::Tensor& rows, at::IntArrayRef like) {
   if (like.size() == 2) return rows;
   std::vector<int64_t> sizes(like.begin(), like.end());
   sizes.back() = rows.size(1);
-  return rows.reshape(sizes);
+  return at::_unsafe_view(rows, sizes);
 }
 
 // What of a call is no leaf.
@@ -483,18 +484,17 @@ struct AdapterInputs {
   std::vector<int64_t> need;  // gradients of x, weight, down, up
 };
 
-// Of tokens x features: other shapes are views that autograd takes before and behind this, as a view
-// made in here could not be changed in place.
 struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
   enum { kX, kDown, kUp, kScale, kOrder, kEnds, kLow, kLargest, kMatrix, kMatrixScale, kTokens,
          kTokensScale };
 
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows,
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x,
                             const std::optional<at::Tensor>& weight, const at::Tensor& down,
                             const at::Tensor& up, const AdapterInputs& in) {
     const Rounding nearest{in.format, SRS_RULE_NEAREST, 0u};
     const std::vector<int64_t>& need = in.need;
     Blocks matrix = in.kept, matrix_t = in.turned, tokens_t;
+    const at::Tensor rows = flat(x);
     if (weight.has_value()) {
       matrix_t = {};
       quantize(*weight, nearest, true, 0u, need[0] ? kBoth : kRows, &matrix,
@@ -515,7 +515,8 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
         in.grad.format, in.grad.rule, (int64_t)in.grad.seed,
         (int64_t)(weight.has_value() ? weight->scalar_type() : at::kFloat)};
     ctx->saved_data["factor"] = in.factor;
-    return y;
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    return shaped(y, x.sizes());
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -524,7 +525,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
     const std::vector<int64_t> s = ctx->saved_data["how"].toIntVector();
     const double factor = ctx->saved_data["factor"].toDouble();
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor dy = aligned(grads[0], false);
+    const at::Tensor dy = aligned(flat(grads[0]), false);
     const c10::cuda::OptionalCUDAGuard guard(dy.device());
     const Rounding how{(int)s[0], (int)s[1], (uint32_t)s[2]};
     const at::Tensor &order = saved[kOrder], &ends = saved[kEnds];
@@ -536,7 +537,7 @@ struct AdapterLinear : torch::autograd::Function<AdapterLinear> {
       const at::Tensor dx =
           adapter_product(dy, how, {saved[kMatrix], saved[kMatrixScale]}, saved[kDown], saved[kUp],
                           saved[kScale], factor, order, ends, true, need[2] ? &back : nullptr);
-      if (need[0]) out[0] = dx;
+      if (need[0]) out[0] = shaped(dx, ctx->saved_data["sizes"].toIntVector());
       if (need[2]) sums.push_back({saved[kX], &back, false, {}});
     }
     if (need[3]) sums.push_back({dy, &low, true, {}});
@@ -754,9 +755,8 @@ PyObject* py_adapter_linear(PyObject*, PyObject* args) {
       in.order = order.to(at::kInt);
       in.ends = checked_ends(ends, x, "adapter_linear");
     }
-    const at::Tensor y = AdapterLinear::apply(
-        flat(x), weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt, down, up, in);
-    return THPVariable_Wrap(shaped(y, x.sizes()));
+    return THPVariable_Wrap(AdapterLinear::apply(
+        x, weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt, down, up, in));
   }
   c10::NoGradGuard no_grad;
   const Rounding nearest{format, SRS_RULE_NEAREST, 0u};

@@ -26,30 +26,35 @@ def _matrix(x):
 
 
 class _BlockLinear(torch.autograd.Function):
-    # of a matrix: a view made in here could not be changed in place
     @staticmethod
     def forward(ctx, x, weight, dtype, grad_dtype, grad_rounding, seed, need_x, need_w):
-        tokens = quantize_blocks(x, dtype=dtype, orientation="both" if need_w else "rows")
+        tokens = quantize_blocks(_matrix(x), dtype=dtype,
+                                 orientation="both" if need_w else "rows")
         matrix = quantize_blocks(weight, dtype=dtype, block=(BLOCK, BLOCK),
                                  orientation="both" if need_x else "rows")
         tokens, tokens_t = tokens if need_w else (tokens, None)
         matrix, matrix_t = matrix if need_x else (matrix, None)
         ctx.save_for_backward(*(tokens_t or ()), *(matrix_t or ()))
-        ctx.settings = (grad_dtype, grad_rounding, seed, x.dtype, weight.dtype, need_x, need_w)
-        return matmul_blocks(tokens, matrix, dtype=x.dtype)
+        ctx.settings = (grad_dtype, grad_rounding, seed, x.shape, x.dtype, weight.dtype, need_x,
+                        need_w)
+        y = matmul_blocks(tokens, matrix, dtype=x.dtype)
+        if x.dim() == 2:
+            return y
+        # no view: autograd refuses to change one in place that was made inside a function
+        return torch.ops.aten._unsafe_view(y, (*x.shape[:-1], weight.shape[0]))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        grad_dtype, rounding, seed, x_dtype, w_dtype, need_x, need_w = ctx.settings
+        grad_dtype, rounding, seed, shape, x_dtype, w_dtype, need_x, need_w = ctx.settings
         saved = list(ctx.saved_tensors)
         tokens_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_w else None
         matrix_t = BlockTensor(saved.pop(0), saved.pop(0)) if need_x else None
         orientation = "both" if need_x and need_w else "rows" if need_x else "columns"
-        got = quantize_blocks(dy, dtype=grad_dtype, rounding=rounding, seed=seed,
+        got = quantize_blocks(_matrix(dy), dtype=grad_dtype, rounding=rounding, seed=seed,
                               orientation=orientation)
         rows, columns = got if orientation == "both" else (got, got)
-        dx = matmul_blocks(rows, matrix_t, dtype=x_dtype) if need_x else None
+        dx = matmul_blocks(rows, matrix_t, dtype=x_dtype).reshape(shape) if need_x else None
         dw = matmul_blocks(columns, tokens_t, dtype=w_dtype) if need_w else None
         return dx, dw, None, None, None, None, None, None
 
@@ -77,9 +82,8 @@ def block_linear(x, weight, *, dtype=torch.float8_e4m3fn, grad_dtype=torch.float
     check_blocks(grad_dtype, grad_rounding)
     # asked here: inside a Function inputs "need" gradients under torch.no_grad() as well
     grad = torch.is_grad_enabled()
-    y = _BlockLinear.apply(_matrix(x), weight, dtype, grad_dtype, grad_rounding, seed,
-                           grad and x.requires_grad, grad and weight.requires_grad)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
+    return _BlockLinear.apply(x, weight, dtype, grad_dtype, grad_rounding, seed,
+                              grad and x.requires_grad, grad and weight.requires_grad)
 
 
 def _rank():
