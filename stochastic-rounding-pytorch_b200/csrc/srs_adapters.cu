@@ -13,7 +13,7 @@
 // Tokens are taken in the order of their adapters (srs_group_rows), gathered where they are
 // read and scattered where results are written.  h and g are FP32; where a tensor core takes them
 // they are split into a pair of 16-bit numbers.  A pair loses 2^-17 of them in BF16 and 2^-22 in
-// FP16, a 256th and a 1024th of what the result's own rounding may: with three BF16 numbers in the
+// FP16, a 512th and a 2048th of what the result's own rounding may: with three BF16 numbers in the
 // gradients' sums the results' distance from FP64 was the same to five digits (0.001654 of their
 // size), and calls were 1 to 4 % slower.
 #include <cooperative_groups.h>
